@@ -87,6 +87,20 @@ SIGNATURES = {
          c_int, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p, c_size_t, c_int, c_uint, c_void_p],
     ),
     "b200_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "b200_sample_rows": (
+        c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p, c_float, c_void_p,
+                c_float, c_int, c_void_p],
+    ),
+    "b200_draft_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]),
+    "b200_paged_tree_attn_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "b200_paged_tree_attn": (
+        c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_void_p, c_size_t, c_int, c_uint, c_void_p],
+    ),
+    "b200_accept_drafts": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_void_p],
+    ),
     "b200_kv_gather_dense": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,

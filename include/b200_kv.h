@@ -270,6 +270,52 @@ int b200_argmax_rows_keys(int64_t* keys, const void* x, int64_t rows, int64_t co
                           int64_t col_offset, int dtype, void* stream);
 int b200_argmax_keys_decode(int64_t* out, const int64_t* keys, int64_t rows, void* stream);
 
+/* Drawn token: out[r] from the weights exp((x[r, i] - max x[r]) / temperature), -inf counting 0.  In the descending order of the logits (the
+ * lowest index first among equals) the first top_k are kept (<= 0: all), of these the ones before which the weights sum to less than top_p of
+ * theirs all (>= 1: all), of these the ones with at least min_p of the largest weight (<= 0: all); the order's first is always kept.  The token
+ * is the first index at which the kept weights, summed up in the row's order, exceed u[r] of their sum; u in [0, 1), what is outside counts as
+ * the nearest number inside.  temperature <= 0, or a row whose largest logit is NaN or infinite: b200_argmax_rows' token.  Weights in 64
+ * bits, sums exact to 2^-(62 - log2 cols) of the largest weight: a row's token does not depend on the other rows.  Settings: fp32 / int32 [rows], or NULL
+ * for the *_all value in every row.  cols <= 2^20. */
+#define B200_MAX_SAMPLE_COLS (1 << 20)
+int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64_t cols, int64_t row_stride, const float* u, const float* temperature,
+                     float temperature_all, const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                     float min_p_all, int dtype, void* stream);
+
+/*
+ * Drafted tokens.  A sequence's tree has up to 64 nodes: node 0 is its root, the last token that is certain, whose keys and values are not yet in the
+ * cache; parents[b, t] < t for the others.  Its nodes' keys and values are appended at the places behind the context in the order of their
+ * numbers, so that context_lens[b] counts them; draft_lens (int32[B], NULL: all `nodes`) tells how many nodes a sequence has.  (The reference:
+ * TreeDraftBuffer and the verification pass of worker/engines/speculative.py:128-471.)
+ *
+ * b200_draft_tree: visible[b, t] (int64 bit masks, bit s: node s) the node and all above it, depth[b, t] its distance from the root.  A
+ * node whose parent is not before it sees only itself; nodes behind the sequence's last see nothing.  parents' rows parent_stride apart.
+ *
+ * b200_paged_tree_attn: out[b, t, h] = softmax(q k scale) v over the context (the first context_lens[b] - n tokens, n the sequence's nodes) and the
+ * nodes in visible[b, t], any set of them.  A row that sees nothing, and rows behind the sequence's last node, are 0.  Keys that no row of a call may see
+ * are not read (stale slots may hold anything); NaN and infinities in a node's values reach the rows that see it only.  A table entry outside
+ * the pool reads as zeros.  At most table_cols pages of a sequence are read.  q: [B, nodes, Hq, D], rows of a node contiguous; out contiguous.
+ *   workspace : b200_paged_tree_attn_workspace bytes, 16-byte aligned, any contents; calls that may run at the same time need their own.
+ *
+ * b200_accept_drafts: node t fits if its token is chosen[b, parent] (the first of siblings with the same token), and is taken if all of
+ * visible[b, t] fits.  count[b]: taken nodes, the root among them; path[b, k] the k-th, -1 behind the last; new_tokens[b, k] = chosen[b, path[b, k]],
+ * -1 behind; new_lens[b] the context and the taken nodes.  Keys and values of path[b, k] move to the k-th place behind the context in
+ * every pool of k_pools / v_pools (device arrays of n_layers pool addresses; n_layers 0: nothing moves).  Pages of these places belong to one sequence.
+ */
+#define B200_MAX_DRAFT_NODES 64
+int b200_draft_tree(int64_t* visible, int32_t* depth, const int32_t* parents, int64_t parent_stride, const int32_t* draft_lens, int B,
+                    int nodes, void* stream);
+size_t b200_paged_tree_attn_workspace(int B, int nodes, int Hq, int Hkv, int D, int block_size, int dtype);
+int b200_paged_tree_attn(void* out, const void* q, int64_t q_batch_stride, int64_t q_node_stride, const void* k_pool, const void* v_pool,
+                         const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, const int32_t* draft_lens,
+                         const int64_t* visible, int64_t visible_stride, int B, int nodes, int Hq, int Hkv, int D, int block_size,
+                         int64_t max_blocks, float scale, void* workspace, size_t workspace_bytes, int dtype, unsigned flags, void* stream);
+int b200_accept_drafts(int32_t* count, int32_t* path, int64_t* new_tokens, int32_t* new_lens, const int64_t* tokens, int64_t token_stride,
+                       const int64_t* chosen, int64_t chosen_stride, const int32_t* parents, int64_t parent_stride, const int64_t* visible,
+                       int64_t visible_stride, void* const* k_pools, void* const* v_pools, int n_layers, const int32_t* block_tables,
+                       int table_stride, int table_cols, const int32_t* context_lens, const int32_t* draft_lens, int B, int nodes, int Hkv, int D,
+                       int block_size, int64_t max_blocks, int dtype, void* stream);
+
 /*
  * Gather to dense: the first n_tokens tokens of B sequences, read through their block-table rows, written as
  *   k_out, v_out : [B, Hkv, n_tokens, D]

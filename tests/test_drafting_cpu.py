@@ -1,0 +1,124 @@
+"""What the drawing and drafting entry points refuse, without a GPU: Python's checks against a recorder, the C ABI's on null pointers."""
+import types
+
+import pytest
+import torch
+
+import dgi_b200  # noqa: F401
+from dgi_b200 import _lib, ops
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    made = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: made.append(name) or 0
+
+    class Guard:
+        __enter__ = __exit__ = lambda self, *a: None
+
+    monkeypatch.setattr(ops, "_lib", types.SimpleNamespace(load=Library, check=_lib.check, B200LibraryError=_lib.B200LibraryError))
+    monkeypatch.setattr(ops, "_need_cuda", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_on", lambda device: Guard())
+    return made
+
+
+def refused(made, call, *changes):
+    """`call(**change)` raises ValueError or TypeError and launches nothing; with no change it launches once."""
+    call()
+    launches = len([n for n in made if not n.endswith("_workspace")])
+    assert launches == 1
+    for change in changes:
+        with pytest.raises((ValueError, TypeError)):
+            call(**change)
+    assert len([n for n in made if not n.endswith("_workspace")]) == launches
+
+
+def test_sample_rows(recorded):
+    x, u, i = torch.zeros(3, 8), torch.zeros(3), torch.zeros(3, dtype=torch.int32)
+
+    def call(x=x, u=u, **kw):
+        return ops.sample_rows(x, u, **kw)
+
+    refused(recorded, call, dict(x=torch.zeros(8)), dict(x=torch.zeros(8, 3).t()), dict(x=x.double()), dict(u=torch.zeros(2)), dict(u=u.double()),
+            dict(u=torch.zeros(6)[::2]), dict(u=torch.zeros(3, device="meta")), dict(temperature=i), dict(temperature=torch.zeros(4)), dict(top_k=u),
+            dict(top_k=i.long()), dict(top_p=u.double()), dict(min_p=torch.zeros(3, 1)), dict(out=i), dict(out=torch.zeros(4, dtype=torch.int64)))
+
+
+def test_draft_tree(recorded):
+    par, n = torch.zeros(2, 5, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+    def call(par=par, n=n):
+        return ops.draft_tree(par, n)
+
+    refused(recorded, call, dict(par=par.long()), dict(par=par[0]), dict(par=torch.zeros(5, 2, dtype=torch.int32).t()), dict(n=n.long()),
+            dict(n=torch.zeros(3, dtype=torch.int32)))
+
+
+def test_paged_tree_attention(recorded):
+    i32 = torch.int32
+    base = dict(q=torch.zeros(2, 3, 4, 8), k_pool=torch.zeros(5, 2, 16, 8), v_pool=torch.zeros(5, 2, 16, 8), block_tables=torch.zeros(2, 4, dtype=i32),
+                context_lens=torch.zeros(2, dtype=i32), visible=torch.zeros(2, 3, dtype=torch.int64))
+
+    def call(**change):
+        return ops.paged_tree_attention(**{**base, **change})
+
+    refused(recorded, call, dict(q=torch.zeros(2, 3, 32)), dict(q=torch.zeros(2, 3, 4, 9)), dict(q=base["q"].half()), dict(q=torch.zeros(2, 3, 3, 8)),
+            dict(q=torch.zeros(2, 4, 3, 8).transpose(1, 2)), dict(k_pool=base["k_pool"].transpose(1, 2)), dict(v_pool=torch.zeros(5, 2, 16, 16)),
+            dict(block_tables=base["block_tables"].long()), dict(block_tables=torch.zeros(3, 4, dtype=i32)), dict(block_tables=torch.zeros(2, 0, dtype=i32)),
+            dict(context_lens=torch.zeros(2)), dict(visible=torch.zeros(2, 3, dtype=i32)), dict(visible=torch.zeros(2, 4, dtype=torch.int64)),
+            dict(draft_lens=torch.zeros(2)), dict(out=torch.zeros(2, 3, 4, 8).half()), dict(out=torch.zeros(2, 3, 4, 16)[..., ::2]),
+            dict(v_pool=torch.zeros(5, 2, 16, 8, device="meta")), dict(visible=torch.zeros(2, 3, dtype=torch.int64, device="meta")))
+
+
+def test_accept_drafts(recorded):
+    i32, i64 = torch.int32, torch.int64
+    base = dict(tokens=torch.zeros(2, 3, dtype=i64), chosen=torch.zeros(2, 3, dtype=i64), parents=torch.zeros(2, 3, dtype=i32),
+                visible=torch.zeros(2, 3, dtype=i64), k_ptrs=torch.zeros(4, dtype=i64), v_ptrs=torch.zeros(4, dtype=i64), pool_shape=(5, 2, 16, 8),
+                dtype=torch.float32, block_tables=torch.zeros(2, 4, dtype=i32), context_lens=torch.zeros(2, dtype=i32))
+
+    def call(**change):
+        return ops.accept_drafts(**{**base, **change})
+
+    refused(recorded, call, dict(tokens=base["tokens"].int()), dict(tokens=base["tokens"][0]), dict(chosen=torch.zeros(2, 4, dtype=i64)),
+            dict(parents=base["parents"].long()), dict(visible=base["visible"].int()), dict(k_ptrs=None), dict(v_ptrs=torch.zeros(3, dtype=i64)),
+            dict(k_ptrs=torch.zeros(4, dtype=i32)), dict(block_tables=torch.zeros(2, 4)), dict(context_lens=torch.zeros(3, dtype=i32)),
+            dict(draft_lens=torch.zeros(2, dtype=i64)))
+
+
+def test_the_library_refuses():
+    lib = _lib.load()
+
+    def says(rc, code, text):
+        assert rc == code and text in lib.b200_last_error()
+
+    says(lib.b200_sample_rows(None, None, 2, 8, 8, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 7, None), -1, b"unsupported dtype")
+    says(lib.b200_sample_rows(None, None, 2, 8, 7, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -1, b"bad sizes")
+    says(lib.b200_sample_rows(None, None, 2, 8, 8, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -1, b"null pointer")
+    says(lib.b200_sample_rows(None, None, 2, (1 << 20) + 1, 1 << 21, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -2, b"rows of")
+    assert lib.b200_sample_rows(None, None, 0, 8, 8, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None) == 0
+    says(lib.b200_draft_tree(None, None, None, 3, None, 2, 65, None), -2, b"at most 64")
+    says(lib.b200_draft_tree(None, None, None, 3, None, 2, 3, None), -1, b"null pointer")
+    attn = lambda nodes=3, hq=4, hkv=2, dtype=2, cols=4: lib.b200_paged_tree_attn(  # noqa: E731
+        None, None, 0, 0, None, None, None, 4, cols, None, None, None, 3, 2, nodes, hq, hkv, 64, 16, 10, 1.0, None, 0, dtype, 0, None)
+    says(attn(nodes=65), -2, b"at most 64")
+    says(attn(hq=5), -2, b"multiple")
+    says(attn(dtype=9), -1, b"unsupported dtype")
+    says(attn(cols=0), -1, b"bad sizes")
+    says(attn(), -1, b"null pointer")
+    accept = lambda nodes=3, layers=2, dtype=2: lib.b200_accept_drafts(  # noqa: E731
+        None, None, None, None, None, 3, None, 3, None, 3, None, 3, None, None, layers, None, 4, 4, None, None, 2, nodes, 2, 64, 16, 10, dtype, None)
+    says(accept(nodes=65), -2, b"at most 64")
+    says(accept(dtype=5), -1, b"unsupported dtype")
+    says(accept(layers=40000), -2, b"layers")
+    says(accept(), -1, b"null pointer")
+
+
+def test_no_cpu_form():
+    with pytest.raises(_lib.B200LibraryError):
+        ops.sample_rows(torch.zeros(1, 4), torch.zeros(1))
+    with pytest.raises(_lib.B200LibraryError):
+        ops.draft_tree(torch.zeros(1, 4, dtype=torch.int32))
