@@ -47,6 +47,7 @@
 
 #include "../../include/b200_mixers.h"
 #include "b200_common.cuh"
+#include "b200_tcgen05.cuh"
 #include "b200_tile_attn.cuh"
 
 namespace b200 {
@@ -56,186 +57,6 @@ constexpr int kRows = kTileRows, kKeys = 64;
 constexpr int kLoad = 128;                // threads that copy pages; kRows more per half do the softmax, one warp issues products
 constexpr int kBlk = kKeys * 128;        // bytes of 64 keys x 64 columns
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-  // no memory clobber: the rows of the next copies may be looked up in between (the group's commit and wait carry it)
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0));
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void fence_smem_to_mma() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ bool bar_done(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// false when the barrier did not complete within about a second (or an earlier wait of the CTA already failed)
-__device__ __forceinline__ bool bar_wait1(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (bar_done(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!bar_done(bar, parity)) {
-    if (*dead || clock64() - t0 > 2000000000ll) {
-      *dead = 1;
-      return false;
-    }
-  }
-  return true;
-}
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {   // by a whole warp
-  const bool ok = bar_wait1(bar, parity, dead);
-  __syncwarp();
-  return ok;
-}
-
-// operand in 128-byte lines, 16-byte pieces swizzled by the line's number in its group of eight; `stride` between groups of eight
-// lines, `lead` between blocks of 64 columns (transposed reads only)
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>((lead >> 4) & 0x3FFF) << 16) |
-         (static_cast<uint64_t>((stride >> 4) & 0x3FFF) << 32) | (1ull << 46) | (2ull << 61);
-}
-template <typename T>
-__device__ __forceinline__ constexpr uint32_t instr(int n, bool b_transposed) {
-  constexpr uint32_t type = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
-  return (1u << 4) | (type << 7) | (type << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n / 8) << 17) |
-         (static_cast<uint32_t>(kRows / 16) << 24);
-}
-// Executed by a whole warp: one elected lane issues.  Operands that are the same in all lanes stay in uniform registers that way; a
-// branch on the lane makes every operand of every product pass through a register move, which was most of the walk's time.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
-      : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile(
-      "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ void tm_ld32(float (&r)[32], uint32_t addr) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-        "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]),
-        "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]),
-        "=r"(u[30]), "=r"(u[31])
-      : "r"(addr));
-}
-__device__ __forceinline__ void tm_ld16(float (&r)[16], uint32_t addr) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-        "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-      : "r"(addr));
-}
-__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&u)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(u[0]),
-      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]),
-      "r"(u[13]), "r"(u[14]), "r"(u[15])
-      : "memory");
-}
-
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 both(float x) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ f32x2 pair(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void apart(float& a, float& b, f32x2 v) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// a warp's 32 rows of N columns times the lanes' factors, W columns at a time
-template <int N, int W>
-__device__ __forceinline__ void scale_rows(uint32_t addr, float k) {
-  const f32x2 kk = both(k);
-#pragma unroll 1
-  for (int c = 0; c < N; c += W) {
-    float o[W];
-    if constexpr (W == 16) tm_ld16(o, addr + c);
-    else tm_ld32(o, addr + c);
-    tc_wait_ld();
-#pragma unroll
-    for (int x = 0; x < W; x += 16) {
-      uint32_t w[16];
-#pragma unroll
-      for (int u = 0; u < 16; u += 2) {
-        float lo, hi;
-        apart(lo, hi, mul2(pair(o[x + u], o[x + u + 1]), kk));
-        w[u] = __float_as_uint(lo), w[u + 1] = __float_as_uint(hi);
-      }
-      tm_st16(addr + c + x, w);
-    }
-  }
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-// (a, b) <- (a, b) * k + m
-__device__ __forceinline__ void scale_shift(float& a, float& b, f32x2 k, f32x2 m) {
-  asm("{\n.reg .b64 t;\nmov.b64 t, {%0, %1};\nfma.rn.f32x2 t, t, %2, %3;\nmov.b64 {%0, %1}, t;\n}\n" : "+f"(a), "+f"(b) : "l"(k), "l"(m));
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
 
 // Columns c .. c + 31 of a lane's row to its warp's rows in shared memory, as type O, 16-byte pieces swizzled by the row's number in its group
 // of eight
@@ -824,18 +645,6 @@ tile_attn_kernel(const TileAttn A, const __grid_constant__ CUtensorMap k_map, co
   tc_fence_before();
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(P::kTm));
-}
-
-using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                            const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-Encode tensor_map_encode() {
-  static const Encode encode = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess) p = nullptr;
-    return reinterpret_cast<Encode>(p);
-  }();
-  return encode;
 }
 
 // The pool as rows of `width` elements, fetched in boxes of 64 columns x one page; made for the launch (a microsecond) and not kept.

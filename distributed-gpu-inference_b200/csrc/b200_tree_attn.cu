@@ -2,8 +2,10 @@
 //
 //   out[t, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(q[t, h] k_j scale - max),   j in the context, or bit j of visible[t]
 #include <algorithm>
+#include <type_traits>
 
 #include "b200_common.cuh"
+#include "b200_tcgen05.cuh"
 
 namespace b200 {
 namespace {
@@ -113,6 +115,565 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const Tre
   }
 }
 
+// ---- 16-bit types, heads of 64 or 128, pages that divide 64 keys (or are multiples of 64) ------------------------------------------------------
+// The rows of a sequence and kv head - its nodes times the rep = Hq / Hkv query heads, node by node - go in blocks of 128; a CTA keeps to one
+// block's number.  Keys go in tiles of 64, and the tiles of all sequences and kv heads, one after another, in equal shares to the workers: a CTA
+// per row block that walk the same keys side by side.  Whole walks (a sequence's and head's every tile) are written out; what a share's
+// ends cut leaves (maximum, sum, output) in the workspace, at most two pieces a worker, for tree_merge_kernel, which puts a row's pieces together in the order of
+// their keys and writes the zeros of rows without a node.
+//
+//   S = Q K^T   tcgen05.mma, 128 x 64, both operands in shared memory (128-byte swizzled lines), S in tensor memory, two of them
+//   P           four warps, one thread per row: mask, running maximum, exp2 in fp32; rounded to the storage type into the tensor memory S
+//               was in.  The largest weight is 1 and loses nothing by it; the sum is taken before the rounding
+//   O += P V    tcgen05.mma, P from tensor memory, O in tensor memory in fp32
+//
+// Three warps copy (one keys, two values), boxes of a page by 64 columns; the tiles that reach into the drafted tokens have their values copied by the
+// threads themselves, zeros for slots behind the last token and for values that are no numbers: 0 x NaN would reach rows that do not see
+// them.  Rows that do get them in the end.
+constexpr int kRows = 128, kKeys = 64, kBlk = kKeys * 128;
+// threads: rows, copies of keys and of values, products.  Eight warps: two CTAs' leave each thread 128 registers (nine: 96)
+constexpr int kSoft = 128, kLoadK = 32, kLoadV = 64, kNT = kSoft + kLoadK + kLoadV + 32;
+constexpr int kCtasPerSm = 2;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct Plan {
+  static constexpr int kBufs = D == 128 ? 2 : 4;        // of keys, and of values
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + (D / 64) * kRows * 128;
+  static constexpr int kV = kK + kBufs * (D / 64) * kBlk;
+  static constexpr int kBar = kV + kBufs * (D / 64) * kBlk;
+  static constexpr int kFlags = kBar + 8 * (1 + 4 * kBufs + 4);     // tensor memory's address, failure, values that are no numbers
+  static constexpr int kEnd = kFlags + 16;
+  static constexpr int kO = 2 * kKeys, kTm = 256;     // columns of tensor memory: S0 | S1 | O
+  static_assert((kEnd + 1024 + 1024) * kCtasPerSm <= 228 * 1024, "shared memory");
+};
+
+struct Shares {
+  float2* ml;               // [worker][row block][2][rows]: maximum (of scores in powers of two), sum
+  float4* o;                // [worker][row block][2][D / 4][rows]
+  int rows, blocks, workers;        // of a block that are kept (multiple of 32)
+};
+
+// Tiles of a sequence
+__device__ __forceinline__ int tiles_of(const TreeAttn& A, int b) {
+  int keys, n;
+  lengths(A, b, &keys, &n);
+  return n > 0 ? (keys + kKeys - 1) / kKeys : 0;
+}
+
+// A worker's way through the tiles
+struct Walk {
+  int b, g, t, nt;          // sequence, kv head, tile of nt
+  int64_t left;             // tiles
+  __device__ __forceinline__ void next(const TreeAttn& A) {
+    --left;
+    if (++t < nt || left <= 0) return;
+    t = 0;
+    if (++g < A.Hkv) return;
+    g = 0;
+    do
+      if (++b >= A.B) {
+        left = 0;
+        return;
+      }
+    while ((nt = tiles_of(A, b)) == 0);
+  }
+};
+
+// Tiles of all sequences and heads; by a whole warp
+__device__ __forceinline__ int64_t all_tiles(const TreeAttn& A) {
+  int64_t total = 0;
+  for (int b0 = 0; b0 < A.B; b0 += 32) {
+    const int b = b0 + (threadIdx.x & 31);
+    int n = b < A.B ? tiles_of(A, b) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    total += n;
+  }
+  return total * A.Hkv;
+}
+__device__ __forceinline__ int64_t share_of(int64_t total, int workers) { return max((total + workers - 1) / workers, static_cast<int64_t>(1)); }
+
+__device__ __forceinline__ Walk walk_of(const TreeAttn& A, int worker, int workers) {
+  const int64_t total = all_tiles(A), share = share_of(total, workers), from = worker * share;
+  Walk w{0, 0, 0, 0, min(share, total - from)};
+  if (w.left <= 0) return w;
+  int64_t before = 0;       // tiles of a head of the sequences before
+  for (int b0 = 0; b0 < A.B; b0 += 32) {
+    const int lane = threadIdx.x & 31, b = b0 + lane;
+    const int n = b < A.B ? tiles_of(A, b) : 0;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, from < (before + upto) * A.Hkv);
+    if (here) {
+      const int first = __ffs(here) - 1;
+      const int nt = __shfl_sync(0xffffffffu, n, first);
+      const int64_t in = from - (before + __shfl_sync(0xffffffffu, upto - n, first)) * A.Hkv;
+      w.b = b0 + first;
+      w.nt = nt;
+      w.g = static_cast<int>(in / nt);
+      w.t = static_cast<int>(in - static_cast<int64_t>(w.g) * nt);
+      return w;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return w;
+}
+
+__device__ __forceinline__ uint32_t line(uint32_t base, int r, int ch, int rows) {     // 16-byte piece ch of row r: blocks of 64 columns, swizzled lines
+  return base + (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+}
+
+template <typename T>
+__device__ __forceinline__ bool no_number(uint32_t two) {        // either half
+  constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+  return (two & e) == e || ((two >> 16) & e) == e;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t numbers_only(uint32_t two) {
+  constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+  if ((two & e) == e) two &= 0xffff0000u;
+  if (((two >> 16) & e) == e) two &= 0xffffu;
+  return two;
+}
+
+// What was left out of the products: values of drafted tokens that are no numbers, columns c .. c + 31 of head g, for a row that sees the tokens `seen` of
+// the keys k0 .. k1 - 1.  Hardly ever called.
+template <typename T, int D>
+__device__ __noinline__ void add_no_numbers(float* o, const TreeAttn& A, int b, int g, int base, int k0, int k1, uint64_t seen, int c) {
+  for (int j = max(k0, base); j < k1; ++j) {
+    if (!(seen >> (j - base) & 1)) continue;
+    const int64_t page = A.block_tables[static_cast<int64_t>(b) * A.table_stride + j / A.bs];
+    if (page < 0 || page >= A.max_blocks) continue;
+    const T* v = static_cast<const T*>(A.v_pool) + ((page * A.Hkv + g) * A.bs + j % A.bs) * D + c;
+    for (int x = 0; x < 32; ++x) {
+      const float f = Cvt<T>::to_f32(v[x]);
+      if (!(fabsf(f) < INFINITY)) o[x] += f;
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT, kCtasPerSm)
+tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using P = Plan<D>;
+  constexpr int NB = P::kBufs;
+  extern __shared__ unsigned char raw_smem[];
+  unsigned char* sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
+  const uint32_t sm0 = smem_u32(sm);
+  // queries in; keys of a buffer in, and read; values of a buffer in; P V of a value buffer done; S of a buffer done, P of a buffer written
+  const uint32_t bar_q = sm0 + P::kBar, bar_k = bar_q + 8, bar_ke = bar_k + 8 * NB, bar_v = bar_ke + 8 * NB, bar_o = bar_v + 8 * NB, bar_s = bar_o + 8 * NB, bar_p = bar_s + 16;
+  volatile uint32_t* tm_slot = reinterpret_cast<volatile uint32_t*>(sm + P::kFlags);
+  volatile int* dead = reinterpret_cast<volatile int*>(sm + P::kFlags + 4);
+  volatile int* strange = reinterpret_cast<volatile int*>(sm + P::kFlags + 8);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int worker = blockIdx.x / W.blocks, block = blockIdx.x - worker * W.blocks;
+  const int rep = A.Hq / A.Hkv, row0 = block * kRows;
+  const int soft_warps = (min(kRows, A.nodes * rep - row0) + 31) / 32;
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (tid == 0) {
+    auto init = [](uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); };
+    init(bar_q, soft_warps * 32);
+    for (int b = 0; b < NB; ++b) {
+      init(bar_k + 8 * b, kLoadK);
+      init(bar_ke + 8 * b, 1);
+      init(bar_v + 8 * b, kLoadV);
+      init(bar_o + 8 * b, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      init(bar_s + 8 * b, 1);
+      init(bar_p + 8 * b, soft_warps * 32);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *dead = 0;
+    *strange = 0;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm0 + P::kFlags), "n"(P::kTm) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = __shfl_sync(0xffffffffu, *tm_slot, 0);
+  Walk w = walk_of(A, worker, W.workers);
+
+  if (warp >= kSoft / 32 && warp < (kSoft + kLoadK + kLoadV) / 32) {
+    // ---- copies ------------------------------------------------------------------------------------------------------------------------------
+    const bool values = warp >= (kSoft + kLoadK) / 32;
+    const int me = tid - kSoft - kLoadK;        // of those that copy values
+    const int my_page = values ? lane * 2 + me / 32 : lane;       // two warps take turns
+    const int box = min(A.bs, kKeys), n_pages = kKeys / box;
+    const uint32_t bar_in = values ? bar_v : bar_k, bar_free = values ? bar_o : bar_ke, bufs = sm0 + (values ? P::kV : P::kK);
+    const CUtensorMap* map = values ? &v_map : &k_map;
+    int keys = 0, n = 0;
+    auto page_of = [&](const Walk& at) -> int64_t {     // this thread's page of a tile; -1: none
+      if (at.left <= 0 || my_page >= n_pages) return -1;
+      int k, d;
+      lengths(A, at.b, &k, &d);
+      const int j = at.t * kKeys + my_page * box;
+      if (j >= k) return -1;
+      const int64_t page = A.block_tables[static_cast<int64_t>(at.b) * A.table_stride + j / A.bs];
+      return page < 0 || page >= A.max_blocks ? A.max_blocks : page;      // (behind the pool: the copy brings zeros)
+    };
+    int64_t page = page_of(w);
+    for (int i = 0; w.left > 0; ++i) {
+      const Walk now = w;
+      lengths(A, now.b, &keys, &n);
+      w.next(A);
+      const int64_t next_page = page_of(w);
+      if (i >= NB) bar_wait(bar_free + 8 * (i % NB), (i / NB - 1) & 1, dead);
+      const uint32_t base = bufs + (i % NB) * (D / 64) * kBlk, bar = bar_in + 8 * (i % NB);
+      const int j0 = now.t * kKeys;
+      if (!values || j0 + kKeys <= keys - n) {
+        if (page >= 0) {
+          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((D / 64) * box * 128) : "memory");
+          const int row = static_cast<int>((page * A.Hkv + now.g) * A.bs) + (A.bs > kKeys ? j0 % A.bs : 0);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(base + c * kBlk + my_page * box * 128),
+                         "l"(map), "r"(64 * c), "r"(row), "r"(bar) : "memory");
+        }
+      } else {
+        bool odd = false;
+        constexpr int kCh = D / 8, kAhead = 4;
+#pragma unroll 1
+        for (int u0 = 0; u0 < kKeys * kCh / kLoadV; u0 += kAhead) {
+          int4 v[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int c = me + (u0 + u) * kLoadV, key = c / kCh, ch = c - key * kCh, j = j0 + key;
+            v[u] = make_int4(0, 0, 0, 0);
+            if (j < keys) {
+              const int64_t pg = A.block_tables[static_cast<int64_t>(now.b) * A.table_stride + j / A.bs];
+              if (pg >= 0 && pg < A.max_blocks) v[u] = *reinterpret_cast<const int4*>(static_cast<const T*>(A.v_pool) + ((pg * A.Hkv + now.g) * A.bs + j % A.bs) * D + ch * 8);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int c = me + (u0 + u) * kLoadV, key = c / kCh, ch = c - key * kCh;
+            uint32_t x[4] = {static_cast<uint32_t>(v[u].x), static_cast<uint32_t>(v[u].y), static_cast<uint32_t>(v[u].z), static_cast<uint32_t>(v[u].w)};
+            if (j0 + key >= keys - n) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                odd = odd || no_number<T>(x[e]);
+                x[e] = numbers_only<T>(x[e]);
+              }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(base, key, ch, kKeys)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+        }
+        if (odd) *strange = 1;
+        fence_smem_to_mma();
+      }
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+      page = next_page;
+    }
+  } else if (warp == kNT / 32 - 1) {
+    // ---- products ----------------------------------------------------------------------------------------------------------------------------
+    auto scores = [&](int i) {
+      const uint32_t k = sm0 + P::kK + (i % NB) * (D / 64) * kBlk;
+      bar_wait(bar_k + 8 * (i % NB), (i / NB) & 1, dead);
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        mma_ss(tm + (i & 1) * kKeys, operand(sm0 + P::kQ + (kk >> 2) * (kRows * 128) + (kk & 3) * 32, 16, 1024),
+               operand(k + (kk >> 2) * kBlk + (kk & 3) * 32, 16, 1024), instr<T>(kKeys, false), kk > 0);
+      mma_commit(bar_s + 8 * (i & 1));
+      mma_commit(bar_ke + 8 * (i % NB));
+    };
+    int i = 0;
+    for (int seg = 0; w.left > 0; ++seg) {
+      const int tiles = static_cast<int>(min(static_cast<int64_t>(w.nt - w.t), w.left));
+      bar_wait(bar_q, seg & 1, dead);       // queries are in, the rows before them out
+      tc_fence_after();
+      scores(i);
+      for (int x = 0; x < tiles; ++x, ++i) {
+        if (x + 1 < tiles) {
+          // S of the next tile goes where P of the one before is being read
+          if (x > 0) bar_wait(bar_o + 8 * ((i - 1) % NB), ((i - 1) / NB) & 1, dead);
+          scores(i + 1);
+        }
+        bar_wait(bar_v + 8 * (i % NB), (i / NB) & 1, dead);
+        bar_wait(bar_p + 8 * (i & 1), (i >> 1) & 1, dead);
+        tc_fence_after();
+        const uint32_t v = sm0 + P::kV + (i % NB) * (D / 64) * kBlk;
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts(tm + P::kO, tm + (i & 1) * kKeys + 8 * kk, operand(v + kk * 2048, kBlk, 1024), instr<T>(D, true), x > 0 || kk > 0);
+        mma_commit(bar_o + 8 * (i % NB));
+      }
+      w.t += tiles - 1;
+      w.left -= tiles - 1;
+      w.next(A);
+    }
+    __syncwarp();
+  } else if (warp < soft_warps) {
+    // ---- softmax: thread = row ---------------------------------------------------------------------------------------------------------------
+    const int node = (row0 + tid) / rep;
+    const uint32_t tm_row = tm + (static_cast<uint32_t>(32 * warp) << 16);
+    const float k2 = A.scale > 0.f ? A.scale * kLog2e : 1.f;       // weight = 2^(s k2 - m)
+    const int per = W.rows;
+    int i = 0;
+    while (w.left > 0) {
+      const int b = w.b, g = w.g, t0 = w.t, tiles = static_cast<int>(min(static_cast<int64_t>(w.nt - w.t), w.left));
+      int keys, n;
+      lengths(A, b, &keys, &n);
+      const int base = keys - n;
+      const bool live = node < n;
+      {
+        constexpr int kCh = D / 8;
+        const T* q = static_cast<const T*>(A.q) + b * A.q_batch_stride;
+#pragma unroll 8
+        for (int u = 0; u < kCh; ++u) {
+          const int c = lane + u * 32, r = 32 * warp + c / kCh, ch = c % kCh;       // a warp's rows by itself
+          const int t = (row0 + r) / rep, h = g * rep + row0 + r - t * rep;
+          const bool in = t < n;
+          cp16(line(sm0 + P::kQ, r, ch, kRows), in ? q + t * A.q_node_stride + static_cast<int64_t>(h) * D + ch * 8 : q, in);
+        }
+        cp_commit();
+        cp_wait<0>();
+        fence_smem_to_mma();
+        tc_fence_before();
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_q) : "memory");
+      }
+      uint64_t seen = live ? static_cast<uint64_t>(A.visible[b * A.visible_stride + node]) : 0ull;
+      if (n < 64) seen &= (1ull << n) - 1;
+      float m_ref = -INFINITY, l = 0.f;     // the maximum in powers of two; -inf until the row sees a key
+      bool ok = true;
+      for (int x = 0; x < tiles; ++x, ++i) {
+        const int j0 = (t0 + x) * kKeys;
+        ok = bar_wait(bar_s + 8 * (i & 1), (i >> 1) & 1, dead) && ok;
+        tc_fence_after();
+        float s[2][32];
+        tm_ld32(s[0], tm_row + (i & 1) * kKeys);
+        tm_ld32(s[1], tm_row + (i & 1) * kKeys + 32);
+        tc_wait_ld();
+        if (A.scale <= 0.f) {
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) s[c >> 5][c & 31] *= A.scale * kLog2e;
+        }
+        if (j0 + kKeys > base) {        // bit c: key j0 + c is seen
+          const int past = base - j0;
+          const uint64_t keep = past > 0 ? (seen << past) | ((1ull << past) - 1) : (past > -64 ? seen >> -past : 0ull);
+          const uint32_t half[2] = {static_cast<uint32_t>(keep), static_cast<uint32_t>(keep >> 32)};
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c)
+            if (!(half[c >> 5] >> (c & 31) & 1)) s[c >> 5][c & 31] = -INFINITY;
+        }
+        float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+        for (int c = 4; c < kKeys - 4; c += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], s[c >> 5][(c & 31) + u], s[(c + 4) >> 5][((c + 4) & 31) + u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[1][28 + u]);
+        const float m_new = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * k2;
+        const bool grow = m_new > m_ref;
+        const float corr = grow ? exp2_fast(m_ref - m_new) : 1.0f;      // 0 where nothing was seen before
+        if (grow) m_ref = m_new;
+        if (x > 0 && __any_sync(0xffffffffu, grow)) {
+          ok = bar_wait(bar_o + 8 * ((i - 1) % NB), ((i - 1) / NB) & 1, dead) && ok;
+          tc_fence_after();
+          scale_rows<D, 16>(tm_row + P::kO, corr);
+        }
+        const f32x2 kk = both(k2), mm = both(m_ref == -INFINITY ? 0.f : -m_ref);      // a row that sees no key yet keeps weights 0
+        f32x2 sum[2] = {0ull, 0ull};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          uint32_t p[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float u = s[y][c], v = s[y][c + 1];
+            scale_shift(u, v, kk, mm);
+            u = exp2_fast(u);
+            v = exp2_fast(v);
+            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pair(u, v));
+            p[c >> 1] = pack2<T>(u, v);
+          }
+          tm_st16(tm_row + (i & 1) * kKeys + y * 16, p);
+        }
+        float part[4];
+        apart(part[0], part[1], sum[0]);
+        apart(part[2], part[3], sum[1]);
+        l = fmaf(l, corr, (part[0] + part[1]) + (part[2] + part[3]));
+        tc_wait_st();
+        tc_fence_before();
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_p + 8 * (i & 1)) : "memory");
+      }
+      ok = bar_wait(bar_o + 8 * ((i - 1) % NB), ((i - 1) / NB) & 1, dead) && ok;
+      tc_fence_after();
+      ok = ok && !*dead;
+      const bool whole = t0 == 0 && tiles == w.nt, odd = *strange != 0;
+      const int64_t piece = (static_cast<int64_t>(worker) * W.blocks + block) * 2 + (t0 == 0);
+      float f = 1.f;
+      if (whole) f = ok ? (l == 0.f ? 0.f : 1.0f / l) : NAN;
+      else if (tid < per) W.ml[piece * per + tid] = make_float2(m_ref, ok ? l : NAN);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        __syncwarp();
+        tm_ld32(o, tm_row + P::kO + c);
+        tc_wait_ld();
+        if (odd && live) {
+          float other[32];      // (an array that a function sees is kept in memory)
+#pragma unroll
+          for (int u = 0; u < 32; ++u) other[u] = o[u];
+          add_no_numbers<T, D>(other, A, b, g, base, t0 * kKeys, min((t0 + tiles) * kKeys, keys), seen, c);
+#pragma unroll
+          for (int u = 0; u < 32; ++u) o[u] = other[u];
+        }
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < 32; u += 4) W.o[(piece * (D / 4) + (c + u) / 4) * per + tid] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 32; u += 8) {
+            uint32_t p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = pack2<T>(o[u + 2 * e] * f, o[u + 2 * e + 1] * f);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(sm0 + P::kQ, tid, (c + u) / 8, kRows)), "r"(p[0]), "r"(p[1]), "r"(p[2]),
+                         "r"(p[3]) : "memory");
+          }
+        }
+      }
+      if (whole) {      // from where the warp's queries were (they have been read), rows side by side
+        __syncwarp();
+        constexpr int kCh = D / 8;
+#pragma unroll 4
+        for (int u = 0; u < kCh; ++u) {
+          const int c = lane + u * 32, r = c / kCh, ch = c % kCh, at = row0 + 32 * warp + r, t = at / rep, h = g * rep + at - t * rep;
+          if (t < n) {
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(line(sm0 + P::kQ, 32 * warp + r, ch, kRows)) : "memory");
+            *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + ((static_cast<int64_t>(b) * A.nodes + t) * A.Hq + h) * D + ch * 8) = v;
+          }
+        }
+        __syncwarp();
+      }
+      w.t += tiles - 1;
+      w.left -= tiles - 1;
+      w.next(A);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(P::kTm));
+}
+
+// One CTA per (sequence and kv head, 32 rows): what the workers' ends cut in pieces is put together, rows without a node become 0.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttn A, const Shares W) {
+  const int b = blockIdx.x / A.Hkv, g = blockIdx.x - b * A.Hkv, rep = A.Hq / A.Hkv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at0 = blockIdx.y * 32, row = at0 + lane, t = row / rep, h = g * rep + row - t * rep;
+  int keys, n;
+  lengths(A, b, &keys, &n);
+  const int nt = tiles_of(A, b);
+  int64_t before = 0, all = 0;
+  for (int b0 = 0; b0 < A.B; b0 += 32) {
+    int m = b0 + lane < A.B ? tiles_of(A, b0 + lane) : 0, low = b0 + lane < b ? m : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o), low += __shfl_xor_sync(0xffffffffu, low, o);
+    all += m;
+    before += low;
+  }
+  const int64_t share = share_of(all * A.Hkv, W.workers), from = before * A.Hkv + static_cast<int64_t>(g) * nt;
+  const int first = static_cast<int>(from / share), last = nt > 0 ? static_cast<int>((from + nt - 1) / share) : first;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (row >= A.nodes * rep) return;
+  T* out = static_cast<T*>(A.out) + ((static_cast<int64_t>(b) * A.nodes + t) * A.Hq + h) * D;
+  if (t < n && first == last) return;
+  const int in_block = row % kRows, block = row / kRows;
+  float top = -INFINITY, sum = 0.f;
+  bool odd = false;
+  if (t < n) {
+    for (int p = first; p <= last; ++p) {
+      const float2 ml = W.ml[((static_cast<int64_t>(p) * W.blocks + block) * 2 + (p == first)) * W.rows + in_block];
+      odd = odd || ml.y != ml.y;
+      top = fmaxf(top, ml.x);
+    }
+  }
+  for (int c4 = warp; c4 < D / 4; c4 += 8) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    sum = 0.f;
+    if (t < n) {
+      for (int p = first; p <= last; ++p) {
+        const int64_t piece = (static_cast<int64_t>(p) * W.blocks + block) * 2 + (p == first);
+        const float2 ml = W.ml[piece * W.rows + in_block];
+        if (ml.x == -INFINITY) continue;
+        const float k = exp2_fast(ml.x - top);
+        const float4 v = W.o[(piece * (D / 4) + c4) * W.rows + in_block];
+        sum = fmaf(ml.y, k, sum);
+        o.x = fmaf(v.x, k, o.x), o.y = fmaf(v.y, k, o.y), o.z = fmaf(v.z, k, o.z), o.w = fmaf(v.w, k, o.w);
+      }
+      const float f = odd ? NAN : (sum == 0.f ? 0.f : 1.0f / sum);
+      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+    }
+    *reinterpret_cast<uint2*>(out + c4 * 4) = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
+  }
+}
+
+// The pool as rows, fetched in boxes of 64 columns x a page (or 64 rows of one); rows behind the pool read as zeros.  Made for the launch and not kept.
+template <typename T>
+bool pool_map(CUtensorMap* map, const void* pool, const TreeAttn& A) {
+  const Encode encode = tensor_map_encode();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(A.D), static_cast<cuuint64_t>(A.max_blocks * A.Hkv * A.bs)}, strides[1] = {2ull * A.D};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(std::min(A.bs, kKeys))}, step[2] = {1, 1};
+  return encode(map, std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(pool),
+                dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+Shares shares_of(int nodes, int Hq, int Hkv) {
+  Shares W{};
+  const int rows = nodes * (Hq / Hkv);
+  W.blocks = (rows + kRows - 1) / kRows;
+  W.rows = std::min(kRows, (rows + 31) / 32 * 32);
+  W.workers = std::max(1, kCtasPerSm * kNumSMs / W.blocks);
+  return W;
+}
+size_t sums_bytes(const Shares& W) { return static_cast<size_t>(W.workers) * W.blocks * 2 * W.rows * sizeof(float2); }
+
+bool tiles_serve(int Hq, int Hkv, int D, int bs, int dtype) {
+  return (dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16) && (D == 64 || D == 128) && ((bs >= 8 && kKeys % bs == 0) || bs % kKeys == 0) && Hq / Hkv <= 1 << 16;
+}
+
+template <typename T, int D>
+int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap& v_map, void* workspace, cudaStream_t stream) {
+  const char* name = "b200_paged_tree_attn";
+  Shares W = shares_of(A.nodes, A.Hq, A.Hkv);
+  W.ml = static_cast<float2*>(workspace);
+  W.o = reinterpret_cast<float4*>(static_cast<char*>(workspace) + sums_bytes(W));
+  auto kern = tree_attn_kernel<T, D>;
+  constexpr int smem = Plan<D>::kEnd + 1024;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  kern<<<W.workers * W.blocks, kNT, smem, stream>>>(A, W, k_map, v_map);
+  if (int rc = check_launch(name)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(A.B) * A.Hkv, (A.nodes * (A.Hq / A.Hkv) + 31) / 32);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D>, A, static_cast<const Shares>(W));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
+  }
+  return 0;
+}
+
 template <typename T>
 int launch_any(const TreeAttn& A, cudaStream_t stream) {
   if (A.D > kAnyMostD) return fail(B200_ESHAPE, "b200_paged_tree_attn: head size %d, at most %d", A.D, kAnyMostD);
@@ -129,7 +690,11 @@ using namespace b200;
 
 extern "C" {
 
-size_t b200_paged_tree_attn_workspace(int B, int nodes, int Hq, int Hkv, int D, int block_size, int dtype) { return 0; }
+size_t b200_paged_tree_attn_workspace(int B, int nodes, int Hq, int Hkv, int D, int block_size, int dtype) {
+  if (nodes <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || !tiles_serve(Hq, Hkv, D, block_size, dtype)) return 0;
+  const Shares W = shares_of(nodes, Hq, Hkv);
+  return sums_bytes(W) + static_cast<size_t>(W.workers) * W.blocks * 2 * W.rows * D * sizeof(float);
+}
 
 int b200_paged_tree_attn(void* out, const void* q, int64_t q_batch_stride, int64_t q_node_stride, const void* k_pool, const void* v_pool,
                          const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, const int32_t* draft_lens,
@@ -147,6 +712,21 @@ int b200_paged_tree_attn(void* out, const void* q, int64_t q_batch_stride, int64
   const TreeAttn A{out, q, k_pool, v_pool, q_batch_stride, q_node_stride, block_tables, table_stride, table_cols, context_lens, draft_lens, visible,
                    visible_stride, B, nodes, Hq, Hkv, D, block_size, max_blocks, scale};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // rows of 16-byte pieces, pages and rows whose numbers fit
+  const bool pieces = aligned16(q) && aligned16(out) && aligned16(k_pool) && aligned16(v_pool) && q_batch_stride % 8 == 0 && q_node_stride % 8 == 0;
+  if (tiles_serve(Hq, Hkv, D, block_size, dtype) && !(flags & B200_ATTN_FORCE_GENERIC) && pieces && max_blocks < INT32_MAX / (static_cast<int64_t>(Hkv) * block_size) - 1 &&
+      static_cast<int64_t>(B) * Hkv <= INT32_MAX && nodes * static_cast<int64_t>(Hq / Hkv) <= 32 * 65535) {
+    if (!workspace || workspace_bytes < b200_paged_tree_attn_workspace(B, nodes, Hq, Hkv, D, block_size, dtype))
+      return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace_bytes);
+    if (!aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
+    CUtensorMap k_map, v_map;
+    auto go = [&](auto* tag) {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      if (!pool_map<T>(&k_map, k_pool, A) || !pool_map<T>(&v_map, v_pool, A)) return fail(B200_EINVAL, "%s: no tensor map of the pools", name);
+      return D == 128 ? launch_tiles<T, 128>(A, k_map, v_map, workspace, s) : launch_tiles<T, 64>(A, k_map, v_map, workspace, s);
+    };
+    return dtype == B200_DTYPE_BF16 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr));
+  }
   switch (dtype) {
     case B200_DTYPE_F16: return launch_any<__half>(A, s);
     case B200_DTYPE_BF16: return launch_any<__nv_bfloat16>(A, s);
