@@ -2,19 +2,25 @@
 //
 //   w_i   = 2^((x_i - max x) * log2(e) / t), 0 for -inf
 //   order = descending logits, the lowest index first among equals
-//   kept  = the first k of the order; of these the ones before which the weights sum to less than p of theirs all; of these w_i >= min_p
-//           (each a beginning of the order: what is kept is the keys above some key, and the first m of that key itself)
+//   kept  = the first k of the order; of these the ones before which the weights sum to less than p of theirs all; of these w_i >= min_p:
+//           a beginning of the order, down to some (key, index)
 //   token = the first index, in the row's own order, up to which the kept weights sum to more than u of them all
 //
-// Whether a token is the one decides on sums of up to a quarter of a million weights, next to a border more often than 32 bits tell apart: the
-// weights are computed in 64 bits (argument reduced to 1/256 of a power of two, table and a polynomial of degree 4 after Tang's table-driven exponential,
-// 2^-52) and summed as whole numbers of 2^-frac (frac = 62 - log2 of the row's length, 45 for 128 k): sums do not depend on their order, so
-// neither does the token on how rows are spread over CTAs, on warps or on atomics.
+// Whether a token is the one decides on sums of up to a million weights.  They are summed as whole numbers of 2^-frac (frac = 62 - log2 of the row's
+// length, at most 44), so no sum depends on its order: neither on how a row is spread over CTAs, nor on warps or atomics.  A weight is computed in
+// pairs of floats to 2^-31 of itself (256 steps of a power of two from a table, a polynomial of degree 3 between them, after Tang's table-driven
+// exponential): errors of independent weights leave one token in 10^7 rows of 128 k another one than 64 bits would.
 //
-// A row has a cluster of CTAs; each holds its part of the row in shared memory from the only pass over it, if the parts fit.  Blocks of 256 elements, eight
-// side by side per lane.  Passes: (1) load, maximum; (2) where k limits: the k-th key by its digits of 8 bits, from counts; (3) where p does: the same from
-// sums of weights; (4) kept weights per block; then the block, the lane and the element in which u falls.  Digits are counted in 16 columns per
-// digit, one for every other lane, so that logits of few exponents do not meet at few addresses.
+// A row has a cluster of CTAs; each holds its part of the row in shared memory from the only pass over it in memory, if the parts fit.  Blocks of 256
+// elements, eight side by side per lane.
+//   all rows        load, maximum
+//   k, or p         numbers of elements in 1024 ranges of log w (0 .. -46).  k: all elements down to the range that the k-th is in go in a list; p: from
+//                   the middles of the ranges it is known to some tenths of a per cent where the weights sum to p of all, the elements of these ranges go in
+//                   the list, and exact sums are taken of what is above and of all
+//   list (4096)     sorted by the cluster's first CTA, cut by k, p and min_p; where nothing is above the list, what it keeps is sorted by index and drawn from
+//   other rows      kept weights of each block; the block, the lane and the element in which u falls
+// Where that does not serve - k over 2048, or ranges of more than 4096 elements, equal logits above all - the last key is found by its digits of 8 bits
+// from counts or sums in the whole row.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -27,9 +33,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBlock = 256;         // elements
-constexpr int kDigits = 256, kColumns = 16;
+constexpr int kRanges = 1024, kRangeColumns = 8;        // columns: lanes that fall in the same range meet at fewer addresses
+constexpr int kDigits = 256, kColumns = 8;
+constexpr int kList = 4096, kMostK = 2048;
 using u64 = unsigned long long;
 
 struct Sample {
@@ -71,6 +79,19 @@ template <>
 __device__ __forceinline__ float value<__half>(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
 template <>
 __device__ __forceinline__ float value<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+// largest of two, NaN if one is
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 template <typename T>
 constexpr uint32_t kMinusInf = sizeof(T) == 4 ? 0xff800000u : (std::is_same_v<T, __half> ? 0xfc00u : 0xff80u);
 
@@ -84,38 +105,63 @@ struct Eight {      // bits of eight elements
 };
 
 struct alignas(16) Shared {
-  double table[256];                            // 2^(j / 256)
-  uint32_t cnt[kDigits * kColumns], lo[kDigits * kColumns], hi[kDigits * kColumns];
-  u64 mass[2][kDigits];                         // this CTA's sums, read by the cluster
-  uint32_t count[2][kDigits];
-  u64 all_mass[kDigits];                        // the cluster's
-  uint32_t all_count[kDigits];
-  u64 warp_part[kWarps];
-  u64 best;                                     // read by the cluster
-  u64 kept;
-  u64 equal;
-  u64 level[4];                                 // digit, sum above it, count and mass in it
-  u64 at[4];
+  uint2 table[256];             // 2^(30 + j / 256): as a whole number, as a float
+  union {
+    uint32_t ranges[kRanges * kRangeColumns];
+    struct {
+      uint32_t cnt[kDigits * kColumns], lo[kDigits * kColumns], hi[kDigits * kColumns];
+    };
+    u64 list[kList];
+  };
+  union {
+    uint32_t range_count[kRanges];      // this CTA's, read by the cluster
+    struct {
+      u64 mass[2][kDigits];             // likewise
+      uint32_t count[2][kDigits];
+      u64 all_mass[kDigits];            // the cluster's
+      uint32_t all_count[kDigits];
+    };
+  };
+  u64 part[kWarps];
+  // read by the cluster
+  uint32_t best;                        // largest key
+  uint32_t first;                       // lowest index of the row's maximum
+  uint32_t listed;
+  int failed;
+  u64 sum_all, sum_above, kept, equal;
+  u64 cut;                              // (key, ~index) of the last that is kept
+  // this CTA's
+  u64 level[4], at[4];
+  int from, to, n;
 };
 
-// weights
+// weights, as whole numbers of 2^-frac
+template <typename T>
 struct Weigh {
-  double top, scale;        // maximum; 256 log2(e) / t
-  double one, least;        // 2^(52 - frac), whose last bit is 2^-frac; arguments below this are weights of 0
-  const double* table;
-  __device__ __forceinline__ double operator()(float x) const {
-    const double y = (static_cast<double>(x) - top) * scale;
-    if (!(y > least)) return 0.0;
-    const double shift = 6755399441055744.0;     // 3 * 2^51: the nearest whole number is in the last bits
-    const double r = y + shift;
-    const int n = __double2loint(r);
-    const double f = y - (r - shift);
-    constexpr double c1 = 0.69314718055994530942 / 256, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
-    const double p = fma(fma(fma(fma(f, c4, c3), f, c2), f, c1), f, 1.0);
-    const double w = table[n & 255] * p;
-    return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w));
+  float top, scale, scale_low, lowest;  // maximum; 256 log2(e) / t in two parts; arguments from this on down give 0
+  int up;                               // frac - 30
+  const uint2* table;
+  __device__ __forceinline__ float argument(float x) const { return __fmul_rn(x - top, scale); }
+  __device__ __forceinline__ bool some(float y) const { return y > lowest; }        // not of no number: -inf without a scale
+  __device__ __forceinline__ u64 operator()(float x) const {
+    const float d = x - top, y = __fmul_rn(d, scale);
+    if (!some(y)) return 0;
+    float low = fmaf(d, scale_low, fmaf(d, scale, -y));
+    if constexpr (sizeof(T) == 4) {     // what the difference lost (Knuth's sum); one of 16-bit numbers that matters loses nothing
+      const float v = d - x;
+      low = fmaf((x - (d - v)) - (top + v), scale, low);
+    }
+    const float shift = 12582912.f, r = y + shift;        // 3 * 2^22: the nearest whole number is in the last bits
+    const int n = __float_as_int(r) - 0x4b400000;
+    const float f = (y - (r - shift)) + low;
+    constexpr float c1 = 0.69314718055994530942 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
+    const uint2 step = table[n & 255];
+    const float q = f * fmaf(fmaf(f, c3, c2), f, c1);
+    const uint32_t w = step.x + (__float_as_int(fmaf(q, __uint_as_float(step.y), shift)) - 0x4b400000);
+    return (static_cast<u64>(w) << up) >> -(n >> 8);
   }
-  __device__ __forceinline__ u64 whole(double w) const { return __double_as_longlong(w + one) - __double_as_longlong(one); }
+  // range of an argument
+  __device__ __forceinline__ int range(float y) const { return __float_as_int(fmaf(y, -1.0f / 11.5f, 8388608.f)) & (kRanges - 1); }
 };
 
 template <typename V>
@@ -125,32 +171,63 @@ __device__ __forceinline__ V warp_sum_of(V v) {
   return v;
 }
 // sum of the values of lower lanes
-__device__ __forceinline__ u64 warp_before(u64 v) {
-  u64 s = v;
+template <typename V>
+__device__ __forceinline__ V warp_before(V v) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 up = __shfl_up_sync(0xffffffffu, s, o);
-    if ((threadIdx.x & 31) >= o) s += up;
+    const V up = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += up;
   }
-  return s - v;
+  const V shifted = __shfl_up_sync(0xffffffffu, v, 1);
+  return (threadIdx.x & 31) ? shifted : V(0);
 }
 // sum of the values of lower threads; *all: of the CTA's
-__device__ __forceinline__ u64 cta_before(u64 v, u64* part, u64* all) {
+template <typename V>
+__device__ __forceinline__ V cta_before(V v, V* part, V* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const u64 in_warp = warp_before(v);
+  const V in_warp = warp_before(v);
   __syncthreads();
   if (lane == 31) part[warp] = in_warp + v;
   __syncthreads();
-  u64 before = 0, total = 0;
-  const u64 mine = part[lane];
-  before = warp_sum_of(lane < warp ? mine : 0ull);
-  total = warp_sum_of(mine);
+  V before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const V x = part[w];
+    if (w < warp) before += x;
+    total += x;
+  }
   *all = total;
   return before + in_warp;
 }
 
+// the first n of `list` in descending order; what is behind them, up to the next power of two, is overwritten
+__device__ __forceinline__ void sort_down(u64* list, int n) {
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2) {
+    for (int step = run / 2; step > 0; step /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int at = 2 * i - (i & (step - 1));
+        const u64 a = list[at], b = list[at + step];
+        if ((a < b) == ((at & run) == 0)) list[at] = b, list[at + step] = a;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// f of 2^64, within 0 .. 2^64 - 1; not a number: 0
+__device__ __forceinline__ u64 fraction(float f) { return f > 0.f ? (f < 1.f ? static_cast<u64>(static_cast<double>(f) * 18446744073709551616.0) : ~0ull) : 0ull; }
+// weights before a kept one sum to less than this: the next whole number from p of `all` on
+__device__ __forceinline__ u64 limit_of(float p, u64 all) {
+  const u64 f = fraction(p);
+  return max(__umul64hi(f, all) + (f * all ? 1 : 0), 1ull);
+}
+
 template <typename T, bool HELD>
-__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const Sample A) {
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   Shared& S = *reinterpret_cast<Shared*>(dynamic);
   cg::cluster_group cluster = cg::this_cluster();
@@ -165,8 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const Sample A
   const int block0 = rank * A.blocks_per_cta;
   const int n_blocks = max(0, min(A.blocks_per_cta, (end + kBlock - 1) / kBlock - block0));
   u64* block_mass = reinterpret_cast<u64*>(dynamic + sizeof(Shared));
-  uint32_t* block_equal = reinterpret_cast<uint32_t*>(block_mass + ((A.blocks_per_cta + 1) & ~1));
-  uint32_t* held = block_equal + ((A.blocks_per_cta + 3) & ~3);
+  uint32_t* held = reinterpret_cast<uint32_t*>(block_mass + ((A.blocks_per_cta + 1) & ~1));
   constexpr int kWords = sizeof(T) * 2;     // of eight elements
 
   auto from_memory = [&](int block) {       // what is not the row's reads as -inf
@@ -208,219 +284,425 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const Sample A
       return from_memory(block);
     }
   };
+  auto index_of = [&](int block, int e) { return (block0 + block) * kBlock + lane * 8 + e - head; };
+  auto composite = [&](float f, int index) { return static_cast<u64>(Key<float>::of(__float_as_uint(f))) << 32 | (0xffffffffu - static_cast<uint32_t>(index)); };
+  auto logit_of = [&](u64 c) { return __uint_as_float(Key<float>::bits(static_cast<uint32_t>(c >> 32))); };
 
-  // ---- the largest logit and where it is first ---------------------------------------------------------------------------------------------
-  if (tid < 256) S.table[tid] = exp2(tid / 256.0);
-  u64 best = 0;
-  for (int b = warp; b < n_blocks; b += kWarps) {
-    const Eight<T> v = from_memory(b);
-    if constexpr (HELD) {
-      uint4* p = reinterpret_cast<uint4*>(held + (b * 32 + lane) * kWords);
-#pragma unroll
-      for (int c = 0; c < kWords; c += 4) p[c / 4] = make_uint4(v.w[c], v.w[c + 1], v.w[c + 2], v.w[c + 3]);
-    }
-    const int at = (block0 + b) * kBlock + lane * 8 - head;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float f = value<T>(v[e]);
-      const uint32_t order = f != f ? 0xffffffffu : Key<float>::of(__float_as_uint(f));
-      const u64 key = static_cast<u64>(order) << 32 | (0xffffffffu - static_cast<uint32_t>(at + e));
-      if (at + e >= 0 && at + e < A.cols && key > best) best = key;
-    }
+  // ---- the largest logit ---------------------------------------------------------------------------------------------------------------------
+  if (tid < 256) {
+    const double step = exp2(30.0 + tid / 256.0);
+    S.table[tid] = make_uint2(static_cast<uint32_t>(__double2ll_rn(step)), __float_as_uint(static_cast<float>(step)));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) S.warp_part[warp] = best;
+  if (tid == 0) S.first = 0xffffffffu, S.listed = 0, S.failed = 0, S.sum_all = S.sum_above = 0, S.best = 0;
   __syncthreads();
-  if (warp == 0) {
-    best = S.warp_part[lane];
+  float top = -INFINITY;
+  {
+    constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+    [[maybe_unused]] uint32_t top2 = kMinusInf<T> | kMinusInf<T> << 16;
+    for (int b = warp; b < n_blocks; b += kAhead * kWarps) {
+      Eight<T> v[kAhead];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) S.best = best;
+      for (int u = 0; u < kAhead; ++u)
+        if (b + u * kWarps < n_blocks) v[u] = from_memory(b + u * kWarps);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (b + u * kWarps >= n_blocks) break;
+        if constexpr (HELD) {
+          uint4* p = reinterpret_cast<uint4*>(held + ((b + u * kWarps) * 32 + lane) * kWords);
+#pragma unroll
+          for (int c = 0; c < kWords; c += 4) p[c / 4] = make_uint4(v[u].w[c], v[u].w[c + 1], v[u].w[c + 2], v[u].w[c + 3]);
+        }
+#pragma unroll
+        for (int c = 0; c < kWords; ++c) {
+          if constexpr (sizeof(T) == 4) top = larger(top, __uint_as_float(v[u].w[c]));
+          else top2 = larger2<T>(top2, v[u].w[c]);
+        }
+      }
+    }
+    if constexpr (sizeof(T) == 2) top = larger(value<T>(top2 & 0xffffu), value<T>(top2 >> 16));
+    const uint32_t mine = __reduce_max_sync(0xffffffffu, top != top ? 0xffffffffu : Key<float>::of(__float_as_uint(top)));
+    if (lane == 0) atomicMax(&S.best, mine);
   }
   cluster.sync();
-  best = 0;
+  uint32_t best = 0;
   for (int r = 0; r < n_cta; ++r) best = max(best, *cluster.map_shared_rank(&S.best, r));
-  const float top = __uint_as_float(Key<float>::bits(static_cast<uint32_t>(best >> 32)));
+  top = __uint_as_float(best == 0xffffffffu ? 0x7fffffffu : Key<float>::bits(best));
   const float t = A.temperature ? A.temperature[row] : A.t0;
-  // no temperature, or a largest logit that is no number: the greedy token
-  if (!(t > 0.f) || !(fabsf(top) < INFINITY)) {
-    if (rank == 0 && tid == 0) A.out[row] = 0xffffffffu - static_cast<uint32_t>(best);
-    cluster.sync();       // the others may still read this CTA's
+  if (!(t > 0.f) || !(fabsf(top) < INFINITY)) {      // no temperature, or a largest logit that is no number: the first of the largest
+    uint32_t first = 0xffffffffu;
+    for (int b = warp; b < n_blocks; b += kWarps) {
+      const Eight<T> v = load(b);
+#pragma unroll
+      for (int e = 7; e >= 0; --e) {
+        const float f = value<T>(v[e]);
+        const int index = index_of(b, e);
+        if ((f == top || (f != f && top != top)) && index >= 0 && index < A.cols) first = min(first, static_cast<uint32_t>(index));
+      }
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0 && first != 0xffffffffu) atomicMin(cluster.map_shared_rank(&S.first, 0), first);
+    cluster.sync();
+    if (rank == 0 && tid == 0) A.out[row] = S.first;
     return;
   }
   int k = A.top_k ? A.top_k[row] : A.k0;
-  float p = A.top_p ? A.top_p[row] : A.p0, least = A.min_p ? A.min_p[row] : A.m0, u = A.u[row];
+  const float p = A.top_p ? A.top_p[row] : A.p0, least = A.min_p ? A.min_p[row] : A.m0, u = A.u[row];
   if (k <= 0 || k >= A.cols) k = 0;
   const bool by_mass = p < 1.0f;
-  least = least > 0.f ? fminf(least, 1.0f) : 0.f;       // not a number: no limit
-  Weigh weigh;
-  weigh.top = top;
-  weigh.scale = 369.32993046757463 / static_cast<double>(t);     // 256 log2(e)
-  weigh.one = __hiloint2double((1023 + 52 - A.frac) << 20, 0);
-  weigh.least = -256.0 * (A.frac + 2);
-  weigh.table = S.table;
+  // not a number: no limit
+  const u64 least_weight = least > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(least, 1.0f)) * static_cast<double>(1ull << A.frac))) : 0ull;
+  Weigh<T> weigh;
+  {
+    const double scale = 369.32993046757463 / static_cast<double>(t);     // 256 log2(e)
+    weigh.top = top;
+    weigh.scale = static_cast<float>(fmin(scale, 3e38));
+    weigh.scale_low = scale < 3e38 ? static_cast<float>(scale - weigh.scale) : 0.f;
+    weigh.lowest = -256.0f * (A.frac + 1);
+    weigh.up = A.frac - 30;
+    weigh.table = S.table;
+  }
 
-  // ---- the key that a number of elements, or a sum of weights, ends in ----------------------------------------------------------------------
-  // Of the elements of key >= lowest: the key at which the running count (by weight: sum) from the largest on reaches `target`.  What is still
-  // to be reached in it is left in *rest, its elements in *equal.  target 0: `share` of the sum of all, less `minus`.
-  int parity = 0;
-  auto select = [&](auto weighted, uint32_t lowest, u64 target, float share, u64 minus, u64* rest, u64* equal) -> uint32_t {
-    constexpr bool WEIGHTED = decltype(weighted)::value;
-    uint32_t prefix = 0;
-    for (int shift = Key<T>::kBits - 8; shift >= 0; shift -= 8) {
-      for (int i = tid; i < kDigits * kColumns; i += kThreads) {
-        S.cnt[i] = 0;
-        if (WEIGHTED) S.lo[i] = S.hi[i] = 0;
+  u64 cut = 0;            // kept: (key, ~index) from this on
+  bool summed = false;    // the blocks' sums are there already
+  bool search = k || by_mass;
+  if (search && k <= kMostK) {
+    // ---- elements in each range of log w --------------------------------------------------------------------------------------------------------
+    for (int i = tid; i < kRanges * kRangeColumns / 4; i += kThreads) reinterpret_cast<uint4*>(S.ranges)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int b = warp; b < n_blocks; b += kWarps) {
+      const Eight<T> v = load(b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = weigh.argument(value<T>(v[e]));
+        if (weigh.some(y)) atomicAdd(&S.ranges[weigh.range(y) * kRangeColumns + (lane & (kRangeColumns - 1))], 1u);
+      }
+    }
+    __syncthreads();
+    constexpr int kMine = kRanges / kThreads;
+    uint32_t c[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      c[i] = 0;
+#pragma unroll
+      for (int j = 0; j < kRangeColumns; j += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(&S.ranges[(tid * kMine + i) * kRangeColumns + j]);
+        c[i] += q.x + q.y + q.z + q.w;
+      }
+      S.range_count[tid * kMine + i] = c[i];
+    }
+    if (tid == 0) S.from = 0, S.to = kRanges - 1;
+    cluster.sync();
+    // numbers, and weights as the middles of the ranges have them (whole numbers: the same sums in all CTAs)
+    u64 m[kMine], m_mine = 0, m_all, n_mine = 0, n_all;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      c[i] = 0;
+      for (int r = 0; r < n_cta; ++r) c[i] += cluster.map_shared_rank(S.range_count, r)[tid * kMine + i];
+      m[i] = c[i] * static_cast<u64>(exp2f(40.f - (tid * kMine + i) * (11.5f / 256.f)));
+      n_mine += c[i];
+      m_mine += m[i];
+    }
+    u64 n = cta_before(n_mine, S.part, &n_all);
+    int listing;
+    if (k) {       // down to the range of the k-th
+      if (tid == 0) S.n = static_cast<int>(n_all);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (n < k && k <= n + c[i]) S.to = tid * kMine + i, S.n = static_cast<int>(n + c[i]);
+        n += c[i];
       }
       __syncthreads();
+      listing = S.n;
+    } else {       // the ranges within 0.3 % of the whole around p of it
+      u64 before = cta_before(m_mine, S.part, &m_all);
+      const u64 low = __umul64hi(fraction(p - 0.003f), m_all), high = __umul64hi(fraction(p + 0.003f), m_all) + 1;
+      if (tid == 0) S.at[0] = 0, S.at[1] = n_all;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        if (before < low && low <= before + m[i]) S.from = tid * kMine + i, S.at[0] = n;
+        if (before < high && high <= before + m[i]) S.to = tid * kMine + i, S.at[1] = n + c[i];
+        n += c[i];
+        before += m[i];
+      }
+      __syncthreads();
+      const bool all_of_it = S.at[1] <= kList;        // nothing above the list
+      listing = static_cast<int>(all_of_it ? S.at[1] : S.at[1] - S.at[0]);
+      __syncthreads();
+      if (all_of_it && tid == 0) S.from = 0;
+      __syncthreads();
+    }
+    const int from = S.from, to = S.to;
+    if (listing <= kList) {       // (the same in all CTAs)
+      // ---- the list; a row without k: exact sums of all, of what is above the list, and of the blocks' part of that ------------------------------
+      u64 all = 0, above = 0;
       for (int b = warp; b < n_blocks; b += kWarps) {
         const Eight<T> v = load(b);
+        u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint32_t key = Key<T>::of(v[e]);
-          if (key < lowest || (shift + 8 < 32 && key >> (shift + 8) != prefix)) continue;
-          const int slot = ((key >> shift) & 255) * kColumns + (lane & (kColumns - 1));
-          atomicAdd(&S.cnt[slot], 1u);
-          if constexpr (WEIGHTED) {
-            const u64 w = weigh.whole(weigh(value<T>(v[e])));
-            if (w) {
-              const uint32_t old = atomicAdd(&S.lo[slot], static_cast<uint32_t>(w));
-              const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + static_cast<uint32_t>(w) < old ? 1u : 0u);
-              if (up) atomicAdd(&S.hi[slot], up);
+          const float f = value<T>(v[e]), y = weigh.argument(f);
+          const int range = weigh.some(y) ? weigh.range(y) : kRanges;
+          if (range >= from && range <= to) {
+            const uint32_t at = atomicAdd(&S.listed, 1u);
+            if (at < kList) S.list[at] = composite(f, index_of(b, e));
+          }
+          if (!k) {
+            const u64 w = weigh(f);
+            all += w;
+            if (range < from) {
+              above += w;
+              if (w >= least_weight) sum += w;
+            }
+          }
+        }
+        if (from > 0) {
+          sum = warp_sum_of(sum);
+          if (lane == 0) block_mass[b] = sum;
+        }
+      }
+      if (!k) {
+        all = warp_sum_of(all);
+        above = warp_sum_of(above);
+        if (lane == 0) {
+          atomicAdd(&S.sum_all, all);
+          atomicAdd(&S.sum_above, above);
+        }
+      }
+      cluster.sync();
+      if (rank == 0) {
+        int listed = S.listed;
+        for (int r = 1; r < n_cta; ++r) {
+          const int more = min(static_cast<int>(*cluster.map_shared_rank(&S.listed, r)), kList - listed);
+          const u64* theirs = cluster.map_shared_rank(S.list, r);
+          for (int i = tid; i < more; i += kThreads) S.list[listed + i] = theirs[i];
+          listed += more;
+        }
+        sort_down(S.list, listed);
+        u64 whole = 0, over = 0;
+        if (!k) {
+          for (int r = 0; r < n_cta; ++r) {
+            whole += *cluster.map_shared_rank(&S.sum_all, r);
+            over += *cluster.map_shared_rank(&S.sum_above, r);
+          }
+        }
+        int keep = k ? min(k, listed) : listed;
+        {
+          const int per = (keep + kThreads - 1) / kThreads, i0 = min(tid * per, keep), i1 = min(i0 + per, keep);
+          u64 mine = 0, sum;
+          for (int i = i0; i < i1; ++i) mine += weigh(logit_of(S.list[i]));
+          u64 upto = over + cta_before(mine, S.part, &sum);
+          const u64 limit = by_mass ? limit_of(p, k ? sum : whole) : ~0ull;
+          if (tid == 0) {
+            S.n = 0;
+            if (!k && (over >= limit || over + sum < limit)) S.failed = 1;      // p of all is reached above the list, or below it
+          }
+          __syncthreads();
+          int fit = 0;
+          for (int i = i0; i < i1; ++i) {
+            const u64 w = weigh(logit_of(S.list[i]));
+            if (upto < limit && w >= least_weight) ++fit;
+            upto += w;
+          }
+          if (fit) atomicAdd(&S.n, fit);
+          __syncthreads();
+          keep = S.n;
+        }
+        if (S.failed) {
+        } else if (from > 0) {      // kept ones to their blocks
+          for (int i = tid; i < keep; i += kThreads) {
+            const int place = static_cast<int>(0xffffffffu - static_cast<uint32_t>(S.list[i])) + head, b = place / kBlock, r = b / A.blocks_per_cta;
+            u64* sums = reinterpret_cast<u64*>(cluster.map_shared_rank(dynamic, r) + sizeof(Shared));
+            atomicAdd(&sums[b - r * A.blocks_per_cta], weigh(logit_of(S.list[i])));
+          }
+          if (tid == 0) S.cut = keep ? S.list[keep - 1] : S.list[0] + 1;        // none kept: min_p decides in what is above
+        } else {        // all that is kept is in the list: by index
+          for (int i = tid; i < keep; i += kThreads) S.list[i] = ~(S.list[i] >> 32 | static_cast<u64>(0xffffffffu - static_cast<uint32_t>(S.list[i])) << 32);
+          __syncthreads();
+          sort_down(S.list, keep);
+          const int per = (keep + kThreads - 1) / kThreads, i0 = min(tid * per, keep), i1 = min(i0 + per, keep);
+          auto weight_at = [&](int i) { return weigh(logit_of(~S.list[i] << 32)); };
+          u64 mine = 0, sum;
+          for (int i = i0; i < i1; ++i) mine += weight_at(i);
+          u64 upto = cta_before(mine, S.part, &sum);
+          const u64 goal = __umul64hi(fraction(u), sum);
+          if (upto <= goal && goal < upto + mine) {
+            for (int i = i0; i < i1; ++i) {
+              upto += weight_at(i);
+              if (goal < upto) {
+                A.out[row] = static_cast<int64_t>(~S.list[i] >> 32);
+                break;
+              }
             }
           }
         }
       }
-      __syncthreads();
-      for (int i = tid; i < kDigits * 4; i += kThreads) {       // four threads a digit
-        const int first = (i >> 2) * kColumns + (i & 3) * (kColumns / 4);
-        uint32_t n = 0;
-        u64 m = 0;
-#pragma unroll
-        for (int c = 0; c < kColumns / 4; ++c) {
-          n += S.cnt[first + c];
-          if (WEIGHTED) m += S.lo[first + c] + (static_cast<u64>(S.hi[first + c]) << 32);
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          n += __shfl_xor_sync(0xffffffffu, n, o);
-          if (WEIGHTED) m += __shfl_xor_sync(0xffffffffu, m, o);
-        }
-        if ((i & 3) == 0) {
-          S.count[parity][i >> 2] = n;
-          if (WEIGHTED) S.mass[parity][i >> 2] = m;
-        }
-      }
       cluster.sync();
-      if (tid < kDigits) {
-        uint32_t n = 0;
-        u64 m = 0;
-        for (int r = 0; r < n_cta; ++r) {
-          n += *cluster.map_shared_rank(&S.count[parity][tid], r);
-          if (WEIGHTED) m += *cluster.map_shared_rank(&S.mass[parity][tid], r);
-        }
-        S.all_count[tid] = n;
-        if (WEIGHTED) S.all_mass[tid] = m;
+      if (*cluster.map_shared_rank(&S.failed, 0) == 0) {
+        cut = *cluster.map_shared_rank(&S.cut, 0);
+        search = false;
+        summed = true;
       }
-      parity ^= 1;      // the others read this level's until they come to the next level's barrier
-      __syncthreads();
-      if (warp == 0) {        // eight digits a lane, the largest first
-        u64 mine = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int d = kDigits - 1 - (lane * 8 + j);
-          mine += WEIGHTED ? S.all_mass[d] : S.all_count[d];
+      cluster.sync();       // the others read the first CTA's; and the list is where digits are counted
+      if (summed && from == 0) return;
+    }
+  }
+
+  if (search) {
+    // ---- by digits: the key that a number of elements, or a sum of weights, ends in -----------------------------------------------------------
+    // Of the elements of key >= lowest: the key at which the running count (by weight: sum) from the largest on reaches `target`.  What is still
+    // to be reached in it is left in *rest, its elements in *equal.  target 0: `p` of the sum of all, less `minus`.
+    int parity = 0;
+    auto select = [&](auto weighted, uint32_t lowest, u64 target, u64 minus, u64* rest, u64* equal) -> uint32_t {
+      constexpr bool WEIGHTED = decltype(weighted)::value;
+      uint32_t prefix = 0;
+      for (int shift = Key<T>::kBits - 8; shift >= 0; shift -= 8) {
+        for (int i = tid; i < kDigits * kColumns; i += kThreads) {
+          S.cnt[i] = 0;
+          if (WEIGHTED) S.lo[i] = S.hi[i] = 0;
         }
-        u64 above = warp_before(mine);
-        if (WEIGHTED && target == 0) {
-          const u64 all = warp_sum_of(mine) - minus;
-          // the weights before a kept one sum to less than share * all: to less than the next whole number
-          const u64 f = share > 0.f ? static_cast<u64>(static_cast<double>(share) * 18446744073709551616.0) : 0ull;
-          target = max(__umul64hi(f, all) + (f * all ? 1 : 0), 1ull);
-        }
+        __syncthreads();
+        for (int b = warp; b < n_blocks; b += kWarps) {
+          const Eight<T> v = load(b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int d = kDigits - 1 - (lane * 8 + j);
-          const u64 in = WEIGHTED ? S.all_mass[d] : S.all_count[d];
-          if (above < target && target <= above + in) {
-            S.level[0] = d;
-            S.level[1] = target - above;
-            S.level[2] = S.all_count[d];
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t key = Key<T>::of(v[e]);
+            if (key < lowest || (shift + 8 < 32 && key >> (shift + 8) != prefix)) continue;
+            const int slot = ((key >> shift) & 255) * kColumns + (lane & (kColumns - 1));
+            atomicAdd(&S.cnt[slot], 1u);
+            if constexpr (WEIGHTED) {
+              const u64 w = weigh(value<T>(v[e]));
+              if (w) {
+                const uint32_t old = atomicAdd(&S.lo[slot], static_cast<uint32_t>(w));
+                const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + static_cast<uint32_t>(w) < old ? 1u : 0u);
+                if (up) atomicAdd(&S.hi[slot], up);
+              }
+            }
           }
-          above += in;
         }
-      }
-      __syncthreads();
-      prefix = prefix << 8 | static_cast<uint32_t>(S.level[0]);
-      target = S.level[1];
-      *equal = S.level[2];
-    }
-    *rest = target;
-    return prefix;
-  };
-
-  // kept: keys above `cut`, and the first `equals` of key `cut`
-  uint32_t cut = 0;
-  u64 equals = 0;
-  if (k) {
-    u64 there = 0;
-    cut = select(std::false_type{}, 0u, static_cast<u64>(k), 0.f, 0ull, &equals, &there);
-    if (by_mass) {
-      const u64 each = weigh.whole(weigh(value<T>(Key<T>::bits(cut))));
-      u64 rest = 0, in = 0;
-      const uint32_t at = select(std::true_type{}, cut, 0ull, p, (there - equals) * each, &rest, &in);
-      const u64 w = weigh.whole(weigh(value<T>(Key<T>::bits(at))));
-      equals = (rest + w - 1) / w;
-      cut = at;
-    }
-  } else if (by_mass) {
-    u64 rest = 0, in = 0;
-    cut = select(std::true_type{}, 0u, 0ull, p, 0ull, &rest, &in);
-    const u64 w = weigh.whole(weigh(value<T>(Key<T>::bits(cut))));
-    equals = (rest + w - 1) / w;
-  }
-  const double cut_weight = weigh(value<T>(Key<T>::bits(cut)));
-  const u64 each = weigh.whole(cut_weight);
-  if (equals && cut_weight < least) equals = 0;
-
-  // ---- kept weights of each block, without those of key `cut`, which are counted ------------------------------------------------------------
-  for (int b = warp; b < n_blocks; b += kWarps) {
-    const Eight<T> v = load(b);
-    u64 sum = 0;
-    uint32_t same = 0;
+        __syncthreads();
+        if (tid < kDigits) {
+          uint32_t n = 0;
+          u64 m = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t key = Key<T>::of(v[e]);
-      if (key > cut) {
-        const double w = weigh(value<T>(v[e]));
-        if (w >= least) sum += weigh.whole(w);
+          for (int c = 0; c < kColumns; ++c) {
+            n += S.cnt[tid * kColumns + c];
+            if (WEIGHTED) m += S.lo[tid * kColumns + c] + (static_cast<u64>(S.hi[tid * kColumns + c]) << 32);
+          }
+          S.count[parity][tid] = n;
+          if (WEIGHTED) S.mass[parity][tid] = m;
+        }
+        cluster.sync();
+        if (tid < kDigits) {
+          uint32_t n = 0;
+          u64 m = 0;
+          for (int r = 0; r < n_cta; ++r) {
+            n += *cluster.map_shared_rank(&S.count[parity][tid], r);
+            if (WEIGHTED) m += *cluster.map_shared_rank(&S.mass[parity][tid], r);
+          }
+          S.all_count[tid] = n;
+          if (WEIGHTED) S.all_mass[tid] = m;
+        }
+        parity ^= 1;      // the others read this level's until they come to the next level's barrier
+        __syncthreads();
+        if (warp == 0) {        // eight digits a lane, the largest first
+          u64 mine = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int d = kDigits - 1 - (lane * 8 + j);
+            mine += WEIGHTED ? S.all_mass[d] : S.all_count[d];
+          }
+          u64 above = warp_before(mine);
+          if (WEIGHTED && target == 0) target = limit_of(p, warp_sum_of(mine) - minus);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int d = kDigits - 1 - (lane * 8 + j);
+            const u64 in = WEIGHTED ? S.all_mass[d] : S.all_count[d];
+            if (above < target && target <= above + in) {
+              S.level[0] = d;
+              S.level[1] = target - above;
+              S.level[2] = S.all_count[d];
+            }
+            above += in;
+          }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | static_cast<uint32_t>(S.level[0]);
+        target = S.level[1];
+        *equal = S.level[2];
       }
-      same += key == cut;
+      *rest = target;
+      return prefix;
+    };
+    uint32_t last = 0;
+    u64 equals = 0, there = 0, rest = 0, in = 0;      // kept: keys above `last` and the first `equals` of it
+    if (k) last = select(std::false_type{}, 0u, static_cast<u64>(k), 0ull, &equals, &there);
+    if (by_mass) {
+      const u64 each = k ? weigh(value<T>(Key<T>::bits(last))) : 0ull;
+      last = select(std::true_type{}, last, 0ull, (there - equals) * each, &rest, &in);
+      const u64 w = weigh(value<T>(Key<T>::bits(last)));
+      equals = (rest + w - 1) / w;
     }
-    sum = warp_sum_of(sum);
-    same = warp_sum_of(same);
-    if (lane == 0) {
-      block_mass[b] = sum;
-      block_equal[b] = same;
+    // where the last of them is
+    uint32_t same_mine = 0;
+    const int per = (n_blocks + kWarps - 1) / kWarps, b0 = min(warp * per, n_blocks), b1 = min(b0 + per, n_blocks);        // a warp's blocks are side by side here
+    for (int b = b0; b < b1; ++b) {
+      const Eight<T> v = load(b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) same_mine += Key<T>::of(v[e]) == last;
     }
+    same_mine = __reduce_add_sync(0xffffffffu, same_mine);
+    u64 same = 0;
+    u64 seen = cta_before(lane == 0 ? static_cast<u64>(same_mine) : 0ull, S.part, &same);
+    seen = __shfl_sync(0xffffffffu, seen, 0);
+    if (tid == 0) S.equal = same;
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) seen += *cluster.map_shared_rank(&S.equal, r);
+    if (seen < equals && equals <= seen + same_mine) {        // this warp's
+      for (int b = b0; b < b1; ++b) {
+        const Eight<T> v = load(b);
+        uint32_t here = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) here += Key<T>::of(v[e]) == last;
+        u64 upto = seen + warp_before(here);
+        seen += __reduce_add_sync(0xffffffffu, here);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (Key<T>::of(v[e]) == last && ++upto == equals) {
+            const u64 c = composite(value<T>(v[e]), index_of(b, e));
+            for (int r = 0; r < n_cta; ++r) *cluster.map_shared_rank(&S.cut, r) = c;
+          }
+        }
+        if (seen >= equals) break;
+      }
+    }
+    cluster.sync();
+    cut = S.cut;
   }
-  __syncthreads();
+
+  auto kept_weight = [&](float f, int index) -> u64 {
+    if (composite(f, index) < cut) return 0;
+    const u64 w = weigh(f);
+    return w >= least_weight ? w : 0;
+  };
+  // ---- kept weights of each block ----------------------------------------------------------------------------------------------------------------
+  if (!summed) {
+    for (int b = warp; b < n_blocks; b += kWarps) {
+      const Eight<T> v = load(b);
+      u64 sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += kept_weight(value<T>(v[e]), index_of(b, e));
+      sum = warp_sum_of(sum);
+      if (lane == 0) block_mass[b] = sum;
+    }
+    __syncthreads();
+  }
   const int per = (n_blocks + kThreads - 1) / kThreads, b0 = min(tid * per, n_blocks), b1 = min(b0 + per, n_blocks);
-  u64 same = 0, all = 0;
-  for (int b = b0; b < b1; ++b) same += block_equal[b];
-  u64 same_before = cta_before(same, S.warp_part, &all);
-  if (tid == 0) S.equal = all;
-  cluster.sync();
-  for (int r = 0; r < rank; ++r) same_before += *cluster.map_shared_rank(&S.equal, r);
-  u64 mine = 0, seen = same_before;
-  for (int b = b0; b < b1; ++b) {
-    const u64 left = equals > seen ? equals - seen : 0;
-    mine += block_mass[b] + min(left, static_cast<u64>(block_equal[b])) * each;
-    seen += block_equal[b];
-  }
-  u64 before = cta_before(mine, S.warp_part, &all);
-  if (tid == 0) S.kept = all;
+  u64 mine = 0, all = 0;
+  for (int b = b0; b < b1; ++b) mine += block_mass[b];
+  u64 before = cta_before(mine, S.part, &all);
+  if (tid == 0) S.kept = all, S.at[0] = ~0ull;
   cluster.sync();
   u64 total = 0, lower = 0;
   for (int r = 0; r < n_cta; ++r) {
@@ -428,59 +710,39 @@ __global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const Sample A
     total += m;
     if (r < rank) lower += m;
   }
-  // u of the sum, rounded down; u below 0 or no number counts as 0, 1 and above as the largest below 1
-  const u64 f = u > 0.f ? (u < 1.f ? static_cast<u64>(static_cast<double>(u) * 18446744073709551616.0) : ~0ull) : 0ull;
-  const u64 goal = __umul64hi(f, total);
+  const u64 goal = __umul64hi(fraction(u), total);
   before += lower;
-  if (tid == 0) S.at[0] = ~0ull;
-  __syncthreads();
   if (before <= goal && goal < before + mine) {
-    seen = same_before;
     for (int b = b0; b < b1; ++b) {
-      const u64 left = equals > seen ? equals - seen : 0;
-      const u64 in = block_mass[b] + min(left, static_cast<u64>(block_equal[b])) * each;
-      if (goal < before + in) {
+      if (goal < before + block_mass[b]) {
         S.at[0] = b;
         S.at[1] = goal - before;
-        S.at[2] = left;
         break;
       }
-      before += in;
-      seen += block_equal[b];
+      before += block_mass[b];
     }
   }
   __syncthreads();
   if (warp == 0 && S.at[0] != ~0ull) {
     const int b = static_cast<int>(S.at[0]);
-    const u64 to = S.at[1], left = S.at[2];
+    const u64 to = S.at[1];
     const Eight<T> v = load(b);
-    uint32_t mine_same = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mine_same += Key<T>::of(v[e]) == cut;
-    u64 rank_of = warp_before(mine_same), w[8], sum = 0;
+    u64 w[8], sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t key = Key<T>::of(v[e]);
-      w[e] = 0;
-      if (key > cut) {
-        const double d = weigh(value<T>(v[e]));
-        if (d >= least) w[e] = weigh.whole(d);
-      } else if (key == cut && rank_of++ < left) {
-        w[e] = each;
-      }
+      w[e] = kept_weight(value<T>(v[e]), index_of(b, e));
       sum += w[e];
     }
     u64 run = warp_before(sum);
     if (run <= to && to < run + sum) {
-      int found = 0;
+      int found = 7;
+      run += sum;
 #pragma unroll
       for (int e = 7; e >= 0; --e) {       // the first whose running sum passes
-        u64 upto = run;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) upto += i <= e ? w[i] : 0;
-        if (upto > to) found = e;
+        if (run > to) found = e;
+        run -= w[e];
       }
-      A.out[row] = static_cast<int64_t>(block0 + b) * kBlock + lane * 8 + found - head;
+      A.out[row] = index_of(b, found);
     }
   }
   cluster.sync();       // the others may still read this CTA's
@@ -492,18 +754,20 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
   const int blocks = (A.cols + 7 + kBlock - 1) / kBlock;      // with the places before the row
   auto bytes = [&](int ctas, bool held) {
     const size_t per = (blocks + ctas - 1) / ctas;
-    return sizeof(Shared) + ((per + 1) & ~size_t{1}) * 8 + ((per + 3) & ~size_t{3}) * 4 + (held ? per * kBlock * sizeof(T) : 0);
+    return sizeof(Shared) + ((per + 1) & ~size_t{1}) * 8 + (held ? per * kBlock * sizeof(T) : 0);
   };
+  // two CTAs per SM where eight of a cluster can hold a row that way
+  constexpr size_t kHalf = 113 * 1024;
   int ctas = 1;
-  while (ctas < 8 && bytes(ctas, true) > kMaxSmem) ctas *= 2;
+  while (ctas < 8 && bytes(ctas, true) > kHalf) ctas *= 2;
   const bool held = bytes(ctas, true) <= kMaxSmem;
-  while (ctas < 8 && 2 * ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 16 * ctas) ctas *= 2;
+  while (ctas < 8 && 2 * ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 8 * ctas) ctas *= 2;
   const size_t smem = bytes(ctas, held);
   if (smem > kMaxSmem) return fail(B200_ESHAPE, "%s: rows of %d", name, A.cols);
   A.blocks_per_cta = (blocks + ctas - 1) / ctas;
   int bits = 0;
   while ((1ll << bits) < A.cols) ++bits;
-  A.frac = std::min(62 - bits, 50);
+  A.frac = std::min(62 - bits, 44);
   auto kern = held ? sample_rows_kernel<T, true> : sample_rows_kernel<T, false>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   cudaLaunchConfig_t cfg{};
