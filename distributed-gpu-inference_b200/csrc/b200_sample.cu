@@ -15,9 +15,9 @@
 // elements, eight side by side per lane.
 //   all rows        load, maximum
 //   k, or p         numbers of elements in 1024 ranges of log w (0 .. -46).  k: all elements down to the range that the k-th is in go in a list; p: from
-//                   the middles of the ranges it is known to some tenths of a per cent where the weights sum to p of all, the elements of these ranges go in
+//                   these, to first order in where the elements lie in their ranges, it is known to some 10^-4 where the weights sum to p of all, the elements of these ranges go in
 //                   the list, and exact sums are taken of what is above and of all
-//   list (4096)     sorted by the cluster's first CTA, cut by k, p and min_p; where nothing is above the list, what it keeps is sorted by index and drawn from
+//   list (4096)     searched by the cluster's first CTA for the last that k keeps, then p; where nothing is above the list, for the token too
 //   other rows      kept weights of each block; the block, the lane and the element in which u falls
 // Where that does not serve - k over 2048, or ranges of more than 4096 elements, equal logits above all - the last key is found by its digits of 8 bits
 // from counts or sums in the whole row.
@@ -36,8 +36,12 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBlock = 256;         // elements
 constexpr int kRanges = 1024, kRangeColumns = 8;        // columns: lanes that fall in the same range meet at fewer addresses
+constexpr float kRangeSteps = 11.5f;      // of 1/256 in log2
 constexpr int kDigits = 256, kColumns = 8;
 constexpr int kList = 4096, kMostK = 2048;
+constexpr int kIndexBits = 20;
+constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
+static_assert(B200_MAX_SAMPLE_COLS <= 1 << kIndexBits, "indexes");
 using u64 = unsigned long long;
 
 struct Sample {
@@ -114,7 +118,7 @@ struct alignas(16) Shared {
     u64 list[kList];
   };
   union {
-    uint32_t range_count[kRanges];      // this CTA's, read by the cluster
+    u64 range_count[kRanges];           // this CTA's, read by the cluster: elements << 32 | their steps into the range
     struct {
       u64 mass[2][kDigits];             // likewise
       uint32_t count[2][kDigits];
@@ -131,9 +135,12 @@ struct alignas(16) Shared {
   u64 sum_all, sum_above, kept, equal;
   u64 cut;                              // (key, ~index) of the last that is kept
   // this CTA's
-  u64 level[4], at[4];
+  u64 level[4], at[4], ends[2];
+  uint32_t few;
   int from, to, n;
 };
+constexpr int kBins = kThreads, kFew = 256;       // of Shared::range_count, where the list is searched
+static_assert(kBins + 2 * kFew <= kRanges, "room for bins and a bin's elements");
 
 // weights, as whole numbers of 2^-frac
 template <typename T>
@@ -160,8 +167,11 @@ struct Weigh {
     const uint32_t w = step.x + (__float_as_int(fmaf(q, __uint_as_float(step.y), shift)) - 0x4b400000);
     return (static_cast<u64>(w) << up) >> -(n >> 8);
   }
-  // range of an argument
-  __device__ __forceinline__ int range(float y) const { return __float_as_int(fmaf(y, -1.0f / 11.5f, 8388608.f)) & (kRanges - 1); }
+  // steps of an argument, 1 << log_steps a range
+  float per_step;
+  int log_steps;
+  __device__ __forceinline__ int steps(float y) const { return __float_as_int(fmaf(y, per_step, 8388608.f)) & 0x7fffff; }
+  __device__ __forceinline__ int range(float y) const { return steps(y) >> log_steps; }
 };
 
 template <typename V>
@@ -189,33 +199,15 @@ __device__ __forceinline__ V cta_before(V v, V* part, V* all) {
   __syncthreads();
   if (lane == 31) part[warp] = in_warp + v;
   __syncthreads();
-  V before = 0, total = 0;
+  V upto = part[lane & (kWarps - 1)];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const V x = part[w];
-    if (w < warp) before += x;
-    total += x;
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const V up = __shfl_up_sync(0xffffffffu, upto, o, kWarps);
+    if ((lane & (kWarps - 1)) >= o) upto += up;
   }
+  const V before = __shfl_sync(0xffffffffu, upto, max(warp - 1, 0), kWarps), total = __shfl_sync(0xffffffffu, upto, kWarps - 1, kWarps);
   *all = total;
-  return before + in_warp;
-}
-
-// the first n of `list` in descending order; what is behind them, up to the next power of two, is overwritten
-__device__ __forceinline__ void sort_down(u64* list, int n) {
-  int size = 2;
-  while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
-  __syncthreads();
-  for (int run = 2; run <= size; run *= 2) {
-    for (int step = run / 2; step > 0; step /= 2) {
-      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-        const int at = 2 * i - (i & (step - 1));
-        const u64 a = list[at], b = list[at + step];
-        if ((a < b) == ((at & run) == 0)) list[at] = b, list[at + step] = a;
-      }
-      __syncthreads();
-    }
-  }
+  return (warp ? before : V(0)) + in_warp;
 }
 
 // f of 2^64, within 0 .. 2^64 - 1; not a number: 0
@@ -285,8 +277,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     }
   };
   auto index_of = [&](int block, int e) { return (block0 + block) * kBlock + lane * 8 + e - head; };
-  auto composite = [&](float f, int index) { return static_cast<u64>(Key<float>::of(__float_as_uint(f))) << 32 | (0xffffffffu - static_cast<uint32_t>(index)); };
-  auto logit_of = [&](u64 c) { return __uint_as_float(Key<float>::bits(static_cast<uint32_t>(c >> 32))); };
+  // an element's place in the order: its key over its index, upside down
+  auto composite = [&](uint32_t bits, int index) { return static_cast<u64>(Key<T>::of(bits)) << kIndexBits | (kIndexMask - static_cast<uint32_t>(index)); };
+  auto logit_of = [&](u64 c) { return value<T>(Key<T>::bits(static_cast<uint32_t>(c >> kIndexBits))); };
 
   // ---- the largest logit ---------------------------------------------------------------------------------------------------------------------
   if (tid < 256) {
@@ -360,6 +353,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     weigh.lowest = -256.0f * (A.frac + 1);
     weigh.up = A.frac - 30;
     weigh.table = S.table;
+    // elements and their steps, added up as two halves of a number: 32 elements a block and column, so 65536 is not reached
+    weigh.log_steps = A.blocks_per_cta <= 136 ? 4 : 2;
+    weigh.per_step = static_cast<float>(1 << weigh.log_steps) / -kRangeSteps;
   }
 
   u64 cut = 0;            // kept: (key, ~index) from this on
@@ -374,31 +370,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = weigh.argument(value<T>(v[e]));
-        if (weigh.some(y)) atomicAdd(&S.ranges[weigh.range(y) * kRangeColumns + (lane & (kRangeColumns - 1))], 1u);
+        if (weigh.some(y)) {
+          const int at = weigh.steps(y);
+          atomicAdd(&S.ranges[(at >> weigh.log_steps) * kRangeColumns + (lane & (kRangeColumns - 1))], 0x10000u | (at & ((1 << weigh.log_steps) - 1)));
+        }
       }
     }
     __syncthreads();
     constexpr int kMine = kRanges / kThreads;
-    uint32_t c[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      c[i] = 0;
+      uint32_t c = 0, steps = 0;
 #pragma unroll
-      for (int j = 0; j < kRangeColumns; j += 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(&S.ranges[(tid * kMine + i) * kRangeColumns + j]);
-        c[i] += q.x + q.y + q.z + q.w;
+      for (int j = 0; j < kRangeColumns; ++j) {
+        const uint32_t q = S.ranges[(tid * kMine + i) * kRangeColumns + (j + tid) % kRangeColumns];
+        c += q >> 16;
+        steps += q & 0xffffu;
       }
-      S.range_count[tid * kMine + i] = c[i];
+      S.range_count[tid * kMine + i] = static_cast<u64>(c) << 32 | steps;
     }
     if (tid == 0) S.from = 0, S.to = kRanges - 1;
     cluster.sync();
-    // numbers, and weights as the middles of the ranges have them (whole numbers: the same sums in all CTAs)
+    // numbers, and weights to second order of the steps (as whole numbers: the same sums in all CTAs)
+    uint32_t c[kMine];
     u64 m[kMine], m_mine = 0, m_all, n_mine = 0, n_all;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      c[i] = 0;
-      for (int r = 0; r < n_cta; ++r) c[i] += cluster.map_shared_rank(S.range_count, r)[tid * kMine + i];
-      m[i] = c[i] * static_cast<u64>(exp2f(40.f - (tid * kMine + i) * (11.5f / 256.f)));
+      u64 both = 0;
+      for (int r = 0; r < n_cta; ++r) both += cluster.map_shared_rank(S.range_count, r)[tid * kMine + i];
+      c[i] = static_cast<uint32_t>(both >> 32);
+      const float of = static_cast<float>(c[i]), into = static_cast<float>(static_cast<uint32_t>(both)) / (1 << weigh.log_steps) - 0.5f * of;
+      m[i] = static_cast<u64>(exp2f(40.f - (tid * kMine + i + 0.5f) * (kRangeSteps / 256.f)) * fmaf(into, -0.69314718f * kRangeSteps / 256.f, of));
       n_mine += c[i];
       m_mine += m[i];
     }
@@ -414,9 +416,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       }
       __syncthreads();
       listing = S.n;
-    } else {       // the ranges within 0.3 % of the whole around p of it
+    } else {       // the ranges within 0.05 % of the whole around p of it
       u64 before = cta_before(m_mine, S.part, &m_all);
-      const u64 low = __umul64hi(fraction(p - 0.003f), m_all), high = __umul64hi(fraction(p + 0.003f), m_all) + 1;
+      const u64 low = __umul64hi(fraction(p - 0.0005f), m_all), high = __umul64hi(fraction(p + 0.0005f), m_all) + 1;
       if (tid == 0) S.at[0] = 0, S.at[1] = n_all;
       __syncthreads();
 #pragma unroll
@@ -437,31 +439,38 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     if (listing <= kList) {       // (the same in all CTAs)
       // ---- the list; a row without k: exact sums of all, of what is above the list, and of the blocks' part of that ------------------------------
       u64 all = 0, above = 0;
-      for (int b = warp; b < n_blocks; b += kWarps) {
-        const Eight<T> v = load(b);
-        u64 sum = 0;
+      const int first_step = from << weigh.log_steps, steps = (to + 1 - from) << weigh.log_steps;
+      auto gather = [&](auto sums, auto limited) {
+        for (int b = warp; b < n_blocks; b += kWarps) {
+          const Eight<T> v = load(b);
+          u64 sum = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = value<T>(v[e]), y = weigh.argument(f);
-          const int range = weigh.some(y) ? weigh.range(y) : kRanges;
-          if (range >= from && range <= to) {
-            const uint32_t at = atomicAdd(&S.listed, 1u);
-            if (at < kList) S.list[at] = composite(f, index_of(b, e));
-          }
-          if (!k) {
-            const u64 w = weigh(f);
-            all += w;
-            if (range < from) {
-              above += w;
-              if (w >= least_weight) sum += w;
+          for (int e = 0; e < 8; ++e) {
+            const float f = value<T>(v[e]), y = weigh.argument(f);
+            const int step = weigh.some(y) ? weigh.steps(y) - first_step : 1 << 24;
+            if (static_cast<unsigned>(step) < static_cast<unsigned>(steps)) {
+              const uint32_t at = atomicAdd(&S.listed, 1u);
+              if (at < kList) S.list[at] = composite(v[e], index_of(b, e));
+            }
+            if constexpr (decltype(sums)::value) {
+              const u64 w = weigh(f);
+              all += w;
+              if (step < 0) {
+                if (decltype(limited)::value) above += w;
+                if (!decltype(limited)::value || w >= least_weight) sum += w;
+              }
             }
           }
+          if (decltype(sums)::value && from > 0) {
+            if (!decltype(limited)::value) above += sum;
+            sum = warp_sum_of(sum);
+            if (lane == 0) block_mass[b] = sum;
+          }
         }
-        if (from > 0) {
-          sum = warp_sum_of(sum);
-          if (lane == 0) block_mass[b] = sum;
-        }
-      }
+      };
+      if (k) gather(std::false_type{}, std::false_type{});
+      else if (least_weight) gather(std::true_type{}, std::true_type{});
+      else gather(std::true_type{}, std::false_type{});
       if (!k) {
         all = warp_sum_of(all);
         above = warp_sum_of(above);
@@ -472,70 +481,118 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       }
       cluster.sync();
       if (rank == 0) {
-        int listed = S.listed;
+        int n = S.listed;
         for (int r = 1; r < n_cta; ++r) {
-          const int more = min(static_cast<int>(*cluster.map_shared_rank(&S.listed, r)), kList - listed);
+          const int more = min(static_cast<int>(*cluster.map_shared_rank(&S.listed, r)), kList - n);
           const u64* theirs = cluster.map_shared_rank(S.list, r);
-          for (int i = tid; i < more; i += kThreads) S.list[listed + i] = theirs[i];
-          listed += more;
+          for (int i = tid; i < more; i += kThreads) S.list[n + i] = theirs[i];
+          n += more;
         }
-        sort_down(S.list, listed);
-        u64 whole = 0, over = 0;
-        if (!k) {
+        if (tid == 0) S.ends[0] = ~0ull, S.ends[1] = 0;
+        __syncthreads();
+        {
+          u64 lo = ~0ull, hi = 0;
+          for (int i = tid; i < n; i += kThreads) lo = min(lo, S.list[i]), hi = max(hi, S.list[i]);
+          if (tid < n) {
+            atomicMin(&S.ends[0], lo);
+            atomicMax(&S.ends[1], hi);
+          }
+        }
+        __syncthreads();
+        const u64 lowest_listed = S.ends[0], highest_listed = S.ends[1];
+        // The element of the list at which the running value (1 or the weight) from `upto` on reaches `target`, of those from `lowest` on, in the
+        // list's order or by index: by the sums of 512 equal parts of what is left, until a part has few elements.
+        u64* bins = S.range_count;
+        u64 *few = bins + kBins, *few_value = few + kFew;
+        auto find = [&](auto by_index, u64 lo, u64 hi, u64 lowest, auto&& value_of, u64 upto, u64 target) -> u64 {
+          auto order = [&](u64 c) { return decltype(by_index)::value ? c & kIndexMask : c; };
+          while (true) {
+            const int shift = max(0, 64 - __clzll(hi - lo) - 9);
+            bins[tid] = 0;
+            if (tid == 0) S.few = 0, S.at[0] = ~0ull;
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+              const u64 c = S.list[i], o = order(c);
+              if (c >= lowest && o >= lo && o <= hi) atomicAdd(&bins[(hi - o) >> shift], value_of(c));
+            }
+            __syncthreads();
+            u64 unused;
+            const u64 in = bins[tid], before = upto + cta_before(in, S.part, &unused);
+            if (before < target && target <= before + in) S.at[0] = tid, S.at[1] = before;
+            __syncthreads();
+            if (S.at[0] == ~0ull) return 0;       // not in the list
+            const u64 bin = S.at[0];
+            upto = S.at[1];
+            for (int i = tid; i < n; i += kThreads) {
+              const u64 c = S.list[i], o = order(c);
+              if (c >= lowest && o >= lo && o <= hi && (hi - o) >> shift == bin) {
+                const uint32_t at = atomicAdd(&S.few, 1u);
+                if (at < kFew) few[at] = c, few_value[at] = value_of(c);
+              }
+            }
+            __syncthreads();
+            const int m = S.few;
+            if (m <= kFew) {
+              if (tid < m) {
+                u64 before_mine = upto;
+                for (int j = 0; j < m; ++j)
+                  if (order(few[j]) > order(few[tid])) before_mine += few_value[j];
+                if (before_mine < target && target <= before_mine + few_value[tid]) S.at[2] = few[tid];
+              }
+              __syncthreads();
+              const u64 c = S.at[2];
+              __syncthreads();
+              return c;
+            }
+            hi -= bin << shift;
+            lo = max(lo, hi - ((1ull << shift) - 1));
+            __syncthreads();
+          }
+        };
+        auto weight_of = [&](u64 c) { return weigh(logit_of(c)); };
+        auto kept_of = [&](u64 c) -> u64 {
+          const u64 w = weigh(logit_of(c));
+          return w >= least_weight ? w : 0;
+        };
+        auto sum_from = [&](u64 lowest, auto&& value_of) {
+          u64 mine = 0, sum;
+          for (int i = tid; i < n; i += kThreads) mine += S.list[i] >= lowest ? value_of(S.list[i]) : 0;
+          cta_before(mine, S.part, &sum);
+          return sum;
+        };
+        u64 whole = 0, over = 0, mine = 0;
+        if (k) {
+          if (n > k) mine = find(std::false_type{}, lowest_listed, highest_listed, 0ull, [](u64) { return 1ull; }, 0ull, static_cast<u64>(k));
+          if (by_mass) whole = sum_from(mine, weight_of);
+        } else {
           for (int r = 0; r < n_cta; ++r) {
             whole += *cluster.map_shared_rank(&S.sum_all, r);
             over += *cluster.map_shared_rank(&S.sum_above, r);
           }
         }
-        int keep = k ? min(k, listed) : listed;
-        {
-          const int per = (keep + kThreads - 1) / kThreads, i0 = min(tid * per, keep), i1 = min(i0 + per, keep);
-          u64 mine = 0, sum;
-          for (int i = i0; i < i1; ++i) mine += weigh(logit_of(S.list[i]));
-          u64 upto = over + cta_before(mine, S.part, &sum);
-          const u64 limit = by_mass ? limit_of(p, k ? sum : whole) : ~0ull;
-          if (tid == 0) {
-            S.n = 0;
-            if (!k && (over >= limit || over + sum < limit)) S.failed = 1;      // p of all is reached above the list, or below it
-          }
-          __syncthreads();
-          int fit = 0;
-          for (int i = i0; i < i1; ++i) {
-            const u64 w = weigh(logit_of(S.list[i]));
-            if (upto < limit && w >= least_weight) ++fit;
-            upto += w;
-          }
-          if (fit) atomicAdd(&S.n, fit);
-          __syncthreads();
-          keep = S.n;
+        bool failed = false;
+        if (by_mass) {
+          const u64 limit = limit_of(p, whole);
+          const u64 last = over < limit ? find(std::false_type{}, lowest_listed, highest_listed, mine, weight_of, over, limit) : 0;
+          failed = last == 0;     // p of all is reached above the list, or below it
+          mine = last;
         }
-        if (S.failed) {
+        if (failed) {
+          if (tid == 0) S.failed = 1;
         } else if (from > 0) {      // kept ones to their blocks
-          for (int i = tid; i < keep; i += kThreads) {
-            const int place = static_cast<int>(0xffffffffu - static_cast<uint32_t>(S.list[i])) + head, b = place / kBlock, r = b / A.blocks_per_cta;
-            u64* sums = reinterpret_cast<u64*>(cluster.map_shared_rank(dynamic, r) + sizeof(Shared));
-            atomicAdd(&sums[b - r * A.blocks_per_cta], weigh(logit_of(S.list[i])));
-          }
-          if (tid == 0) S.cut = keep ? S.list[keep - 1] : S.list[0] + 1;        // none kept: min_p decides in what is above
-        } else {        // all that is kept is in the list: by index
-          for (int i = tid; i < keep; i += kThreads) S.list[i] = ~(S.list[i] >> 32 | static_cast<u64>(0xffffffffu - static_cast<uint32_t>(S.list[i])) << 32);
-          __syncthreads();
-          sort_down(S.list, keep);
-          const int per = (keep + kThreads - 1) / kThreads, i0 = min(tid * per, keep), i1 = min(i0 + per, keep);
-          auto weight_at = [&](int i) { return weigh(logit_of(~S.list[i] << 32)); };
-          u64 mine = 0, sum;
-          for (int i = i0; i < i1; ++i) mine += weight_at(i);
-          u64 upto = cta_before(mine, S.part, &sum);
-          const u64 goal = __umul64hi(fraction(u), sum);
-          if (upto <= goal && goal < upto + mine) {
-            for (int i = i0; i < i1; ++i) {
-              upto += weight_at(i);
-              if (goal < upto) {
-                A.out[row] = static_cast<int64_t>(~S.list[i] >> 32);
-                break;
-              }
+          for (int i = tid; i < n; i += kThreads) {
+            const u64 c = S.list[i], w = c >= mine ? kept_of(c) : 0;
+            if (w) {
+              const int place = static_cast<int>(kIndexMask - (static_cast<uint32_t>(c) & kIndexMask)) + head, b = place / kBlock, r = b / A.blocks_per_cta;
+              u64* sums = reinterpret_cast<u64*>(cluster.map_shared_rank(dynamic, r) + sizeof(Shared));
+              atomicAdd(&sums[b - r * A.blocks_per_cta], w);
             }
           }
+          if (tid == 0) S.cut = mine;
+        } else {        // all that is kept is in the list
+          const u64 goal = __umul64hi(fraction(u), sum_from(mine, kept_of));
+          const u64 c = find(std::true_type{}, static_cast<u64>(kIndexMask + 1 - A.cols), static_cast<u64>(kIndexMask), mine, kept_of, 0ull, goal + 1);
+          if (tid == 0) A.out[row] = kIndexMask - (static_cast<uint32_t>(c) & kIndexMask);
         }
       }
       cluster.sync();
@@ -670,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (Key<T>::of(v[e]) == last && ++upto == equals) {
-            const u64 c = composite(value<T>(v[e]), index_of(b, e));
+            const u64 c = composite(v[e], index_of(b, e));
             for (int r = 0; r < n_cta; ++r) *cluster.map_shared_rank(&S.cut, r) = c;
           }
         }
@@ -681,9 +738,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     cut = S.cut;
   }
 
-  auto kept_weight = [&](float f, int index) -> u64 {
-    if (composite(f, index) < cut) return 0;
-    const u64 w = weigh(f);
+  auto kept_weight = [&](uint32_t bits, int index) -> u64 {
+    if (composite(bits, index) < cut) return 0;
+    const u64 w = weigh(value<T>(bits));
     return w >= least_weight ? w : 0;
   };
   // ---- kept weights of each block ----------------------------------------------------------------------------------------------------------------
@@ -692,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       const Eight<T> v = load(b);
       u64 sum = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += kept_weight(value<T>(v[e]), index_of(b, e));
+      for (int e = 0; e < 8; ++e) sum += kept_weight(v[e], index_of(b, e));
       sum = warp_sum_of(sum);
       if (lane == 0) block_mass[b] = sum;
     }
@@ -730,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     u64 w[8], sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[e] = kept_weight(value<T>(v[e]), index_of(b, e));
+      w[e] = kept_weight(v[e], index_of(b, e));
       sum += w[e];
     }
     u64 run = warp_before(sum);
