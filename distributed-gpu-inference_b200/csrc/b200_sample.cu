@@ -108,6 +108,29 @@ struct Eight {      // bits of eight elements
   }
 };
 
+// 2^(30 + j / 256), as a whole number and as a float's bits
+struct Steps {
+  uint32_t whole[256];
+  float number[256];
+};
+constexpr Steps make_steps() {
+  // 2^(1/256), 2^(1/128) ... 2^(1/2)
+  constexpr double roots[8] = {1.0027112750502024854, 1.0054299011128028214, 1.0108892860517004600, 1.0218971486541166782, 1.0442737824274138403,
+                               1.0905077326652576592, 1.1892071150027210667, 1.4142135623730950488};
+  Steps t{};
+  for (int j = 0; j < 256; ++j) {
+    double x = 1073741824.0;
+    for (int b = 0; b < 8; ++b)
+      if (j >> b & 1) x *= roots[b];
+    t.whole[j] = static_cast<uint32_t>(x + 0.5);
+    t.number[j] = static_cast<float>(x);
+  }
+  return t;
+}
+__device__ constexpr Steps kSteps = make_steps();
+
+constexpr int kMostCtas = 8;      // of a cluster
+
 struct alignas(16) Shared {
   uint2 table[256];             // 2^(30 + j / 256): as a whole number, as a float
   union {
@@ -281,11 +304,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   auto composite = [&](uint32_t bits, int index) { return static_cast<u64>(Key<T>::of(bits)) << kIndexBits | (kIndexMask - static_cast<uint32_t>(index)); };
   auto logit_of = [&](u64 c) { return value<T>(Key<T>::bits(static_cast<uint32_t>(c >> kIndexBits))); };
 
+  // the CTAs' values of the cluster, all asked for before the first is needed
+  auto of_all = [&](auto* mine, auto* values) {
+#pragma unroll
+    for (int r = 0; r < kMostCtas; ++r) values[r] = r < n_cta ? *cluster.map_shared_rank(mine, r) : 0;
+  };
+  auto sum_of_all = [&](auto* mine) {
+    std::remove_pointer_t<decltype(mine)> v[kMostCtas], sum = 0;
+    of_all(mine, v);
+#pragma unroll
+    for (int r = 0; r < kMostCtas; ++r) sum += v[r];
+    return sum;
+  };
+
   // ---- the largest logit ---------------------------------------------------------------------------------------------------------------------
-  if (tid < 256) {
-    const double step = exp2(30.0 + tid / 256.0);
-    S.table[tid] = make_uint2(static_cast<uint32_t>(__double2ll_rn(step)), __float_as_uint(static_cast<float>(step)));
-  }
+  const float t = A.temperature ? A.temperature[row] : A.t0, p = A.top_p ? A.top_p[row] : A.p0, least = A.min_p ? A.min_p[row] : A.m0, u = A.u[row];
+  int k = A.top_k ? A.top_k[row] : A.k0;
+  if (tid < 256) S.table[tid] = make_uint2(kSteps.whole[tid], __float_as_uint(kSteps.number[tid]));
   if (tid == 0) S.first = 0xffffffffu, S.listed = 0, S.failed = 0, S.sum_all = S.sum_above = 0, S.best = 0;
   __syncthreads();
   float top = -INFINITY;
@@ -318,9 +353,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   }
   cluster.sync();
   uint32_t best = 0;
-  for (int r = 0; r < n_cta; ++r) best = max(best, *cluster.map_shared_rank(&S.best, r));
+  {
+    uint32_t v[kMostCtas];
+    of_all(&S.best, v);
+#pragma unroll
+    for (int r = 0; r < kMostCtas; ++r) best = max(best, v[r]);
+  }
   top = __uint_as_float(best == 0xffffffffu ? 0x7fffffffu : Key<float>::bits(best));
-  const float t = A.temperature ? A.temperature[row] : A.t0;
   if (!(t > 0.f) || !(fabsf(top) < INFINITY)) {      // no temperature, or a largest logit that is no number: the first of the largest
     uint32_t first = 0xffffffffu;
     for (int b = warp; b < n_blocks; b += kWarps) {
@@ -338,8 +377,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     if (rank == 0 && tid == 0) A.out[row] = S.first;
     return;
   }
-  int k = A.top_k ? A.top_k[row] : A.k0;
-  const float p = A.top_p ? A.top_p[row] : A.p0, least = A.min_p ? A.min_p[row] : A.m0, u = A.u[row];
   if (k <= 0 || k >= A.cols) k = 0;
   const bool by_mass = p < 1.0f;
   // not a number: no limit
@@ -396,8 +433,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     u64 m[kMine], m_mine = 0, m_all, n_mine = 0, n_all;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      u64 both = 0;
-      for (int r = 0; r < n_cta; ++r) both += cluster.map_shared_rank(S.range_count, r)[tid * kMine + i];
+      const u64 both = sum_of_all(&S.range_count[tid * kMine + i]);
       c[i] = static_cast<uint32_t>(both >> 32);
       const float of = static_cast<float>(c[i]), into = static_cast<float>(static_cast<uint32_t>(both)) / (1 << weigh.log_steps) - 0.5f * of;
       m[i] = static_cast<u64>(exp2f(40.f - (tid * kMine + i + 0.5f) * (kRangeSteps / 256.f)) * fmaf(into, -0.69314718f * kRangeSteps / 256.f, of));
@@ -444,14 +480,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
         for (int b = warp; b < n_blocks; b += kWarps) {
           const Eight<T> v = load(b);
           u64 sum = 0;
+          unsigned hits = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float f = value<T>(v[e]), y = weigh.argument(f);
             const int step = weigh.some(y) ? weigh.steps(y) - first_step : 1 << 24;
-            if (static_cast<unsigned>(step) < static_cast<unsigned>(steps)) {
-              const uint32_t at = atomicAdd(&S.listed, 1u);
-              if (at < kList) S.list[at] = composite(v[e], index_of(b, e));
-            }
+            if (static_cast<unsigned>(step) < static_cast<unsigned>(steps)) hits |= 1u << e;
             if constexpr (decltype(sums)::value) {
               const u64 w = weigh(f);
               all += w;
@@ -460,6 +494,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
                 if (!decltype(limited)::value || w >= least_weight) sum += w;
               }
             }
+          }
+          if (hits) {
+            uint32_t at = atomicAdd(&S.listed, static_cast<uint32_t>(__popc(hits)));
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (hits >> e & 1 && at < kList) S.list[at++] = composite(v[e], index_of(b, e));
           }
           if (decltype(sums)::value && from > 0) {
             if (!decltype(limited)::value) above += sum;
@@ -481,13 +521,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       }
       cluster.sync();
       if (rank == 0) {
-        int n = S.listed;
-        for (int r = 1; r < n_cta; ++r) {
-          const int more = min(static_cast<int>(*cluster.map_shared_rank(&S.listed, r)), kList - n);
-          const u64* theirs = cluster.map_shared_rank(S.list, r);
-          for (int i = tid; i < more; i += kThreads) S.list[n + i] = theirs[i];
-          n += more;
+        uint32_t lists[kMostCtas];
+        of_all(&S.listed, lists);
+        int n = lists[0];
+        for (int i = tid; i - tid < kList; i += kThreads) {       // a round of all lists at a time
+          u64 v[kMostCtas];
+          bool more = false;
+#pragma unroll
+          for (int r = 1; r < kMostCtas; ++r)
+            if (r < n_cta && i < lists[r]) v[r] = *cluster.map_shared_rank(&S.list[i], r);
+          int to = n;
+#pragma unroll
+          for (int r = 1; r < kMostCtas; ++r) {
+            if (r < n_cta && i < lists[r] && to + i < kList) S.list[to + i] = v[r];
+            to += lists[r];
+            more = more || i - tid + kThreads < lists[r];
+          }
+          if (!more) break;
         }
+#pragma unroll
+        for (int r = 1; r < kMostCtas; ++r) n += lists[r];
+        n = min(n, kList);
         if (tid == 0) S.ends[0] = ~0ull, S.ends[1] = 0;
         __syncthreads();
         {
@@ -507,22 +561,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
         auto find = [&](auto by_index, u64 lo, u64 hi, u64 lowest, auto&& value_of, u64 upto, u64 target) -> u64 {
           auto order = [&](u64 c) { return decltype(by_index)::value ? c & kIndexMask : c; };
           while (true) {
-            const int shift = max(0, 64 - __clzll(hi - lo) - 9);
+            int shift = 63;       // one part
+            u64 bin = 0;
             bins[tid] = 0;
-            if (tid == 0) S.few = 0, S.at[0] = ~0ull;
+            if (tid == 0) S.few = 0, S.at[0] = ~0ull, S.at[2] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
-              const u64 c = S.list[i], o = order(c);
-              if (c >= lowest && o >= lo && o <= hi) atomicAdd(&bins[(hi - o) >> shift], value_of(c));
+            if (n > kFew) {
+              shift = max(0, 64 - __clzll(hi - lo) - 9);
+              for (int i = tid; i < n; i += kThreads) {
+                const u64 c = S.list[i], o = order(c);
+                if (c >= lowest && o >= lo && o <= hi) atomicAdd(&bins[(hi - o) >> shift], value_of(c));
+              }
+              __syncthreads();
+              u64 unused;
+              const u64 in = bins[tid], before = upto + cta_before(in, S.part, &unused);
+              if (before < target && target <= before + in) S.at[0] = tid, S.at[1] = before;
+              __syncthreads();
+              if (S.at[0] == ~0ull) return 0;       // not in the list
+              bin = S.at[0];
+              upto = S.at[1];
             }
-            __syncthreads();
-            u64 unused;
-            const u64 in = bins[tid], before = upto + cta_before(in, S.part, &unused);
-            if (before < target && target <= before + in) S.at[0] = tid, S.at[1] = before;
-            __syncthreads();
-            if (S.at[0] == ~0ull) return 0;       // not in the list
-            const u64 bin = S.at[0];
-            upto = S.at[1];
             for (int i = tid; i < n; i += kThreads) {
               const u64 c = S.list[i], o = order(c);
               if (c >= lowest && o >= lo && o <= hi && (hi - o) >> shift == bin) {
@@ -565,10 +623,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           if (n > k) mine = find(std::false_type{}, lowest_listed, highest_listed, 0ull, [](u64) { return 1ull; }, 0ull, static_cast<u64>(k));
           if (by_mass) whole = sum_from(mine, weight_of);
         } else {
-          for (int r = 0; r < n_cta; ++r) {
-            whole += *cluster.map_shared_rank(&S.sum_all, r);
-            over += *cluster.map_shared_rank(&S.sum_above, r);
-          }
+          whole = sum_of_all(&S.sum_all);
+          over = sum_of_all(&S.sum_above);
         }
         bool failed = false;
         if (by_mass) {
@@ -652,14 +708,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
         }
         cluster.sync();
         if (tid < kDigits) {
-          uint32_t n = 0;
-          u64 m = 0;
-          for (int r = 0; r < n_cta; ++r) {
-            n += *cluster.map_shared_rank(&S.count[parity][tid], r);
-            if (WEIGHTED) m += *cluster.map_shared_rank(&S.mass[parity][tid], r);
-          }
-          S.all_count[tid] = n;
-          if (WEIGHTED) S.all_mass[tid] = m;
+          S.all_count[tid] = sum_of_all(&S.count[parity][tid]);
+          if (WEIGHTED) S.all_mass[tid] = sum_of_all(&S.mass[parity][tid]);
         }
         parity ^= 1;      // the others read this level's until they come to the next level's barrier
         __syncthreads();
@@ -762,10 +812,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   if (tid == 0) S.kept = all, S.at[0] = ~0ull;
   cluster.sync();
   u64 total = 0, lower = 0;
-  for (int r = 0; r < n_cta; ++r) {
-    const u64 m = *cluster.map_shared_rank(&S.kept, r);
-    total += m;
-    if (r < rank) lower += m;
+  {
+    u64 v[kMostCtas];
+    of_all(&S.kept, v);
+#pragma unroll
+    for (int r = 0; r < kMostCtas; ++r) {
+      total += v[r];
+      if (r < rank) lower += v[r];
+    }
   }
   const u64 goal = __umul64hi(fraction(u), total);
   before += lower;
