@@ -39,9 +39,6 @@ constexpr int kRanges = 1024, kRangeColumns = 8;        // columns: lanes that f
 constexpr float kRangeSteps = 11.5f;      // of 1/256 in log2
 constexpr int kDigits = 256, kColumns = 8;
 constexpr int kList = 4096, kMostK = 2048;
-constexpr int kIndexBits = 20;
-constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
-static_assert(B200_MAX_SAMPLE_COLS <= 1 << kIndexBits, "indexes");
 using u64 = unsigned long long;
 
 struct Sample {
@@ -53,7 +50,7 @@ struct Sample {
   const int32_t* top_k;
   float t0, p0, m0;
   int k0;
-  int blocks_per_cta, frac;
+  int blocks_per_cta, frac, index_bits;
 };
 
 // ---- keys: whole numbers in the order of the logits; both zeros are one ------------------------------------------------------------------
@@ -135,6 +132,7 @@ struct alignas(16) Shared {
   uint2 table[256];             // 2^(30 + j / 256): as a whole number, as a float
   union {
     uint32_t ranges[kRanges * kRangeColumns];
+    u64 range_sum[kRanges];             // the cluster's range_count
     struct {
       uint32_t cnt[kDigits * kColumns], lo[kDigits * kColumns], hi[kDigits * kColumns];
     };
@@ -301,8 +299,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   };
   auto index_of = [&](int block, int e) { return (block0 + block) * kBlock + lane * 8 + e - head; };
   // an element's place in the order: its key over its index, upside down
-  auto composite = [&](uint32_t bits, int index) { return static_cast<u64>(Key<T>::of(bits)) << kIndexBits | (kIndexMask - static_cast<uint32_t>(index)); };
-  auto logit_of = [&](u64 c) { return value<T>(Key<T>::bits(static_cast<uint32_t>(c >> kIndexBits))); };
+  const uint32_t index_mask = (1u << A.index_bits) - 1;
+  auto composite = [&](uint32_t bits, int index) { return static_cast<u64>(Key<T>::of(bits)) << A.index_bits | (index_mask - static_cast<uint32_t>(index)); };
+  auto key_in = [&](u64 c) { return static_cast<uint32_t>(c >> A.index_bits); };
+  auto index_in = [&](u64 c) { return index_mask - (static_cast<uint32_t>(c) & index_mask); };
+  auto logit_of = [&](u64 c) { return value<T>(Key<T>::bits(key_in(c))); };
 
   // the CTAs' values of the cluster, all asked for before the first is needed
   auto of_all = [&](auto* mine, auto* values) {
@@ -428,12 +429,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     }
     if (tid == 0) S.from = 0, S.to = kRanges - 1;
     cluster.sync();
+    // each CTA sums a part of the ranges for all (all of them in every CTA: 10000 clocks instead of 4000)
+    for (int i = tid; i < kRanges / n_cta; i += kThreads) {
+      const int range = rank * (kRanges / n_cta) + i;
+      const u64 sum = sum_of_all(&S.range_count[range]);
+#pragma unroll
+      for (int r = 0; r < kMostCtas; ++r)
+        if (r < n_cta) *cluster.map_shared_rank(&S.range_sum[range], r) = sum;
+    }
+    cluster.sync();
     // numbers, and weights to second order of the steps (as whole numbers: the same sums in all CTAs)
     uint32_t c[kMine];
     u64 m[kMine], m_mine = 0, m_all, n_mine = 0, n_all;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const u64 both = sum_of_all(&S.range_count[tid * kMine + i]);
+      const u64 both = S.range_sum[tid * kMine + i];
       c[i] = static_cast<uint32_t>(both >> 32);
       const float of = static_cast<float>(c[i]), into = static_cast<float>(static_cast<uint32_t>(both)) / (1 << weigh.log_steps) - 0.5f * of;
       m[i] = static_cast<u64>(exp2f(40.f - (tid * kMine + i + 0.5f) * (kRangeSteps / 256.f)) * fmaf(into, -0.69314718f * kRangeSteps / 256.f, of));
@@ -520,6 +530,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
         }
       }
       cluster.sync();
+      if (k && rank > 0) {
+        cluster.sync();
+        return;
+      }
       if (rank == 0) {
         uint32_t lists[kMostCtas];
         of_all(&S.listed, lists);
@@ -542,12 +556,59 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
 #pragma unroll
         for (int r = 1; r < kMostCtas; ++r) n += lists[r];
         n = min(n, kList);
+        if (k) cluster.sync();        // the others are not needed any more
+        __syncthreads();
+        if (n <= kFew && from == 0) {
+          // few elements: every two of them are compared, by 512 threads together
+          u64* weights = S.range_count;
+          int parts = kThreads;
+          while (parts > 32 || (kThreads / parts) < n) parts /= 2;
+          const int i = tid / parts, part = tid & (parts - 1);
+          const u64 c = i < n ? S.list[i] : 0, w = i < n ? weigh(logit_of(c)) : 0;
+          if (part == 0 && i < n) weights[i] = w;
+          u64 whole = k ? 0 : sum_of_all(&S.sum_all);
+          __syncthreads();
+          auto before_mine = [&](auto&& earlier, u64* count) {
+            u64 sum = 0, n_before = 0;
+            for (int j = part; j < n; j += parts)
+              if (earlier(S.list[j])) sum += weights[j], ++n_before;
+            for (int o = 1; o < parts; o <<= 1) {
+              sum += __shfl_xor_sync(0xffffffffu, sum, o);
+              n_before += __shfl_xor_sync(0xffffffffu, n_before, o);
+            }
+            *count = n_before;
+            return sum;
+          };
+          u64 place, unused, sum;
+          const u64 heavier = before_mine([&](u64 o) { return o > c; }, &place);
+          bool keep = i < n && (!k || place < k);
+          if (by_mass) {
+            cta_before(keep && part == 0 ? w : 0ull, S.part, &sum);
+            const u64 limit = limit_of(p, k ? sum : whole);
+            if (!k && sum < limit && tid == 0) S.failed = 1;       // p of all is reached below the list
+            keep = keep && heavier < limit;
+          }
+          keep = keep && w >= least_weight;
+          __syncthreads();
+          if (part == 0 && i < n) weights[i] = keep ? w : 0;
+          cta_before(keep && part == 0 ? w : 0ull, S.part, &sum);
+          const u64 goal = __umul64hi(fraction(u), sum);
+          const u64 lower = before_mine([&](u64 o) { return (o & index_mask) > (c & index_mask); }, &unused);
+          if (keep && part == 0 && !S.failed && lower <= goal && goal < lower + w) A.out[row] = index_in(c);
+          n = 0;
+        }
+        if (n > 0) {
         if (tid == 0) S.ends[0] = ~0ull, S.ends[1] = 0;
         __syncthreads();
         {
           u64 lo = ~0ull, hi = 0;
           for (int i = tid; i < n; i += kThreads) lo = min(lo, S.list[i]), hi = max(hi, S.list[i]);
-          if (tid < n) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+          }
+          if (lane == 0) {
             atomicMin(&S.ends[0], lo);
             atomicMax(&S.ends[1], hi);
           }
@@ -559,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
         u64* bins = S.range_count;
         u64 *few = bins + kBins, *few_value = few + kFew;
         auto find = [&](auto by_index, u64 lo, u64 hi, u64 lowest, auto&& value_of, u64 upto, u64 target) -> u64 {
-          auto order = [&](u64 c) { return decltype(by_index)::value ? c & kIndexMask : c; };
+          auto order = [&](u64 c) { return decltype(by_index)::value ? c & index_mask : c; };
           while (true) {
             int shift = 63;       // one part
             u64 bin = 0;
@@ -639,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           for (int i = tid; i < n; i += kThreads) {
             const u64 c = S.list[i], w = c >= mine ? kept_of(c) : 0;
             if (w) {
-              const int place = static_cast<int>(kIndexMask - (static_cast<uint32_t>(c) & kIndexMask)) + head, b = place / kBlock, r = b / A.blocks_per_cta;
+              const int place = static_cast<int>(index_in(c)) + head, b = place / kBlock, r = b / A.blocks_per_cta;
               u64* sums = reinterpret_cast<u64*>(cluster.map_shared_rank(dynamic, r) + sizeof(Shared));
               atomicAdd(&sums[b - r * A.blocks_per_cta], w);
             }
@@ -647,10 +708,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           if (tid == 0) S.cut = mine;
         } else {        // all that is kept is in the list
           const u64 goal = __umul64hi(fraction(u), sum_from(mine, kept_of));
-          const u64 c = find(std::true_type{}, static_cast<u64>(kIndexMask + 1 - A.cols), static_cast<u64>(kIndexMask), mine, kept_of, 0ull, goal + 1);
-          if (tid == 0) A.out[row] = kIndexMask - (static_cast<uint32_t>(c) & kIndexMask);
+          const u64 c = find(std::true_type{}, static_cast<u64>(index_mask + 1 - A.cols), static_cast<u64>(index_mask), mine, kept_of, 0ull, goal + 1);
+          if (tid == 0) A.out[row] = index_in(c);
+        }
         }
       }
+      if (k) return;
       cluster.sync();
       if (*cluster.map_shared_rank(&S.failed, 0) == 0) {
         cut = *cluster.map_shared_rank(&S.cut, 0);
@@ -788,21 +851,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     cut = S.cut;
   }
 
+  const uint32_t cut_key = key_in(cut), cut_index = index_in(cut);
   auto kept_weight = [&](uint32_t bits, int index) -> u64 {
-    if (composite(bits, index) < cut) return 0;
+    const uint32_t key = Key<T>::of(bits);
+    if (key < cut_key || (key == cut_key && static_cast<uint32_t>(index) > cut_index)) return 0;
     const u64 w = weigh(value<T>(bits));
     return w >= least_weight ? w : 0;
   };
   // ---- kept weights of each block ----------------------------------------------------------------------------------------------------------------
   if (!summed) {
-    for (int b = warp; b < n_blocks; b += kWarps) {
-      const Eight<T> v = load(b);
-      u64 sum = 0;
+    auto sum_blocks = [&](auto&& weight_of) {
+      for (int b = warp; b < n_blocks; b += kWarps) {
+        const Eight<T> v = load(b);
+        u64 sum = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += kept_weight(v[e], index_of(b, e));
-      sum = warp_sum_of(sum);
-      if (lane == 0) block_mass[b] = sum;
-    }
+        for (int e = 0; e < 8; ++e) sum += weight_of(v[e], index_of(b, e));
+        sum = warp_sum_of(sum);
+        if (lane == 0) block_mass[b] = sum;
+      }
+    };
+    if (cut || least_weight) sum_blocks(kept_weight);
+    else sum_blocks([&](uint32_t bits, int) { return weigh(value<T>(bits)); });
     __syncthreads();
   }
   const int per = (n_blocks + kThreads - 1) / kThreads, b0 = min(tid * per, n_blocks), b1 = min(b0 + per, n_blocks);
@@ -872,13 +941,14 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
   int ctas = 1;
   while (ctas < 8 && bytes(ctas, true) > kHalf) ctas *= 2;
   const bool held = bytes(ctas, true) <= kMaxSmem;
-  while (ctas < 8 && 2 * ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 8 * ctas) ctas *= 2;
+  while (ctas < 8 && ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 8 * ctas) ctas *= 2;
   const size_t smem = bytes(ctas, held);
   if (smem > kMaxSmem) return fail(B200_ESHAPE, "%s: rows of %d", name, A.cols);
   A.blocks_per_cta = (blocks + ctas - 1) / ctas;
   int bits = 0;
   while ((1ll << bits) < A.cols) ++bits;
   A.frac = std::min(62 - bits, 44);
+  A.index_bits = std::max(bits, 1);
   auto kern = held ? sample_rows_kernel<T, true> : sample_rows_kernel<T, false>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   cudaLaunchConfig_t cfg{};
