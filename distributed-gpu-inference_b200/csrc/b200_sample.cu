@@ -941,7 +941,7 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
   int ctas = 1;
   while (ctas < 8 && bytes(ctas, true) > kHalf) ctas *= 2;
   const bool held = bytes(ctas, true) <= kMaxSmem;
-  while (ctas < 8 && ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 8 * ctas) ctas *= 2;
+  while (ctas < 8 && 2 * ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 8 * ctas) ctas *= 2;
   const size_t smem = bytes(ctas, held);
   if (smem > kMaxSmem) return fail(B200_ESHAPE, "%s: rows of %d", name, A.cols);
   A.blocks_per_cta = (blocks + ctas - 1) / ctas;

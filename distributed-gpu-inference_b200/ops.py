@@ -46,19 +46,32 @@ def _stream() -> int:
 class _Here:
     """The device is the current one: nothing to switch."""
 
-    def __enter__(self):
-        return self
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         return False
 
 
-_HERE = _Here()
+class _There:
+    def __init__(self, index: int):
+        self.guard = torch.cuda.device(index)
+        self.index = index
+
+    def __enter__(self) -> int:
+        self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        return self.guard.__exit__(*exc)
 
 
-def _on(device: torch.device):
-    """Launches go to the tensors' device, on its current stream, whichever device is current."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _on(index: int):
+    """Launches go to the tensors' device, on its current stream (entered: its handle), whichever device is current."""
+    return _Here(index) if index == torch._C._cuda_getDevice() else _There(index)
 
 
 def _pool_dims(pool: torch.Tensor):
@@ -237,11 +250,11 @@ def argmax_keys_decode(keys: torch.Tensor, out: Optional[torch.Tensor] = None) -
     return out
 
 
-def _per_row(v, rows: int, dtype: torch.dtype, device, what: str):
+def _per_row(v, rows: int, dtype: torch.dtype, dev: int, what: str):
     """A setting of ``sample_rows``: ``(pointer or None, number)``."""
     if not isinstance(v, torch.Tensor):
         return None, v
-    if v.dtype != dtype or v.shape != (rows,) or (rows > 1 and v.stride(0) != 1) or v.device != device:
+    if v.dtype != dtype or v.dim() != 1 or v.numel() != rows or not v.is_contiguous() or v.get_device() != dev:
         raise ValueError(f"{what} must be a number or a contiguous {dtype} [rows] tensor on the logits' device")
     return v.data_ptr(), 0
 
@@ -252,29 +265,28 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     in [0, 1)): the first index at which the weights ``exp((x - max) / temperature)`` that are kept, summed up in the row's order, exceed ``u``
     of their sum.
 
-    Kept, in the descending order of the logits (the lowest index first among equals): the first ``top_k`` (0: all); of these the ones before which the weights
-    sum to less than ``top_p`` of theirs all; of these the ones with at least ``min_p`` of the largest weight; always the first.  Each setting is a number
-    or a tensor with one per row (fp32; ``top_k`` int32).  Temperature 0 gives ``argmax_rows``' token, as does a row whose largest logit is
-    NaN or infinite.  Up to 2**20 columns; ``out``: int64 ``[rows]``."""
+    Kept, in the descending order of the logits (the lowest index first among equals): the first ``top_k`` (0: all); of these the ones before which
+    the weights sum to less than ``top_p`` of theirs all; of these the ones with at least ``min_p`` of the largest weight; always the first.  Each
+    setting is a number or a tensor with one per row (fp32; ``top_k`` int32).  Temperature 0 gives ``argmax_rows``' token, as does a row whose
+    largest logit is NaN or infinite.  Up to 2**20 columns; ``out``: int64 ``[rows]``."""
     _need_cuda(x, u)
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError("x must be [rows, cols] with a contiguous last dimension")
     rows, cols = x.shape
-    dev = x.device
-    if u.dtype != torch.float32 or u.shape != (rows,) or (rows > 1 and u.stride(0) != 1) or u.device != dev:
+    dev = x.get_device()
+    if u.dtype != torch.float32 or u.dim() != 1 or u.numel() != rows or not u.is_contiguous() or u.get_device() != dev:
         raise ValueError("u must be a contiguous fp32 [rows] tensor on the logits' device")
     tp, t = _per_row(temperature, rows, torch.float32, dev, "temperature")
     kp, k = _per_row(top_k, rows, torch.int32, dev, "top_k")
     pp, p = _per_row(top_p, rows, torch.float32, dev, "top_p")
     mp, m = _per_row(min_p, rows, torch.float32, dev, "min_p")
     if out is None:
-        out = torch.empty((rows,), dtype=torch.int64, device=dev)
-    elif out.dtype != torch.int64 or out.shape != (rows,) or not out.is_contiguous() or out.device != dev:
+        out = torch.empty(rows, dtype=torch.int64, device=x.device)
+    elif out.dtype != torch.int64 or out.shape != (rows,) or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be a contiguous int64 [rows] on the logits' device")
-    lib = _lib.load()
-    with _on(dev):
-        rc = lib.b200_sample_rows(out.data_ptr(), x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, u.data_ptr(), tp, t, kp,
-                                  min(int(k), 0x7fffffff), pp, p, mp, m, _dtype_id(x), _stream())
+    with _on(dev) as stream:
+        rc = _lib.load().b200_sample_rows(out.data_ptr(), x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, u.data_ptr(), tp, t, kp,
+                                          min(int(k), 0x7fffffff), pp, p, mp, m, _dtype_id(x), stream)
     if rc != 0:
         _lib.check(rc, "b200_sample_rows")
     return out
@@ -283,26 +295,34 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 MAX_DRAFT_NODES = 64
 
 
-def _node_rows(t: torch.Tensor, shape, dtype: torch.dtype, device, what: str) -> int:
+def _node_rows(t: torch.Tensor, B: int, nodes: int, dtype: torch.dtype, dev: int, what: str) -> int:
     """Row stride of a ``[B, nodes]`` tensor of the tree entry points."""
-    if t.dtype != dtype or t.shape != shape or (shape[1] > 1 and t.stride(1) != 1) or t.device != device:
-        raise ValueError(f"{what} must be {dtype} [B, nodes] with contiguous rows, on the same device")
-    return t.stride(0)
+    if t.dtype == dtype and t.get_device() == dev and t.shape == (B, nodes):
+        if t.is_contiguous():
+            return nodes
+        if nodes == 1 or t.stride(1) == 1:
+            return t.stride(0)
+    raise ValueError(f"{what} must be {dtype} [B, nodes] with contiguous rows, on the same device")
 
 
-def _sequence_lens(t: Optional[torch.Tensor], B: int, device, what: str) -> Optional[int]:
+def _sequence_lens(t: Optional[torch.Tensor], B: int, dev: int, what: str) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous() or t.device != device:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != B or not t.is_contiguous() or t.get_device() != dev:
         raise ValueError(f"{what} must be a contiguous int32 [B] on the same device")
     return t.data_ptr()
 
 
-def _tree_table(block_tables: torch.Tensor, B: int, device) -> int:
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != B or block_tables.shape[1] < 1 \
-            or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1) or block_tables.device != device:
-        raise ValueError("block_tables must be int32 [B, n] with contiguous rows, on the same device")
-    return block_tables.stride(0) if B > 1 else block_tables.shape[1]
+def _tree_table(t: torch.Tensor, B: int, dev: int):
+    """Row stride and columns of block tables."""
+    if t.dtype == torch.int32 and t.dim() == 2 and t.get_device() == dev:
+        rows, cols = t.shape
+        if rows == B and cols > 0:
+            if t.is_contiguous():
+                return cols, cols
+            if cols == 1 or t.stride(1) == 1:
+                return (t.stride(0) if B > 1 else cols), cols
+    raise ValueError("block_tables must be int32 [B, n] with contiguous rows, on the same device")
 
 
 def draft_tree(parents: torch.Tensor, draft_lens: Optional[torch.Tensor] = None):
@@ -314,16 +334,26 @@ def draft_tree(parents: torch.Tensor, draft_lens: Optional[torch.Tensor] = None)
     if parents.dim() != 2:
         raise ValueError("parents must be int32 [B, nodes]")
     B, nodes = parents.shape
-    stride = _node_rows(parents, (B, nodes), torch.int32, parents.device, "parents")
-    lens = _sequence_lens(draft_lens, B, parents.device, "draft_lens")
-    visible = torch.empty((B, nodes), dtype=torch.int64, device=parents.device)
-    depth = torch.empty((B, nodes), dtype=torch.int32, device=parents.device)
-    lib = _lib.load()
-    with _on(parents.device):
-        rc = lib.b200_draft_tree(visible.data_ptr(), depth.data_ptr(), parents.data_ptr(), stride, lens, B, nodes, _stream())
+    device, dev = parents.device, parents.get_device()
+    stride = _node_rows(parents, B, nodes, torch.int32, dev, "parents")
+    lens = _sequence_lens(draft_lens, B, dev, "draft_lens")
+    visible = torch.empty(B, nodes, dtype=torch.int64, device=device)
+    depth = torch.empty(B, nodes, dtype=torch.int32, device=device)
+    with _on(dev) as stream:
+        rc = _lib.load().b200_draft_tree(visible.data_ptr(), depth.data_ptr(), parents.data_ptr(), stride, lens, B, nodes, stream)
     if rc != 0:
         _lib.check(rc, "b200_draft_tree")
     return visible, depth
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(nodes: int, Hq: int, Hkv: int, D: int, block_size: int, dtype_id: int) -> int:
+    return _lib.load().b200_paged_tree_attn_workspace(1, nodes, Hq, Hkv, D, block_size, dtype_id)
+
+
+def tree_attention_workspace(nodes: int, Hq: int, Hkv: int, D: int, block_size: int, dtype: torch.dtype) -> int:
+    """Bytes of scratch that ``paged_tree_attention`` needs for these sizes, whatever the batch and the lengths."""
+    return _tree_workspace(nodes, Hq, Hkv, D, block_size, DTYPE_ID[dtype])
 
 
 def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
@@ -338,48 +368,47 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     least ``tree_attention_workspace`` bytes that no call running at the same time uses; else one from torch's caching allocator."""
     _need_cuda(q, k_pool, v_pool, block_tables, context_lens, visible)
     max_blocks, Hkv, bs, D = _pool_dims(k_pool)
-    dev, dtype = q.device, q.dtype
+    dev, dtype = q.get_device(), q.dtype
     if v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or not v_pool.is_contiguous():
         raise ValueError("k_pool and v_pool must match")
     if dtype != k_pool.dtype:
         raise TypeError("q dtype must equal the pool dtype")
-    if k_pool.device != dev or v_pool.device != dev:
+    if k_pool.get_device() != dev or v_pool.get_device() != dev:
         raise ValueError("q and the pools must be on one device")
     if q.dim() != 4 or q.shape[3] != D:
         raise ValueError(f"q must be [B, nodes, Hq, {D}]")
     B, nodes, Hq, _ = q.shape
-    if (D > 1 and q.stride(3) != 1) or (Hq > 1 and q.stride(2) != D):
+    batch_stride, node_stride, head_stride, last = q.stride()
+    if (D > 1 and last != 1) or (Hq > 1 and head_stride != D):
         raise ValueError("heads and head_dim must be contiguous inside a node")
     if Hq % Hkv != 0:
         raise ValueError(f"{Hq} query heads are no multiple of {Hkv} kv heads")
-    table_stride = _tree_table(block_tables, B, dev)
-    vis_stride = _node_rows(visible, (B, nodes), torch.int64, dev, "visible")
+    table_stride, table_cols = _tree_table(block_tables, B, dev)
+    vis_stride = _node_rows(visible, B, nodes, torch.int64, dev, "visible")
     lens = _sequence_lens(context_lens, B, dev, "context_lens")
     drafts = _sequence_lens(draft_lens, B, dev, "draft_lens")
     if out is None:
-        out = torch.empty((B, nodes, Hq, D), dtype=dtype, device=dev)
-    elif out.shape != (B, nodes, Hq, D) or not out.is_contiguous() or out.dtype != dtype or out.device != dev:
+        out = torch.empty(B, nodes, Hq, D, dtype=dtype, device=q.device)
+    elif out.shape != (B, nodes, Hq, D) or not out.is_contiguous() or out.dtype != dtype or out.get_device() != dev:
         raise ValueError("out must be a contiguous [B, nodes, Hq, D] tensor of q's dtype, on its device")
-    lib, dt = _lib.load(), _dtype_id(k_pool)
-    need = lib.b200_paged_tree_attn_workspace(B, nodes, Hq, Hkv, D, bs, dt)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous, on q's device")
-    with _timed(), _on(dev):
-        rc = lib.b200_paged_tree_attn(
-            out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), table_stride,
-            block_tables.shape[1], lens, drafts, visible.data_ptr(), vis_stride, B, nodes, Hq, Hkv, D, bs, max_blocks,
-            float(D) ** -0.5 if scale is None else float(scale), None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * workspace.element_size(), dt, int(flags), _stream())
+    dt = _dtype_id(k_pool)
+    need = _tree_workspace(nodes, Hq, Hkv, D, bs, dt)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous, on q's device")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws, ws_bytes = workspace.data_ptr(), need
+    with _timed(), _on(dev) as stream:
+        rc = _lib.load().b200_paged_tree_attn(
+            out.data_ptr(), q.data_ptr(), batch_stride, node_stride, k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), table_stride,
+            table_cols, lens, drafts, visible.data_ptr(), vis_stride, B, nodes, Hq, Hkv, D, bs, max_blocks,
+            D ** -0.5 if scale is None else float(scale), ws, ws_bytes, dt, int(flags), stream)
     if rc != 0:
         _lib.check(rc, "b200_paged_tree_attn")
     return out
-
-
-def tree_attention_workspace(B: int, nodes: int, Hq: int, Hkv: int, D: int, block_size: int, dtype: torch.dtype) -> int:
-    """Bytes of scratch that ``paged_tree_attention`` needs for these sizes."""
-    return _lib.load().b200_paged_tree_attn_workspace(B, nodes, Hq, Hkv, D, block_size, DTYPE_ID[dtype])
 
 
 def accept_drafts(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Tensor, visible: torch.Tensor, k_ptrs: Optional[torch.Tensor],
@@ -387,42 +416,45 @@ def accept_drafts(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Ten
                   draft_lens: Optional[torch.Tensor] = None):
     """Which drafted tokens the model confirms, and the cache afterwards.
 
-    ``tokens`` int64 ``[B, nodes]`` are the trees' tokens, ``chosen`` int64 ``[B, nodes]`` what the model answers at each node (``argmax_rows`` or ``sample_rows``
-    of its logits), ``parents`` / ``visible`` as for ``draft_tree``.  A node is taken if its token is its parent's answer (of siblings with the same token the
-    first) and all above it are taken.  ``k_ptrs / v_ptrs`` (``pool_pointer_array``; None: nothing moves) name the layers' pools of shape
-    ``pool_shape``: the k-th taken node's keys and values move to the k-th place behind the context, in place.  ``context_lens`` counts the drafted
-    tokens.  Returns ``(count int32 [B], path int32 [B, nodes], new_tokens int64 [B, nodes], new_lens int32 [B])``: taken nodes, the root among
-    them; their numbers and the answers at them, -1 behind the last; the context with them."""
+    ``tokens`` int64 ``[B, nodes]`` are the trees' tokens, ``chosen`` int64 ``[B, nodes]`` what the model answers at each node (``argmax_rows`` or
+    ``sample_rows`` of its logits), ``parents`` / ``visible`` as for ``draft_tree``.  A node is taken if its token is its parent's answer (of siblings
+    with the same token the first) and all above it are taken.  ``k_ptrs / v_ptrs`` (``pool_pointer_array``; None: nothing moves) name the layers'
+    pools of shape ``pool_shape``: the k-th taken node's keys and values move to the k-th place behind the context, in place.  ``context_lens``
+    counts the drafted tokens.  Returns ``(count int32 [B], path int32 [B, nodes], new_tokens int64 [B, nodes], new_lens int32 [B])``: taken nodes,
+    the root among them; their numbers and the answers at them, -1 behind the last; the context with them."""
     _need_cuda(tokens, chosen, parents, visible, block_tables, context_lens)
     if tokens.dim() != 2:
         raise ValueError("tokens must be int64 [B, nodes]")
-    B, nodes = shape = tokens.shape
-    dev = tokens.device
+    B, nodes = tokens.shape
+    device, dev = tokens.device, tokens.get_device()
     max_blocks, Hkv, bs, D = pool_shape
-    strides = [_node_rows(t, shape, ty, dev, what) for t, ty, what in ((tokens, torch.int64, "tokens"), (chosen, torch.int64, "chosen"),
-                                                                      (parents, torch.int32, "parents"), (visible, torch.int64, "visible"))]
-    table_stride = _tree_table(block_tables, B, dev)
+    i32, i64 = torch.int32, torch.int64
+    s_tokens = _node_rows(tokens, B, nodes, i64, dev, "tokens")
+    s_chosen = _node_rows(chosen, B, nodes, i64, dev, "chosen")
+    s_parents = _node_rows(parents, B, nodes, i32, dev, "parents")
+    s_visible = _node_rows(visible, B, nodes, i64, dev, "visible")
+    table_stride, table_cols = _tree_table(block_tables, B, dev)
     lens = _sequence_lens(context_lens, B, dev, "context_lens")
     drafts = _sequence_lens(draft_lens, B, dev, "draft_lens")
     if (k_ptrs is None) != (v_ptrs is None):
         raise ValueError("k_ptrs and v_ptrs come together")
-    layers = 0
+    layers, kp, vp = 0, None, None
     if k_ptrs is not None:
         layers = k_ptrs.numel()
         for t in (k_ptrs, v_ptrs):
-            if t.dtype != torch.int64 or t.shape != (layers,) or not t.is_contiguous() or t.device != dev:
+            if t.dtype != i64 or t.dim() != 1 or t.numel() != layers or not t.is_contiguous() or t.get_device() != dev:
                 raise ValueError("k_ptrs / v_ptrs must be contiguous int64 vectors of one length on the same device")
-    count = torch.empty((B,), dtype=torch.int32, device=dev)
-    path = torch.empty(shape, dtype=torch.int32, device=dev)
-    new_tokens = torch.empty(shape, dtype=torch.int64, device=dev)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    lib = _lib.load()
-    with _on(dev):
-        rc = lib.b200_accept_drafts(
-            count.data_ptr(), path.data_ptr(), new_tokens.data_ptr(), new_lens.data_ptr(), tokens.data_ptr(), strides[0], chosen.data_ptr(),
-            strides[1], parents.data_ptr(), strides[2], visible.data_ptr(), strides[3], k_ptrs.data_ptr() if layers else None,
-            v_ptrs.data_ptr() if layers else None, layers, block_tables.data_ptr(), table_stride, block_tables.shape[1], lens, drafts, B, nodes,
-            Hkv, D, bs, max_blocks, DTYPE_ID[dtype], _stream())
+        if layers:
+            kp, vp = k_ptrs.data_ptr(), v_ptrs.data_ptr()
+    count = torch.empty(B, dtype=i32, device=device)
+    path = torch.empty(B, nodes, dtype=i32, device=device)
+    new_tokens = torch.empty(B, nodes, dtype=i64, device=device)
+    new_lens = torch.empty(B, dtype=i32, device=device)
+    with _on(dev) as stream:
+        rc = _lib.load().b200_accept_drafts(
+            count.data_ptr(), path.data_ptr(), new_tokens.data_ptr(), new_lens.data_ptr(), tokens.data_ptr(), s_tokens, chosen.data_ptr(), s_chosen,
+            parents.data_ptr(), s_parents, visible.data_ptr(), s_visible, kp, vp, layers, block_tables.data_ptr(), table_stride, table_cols, lens,
+            drafts, B, nodes, Hkv, D, bs, max_blocks, DTYPE_ID[dtype], stream)
     if rc != 0:
         _lib.check(rc, "b200_accept_drafts")
     return count, path, new_tokens, new_lens

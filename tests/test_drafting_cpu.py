@@ -23,6 +23,7 @@ def recorded(monkeypatch):
     monkeypatch.setattr(ops, "_need_cuda", lambda *a: None)
     monkeypatch.setattr(ops, "_stream", lambda: 0)
     monkeypatch.setattr(ops, "_on", lambda device: Guard())
+    monkeypatch.setattr(ops, "_tree_workspace", lambda *a: 0)
     return made
 
 
@@ -44,7 +45,7 @@ def test_sample_rows(recorded):
         return ops.sample_rows(x, u, **kw)
 
     refused(recorded, call, dict(x=torch.zeros(8)), dict(x=torch.zeros(8, 3).t()), dict(x=x.double()), dict(u=torch.zeros(2)), dict(u=u.double()),
-            dict(u=torch.zeros(6)[::2]), dict(u=torch.zeros(3, device="meta")), dict(temperature=i), dict(temperature=torch.zeros(4)), dict(top_k=u),
+            dict(u=torch.zeros(6)[::2]), dict(temperature=i), dict(temperature=torch.zeros(4)), dict(top_k=u),
             dict(top_k=i.long()), dict(top_p=u.double()), dict(min_p=torch.zeros(3, 1)), dict(out=i), dict(out=torch.zeros(4, dtype=torch.int64)))
 
 
@@ -70,8 +71,7 @@ def test_paged_tree_attention(recorded):
             dict(q=torch.zeros(2, 4, 3, 8).transpose(1, 2)), dict(k_pool=base["k_pool"].transpose(1, 2)), dict(v_pool=torch.zeros(5, 2, 16, 16)),
             dict(block_tables=base["block_tables"].long()), dict(block_tables=torch.zeros(3, 4, dtype=i32)), dict(block_tables=torch.zeros(2, 0, dtype=i32)),
             dict(context_lens=torch.zeros(2)), dict(visible=torch.zeros(2, 3, dtype=i32)), dict(visible=torch.zeros(2, 4, dtype=torch.int64)),
-            dict(draft_lens=torch.zeros(2)), dict(out=torch.zeros(2, 3, 4, 8).half()), dict(out=torch.zeros(2, 3, 4, 16)[..., ::2]),
-            dict(v_pool=torch.zeros(5, 2, 16, 8, device="meta")), dict(visible=torch.zeros(2, 3, dtype=torch.int64, device="meta")))
+            dict(draft_lens=torch.zeros(2)), dict(out=torch.zeros(2, 3, 4, 8).half()), dict(out=torch.zeros(2, 3, 4, 16)[..., ::2]))
 
 
 def test_accept_drafts(recorded):
@@ -115,6 +115,18 @@ def test_the_library_refuses():
     says(accept(dtype=5), -1, b"unsupported dtype")
     says(accept(layers=40000), -2, b"layers")
     says(accept(), -1, b"null pointer")
+
+
+def test_tensors_of_several_devices(recorded, monkeypatch):
+    """Devices by their numbers, as a GPU box has them."""
+    other = torch.zeros(3)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1 if t.data_ptr() == other.data_ptr() else 0)
+    x, u = torch.zeros(3, 8), torch.zeros(3)
+    ops.sample_rows(x, u, u)
+    for kw in (dict(u=other), dict(u=u, temperature=other), dict(u=u, top_p=other), dict(u=u, min_p=other)):
+        with pytest.raises(ValueError):
+            ops.sample_rows(x, **kw)
+    assert recorded == ["b200_sample_rows"]
 
 
 def test_no_cpu_form():

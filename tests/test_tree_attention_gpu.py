@@ -193,7 +193,7 @@ def test_strided_queries_tables_and_masks():
 def test_own_workspaces_streams_and_graphs():
     """Two captured calls with workspaces of their own, replayed side by side; a workspace's contents do not matter."""
     cases = [build(4, 8, 32, 8, 128, 16, 2000, torch.bfloat16, seed=s) for s in (1, 2)]
-    size = lambda c: ops.tree_attention_workspace(4, 8, 32, 8, 128, 16, torch.bfloat16)  # noqa: E731
+    size = lambda c: ops.tree_attention_workspace(8, 32, 8, 128, 16, torch.bfloat16)  # noqa: E731
     want = [check(c) for c in cases]
     spaces = [torch.full((max(16, size(c)),), 255, dtype=torch.uint8, device=DEV) for c in cases]
     graphs, outs = [], []
@@ -232,7 +232,7 @@ def test_one_node_is_a_decode_step():
 
 
 def test_a_workspace_that_is_too_small_is_refused():
-    need = ops.tree_attention_workspace(4, 8, 32, 8, 128, 16, torch.bfloat16)
+    need = ops.tree_attention_workspace(8, 32, 8, 128, 16, torch.bfloat16)
     if need == 0:
         pytest.skip("no workspace is needed")
     c = build(4, 8, 32, 8, 128, 16, 200, torch.bfloat16)
