@@ -166,9 +166,11 @@ __device__ __forceinline__ int tiles_of(const TreeAttn& A, int b) {
 struct Walk {
   int b, g, t, nt;          // sequence, kv head, tile of nt
   int64_t left;             // tiles
-  __device__ __forceinline__ void next(const TreeAttn& A) {
-    --left;
-    if (++t < nt || left <= 0) return;
+  __device__ __forceinline__ int run() const { return static_cast<int>(min(static_cast<int64_t>(nt - t), left)); }       // tiles of this sequence and head
+  __device__ __forceinline__ void skip(const TreeAttn& A, int tiles) {        // no more than these
+    left -= tiles;
+    t += tiles;
+    if (t < nt || left <= 0) return;
     t = 0;
     if (++g < A.Hkv) return;
     g = 0;
@@ -181,28 +183,47 @@ struct Walk {
   }
 };
 
-// Tiles of all sequences and heads; by a whole warp
-__device__ __forceinline__ int64_t all_tiles(const TreeAttn& A) {
-  int64_t total = 0;
-  for (int b0 = 0; b0 < A.B; b0 += 32) {
-    const int b = b0 + (threadIdx.x & 31);
-    int n = b < A.B ? tiles_of(A, b) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total += n;
-  }
-  return total * A.Hkv;
-}
 __device__ __forceinline__ int64_t share_of(int64_t total, int workers) { return max((total + workers - 1) / workers, static_cast<int64_t>(1)); }
 
+// Tiles of 32 sequences at a time, a lane each; the first 128 are looked up once
+struct Lookup {
+  int n[4];
+  __device__ __forceinline__ explicit Lookup(const TreeAttn& A) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = i * 32 + (threadIdx.x & 31);
+      n[i] = b < A.B ? tiles_of(A, b) : 0;
+    }
+  }
+  __device__ __forceinline__ int at(const TreeAttn& A, int round) const {
+    if (round < 4) return round == 0 ? n[0] : round == 1 ? n[1] : round == 2 ? n[2] : n[3];
+    const int b = round * 32 + (threadIdx.x & 31);
+    return b < A.B ? tiles_of(A, b) : 0;
+  }
+};
+
+// Tiles of a head of the sequences before b, and of all
+__device__ __forceinline__ void tiles_before(const TreeAttn& A, const Lookup& look, int b, int64_t* before, int64_t* all) {
+  *before = *all = 0;
+  for (int round = 0; round * 32 < A.B; ++round) {
+    const int n = look.at(A, round);
+    *all += __reduce_add_sync(0xffffffffu, n);
+    *before += __reduce_add_sync(0xffffffffu, round * 32 + static_cast<int>(threadIdx.x & 31) < b ? n : 0);
+  }
+}
+
+// Where a worker begins; by a whole warp
 __device__ __forceinline__ Walk walk_of(const TreeAttn& A, int worker, int workers) {
-  const int64_t total = all_tiles(A), share = share_of(total, workers), from = worker * share;
+  const Lookup look(A);
+  int64_t none, total;
+  tiles_before(A, look, 0, &none, &total);
+  total *= A.Hkv;
+  const int64_t share = share_of(total, workers), from = worker * share;
   Walk w{0, 0, 0, 0, min(share, total - from)};
   if (w.left <= 0) return w;
   int64_t before = 0;       // tiles of a head of the sequences before
-  for (int b0 = 0; b0 < A.B; b0 += 32) {
-    const int lane = threadIdx.x & 31, b = b0 + lane;
-    const int n = b < A.B ? tiles_of(A, b) : 0;
+  for (int round = 0; round * 32 < A.B; ++round) {
+    const int lane = threadIdx.x & 31, n = look.at(A, round);
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -214,7 +235,7 @@ __device__ __forceinline__ Walk walk_of(const TreeAttn& A, int worker, int worke
       const int first = __ffs(here) - 1;
       const int nt = __shfl_sync(0xffffffffu, n, first);
       const int64_t in = from - (before + __shfl_sync(0xffffffffu, upto - n, first)) * A.Hkv;
-      w.b = b0 + first;
+      w.b = round * 32 + first;
       w.nt = nt;
       w.g = static_cast<int>(in / nt);
       w.t = static_cast<int>(in - static_cast<int64_t>(w.g) * nt);
@@ -242,27 +263,29 @@ __device__ __forceinline__ uint32_t numbers_only(uint32_t two) {
   return two;
 }
 
-// What was left out of the products: values of drafted tokens that are no numbers, columns c .. c + 31 of head g, for a row that sees the tokens `seen` of
-// the keys k0 .. k1 - 1.  Hardly ever called.
+// What was left out of the products: values of drafted tokens that are no numbers, `cols` columns from c on of head g, for a row that sees the tokens
+// `seen` of the keys k0 .. k1 - 1.  Hardly ever called.
 template <typename T, int D>
-__device__ __noinline__ void add_no_numbers(float* o, const TreeAttn& A, int b, int g, int base, int k0, int k1, uint64_t seen, int c) {
+__device__ __noinline__ void add_no_numbers(float* o, const TreeAttn& A, int b, int g, int base, int k0, int k1, uint64_t seen, int c, int cols) {
   for (int j = max(k0, base); j < k1; ++j) {
     if (!(seen >> (j - base) & 1)) continue;
     const int64_t page = A.block_tables[static_cast<int64_t>(b) * A.table_stride + j / A.bs];
     if (page < 0 || page >= A.max_blocks) continue;
     const T* v = static_cast<const T*>(A.v_pool) + ((page * A.Hkv + g) * A.bs + j % A.bs) * D + c;
-    for (int x = 0; x < 32; ++x) {
+    for (int x = 0; x < cols; ++x) {
       const float f = Cvt<T>::to_f32(v[x]);
       if (!(fabsf(f) < INFINITY)) o[x] += f;
     }
   }
 }
 
-template <typename T, int D>
+// SPLIT > 1: 128 / SPLIT rows, each in the lanes of SPLIT warps, which take a part of a tile's keys each: with 32 rows in one warp, its
+// exponentials alone were 512 clocks a tile.  Their outputs, each of its own keys, are put together at the end of a walk.
+template <typename T, int D, int SPLIT>
 __global__ void __launch_bounds__(kNT, kCtasPerSm)
 tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using P = Plan<D>;
-  constexpr int NB = P::kBufs;
+  constexpr int NB = P::kBufs, kRowWarps = 4 / SPLIT, kMine = kKeys / SPLIT;      // warps with rows of their own; keys of a tile for a warp
   extern __shared__ unsigned char raw_smem[];
   unsigned char* sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
   const uint32_t sm0 = smem_u32(sm);
@@ -274,7 +297,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int worker = blockIdx.x / W.blocks, block = blockIdx.x - worker * W.blocks;
   const int rep = A.Hq / A.Hkv, row0 = block * kRows;
-  const int soft_warps = (min(kRows, A.nodes * rep - row0) + 31) / 32;
+  const int row_warps = (min(kRows, A.nodes * rep - row0) + 31) / 32, soft_warps = SPLIT > 1 ? 4 : row_warps;       // SPLIT > 1: no more rows than fit
 
   asm volatile("griddepcontrol.launch_dependents;");
   if (tid == 0) {
@@ -298,82 +321,84 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm0 + P::kFlags), "n"(P::kTm) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  Walk w = walk_of(A, worker, W.workers);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = __shfl_sync(0xffffffffu, *tm_slot, 0);
-  Walk w = walk_of(A, worker, W.workers);
 
   if (warp >= kSoft / 32 && warp < (kSoft + kLoadK + kLoadV) / 32) {
     // ---- copies ------------------------------------------------------------------------------------------------------------------------------
     const bool values = warp >= (kSoft + kLoadK) / 32;
     const int me = tid - kSoft - kLoadK;        // of those that copy values
+    const int box = min(A.bs, kKeys), n_pages = kKeys / box, ahead = 32 / n_pages;      // rows of a copy, copies and (below) tiles of a look-up
     const int my_page = values ? lane * 2 + me / 32 : lane;       // two warps take turns
-    const int box = min(A.bs, kKeys), n_pages = kKeys / box;
     const uint32_t bar_in = values ? bar_v : bar_k, bar_free = values ? bar_o : bar_ke, bufs = sm0 + (values ? P::kV : P::kK);
     const CUtensorMap* map = values ? &v_map : &k_map;
-    int keys = 0, n = 0;
-    auto page_of = [&](const Walk& at) -> int64_t {     // this thread's page of a tile; -1: none
-      if (at.left <= 0 || my_page >= n_pages) return -1;
-      int k, d;
-      lengths(A, at.b, &k, &d);
-      const int j = at.t * kKeys + my_page * box;
-      if (j >= k) return -1;
-      const int64_t page = A.block_tables[static_cast<int64_t>(at.b) * A.table_stride + j / A.bs];
-      return page < 0 || page >= A.max_blocks ? A.max_blocks : page;      // (behind the pool: the copy brings zeros)
-    };
-    int64_t page = page_of(w);
-    for (int i = 0; w.left > 0; ++i) {
-      const Walk now = w;
-      lengths(A, now.b, &keys, &n);
-      w.next(A);
-      const int64_t next_page = page_of(w);
-      if (i >= NB) bar_wait(bar_free + 8 * (i % NB), (i / NB - 1) & 1, dead);
-      const uint32_t base = bufs + (i % NB) * (D / 64) * kBlk, bar = bar_in + 8 * (i % NB);
-      const int j0 = now.t * kKeys;
-      if (!values || j0 + kKeys <= keys - n) {
-        if (page >= 0) {
-          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((D / 64) * box * 128) : "memory");
-          const int row = static_cast<int>((page * A.Hkv + now.g) * A.bs) + (A.bs > kKeys ? j0 % A.bs : 0);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(base + c * kBlk + my_page * box * 128),
-                         "l"(map), "r"(64 * c), "r"(row), "r"(bar) : "memory");
+    for (int i = 0; w.left > 0;) {
+      const int b = w.b, g = w.g, run = w.run(), t0 = w.t;
+      int keys, n;
+      lengths(A, b, &keys, &n);
+      const int32_t* table = A.block_tables + static_cast<int64_t>(b) * A.table_stride;
+      // 32 pages at a time, the next ones under way: of tile at + lane / n_pages; -1: none, behind the pool (copies bring zeros): outside it
+      auto look_up = [&](int at) -> int {
+        const int t = at + lane / n_pages, j = t * kKeys + lane % n_pages * box;
+        if (t >= t0 + run || j >= keys) return -1;
+        const int page = table[j / A.bs];
+        return page < 0 || page >= A.max_blocks ? static_cast<int>(A.max_blocks) : page;
+      };
+      int pages = look_up(t0), later = look_up(t0 + ahead);
+      for (int x = 0; x < run; ++x, ++i) {
+        const int in = x % ahead;
+        if (x > 0 && in == 0) {
+          pages = later;
+          later = look_up(t0 + x + ahead);
         }
-      } else {
-        bool odd = false;
-        constexpr int kCh = D / 8, kAhead = 4;
-#pragma unroll 1
-        for (int u0 = 0; u0 < kKeys * kCh / kLoadV; u0 += kAhead) {
-          int4 v[kAhead];
+        if (i >= NB) bar_wait(bar_free + 8 * (i % NB), (i / NB - 1) & 1, dead);
+        const uint32_t base = bufs + (i % NB) * (D / 64) * kBlk, bar = bar_in + 8 * (i % NB);
+        const int j0 = (t0 + x) * kKeys;
+        if (!values || j0 + kKeys <= keys - n) {
+          const int page = __shfl_sync(0xffffffffu, pages, in * n_pages + (my_page < n_pages ? my_page : 0));
+          if (my_page < n_pages && page >= 0) {
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((D / 64) * box * 128) : "memory");
+            const int row = (page * A.Hkv + g) * A.bs + (A.bs > kKeys ? j0 % A.bs : 0);
 #pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            const int c = me + (u0 + u) * kLoadV, key = c / kCh, ch = c - key * kCh, j = j0 + key;
+            for (int c = 0; c < D / 64; ++c)
+              asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(base + c * kBlk + my_page * box * 128),
+                           "l"(map), "r"(64 * c), "r"(row), "r"(bar) : "memory");
+          }
+        } else {
+          // all loads before the first store
+          bool odd = false;
+          constexpr int kCh = D / 8, kPer = kKeys * kCh / kLoadV;
+          int4 v[kPer];
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) {
+            const int c = me + u * kLoadV, key = c / kCh, ch = c - key * kCh;
+            const int page = __shfl_sync(0xffffffffu, pages, in * n_pages + key / box);
             v[u] = make_int4(0, 0, 0, 0);
-            if (j < keys) {
-              const int64_t pg = A.block_tables[static_cast<int64_t>(now.b) * A.table_stride + j / A.bs];
-              if (pg >= 0 && pg < A.max_blocks) v[u] = *reinterpret_cast<const int4*>(static_cast<const T*>(A.v_pool) + ((pg * A.Hkv + now.g) * A.bs + j % A.bs) * D + ch * 8);
-            }
+            if (j0 + key < keys && page < A.max_blocks)
+              v[u] = *reinterpret_cast<const int4*>(static_cast<const T*>(A.v_pool) + ((static_cast<int64_t>(page) * A.Hkv + g) * A.bs + (j0 + key) % A.bs) * D + ch * 8);
           }
 #pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            const int c = me + (u0 + u) * kLoadV, key = c / kCh, ch = c - key * kCh;
-            uint32_t x[4] = {static_cast<uint32_t>(v[u].x), static_cast<uint32_t>(v[u].y), static_cast<uint32_t>(v[u].z), static_cast<uint32_t>(v[u].w)};
+          for (int u = 0; u < kPer; ++u) {
+            const int c = me + u * kLoadV, key = c / kCh, ch = c - key * kCh;
+            uint32_t y[4] = {static_cast<uint32_t>(v[u].x), static_cast<uint32_t>(v[u].y), static_cast<uint32_t>(v[u].z), static_cast<uint32_t>(v[u].w)};
             if (j0 + key >= keys - n) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                odd = odd || no_number<T>(x[e]);
-                x[e] = numbers_only<T>(x[e]);
+                odd = odd || no_number<T>(y[e]);
+                y[e] = numbers_only<T>(y[e]);
               }
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(base, key, ch, kKeys)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(base, key, ch, kKeys)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
           }
+          if (odd) *strange = 1;
+          fence_smem_to_mma();
         }
-        if (odd) *strange = 1;
-        fence_smem_to_mma();
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
       }
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-      page = next_page;
+      w.skip(A, run);
     }
   } else if (warp == kNT / 32 - 1) {
     // ---- products ----------------------------------------------------------------------------------------------------------------------------
@@ -390,12 +415,12 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
     };
     int i = 0;
     for (int seg = 0; w.left > 0; ++seg) {
-      const int tiles = static_cast<int>(min(static_cast<int64_t>(w.nt - w.t), w.left));
+      const int run = w.run();
       bar_wait(bar_q, seg & 1, dead);       // queries are in, the rows before them out
       tc_fence_after();
       scores(i);
-      for (int x = 0; x < tiles; ++x, ++i) {
-        if (x + 1 < tiles) {
+      for (int x = 0; x < run; ++x, ++i) {
+        if (x + 1 < run) {
           // S of the next tile goes where P of the one before is being read
           if (x > 0) bar_wait(bar_o + 8 * ((i - 1) % NB), ((i - 1) / NB) & 1, dead);
           scores(i + 1);
@@ -409,33 +434,33 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
           mma_ts(tm + P::kO, tm + (i & 1) * kKeys + 8 * kk, operand(v + kk * 2048, kBlk, 1024), instr<T>(D, true), x > 0 || kk > 0);
         mma_commit(bar_o + 8 * (i % NB));
       }
-      w.t += tiles - 1;
-      w.left -= tiles - 1;
-      w.next(A);
+      w.skip(A, run);
     }
     __syncwarp();
   } else if (warp < soft_warps) {
     // ---- softmax: thread = row ---------------------------------------------------------------------------------------------------------------
-    const int node = (row0 + tid) / rep;
+    const int my_row = warp % kRowWarps * 32 + lane, part = warp / kRowWarps, node = (row0 + my_row) / rep;       // part: of the keys
     const uint32_t tm_row = tm + (static_cast<uint32_t>(32 * warp) << 16);
     const float k2 = A.scale > 0.f ? A.scale * kLog2e : 1.f;       // weight = 2^(s k2 - m)
     const int per = W.rows;
     int i = 0;
     while (w.left > 0) {
-      const int b = w.b, g = w.g, t0 = w.t, tiles = static_cast<int>(min(static_cast<int64_t>(w.nt - w.t), w.left));
+      const int b = w.b, g = w.g, t0 = w.t, run = w.run();
       int keys, n;
       lengths(A, b, &keys, &n);
       const int base = keys - n;
       const bool live = node < n;
+      uint64_t seen = live ? static_cast<uint64_t>(A.visible[b * A.visible_stride + node]) : 0ull;
+      if (n < 64) seen &= (1ull << n) - 1;
       {
         constexpr int kCh = D / 8;
         const T* q = static_cast<const T*>(A.q) + b * A.q_batch_stride;
 #pragma unroll 8
         for (int u = 0; u < kCh; ++u) {
-          const int c = lane + u * 32, r = 32 * warp + c / kCh, ch = c % kCh;       // a warp's rows by itself
-          const int t = (row0 + r) / rep, h = g * rep + row0 + r - t * rep;
+          const int c = lane + u * 32, r = c / kCh, ch = c % kCh, at = row0 + warp % kRowWarps * 32 + r;       // a warp's rows by itself
+          const int t = at / rep, h = g * rep + at - t * rep;
           const bool in = t < n;
-          cp16(line(sm0 + P::kQ, r, ch, kRows), in ? q + t * A.q_node_stride + static_cast<int64_t>(h) * D + ch * 8 : q, in);
+          cp16(line(sm0 + P::kQ, 32 * warp + r, ch, kRows), in ? q + t * A.q_node_stride + static_cast<int64_t>(h) * D + ch * 8 : q, in);
         }
         cp_commit();
         cp_wait<0>();
@@ -443,40 +468,46 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
         tc_fence_before();
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_q) : "memory");
       }
-      uint64_t seen = live ? static_cast<uint64_t>(A.visible[b * A.visible_stride + node]) : 0ull;
-      if (n < 64) seen &= (1ull << n) - 1;
-      float m_ref = -INFINITY, l = 0.f;     // the maximum in powers of two; -inf until the row sees a key
+      float m_ref = -INFINITY, l = 0.f;     // a power of two that the weights are relative to; -inf until the row sees a key
       bool ok = true;
-      for (int x = 0; x < tiles; ++x, ++i) {
+      for (int x = 0; x < run; ++x, ++i) {
         const int j0 = (t0 + x) * kKeys;
         ok = bar_wait(bar_s + 8 * (i & 1), (i >> 1) & 1, dead) && ok;
         tc_fence_after();
-        float s[2][32];
-        tm_ld32(s[0], tm_row + (i & 1) * kKeys);
-        tm_ld32(s[1], tm_row + (i & 1) * kKeys + 32);
+        float s[kMine];
+        if constexpr (SPLIT == 1) {
+          tm_ld32(*reinterpret_cast<float(*)[32]>(s), tm_row + (i & 1) * kKeys);
+          tm_ld32(*reinterpret_cast<float(*)[32]>(s + 32), tm_row + (i & 1) * kKeys + 32);
+        } else if constexpr (SPLIT == 2) {
+          tm_ld32(*reinterpret_cast<float(*)[32]>(s), tm_row + (i & 1) * kKeys + 32 * part);
+        } else {
+          tm_ld16(*reinterpret_cast<float(*)[16]>(s), tm_row + (i & 1) * kKeys + 16 * part);
+        }
         tc_wait_ld();
         if (A.scale <= 0.f) {
 #pragma unroll
-          for (int c = 0; c < kKeys; ++c) s[c >> 5][c & 31] *= A.scale * kLog2e;
+          for (int c = 0; c < kMine; ++c) s[c] *= A.scale * kLog2e;
         }
         if (j0 + kKeys > base) {        // bit c: key j0 + c is seen
           const int past = base - j0;
-          const uint64_t keep = past > 0 ? (seen << past) | ((1ull << past) - 1) : (past > -64 ? seen >> -past : 0ull);
+          uint64_t keep = past > 0 ? (seen << past) | ((1ull << past) - 1) : (past > -64 ? seen >> -past : 0ull);
+          if (SPLIT > 1) keep >>= part * kMine;
           const uint32_t half[2] = {static_cast<uint32_t>(keep), static_cast<uint32_t>(keep >> 32)};
 #pragma unroll
-          for (int c = 0; c < kKeys; ++c)
-            if (!(half[c >> 5] >> (c & 31) & 1)) s[c >> 5][c & 31] = -INFINITY;
+          for (int c = 0; c < kMine; ++c)
+            if (!(half[c >> 5] >> (c & 31) & 1)) s[c] = -INFINITY;
         }
-        float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+        float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < kKeys - 4; c += 8) {
+        for (int c = 4; c < kMine - 4; c += 8) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], s[c >> 5][(c & 31) + u], s[(c + 4) >> 5][((c + 4) & 31) + u]);
+          for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], s[c + u], s[c + 4 + u]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[1][28 + u]);
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], s[kMine - 4 + u]);
         const float m_new = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * k2;
-        const bool grow = m_new > m_ref;
+        // the reference moves once the maximum is 2^8 above it: weights keep their digits wherever they lie, sums and outputs are fp32
+        const bool grow = m_new > m_ref + 8.f;
         const float corr = grow ? exp2_fast(m_ref - m_new) : 1.0f;      // 0 where nothing was seen before
         if (grow) m_ref = m_new;
         if (x > 0 && __any_sync(0xffffffffu, grow)) {
@@ -486,24 +517,32 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
         }
         const f32x2 kk = both(k2), mm = both(m_ref == -INFINITY ? 0.f : -m_ref);      // a row that sees no key yet keeps weights 0
         f32x2 sum[2] = {0ull, 0ull};
+        uint32_t p[32];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t p[16];
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float u = s[y][c], v = s[y][c + 1];
-            scale_shift(u, v, kk, mm);
-            u = exp2_fast(u);
-            v = exp2_fast(v);
-            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pair(u, v));
-            p[c >> 1] = pack2<T>(u, v);
+        for (int c = 0; c < kMine; c += 2) {
+          float u = s[c], v = s[c + 1];
+          scale_shift(u, v, kk, mm);
+          u = exp2_fast(u);
+          v = exp2_fast(v);
+          sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pair(u, v));
+          p[c >> 1] = pack2<T>(u, v);
+          if constexpr (SPLIT == 1) {
+            if (c % 32 == 30) tm_st16(tm_row + (i & 1) * kKeys + c / 32 * 16, *reinterpret_cast<uint32_t(*)[16]>(p + c / 32 * 16));
           }
-          tm_st16(tm_row + (i & 1) * kKeys + y * 16, p);
         }
-        float part[4];
-        apart(part[0], part[1], sum[0]);
-        apart(part[2], part[3], sum[1]);
-        l = fmaf(l, corr, (part[0] + part[1]) + (part[2] + part[3]));
+        if constexpr (SPLIT > 1) {      // the other warps' keys: 0
+          uint32_t z[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) z[c] = SPLIT == 4 ? ((c < 8) == (part % 2 == 0) ? p[c & 7] : 0u) : p[c];
+          uint32_t none[16] = {};
+          const bool second = SPLIT == 4 ? part >= 2 : part == 1;
+          tm_st16(tm_row + (i & 1) * kKeys + (second ? 16 : 0), z);
+          tm_st16(tm_row + (i & 1) * kKeys + (second ? 0 : 16), none);
+        }
+        float some[4];
+        apart(some[0], some[1], sum[0]);
+        apart(some[2], some[3], sum[1]);
+        l = fmaf(l, corr, (some[0] + some[1]) + (some[2] + some[3]));
         tc_wait_st();
         tc_fence_before();
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_p + 8 * (i & 1)) : "memory");
@@ -511,40 +550,84 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
       ok = bar_wait(bar_o + 8 * ((i - 1) % NB), ((i - 1) / NB) & 1, dead) && ok;
       tc_fence_after();
       ok = ok && !*dead;
-      const bool whole = t0 == 0 && tiles == w.nt, odd = *strange != 0;
+      const bool whole = t0 == 0 && run == w.nt, odd = *strange != 0;
       const int64_t piece = (static_cast<int64_t>(worker) * W.blocks + block) * 2 + (t0 == 0);
-      float f = 1.f;
-      if (whole) f = ok ? (l == 0.f ? 0.f : 1.0f / l) : NAN;
-      else if (tid < per) W.ml[piece * per + tid] = make_float2(m_ref, ok ? l : NAN);
+      auto others_too = [&] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+      float scaled = 1.f;      // this warp's output to the row's common reference
+      if constexpr (SPLIT > 1) {
+        float2* ml = reinterpret_cast<float2*>(sm + P::kK - 1024);        // behind the rows that are put together below
+        ml[tid] = make_float2(m_ref, ok ? l : NAN);
+        others_too();
+        float top = -INFINITY;
+#pragma unroll
+        for (int y = 0; y < SPLIT; ++y) top = fmaxf(top, ml[my_row + y * (kRows / SPLIT)].x);
+        l = 0.f;
+#pragma unroll
+        for (int y = 0; y < SPLIT; ++y) {
+          const float2 one = ml[my_row + y * (kRows / SPLIT)];
+          l = fmaf(one.y, one.x == -INFINITY ? 0.f : exp2_fast(one.x - top), l);
+        }
+        scaled = m_ref == -INFINITY ? 0.f : exp2_fast(m_ref - top);
+        m_ref = top;
+        ok = l == l;
+      }
+      const float f = !whole ? 1.f : ok ? (l == 0.f ? 0.f : 1.0f / l) : NAN;
+      if (!whole && part == 0) W.ml[piece * per + my_row] = make_float2(m_ref, ok ? l : NAN);
+      T* out = static_cast<T*>(A.out) + static_cast<int64_t>(b) * A.nodes * A.Hq * D;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
+        constexpr int kCols = 32 / SPLIT;       // of the 32 that this warp finishes, from c + part * kCols on
         float o[32];
         __syncwarp();
         tm_ld32(o, tm_row + P::kO + c);
         tc_wait_ld();
+        if constexpr (SPLIT > 1) {
+          // [part][column / 4][row] of four columns
+          float4* all = reinterpret_cast<float4*>(sm + P::kQ);
+          constexpr int kSet = kRows / SPLIT;
+          others_too();
+#pragma unroll
+          for (int u = 0; u < 32; u += 4) all[(part * 8 + u / 4) * kSet + my_row] = make_float4(o[u] * scaled, o[u + 1] * scaled, o[u + 2] * scaled, o[u + 3] * scaled);
+          others_too();
+#pragma unroll
+          for (int u = 0; u < kCols; u += 4) {
+            float4 sum = all[(part * kCols + u) / 4 * kSet + my_row];
+#pragma unroll
+            for (int y = 1; y < SPLIT; ++y) {
+              const float4 more = all[(y * 8 + (part * kCols + u) / 4) * kSet + my_row];
+              sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+            }
+            o[u] = sum.x, o[u + 1] = sum.y, o[u + 2] = sum.z, o[u + 3] = sum.w;
+          }
+        }
+        const int c0 = c + part * kCols;
         if (odd && live) {
-          float other[32];      // (an array that a function sees is kept in memory)
+          float other[kCols];      // (an array that a function sees is kept in memory)
 #pragma unroll
-          for (int u = 0; u < 32; ++u) other[u] = o[u];
-          add_no_numbers<T, D>(other, A, b, g, base, t0 * kKeys, min((t0 + tiles) * kKeys, keys), seen, c);
+          for (int u = 0; u < kCols; ++u) other[u] = o[u];
+          add_no_numbers<T, D>(other, A, b, g, base, t0 * kKeys, min((t0 + run) * kKeys, keys), seen, c0, kCols);
 #pragma unroll
-          for (int u = 0; u < 32; ++u) o[u] = other[u];
+          for (int u = 0; u < kCols; ++u) o[u] = other[u];
         }
         if (!whole) {
 #pragma unroll
-          for (int u = 0; u < 32; u += 4) W.o[(piece * (D / 4) + (c + u) / 4) * per + tid] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+          for (int u = 0; u < kCols; u += 4) W.o[(piece * (D / 4) + (c0 + u) / 4) * per + my_row] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
         } else {
 #pragma unroll
-          for (int u = 0; u < 32; u += 8) {
-            uint32_t p[4];
+          for (int u = 0; u < kCols; u += 8) {
+            uint32_t y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = pack2<T>(o[u + 2 * e] * f, o[u + 2 * e + 1] * f);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(sm0 + P::kQ, tid, (c + u) / 8, kRows)), "r"(p[0]), "r"(p[1]), "r"(p[2]),
-                         "r"(p[3]) : "memory");
+            for (int e = 0; e < 4; ++e) y[e] = pack2<T>(o[u + 2 * e] * f, o[u + 2 * e + 1] * f);
+            if constexpr (SPLIT == 1) {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(sm0 + P::kQ, tid, (c + u) / 8, kRows)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+            } else if (live) {
+              const int t = node, h = g * rep + row0 + my_row - t * rep;
+              *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(t) * A.Hq + h) * D + c0 + u) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
           }
         }
       }
-      if (whole) {      // from where the warp's queries were (they have been read), rows side by side
+      if (SPLIT == 1 && whole) {      // from where the warp's queries were (they have been read), rows side by side
         __syncwarp();
         constexpr int kCh = D / 8;
 #pragma unroll 4
@@ -553,14 +636,13 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
           if (t < n) {
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(line(sm0 + P::kQ, 32 * warp + r, ch, kRows)) : "memory");
-            *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + ((static_cast<int64_t>(b) * A.nodes + t) * A.Hq + h) * D + ch * 8) = v;
+            *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(t) * A.Hq + h) * D + ch * 8) = v;
           }
         }
-        __syncwarp();
       }
-      w.t += tiles - 1;
-      w.left -= tiles - 1;
-      w.next(A);
+      if constexpr (SPLIT > 1) others_too();       // the next queries go where the outputs were
+      __syncwarp();
+      w.skip(A, run);
     }
   }
   tc_fence_before();
@@ -576,14 +658,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttn A, const
   int keys, n;
   lengths(A, b, &keys, &n);
   const int nt = tiles_of(A, b);
-  int64_t before = 0, all = 0;
-  for (int b0 = 0; b0 < A.B; b0 += 32) {
-    int m = b0 + lane < A.B ? tiles_of(A, b0 + lane) : 0, low = b0 + lane < b ? m : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o), low += __shfl_xor_sync(0xffffffffu, low, o);
-    all += m;
-    before += low;
-  }
+  int64_t before, all;
+  tiles_before(A, Lookup(A), b, &before, &all);
   const int64_t share = share_of(all * A.Hkv, W.workers), from = before * A.Hkv + static_cast<int64_t>(g) * nt;
   const int first = static_cast<int>(from / share), last = nt > 0 ? static_cast<int>((from + nt - 1) / share) : first;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -652,7 +728,8 @@ int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap&
   Shares W = shares_of(A.nodes, A.Hq, A.Hkv);
   W.ml = static_cast<float2*>(workspace);
   W.o = reinterpret_cast<float4*>(static_cast<char*>(workspace) + sums_bytes(W));
-  auto kern = tree_attn_kernel<T, D>;
+  const int rows = A.nodes * (A.Hq / A.Hkv);
+  auto kern = rows <= 32 ? tree_attn_kernel<T, D, 4> : rows <= 64 ? tree_attn_kernel<T, D, 2> : tree_attn_kernel<T, D, 1>;
   constexpr int smem = Plan<D>::kEnd + 1024;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   kern<<<W.workers * W.blocks, kNT, smem, stream>>>(A, W, k_map, v_map);
