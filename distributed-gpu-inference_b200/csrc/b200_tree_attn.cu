@@ -165,8 +165,8 @@ __device__ __forceinline__ int tiles_of(const TreeAttn& A, int b) {
 // A worker's way through the tiles
 struct Walk {
   int b, g, t, nt;          // sequence, kv head, tile of nt
-  int64_t left;             // tiles
-  __device__ __forceinline__ int run() const { return static_cast<int>(min(static_cast<int64_t>(nt - t), left)); }       // tiles of this sequence and head
+  int left;                 // tiles
+  __device__ __forceinline__ int run() const { return min(nt - t, left); }       // tiles of this sequence and head
   __device__ __forceinline__ void skip(const TreeAttn& A, int tiles) {        // no more than these
     left -= tiles;
     t += tiles;
@@ -183,7 +183,8 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ int64_t share_of(int64_t total, int workers) { return max((total + workers - 1) / workers, static_cast<int64_t>(1)); }
+// (tiles have numbers of 31 bits: the launch sees to it; a division of 64 costs 500 clocks)
+__device__ __forceinline__ int share_of(int total, int workers) { return max(static_cast<int>((static_cast<unsigned>(total) + workers - 1) / workers), 1); }
 
 // Tiles of 32 sequences at a time, a lane each; the first 128 are looked up once
 struct Lookup {
@@ -203,7 +204,7 @@ struct Lookup {
 };
 
 // Tiles of a head of the sequences before b, and of all
-__device__ __forceinline__ void tiles_before(const TreeAttn& A, const Lookup& look, int b, int64_t* before, int64_t* all) {
+__device__ __forceinline__ void tiles_before(const TreeAttn& A, const Lookup& look, int b, int* before, int* all) {
   *before = *all = 0;
   for (int round = 0; round * 32 < A.B; ++round) {
     const int n = look.at(A, round);
@@ -215,13 +216,15 @@ __device__ __forceinline__ void tiles_before(const TreeAttn& A, const Lookup& lo
 // Where a worker begins; by a whole warp
 __device__ __forceinline__ Walk walk_of(const TreeAttn& A, int worker, int workers) {
   const Lookup look(A);
-  int64_t none, total;
+  int none, total;
   tiles_before(A, look, 0, &none, &total);
   total *= A.Hkv;
-  const int64_t share = share_of(total, workers), from = worker * share;
+  const int share = share_of(total, workers);
+  if (worker > total / share) return Walk{0, 0, 0, 0, 0};
+  const int from = worker * share;
   Walk w{0, 0, 0, 0, min(share, total - from)};
   if (w.left <= 0) return w;
-  int64_t before = 0;       // tiles of a head of the sequences before
+  int before = 0;       // tiles of a head of the sequences before
   for (int round = 0; round * 32 < A.B; ++round) {
     const int lane = threadIdx.x & 31, n = look.at(A, round);
     int upto = n;
@@ -232,13 +235,12 @@ __device__ __forceinline__ Walk walk_of(const TreeAttn& A, int worker, int worke
     }
     const unsigned here = __ballot_sync(0xffffffffu, from < (before + upto) * A.Hkv);
     if (here) {
-      const int first = __ffs(here) - 1;
-      const int nt = __shfl_sync(0xffffffffu, n, first);
-      const int64_t in = from - (before + __shfl_sync(0xffffffffu, upto - n, first)) * A.Hkv;
+      const int first = __ffs(here) - 1, nt = __shfl_sync(0xffffffffu, n, first);
+      const int in = from - (before + __shfl_sync(0xffffffffu, upto - n, first)) * A.Hkv;
       w.b = round * 32 + first;
       w.nt = nt;
-      w.g = static_cast<int>(in / nt);
-      w.t = static_cast<int>(in - static_cast<int64_t>(w.g) * nt);
+      w.g = in / nt;
+      w.t = in - w.g * nt;
       return w;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -650,49 +652,74 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(P::kTm));
 }
 
-// One CTA per (sequence and kv head, 32 rows): what the workers' ends cut in pieces is put together, rows without a node become 0.
-template <typename T, int D>
+// One CTA per (sequence and kv head, 32 rows, a part of the columns): what the workers' ends cut in pieces is put together, rows without a node become 0.
+// Bound by the latency of its loads: all that it needs before the pieces is done before the kernel ahead ends, and pieces are asked for several at a
+// time (one after another: 7 us behind a walk of three tiles, and 11 behind the 64 sequences of 2k).
+template <typename T, int D, int PER>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttn A, const Shares W) {
   const int b = blockIdx.x / A.Hkv, g = blockIdx.x - b * A.Hkv, rep = A.Hq / A.Hkv;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at0 = blockIdx.y * 32, row = at0 + lane, t = row / rep, h = g * rep + row - t * rep;
-  int keys, n;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane, t = row / rep, h = g * rep + row - t * rep;
+  int keys, n, before, all;
   lengths(A, b, &keys, &n);
-  const int nt = tiles_of(A, b);
-  int64_t before, all;
+  const int nt = n > 0 ? (keys + kKeys - 1) / kKeys : 0;
   tiles_before(A, Lookup(A), b, &before, &all);
-  const int64_t share = share_of(all * A.Hkv, W.workers), from = before * A.Hkv + static_cast<int64_t>(g) * nt;
-  const int first = static_cast<int>(from / share), last = nt > 0 ? static_cast<int>((from + nt - 1) / share) : first;
+  const int share = share_of(all * A.Hkv, W.workers), from = before * A.Hkv + g * nt;
+  const int first = from / share, last = nt > 0 ? (from + nt - 1) / share : first;
+  const bool live = t < n;
+  const bool nothing = row >= A.nodes * rep || (live && first == last);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= A.nodes * rep) return;
-  T* out = static_cast<T*>(A.out) + ((static_cast<int64_t>(b) * A.nodes + t) * A.Hq + h) * D;
-  if (t < n && first == last) return;
-  const int in_block = row % kRows, block = row / kRows;
+  if (__all_sync(0xffffffffu, nothing)) return;
+  const int in_block = row % kRows, block = row / kRows, c0 = (blockIdx.z * 8 + warp) * PER;
+  auto piece_of = [&](int p) { return (static_cast<int64_t>(p) * W.blocks + block) * 2 + (p == first); };
   float top = -INFINITY, sum = 0.f;
   bool odd = false;
-  if (t < n) {
-    for (int p = first; p <= last; ++p) {
-      const float2 ml = W.ml[((static_cast<int64_t>(p) * W.blocks + block) * 2 + (p == first)) * W.rows + in_block];
-      odd = odd || ml.y != ml.y;
-      top = fmaxf(top, ml.x);
+  float4 o[PER];
+#pragma unroll
+  for (int c = 0; c < PER; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live && !nothing) {
+    constexpr int kAhead = 8 / PER;
+    for (int p0 = first; p0 <= last; p0 += kAhead) {
+      float2 ml[kAhead];
+      float4 v[kAhead][PER];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (p0 + u > last) continue;
+        const int64_t piece = piece_of(p0 + u);
+        ml[u] = W.ml[piece * W.rows + in_block];
+#pragma unroll
+        for (int c = 0; c < PER; ++c) v[u][c] = W.o[(piece * (D / 4) + c0 + c) * W.rows + in_block];
+      }
+      float now = top;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (p0 + u <= last) {
+          odd = odd || ml[u].y != ml[u].y;
+          now = fmaxf(now, ml[u].x);
+        }
+      if (now == -INFINITY) continue;
+      const float was = top == -INFINITY ? 0.f : exp2_fast(top - now);
+      top = now;
+      sum *= was;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) o[c].x *= was, o[c].y *= was, o[c].z *= was, o[c].w *= was;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (p0 + u > last || ml[u].x == -INFINITY) continue;
+        const float k = exp2_fast(ml[u].x - now);
+        sum = fmaf(ml[u].y, k, sum);
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          o[c].x = fmaf(v[u][c].x, k, o[c].x), o[c].y = fmaf(v[u][c].y, k, o[c].y), o[c].z = fmaf(v[u][c].z, k, o[c].z), o[c].w = fmaf(v[u][c].w, k, o[c].w);
+      }
     }
   }
-  for (int c4 = warp; c4 < D / 4; c4 += 8) {
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    sum = 0.f;
-    if (t < n) {
-      for (int p = first; p <= last; ++p) {
-        const int64_t piece = (static_cast<int64_t>(p) * W.blocks + block) * 2 + (p == first);
-        const float2 ml = W.ml[piece * W.rows + in_block];
-        if (ml.x == -INFINITY) continue;
-        const float k = exp2_fast(ml.x - top);
-        const float4 v = W.o[(piece * (D / 4) + c4) * W.rows + in_block];
-        sum = fmaf(ml.y, k, sum);
-        o.x = fmaf(v.x, k, o.x), o.y = fmaf(v.y, k, o.y), o.z = fmaf(v.z, k, o.z), o.w = fmaf(v.w, k, o.w);
-      }
-      const float f = odd ? NAN : (sum == 0.f ? 0.f : 1.0f / sum);
-      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-    }
-    *reinterpret_cast<uint2*>(out + c4 * 4) = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
+  if (nothing) return;
+  const float f = odd ? NAN : (sum == 0.f ? 0.f : 1.0f / sum);
+  T* out = static_cast<T*>(A.out) + ((static_cast<int64_t>(b) * A.nodes + t) * A.Hq + h) * D + c0 * 4;
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const uint2 y = live ? make_uint2(pack2<T>(o[c].x * f, o[c].y * f), pack2<T>(o[c].z * f, o[c].w * f)) : make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(out + c * 4) = y;
   }
 }
 
@@ -735,7 +762,11 @@ int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap&
   kern<<<W.workers * W.blocks, kNT, smem, stream>>>(A, W, k_map, v_map);
   if (int rc = check_launch(name)) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(A.B) * A.Hkv, (A.nodes * (A.Hq / A.Hkv) + 31) / 32);
+  // columns are divided while there are fewer CTAs than SMs
+  constexpr int kMost = D / 32;
+  const unsigned groups = static_cast<unsigned>(rows + 31) / 32;
+  const bool divided = static_cast<int64_t>(A.B) * A.Hkv * groups < kNumSMs;
+  cfg.gridDim = dim3(static_cast<unsigned>(A.B) * A.Hkv, groups, divided ? kMost : 1);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -743,7 +774,8 @@ int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap&
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D>, A, static_cast<const Shares>(W));
+  const cudaError_t e = divided ? cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D, 1>, A, static_cast<const Shares>(W))
+                                : cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D, kMost>, A, static_cast<const Shares>(W));
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
@@ -792,7 +824,7 @@ int b200_paged_tree_attn(void* out, const void* q, int64_t q_batch_stride, int64
   // rows of 16-byte pieces, pages and rows whose numbers fit
   const bool pieces = aligned16(q) && aligned16(out) && aligned16(k_pool) && aligned16(v_pool) && q_batch_stride % 8 == 0 && q_node_stride % 8 == 0;
   if (tiles_serve(Hq, Hkv, D, block_size, dtype) && !(flags & B200_ATTN_FORCE_GENERIC) && pieces && max_blocks < INT32_MAX / (static_cast<int64_t>(Hkv) * block_size) - 1 &&
-      static_cast<int64_t>(B) * Hkv <= INT32_MAX && nodes * static_cast<int64_t>(Hq / Hkv) <= 32 * 65535) {
+      (static_cast<int64_t>(table_cols) * block_size / kKeys + 1) * B < INT32_MAX / Hkv - 1024 && nodes * static_cast<int64_t>(Hq / Hkv) <= 32 * 65535) {
     if (!workspace || workspace_bytes < b200_paged_tree_attn_workspace(B, nodes, Hq, Hkv, D, block_size, dtype))
       return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace_bytes);
     if (!aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
