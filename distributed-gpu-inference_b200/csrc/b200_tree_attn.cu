@@ -37,11 +37,11 @@ __device__ __forceinline__ void lengths(const TreeAttn& A, int b, int* keys, int
 // (fp32, head sizes other than 64 and 128, pages that do not divide 64 keys).
 constexpr int kAnyWarps = 4, kAnyMostD = 256;
 
-template <typename T>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const TreeAttn A, bool vec) {
-  constexpr int kVec = 16 / sizeof(T), kCols = kAnyMostD / 32;
-  __shared__ __align__(16) float q_s[kAnyMostD];
-  __shared__ float out_s[kAnyWarps][kAnyMostD], m_s[kAnyWarps], l_s[kAnyWarps];
+  constexpr int kVec = 16 / sizeof(T), kAhead = 32 / COLS < 8 ? 32 / COLS : 8, kMostD = 32 * COLS;        // rows of values under way
+  __shared__ __align__(16) float q_s[kMostD];
+  __shared__ float out_s[kAnyWarps][kMostD], m_s[kAnyWarps], l_s[kAnyWarps];
   const int h = blockIdx.x, t = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int keys, n;
   lengths(A, b, &keys, &n);
@@ -51,11 +51,11 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const Tre
     return;
   }
   const T* q = static_cast<const T*>(A.q) + b * A.q_batch_stride + t * A.q_node_stride + static_cast<int64_t>(h) * A.D;
-  for (int d = threadIdx.x; d < kAnyMostD; d += blockDim.x) q_s[d] = d < A.D ? Cvt<T>::to_f32(q[d]) * A.scale : 0.f;
+  for (int d = threadIdx.x; d < kMostD; d += blockDim.x) q_s[d] = d < A.D ? Cvt<T>::to_f32(q[d]) * A.scale : 0.f;
   __syncthreads();
   const int base = keys - n, g = h / (A.Hq / A.Hkv);
   const uint64_t seen = static_cast<uint64_t>(A.visible[b * A.visible_stride + t]);
-  float m = -INFINITY, l = 0.f, acc[kCols] = {};
+  float m = -INFINITY, l = 0.f, acc[COLS] = {};
   for (int j0 = warp * 32; j0 < keys; j0 += kAnyWarps * 32) {
     const int j = j0 + lane;
     const bool live = j < keys && (j < base || (seen >> (j - base) & 1));
@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const Tre
     if (at >= 0) {
       const T* k = static_cast<const T*>(A.k_pool) + at;
       if (vec) {
+#pragma unroll 8
         for (int d = 0; d < A.D; d += kVec) {
           const int4 raw = *reinterpret_cast<const int4*>(k + d);
           const T* e = reinterpret_cast<const T*>(&raw);
@@ -84,19 +85,26 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const Tre
     m = top;
     l = fmaf(l, corr, warp_sum(w));
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] *= corr;
-    for (int i = 0; i < 32; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const int64_t vi = __shfl_sync(0xffffffffu, at, i);
-      if (wi == 0.f || vi < 0) continue;
-      const T* v = static_cast<const T*>(A.v_pool) + vi;
+    for (int c = 0; c < COLS; ++c) acc[c] *= corr;
+    for (int i = 0; i < 32; i += kAhead) {
+      float wi[kAhead], v[kAhead][COLS];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
-        if (c * 32 + lane < A.D) acc[c] = fmaf(wi, Cvt<T>::to_f32(v[c * 32 + lane]), acc[c]);
+      for (int u = 0; u < kAhead; ++u) {
+        wi[u] = __shfl_sync(0xffffffffu, w, i + u);
+        const int64_t vi = __shfl_sync(0xffffffffu, at, i + u);
+        const T* row = static_cast<const T*>(A.v_pool) + vi;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) v[u][c] = wi[u] != 0.f && vi >= 0 && c * 32 + lane < A.D ? Cvt<T>::to_f32(row[c * 32 + lane]) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[c] = fmaf(wi[u], v[u][c], acc[c]);
+      }
     }
   }
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) out_s[warp][c * 32 + lane] = acc[c];
+  for (int c = 0; c < COLS; ++c) out_s[warp][c * 32 + lane] = acc[c];
   if (lane == 0) m_s[warp] = m, l_s[warp] = l;
   __syncthreads();
   float top = -INFINITY, sum = 0.f, k[kAnyWarps];
@@ -153,6 +161,7 @@ struct Shares {
   float2* ml;               // [worker][row block][2][rows]: maximum (of scores in powers of two), sum
   float4* o;                // [worker][row block][2][D / 4][rows]
   int rows, blocks, workers;        // of a block that are kept (multiple of 32)
+  bool whole;               // a worker for each sequence and kv head: no pieces, and nothing behind this kernel
 };
 
 // Tiles of a sequence
@@ -323,7 +332,13 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm0 + P::kFlags), "n"(P::kTm) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  Walk w = walk_of(A, worker, W.workers);
+  Walk w;
+  if (W.whole) {
+    const int b = worker / A.Hkv, nt = tiles_of(A, b);
+    w = Walk{b, worker - b * A.Hkv, 0, nt, nt};
+  } else {
+    w = walk_of(A, worker, W.workers);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -445,6 +460,16 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
     const uint32_t tm_row = tm + (static_cast<uint32_t>(32 * warp) << 16);
     const float k2 = A.scale > 0.f ? A.scale * kLog2e : 1.f;       // weight = 2^(s k2 - m)
     const int per = W.rows;
+    if (W.whole) {        // rows without a node
+      int keys, n;
+      lengths(A, w.b, &keys, &n);
+      constexpr int kCh = D / 8;
+      for (int c = tid; c < kRows * kCh; c += soft_warps * 32) {
+        const int at = row0 + c / kCh, t = at / rep;
+        if (t >= n && t < A.nodes)
+          *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + ((static_cast<int64_t>(w.b) * A.nodes + t) * A.Hq + w.g * rep + at - t * rep) * D + c % kCh * 8) = make_uint4(0, 0, 0, 0);
+      }
+    }
     int i = 0;
     while (w.left > 0) {
       const int b = w.b, g = w.g, t0 = w.t, run = w.run();
@@ -756,11 +781,16 @@ int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap&
   W.ml = static_cast<float2*>(workspace);
   W.o = reinterpret_cast<float4*>(static_cast<char*>(workspace) + sums_bytes(W));
   const int rows = A.nodes * (A.Hq / A.Hkv);
+  // Walks of up to eight tiles are not divided: a second launch costs the host 5 us and the device 2, each tile here one.  (One sequence at 160 behind
+  // 8 kv heads of 128, a call after the other: undivided 16.9 us, divided 20.4.)
+  W.whole = static_cast<int64_t>(A.table_cols) * A.bs <= 8 * kKeys && static_cast<int64_t>(A.B) * A.Hkv * W.blocks <= INT32_MAX;
+  if (W.whole) W.workers = A.B * A.Hkv;
   auto kern = rows <= 32 ? tree_attn_kernel<T, D, 4> : rows <= 64 ? tree_attn_kernel<T, D, 2> : tree_attn_kernel<T, D, 1>;
   constexpr int smem = Plan<D>::kEnd + 1024;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   kern<<<W.workers * W.blocks, kNT, smem, stream>>>(A, W, k_map, v_map);
   if (int rc = check_launch(name)) return rc;
+  if (W.whole) return 0;
   cudaLaunchConfig_t cfg{};
   // columns are divided while there are fewer CTAs than SMs
   constexpr int kMost = D / 32;
@@ -788,7 +818,8 @@ int launch_any(const TreeAttn& A, cudaStream_t stream) {
   if (A.D > kAnyMostD) return fail(B200_ESHAPE, "b200_paged_tree_attn: head size %d, at most %d", A.D, kAnyMostD);
   if (A.B > 65535) return fail(B200_ESHAPE, "b200_paged_tree_attn: %d sequences", A.B);
   const bool vec = A.D * sizeof(T) % 16 == 0 && aligned16(A.k_pool);
-  tree_attn_any_kernel<T><<<dim3(A.Hq, A.nodes, A.B), kAnyWarps * 32, 0, stream>>>(A, vec);
+  auto kern = A.D <= 64 ? tree_attn_any_kernel<T, 2> : A.D <= 128 ? tree_attn_any_kernel<T, 4> : tree_attn_any_kernel<T, 8>;
+  kern<<<dim3(A.Hq, A.nodes, A.B), kAnyWarps * 32, 0, stream>>>(A, vec);
   return check_launch("b200_paged_tree_attn");
 }
 

@@ -238,3 +238,21 @@ def test_a_workspace_that_is_too_small_is_refused():
     c = build(4, 8, 32, 8, 128, 16, 200, torch.bfloat16)
     with pytest.raises(_lib.B200LibraryError, match="workspace"):
         check(c, workspace=torch.empty(need - 1, dtype=torch.uint8, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,nodes,Hq,Hkv,D,page,context", [(1, 8, 32, 8, 128, 16, 160), (40, 3, 8, 8, 64, 16, 300), (3, 64, 16, 2, 128, 16, 400),
+                                                           (5, 20, 12, 4, 64, 32, 100), (3, 33, 6, 2, 128, 64, 448)])
+def test_short_tables_and_the_same_behind_long_ones(B, nodes, Hq, Hkv, D, page, context, dtype):
+    """Tables of up to 512 keys are walked in one piece: the same formula, rows behind the last node 0, sequences without one."""
+    for tree in (True, False):
+        c = build(B, nodes, Hq, Hkv, D, page, context, dtype, seed=B + nodes, tree=tree)
+        out = torch.full_like(c["q"], 7.0)
+        check(c, out=out)
+        for b, n in enumerate(c["draft_lens"].tolist()):
+            assert bool((out[b, n:] == 0).all())
+        wide = torch.full((B, 600 // page + 9), -3, dtype=torch.int32, device=DEV)
+        wide[:, :c["block_tables"].shape[1]] = c["block_tables"]
+        check(dict(c, block_tables=wide))
+    c["draft_lens"].zero_()
+    assert bool((check(c) == 0).all()) and bool((check(dict(c, block_tables=wide)) == 0).all())
