@@ -15,22 +15,109 @@ blocks that somebody else filled: the receiving side of a prefill→decode hand-
 from the host tier).
 
 What it calls: only ``ModelShard.forward`` / ``get_logits`` (the reference surface) and, through the layers,
-the C-ABI kernels.  Greedy (argmax) sampling, which is what the parity contract is defined on.
+the C-ABI kernels.  Tokens are greedy (argmax), which is what the parity contract is defined on, unless ``sampling`` says
+otherwise (``drafting.Sampling`` per sequence: ``ops.sample_rows``).  ``verify_trees`` checks drafted tokens, a tree per sequence, in one
+pass; ``generate_drafted`` decodes that way.
 """
 from __future__ import annotations
 
-from typing import Any, Dict, List, Optional, Sequence
+from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
+from .drafting import PromptLookup, Sampling, pad_trees, settings
 from .paged_layer import PagedBatchState, PagedLayerKV, rope_tables
 from .worker.distributed.kv_cache import CacheBlock, KVCachePool, RadixPrefixIndex
 from .worker.distributed.model_shard import ModelShard
 from . import ops
 
 
+class _TreeStep:
+    """One pass over trees of ``nodes`` drafted tokens: static buffers and the captured graph."""
+
+    def __init__(self, engine: "PagedDecodeEngine", nodes: int):
+        self.e, self.nodes = engine, nodes
+        B, dev = engine.batch, engine.device
+        self.tokens = torch.zeros((B, nodes), dtype=torch.int64, device=dev)
+        self.parents = torch.full((B, nodes), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros((B,), dtype=torch.int32, device=dev)
+        need = ops.tree_attention_workspace(nodes, engine.Hq, engine.Hkv, engine.D, engine.block_size, engine.dtype)
+        self.workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        self.count = torch.zeros((B,), dtype=torch.int32, device=dev)
+        self.new = torch.zeros((B, nodes), dtype=torch.int64, device=dev)
+        self.graph: Optional[torch.cuda.CUDAGraph] = None
+
+    def body(self) -> None:
+        e, B, T, bs = self.e, self.e.batch, self.nodes, self.e.block_size
+        tables = e.block_tables[:B]
+        context = e.context_lens[:B]
+        node = torch.arange(T, device=e.device)
+        place = context[:, None] + node
+        slots = tables.gather(1, (place // bs).clamp(max=tables.shape[1] - 1)).to(torch.int64) * bs + place % bs
+        slots = torch.where(node < self.lens[:, None], slots, -1)       # no token: nothing is appended
+        visible, depth = ops.draft_tree(self.parents, self.lens)
+        pos = (context[:, None] + depth).to(torch.int64)
+        total = context + self.lens
+        st = PagedBatchState(block_tables=tables, context_lens=total, slot_mapping=slots.reshape(-1), max_context_len=e.max_seq_len,
+                             workspace=self.workspace, visible=visible, draft_lens=self.lens)
+        st.cos, st.sin = rope_tables(pos, e.inv_freq, e.dtype, e.rope_scaling)
+        h = self.tokens
+        for shard, handles in zip(e.shards, e._handles):
+            h, _ = shard.forward(h, position_ids=pos, past_key_values=[PagedLayerKV(hd.k_pool, hd.v_pool, st) for hd in handles], use_cache=True)
+        logits = e.shards[-1].get_logits(h)
+        chosen = e._choose(logits.reshape(B * T, -1), 0, pos + 1).view(B, T)
+        for i, (pool, handles) in enumerate(zip(e.pools, e._handles)):
+            k, v = e._pool_ptrs[i]
+            out = ops.accept_drafts(self.tokens, chosen, self.parents, visible, k, v, tuple(handles[0].k_pool.shape), e.dtype, tables, total,
+                                    draft_lens=self.lens)
+        self.count.copy_(out[0])
+        self.new.copy_(out[2])
+        context.copy_(out[3])
+
+    def run(self, tokens: torch.Tensor, parents: torch.Tensor, lens: List[int]) -> Tuple[List[int], List[List[int]]]:
+        e = self.e
+        self.tokens.copy_(tokens)
+        self.parents.copy_(parents)
+        self.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        for i, handles in enumerate(e._handles):
+            if e._pool_ptrs[i] is None:
+                e._pool_ptrs[i] = (ops.pool_pointer_array([h.k_pool for h in handles]), ops.pool_pointer_array([h.v_pool for h in handles]))
+        if not e.use_cuda_graph or e.logits_log is not None:
+            self.body()
+        else:
+            if self.graph is None:
+                self.graph = self._capture()
+            self.graph.replay()
+        count, new = self.count.tolist(), self.new.tolist()
+        for b, n in enumerate(count):
+            e._host_lens[b] += n
+        return count, new
+
+    def _capture(self) -> torch.cuda.CUDAGraph:
+        e = self.e
+        saved = e.context_lens.clone()
+        # The warm-up runs on single nodes, whose place the pass itself fills: a path that it moved would be gone for it
+        lens = self.lens.clone()
+        self.lens.clamp_(max=1)
+        side = torch.cuda.Stream(device=e.device)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # outside capture: cuBLAS handles, lazy module loads
+            for _ in range(2):
+                e.context_lens.copy_(saved)
+                self.body()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self.body()
+        e.context_lens.copy_(saved)
+        self.lens.copy_(lens)
+        return graph
+
+
 class PagedDecodeEngine:
-    """Greedy decoding of a fixed batch through a chain of shards that live on one CUDA device."""
+    """Decoding of a fixed batch through a chain of shards that live on one CUDA device."""
 
     def __init__(
         self,
@@ -146,6 +233,13 @@ class PagedDecodeEngine:
         self._pin_out = torch.zeros((max_batch,), dtype=torch.int64).pin_memory()
         self.batch = 0
         self._borrowed = False
+        # how tokens are chosen: None = greedy; settings and random numbers of each sequence (of the token at each position) on the device
+        self.sampling: Optional[List[Sampling]] = None
+        self._temperature, self._top_p, self._min_p = (torch.zeros((max_batch,), dtype=torch.float32, device=dev) for _ in range(3))
+        self._top_k = torch.zeros((max_batch,), dtype=torch.int32, device=dev)
+        self._numbers: Optional[torch.Tensor] = None
+        self._trees: Dict[int, "_TreeStep"] = {}    # by nodes
+        self._pool_ptrs = [None] * len(self.shards)
         # prefix cache across requests: one index per shard pool, holding its own reference on the cached blocks
         self.prefix_index: Optional[List[RadixPrefixIndex]] = (
             [RadixPrefixIndex(pool, hold=True) for pool in self.pools] if prefix_cache else None)
@@ -211,6 +305,7 @@ class PagedDecodeEngine:
         self.cached_blocks = n_cached
         self._graph = None
         self._graph_chained = None
+        self._trees = {}
         self._set_prefix(n_shared if batch > 1 else 0)
         self._shared_blocks = n_shared
 
@@ -293,6 +388,7 @@ class PagedDecodeEngine:
         if not same_shape:
             self._graph = None
             self._graph_chained = None
+            self._trees = {}
         self._set_prefix(0)
         self._shared_blocks, self.cached_blocks, self._prefix_tokens = 0, 0, None
 
@@ -331,8 +427,40 @@ class PagedDecodeEngine:
             logits = self.shards[-1].get_logits(h[:, -1:, :])[:, 0, :]
             if self.logits_log is not None:
                 self.logits_log.append((lo, hi, logits.float().clone()))
-            return ops.argmax_rows(logits)
+            return self._choose(logits, lo, torch.full((n,), past_len + P, dtype=torch.int64, device=self.device))
         return h
+
+    # ---- the next token --------------------------------------------------------------------------------
+    def set_sampling(self, sampling: Optional[Sequence[Sampling]]) -> None:
+        """How the sequences ``0 .. len(sampling) - 1`` choose their tokens from now on; None: greedily."""
+        rows = None if sampling is None else list(sampling)
+        if rows is not None and all(s.temperature == 0.0 for s in rows):
+            rows = None
+        if (rows is None) != (self.sampling is None):       # captured steps choose one way or the other
+            self._graph = self._graph_chained = None
+            self._trees = {}
+        self.sampling = rows
+        if rows is None:
+            return
+        if len(rows) > self.max_batch:
+            raise ValueError("more settings than the engine has sequences")
+        if not (self.is_first and self.is_last) or self.external_head:
+            raise RuntimeError("sampling needs an engine with the whole model")
+        if self._numbers is None:
+            self._numbers = torch.zeros((self.max_batch, self.max_seq_len + 1), dtype=torch.float32, device=self.device)
+        for buf, values in zip((self._temperature, self._top_k, self._top_p, self._min_p), settings(rows)):
+            buf[:len(rows)].copy_(torch.from_numpy(values))
+        self._numbers[:len(rows)].copy_(torch.from_numpy(np.stack([s.numbers(self.max_seq_len + 1) for s in rows])))
+
+    def _choose(self, logits: torch.Tensor, lo: int, pos: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The tokens at positions ``pos`` (int64) of the sequences from ``lo`` on, one or several rows of logits for each."""
+        if self.sampling is None:
+            return ops.argmax_rows(logits, out=out)  # one CTA per row; torch's reduce takes 46 us here
+        n = pos.shape[0]
+        each = logits.shape[0] // n
+        rows = [b[lo:lo + n] if each == 1 else b[lo:lo + n].repeat_interleave(each) for b in (self._temperature, self._top_k, self._top_p, self._min_p)]
+        u = self._numbers[lo:lo + n].gather(1, pos.reshape(n, each).clamp(max=self.max_seq_len)).reshape(-1)
+        return ops.sample_rows(logits, u, temperature=rows[0], top_k=rows[1], top_p=rows[2], min_p=rows[3], out=out)
 
     @torch.no_grad()
     def prefill(self, prompt_ids: torch.Tensor) -> torch.Tensor:
@@ -385,7 +513,7 @@ class PagedDecodeEngine:
             self.hn_out[:B].copy_(h[:, 0, :])
         elif self.is_last:
             logits = self.shards[-1].get_logits(h)[:, 0, :]
-            ops.argmax_rows(logits, out=self.next_tokens[:B])  # one CTA per row; torch's reduce takes 46 us here
+            self._choose(logits, 0, pos + 1, out=self.next_tokens[:B])
             if self.logits_log is not None:  # eager launches only: the margins behind every token
                 self.logits_log.append((0, B, logits.float().clone()))
         else:
@@ -476,12 +604,61 @@ class PagedDecodeEngine:
             self._host_lens[b] += 1
         return self._pin_out[:B].clone()
 
+    # ---- drafted tokens -------------------------------------------------------------------------------
     @torch.no_grad()
-    def generate(self, prompt_ids: torch.Tensor, max_new_tokens: int, shared_prefix_len: int = 0) -> torch.Tensor:
-        """Greedy generation: tokens [B, max_new_tokens] on the host.  ``shared_prefix_len``: leading tokens that are
+    def verify_trees(self, tokens: torch.Tensor, parents: torch.Tensor, draft_lens: Optional[torch.Tensor] = None) -> Tuple[List[int], List[List[int]]]:
+        """One pass over a tree of drafted tokens per sequence: ``(count, new tokens)`` of each, on the host.
+
+        ``tokens`` int64 and ``parents`` int32 ``[batch, nodes]`` (host or device): node 0 is the sequence's last token, which no step has
+        seen yet, the others come behind their parents; ``draft_lens`` int32 ``[batch]`` how many nodes a sequence has (0: it rests).  The
+        model runs once over all nodes; the nodes whose tokens are the model's own choices stay in the cache, side by side behind the context,
+        and a sequence gets ``count`` new tokens: one for each of them.  The choices are the ones that single steps would have made."""
+        if not (self.is_first and self.is_last) or self.external_head:
+            raise RuntimeError("verify_trees() drives a whole model")
+        B = self.batch
+        if tokens.shape != parents.shape or tokens.dim() != 2 or tokens.shape[0] != B:
+            raise ValueError("tokens and parents must be [batch, nodes]")
+        nodes = tokens.shape[1]
+        if not 1 <= nodes <= ops.MAX_DRAFT_NODES:
+            raise ValueError(f"1 to {ops.MAX_DRAFT_NODES} nodes per sequence")
+        lens = [nodes] * B if draft_lens is None else [int(n) for n in draft_lens]
+        if len(lens) != B or min(lens) < 0 or max(lens) > nodes:
+            raise ValueError("draft_lens must be [batch], 0 to nodes")
+        for b in range(B):
+            held = len(self._seq_blocks[b][0][0]) * self.block_size
+            if lens[b] and self._host_lens[b] + lens[b] > min(held, self.max_seq_len):
+                raise ValueError(f"Maximum length exceeded: {self._host_lens[b]} + {lens[b]} > {min(held, self.max_seq_len)}")
+        step = self._trees.get(nodes)
+        if step is None:
+            step = self._trees[nodes] = _TreeStep(self, nodes)
+        return step.run(tokens, parents, lens)
+
+    @torch.no_grad()
+    def generate_drafted(self, prompt_ids: torch.Tensor, max_new_tokens: int, drafter: Optional[Callable] = None,
+                         sampling: Optional[Sequence[Sampling]] = None, nodes: int = 8) -> torch.Tensor:
+        """``generate``'s tokens with several of them per pass: ``drafter(tokens of a sequence so far) -> (tokens, parents)`` proposes a tree
+        of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``), and ``verify_trees`` checks it."""
+        B, P = prompt_ids.shape
+        drafter = drafter or PromptLookup(nodes)
+        self.set_sampling(sampling)
+        self.allocate(B, P + max_new_tokens + nodes - 1)
+        told = [row + [tok] for row, tok in zip(prompt_ids.tolist(), self.prefill(prompt_ids).tolist())]
+        want = P + max_new_tokens
+        while any(len(t) < want for t in told):
+            tokens, parents, lens = pad_trees([drafter(t) if len(t) < want else None for t in told], nodes)
+            count, new = self.verify_trees(torch.from_numpy(tokens), torch.from_numpy(parents), torch.from_numpy(lens))
+            for b in range(B):
+                told[b].extend(new[b][:min(count[b], want - len(told[b]))])
+        return torch.tensor([t[P:] for t in told], dtype=torch.int64)
+
+    @torch.no_grad()
+    def generate(self, prompt_ids: torch.Tensor, max_new_tokens: int, shared_prefix_len: int = 0,
+                 sampling: Optional[Sequence[Sampling]] = None) -> torch.Tensor:
+        """Generation (greedy unless ``sampling`` has settings for every sequence): tokens [B, max_new_tokens] on the host.  ``shared_prefix_len``: leading tokens that are
         identical in every prompt and whose KV blocks should be shared (computed once, reference-counted); with
         ``prefix_cache=True`` they are also kept for later calls, which then skip recomputing them."""
         B, P = prompt_ids.shape
+        self.set_sampling(sampling)
         n_pre = min(shared_prefix_len, P - 1)
         self.allocate(B, P + max_new_tokens, shared_prefix_len=n_pre,
                       prefix_tokens=prompt_ids[0, :n_pre].tolist() if self.prefix_index is not None and n_pre else None)
@@ -494,8 +671,8 @@ class PagedDecodeEngine:
 
     @torch.no_grad()
     def generate_ragged(self, prompts: Sequence[Sequence[int]], max_new_tokens: int,
-                        shared_prefix_len: int = 0) -> List[List[int]]:
-        """Greedy generation for prompts of DIFFERENT lengths as one decode batch.
+                        shared_prefix_len: int = 0, sampling: Optional[Sequence[Sampling]] = None) -> List[List[int]]:
+        """Generation (greedy unless ``sampling`` has settings for every prompt) for prompts of DIFFERENT lengths as one decode batch.
 
         The prompt pass runs once per distinct length (sequences are ordered by length so that each length is a
         contiguous slice of the batch); the decode steps then run over all sequences together — context lengths,
@@ -512,6 +689,9 @@ class PagedDecodeEngine:
             return []
         if min(lens) < 1:
             raise ValueError("empty prompt")
+        if sampling is not None and len(sampling) != B:
+            raise ValueError("sampling needs settings for every prompt")
+        self.set_sampling(None if sampling is None else [sampling[i] for i in order])
         n_pre = max(0, min(shared_prefix_len, min(lens) - 1))
         head = list(prompts[order[0]][:n_pre])
         if n_pre and any(list(p[:n_pre]) != head for p in prompts):
@@ -555,8 +735,8 @@ class PagedDecodeEngine:
     def batch_inference(self, params_list: List[Dict[str, Any]]) -> List[Any]:
         """Engine hook the reference's batcher looks for: one result (or Exception) per request.
 
-        Each request carries ``input_ids`` (list[int]) and ``max_new_tokens``; prompts of different lengths are
-        decoded together as one batch (``generate_ragged``).
+        Each request carries ``input_ids`` (list[int]) and ``max_new_tokens``, and with ``do_sample`` its sampling parameters
+        (``drafting.Sampling.of_request``); prompts of different lengths are decoded together as one batch (``generate_ragged``).
         """
         results: List[Any] = [None] * len(params_list)
         good: List[int] = []
@@ -564,6 +744,7 @@ class PagedDecodeEngine:
             try:
                 if len(p["input_ids"]) < 1:
                     raise ValueError("empty input_ids")
+                Sampling.of_request(p)
                 good.append(i)
             except Exception as exc:  # noqa: BLE001 - per-item failure is part of the protocol
                 results[i] = exc
@@ -571,7 +752,8 @@ class PagedDecodeEngine:
             part = good[lo:lo + self.max_batch]
             try:
                 n_new = max(int(params_list[i].get("max_new_tokens", 16)) for i in part)
-                toks = self.generate_ragged([params_list[i]["input_ids"] for i in part], n_new)
+                toks = self.generate_ragged([params_list[i]["input_ids"] for i in part], n_new,
+                                            sampling=[Sampling.of_request(params_list[i]) for i in part])
                 for row, i in enumerate(part):
                     want = int(params_list[i].get("max_new_tokens", 16))
                     results[i] = {"output_ids": toks[row][:want],

@@ -158,6 +158,10 @@ class PagedBatchState:
     prefix_splits: int = 0
     suffix_splits: int = 0
     past_len: int = 0
+    # drafted tokens (T nodes of a tree per sequence): visible int64 [B, T] says which of them each node sees besides the context, draft_lens
+    # int32 [B] how many nodes a sequence has (None: T); context_lens counts them
+    visible: Optional[torch.Tensor] = None
+    draft_lens: Optional[torch.Tensor] = None
     # MLP output of the previous layer whose residual add was deferred (see PagedLlamaDecoderLayer.defer_residual)
     pending_residual: Optional[torch.Tensor] = None
 
@@ -509,7 +513,7 @@ class PagedLlamaDecoderLayer(nn.Module):
         B, T, _ = hidden_states.shape
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
 
-        if T == 1 and self._qkv_w is None and st.pending_residual is None and not self.defer_residual and st.prefix_blocks == 0:
+        if T == 1 and st.visible is None and self._qkv_w is None and st.pending_residual is None and not self.defer_residual and st.prefix_blocks == 0:
             h = self._one_call(hidden_states, position_ids, past_key_value, st)
             if h is not None:
                 return h, (past_key_value if use_cache else None)
@@ -540,7 +544,13 @@ class PagedLlamaDecoderLayer(nn.Module):
                 raise ValueError("position_ids (or precomputed RoPE tables in the batch state) are required")
             cos, sin = rope_tables(position_ids, self.inv_freq, x.dtype, self.rope_attention_scaling)
 
-        if T == 1:
+        if st.visible is not None:
+            # drafted tokens: RoPE by each node's own position, the append behind the context in the order of the nodes, attention of the trees
+            ops.rope_kv_append(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cos.reshape(B * T, D), sin.reshape(B * T, D),
+                               past_key_value.k_pool, past_key_value.v_pool, st.slot_mapping)
+            attn = ops.paged_tree_attention(q, past_key_value.k_pool, past_key_value.v_pool, st.block_tables, st.context_lens, st.visible,
+                                            draft_lens=st.draft_lens, workspace=st.workspace).view(B, T, Hq * D)
+        elif T == 1:
             # decode: RoPE on q (in place) and k, append of k / v, all in one launch; then paged attention
             qf = q[:, 0]  # [B, Hq, D], row stride = projection width
             cos2, sin2 = cos.reshape(B, D), sin.reshape(B, D)

@@ -25,6 +25,7 @@ import torch
 import torch.nn.functional as F
 
 from . import mixer_ops
+from .drafting import Sampling, settings
 from .paged_layer import RaggedBatchState, RaggedLayerCache
 from .worker.distributed.kv_cache import CacheBlock, KVCachePool, RecurrentStatePool
 from .worker.distributed.model_shard import ModelShard
@@ -292,8 +293,9 @@ class RaggedStepEngine:
     # ---- scheduler -----------------------------------------------------------------------------------------------
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, prefill_chunk: int = 512,
-                 token_budget: int = 4096, eos_token_id: Optional[int] = None) -> List[List[int]]:
-        """Greedy generation for any number of prompts with continuous batching: up to ``max_seqs`` requests are
+                 token_budget: int = 4096, eos_token_id: Optional[int] = None,
+                 sampling: Optional[Sequence[Sampling]] = None) -> List[List[int]]:
+        """Generation (greedy unless ``sampling`` has settings for every prompt) for any number of prompts with continuous batching: up to ``max_seqs`` requests are
         live; each step carries one token of every decoding request plus prompt chunks (``prefill_chunk`` tokens at
         most per request) while the step's ``token_budget`` lasts.  A request is admitted when a slot is free and the
         pages for its prompt and its new tokens are not promised to the live ones.  Returns the new tokens in the
@@ -304,6 +306,11 @@ class RaggedStepEngine:
         out: List[List[int]] = [[] for _ in prompts]
         if max_new_tokens <= 0:
             return out
+        if sampling is not None and len(sampling) != len(prompts):
+            raise ValueError("sampling needs settings for every prompt")
+        if sampling is not None and all(s.temperature == 0.0 for s in sampling):
+            sampling = None
+        numbers = None if sampling is None else [s.numbers(len(p) + max_new_tokens) for s, p in zip(sampling, prompts)]
         need_blocks = [(len(p) + max_new_tokens + bs - 1) // bs for p in prompts]
         for i, p in enumerate(prompts):
             if len(p) < 1:
@@ -342,7 +349,12 @@ class RaggedStepEngine:
             logits = self.step(entries)
             if logits is None:
                 continue
-            toks = ops.argmax_rows(logits).tolist()
+            if numbers is None:
+                toks = ops.argmax_rows(logits).tolist()
+            else:        # the number of a token's position, whatever else the step carries
+                u = np.array([numbers[i][len(prompts[i]) + len(out[i])] for i in owners], np.float32)
+                t, k, p, m, u = (torch.from_numpy(a).to(self.device) for a in (*settings([sampling[i] for i in owners]), u))
+                toks = ops.sample_rows(logits, u, temperature=t, top_k=k, top_p=p, min_p=m).tolist()
             for i, tok in zip(owners, toks):
                 out[i].append(tok)
                 live[i]["next"] = tok
@@ -354,20 +366,23 @@ class RaggedStepEngine:
 
     # ---- ContinuousBatcher protocol (reference: worker/batch_processor.py:302-336) ----------------------------------
     def batch_inference(self, params_list: List[Dict[str, Any]]) -> List[Any]:
-        """One result (or Exception) per request; each carries ``input_ids`` and ``max_new_tokens``."""
+        """One result (or Exception) per request; each carries ``input_ids`` and ``max_new_tokens``, and with ``do_sample`` its sampling
+        parameters (``drafting.Sampling.of_request``)."""
         results: List[Any] = [None] * len(params_list)
         good = []
         for i, p in enumerate(params_list):
             try:
                 if len(p["input_ids"]) < 1:
                     raise ValueError("empty input_ids")
+                Sampling.of_request(p)
                 good.append(i)
             except Exception as exc:  # noqa: BLE001 - per-item failure is part of the protocol
                 results[i] = exc
         if good:
             try:
                 n_new = max(int(params_list[i].get("max_new_tokens", 16)) for i in good)
-                rows = self.generate([params_list[i]["input_ids"] for i in good], n_new)
+                rows = self.generate([params_list[i]["input_ids"] for i in good], n_new,
+                                     sampling=[Sampling.of_request(params_list[i]) for i in good])
                 for row, i in zip(rows, good):
                     want = int(params_list[i].get("max_new_tokens", 16))
                     results[i] = {"output_ids": row[:want],

@@ -8,8 +8,8 @@ the method the reference's ``ContinuousBatcher`` prefers (worker/batch_processor
 implements.  Requests that start with the same system message are decoded as one batch with their common prefix
 blocks shared.
 
-Only greedy decoding is implemented (temperature / top_p / top_k are accepted and ignored): that is what the parity
-contract of this path is defined on.
+Decoding is greedy, which is what the parity contract of this path is defined on, and temperature / top_p / top_k alone change nothing;
+a request with ``do_sample`` draws its tokens by them (``drafting.Sampling.of_request``; ``min_p`` and ``seed`` too).
 """
 from __future__ import annotations
 
@@ -19,6 +19,7 @@ from typing import Any, Dict, List, Optional
 
 import torch
 
+from ...drafting import Sampling
 from ...engine import PagedDecodeEngine
 from ..distributed.model_shard import ModelShard
 
@@ -164,7 +165,7 @@ class PagedLLMEngine:
         for i, p in enumerate(params_list):
             try:
                 ids, n_sys = self._ids_of(p)
-                parsed[i] = (ids, n_sys, int(p.get("max_tokens", p.get("max_new_tokens", 16))))
+                parsed[i] = (ids, n_sys, int(p.get("max_tokens", p.get("max_new_tokens", 16))), Sampling.of_request(p))
                 groups.setdefault((len(ids), tuple(ids[:n_sys])), []).append(i)
             except Exception as exc:  # noqa: BLE001
                 results[i] = exc
@@ -184,7 +185,8 @@ class PagedLLMEngine:
                     if longest + n_new > eng.max_seq_len:
                         raise ValueError(f"prompt of {longest} tokens + {n_new} new tokens exceeds max_model_len")
                     share = len(sys_ids) if (len(part) > 1 or eng.prefix_index is not None) else 0
-                    rows = eng.generate_ragged([parsed[i][0] for i in part], n_new, shared_prefix_len=share)
+                    rows = eng.generate_ragged([parsed[i][0] for i in part], n_new, shared_prefix_len=share,
+                                               sampling=[parsed[i][3] for i in part])
                     # tokens whose KV was not computed for this request: the sequence that owns the shared blocks
                     # (the shortest prompt) only skips what an EARLIER call left in the prefix cache, the others also
                     # skip what that sequence has just computed
@@ -206,7 +208,8 @@ class PagedLLMEngine:
         for i, p in enumerate(params_list):
             try:
                 ids, _n_sys = self._ids_of(p)
-                rows.append({"input_ids": ids, "max_new_tokens": int(p.get("max_tokens", p.get("max_new_tokens", 16)))})
+                Sampling.of_request(p)
+                rows.append({**p, "input_ids": ids, "max_new_tokens": int(p.get("max_tokens", p.get("max_new_tokens", 16)))})
                 owners.append(i)
             except Exception as exc:  # noqa: BLE001
                 results[i] = exc

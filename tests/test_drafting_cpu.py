@@ -134,3 +134,37 @@ def test_no_cpu_form():
         ops.sample_rows(torch.zeros(1, 4), torch.zeros(1))
     with pytest.raises(_lib.B200LibraryError):
         ops.draft_tree(torch.zeros(1, 4, dtype=torch.int32))
+
+
+def test_sampling_settings():
+    from dgi_b200.drafting import GREEDY, Sampling, settings
+
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(min_p=-0.1), dict(min_p=2.0)):
+        with pytest.raises(ValueError):
+            Sampling(**bad)
+    assert Sampling.of_request({"temperature": 0.3}) == GREEDY
+    assert Sampling.of_request({"do_sample": True}) == Sampling(0.7, 50, 0.9, 0.0, 0)
+    assert Sampling.of_request({"do_sample": True, "temperature": 1, "top_k": 0, "top_p": 1, "min_p": 0.1, "seed": 4}) == Sampling(1.0, 0, 1.0, 0.1, 4)
+    t, k, p, m = settings([GREEDY, Sampling(0.5, 7, 0.9, 0.1)])
+    assert t.tolist() == [0.0, 0.5] and k.tolist() == [0, 7] and abs(p[1] - 0.9) < 1e-6 and abs(m[1] - 0.1) < 1e-6
+    a = Sampling(seed=3).numbers(100)
+    assert (a[:40] == Sampling(seed=3).numbers(40)).all() and (a >= 0).all() and (a < 1).all() and (a != Sampling(seed=4).numbers(100)).any()
+
+
+def test_prompt_lookup_and_padding():
+    from dgi_b200.drafting import PromptLookup, pad_trees
+
+    look = PromptLookup(nodes=6, longest=2, branches=2)
+    assert look([5]) == ([5], [-1]) and look([1, 2, 3]) == ([3], [-1])
+    # "1 2" was followed by 3 4 and, before, by 3 9: one branch to 3, then two of two tokens
+    assert look([1, 2, 3, 9, 1, 2, 3, 4, 1, 2]) == ([2, 3, 4, 1, 9, 1], [-1, 0, 1, 2, 1, 4])
+    tokens, parents = look(list(range(20)) * 3)
+    assert len(tokens) <= 6 and tokens[0] == 19 and all(0 <= p < t for t, p in enumerate(parents) if t)
+    for bad in (dict(nodes=0), dict(nodes=65), dict(longest=0), dict(branches=0)):
+        with pytest.raises(ValueError):
+            PromptLookup(**bad)
+    t, p, n = pad_trees([([4, 5], [-1, 0]), None], 3)
+    assert t.tolist() == [[4, 5, 0], [0, 0, 0]] and p.tolist() == [[-1, 0, -1], [-1, -1, -1]] and n.tolist() == [2, 0]
+    for bad in (([1, 2], [-1, 1]), ([1, 2], [-1]), ([], []), ([1] * 4, [-1, 0, 0, 0])):
+        with pytest.raises(ValueError):
+            pad_trees([bad], 3)
