@@ -371,10 +371,13 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
           pages = later;
           later = look_up(t0 + x + ahead);
         }
-        if (i >= NB) bar_wait(bar_free + 8 * (i % NB), (i / NB - 1) & 1, dead);
+        auto free_again = [&] {
+          if (i >= NB) bar_wait(bar_free + 8 * (i % NB), (i / NB - 1) & 1, dead);
+        };
         const uint32_t base = bufs + (i % NB) * (D / 64) * kBlk, bar = bar_in + 8 * (i % NB);
         const int j0 = (t0 + x) * kKeys;
         if (!values || j0 + kKeys <= keys - n) {
+          free_again();
           const int page = __shfl_sync(0xffffffffu, pages, in * n_pages + (my_page < n_pages ? my_page : 0));
           if (my_page < n_pages && page >= 0) {
             asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((D / 64) * box * 128) : "memory");
@@ -385,7 +388,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
                            "l"(map), "r"(64 * c), "r"(row), "r"(bar) : "memory");
           }
         } else {
-          // all loads before the first store
+          // all loads before the buffer is free and the first store
           bool odd = false;
           constexpr int kCh = D / 8, kPer = kKeys * kCh / kLoadV;
           int4 v[kPer];
@@ -397,6 +400,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
             if (j0 + key < keys && page < A.max_blocks)
               v[u] = *reinterpret_cast<const int4*>(static_cast<const T*>(A.v_pool) + ((static_cast<int64_t>(page) * A.Hkv + g) * A.bs + (j0 + key) % A.bs) * D + ch * 8);
           }
+          free_again();
 #pragma unroll
           for (int u = 0; u < kPer; ++u) {
             const int c = me + u * kLoadV, key = c / kCh, ch = c - key * kCh;
