@@ -297,6 +297,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       return from_memory(block);
     }
   };
+  // a warp's blocks, one after another; what comes from memory is asked for a block ahead
+  auto each_block = [&](auto&& f) {
+    if constexpr (HELD) {
+      for (int b = warp; b < n_blocks; b += kWarps) f(b, load(b));
+    } else {
+      if (warp >= n_blocks) return;
+      Eight<T> next = load(warp);
+      for (int b = warp; b < n_blocks; b += kWarps) {
+        const Eight<T> v = next;
+        if (b + kWarps < n_blocks) next = load(b + kWarps);
+        f(b, v);
+      }
+    }
+  };
   auto index_of = [&](int block, int e) { return (block0 + block) * kBlock + lane * 8 + e - head; };
   // an element's place in the order: its key over its index, upside down
   const uint32_t index_mask = (1u << A.index_bits) - 1;
@@ -363,15 +377,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   top = __uint_as_float(best == 0xffffffffu ? 0x7fffffffu : Key<float>::bits(best));
   if (!(t > 0.f) || !(fabsf(top) < INFINITY)) {      // no temperature, or a largest logit that is no number: the first of the largest
     uint32_t first = 0xffffffffu;
-    for (int b = warp; b < n_blocks; b += kWarps) {
-      const Eight<T> v = load(b);
+    each_block([&](int b, const Eight<T>& v) {
 #pragma unroll
       for (int e = 7; e >= 0; --e) {
         const float f = value<T>(v[e]);
         const int index = index_of(b, e);
         if ((f == top || (f != f && top != top)) && index >= 0 && index < A.cols) first = min(first, static_cast<uint32_t>(index));
       }
-    }
+    });
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0 && first != 0xffffffffu) atomicMin(cluster.map_shared_rank(&S.first, 0), first);
     cluster.sync();
@@ -403,8 +416,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     // ---- elements in each range of log w --------------------------------------------------------------------------------------------------------
     for (int i = tid; i < kRanges * kRangeColumns / 4; i += kThreads) reinterpret_cast<uint4*>(S.ranges)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int b = warp; b < n_blocks; b += kWarps) {
-      const Eight<T> v = load(b);
+    each_block([&](int, const Eight<T>& v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = weigh.argument(value<T>(v[e]));
@@ -413,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           atomicAdd(&S.ranges[(at >> weigh.log_steps) * kRangeColumns + (lane & (kRangeColumns - 1))], 0x10000u | (at & ((1 << weigh.log_steps) - 1)));
         }
       }
-    }
+    });
     __syncthreads();
     constexpr int kMine = kRanges / kThreads;
 #pragma unroll
@@ -487,8 +499,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       u64 all = 0, above = 0;
       const int first_step = from << weigh.log_steps, steps = (to + 1 - from) << weigh.log_steps;
       auto gather = [&](auto sums, auto limited) {
-        for (int b = warp; b < n_blocks; b += kWarps) {
-          const Eight<T> v = load(b);
+        each_block([&](int b, const Eight<T>& v) {
           u64 sum = 0;
           unsigned hits = 0;
 #pragma unroll
@@ -516,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
             sum = warp_sum_of(sum);
             if (lane == 0) block_mass[b] = sum;
           }
-        }
+        });
       };
       if (k) gather(std::false_type{}, std::false_type{});
       else if (least_weight) gather(std::true_type{}, std::true_type{});
@@ -739,8 +750,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           if (WEIGHTED) S.lo[i] = S.hi[i] = 0;
         }
         __syncthreads();
-        for (int b = warp; b < n_blocks; b += kWarps) {
-          const Eight<T> v = load(b);
+        each_block([&](int, const Eight<T>& v) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint32_t key = Key<T>::of(v[e]);
@@ -756,7 +766,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
               }
             }
           }
-        }
+        });
         __syncthreads();
         if (tid < kDigits) {
           uint32_t n = 0;
@@ -861,14 +871,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   // ---- kept weights of each block ----------------------------------------------------------------------------------------------------------------
   if (!summed) {
     auto sum_blocks = [&](auto&& weight_of) {
-      for (int b = warp; b < n_blocks; b += kWarps) {
-        const Eight<T> v = load(b);
+      each_block([&](int b, const Eight<T>& v) {
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += weight_of(v[e], index_of(b, e));
         sum = warp_sum_of(sum);
         if (lane == 0) block_mass[b] = sum;
-      }
+      });
     };
     if (cut || least_weight) sum_blocks(kept_weight);
     else sum_blocks([&](uint32_t bits, int) { return weigh(value<T>(bits)); });
@@ -936,12 +945,13 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
     const size_t per = (blocks + ctas - 1) / ctas;
     return sizeof(Shared) + ((per + 1) & ~size_t{1}) * 8 + (held ? per * kBlock * sizeof(T) : 0);
   };
-  // two CTAs per SM where eight of a cluster can hold a row that way
+  // Two CTAs per SM.  As many for a row as the rows leave room for in one round, each with a part worth a cluster's barriers (1500 clocks each); the parts
+  // stay in shared memory if they fit, else they are read again, from the second level of the cache for the most part.  (Rows cut until they fit, in seven
+  // rounds: 256 rows of 128 k in 32 bits 288 us, against %s.)
   constexpr size_t kHalf = 113 * 1024;
   int ctas = 1;
-  while (ctas < 8 && bytes(ctas, true) > kHalf) ctas *= 2;
-  const bool held = bytes(ctas, true) <= kMaxSmem;
-  while (ctas < 8 && 2 * ctas * static_cast<int64_t>(rows) <= kNumSMs && blocks >= 8 * ctas) ctas *= 2;
+  while (ctas < kMostCtas && 2 * ctas * static_cast<int64_t>(rows) <= (blocks >= 128 * ctas ? 2 : 1) * kNumSMs && blocks >= 16 * ctas) ctas *= 2;
+  const bool held = bytes(ctas, true) <= kHalf;
   const size_t smem = bytes(ctas, held);
   if (smem > kMaxSmem) return fail(B200_ESHAPE, "%s: rows of %d", name, A.cols);
   A.blocks_per_cta = (blocks + ctas - 1) / ctas;
