@@ -6,10 +6,11 @@
 //           a beginning of the order, down to some (key, index)
 //   token = the first index, in the row's own order, up to which the kept weights sum to more than u of them all
 //
-// Whether a token is the one decides on sums of up to a million weights.  They are summed as whole numbers of 2^-frac (frac = 62 - log2 of the row's
-// length, at most 44), so no sum depends on its order: neither on how a row is spread over CTAs, nor on warps or atomics.  A weight is computed in
-// pairs of floats to 2^-31 of itself (256 steps of a power of two from a table, a polynomial of degree 3 between them, after Tang's table-driven
-// exponential): errors of independent weights leave one token in 10^7 rows of 128 k another one than 64 bits would.
+// Whether a token is the one decides on sums of up to a million weights.  They are summed as multiples of 2^-frac (frac = 62 - log2 of the row's
+// length, at most 44) - in doubles while 53 bits hold every sum, a thread's, then as whole numbers -, so no sum depends on its order: neither on how a
+// row is spread over CTAs, nor on warps or atomics.  A weight is computed to 2^-31 of itself (the argument in a pair of floats, 256 steps of a power of two from a
+// table, a polynomial of degree 3 between them, after Tang's table-driven exponential; set to its exponent and rounded by the double unit, which has
+// nothing else to do): errors of independent weights leave one token in 10^7 rows of 128 k another one than 64 bits would.
 //
 // A row has a cluster of CTAs; each holds its part of the row in shared memory from the only pass over it in memory, if the parts fit.  Blocks of 256
 // elements, eight side by side per lane.
@@ -36,7 +37,9 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBlock = 256;         // elements
 constexpr int kRanges = 1024, kRangeColumns = 8;        // columns: lanes that fall in the same range meet at fewer addresses
-constexpr float kRangeSteps = 11.5f;      // of 1/256 in log2
+constexpr float kRange = 11.5f;           // of 1/256 in log2
+constexpr int kStepBits = 3, kCountShift = 17, kMostBlocks = 580;       // eight steps a range; elements and steps of a CTA's column share 32 bits
+static_assert(32 * kMostBlocks * ((1 << kStepBits) - 1) < 1 << kCountShift && 32 * kMostBlocks < 1 << (32 - kCountShift), "blocks of a CTA");
 constexpr int kDigits = 256, kColumns = 8;
 constexpr int kList = 4096, kMostK = 2048;
 using u64 = unsigned long long;
@@ -119,7 +122,7 @@ constexpr Steps make_steps() {
     double x = 1073741824.0;
     for (int b = 0; b < 8; ++b)
       if (j >> b & 1) x *= roots[b];
-    t.whole[j] = static_cast<uint32_t>(x + 0.5);
+    t.whole[j] = static_cast<uint32_t>(x + 0.5) - 0x4b400000u;        // (less the bits of 3 * 2^22, which come with what is added)
     t.number[j] = static_cast<float>(x);
   }
   return t;
@@ -129,7 +132,7 @@ __device__ constexpr Steps kSteps = make_steps();
 constexpr int kMostCtas = 8;      // of a cluster
 
 struct alignas(16) Shared {
-  uint2 table[256];             // 2^(30 + j / 256): as a whole number, as a float
+  uint2 table[256];             // Steps
   union {
     uint32_t ranges[kRanges * kRangeColumns];
     u64 range_sum[kRanges];             // the cluster's range_count
@@ -163,36 +166,36 @@ struct alignas(16) Shared {
 constexpr int kBins = kThreads, kFew = 256;       // of Shared::range_count, where the list is searched
 static_assert(kBins + 2 * kFew <= kRanges, "room for bins and a bin's elements");
 
-// weights, as whole numbers of 2^-frac
+// weights: multiples of 2^-frac
 template <typename T>
 struct Weigh {
-  float top, scale, scale_low, lowest;  // maximum; 256 log2(e) / t in two parts; arguments from this on down give 0
-  int up;                               // frac - 30
+  float top, scale, scale_low;          // maximum; 256 log2(e) / t in two parts
+  float lowest, floor;                  // arguments from `lowest` on down give 0, those below `floor` count as it
+  double one;                           // 2^(52 - frac), whose last bit is 2^-frac
   const uint2* table;
   __device__ __forceinline__ float argument(float x) const { return __fmul_rn(x - top, scale); }
   __device__ __forceinline__ bool some(float y) const { return y > lowest; }        // not of no number: -inf without a scale
-  __device__ __forceinline__ u64 operator()(float x) const {
+  __device__ __forceinline__ double operator()(float x) const {
     const float d = x - top, y = __fmul_rn(d, scale);
-    if (!some(y)) return 0;
     float low = fmaf(d, scale_low, fmaf(d, scale, -y));
     if constexpr (sizeof(T) == 4) {     // what the difference lost (Knuth's sum); one of 16-bit numbers that matters loses nothing
       const float v = d - x;
       low = fmaf((x - (d - v)) - (top + v), scale, low);
     }
-    const float shift = 12582912.f, r = y + shift;        // 3 * 2^22: the nearest whole number is in the last bits
-    const int n = __float_as_int(r) - 0x4b400000;
-    const float f = (y - (r - shift)) + low;
+    const float shift = 12582912.f, z = fmaxf(y, floor), r = z + shift;        // 3 * 2^22: the nearest whole number n is in the last bits
+    const uint32_t n = __float_as_uint(r);
+    const float f = (z - (r - shift)) + low;        // (below the floor no number or any: 2^-50 of 32 bits is 0 all the same)
     constexpr float c1 = 0.69314718055994530942 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
     const uint2 step = table[n & 255];
     const float q = f * fmaf(fmaf(f, c3, c2), f, c1);
-    const uint32_t w = step.x + (__float_as_int(fmaf(q, __uint_as_float(step.y), shift)) - 0x4b400000);
-    return (static_cast<u64>(w) << up) >> -(n >> 8);
+    const uint32_t w = step.x + __float_as_uint(fmaf(q, __uint_as_float(step.y), shift));       // 2^30 times what is left of the exponent
+    const double exponent = __hiloint2double((n & ~255u) * 4096u + ((1023u - 30u << 20) - (0x4b400000u << 12)), 0);
+    return fma(__hiloint2double(0x43300000, w) - 4503599627370496.0, exponent, one) - one;
   }
-  // steps of an argument, 1 << log_steps a range
-  float per_step;
-  int log_steps;
-  __device__ __forceinline__ int steps(float y) const { return __float_as_int(fmaf(y, per_step, 8388608.f)) & 0x7fffff; }
-  __device__ __forceinline__ int range(float y) const { return steps(y) >> log_steps; }
+  __device__ __forceinline__ u64 whole(double w) const { return __double_as_longlong(w + one) - __double_as_longlong(one); }      // w < one
+  __device__ __forceinline__ u64 number(float x) const { return whole((*this)(x)); }
+  // place of an argument, in steps
+  __device__ __forceinline__ float steps(float y) const { return fmaf(y, -(1 << kStepBits) / kRange, 8388608.f); }
 };
 
 template <typename V>
@@ -393,8 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   }
   if (k <= 0 || k >= A.cols) k = 0;
   const bool by_mass = p < 1.0f;
-  // not a number: no limit
-  const u64 least_weight = least > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(least, 1.0f)) * static_cast<double>(1ull << A.frac))) : 0ull;
+  // (min_p no number: no limit)
   Weigh<T> weigh;
   {
     const double scale = 369.32993046757463 / static_cast<double>(t);     // 256 log2(e)
@@ -402,12 +404,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     weigh.scale = static_cast<float>(fmin(scale, 3e38));
     weigh.scale_low = scale < 3e38 ? static_cast<float>(scale - weigh.scale) : 0.f;
     weigh.lowest = -256.0f * (A.frac + 1);
-    weigh.up = A.frac - 30;
+    weigh.floor = -256.0f * (A.frac + 8);
+    weigh.one = __hiloint2double((1023 + 52 - A.frac) << 20, 0);
     weigh.table = S.table;
-    // elements and their steps, added up as two halves of a number: 32 elements a block and column, so 65536 is not reached
-    weigh.log_steps = A.blocks_per_cta <= 136 ? 4 : 2;
-    weigh.per_step = static_cast<float>(1 << weigh.log_steps) / -kRangeSteps;
   }
+  const double least_weight = least > 0.f ? ceil(static_cast<double>(fminf(least, 1.0f)) * static_cast<double>(1ull << A.frac)) / static_cast<double>(1ull << A.frac) : 0.0;
+
+  const u64 least_number = weigh.whole(least_weight);
+  // a block's sum from the lanes' (of eight weights, 24 bits at a time)
+  auto set_block = [&](int b, double mine) {
+    const u64 m = weigh.whole(mine);
+    const uint32_t low = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(m) & 0xffffffu), high = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(m >> 24));
+    if (lane == 0) block_mass[b] = (static_cast<u64>(high) << 24) + low;
+  };
 
   u64 cut = 0;            // kept: (key, ~index) from this on
   bool summed = false;    // the blocks' sums are there already
@@ -421,8 +430,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       for (int e = 0; e < 8; ++e) {
         const float y = weigh.argument(value<T>(v[e]));
         if (weigh.some(y)) {
-          const int at = weigh.steps(y);
-          atomicAdd(&S.ranges[(at >> weigh.log_steps) * kRangeColumns + (lane & (kRangeColumns - 1))], 0x10000u | (at & ((1 << weigh.log_steps) - 1)));
+          const uint32_t at = __float_as_uint(weigh.steps(y)) & 0x7fffffu;
+          atomicAdd(&S.ranges[(at >> kStepBits) * kRangeColumns + (lane & (kRangeColumns - 1))], 1u << kCountShift | (at & ((1 << kStepBits) - 1)));
         }
       }
     });
@@ -434,8 +443,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
 #pragma unroll
       for (int j = 0; j < kRangeColumns; ++j) {
         const uint32_t q = S.ranges[(tid * kMine + i) * kRangeColumns + (j + tid) % kRangeColumns];
-        c += q >> 16;
-        steps += q & 0xffffu;
+        c += q >> kCountShift;
+        steps += q & ((1u << kCountShift) - 1);
       }
       S.range_count[tid * kMine + i] = static_cast<u64>(c) << 32 | steps;
     }
@@ -457,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     for (int i = 0; i < kMine; ++i) {
       const u64 both = S.range_sum[tid * kMine + i];
       c[i] = static_cast<uint32_t>(both >> 32);
-      const float of = static_cast<float>(c[i]), into = static_cast<float>(static_cast<uint32_t>(both)) / (1 << weigh.log_steps) - 0.5f * of;
-      m[i] = static_cast<u64>(exp2f(40.f - (tid * kMine + i + 0.5f) * (kRangeSteps / 256.f)) * fmaf(into, -0.69314718f * kRangeSteps / 256.f, of));
+      const float of = static_cast<float>(c[i]), into = static_cast<float>(static_cast<uint32_t>(both)) / (1 << kStepBits) - 0.5f * of;
+      m[i] = static_cast<u64>(exp2f(40.f - (tid * kMine + i + 0.5f) * (kRange / 256.f)) * fmaf(into, -0.69314718f * kRange / 256.f, of));
       n_mine += c[i];
       m_mine += m[i];
     }
@@ -496,27 +505,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     const int from = S.from, to = S.to;
     if (listing <= kList) {       // (the same in all CTAs)
       // ---- the list; a row without k: exact sums of all, of what is above the list, and of the blocks' part of that ------------------------------
-      u64 all = 0, above = 0;
-      const int first_step = from << weigh.log_steps, steps = (to + 1 - from) << weigh.log_steps;
+      double all = 0, above = 0;
+      const float from_step = 8388608.f + (from << kStepBits), to_step = 8388608.f + ((to + 1) << kStepBits);
       auto gather = [&](auto sums, auto limited) {
         each_block([&](int b, const Eight<T>& v) {
-          u64 sum = 0;
+          double sum = 0;
           unsigned hits = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float f = value<T>(v[e]), y = weigh.argument(f);
-            const int step = weigh.some(y) ? weigh.steps(y) - first_step : 1 << 24;
-            if (static_cast<unsigned>(step) < static_cast<unsigned>(steps)) hits |= 1u << e;
+            const float f = value<T>(v[e]), y = weigh.argument(f), step = weigh.steps(y);
+            if (step >= from_step && step < to_step && weigh.some(y)) hits |= 1u << e;
             if constexpr (decltype(sums)::value) {
-              const u64 w = weigh(f);
+              const double w = weigh(f);
               all += w;
-              if (step < 0) {
+              if (step < from_step) {
                 if (decltype(limited)::value) above += w;
                 if (!decltype(limited)::value || w >= least_weight) sum += w;
               }
             }
           }
-          if (hits) {
+          if (hits) {       // (a place for the whole warp's at once costs more instructions than it saves atomics: 182 us against 168 for 256 rows of 128 k)
             uint32_t at = atomicAdd(&S.listed, static_cast<uint32_t>(__popc(hits)));
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -524,20 +532,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           }
           if (decltype(sums)::value && from > 0) {
             if (!decltype(limited)::value) above += sum;
-            sum = warp_sum_of(sum);
-            if (lane == 0) block_mass[b] = sum;
+            set_block(b, sum);
           }
         });
       };
       if (k) gather(std::false_type{}, std::false_type{});
-      else if (least_weight) gather(std::true_type{}, std::true_type{});
+      else if (least_weight > 0) gather(std::true_type{}, std::true_type{});
       else gather(std::true_type{}, std::false_type{});
       if (!k) {
-        all = warp_sum_of(all);
-        above = warp_sum_of(above);
+        const double per_unit = static_cast<double>(1ull << A.frac);
+        const u64 all_mine = warp_sum_of(static_cast<u64>(__double2ll_rn(all * per_unit))), above_mine = warp_sum_of(static_cast<u64>(__double2ll_rn(above * per_unit)));
         if (lane == 0) {
-          atomicAdd(&S.sum_all, all);
-          atomicAdd(&S.sum_above, above);
+          atomicAdd(&S.sum_all, all_mine);
+          atomicAdd(&S.sum_above, above_mine);
         }
       }
       cluster.sync();
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           int parts = kThreads;
           while (parts > 32 || (kThreads / parts) < n) parts /= 2;
           const int i = tid / parts, part = tid & (parts - 1);
-          const u64 c = i < n ? S.list[i] : 0, w = i < n ? weigh(logit_of(c)) : 0;
+          const u64 c = i < n ? S.list[i] : 0, w = i < n ? weigh.number(logit_of(c)) : 0;
           if (part == 0 && i < n) weights[i] = w;
           u64 whole = k ? 0 : sum_of_all(&S.sum_all);
           __syncthreads();
@@ -599,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
             if (!k && sum < limit && tid == 0) S.failed = 1;       // p of all is reached below the list
             keep = keep && heavier < limit;
           }
-          keep = keep && w >= least_weight;
+          keep = keep && w >= least_number;
           __syncthreads();
           if (part == 0 && i < n) weights[i] = keep ? w : 0;
           cta_before(keep && part == 0 ? w : 0ull, S.part, &sum);
@@ -679,10 +686,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
             __syncthreads();
           }
         };
-        auto weight_of = [&](u64 c) { return weigh(logit_of(c)); };
+        auto weight_of = [&](u64 c) { return weigh.number(logit_of(c)); };
         auto kept_of = [&](u64 c) -> u64 {
-          const u64 w = weigh(logit_of(c));
-          return w >= least_weight ? w : 0;
+          const u64 w = weigh.number(logit_of(c));
+          return w >= least_number ? w : 0;
         };
         auto sum_from = [&](u64 lowest, auto&& value_of) {
           u64 mine = 0, sum;
@@ -758,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
             const int slot = ((key >> shift) & 255) * kColumns + (lane & (kColumns - 1));
             atomicAdd(&S.cnt[slot], 1u);
             if constexpr (WEIGHTED) {
-              const u64 w = weigh(value<T>(v[e]));
+              const u64 w = weigh.number(value<T>(v[e]));
               if (w) {
                 const uint32_t old = atomicAdd(&S.lo[slot], static_cast<uint32_t>(w));
                 const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + static_cast<uint32_t>(w) < old ? 1u : 0u);
@@ -819,9 +826,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     u64 equals = 0, there = 0, rest = 0, in = 0;      // kept: keys above `last` and the first `equals` of it
     if (k) last = select(std::false_type{}, 0u, static_cast<u64>(k), 0ull, &equals, &there);
     if (by_mass) {
-      const u64 each = k ? weigh(value<T>(Key<T>::bits(last))) : 0ull;
+      const u64 each = k ? weigh.number(value<T>(Key<T>::bits(last))) : 0ull;
       last = select(std::true_type{}, last, 0ull, (there - equals) * each, &rest, &in);
-      const u64 w = weigh(value<T>(Key<T>::bits(last)));
+      const u64 w = weigh.number(value<T>(Key<T>::bits(last)));
       equals = (rest + w - 1) / w;
     }
     // where the last of them is
@@ -862,24 +869,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   }
 
   const uint32_t cut_key = key_in(cut), cut_index = index_in(cut);
-  auto kept_weight = [&](uint32_t bits, int index) -> u64 {
+  auto kept_weight = [&](uint32_t bits, int index) -> double {
     const uint32_t key = Key<T>::of(bits);
-    if (key < cut_key || (key == cut_key && static_cast<uint32_t>(index) > cut_index)) return 0;
-    const u64 w = weigh(value<T>(bits));
-    return w >= least_weight ? w : 0;
+    if (key < cut_key || (key == cut_key && static_cast<uint32_t>(index) > cut_index)) return 0.0;
+    const double w = weigh(value<T>(bits));
+    return w >= least_weight ? w : 0.0;
   };
   // ---- kept weights of each block ----------------------------------------------------------------------------------------------------------------
   if (!summed) {
     auto sum_blocks = [&](auto&& weight_of) {
       each_block([&](int b, const Eight<T>& v) {
-        u64 sum = 0;
+        double sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += weight_of(v[e], index_of(b, e));
-        sum = warp_sum_of(sum);
-        if (lane == 0) block_mass[b] = sum;
+        set_block(b, sum);
       });
     };
-    if (cut || least_weight) sum_blocks(kept_weight);
+    if (cut || least_weight > 0) sum_blocks(kept_weight);
     else sum_blocks([&](uint32_t bits, int) { return weigh(value<T>(bits)); });
     __syncthreads();
   }
@@ -919,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     u64 w[8], sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[e] = kept_weight(v[e], index_of(b, e));
+      w[e] = weigh.whole(kept_weight(v[e], index_of(b, e)));
       sum += w[e];
     }
     u64 run = warp_before(sum);
@@ -950,7 +956,7 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
   // rounds: 256 rows of 128 k in 32 bits 288 us, against %s.)
   constexpr size_t kHalf = 113 * 1024;
   int ctas = 1;
-  while (ctas < kMostCtas && 2 * ctas * static_cast<int64_t>(rows) <= (blocks >= 128 * ctas ? 2 : 1) * kNumSMs && blocks >= 16 * ctas) ctas *= 2;
+  while (ctas < kMostCtas && (blocks > kMostBlocks * ctas || (2 * ctas * static_cast<int64_t>(rows) <= (blocks >= 128 * ctas ? 2 : 1) * kNumSMs && blocks >= 16 * ctas))) ctas *= 2;
   const bool held = bytes(ctas, true) <= kHalf;
   const size_t smem = bytes(ctas, held);
   if (smem > kMaxSmem) return fail(B200_ESHAPE, "%s: rows of %d", name, A.cols);
