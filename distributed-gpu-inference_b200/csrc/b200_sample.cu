@@ -300,6 +300,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
       return from_memory(block);
     }
   };
+  auto bits_at = [&](int block, int e) -> uint32_t {
+    using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, unsigned short>;
+    if constexpr (HELD) return reinterpret_cast<const Bits*>(held)[(block * 32 + lane) * 8 + e];
+    else return __ldg(reinterpret_cast<const Bits*>(x0) + (block0 + block) * kBlock + lane * 8 + e);
+  };
   // a warp's blocks, one after another; what comes from memory is asked for a block ahead
   auto each_block = [&](auto&& f) {
     if constexpr (HELD) {
@@ -496,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
         before += m[i];
       }
       __syncthreads();
-      const bool all_of_it = S.at[1] <= kList;        // nothing above the list
+      const bool all_of_it = S.at[1] <= kFew;        // nothing above the list: it is compared pairwise (searched, it costs more than the blocks do)
       listing = static_cast<int>(all_of_it ? S.at[1] : S.at[1] - S.at[0]);
       __syncthreads();
       if (all_of_it && tid == 0) S.from = 0;
@@ -524,11 +529,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
               }
             }
           }
-          if (hits) {       // (a place for the whole warp's at once costs more instructions than it saves atomics: 182 us against 168 for 256 rows of 128 k)
+          if (hits) {       // looked up again, one by one: few
             uint32_t at = atomicAdd(&S.listed, static_cast<uint32_t>(__popc(hits)));
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (hits >> e & 1 && at < kList) S.list[at++] = composite(v[e], index_of(b, e));
+            do {
+              const int e = __ffs(hits) - 1;
+              hits &= hits - 1;
+              if (at < kList) S.list[at++] = composite(bits_at(b, e), index_of(b, e));
+            } while (hits);
           }
           if (decltype(sums)::value && from > 0) {
             if (!decltype(limited)::value) above += sum;
