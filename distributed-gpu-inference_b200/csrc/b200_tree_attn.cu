@@ -257,20 +257,42 @@ __device__ __forceinline__ Walk walk_of(const TreeAttn& A, int worker, int worke
   return w;
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// by a whole warp
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, int col, int row, uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\n"
+      "@p cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}\n" ::"r"(to),
+      "l"(map), "r"(col), "r"(row), "r"(bar)
+      : "memory");
+}
+
 __device__ __forceinline__ uint32_t line(uint32_t base, int r, int ch, int rows) {     // 16-byte piece ch of row r: blocks of 64 columns, swizzled lines
   return base + (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
 }
 
+// the larger magnitudes of two pairs, no number if one is none
+template <typename T>
+__device__ __forceinline__ uint32_t magnitudes(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ bool no_number(uint32_t two) {        // either half
   constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
   return (two & e) == e || ((two >> 16) & e) == e;
 }
 template <typename T>
-__device__ __forceinline__ uint32_t numbers_only(uint32_t two) {
-  constexpr uint32_t e = std::is_same_v<T, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
-  if ((two & e) == e) two &= 0xffff0000u;
-  if (((two >> 16) & e) == e) two &= 0xffffu;
+__device__ __forceinline__ int numbers_only(int two) {
+  constexpr int e = std::is_same_v<T, __nv_bfloat16> ? 0x7f80 : 0x7c00;
+  if ((two & e) == e) two &= 0xffff0000;
+  if (((two >> 16) & e) == e) two &= 0xffff;
   return two;
 }
 
@@ -348,8 +370,8 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
     // ---- copies ------------------------------------------------------------------------------------------------------------------------------
     const bool values = warp >= (kSoft + kLoadK) / 32;
     const int me = tid - kSoft - kLoadK;        // of those that copy values
-    const int box = min(A.bs, kKeys), n_pages = kKeys / box, ahead = 32 / n_pages;      // rows of a copy, copies and (below) tiles of a look-up
-    const int my_page = values ? lane * 2 + me / 32 : lane;       // two warps take turns
+    // rows of a copy, copies of a tile, tiles of a look-up (below): powers of two
+    const int box = min(A.bs, kKeys), box_bits = __ffs(box) - 1, page_bits = 6 - box_bits, n_pages = 1 << page_bits, ahead = 32 >> page_bits;
     const uint32_t bar_in = values ? bar_v : bar_k, bar_free = values ? bar_o : bar_ke, bufs = sm0 + (values ? P::kV : P::kK);
     const CUtensorMap* map = values ? &v_map : &k_map;
     for (int i = 0; w.left > 0;) {
@@ -359,14 +381,14 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
       const int32_t* table = A.block_tables + static_cast<int64_t>(b) * A.table_stride;
       // 32 pages at a time, the next ones under way: of tile at + lane / n_pages; -1: none, behind the pool (copies bring zeros): outside it
       auto look_up = [&](int at) -> int {
-        const int t = at + lane / n_pages, j = t * kKeys + lane % n_pages * box;
+        const int t = at + (lane >> page_bits), j = t * kKeys + ((lane & (n_pages - 1)) << box_bits), col = A.bs > kKeys ? j / A.bs : j >> box_bits;
+        const int page = col < A.table_cols ? table[col] : 0;       // (asked for before it is known how many keys there are)
         if (t >= t0 + run || j >= keys) return -1;
-        const int page = table[j / A.bs];
         return page < 0 || page >= A.max_blocks ? static_cast<int>(A.max_blocks) : page;
       };
       int pages = look_up(t0), later = look_up(t0 + ahead);
       for (int x = 0; x < run; ++x, ++i) {
-        const int in = x % ahead;
+        const int in = x & (ahead - 1);
         if (x > 0 && in == 0) {
           pages = later;
           later = look_up(t0 + x + ahead);
@@ -375,46 +397,51 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
           if (i >= NB) bar_wait(bar_free + 8 * (i % NB), (i / NB - 1) & 1, dead);
         };
         const uint32_t base = bufs + (i % NB) * (D / 64) * kBlk, bar = bar_in + 8 * (i % NB);
-        const int j0 = (t0 + x) * kKeys;
+        const int j0 = (t0 + x) * kKeys, in_page = A.bs > kKeys ? j0 % A.bs : 0;
         if (!values || j0 + kKeys <= keys - n) {
           free_again();
-          const int page = __shfl_sync(0xffffffffu, pages, in * n_pages + (my_page < n_pages ? my_page : 0));
-          if (my_page < n_pages && page >= 0) {
-            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((D / 64) * box * 128) : "memory");
-            const int row = (page * A.Hkv + g) * A.bs + (A.bs > kKeys ? j0 % A.bs : 0);
+          // One thread asks for all of them: a copy for each of several lanes took 150 clocks each, 1200 for a tile's keys.  The two warps of the values
+          // take turns with the pages.
+          const int turns = values ? 2 : 1, mine = values ? me / 32 : 0;
+          const int there = __popc(__ballot_sync(0xffffffffu, lane >> page_bits == in && (lane & (n_pages - 1) & (turns - 1)) == mine && pages >= 0));
+          if (there > 0 && elect_one())
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(there * (D / 64) * box * 128) : "memory");
+          __syncwarp();
+          for (int y = mine; y < n_pages; y += turns) {
+            const int page = __shfl_sync(0xffffffffu, pages, (in << page_bits) + y);
+            if (page < 0) break;
+            const int row = (page * A.Hkv + g) * A.bs + in_page;
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-              asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(base + c * kBlk + my_page * box * 128),
-                           "l"(map), "r"(64 * c), "r"(row), "r"(bar) : "memory");
+            for (int c = 0; c < D / 64; ++c) copy_box(base + c * kBlk + y * box * 128, map, 64 * c, row, bar);
           }
         } else {
           // all loads before the buffer is free and the first store
-          bool odd = false;
           constexpr int kCh = D / 8, kPer = kKeys * kCh / kLoadV;
           int4 v[kPer];
+          uint32_t most = 0;
 #pragma unroll
           for (int u = 0; u < kPer; ++u) {
             const int c = me + u * kLoadV, key = c / kCh, ch = c - key * kCh;
-            const int page = __shfl_sync(0xffffffffu, pages, in * n_pages + key / box);
+            const int page = __shfl_sync(0xffffffffu, pages, (in << page_bits) + (key >> box_bits));
             v[u] = make_int4(0, 0, 0, 0);
             if (j0 + key < keys && page < A.max_blocks)
-              v[u] = *reinterpret_cast<const int4*>(static_cast<const T*>(A.v_pool) + ((static_cast<int64_t>(page) * A.Hkv + g) * A.bs + (j0 + key) % A.bs) * D + ch * 8);
+              v[u] = *reinterpret_cast<const int4*>(static_cast<const T*>(A.v_pool) + ((static_cast<int64_t>(page) * A.Hkv + g) * A.bs + in_page + (key & (box - 1))) * D + ch * 8);
+          }
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) most = magnitudes<T>(v[u].x, magnitudes<T>(v[u].y, magnitudes<T>(v[u].z, magnitudes<T>(v[u].w, most))));
+          if (no_number<T>(most)) {       // hardly ever; the context's stay (every row sees them)
+            *strange = 1;
+#pragma unroll
+            for (int u = 0; u < kPer; ++u)
+              if (j0 + (me + u * kLoadV) / kCh >= keys - n)
+                v[u] = make_int4(numbers_only<T>(v[u].x), numbers_only<T>(v[u].y), numbers_only<T>(v[u].z), numbers_only<T>(v[u].w));
           }
           free_again();
 #pragma unroll
           for (int u = 0; u < kPer; ++u) {
             const int c = me + u * kLoadV, key = c / kCh, ch = c - key * kCh;
-            uint32_t y[4] = {static_cast<uint32_t>(v[u].x), static_cast<uint32_t>(v[u].y), static_cast<uint32_t>(v[u].z), static_cast<uint32_t>(v[u].w)};
-            if (j0 + key >= keys - n) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                odd = odd || no_number<T>(y[e]);
-                y[e] = numbers_only<T>(y[e]);
-              }
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(base, key, ch, kKeys)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line(base, key, ch, kKeys)), "r"(v[u].x), "r"(v[u].y), "r"(v[u].z), "r"(v[u].w) : "memory");
           }
-          if (odd) *strange = 1;
           fence_smem_to_mma();
         }
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -464,24 +491,18 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
     const uint32_t tm_row = tm + (static_cast<uint32_t>(32 * warp) << 16);
     const float k2 = A.scale > 0.f ? A.scale * kLog2e : 1.f;       // weight = 2^(s k2 - m)
     const int per = W.rows;
-    if (W.whole) {        // rows without a node
-      int keys, n;
-      lengths(A, w.b, &keys, &n);
-      constexpr int kCh = D / 8;
-      for (int c = tid; c < kRows * kCh; c += soft_warps * 32) {
-        const int at = row0 + c / kCh, t = at / rep;
-        if (t >= n && t < A.nodes)
-          *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + ((static_cast<int64_t>(w.b) * A.nodes + t) * A.Hq + w.g * rep + at - t * rep) * D + c % kCh * 8) = make_uint4(0, 0, 0, 0);
-      }
-    }
+    const float per_rep = 1.0f / rep;
+    auto node_of = [&](int row) { return static_cast<int>((row + 0.5f) * per_rep); };        // (exact: rows have 18 bits; a division takes a hundred clocks)
+    const int whole_b = w.b, whole_g = w.g;
     int i = 0;
     while (w.left > 0) {
       const int b = w.b, g = w.g, t0 = w.t, run = w.run();
       int keys, n;
+      uint64_t seen = node < A.nodes ? static_cast<uint64_t>(A.visible[b * A.visible_stride + node]) : 0ull;
       lengths(A, b, &keys, &n);
       const int base = keys - n;
       const bool live = node < n;
-      uint64_t seen = live ? static_cast<uint64_t>(A.visible[b * A.visible_stride + node]) : 0ull;
+      if (!live) seen = 0;
       if (n < 64) seen &= (1ull << n) - 1;
       {
         constexpr int kCh = D / 8;
@@ -489,7 +510,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
 #pragma unroll 8
         for (int u = 0; u < kCh; ++u) {
           const int c = lane + u * 32, r = c / kCh, ch = c % kCh, at = row0 + warp % kRowWarps * 32 + r;       // a warp's rows by itself
-          const int t = at / rep, h = g * rep + at - t * rep;
+          const int t = node_of(at), h = g * rep + at - t * rep;
           const bool in = t < n;
           cp16(line(sm0 + P::kQ, 32 * warp + r, ch, kRows), in ? q + t * A.q_node_stride + static_cast<int64_t>(h) * D + ch * 8 : q, in);
         }
@@ -586,7 +607,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
       auto others_too = [&] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
       float scaled = 1.f;      // this warp's output to the row's common reference
       if constexpr (SPLIT > 1) {
-        float2* ml = reinterpret_cast<float2*>(sm + P::kK - 1024);        // behind the rows that are put together below
+        float2* ml = reinterpret_cast<float2*>(sm + P::kK - 1024);        // (of the room below)
         ml[tid] = make_float2(m_ref, ok ? l : NAN);
         others_too();
         float top = -INFINITY;
@@ -614,9 +635,9 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
         tc_wait_ld();
         if constexpr (SPLIT > 1) {
           // [part][column / 4][row] of four columns
-          float4* all = reinterpret_cast<float4*>(sm + P::kQ);
           constexpr int kSet = kRows / SPLIT;
-          others_too();
+          float4* all = reinterpret_cast<float4*>(sm + P::kQ) + (D == 128 && c % 64 ? 32 * kSet * SPLIT / 4 : 0);        // in turns, where there is room for two
+          if (D == 64 || c == 0) others_too();
 #pragma unroll
           for (int u = 0; u < 32; u += 4) all[(part * 8 + u / 4) * kSet + my_row] = make_float4(o[u] * scaled, o[u + 1] * scaled, o[u + 2] * scaled, o[u + 3] * scaled);
           others_too();
@@ -663,7 +684,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
         constexpr int kCh = D / 8;
 #pragma unroll 4
         for (int u = 0; u < kCh; ++u) {
-          const int c = lane + u * 32, r = c / kCh, ch = c % kCh, at = row0 + 32 * warp + r, t = at / rep, h = g * rep + at - t * rep;
+          const int c = lane + u * 32, r = c / kCh, ch = c % kCh, at = row0 + 32 * warp + r, t = node_of(at), h = g * rep + at - t * rep;
           if (t < n) {
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(line(sm0 + P::kQ, 32 * warp + r, ch, kRows)) : "memory");
@@ -674,6 +695,16 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
       if constexpr (SPLIT > 1) others_too();       // the next queries go where the outputs were
       __syncwarp();
       w.skip(A, run);
+    }
+    if (W.whole) {        // rows without a node
+      int keys, n;
+      lengths(A, whole_b, &keys, &n);
+      constexpr int kCh = D / 8;
+      for (int c = n < A.nodes ? tid : kRows * kCh; c < kRows * kCh; c += soft_warps * 32) {
+        const int at = row0 + c / kCh, t = node_of(at);
+        if (t >= n && t < A.nodes)
+          *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + ((static_cast<int64_t>(whole_b) * A.nodes + t) * A.Hq + whole_g * rep + at - t * rep) * D + c % kCh * 8) = make_uint4(0, 0, 0, 0);
+      }
     }
   }
   tc_fence_before();
@@ -706,7 +737,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttn A, const
 #pragma unroll
   for (int c = 0; c < PER; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live && !nothing) {
-    constexpr int kAhead = 8 / PER;
+    constexpr int kAhead = PER == 1 ? 16 : 8 / PER;
     for (int p0 = first; p0 <= last; p0 += kAhead) {
       float2 ml[kAhead];
       float4 v[kAhead][PER];
@@ -775,7 +806,7 @@ Shares shares_of(int nodes, int Hq, int Hkv) {
 size_t sums_bytes(const Shares& W) { return static_cast<size_t>(W.workers) * W.blocks * 2 * W.rows * sizeof(float2); }
 
 bool tiles_serve(int Hq, int Hkv, int D, int bs, int dtype) {
-  return (dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16) && (D == 64 || D == 128) && ((bs >= 8 && kKeys % bs == 0) || bs % kKeys == 0) && Hq / Hkv <= 1 << 16;
+  return (dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16) && (D == 64 || D == 128) && ((bs >= 8 && kKeys % bs == 0) || bs % kKeys == 0) && Hq / Hkv <= 1 << 12;
 }
 
 template <typename T, int D>
