@@ -150,6 +150,7 @@ accept_drafts_kernel(const Accept A) {
   if (A.n_layers == 0) return;
   __syncthreads();
   char* pool = static_cast<char*>((blockIdx.y & 1 ? A.v_pools : A.k_pools)[blockIdx.y >> 1]);
+  if ((blockIdx.y & 1) && pool == A.k_pools[blockIdx.y >> 1]) return;       // values that are the keys move once
   const int64_t head_bytes = static_cast<int64_t>(A.bs) * A.row_bytes;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(pool) | static_cast<uintptr_t>(A.row_bytes);
   if ((bits & 15) == 0) move_rows<int4>(pool, src, dst, count, A.Hkv, head_bytes, A.row_bytes);

@@ -286,7 +286,7 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         raise ValueError("out must be a contiguous int64 [rows] on the logits' device")
     with _on(dev) as stream:
         rc = _lib.load().b200_sample_rows(out.data_ptr(), x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, u.data_ptr(), tp, t, kp,
-                                          min(int(k), 0x7fffffff), pp, p, mp, m, _dtype_id(x), stream)
+                                          min(max(int(k), 0), 0x7fffffff), pp, p, mp, m, _dtype_id(x), stream)
     if rc != 0:
         _lib.check(rc, "b200_sample_rows")
     return out

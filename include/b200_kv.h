@@ -292,15 +292,17 @@ int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64_t cols, in
  * node whose parent is not before it sees only itself; nodes behind the sequence's last see nothing.  parents' rows parent_stride apart.
  *
  * b200_paged_tree_attn: out[b, t, h] = softmax(q k scale) v over the context (the first context_lens[b] - n tokens, n the sequence's nodes) and the
- * nodes in visible[b, t], any set of them.  A row that sees nothing, and rows behind the sequence's last node, are 0.  Keys that no row of a call may see
- * are not read (stale slots may hold anything); NaN and infinities in a node's values reach the rows that see it only.  A table entry outside
+ * nodes in visible[b, t], any set of them.  A row that sees nothing, and rows behind the sequence's last node, are 0.  Slots
+ * behind the last token may hold anything; NaN and infinities in a node's values reach the rows that see it only (one in the context's, which
+ * every row sees, may come out as NaN).  A table entry outside
  * the pool reads as zeros.  At most table_cols pages of a sequence are read.  q: [B, nodes, Hq, D], rows of a node contiguous; out contiguous.
  *   workspace : b200_paged_tree_attn_workspace bytes, 16-byte aligned, any contents; calls that may run at the same time need their own.
  *
  * b200_accept_drafts: node t fits if its token is chosen[b, parent] (the first of siblings with the same token), and is taken if all of
  * visible[b, t] fits.  count[b]: taken nodes, the root among them; path[b, k] the k-th, -1 behind the last; new_tokens[b, k] = chosen[b, path[b, k]],
  * -1 behind; new_lens[b] the context and the taken nodes.  Keys and values of path[b, k] move to the k-th place behind the context in
- * every pool of k_pools / v_pools (device arrays of n_layers pool addresses; n_layers 0: nothing moves).  Pages of these places belong to one sequence.
+ * every pool of k_pools / v_pools (device arrays of n_layers pool addresses; n_layers 0: nothing moves).  Pages of these places belong to one
+ *   sequence, and no pool stands twice in a call but for values that are a layer's keys.
  */
 #define B200_MAX_DRAFT_NODES 64
 int b200_draft_tree(int64_t* visible, int32_t* depth, const int32_t* parents, int64_t parent_stride, const int32_t* draft_lens, int B,

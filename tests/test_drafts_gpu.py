@@ -134,6 +134,15 @@ def test_no_drafts_no_pools_and_pages_outside():
     assert out[3].tolist() == [3 + int(out[0][0]), 0, int(out[0][2])]
 
 
+def test_values_that_are_the_keys_move_once():
+    c = case(3, 16, 4, 16, 1, 1, 64, torch.bfloat16, 7)
+    alone = [p.clone() for p in c[6]]
+    run(c[:6] + ([alone[0], alone[1]],))
+    both = c[6][0].clone()
+    run(c[:6] + ([both, both],))
+    assert torch.equal(both, alone[0])
+
+
 def test_captured_and_replayed():
     c = case(4, 16, 3, 16, 2, 2, 64, torch.bfloat16, 5)
     par, lens, tokens, chosen, context, tables, pools = c

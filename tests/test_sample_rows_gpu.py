@@ -76,6 +76,16 @@ def test_rows_of_several_ctas_and_beyond_shared_memory(cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_more_tokens_kept_than_a_list_holds(dtype):
+    """k beyond 2048, and ranges with more equal logits than are listed: the last key by its digits."""
+    x, u = logits(6, 50001, dtype, 21)
+    more = [(1.0, 2049, 1.0, 0.0), (1.0, 5000, 0.9, 0.0), (1.5, 49999, 0.99, 1e-4), (0.7, 2048, 1.0, 0.0), (1.0, 50000, 0.5, 0.0), (2.0, 30000, 1.0, 0.01)]
+    check(x, u, more)
+    check((x * 0.25).round() * 4, u, more)
+    check((x * 0.25).round() * 4, u, [(1.0, 0, 0.9, 0.0), (1.0, 700, 1.0, 0.0), (1.0, 2000, 0.99, 0.0), (3.0, 0, 0.999, 0.0), (1.0, 0, 0.3, 0.1), (1.0, 9, 0.9, 0.0)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_off_the_16_byte_grid_and_apart(dtype):
     wide, u = logits(len(SETTINGS), 5003, dtype, 1)
     for first in (1, 3, 5, 8):
@@ -159,6 +169,9 @@ def test_numbers_for_all_rows_and_a_row_among_many():
     assert a[:5].tolist() == [int(ops.sample_rows(x[i:i + 1], u[i:i + 1], 0.8, 40, 0.9, 0.01)) for i in range(5)]
     assert ops.sample_rows(x[:0], u[:0]).shape == (0,)
     assert torch.equal(ops.sample_rows(x, u, 0.0), ops.argmax_rows(x))
+    assert torch.equal(ops.sample_rows(x, u, 1.0, top_k=-2 ** 40), ops.sample_rows(x, u)) and torch.equal(ops.sample_rows(x, u, top_k=2 ** 40), ops.sample_rows(x, u))
+    nan = float("nan")
+    assert torch.equal(ops.sample_rows(x, u, top_p=nan, min_p=nan), ops.sample_rows(x, u))
 
 
 def test_captured_on_another_stream_and_replayed():

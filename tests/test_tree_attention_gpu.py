@@ -173,6 +173,30 @@ def test_large_scores_and_a_maximum_that_grows_along_the_keys():
     check(c)
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("nodes", [3, 12, 40])
+def test_scales_below_and_at_zero(nodes, scale):
+    check(build(2, nodes, 8, 2, 64, 16, 700, torch.bfloat16, seed=nodes, stale=0.0), scale=scale)
+
+
+def test_many_sequences_and_groups_of_odd_size():
+    """More sequences than a look-up of lengths holds; heads whose rows straddle warps and blocks."""
+    check(build(150, 3, 6, 2, 64, 16, 90, torch.bfloat16, seed=2))
+    wide = build(140, 2, 5, 1, 128, 16, 700, torch.float16, seed=3)
+    check(wide)
+    check(build(2, 61, 21, 3, 128, 16, 900, torch.bfloat16, seed=5))
+
+
+def test_a_context_that_is_infinite_somewhere_is_no_number_there():
+    c = build(2, 6, 8, 2, 128, 16, 900, torch.bfloat16, seed=11, ragged=False, stale=0.0)
+    c["v_pool"][int(c["block_tables"][1, 3]), 0, 5, 9] = float("inf")
+    got = ops.paged_tree_attention(c["q"], c["k_pool"], c["v_pool"], c["block_tables"], c["context_lens"], c["visible"])
+    bad = ~torch.isfinite(got)
+    want = torch.zeros_like(bad)
+    want[1, :, :4, 9] = True
+    assert torch.equal(bad, want)
+
+
 def test_strided_queries_tables_and_masks():
     c = build(3, 10, 8, 2, 64, 16, 150, torch.bfloat16, seed=8)
     qkv = torch.randn((3, 10, 12 * 64), device=DEV).to(torch.bfloat16)
