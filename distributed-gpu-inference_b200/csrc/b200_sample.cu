@@ -620,122 +620,120 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
           const u64 goal = __umul64hi(fraction(u), sum);
           const u64 lower = before_mine([&](u64 o) { return (o & index_mask) > (c & index_mask); }, &unused);
           if (keep && part == 0 && !S.failed && lower <= goal && goal < lower + w) A.out[row] = index_in(c);
-          n = 0;
-        }
-        if (n > 0) {
-        if (tid == 0) S.ends[0] = ~0ull, S.ends[1] = 0;
-        __syncthreads();
-        {
-          u64 lo = ~0ull, hi = 0;
-          for (int i = tid; i < n; i += kThreads) lo = min(lo, S.list[i]), hi = max(hi, S.list[i]);
+        } else {
+          if (tid == 0) S.ends[0] = ~0ull, S.ends[1] = 0;
+          __syncthreads();
+          {
+            u64 lo = ~0ull, hi = 0;
+            for (int i = tid; i < n; i += kThreads) lo = min(lo, S.list[i]), hi = max(hi, S.list[i]);
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            for (int o = 16; o > 0; o >>= 1) {
+              lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+              hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            if (lane == 0) {
+              atomicMin(&S.ends[0], lo);
+              atomicMax(&S.ends[1], hi);
+            }
           }
-          if (lane == 0) {
-            atomicMin(&S.ends[0], lo);
-            atomicMax(&S.ends[1], hi);
-          }
-        }
-        __syncthreads();
-        const u64 lowest_listed = S.ends[0], highest_listed = S.ends[1];
-        // The element of the list at which the running value (1 or the weight) from `upto` on reaches `target`, of those from `lowest` on, in the
-        // list's order or by index: by the sums of 512 equal parts of what is left, until a part has few elements.
-        u64* bins = S.range_count;
-        u64 *few = bins + kBins, *few_value = few + kFew;
-        auto find = [&](auto by_index, u64 lo, u64 hi, u64 lowest, auto&& value_of, u64 upto, u64 target) -> u64 {
-          auto order = [&](u64 c) { return decltype(by_index)::value ? c & index_mask : c; };
-          while (true) {
-            int shift = 63;       // one part
-            u64 bin = 0;
-            bins[tid] = 0;
-            if (tid == 0) S.few = 0, S.at[0] = ~0ull, S.at[2] = 0;
-            __syncthreads();
-            if (n > kFew) {
-              shift = max(0, 64 - __clzll(hi - lo) - 9);
+          __syncthreads();
+          const u64 lowest_listed = S.ends[0], highest_listed = S.ends[1];
+          // The element of the list at which the running value (1 or the weight) from `upto` on reaches `target`, of those from `lowest` on, in the
+          // list's order or by index: by the sums of 512 equal parts of what is left, until a part has few elements.
+          u64* bins = S.range_count;
+          u64 *few = bins + kBins, *few_value = few + kFew;
+          auto find = [&](auto by_index, u64 lo, u64 hi, u64 lowest, auto&& value_of, u64 upto, u64 target) -> u64 {
+            auto order = [&](u64 c) { return decltype(by_index)::value ? c & index_mask : c; };
+            while (true) {
+              int shift = 63;       // one part
+              u64 bin = 0;
+              bins[tid] = 0;
+              if (tid == 0) S.few = 0, S.at[0] = ~0ull, S.at[2] = 0;
+              __syncthreads();
+              if (n > kFew) {
+                shift = max(0, 64 - __clzll(hi - lo) - 9);
+                for (int i = tid; i < n; i += kThreads) {
+                  const u64 c = S.list[i], o = order(c);
+                  if (c >= lowest && o >= lo && o <= hi) atomicAdd(&bins[(hi - o) >> shift], value_of(c));
+                }
+                __syncthreads();
+                u64 unused;
+                const u64 in = bins[tid], before = upto + cta_before(in, S.part, &unused);
+                if (before < target && target <= before + in) S.at[0] = tid, S.at[1] = before;
+                __syncthreads();
+                if (S.at[0] == ~0ull) return 0;       // not in the list
+                bin = S.at[0];
+                upto = S.at[1];
+              }
               for (int i = tid; i < n; i += kThreads) {
                 const u64 c = S.list[i], o = order(c);
-                if (c >= lowest && o >= lo && o <= hi) atomicAdd(&bins[(hi - o) >> shift], value_of(c));
+                if (c >= lowest && o >= lo && o <= hi && (hi - o) >> shift == bin) {
+                  const uint32_t at = atomicAdd(&S.few, 1u);
+                  if (at < kFew) few[at] = c, few_value[at] = value_of(c);
+                }
               }
               __syncthreads();
-              u64 unused;
-              const u64 in = bins[tid], before = upto + cta_before(in, S.part, &unused);
-              if (before < target && target <= before + in) S.at[0] = tid, S.at[1] = before;
+              const int m = S.few;
+              if (m <= kFew) {
+                if (tid < m) {
+                  u64 before_mine = upto;
+                  for (int j = 0; j < m; ++j)
+                    if (order(few[j]) > order(few[tid])) before_mine += few_value[j];
+                  if (before_mine < target && target <= before_mine + few_value[tid]) S.at[2] = few[tid];
+                }
+                __syncthreads();
+                const u64 c = S.at[2];
+                __syncthreads();
+                return c;
+              }
+              hi -= bin << shift;
+              lo = max(lo, hi - ((1ull << shift) - 1));
               __syncthreads();
-              if (S.at[0] == ~0ull) return 0;       // not in the list
-              bin = S.at[0];
-              upto = S.at[1];
             }
+          };
+          auto weight_of = [&](u64 c) { return weigh.number(logit_of(c)); };
+          auto kept_of = [&](u64 c) -> u64 {
+            const u64 w = weigh.number(logit_of(c));
+            return w >= least_number ? w : 0;
+          };
+          auto sum_from = [&](u64 lowest, auto&& value_of) {
+            u64 mine = 0, sum;
+            for (int i = tid; i < n; i += kThreads) mine += S.list[i] >= lowest ? value_of(S.list[i]) : 0;
+            cta_before(mine, S.part, &sum);
+            return sum;
+          };
+          u64 whole = 0, over = 0, mine = 0;
+          if (k) {
+            if (n > k) mine = find(std::false_type{}, lowest_listed, highest_listed, 0ull, [](u64) { return 1ull; }, 0ull, static_cast<u64>(k));
+            if (by_mass) whole = sum_from(mine, weight_of);
+          } else {
+            whole = sum_of_all(&S.sum_all);
+            over = sum_of_all(&S.sum_above);
+          }
+          bool failed = false;
+          if (by_mass) {
+            const u64 limit = limit_of(p, whole);
+            const u64 last = over < limit ? find(std::false_type{}, lowest_listed, highest_listed, mine, weight_of, over, limit) : 0;
+            failed = last == 0;     // p of all is reached above the list, or below it
+            mine = last;
+          }
+          if (failed) {
+            if (tid == 0) S.failed = 1;
+          } else if (from > 0) {      // kept ones to their blocks
             for (int i = tid; i < n; i += kThreads) {
-              const u64 c = S.list[i], o = order(c);
-              if (c >= lowest && o >= lo && o <= hi && (hi - o) >> shift == bin) {
-                const uint32_t at = atomicAdd(&S.few, 1u);
-                if (at < kFew) few[at] = c, few_value[at] = value_of(c);
+              const u64 c = S.list[i], w = c >= mine ? kept_of(c) : 0;
+              if (w) {
+                const int place = static_cast<int>(index_in(c)) + head, b = place / kBlock, r = b / A.blocks_per_cta;
+                u64* sums = reinterpret_cast<u64*>(cluster.map_shared_rank(dynamic, r) + sizeof(Shared));
+                atomicAdd(&sums[b - r * A.blocks_per_cta], w);
               }
             }
-            __syncthreads();
-            const int m = S.few;
-            if (m <= kFew) {
-              if (tid < m) {
-                u64 before_mine = upto;
-                for (int j = 0; j < m; ++j)
-                  if (order(few[j]) > order(few[tid])) before_mine += few_value[j];
-                if (before_mine < target && target <= before_mine + few_value[tid]) S.at[2] = few[tid];
-              }
-              __syncthreads();
-              const u64 c = S.at[2];
-              __syncthreads();
-              return c;
-            }
-            hi -= bin << shift;
-            lo = max(lo, hi - ((1ull << shift) - 1));
-            __syncthreads();
+            if (tid == 0) S.cut = mine;
+          } else {        // all that is kept is in the list
+            const u64 goal = __umul64hi(fraction(u), sum_from(mine, kept_of));
+            const u64 c = find(std::true_type{}, static_cast<u64>(index_mask + 1 - A.cols), static_cast<u64>(index_mask), mine, kept_of, 0ull, goal + 1);
+            if (tid == 0) A.out[row] = index_in(c);
           }
-        };
-        auto weight_of = [&](u64 c) { return weigh.number(logit_of(c)); };
-        auto kept_of = [&](u64 c) -> u64 {
-          const u64 w = weigh.number(logit_of(c));
-          return w >= least_number ? w : 0;
-        };
-        auto sum_from = [&](u64 lowest, auto&& value_of) {
-          u64 mine = 0, sum;
-          for (int i = tid; i < n; i += kThreads) mine += S.list[i] >= lowest ? value_of(S.list[i]) : 0;
-          cta_before(mine, S.part, &sum);
-          return sum;
-        };
-        u64 whole = 0, over = 0, mine = 0;
-        if (k) {
-          if (n > k) mine = find(std::false_type{}, lowest_listed, highest_listed, 0ull, [](u64) { return 1ull; }, 0ull, static_cast<u64>(k));
-          if (by_mass) whole = sum_from(mine, weight_of);
-        } else {
-          whole = sum_of_all(&S.sum_all);
-          over = sum_of_all(&S.sum_above);
-        }
-        bool failed = false;
-        if (by_mass) {
-          const u64 limit = limit_of(p, whole);
-          const u64 last = over < limit ? find(std::false_type{}, lowest_listed, highest_listed, mine, weight_of, over, limit) : 0;
-          failed = last == 0;     // p of all is reached above the list, or below it
-          mine = last;
-        }
-        if (failed) {
-          if (tid == 0) S.failed = 1;
-        } else if (from > 0) {      // kept ones to their blocks
-          for (int i = tid; i < n; i += kThreads) {
-            const u64 c = S.list[i], w = c >= mine ? kept_of(c) : 0;
-            if (w) {
-              const int place = static_cast<int>(index_in(c)) + head, b = place / kBlock, r = b / A.blocks_per_cta;
-              u64* sums = reinterpret_cast<u64*>(cluster.map_shared_rank(dynamic, r) + sizeof(Shared));
-              atomicAdd(&sums[b - r * A.blocks_per_cta], w);
-            }
-          }
-          if (tid == 0) S.cut = mine;
-        } else {        // all that is kept is in the list
-          const u64 goal = __umul64hi(fraction(u), sum_from(mine, kept_of));
-          const u64 c = find(std::true_type{}, static_cast<u64>(index_mask + 1 - A.cols), static_cast<u64>(index_mask), mine, kept_of, 0ull, goal + 1);
-          if (tid == 0) A.out[row] = index_in(c);
-        }
         }
       }
       if (k) return;
