@@ -35,11 +35,11 @@ __device__ __forceinline__ void lengths(const TreeAttn& A, int b, int* keys, int
 // One CTA per (sequence, node, query head); its warps take 32 keys in turns, a lane a key for the scores and a part of the columns for the
 // output, and put their maxima, sums and outputs together at the end.  Bound by the loads' latency; serves what the kernel below does not
 // (fp32, head sizes other than 64 and 128, pages that do not divide 64 keys).
-constexpr int kAnyWarps = 4, kAnyMostD = 256;
+constexpr int kAnyWarps = 8, kAnyMostD = 256;
 
 template <typename T, int COLS>
 __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const TreeAttn A, bool vec) {
-  constexpr int kVec = 16 / sizeof(T), kAhead = 32 / COLS < 8 ? 32 / COLS : 8, kMostD = 32 * COLS;        // rows of values under way
+  constexpr int kVec = 16 / sizeof(T), kAhead = 32 / COLS, kMostD = 32 * COLS;        // rows of values under way
   __shared__ __align__(16) float q_s[kMostD];
   __shared__ float out_s[kAnyWarps][kMostD], m_s[kAnyWarps], l_s[kAnyWarps];
   const int h = blockIdx.x, t = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const Tre
     if (at >= 0) {
       const T* k = static_cast<const T*>(A.k_pool) + at;
       if (vec) {
-#pragma unroll 8
+#pragma unroll 16
         for (int d = 0; d < A.D; d += kVec) {
           const int4 raw = *reinterpret_cast<const int4*>(k + d);
           const T* e = reinterpret_cast<const T*>(&raw);
