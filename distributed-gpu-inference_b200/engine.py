@@ -62,7 +62,8 @@ class _TreeStep:
         st = PagedBatchState(block_tables=tables, context_lens=total, slot_mapping=slots.reshape(-1), max_context_len=e.max_seq_len,
                              workspace=self.workspace, visible=visible, draft_lens=self.lens)
         st.cos, st.sin = rope_tables(pos, e.inv_freq, e.dtype, e.rope_scaling)
-        h = self.tokens
+        # Behind a sequence's last node, and in drafts of other vocabularies, there may be any number: the model gets tokens, only equal ones are taken
+        h = self.tokens.clamp(0, e.shards[0].embed_tokens.weight.shape[0] - 1)
         for shard, handles in zip(e.shards, e._handles):
             h, _ = shard.forward(h, position_ids=pos, past_key_values=[PagedLayerKV(hd.k_pool, hd.v_pool, st) for hd in handles], use_cache=True)
         logits = e.shards[-1].get_logits(h)
@@ -432,23 +433,24 @@ class PagedDecodeEngine:
 
     # ---- the next token --------------------------------------------------------------------------------
     def set_sampling(self, sampling: Optional[Sequence[Sampling]]) -> None:
-        """How the sequences ``0 .. len(sampling) - 1`` choose their tokens from now on; None: greedily."""
+        """How the sequences ``0 .. len(sampling) - 1`` choose their tokens from now on, the ones behind them greedily; None: all greedily."""
         rows = None if sampling is None else list(sampling)
+        if rows is not None and len(rows) > self.max_batch:
+            raise ValueError("more settings than the engine has sequences")
         if rows is not None and all(s.temperature == 0.0 for s in rows):
             rows = None
+        if rows is not None and (not (self.is_first and self.is_last) or self.external_head):
+            raise RuntimeError("sampling needs an engine with the whole model")
         if (rows is None) != (self.sampling is None):       # captured steps choose one way or the other
             self._graph = self._graph_chained = None
             self._trees = {}
         self.sampling = rows
         if rows is None:
             return
-        if len(rows) > self.max_batch:
-            raise ValueError("more settings than the engine has sequences")
-        if not (self.is_first and self.is_last) or self.external_head:
-            raise RuntimeError("sampling needs an engine with the whole model")
         if self._numbers is None:
             self._numbers = torch.zeros((self.max_batch, self.max_seq_len + 1), dtype=torch.float32, device=self.device)
         for buf, values in zip((self._temperature, self._top_k, self._top_p, self._min_p), settings(rows)):
+            buf.zero_()
             buf[:len(rows)].copy_(torch.from_numpy(values))
         self._numbers[:len(rows)].copy_(torch.from_numpy(np.stack([s.numbers(self.max_seq_len + 1) for s in rows])))
 
@@ -611,7 +613,7 @@ class PagedDecodeEngine:
 
         ``tokens`` int64 and ``parents`` int32 ``[batch, nodes]`` (host or device): node 0 is the sequence's last token, which no step has
         seen yet, the others come behind their parents; ``draft_lens`` int32 ``[batch]`` how many nodes a sequence has (0: it rests).  The
-        model runs once over all nodes; the nodes whose tokens are the model's own choices stay in the cache, side by side behind the context,
+        model runs once over all nodes (a token outside its vocabulary is never taken); the nodes whose tokens are the model's own choices stay in the cache, side by side behind the context,
         and a sequence gets ``count`` new tokens: one for each of them.  The choices are the ones that single steps would have made."""
         if not (self.is_first and self.is_last) or self.external_head:
             raise RuntimeError("verify_trees() drives a whole model")
@@ -628,6 +630,10 @@ class PagedDecodeEngine:
             held = len(self._seq_blocks[b][0][0]) * self.block_size
             if lens[b] and self._host_lens[b] + lens[b] > min(held, self.max_seq_len):
                 raise ValueError(f"Maximum length exceeded: {self._host_lens[b]} + {lens[b]} > {min(held, self.max_seq_len)}")
+        vocab = self.shards[0].embed_tokens.weight.shape[0]
+        for n, root in zip(lens, tokens[:, 0].tolist()):
+            if n and not 0 <= root < vocab:
+                raise ValueError(f"a tree's root {root} is no token")
         step = self._trees.get(nodes)
         if step is None:
             step = self._trees[nodes] = _TreeStep(self, nodes)
@@ -637,15 +643,21 @@ class PagedDecodeEngine:
     def generate_drafted(self, prompt_ids: torch.Tensor, max_new_tokens: int, drafter: Optional[Callable] = None,
                          sampling: Optional[Sequence[Sampling]] = None, nodes: int = 8) -> torch.Tensor:
         """``generate``'s tokens with several of them per pass: ``drafter(tokens of a sequence so far) -> (tokens, parents)`` proposes a tree
-        of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``), and ``verify_trees`` checks it."""
+        of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``), and ``verify_trees`` checks it (at the end of
+        ``max_seq_len`` as much of its beginning as there is room for)."""
         B, P = prompt_ids.shape
         drafter = drafter or PromptLookup(nodes)
+        if sampling is not None and len(sampling) != B:
+            raise ValueError("sampling needs settings for every prompt")
         self.set_sampling(sampling)
-        self.allocate(B, P + max_new_tokens + nodes - 1)
+        room = max(P + max_new_tokens, min(P + max_new_tokens + nodes - 1, self.max_seq_len))
+        self.allocate(B, room)
         told = [row + [tok] for row, tok in zip(prompt_ids.tolist(), self.prefill(prompt_ids).tolist())]
         want = P + max_new_tokens
         while any(len(t) < want for t in told):
-            tokens, parents, lens = pad_trees([drafter(t) if len(t) < want else None for t in told], nodes)
+            trees = [drafter(t) if len(t) < want else None for t in told]
+            trees = [tree and tuple(part[:room - len(t) + 1] for part in tree) for tree, t in zip(trees, told)]
+            tokens, parents, lens = pad_trees(trees, nodes)
             count, new = self.verify_trees(torch.from_numpy(tokens), torch.from_numpy(parents), torch.from_numpy(lens))
             for b in range(B):
                 told[b].extend(new[b][:min(count[b], want - len(told[b]))])
@@ -658,6 +670,8 @@ class PagedDecodeEngine:
         identical in every prompt and whose KV blocks should be shared (computed once, reference-counted); with
         ``prefix_cache=True`` they are also kept for later calls, which then skip recomputing them."""
         B, P = prompt_ids.shape
+        if sampling is not None and len(sampling) != B:
+            raise ValueError("sampling needs settings for every prompt")
         self.set_sampling(sampling)
         n_pre = min(shared_prefix_len, P - 1)
         self.allocate(B, P + max_new_tokens, shared_prefix_len=n_pre,

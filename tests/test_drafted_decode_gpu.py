@@ -130,6 +130,61 @@ def test_trees_of_a_16_bit_model_captured_and_not(golden):
     assert out[0] == out[1] and all(len(r) == 48 for r in out[0][0])
 
 
+def test_drafts_that_are_no_tokens(golden):
+    """Drafted numbers outside the vocabulary and whatever stands behind the last node are not taken, and read nothing."""
+    g, cfg, shards = model(golden)
+    prompts, want = torch.tensor(g["prompt_ids"]), g["tokens"]
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=320, prefill_mode="eager")
+    eng.allocate(4, prompts.shape[1] + 20)
+    first = eng.prefill(prompts).cpu()
+    tokens = torch.full((4, 5), -1, dtype=torch.int64)
+    tokens[:, 0] = first
+    tokens[0, 1:] = 10 ** 12
+    tokens[1, 1] = want[1][1]
+    parents = torch.tensor([-1, 0, 1, 0, 90], dtype=torch.int32).expand(4, -1)
+    lens = torch.tensor([5, 2, 1, 0])
+    with pytest.raises(ValueError, match="root"):
+        eng.verify_trees(tokens.roll(1, 1), parents, lens)
+    for on in ("cpu", "cuda"):
+        count, new = eng.verify_trees(tokens.to(on), parents.to(on), lens)
+        assert count == [1, 2, 1, 0]
+        assert [r[:n] for r, n in zip(new, count)] == [want[b][1:1 + n] for b, n in enumerate(count)]
+        eng.allocate(4, prompts.shape[1] + 20)
+        eng.prefill(prompts)
+
+
+def test_trees_at_the_end_of_the_room(golden):
+    g, cfg, shards = model(golden)
+    prompts, want = torch.tensor(g["prompt_ids"]), [t[:40] for t in g["tokens"]]
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=prompts.shape[1] + 40, prefill_mode="eager")
+    know = Knowing([p + t for p, t in zip(g["prompt_ids"], g["tokens"])], 16, 1)
+    assert eng.generate_drafted(prompts, 40, know, nodes=16).tolist() == want
+    assert eng.generate_drafted(prompts, 40, nodes=8).tolist() == want
+    with pytest.raises(ValueError):
+        eng.generate_drafted(prompts, 41, nodes=8)
+
+
+def test_settings_of_fewer_sequences_than_before(golden):
+    g, cfg, shards = model(golden)
+    prompts = torch.tensor(g["prompt_ids"])
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=256, prefill_mode="eager")
+    want = eng.generate(prompts, 10, sampling=SETTINGS)
+    for call in (eng.generate, eng.generate_drafted):
+        with pytest.raises(ValueError):
+            call(prompts, 10, sampling=SETTINGS[:2])
+    eng.set_sampling(SETTINGS)
+    with pytest.raises(ValueError):
+        eng.set_sampling(SETTINGS * 2)
+    assert eng.sampling == SETTINGS
+    eng.set_sampling(SETTINGS[:1])      # the others are greedy from now on
+    eng.allocate(4, prompts.shape[1] + 10)
+    told = [[t] for t in eng.prefill(prompts).tolist()]
+    for _ in range(9):
+        for row, t in zip(told, eng.decode_step(torch.tensor([r[-1] for r in told])).tolist()):
+            row.append(t)
+    assert told[0] == want[0].tolist() and told[1:] == [t[:10] for t in g["tokens"][1:]]
+
+
 def test_refusals(golden):
     g, cfg, shards = model(golden)
     eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=192, prefill_mode="eager")
