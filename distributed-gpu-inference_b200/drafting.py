@@ -16,7 +16,7 @@ import numpy as np
 
 @dataclass(frozen=True)
 class Sampling:
-    """``temperature`` 0: greedy; ``top_k`` 0, ``top_p`` 1, ``min_p`` 0: no limit."""
+    """``temperature`` 0: greedy; ``top_k`` 0, ``top_p`` 1, ``min_p`` 0: no limit; ``seed``: a whole number from 0 on."""
 
     temperature: float = 1.0
     top_k: int = 0
@@ -25,16 +25,21 @@ class Sampling:
     seed: int = 0
 
     def __post_init__(self):
-        if not self.temperature >= 0.0 or self.top_k < 0 or not 0.0 < self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
-            raise ValueError(f"temperature >= 0, top_k >= 0, 0 < top_p <= 1 and 0 <= min_p <= 1 are wanted: {self}")
+        if not self.temperature >= 0.0 or self.top_k < 0 or not 0.0 < self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0 or self.seed < 0:
+            raise ValueError(f"temperature >= 0, top_k >= 0, 0 < top_p <= 1, 0 <= min_p <= 1 and seed >= 0 are wanted: {self}")
 
     @classmethod
     def of_request(cls, params: Dict[str, Any]) -> "Sampling":
-        """From a request's parameters; greedy unless it says ``do_sample``."""
+        """From a request's parameters (absent ones and None: their defaults; without a ``seed`` it is 0, the same tokens each time); greedy unless
+        it says ``do_sample``."""
         if not params.get("do_sample", False):
             return GREEDY
-        return cls(float(params.get("temperature", 0.7)), int(params.get("top_k", 50)), float(params.get("top_p", 0.9)),
-                   float(params.get("min_p", 0.0)), int(params.get("seed", 0)))
+
+        def of(name: str, default):
+            value = params.get(name)
+            return default if value is None else type(default)(value)
+
+        return cls(of("temperature", 0.7), of("top_k", 50), of("top_p", 0.9), of("min_p", 0.0), of("seed", 0))
 
     def numbers(self, n: int) -> np.ndarray:
         """The first ``n`` random numbers of the seed's stream, fp32 in [0, 1)."""
