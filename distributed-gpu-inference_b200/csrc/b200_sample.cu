@@ -1002,7 +1002,7 @@ extern "C" int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64
   const char* name = "b200_sample_rows";
   const int es = dtype_size(dtype);
   if (es == 0) return fail(B200_EINVAL, "%s: unsupported dtype %d", name, dtype);
-  if (rows < 0 || cols <= 0 || row_stride < cols) return fail(B200_EINVAL, "%s: bad sizes", name);
+  if (rows < 0 || cols <= 0 || row_stride < 0) return fail(B200_EINVAL, "%s: bad sizes", name);
   if (cols > B200_MAX_SAMPLE_COLS || rows > (1 << 24)) return fail(B200_ESHAPE, "%s: %lld rows of %lld", name, static_cast<long long>(rows), static_cast<long long>(cols));
   if (rows == 0) return 0;
   if (!out || !x || !u) return fail(B200_EINVAL, "%s: null pointer", name);

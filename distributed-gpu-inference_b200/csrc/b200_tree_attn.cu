@@ -536,7 +536,7 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
           tm_ld16(*reinterpret_cast<float(*)[16]>(s), tm_row + (i & 1) * kKeys + 16 * part);
         }
         tc_wait_ld();
-        if (A.scale <= 0.f) {
+        if (!(A.scale > 0.f)) {
 #pragma unroll
           for (int c = 0; c < kMine; ++c) s[c] *= A.scale * kLog2e;
         }
@@ -709,6 +709,9 @@ tree_attn_kernel(const TreeAttn A, const Shares W, const __grid_constant__ CUten
   }
   tc_fence_before();
   __syncthreads();
+  if (*dead) {      // a wait gave up: what is still under way gets 10 ms to end before its memory is another's
+    for (const long long t0 = clock64(); clock64() - t0 < 20000000ll;) {}
+  }
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(P::kTm));
 }
 

@@ -253,7 +253,7 @@ def argmax_keys_decode(keys: torch.Tensor, out: Optional[torch.Tensor] = None) -
 def _per_row(v, rows: int, dtype: torch.dtype, dev: int, what: str):
     """A setting of ``sample_rows``: ``(pointer or None, number)``."""
     if not isinstance(v, torch.Tensor):
-        return None, v
+        return None, float(v)
     if v.dtype != dtype or v.dim() != 1 or v.numel() != rows or not v.is_contiguous() or v.get_device() != dev:
         raise ValueError(f"{what} must be a number or a contiguous {dtype} [rows] tensor on the logits' device")
     return v.data_ptr(), 0
@@ -261,7 +261,7 @@ def _per_row(v, rows: int, dtype: torch.dtype, dev: int, what: str):
 
 def sample_rows(x: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """A token for each row of logits ``x [rows, cols]`` (contiguous last dim), drawn by the given random numbers ``u`` (fp32 ``[rows]``
+    """A token for each row of logits ``x [rows, cols]`` (contiguous last dim; rows may be the same ones), drawn by the given random numbers ``u`` (fp32 ``[rows]``
     in [0, 1)): the first index at which the weights ``exp((x - max) / temperature)`` that are kept, summed up in the row's order, exceed ``u``
     of their sum.
 
@@ -286,7 +286,7 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         raise ValueError("out must be a contiguous int64 [rows] on the logits' device")
     with _on(dev) as stream:
         rc = _lib.load().b200_sample_rows(out.data_ptr(), x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, u.data_ptr(), tp, t, kp,
-                                          min(max(int(k), 0), 0x7fffffff), pp, p, mp, m, _dtype_id(x), stream)
+                                          int(min(max(k, 0.0), 2147483647.0)), pp, p, mp, m, _dtype_id(x), stream)
     if rc != 0:
         _lib.check(rc, "b200_sample_rows")
     return out
@@ -427,7 +427,7 @@ def accept_drafts(tokens: torch.Tensor, chosen: torch.Tensor, parents: torch.Ten
         raise ValueError("tokens must be int64 [B, nodes]")
     B, nodes = tokens.shape
     device, dev = tokens.device, tokens.get_device()
-    max_blocks, Hkv, bs, D = pool_shape
+    max_blocks, Hkv, bs, D = pool_shape if k_ptrs is not None else (0, 0, 0, 0)
     i32, i64 = torch.int32, torch.int64
     s_tokens = _node_rows(tokens, B, nodes, i64, dev, "tokens")
     s_chosen = _node_rows(chosen, B, nodes, i64, dev, "chosen")

@@ -96,7 +96,7 @@ def test_the_library_refuses():
         assert rc == code and text in lib.b200_last_error()
 
     says(lib.b200_sample_rows(None, None, 2, 8, 8, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 7, None), -1, b"unsupported dtype")
-    says(lib.b200_sample_rows(None, None, 2, 8, 7, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -1, b"bad sizes")
+    says(lib.b200_sample_rows(None, None, 2, 8, -1, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -1, b"bad sizes")
     says(lib.b200_sample_rows(None, None, 2, 8, 8, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -1, b"null pointer")
     says(lib.b200_sample_rows(None, None, 2, (1 << 20) + 1, 1 << 21, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None), -2, b"rows of")
     assert lib.b200_sample_rows(None, None, 0, 8, 8, None, None, 1.0, None, 0, None, 1.0, None, 0.0, 2, None) == 0
@@ -139,12 +139,13 @@ def test_no_cpu_form():
 def test_sampling_settings():
     from dgi_b200.drafting import GREEDY, Sampling, settings
 
-    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(min_p=-0.1), dict(min_p=2.0)):
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(min_p=-0.1), dict(min_p=2.0), dict(seed=-1)):
         with pytest.raises(ValueError):
             Sampling(**bad)
     assert Sampling.of_request({"temperature": 0.3}) == GREEDY
     assert Sampling.of_request({"do_sample": True}) == Sampling(0.7, 50, 0.9, 0.0, 0)
     assert Sampling.of_request({"do_sample": True, "temperature": 1, "top_k": 0, "top_p": 1, "min_p": 0.1, "seed": 4}) == Sampling(1.0, 0, 1.0, 0.1, 4)
+    assert Sampling.of_request({"do_sample": True, "temperature": None, "top_k": None, "top_p": None, "min_p": None, "seed": None}) == Sampling(0.7, 50, 0.9)
     t, k, p, m = settings([GREEDY, Sampling(0.5, 7, 0.9, 0.1)])
     assert t.tolist() == [0.0, 0.5] and k.tolist() == [0, 7] and abs(p[1] - 0.9) < 1e-6 and abs(m[1] - 0.1) < 1e-6
     a = Sampling(seed=3).numbers(100)

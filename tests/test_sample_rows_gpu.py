@@ -174,6 +174,15 @@ def test_numbers_for_all_rows_and_a_row_among_many():
     assert torch.equal(ops.sample_rows(x, u, top_p=nan, min_p=nan), ops.sample_rows(x, u))
 
 
+@pytest.mark.parametrize("cols", [1000, 128256])
+def test_many_tokens_of_one_row(cols):
+    x, _ = logits(1, cols, torch.float32, 21)
+    u = torch.arange(40, device=DEV) / 40
+    assert torch.equal(ops.sample_rows(x.expand(40, -1), u, 0.8, 0, 0.9), ops.sample_rows(x.repeat(40, 1), u, 0.8, 0, 0.9))
+    rows = x[0].as_strided((3, cols - 20), (10, 1))
+    assert torch.equal(ops.sample_rows(rows, u[5:8], np.float32(0.8), np.int32(30)), ops.sample_rows(rows.clone(), u[5:8], 0.8, 30))
+
+
 def test_captured_on_another_stream_and_replayed():
     x, u = logits(6, 4000, torch.bfloat16, 12)
     out = torch.empty(6, dtype=torch.int64, device=DEV)

@@ -173,6 +173,15 @@ def test_large_scores_and_a_maximum_that_grows_along_the_keys():
     check(c)
 
 
+@pytest.mark.parametrize("flags", [0, ops.ATTN_FORCE_GENERIC])
+@pytest.mark.parametrize("nodes", [3, 40])
+def test_a_scale_that_is_no_number(nodes, flags):
+    q, k, v = (torch.randn(s, device="cuda").bfloat16() for s in ((2, nodes, 8, 128), (20, 2, 16, 128), (20, 2, 16, 128)))
+    tables, lens = torch.arange(20, dtype=torch.int32, device="cuda").view(2, 10), torch.tensor([nodes + 70, nodes], dtype=torch.int32, device="cuda")
+    visible, _ = ops.draft_tree(torch.arange(-1, nodes - 1, dtype=torch.int32, device="cuda").expand(2, -1))
+    assert ops.paged_tree_attention(q, k, v, tables, lens, visible, scale=float("nan"), flags=flags).isnan().all()
+
+
 @pytest.mark.parametrize("scale", [-0.1, 0.0])
 @pytest.mark.parametrize("nodes", [3, 12, 40])
 def test_scales_below_and_at_zero(nodes, scale):
