@@ -806,6 +806,11 @@ Shares shares_of(int nodes, int Hq, int Hkv) {
   W.workers = std::max(1, kCtasPerSm * kNumSMs / W.blocks);
   return W;
 }
+// Walks of up to eight tiles are not divided: a second launch costs the host 5 us and the device 2, each tile here one.  (One sequence at 160 behind
+// 8 kv heads of 128, a call after the other: undivided 16.9 us, divided 20.4.)
+bool whole_walks(int B, int nodes, int Hq, int Hkv, int bs, int table_cols) {
+  return static_cast<int64_t>(table_cols) * bs <= B200_TREE_SHORT_KEYS && static_cast<int64_t>(B) * Hkv * shares_of(nodes, Hq, Hkv).blocks <= INT32_MAX;
+}
 size_t sums_bytes(const Shares& W) { return static_cast<size_t>(W.workers) * W.blocks * 2 * W.rows * sizeof(float2); }
 
 bool tiles_serve(int Hq, int Hkv, int D, int bs, int dtype) {
@@ -819,9 +824,7 @@ int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap&
   W.ml = static_cast<float2*>(workspace);
   W.o = reinterpret_cast<float4*>(static_cast<char*>(workspace) + sums_bytes(W));
   const int rows = A.nodes * (A.Hq / A.Hkv);
-  // Walks of up to eight tiles are not divided: a second launch costs the host 5 us and the device 2, each tile here one.  (One sequence at 160 behind
-  // 8 kv heads of 128, a call after the other: undivided 16.9 us, divided 20.4.)
-  W.whole = static_cast<int64_t>(A.table_cols) * A.bs <= 8 * kKeys && static_cast<int64_t>(A.B) * A.Hkv * W.blocks <= INT32_MAX;
+  W.whole = whole_walks(A.B, A.nodes, A.Hq, A.Hkv, A.bs, A.table_cols);
   if (W.whole) W.workers = A.B * A.Hkv;
   auto kern = rows <= 32 ? tree_attn_kernel<T, D, 4> : rows <= 64 ? tree_attn_kernel<T, D, 2> : tree_attn_kernel<T, D, 1>;
   constexpr int smem = Plan<D>::kEnd + 1024;
@@ -894,7 +897,7 @@ int b200_paged_tree_attn(void* out, const void* q, int64_t q_batch_stride, int64
   const bool pieces = aligned16(q) && aligned16(out) && aligned16(k_pool) && aligned16(v_pool) && q_batch_stride % 8 == 0 && q_node_stride % 8 == 0;
   if (tiles_serve(Hq, Hkv, D, block_size, dtype) && !(flags & B200_ATTN_FORCE_GENERIC) && pieces && max_blocks < INT32_MAX / (static_cast<int64_t>(Hkv) * block_size) - 1 &&
       (static_cast<int64_t>(table_cols) * block_size / kKeys + 1) * B < INT32_MAX / Hkv - 1024 && nodes * static_cast<int64_t>(Hq / Hkv) <= 32 * 65535) {
-    if (!workspace || workspace_bytes < b200_paged_tree_attn_workspace(B, nodes, Hq, Hkv, D, block_size, dtype))
+    if (workspace ? workspace_bytes < b200_paged_tree_attn_workspace(B, nodes, Hq, Hkv, D, block_size, dtype) : !whole_walks(B, nodes, Hq, Hkv, block_size, table_cols))
       return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace_bytes);
     if (!aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
     CUtensorMap k_map, v_map;

@@ -293,6 +293,7 @@ def sample_rows(x: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 
 
 MAX_DRAFT_NODES = 64
+TREE_SHORT_KEYS = 512      # block tables of up to this many tokens take no workspace
 
 
 def _node_rows(t: torch.Tensor, B: int, nodes: int, dtype: torch.dtype, dev: int, what: str) -> int:
@@ -365,7 +366,8 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     ``context_lens int32 [B]`` counting the drafted tokens, ``draft_lens int32 [B]`` (None: ``nodes`` everywhere) how many they are.  A node sees
     the context and the drafted tokens of its mask ``visible`` (int64 ``[B, nodes]``, as ``draft_tree`` gives it, or any other).  Rows behind a
     sequence's last node, and rows that see nothing, come out as 0.  Returns ``[B, nodes, Hq, D]`` (``out``, where given).  ``workspace``: at
-    least ``tree_attention_workspace`` bytes that no call running at the same time uses; else one from torch's caching allocator."""
+    least ``tree_attention_workspace`` bytes that no call running at the same time uses; else one from torch's caching allocator (none for tables of
+    up to ``TREE_SHORT_KEYS`` tokens)."""
     _need_cuda(q, k_pool, v_pool, block_tables, context_lens, visible)
     max_blocks, Hkv, bs, D = _pool_dims(k_pool)
     dev, dtype = q.get_device(), q.dtype
@@ -398,7 +400,7 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         if workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous, on q's device")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    elif need:
+    elif need and table_cols * bs > TREE_SHORT_KEYS:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         ws, ws_bytes = workspace.data_ptr(), need
     with _timed(), _on(dev) as stream:

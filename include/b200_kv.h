@@ -297,6 +297,7 @@ int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64_t cols, in
  * every row sees, may come out as NaN).  A table entry outside
  * the pool reads as zeros.  At most table_cols pages of a sequence are read.  q: [B, nodes, Hq, D], rows of a node contiguous; out contiguous.
  *   workspace : b200_paged_tree_attn_workspace bytes, 16-byte aligned, any contents; calls that may run at the same time need their own.
+ *               NULL will do where table_cols pages hold up to B200_TREE_SHORT_KEYS tokens.
  *
  * b200_accept_drafts: node t fits if its token is chosen[b, parent] (the first of siblings with the same token), and is taken if all of
  * visible[b, t] fits.  count[b]: taken nodes, the root among them; path[b, k] the k-th, -1 behind the last; new_tokens[b, k] = chosen[b, path[b, k]],
@@ -305,6 +306,7 @@ int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64_t cols, in
  *   sequence, and no pool stands twice in a call but for values that are a layer's keys.
  */
 #define B200_MAX_DRAFT_NODES 64
+#define B200_TREE_SHORT_KEYS 512
 int b200_draft_tree(int64_t* visible, int32_t* depth, const int32_t* parents, int64_t parent_stride, const int32_t* draft_lens, int B,
                     int nodes, void* stream);
 size_t b200_paged_tree_attn_workspace(int B, int nodes, int Hq, int Hkv, int D, int block_size, int dtype);
