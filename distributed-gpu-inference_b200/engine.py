@@ -75,6 +75,9 @@ class _TreeStep:
         self.count.copy_(out[0])
         self.new.copy_(out[2])
         context.copy_(out[3])
+        # steps that stay on the device go on from a sequence's last new token
+        last = out[2].gather(1, (out[0].to(torch.int64) - 1).clamp(min=0)[:, None])
+        e.ids_buf[:B].copy_(torch.where(out[0][:, None] > 0, last, e.ids_buf[:B]))
 
     def run(self, tokens: torch.Tensor, parents: torch.Tensor, lens: List[int]) -> Tuple[List[int], List[List[int]]]:
         e = self.e
@@ -614,7 +617,8 @@ class PagedDecodeEngine:
         ``tokens`` int64 and ``parents`` int32 ``[batch, nodes]`` (host or device): node 0 is the sequence's last token, which no step has
         seen yet, the others come behind their parents; ``draft_lens`` int32 ``[batch]`` how many nodes a sequence has (0: it rests).  The
         model runs once over all nodes (a token outside its vocabulary is never taken); the nodes whose tokens are the model's own choices stay in the cache, side by side behind the context,
-        and a sequence gets ``count`` new tokens: one for each of them.  The choices are the ones that single steps would have made."""
+        and a sequence gets ``count`` new tokens: one for each of them, the last of them where ``decode_step_device`` goes on.  The choices are the
+        ones that single steps would have made."""
         if not (self.is_first and self.is_last) or self.external_head:
             raise RuntimeError("verify_trees() drives a whole model")
         B = self.batch

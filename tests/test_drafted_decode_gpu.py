@@ -130,6 +130,30 @@ def test_trees_of_a_16_bit_model_captured_and_not(golden):
     assert out[0] == out[1] and all(len(r) == 48 for r in out[0][0])
 
 
+@pytest.mark.parametrize("graph", [True, False])
+def test_behind_a_shared_prefix_and_steps_on_the_device(golden, graph):
+    """Prompts whose first blocks are one sequence's; after a pass over trees steps go on where it ended."""
+    g, cfg, shards = model(golden)
+    head = g["prompt_ids"][0][:32]
+    prompts = torch.tensor([head + p[:9] for p in g["prompt_ids"]])
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=256, prefill_mode="eager", use_cuda_graph=graph)
+    want = eng.generate(prompts, 30)
+    rows = [p + t for p, t in zip(prompts.tolist(), want.tolist())]
+    eng.allocate(4, prompts.shape[1] + 40, shared_prefix_len=32)
+    told = [r + [t] for r, t in zip(prompts.tolist(), eng.prefill(prompts).tolist())]
+    know = Knowing(rows, 9, 4)
+    for rest in (None, 2):
+        trees = [None if b == rest else know(t) for b, t in enumerate(told)]
+        count, new = eng.verify_trees(*(torch.from_numpy(x) for x in pad_trees(trees, 9)))
+        for b in range(4):
+            told[b] += new[b][:count[b]]
+    for _ in range(5):
+        eng.decode_step_device()
+        for b, t in enumerate(eng.next_tokens[:4].tolist()):
+            told[b].append(t)
+    assert all(t == r[:len(t)] for t, r in zip(told, rows)) and min(map(len, told)) >= prompts.shape[1] + 7
+
+
 def test_drafts_that_are_no_tokens(golden):
     """Drafted numbers outside the vocabulary and whatever stands behind the last node are not taken, and read nothing."""
     g, cfg, shards = model(golden)
