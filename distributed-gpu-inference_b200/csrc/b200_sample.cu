@@ -12,8 +12,8 @@
 // table, a polynomial of degree 3 between them, after Tang's table-driven exponential; set to its exponent and rounded by the double unit, which has
 // nothing else to do): errors of independent weights leave one token in 10^7 rows of 128 k another one than 64 bits would.
 //
-// A row has a cluster of CTAs; each holds its part of the row in shared memory from the only pass over it in memory, if the parts fit.  Blocks of 256
-// elements, eight side by side per lane.
+// A row has a cluster of CTAs; each holds its part of the row in shared memory from the only pass over it in memory, if the parts fit; else its three passes
+// read it from memory.  Blocks of 256 elements, eight side by side per lane.
 //   all rows        load, maximum
 //   k, or p         numbers of elements in 1024 ranges of log w (0 .. -46).  k: all elements down to the range that the k-th is in go in a list; p: from
 //                   these, to first order in where the elements lie in their ranges, it is known to some 10^-4 where the weights sum to p of all, the elements of these ranges go in
@@ -22,6 +22,10 @@
 //   other rows      kept weights of each block; the block, the lane and the element in which u falls
 // Where that does not serve - k over 2048, or ranges of more than 4096 elements, equal logits above all - the last key is found by its digits of 8 bits
 // from counts or sums in the whole row.
+//
+// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.6 us on the
+// device; 64 rows of settings of their own 51, the rows without k the longest); many rows by the instructions of the exact weights, about a hundred per element
+// in all passes (256 rows of 128256 in 32 bits, p 0.9 with thousands of tokens kept: 144 us; their bytes take 20, read three times 60).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -957,8 +961,9 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
     return sizeof(Shared) + ((per + 1) & ~size_t{1}) * 8 + (held ? per * kBlock * sizeof(T) : 0);
   };
   // Two CTAs per SM.  As many for a row as the rows leave room for in one round, each with a part worth a cluster's barriers (1500 clocks each); the parts
-  // stay in shared memory if they fit, else they are read again, from the second level of the cache for the most part.  (Rows cut until they fit, in seven
-  // rounds: 256 rows of 128 k in 32 bits 288 us, against %s.)
+  // stay in shared memory if they fit, else they are read again.  (256 rows of 128 k in 32 bits, a call after the other: 160 us; cut until they fit, in
+  // seven rounds of CTAs, 288; every other pass backwards, for what the cache still holds, 162.  37 rows of 32003 in 16 bits: 12.3 us by four CTAs each,
+  // 16.8 by eight.)
   constexpr size_t kHalf = 113 * 1024;
   int ctas = 1;
   while (ctas < kMostCtas && (blocks > kMostBlocks * ctas || (2 * ctas * static_cast<int64_t>(rows) <= (blocks >= 128 * ctas ? 2 : 1) * kNumSMs && blocks >= 16 * ctas))) ctas *= 2;
