@@ -23,9 +23,9 @@
 // Where that does not serve - k over 2048, or ranges of more than 4096 elements, equal logits above all - the last key is found by its digits of 8 bits
 // from counts or sums in the whole row.
 //
-// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.6 us on the
-// device; 64 rows of settings of their own 51, the rows without k the longest); many rows by the instructions of the exact weights, about a hundred per element
-// in all passes (256 rows of 128256 in 32 bits, p 0.9 with thousands of tokens kept: 144 us; their bytes take 20, read three times 60).
+// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.2 us on the
+// device; 64 rows of settings of their own 49, the rows without k the longest); many rows by the instructions of the exact weights, about ninety per element
+// in all passes (256 rows of 128256 in 32 bits, p 0.9 with thousands of tokens kept: 138 us; their bytes take 20, read three times 60).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -173,22 +173,23 @@ static_assert(kBins + 2 * kFew <= kRanges, "room for bins and a bin's elements")
 // weights: multiples of 2^-frac
 template <typename T>
 struct Weigh {
-  float top, scale, scale_low;          // maximum; 256 log2(e) / t in two parts
-  float lowest, floor;                  // arguments from `lowest` on down give 0, those below `floor` count as it
+  // An argument is (x - off) scale - c, scale = 256 log2(e) / t, c = (max - off) scale, each in two parts; one product less than a whole number near it,
+  // in one rounding, is what the polynomial takes.  16-bit types: off = max, c = 0 (a difference that matters is exact).  32 bits: off = 0, and c a
+  // multiple of 2^-5 with a rest; where c passes 2^18, off = max, for then what matters is within a twentieth of the maximum, and exact too.
+  float off, scale, scale_low, c, c_low;
+  float floor, end;                     // arguments below `floor` count as it; steps from `end` on give 0
   double one;                           // 2^(52 - frac), whose last bit is 2^-frac
   const uint2* table;
-  __device__ __forceinline__ float argument(float x) const { return __fmul_rn(x - top, scale); }
-  __device__ __forceinline__ bool some(float y) const { return y > lowest; }        // not of no number: -inf without a scale
+  __device__ __forceinline__ float argument(float x) const {
+    if constexpr (sizeof(T) == 4) return fmaf(x - off, scale, -c);
+    else return __fmul_rn(x - off, scale);
+  }
   __device__ __forceinline__ double operator()(float x) const {
-    const float d = x - top, y = __fmul_rn(d, scale);
-    float low = fmaf(d, scale_low, fmaf(d, scale, -y));
-    if constexpr (sizeof(T) == 4) {     // what the difference lost (Knuth's sum); one of 16-bit numbers that matters loses nothing
-      const float v = d - x;
-      low = fmaf((x - (d - v)) - (top + v), scale, low);
-    }
-    const float shift = 12582912.f, z = fmaxf(y, floor), r = z + shift;        // 3 * 2^22: the nearest whole number n is in the last bits
+    const float d = x - off, shift = 12582912.f, r = fmaxf(argument(x), floor) + shift;        // 3 * 2^22: the nearest whole number n is in the last bits
     const uint32_t n = __float_as_uint(r);
-    const float f = (z - (r - shift)) + low;        // (below the floor no number or any: 2^-50 of 32 bits is 0 all the same)
+    float f;        // (below the floor no number or any: 2^-50 of 32 bits is 0 all the same)
+    if constexpr (sizeof(T) == 4) f = fmaf(d, scale, -(c + (r - shift))) + fmaf(d, scale_low, -c_low);
+    else f = fmaf(d, scale_low, fmaf(d, scale, -(r - shift)));
     constexpr float c1 = 0.69314718055994530942 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
     const uint2 step = table[n & 255];
     const float q = f * fmaf(fmaf(f, c3, c2), f, c1);
@@ -198,7 +199,7 @@ struct Weigh {
   }
   __device__ __forceinline__ u64 whole(double w) const { return __double_as_longlong(w + one) - __double_as_longlong(one); }      // w < one
   __device__ __forceinline__ u64 number(float x) const { return whole((*this)(x)); }
-  // place of an argument, in steps
+  // place of an argument, in steps; none of no number (-inf without a scale)
   __device__ __forceinline__ float steps(float y) const { return fmaf(y, -(1 << kStepBits) / kRange, 8388608.f); }
 };
 
@@ -409,11 +410,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   Weigh<T> weigh;
   {
     const double scale = 369.32993046757463 / static_cast<double>(t);     // 256 log2(e)
-    weigh.top = top;
     weigh.scale = static_cast<float>(fmin(scale, 3e38));
     weigh.scale_low = scale < 3e38 ? static_cast<float>(scale - weigh.scale) : 0.f;
-    weigh.lowest = -256.0f * (A.frac + 1);
+    const double c = static_cast<double>(top) * (static_cast<double>(weigh.scale) + static_cast<double>(weigh.scale_low));
+    const bool apart = sizeof(T) == 4 && fabs(c) <= 262144.0;
+    weigh.off = apart ? 0.f : top;
+    weigh.c = apart ? static_cast<float>(rint(c * 32.0) / 32.0) : 0.f;
+    weigh.c_low = apart ? static_cast<float>(c - static_cast<double>(weigh.c)) : 0.f;
     weigh.floor = -256.0f * (A.frac + 8);
+    weigh.end = weigh.steps(-256.0f * (A.frac + 1)) + 1.f;
     weigh.one = __hiloint2double((1023 + 52 - A.frac) << 20, 0);
     weigh.table = S.table;
   }
@@ -437,9 +442,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     each_block([&](int, const Eight<T>& v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = weigh.argument(value<T>(v[e]));
-        if (weigh.some(y)) {
-          const uint32_t at = __float_as_uint(weigh.steps(y)) & 0x7fffffu;
+        const float step = weigh.steps(weigh.argument(value<T>(v[e])));
+        if (step < weigh.end) {
+          const uint32_t at = __float_as_uint(step) & 0x7fffffu;
           atomicAdd(&S.ranges[(at >> kStepBits) * kRangeColumns + (lane & (kRangeColumns - 1))], 1u << kCountShift | (at & ((1 << kStepBits) - 1)));
         }
       }
@@ -515,15 +520,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
     if (listing <= kList) {       // (the same in all CTAs)
       // ---- the list; a row without k: exact sums of all, of what is above the list, and of the blocks' part of that ------------------------------
       double all = 0, above = 0;
-      const float from_step = 8388608.f + (from << kStepBits), to_step = 8388608.f + ((to + 1) << kStepBits);
+      const float from_step = 8388608.f + (from << kStepBits), to_step = fminf(8388608.f + ((to + 1) << kStepBits), weigh.end);
       auto gather = [&](auto sums, auto limited) {
         each_block([&](int b, const Eight<T>& v) {
           double sum = 0;
           unsigned hits = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float f = value<T>(v[e]), y = weigh.argument(f), step = weigh.steps(y);
-            if (step >= from_step && step < to_step && weigh.some(y)) hits |= 1u << e;
+            const float f = value<T>(v[e]), step = weigh.steps(weigh.argument(f));
+            if (step >= from_step && step < to_step) hits |= 1u << e;
             if constexpr (decltype(sums)::value) {
               const double w = weigh(f);
               all += w;
@@ -961,8 +966,8 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
     return sizeof(Shared) + ((per + 1) & ~size_t{1}) * 8 + (held ? per * kBlock * sizeof(T) : 0);
   };
   // Two CTAs per SM.  As many for a row as the rows leave room for in one round, each with a part worth a cluster's barriers (1500 clocks each); the parts
-  // stay in shared memory if they fit, else they are read again.  (256 rows of 128 k in 32 bits, a call after the other: 160 us; cut until they fit, in
-  // seven rounds of CTAs, 288; every other pass backwards, for what the cache still holds, 162.  37 rows of 32003 in 16 bits: 12.3 us by four CTAs each,
+  // stay in shared memory if they fit, else they are read again.  (256 rows of 128 k in 32 bits, a call after the other: 154 us; with more instructions a
+  // weight 160; then cut until they fit, in seven rounds of CTAs, 288; every other pass backwards, for what the cache still holds, 162.  37 rows of 32003 in 16 bits: 12.3 us by four CTAs each,
   // 16.8 by eight.)
   constexpr size_t kHalf = 113 * 1024;
   int ctas = 1;

@@ -147,6 +147,21 @@ def test_temperatures_at_the_ends(t):
     check(x, u, [(t, 0, 1.0, 0.0), (t, 9, 1.0, 0.0), (t, 0, 0.9, 0.0), (t, 0, 1.0, 0.1)])
 
 
+@pytest.mark.parametrize("offset", [0.0, 7.0, -40.0, 330.0, 709.0, 711.0, -700.0, -730.0, 12000.0, -3e6, 1e30])
+def test_logits_far_from_zero(offset):
+    """Weights are of differences, wherever the logits lie; the largest weight is 1."""
+    x, u = logits(24, 3001, torch.float32, 31)
+    x += offset
+    check(x, u, [((0.05, 0.37, 1.0, 3.3)[i % 4], (0, 50)[i // 4 % 2], (1.0, 0.9)[i // 8 % 2], (0.0, 0.01, 1.0)[i // 8]) for i in range(24)])
+
+
+def test_only_the_largest_weight_is_one():
+    x, u = logits(400, 700, torch.float32, 32)
+    x *= torch.logspace(-3, 3, 400, device=DEV)[:, None]
+    t = torch.logspace(-2, 2, 400, device=DEV)[torch.randperm(400, device=DEV)]
+    assert torch.equal(ops.sample_rows(x, u, t, min_p=1.0), ops.argmax_rows(x))
+
+
 def test_every_token_gets_its_share():
     """Numbers one step apart: a token of probability p is drawn n p times, to within one (its part of [0, 1) holds the steps that fit)."""
     n, cols = 4096, 50
