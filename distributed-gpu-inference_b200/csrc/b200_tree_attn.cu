@@ -1,6 +1,8 @@
 // Attention of a tree of drafted tokens over the paged cache: each node sees the context and the nodes of its mask.
 //
 //   out[t, h] = sum_j w_j v_j / sum_j w_j,   w_j = exp(q[t, h] k_j scale - max),   j in the context, or bit j of visible[t]
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -34,8 +36,8 @@ __device__ __forceinline__ void lengths(const TreeAttn& A, int b, int* keys, int
 // ---- any type, head size and page size ------------------------------------------------------------------------------------------------------
 // One CTA per (sequence, node, query head); its warps take 32 keys in turns, a lane a key for the scores and a part of the columns for the
 // output, and put their maxima, sums and outputs together at the end.  Bound by the loads' latency: 4 sequences x 13 nodes x 8 heads of 64 at 160 keys
-// in fp32 14 us on the device (four warps, eight rows of values under way: 20).  Serves what the kernel below does not (fp32, head sizes other than 64 and
-// 128, pages that do not divide 64 keys).
+// in fp32 14 us on the device (four warps, eight rows of values under way: 20).  Serves what neither kernel below does: few rows behind short tables, rows
+// that are not of 16-byte pieces.
 constexpr int kAnyWarps = 8, kAnyMostD = 256;
 
 template <typename T, int COLS>
@@ -122,6 +124,231 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_attn_any_kernel(const Tre
     for (int w = 0; w < kAnyWarps; ++w) o = fmaf(out_s[w][d], k[w], o);
     out[d] = Cvt<T>::from_f32(sum == 0.f ? 0.f : o / sum);
   }
+}
+
+// The same for many keys: a CTA per (sequence, kv head, block of R = 8 RW rows) - or a cluster of them with a part of the keys each, where there are few -
+// walks tiles of KT keys that its copies bring to shared memory as they are.  A warp has RW rows, a lane KT / 32 keys of each for the scores; for the output
+// a thread has two columns of some rows.  The next tile's keys are under way while this one's weights meet its values, and the values while the next scores are
+// formed.  fp32 arithmetic without tensor cores; bound by shared memory, 12 wavefronts for 32 products a lane at RW = 4: 4 sequences x 64 nodes x 32 heads over 8
+// of 128 at 4k in fp32 746 us, three times what the products alone take at 70 TFLOP/s (each row by itself: 5470).  Values of drafted tokens count only where their weight is not 0.
+template <typename T, int DM, int RW>
+struct RowsPlan {
+  static constexpr int kTile = DM == 256 ? 32 : 64, kRowsOf = 8 * RW;
+  static constexpr int kKeyRow = DM * sizeof(T) + 16, kWeightRow = kRowsOf + 4;      // bytes; numbers
+  static constexpr int kK = 0, kV = kK + kTile * kKeyRow, kQ = kV + kTile * DM * static_cast<int>(sizeof(T)), kP = kQ + kRowsOf * DM * 4,
+                       kStats = kP + kTile * kWeightRow * 4, kPlaces = kStats + 3 * kRowsOf * 4 + (kRowsOf * 4 % 8), kEnd = kPlaces + 2 * kTile * 8;
+  static_assert(kQ >= kRowsOf * DM * 4, "outputs go where keys and values were");
+  static_assert(kPlaces % 8 == 0 && kP % 16 == 0 && kV % 16 == 0 && kQ % 16 == 0, "alignment");
+};
+
+// 16 bytes as numbers
+template <typename T>
+__device__ __forceinline__ void numbers_of(const int4& raw, float* to) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int u = 0; u < static_cast<int>(16 / sizeof(T)); ++u) to[u] = Cvt<T>::to_f32(e[u]);
+}
+
+template <typename T, int DM, int RW>
+__global__ void __launch_bounds__(256, 2) tree_attn_rows_kernel(const TreeAttn A, int blocks) {
+  using P = RowsPlan<T, DM, RW>;
+  constexpr int KT = P::kTile, R = P::kRowsOf, KPL = KT / 32, kVec = 16 / sizeof(T), kGroups = 512 / DM, RG = R / kGroups > 0 ? R / kGroups : 1;
+  extern __shared__ __align__(16) unsigned char sm[];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int unit = blockIdx.x / ctas, block = unit % blocks, b = unit / blocks / A.Hkv, g = unit / blocks - b * A.Hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rep = A.Hq / A.Hkv, row0 = block * R, rows = A.nodes * rep;
+  int keys, n;
+  lengths(A, b, &keys, &n);
+  auto place_out = [&](int row) { return (static_cast<int64_t>(b) * A.nodes + row / rep) * A.Hq + g * rep + row % rep; };
+  T* out = static_cast<T*>(A.out);
+  if (row0 >= n * rep) {        // (the same in the cluster)
+    for (int r = rank; r < min(R, rows - row0); r += ctas)
+      for (int d = tid; d < A.D; d += blockDim.x) out[place_out(row0 + r) * A.D + d] = Cvt<T>::from_f32(0.f);
+    return;
+  }
+  float* q_s = reinterpret_cast<float*>(sm + P::kQ);
+  float* p_s = reinterpret_cast<float*>(sm + P::kP);
+  float *corr_s = reinterpret_cast<float*>(sm + P::kStats), *m_s = corr_s + R, *l_s = m_s + R;
+  int64_t* places = reinterpret_cast<int64_t*>(sm + P::kPlaces);
+  const int tiles = (keys + KT - 1) / KT, per = (tiles + ctas - 1) / ctas, t0 = min(rank * per, tiles), t1 = min(t0 + per, tiles), base = keys - n;
+
+  auto look_up = [&](int tile) {        // element of the pools; outside them, and behind the last key: zeros
+    if (tid < KT) {
+      const int j = tile * KT + tid;
+      int64_t at = -1;
+      if (j < keys) {
+        const int64_t page = A.block_tables[static_cast<int64_t>(b) * A.table_stride + j / A.bs];
+        if (page >= 0 && page < A.max_blocks) at = ((page * A.Hkv + g) * A.bs + j % A.bs) * A.D;
+      }
+      places[(tile & 1) * KT + tid] = at;
+    }
+  };
+  auto copy = [&](int tile, const void* pool, uint32_t to, int row_bytes) {
+    constexpr int kCh = DM / kVec;
+    const int ch_of = A.D / kVec;
+    for (int c = tid; c < KT * kCh; c += 256) {
+      const int key = c / kCh, ch = c % kCh;
+      const int64_t at = places[(tile & 1) * KT + key];
+      if (ch < ch_of) cp16(to + key * row_bytes + ch * 16, static_cast<const T*>(pool) + (at >= 0 ? at + ch * kVec : 0), at >= 0);
+    }
+  };
+  const uint32_t k_at = smem_u32(sm + P::kK), v_at = smem_u32(sm + P::kV);
+  look_up(t0);
+  look_up(t0 + 1);
+  __syncthreads();
+  if (t0 < t1) copy(t0, A.k_pool, k_at, P::kKeyRow);
+  cp_commit();
+  if (t0 < t1) copy(t0, A.v_pool, v_at, DM * sizeof(T));
+  cp_commit();
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int r = warp * RW + i, row = row0 + r, t = row / rep;
+    const T* q = static_cast<const T*>(A.q) + b * A.q_batch_stride + t * A.q_node_stride + static_cast<int64_t>(g * rep + row - t * rep) * A.D;
+#pragma unroll
+    for (int d = lane; d < DM; d += 32) q_s[r * DM + d] = d < A.D && t < n ? Cvt<T>::to_f32(q[d]) * A.scale : 0.f;
+  }
+  uint64_t seen[RW];
+  bool live[RW];
+  float m[RW], l[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const int t = (row0 + warp * RW + r) / rep;
+    live[r] = t < n;
+    seen[r] = live[r] ? static_cast<uint64_t>(A.visible[b * A.visible_stride + t]) : 0ull;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+  }
+  const int pair = tid % (DM / 2), first = tid / (DM / 2) * RG;        // columns 2 pair, 2 pair + 1 of rows first ..
+  const bool mine = first < R;
+  float acc[RG][2] = {};
+  for (int tile = t0; tile < t1; ++tile) {
+    cp_wait<1>();
+    __syncthreads();
+    float s[RW][KPL] = {};
+    const int4* k_row[KPL];
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) k_row[i] = reinterpret_cast<const int4*>(sm + P::kK + (i * 32 + lane) * P::kKeyRow);
+#pragma unroll 4
+    for (int d = 0; d < A.D; d += kVec) {
+      float k[KPL][kVec];
+#pragma unroll
+      for (int i = 0; i < KPL; ++i) numbers_of<T>(k_row[i][d / kVec], k[i]);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+#pragma unroll
+        for (int u = 0; u < kVec; u += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(q_s + (warp * RW + r) * DM + d + u);
+#pragma unroll
+          for (int i = 0; i < KPL; ++i) s[r][i] = fmaf(q.x, k[i][u], fmaf(q.y, k[i][u + 1], fmaf(q.z, k[i][u + 2], fmaf(q.w, k[i][u + 3], s[r][i]))));
+        }
+      }
+    }
+    float p[KPL][RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      bool sees[KPL];
+      float top = m[r];
+#pragma unroll
+      for (int i = 0; i < KPL; ++i) {
+        const int j = tile * KT + i * 32 + lane;
+        sees[i] = live[r] && j < keys && (j < base || (seen[r] >> (j - base) & 1));
+        top = fmaxf(top, sees[i] ? s[r][i] : -INFINITY);
+      }
+      top = warp_max(top);
+      const float from = top == -INFINITY ? 0.f : top, corr = m[r] == -INFINITY ? 0.f : expf(m[r] - from);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < KPL; ++i) {
+        p[i][r] = sees[i] ? expf(s[r][i] - from) : 0.f;
+        sum += p[i][r];
+      }
+      l[r] = fmaf(l[r], corr, warp_sum(sum));
+      m[r] = top;
+      if (lane == 0) corr_s[warp * RW + r] = corr;
+    }
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+      float* to = p_s + (i * 32 + lane) * P::kWeightRow + warp * RW;
+      if constexpr (RW == 4) *reinterpret_cast<float4*>(to) = make_float4(p[i][0], p[i][1], p[i][2], p[i][3]);
+      else
+#pragma unroll
+        for (int r = 0; r < RW; ++r) to[r] = p[i][r];
+    }
+    if (tile + 1 < t1) look_up(tile + 2);
+    __syncthreads();
+    if (tile + 1 < t1) copy(tile + 1, A.k_pool, k_at, P::kKeyRow);
+    cp_commit();
+    cp_wait<1>();
+    __syncthreads();
+    if (mine) {
+#pragma unroll
+      for (int r = 0; r < RG; ++r) {
+        const float corr = corr_s[first + r];
+        acc[r][0] *= corr;
+        acc[r][1] *= corr;
+      }
+      auto weigh = [&](auto drafted) {
+#pragma unroll 4
+        for (int key = 0; key < KT; ++key) {
+          float v[2], w[RG];
+          const T* e = reinterpret_cast<const T*>(sm + P::kV) + key * DM + 2 * pair;
+          if constexpr (sizeof(T) == 4) {
+            const float2 two = *reinterpret_cast<const float2*>(e);
+            v[0] = two.x, v[1] = two.y;
+          } else {
+            const uint32_t two = *reinterpret_cast<const uint32_t*>(e);
+            const T* h = reinterpret_cast<const T*>(&two);
+            v[0] = Cvt<T>::to_f32(h[0]), v[1] = Cvt<T>::to_f32(h[1]);
+          }
+          const float* from = p_s + key * P::kWeightRow + first;
+#pragma unroll
+          for (int r = 0; r < RG; ++r) w[r] = from[r];
+#pragma unroll
+          for (int r = 0; r < RG; ++r) {
+            const bool counts = !decltype(drafted)::value || w[r] != 0.f;
+            acc[r][0] = fmaf(w[r], counts ? v[0] : 0.f, acc[r][0]);
+            acc[r][1] = fmaf(w[r], counts ? v[1] : 0.f, acc[r][1]);
+          }
+        }
+      };
+      if (tile * KT + KT > base) weigh(std::true_type{});
+      else weigh(std::false_type{});
+    }
+    __syncthreads();
+    if (tile + 1 < t1) copy(tile + 1, A.v_pool, v_at, DM * sizeof(T));
+    cp_commit();
+  }
+  // ---- outputs, of the cluster's parts of the keys -------------------------------------------------------------------------------------------
+  cp_wait<0>();
+  __syncthreads();
+  if (lane == 0) {
+#pragma unroll
+    for (int r = 0; r < RW; ++r) m_s[warp * RW + r] = m[r], l_s[warp * RW + r] = l[r];
+  }
+  float* o_s = reinterpret_cast<float*>(sm);
+  if (mine) {
+#pragma unroll
+    for (int r = 0; r < RG; ++r) *reinterpret_cast<float2*>(o_s + (first + r) * DM + 2 * pair) = make_float2(acc[r][0], acc[r][1]);
+  }
+  cluster.sync();
+  for (int r = rank + ctas * warp; r < min(R, rows - row0); r += ctas * 8) {        // a warp a row, a lane a CTA's part of it
+    const float mc = lane < ctas ? *cluster.map_shared_rank(m_s + r, lane) : -INFINITY, lc = lane < ctas ? *cluster.map_shared_rank(l_s + r, lane) : 0.f;
+    const float top = warp_max(mc), k = mc == -INFINITY ? (lc != lc ? 1.f : 0.f) : expf(mc - top), sum = warp_sum(lc * k);
+    T* to = out + place_out(row0 + r) * A.D;
+#pragma unroll
+    for (int d0 = 0; d0 < DM; d0 += 32) {
+      float o = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float kc = __shfl_sync(0xffffffffu, k, c);
+        if (c < ctas) o = fmaf(*cluster.map_shared_rank(o_s + r * DM + d0 + lane, c), kc, o);
+      }
+      if (d0 + lane < A.D) to[d0 + lane] = Cvt<T>::from_f32(sum == 0.f ? 0.f : o / sum);
+    }
+  }
+  cluster.sync();       // the others may still read this CTA's
 }
 
 // ---- 16-bit types, heads of 64 or 128, pages that divide 64 keys (or are multiples of 64) ------------------------------------------------------
@@ -860,11 +1087,53 @@ int launch_tiles(const TreeAttn& A, const CUtensorMap& k_map, const CUtensorMap&
   return 0;
 }
 
+// Rows share their keys where block tables hold more tokens than this, or where there are more rows in all.  (fp32, heads of 64, 1 x 8 rows behind 200 / 400 /
+// 800 / 1600 tokens: each by itself 9 / 14 / 26 / 43 us, sharing 10 / 16 / 16 / 16; 416 rows 14 / 23 / 42 / 75 and 16 / 25 / 24 / 33; 2048 rows behind 30: 32
+// and 13, behind 1600: 340 and 54.)
+constexpr int kRowsFromTokens = 512, kRowsFromRows = 1024;
+
+template <typename T, int DM, int RW>
+int launch_rows(const TreeAttn& A, cudaStream_t stream) {
+  using P = RowsPlan<T, DM, RW>;
+  const char* name = "b200_paged_tree_attn";
+  const int blocks = (A.nodes * (A.Hq / A.Hkv) + P::kRowsOf - 1) / P::kRowsOf;
+  const int64_t units = static_cast<int64_t>(A.B) * A.Hkv * blocks, tiles = (static_cast<int64_t>(A.table_cols) * A.bs + P::kTile - 1) / P::kTile;
+  int ctas = 1;
+  while (ctas < 8 && units * ctas * 2 <= 2 * kNumSMs && tiles >= ctas * 4) ctas *= 2;
+  if (units * ctas > INT32_MAX) return fail(B200_ESHAPE, "%s: %d sequences", name, A.B);
+  auto kern = tree_attn_rows_kernel<T, DM, RW>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kEnd);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * ctas));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = P::kEnd;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, A, blocks);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
+  }
+  return 0;
+}
+template <typename T, int DM>
+int launch_rows_of(const TreeAttn& A, cudaStream_t stream) {
+  const int rows = A.nodes * (A.Hq / A.Hkv);
+  return rows <= 8 ? launch_rows<T, DM, 1>(A, stream) : rows <= 16 ? launch_rows<T, DM, 2>(A, stream) : launch_rows<T, DM, 4>(A, stream);
+}
+
 template <typename T>
 int launch_any(const TreeAttn& A, cudaStream_t stream) {
   if (A.D > kAnyMostD) return fail(B200_ESHAPE, "b200_paged_tree_attn: head size %d, at most %d", A.D, kAnyMostD);
-  if (A.B > 65535) return fail(B200_ESHAPE, "b200_paged_tree_attn: %d sequences", A.B);
   const bool vec = A.D * sizeof(T) % 16 == 0 && aligned16(A.k_pool);
+  if (vec && aligned16(A.v_pool) && (static_cast<int64_t>(A.table_cols) * A.bs > kRowsFromTokens || static_cast<int64_t>(A.B) * A.nodes * A.Hq > kRowsFromRows))
+    return A.D <= 64 ? launch_rows_of<T, 64>(A, stream) : A.D <= 128 ? launch_rows_of<T, 128>(A, stream) : launch_rows_of<T, 256>(A, stream);
+  if (A.B > 65535) return fail(B200_ESHAPE, "b200_paged_tree_attn: %d sequences", A.B);
   auto kern = A.D <= 64 ? tree_attn_any_kernel<T, 2> : A.D <= 128 ? tree_attn_any_kernel<T, 4> : tree_attn_any_kernel<T, 8>;
   kern<<<dim3(A.Hq, A.nodes, A.B), kAnyWarps * 32, 0, stream>>>(A, vec);
   return check_launch("b200_paged_tree_attn");

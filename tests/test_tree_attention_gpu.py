@@ -111,6 +111,45 @@ def test_against_the_formula(B, nodes, Hq, Hkv, D, page, context, dtype):
     check(even, scale=0.3)
 
 
+SHARED = [  # types and sizes without tensor cores, tables of many tokens or many rows
+    (1, 1, 4, 2, 64, 16, 2500), (2, 3, 8, 2, 96, 24, 1300), (1, 4, 16, 4, 128, 16, 5000), (3, 13, 8, 2, 64, 5, 700), (2, 64, 16, 2, 256, 16, 600),
+    (40, 8, 32, 8, 64, 16, 70), (5, 2, 6, 3, 20, 7, 900), (64, 1, 2, 2, 200, 16, 640), (2, 16, 4, 4, 256, 16, 1000), (7, 9, 9, 3, 128, 16, 530),
+    (300, 2, 2, 2, 40, 16, 3), (1, 64, 64, 1, 64, 16, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,nodes,Hq,Hkv,D,page,context", SHARED)
+def test_rows_that_share_their_keys_without_tensor_cores(B, nodes, Hq, Hkv, D, page, context, dtype):
+    check(build(B, nodes, Hq, Hkv, D, page, context, dtype, seed=nodes + D), flags=ops.ATTN_FORCE_GENERIC)
+    check(build(B, nodes, Hq, Hkv, D, page, context, dtype, seed=nodes, tree=False), flags=ops.ATTN_FORCE_GENERIC)
+    even = build(B, nodes, Hq, Hkv, D, page, context, dtype, seed=1, ragged=False)
+    even["draft_lens"] = None
+    check(even, scale=0.3, flags=ops.ATTN_FORCE_GENERIC)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 96, 256])
+def test_no_numbers_among_rows_that_share_their_keys(D, dtype):
+    """A node without numbers, and what stands behind the last node: rows that do not see them stay as they are."""
+    B, nodes, page = 2, 20, 16
+    c = build(B, nodes, 8, 2, D, page, 900, dtype, seed=5, ragged=False)
+    clean = ops.paged_tree_attention(**c, flags=ops.ATTN_FORCE_GENERIC)
+    lens, seen = c["context_lens"].tolist(), c["visible"].tolist()
+    for b in range(B):
+        for place in [lens[b] - nodes + 7] + list(range(lens[b], -(-lens[b] // page) * page)):
+            at = int(c["block_tables"][b, place // page])
+            c["k_pool"][at, :, place % page] = float("nan")
+            c["v_pool"][at, :, place % page] = float("inf")
+    got = ops.paged_tree_attention(**c, flags=ops.ATTN_FORCE_GENERIC)
+    for b in range(B):
+        for t in range(nodes):
+            if seen[b][t] >> 7 & 1:
+                assert got[b, t].isnan().all()
+            else:
+                assert torch.equal(got[b, t], clean[b, t])
+
+
 @pytest.mark.parametrize("context", [63, 64, 65, 127, 128, 129, 4000, 20001])
 @pytest.mark.parametrize("nodes", [1, 16, 63, 64])
 def test_lengths_around_a_tile(nodes, context):
