@@ -67,7 +67,7 @@ class _TreeStep:
         for shard, handles in zip(e.shards, e._handles):
             h, _ = shard.forward(h, position_ids=pos, past_key_values=[PagedLayerKV(hd.k_pool, hd.v_pool, st) for hd in handles], use_cache=True)
         logits = e.shards[-1].get_logits(h)
-        chosen = e._choose(logits.reshape(B * T, -1), 0, pos + 1).view(B, T)
+        chosen = e._choose(logits.reshape(B * T, -1), 0, lambda: pos + 1).view(B, T)
         for i, (pool, handles) in enumerate(zip(e.pools, e._handles)):
             k, v = e._pool_ptrs[i]
             out = ops.accept_drafts(self.tokens, chosen, self.parents, visible, k, v, tuple(handles[0].k_pool.shape), e.dtype, tables, total,
@@ -431,7 +431,7 @@ class PagedDecodeEngine:
             logits = self.shards[-1].get_logits(h[:, -1:, :])[:, 0, :]
             if self.logits_log is not None:
                 self.logits_log.append((lo, hi, logits.float().clone()))
-            return self._choose(logits, lo, torch.full((n,), past_len + P, dtype=torch.int64, device=self.device))
+            return self._choose(logits, lo, lambda: torch.full((n,), past_len + P, dtype=torch.int64, device=self.device))
         return h
 
     # ---- the next token --------------------------------------------------------------------------------
@@ -457,10 +457,11 @@ class PagedDecodeEngine:
             buf[:len(rows)].copy_(torch.from_numpy(values))
         self._numbers[:len(rows)].copy_(torch.from_numpy(np.stack([s.numbers(self.max_seq_len + 1) for s in rows])))
 
-    def _choose(self, logits: torch.Tensor, lo: int, pos: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The tokens at positions ``pos`` (int64) of the sequences from ``lo`` on, one or several rows of logits for each."""
+    def _choose(self, logits: torch.Tensor, lo: int, places: Callable[[], torch.Tensor], out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The tokens at positions ``places()`` (int64; drawn tokens only) of the sequences from ``lo`` on, one or several rows of logits for each."""
         if self.sampling is None:
             return ops.argmax_rows(logits, out=out)  # one CTA per row; torch's reduce takes 46 us here
+        pos = places()
         n = pos.shape[0]
         each = logits.shape[0] // n
         rows = [b[lo:lo + n] if each == 1 else b[lo:lo + n].repeat_interleave(each) for b in (self._temperature, self._top_k, self._top_p, self._min_p)]
@@ -518,7 +519,7 @@ class PagedDecodeEngine:
             self.hn_out[:B].copy_(h[:, 0, :])
         elif self.is_last:
             logits = self.shards[-1].get_logits(h)[:, 0, :]
-            self._choose(logits, 0, pos + 1, out=self.next_tokens[:B])
+            self._choose(logits, 0, lambda: pos + 1, out=self.next_tokens[:B])
             if self.logits_log is not None:  # eager launches only: the margins behind every token
                 self.logits_log.append((0, B, logits.float().clone()))
         else:
