@@ -23,9 +23,9 @@
 // Where that does not serve - k over 2048, or ranges of more than 4096 elements, equal logits above all - the last key is found by its digits of 8 bits
 // from counts or sums in the whole row.
 //
-// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.2 us on the
+// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.1 us on the
 // device; 64 rows of settings of their own 49, the rows without k the longest); many rows by the instructions of the exact weights, about ninety per element
-// in all passes (256 rows of 128256 in 32 bits, p 0.9 with thousands of tokens kept: 138 us; their bytes take 20, read three times 60).
+// in all passes (256 rows of 128256 in 32 bits, p 0.9 with thousands of tokens kept: 137 us; their bytes take 20, read three times 60).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -966,7 +966,7 @@ int launch_sample(Sample A, int rows, cudaStream_t stream) {
     return sizeof(Shared) + ((per + 1) & ~size_t{1}) * 8 + (held ? per * kBlock * sizeof(T) : 0);
   };
   // Two CTAs per SM.  As many for a row as the rows leave room for in one round, each with a part worth a cluster's barriers (1500 clocks each); the parts
-  // stay in shared memory if they fit, else they are read again.  (256 rows of 128 k in 32 bits, a call after the other: 154 us; with more instructions a
+  // stay in shared memory if they fit, else they are read again.  (256 rows of 128 k in 32 bits, a call after the other: 148 - 154 us; with more instructions a
   // weight 160; then cut until they fit, in seven rounds of CTAs, 288; every other pass backwards, for what the cache still holds, 162.  37 rows of 32003 in 16 bits: 12.3 us by four CTAs each,
   // 16.8 by eight.)
   constexpr size_t kHalf = 113 * 1024;

@@ -36,7 +36,7 @@ __device__ __forceinline__ void lengths(const TreeAttn& A, int b, int* keys, int
 // ---- any type, head size and page size ------------------------------------------------------------------------------------------------------
 // One CTA per (sequence, node, query head); its warps take 32 keys in turns, a lane a key for the scores and a part of the columns for the
 // output, and put their maxima, sums and outputs together at the end.  Bound by the loads' latency: 4 sequences x 13 nodes x 8 heads of 64 at 160 keys
-// in fp32 14 us on the device (four warps, eight rows of values under way: 20).  Serves what neither kernel below does: few rows behind short tables, rows
+// in fp32 11 - 14 us on the device (four warps, eight rows of values under way: 20).  Serves what neither kernel below does: few rows behind short tables, rows
 // that are not of 16-byte pieces.
 constexpr int kAnyWarps = 8, kAnyMostD = 256;
 
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(256, 2) tree_attn_rows_kernel(const TreeAttn A
 //
 // Bound.  Few rows: memory, 64 sequences x 8 nodes at 2k (32 heads over 8 of 128) 84 us on the device, 4.9 TB/s of the 6.55 that a copy reaches: SMs are
 // not served evenly, and each walk begins with three dependent loads (lengths, table, keys).  Two to four times the workers, so that late ones do less:
-// 98 to 114 us for 90.  Many rows: the softmax's chain of a tile, 8 x 64 nodes at 32k (64 heads over 8) 521 us on the device and 605 a call after the
+// 98 to 114 us for 90.  Many rows: the softmax's chain of a tile, 8 x 64 nodes at 32k (64 heads over 8) 514 us on the device and 607 a call after the
 // other, 1.05 PFLOP/s; exponential unit 57 %, tensor cores 53 %, issue slots 46 %.  A part of the exponentials as polynomials took 656 for 590.
 constexpr int kRows = 128, kKeys = 64, kBlk = kKeys * 128;
 // threads: rows, copies of keys and of values, products.  Eight warps: two CTAs' leave each thread 128 registers (nine: 96)
