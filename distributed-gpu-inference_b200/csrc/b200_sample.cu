@@ -25,7 +25,7 @@
 //
 // Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.1 us on the
 // device; 64 rows of settings of their own 49, the rows without k the longest); many rows by the instructions of the exact weights, about ninety per element
-// in all passes (256 rows of 128256 in 32 bits, p 0.9 with thousands of tokens kept: 137 us; their bytes take 20, read three times 60).
+// in all passes (256 rows of 128256 in 32 bits, p 0.95 with thousands of tokens kept: 137 us; their bytes take 20, read three times 60).
 #include <cooperative_groups.h>
 
 #include <algorithm>
