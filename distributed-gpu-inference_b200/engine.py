@@ -34,11 +34,12 @@ from . import ops
 
 
 class _TreeStep:
-    """One pass over trees of ``nodes`` drafted tokens: static buffers and the captured graph."""
+    """One pass over trees of ``nodes`` drafted tokens of the engine's present number of sequences: static buffers and the captured graph, which are of
+    that number; tables, lengths and settings are read from the engine's own buffers at each pass."""
 
     def __init__(self, engine: "PagedDecodeEngine", nodes: int):
-        self.e, self.nodes = engine, nodes
-        B, dev = engine.batch, engine.device
+        self.e, self.nodes, self.batch = engine, nodes, engine.batch
+        B, dev = self.batch, engine.device
         self.tokens = torch.zeros((B, nodes), dtype=torch.int64, device=dev)
         self.parents = torch.full((B, nodes), -1, dtype=torch.int32, device=dev)
         self.lens = torch.zeros((B,), dtype=torch.int32, device=dev)
@@ -49,7 +50,7 @@ class _TreeStep:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
 
     def body(self) -> None:
-        e, B, T, bs = self.e, self.e.batch, self.nodes, self.e.block_size
+        e, B, T, bs = self.e, self.batch, self.nodes, self.e.block_size
         tables = e.block_tables[:B]
         context = e.context_lens[:B]
         node = torch.arange(T, device=e.device)
@@ -242,7 +243,7 @@ class PagedDecodeEngine:
         self._temperature, self._top_p, self._min_p = (torch.zeros((max_batch,), dtype=torch.float32, device=dev) for _ in range(3))
         self._top_k = torch.zeros((max_batch,), dtype=torch.int32, device=dev)
         self._numbers: Optional[torch.Tensor] = None
-        self._trees: Dict[int, "_TreeStep"] = {}    # by nodes
+        self._trees: Dict[int, "_TreeStep"] = {}    # by nodes; all of one batch size
         self._pool_ptrs = [None] * len(self.shards)
         # prefix cache across requests: one index per shard pool, holding its own reference on the cached blocks
         self.prefix_index: Optional[List[RadixPrefixIndex]] = (
@@ -309,6 +310,7 @@ class PagedDecodeEngine:
         self.cached_blocks = n_cached
         self._graph = None
         self._graph_chained = None
+        self._graph_key = None
         self._trees = {}
         self._set_prefix(n_shared if batch > 1 else 0)
         self._shared_blocks = n_shared
@@ -392,7 +394,7 @@ class PagedDecodeEngine:
         if not same_shape:
             self._graph = None
             self._graph_chained = None
-            self._trees = {}
+        self._trees = {nodes: step for nodes, step in self._trees.items() if step.batch == batch}
         self._set_prefix(0)
         self._shared_blocks, self.cached_blocks, self._prefix_tokens = 0, 0, None
 
@@ -640,7 +642,7 @@ class PagedDecodeEngine:
             if n and not 0 <= root < vocab:
                 raise ValueError(f"a tree's root {root} is no token")
         step = self._trees.get(nodes)
-        if step is None:
+        if step is None or step.batch != B:
             step = self._trees[nodes] = _TreeStep(self, nodes)
         return step.run(tokens, parents, lens)
 

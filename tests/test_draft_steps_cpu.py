@@ -1,0 +1,85 @@
+"""What the paged engine keeps between calls, without a GPU: its tables and pools on the CPU, a recorder in the place of a pass over trees."""
+import types
+
+import pytest
+import torch
+
+import dgi_b200  # noqa: F401
+from dgi_b200 import engine as E
+from dgi_b200.paged_layer import PagedBatchState
+from dgi_b200.worker.distributed.kv_cache import KVCachePool
+
+MAX_BATCH, BLOCK, PER_SEQ, VOCAB = 4, 4, 8, 50
+
+
+@pytest.fixture
+def engine():
+    """A whole model's engine of four sequences of 32 tokens; what would need a GPU (prompts, steps) is not called."""
+    e = object.__new__(E.PagedDecodeEngine)
+    e.max_batch, e.block_size, e.blocks_per_seq, e.max_seq_len = MAX_BATCH, BLOCK, PER_SEQ, BLOCK * PER_SEQ
+    e.device, e.dtype, e.use_cuda_graph, e.logits_log = torch.device("cpu"), torch.float32, True, None
+    e.is_first = e.is_last = True
+    e.external_head = False
+    e.Hq, e.Hkv, e.D = 4, 2, 8
+    e.shards = [types.SimpleNamespace(embed_tokens=torch.nn.Embedding(VOCAB, 4))]
+    e.pools = [KVCachePool(num_layers=2, num_heads=2, head_dim=8, block_size=BLOCK, max_blocks_per_layer=MAX_BATCH * PER_SEQ, device="cpu", dtype=torch.float32)]
+    e.block_tables = torch.zeros((MAX_BATCH, PER_SEQ), dtype=torch.int32)
+    e.context_lens = torch.zeros(MAX_BATCH, dtype=torch.int32)
+    e.state = PagedBatchState(e.block_tables, e.context_lens, torch.zeros(MAX_BATCH, dtype=torch.int64), BLOCK * PER_SEQ)
+    e._seq_blocks, e._host_lens = [None] * MAX_BATCH, [0] * MAX_BATCH
+    e._graph = e._graph_chained = e.prefix_index = e._numbers = e.sampling = None
+    e._trees, e._borrowed, e.batch = {}, False, 0
+    e._temperature, e._top_p, e._min_p = (torch.zeros(MAX_BATCH) for _ in range(3))
+    e._top_k = torch.zeros(MAX_BATCH, dtype=torch.int32)
+    return e
+
+
+@pytest.fixture
+def passes(monkeypatch):
+    """(sequences that the step was made for, nodes, shape of the tokens, how many steps had been made before it) of each pass over trees."""
+    made, steps = [], []
+
+    class Step:
+        def __init__(self, engine, nodes):
+            self.batch, self.nodes, self.number = engine.batch, nodes, len(steps)
+            steps.append(nodes)
+
+        def run(self, tokens, parents, lens):
+            made.append((self.batch, self.nodes, tuple(tokens.shape), self.number))
+            return [0] * tokens.shape[0], [[-1] * self.nodes] * tokens.shape[0]
+
+    monkeypatch.setattr(E, "_TreeStep", Step)
+    return made
+
+
+def adopt(e, n, tokens=9):
+    e.adopt_sequences([[pool.allocate_sequence(tokens + 8) for pool in e.pools] for _ in range(n)], [tokens] * n)
+
+
+def verify(e, nodes=3):
+    n = e.batch
+    return e.verify_trees(torch.zeros((n, nodes), dtype=torch.int64), torch.full((n, nodes), -1, dtype=torch.int32))
+
+
+def test_a_pass_over_trees_is_of_its_batch(engine, passes):
+    """A step holds buffers and a captured pass of one number of sequences: it serves no other number, whatever single steps were captured for."""
+    engine._graph_key = (1, 0)          # a single step of one sequence had been captured
+    engine.allocate(4, 20)
+    verify(engine)
+    adopt(engine, 1)
+    verify(engine)
+    adopt(engine, 3)
+    verify(engine)
+    engine._graph_key = (2, 0)
+    adopt(engine, 2)
+    verify(engine)
+    assert [p[:3] for p in passes] == [(n, 3, (n, 3)) for n in (4, 1, 3, 2)]
+
+
+def test_a_pass_over_trees_is_kept_for_its_batch(engine, passes):
+    """Sequences handed over in turn, as many as before: the captured pass serves them, though no single step was captured."""
+    for _ in range(3):
+        adopt(engine, 2)
+        verify(engine)
+        verify(engine, 5)
+    assert [p[3] for p in passes] == [0, 1] * 3

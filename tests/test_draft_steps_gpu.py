@@ -1,0 +1,65 @@
+"""Passes over trees and drawn tokens between other calls of one engine: what a call leaves behind, and what it leaves alone."""
+import pytest
+import torch
+
+import dgi_b200  # noqa: F401
+from dgi_b200.drafting import pad_trees
+from dgi_b200.engine import PagedDecodeEngine
+from test_drafted_decode_gpu import Knowing, model
+
+pytestmark = pytest.mark.gpu
+
+
+def adopt(eng, prompts, room):
+    """The prompts in blocks of the caller's own; their first tokens."""
+    blocks = [[pool.allocate_sequence(prompts.shape[1] + room) for pool in eng.pools] for _ in range(prompts.shape[0])]
+    eng.adopt_sequences(blocks, [0] * prompts.shape[0])
+    return blocks, [[t] for t in eng.prefill(prompts).tolist()]
+
+
+@pytest.mark.parametrize("others", [1, 2])
+def test_trees_of_fewer_sequences_than_the_pass_before(golden, others):
+    """A step captured for one sequence, a pass over trees of four, then `others` handed over: their tokens, and nobody else's blocks."""
+    g, cfg, shards = model(golden)
+    prompts, want = torch.tensor(g["prompt_ids"]), g["tokens"]
+    rows = [p + t for p, t in zip(g["prompt_ids"], want)]
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=256, prefill_mode="eager", spare_blocks=40)
+    assert eng.generate(prompts[:others], 6).tolist() == [t[:6] for t in want[:others]]
+    assert eng.generate_drafted(prompts, 20, Knowing(rows, 9, 1), nodes=9).tolist() == [t[:20] for t in want]
+    blocks, told = adopt(eng, prompts[2:2 + others], 30)
+    slots = []
+    for li in range(cfg.num_hidden_layers):
+        mine = {blk.slot for seq in blocks for blk in seq[0][li]}
+        slots.append([i for i in range(eng.pools[0].layer(li).key_pool.shape[0]) if i not in mine])
+    pools = [(eng.pools[0].layer(li).key_pool, eng.pools[0].layer(li).value_pool) for li in range(cfg.num_hidden_layers)]
+    before = [[p[s].clone() for p in two] for two, s in zip(pools, slots)]
+    know = Knowing(rows, 9, 2)
+    for _ in range(3):
+        trees = [know(g["prompt_ids"][2 + b] + told[b]) for b in range(others)]
+        count, new = eng.verify_trees(*(torch.from_numpy(x) for x in pad_trees(trees, 9)))
+        assert len(count) == len(new) == others
+        for b in range(others):
+            told[b] += new[b][:count[b]]
+    assert all(torch.equal(x, p[s]) for was, two, s in zip(before, pools, slots) for x, p in zip(was, two))
+    assert told == [w[:len(t)] for t, w in zip(told, want[2:])] and min(map(len, told)) >= 4
+    assert eng._host_lens == [prompts.shape[1] + len(t) - 1 for t in told] + [0] * (4 - others)
+    for _ in range(3):        # single steps go on from there
+        eng.decode_step_device()
+        for b, t in enumerate(eng.next_tokens[:others].tolist()):
+            told[b].append(t)
+    assert told == [w[:len(t)] for t, w in zip(told, want[2:])]
+
+
+def test_trees_of_more_sequences_than_the_pass_before(golden):
+    g, cfg, shards = model(golden)
+    prompts, want = torch.tensor(g["prompt_ids"]), g["tokens"]
+    rows = [p + t for p, t in zip(g["prompt_ids"], want)]
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=256, prefill_mode="eager", spare_blocks=60)
+    for n in (1, 4, 2, 2):
+        _, told = adopt(eng, prompts[:n], 30)
+        know = Knowing(rows, 8, n)
+        for _ in range(2):
+            count, new = eng.verify_trees(*(torch.from_numpy(x) for x in pad_trees([know(g["prompt_ids"][b] + told[b]) for b in range(n)], 8)))
+            for b in range(n):
+                told[b] += new[b][:count[b]]
+        assert told == [w[:len(t)] for t, w in zip(told, want)] and len(told) == n
