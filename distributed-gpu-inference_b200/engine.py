@@ -21,6 +21,7 @@ pass; ``generate_drafted`` decodes that way.
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -438,7 +439,8 @@ class PagedDecodeEngine:
 
     # ---- the next token --------------------------------------------------------------------------------
     def set_sampling(self, sampling: Optional[Sequence[Sampling]]) -> None:
-        """How the sequences ``0 .. len(sampling) - 1`` choose their tokens from now on, the ones behind them greedily; None: all greedily."""
+        """How the sequences ``0 .. len(sampling) - 1`` choose their tokens from now on, the ones behind them greedily; None: all greedily.
+        ``generate``, ``generate_ragged``, ``generate_drafted`` and ``batch_inference`` go by their own arguments, and leave these as they are."""
         rows = None if sampling is None else list(sampling)
         if rows is not None and len(rows) > self.max_batch:
             raise ValueError("more settings than the engine has sequences")
@@ -446,18 +448,28 @@ class PagedDecodeEngine:
             rows = None
         if rows is not None and (not (self.is_first and self.is_last) or self.external_head):
             raise RuntimeError("sampling needs an engine with the whole model")
+        if rows is not None:
+            if self._numbers is None:
+                self._numbers = torch.zeros((self.max_batch, self.max_seq_len + 1), dtype=torch.float32, device=self.device)
+            for buf, values in zip((self._temperature, self._top_k, self._top_p, self._min_p), settings(rows)):
+                buf.zero_()
+                buf[:len(rows)].copy_(torch.from_numpy(values))
+            self._numbers[:len(rows)].copy_(torch.from_numpy(np.stack([s.numbers(self.max_seq_len + 1) for s in rows])))
         if (rows is None) != (self.sampling is None):       # captured steps choose one way or the other
             self._graph = self._graph_chained = None
             self._trees = {}
         self.sampling = rows
-        if rows is None:
-            return
-        if self._numbers is None:
-            self._numbers = torch.zeros((self.max_batch, self.max_seq_len + 1), dtype=torch.float32, device=self.device)
-        for buf, values in zip((self._temperature, self._top_k, self._top_p, self._min_p), settings(rows)):
-            buf.zero_()
-            buf[:len(rows)].copy_(torch.from_numpy(values))
-        self._numbers[:len(rows)].copy_(torch.from_numpy(np.stack([s.numbers(self.max_seq_len + 1) for s in rows])))
+
+    @contextlib.contextmanager
+    def _sampling_of(self, sampling: Optional[Sequence[Sampling]]):
+        """A call's settings, while it lasts; then the engine's are again what they were."""
+        own = self.sampling
+        self.set_sampling(sampling)
+        try:
+            yield
+        finally:
+            if own is not None or self.sampling is not None:
+                self.set_sampling(own)
 
     def _choose(self, logits: torch.Tensor, lo: int, places: Callable[[], torch.Tensor], out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The tokens at positions ``places()`` (int64; drawn tokens only) of the sequences from ``lo`` on, one or several rows of logits for each."""
@@ -656,19 +668,19 @@ class PagedDecodeEngine:
         drafter = drafter or PromptLookup(nodes)
         if sampling is not None and len(sampling) != B:
             raise ValueError("sampling needs settings for every prompt")
-        self.set_sampling(sampling)
-        room = max(P + max_new_tokens, min(P + max_new_tokens + nodes - 1, self.max_seq_len))
-        self.allocate(B, room)
-        told = [row + [tok] for row, tok in zip(prompt_ids.tolist(), self.prefill(prompt_ids).tolist())]
-        want = P + max_new_tokens
-        while any(len(t) < want for t in told):
-            trees = [drafter(t) if len(t) < want else None for t in told]
-            trees = [tree and tuple(part[:room - len(t) + 1] for part in tree) for tree, t in zip(trees, told)]
-            tokens, parents, lens = pad_trees(trees, nodes)
-            count, new = self.verify_trees(torch.from_numpy(tokens), torch.from_numpy(parents), torch.from_numpy(lens))
-            for b in range(B):
-                told[b].extend(new[b][:min(count[b], want - len(told[b]))])
-        return torch.tensor([t[P:] for t in told], dtype=torch.int64)
+        with self._sampling_of(sampling):
+            room = max(P + max_new_tokens, min(P + max_new_tokens + nodes - 1, self.max_seq_len))
+            self.allocate(B, room)
+            told = [row + [tok] for row, tok in zip(prompt_ids.tolist(), self.prefill(prompt_ids).tolist())]
+            want = P + max_new_tokens
+            while any(len(t) < want for t in told):
+                trees = [drafter(t) if len(t) < want else None for t in told]
+                trees = [tree and tuple(part[:room - len(t) + 1] for part in tree) for tree, t in zip(trees, told)]
+                tokens, parents, lens = pad_trees(trees, nodes)
+                count, new = self.verify_trees(torch.from_numpy(tokens), torch.from_numpy(parents), torch.from_numpy(lens))
+                for b in range(B):
+                    told[b].extend(new[b][:min(count[b], want - len(told[b]))])
+            return torch.tensor([t[P:] for t in told], dtype=torch.int64)
 
     @torch.no_grad()
     def generate(self, prompt_ids: torch.Tensor, max_new_tokens: int, shared_prefix_len: int = 0,
@@ -679,16 +691,16 @@ class PagedDecodeEngine:
         B, P = prompt_ids.shape
         if sampling is not None and len(sampling) != B:
             raise ValueError("sampling needs settings for every prompt")
-        self.set_sampling(sampling)
-        n_pre = min(shared_prefix_len, P - 1)
-        self.allocate(B, P + max_new_tokens, shared_prefix_len=n_pre,
-                      prefix_tokens=prompt_ids[0, :n_pre].tolist() if self.prefix_index is not None and n_pre else None)
-        nxt = self.prefill(prompt_ids).cpu()
-        out = [nxt]
-        for _ in range(max_new_tokens - 1):
-            nxt = self.decode_step(nxt)
-            out.append(nxt)
-        return torch.stack(out, dim=1)
+        with self._sampling_of(sampling):
+            n_pre = min(shared_prefix_len, P - 1)
+            self.allocate(B, P + max_new_tokens, shared_prefix_len=n_pre,
+                          prefix_tokens=prompt_ids[0, :n_pre].tolist() if self.prefix_index is not None and n_pre else None)
+            nxt = self.prefill(prompt_ids).cpu()
+            out = [nxt]
+            for _ in range(max_new_tokens - 1):
+                nxt = self.decode_step(nxt)
+                out.append(nxt)
+            return torch.stack(out, dim=1)
 
     @torch.no_grad()
     def generate_ragged(self, prompts: Sequence[Sequence[int]], max_new_tokens: int,
@@ -712,45 +724,45 @@ class PagedDecodeEngine:
             raise ValueError("empty prompt")
         if sampling is not None and len(sampling) != B:
             raise ValueError("sampling needs settings for every prompt")
-        self.set_sampling(None if sampling is None else [sampling[i] for i in order])
-        n_pre = max(0, min(shared_prefix_len, min(lens) - 1))
-        head = list(prompts[order[0]][:n_pre])
-        if n_pre and any(list(p[:n_pre]) != head for p in prompts):
-            raise ValueError("prompts do not share the declared prefix")
-        self.allocate(B, max(lens) + max_new_tokens, shared_prefix_len=n_pre,
-                      prefix_tokens=head if self.prefix_index is not None and n_pre else None)
-        bs = self.block_size
-        shared, cached = self._shared_blocks * bs, self.cached_blocks * bs
-        first = torch.empty((B,), dtype=torch.int64, device=self.device)
-        lo = 0
-        if shared > 0:
-            # the shortest prompt's sequence computes what is left of the shared blocks, then its own tokens
-            ids = torch.tensor([list(prompts[order[0]])[cached:]], dtype=torch.int64, device=self.device)
-            first[0:1] = self.prefill_chunk(0, 1, ids, past_len=cached)
-            if self.prefix_index is not None and self._prefix_tokens is not None:
-                for si, idx in enumerate(self.prefix_index):
-                    idx.insert(self._prefix_tokens, [lb[:shared // bs] for lb in self._seq_blocks[0][si]])
-            lo = 1
-        while lo < B:
-            hi = lo
-            while hi < B and lens[hi] == lens[lo]:
-                hi += 1
-            for c0 in range(lo, hi, self.prefill_chunk_size):
-                c1 = min(hi, c0 + self.prefill_chunk_size)
-                ids = torch.tensor([list(prompts[order[i]])[shared:] for i in range(c0, c1)], dtype=torch.int64,
-                                   device=self.device)
-                first[c0:c1] = self.prefill_chunk(c0, c1, ids, past_len=shared)
-            lo = hi
-        out = [first.cpu()]
-        nxt = out[0]
-        for _ in range(max_new_tokens - 1):
-            nxt = self.decode_step(nxt)
-            out.append(nxt)
-        toks = torch.stack(out, dim=1).tolist()
-        result: List[List[int]] = [[] for _ in range(B)]
-        for pos, i in enumerate(order):
-            result[i] = toks[pos]
-        return result
+        with self._sampling_of(None if sampling is None else [sampling[i] for i in order]):
+            n_pre = max(0, min(shared_prefix_len, min(lens) - 1))
+            head = list(prompts[order[0]][:n_pre])
+            if n_pre and any(list(p[:n_pre]) != head for p in prompts):
+                raise ValueError("prompts do not share the declared prefix")
+            self.allocate(B, max(lens) + max_new_tokens, shared_prefix_len=n_pre,
+                          prefix_tokens=head if self.prefix_index is not None and n_pre else None)
+            bs = self.block_size
+            shared, cached = self._shared_blocks * bs, self.cached_blocks * bs
+            first = torch.empty((B,), dtype=torch.int64, device=self.device)
+            lo = 0
+            if shared > 0:
+                # the shortest prompt's sequence computes what is left of the shared blocks, then its own tokens
+                ids = torch.tensor([list(prompts[order[0]])[cached:]], dtype=torch.int64, device=self.device)
+                first[0:1] = self.prefill_chunk(0, 1, ids, past_len=cached)
+                if self.prefix_index is not None and self._prefix_tokens is not None:
+                    for si, idx in enumerate(self.prefix_index):
+                        idx.insert(self._prefix_tokens, [lb[:shared // bs] for lb in self._seq_blocks[0][si]])
+                lo = 1
+            while lo < B:
+                hi = lo
+                while hi < B and lens[hi] == lens[lo]:
+                    hi += 1
+                for c0 in range(lo, hi, self.prefill_chunk_size):
+                    c1 = min(hi, c0 + self.prefill_chunk_size)
+                    ids = torch.tensor([list(prompts[order[i]])[shared:] for i in range(c0, c1)], dtype=torch.int64,
+                                       device=self.device)
+                    first[c0:c1] = self.prefill_chunk(c0, c1, ids, past_len=shared)
+                lo = hi
+            out = [first.cpu()]
+            nxt = out[0]
+            for _ in range(max_new_tokens - 1):
+                nxt = self.decode_step(nxt)
+                out.append(nxt)
+            toks = torch.stack(out, dim=1).tolist()
+            result: List[List[int]] = [[] for _ in range(B)]
+            for pos, i in enumerate(order):
+                result[i] = toks[pos]
+            return result
 
     # ---- ContinuousBatcher protocol (reference: worker/batch_processor.py:302-336) ---------------------
     def batch_inference(self, params_list: List[Dict[str, Any]]) -> List[Any]:

@@ -6,6 +6,7 @@ import torch
 
 import dgi_b200  # noqa: F401
 from dgi_b200 import engine as E
+from dgi_b200.drafting import GREEDY, Sampling
 from dgi_b200.paged_layer import PagedBatchState
 from dgi_b200.worker.distributed.kv_cache import KVCachePool
 
@@ -83,3 +84,73 @@ def test_a_pass_over_trees_is_kept_for_its_batch(engine, passes):
         verify(engine)
         verify(engine, 5)
     assert [p[3] for p in passes] == [0, 1] * 3
+
+
+OWN, CALL = [Sampling(0.9, 0, 1.0, 0.0, 1), GREEDY], [Sampling(1.2, 7, 0.8, 0.1, 2), Sampling(0.5, 0, 1.0, 0.0, 3)]
+
+
+@pytest.fixture
+def told(engine, passes):
+    """The settings that the engine's passes found, in turn: temperatures of the first two sequences, None where it decoded greedily."""
+    seen = []
+
+    def record(n):
+        seen.append(None if engine.sampling is None else engine._temperature[:2].tolist())
+        return torch.zeros(n, dtype=torch.int64)
+
+    engine.prefill = lambda prompts: record(len(prompts))
+    engine.prefill_chunk = lambda lo, hi, ids, past_len=0: record(hi - lo)
+    engine.decode_step = lambda tokens: record(len(tokens))
+    engine.prefill_chunk_size = 8
+    engine._shared_blocks = engine.cached_blocks = 0
+
+    def verify(tokens, parents, lens):
+        n = tokens.shape[0]
+        return [1] * n, record(n)[:, None].tolist()
+
+    engine.verify_trees = verify
+    return seen
+
+
+def calls(e, sampling):
+    prompts = torch.zeros((2, 5), dtype=torch.int64)
+    ask = [{"input_ids": [0] * 5, "max_new_tokens": 3, "do_sample": s.temperature > 0, "temperature": s.temperature} for s in sampling or [GREEDY] * 2]
+    return [lambda: e.generate(prompts, 3, sampling=sampling), lambda: e.generate_drafted(prompts, 3, sampling=sampling),
+            lambda: e.generate_ragged([[0] * 5, [0] * 6], 3, sampling=sampling), lambda: e.batch_inference(ask)]
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_a_calls_settings_end_with_it(engine, told, which):
+    want = [pytest.approx(s.temperature) for s in CALL]
+    for own in (None, OWN):
+        engine.set_sampling(own)
+        buffers = (engine._temperature, engine._top_k, engine._top_p, engine._min_p)
+        before = [b.clone() for b in buffers], None if own is None else engine._numbers.clone()
+        for sampling in (CALL, None):
+            told.clear()
+            calls(engine, sampling)[which]()
+            assert len(told) >= 3 and all(t == (None if sampling is None else want) for t in told)
+            assert engine.sampling == own
+            if own is not None:
+                assert all(torch.equal(a, b) for a, b in zip(buffers, before[0])) and torch.equal(engine._numbers[:2], before[1][:2])
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_a_calls_settings_end_with_it_when_it_fails(engine, told, which):
+    def fails(*a, **kw):
+        raise RuntimeError("no room")
+
+    engine.allocate = fails
+    for own in (None, OWN):
+        engine.set_sampling(own)
+        with pytest.raises(RuntimeError, match="no room"):
+            calls(engine, CALL)[which]()
+        assert engine.sampling == own
+
+
+def test_settings_that_are_refused_change_nothing(engine, told):
+    engine.set_sampling(OWN)
+    engine.external_head = True
+    with pytest.raises(RuntimeError, match="whole model"):
+        engine.generate(torch.zeros((2, 5), dtype=torch.int64), 3, sampling=CALL)
+    assert engine.sampling == OWN and not told

@@ -3,9 +3,9 @@ import pytest
 import torch
 
 import dgi_b200  # noqa: F401
-from dgi_b200.drafting import pad_trees
+from dgi_b200.drafting import Sampling, pad_trees
 from dgi_b200.engine import PagedDecodeEngine
-from test_drafted_decode_gpu import Knowing, model
+from test_drafted_decode_gpu import SETTINGS, Knowing, model
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,38 @@ def test_trees_of_more_sequences_than_the_pass_before(golden):
             for b in range(n):
                 told[b] += new[b][:count[b]]
         assert told == [w[:len(t)] for t, w in zip(told, want)] and len(told) == n
+
+
+def single_steps(eng, prompts, n):
+    eng.allocate(prompts.shape[0], prompts.shape[1] + n)
+    told = [[t] for t in eng.prefill(prompts).tolist()]
+    for _ in range(n - 1):
+        for row, t in zip(told, eng.decode_step(torch.tensor([r[-1] for r in told])).tolist()):
+            row.append(t)
+    return told
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_a_calls_settings_end_with_it(golden, graph):
+    """Behind a call that drew: prompts, single steps, sequences handed over and trees go by the engine's own settings, greedily or not."""
+    g, cfg, shards = model(golden)
+    prompts, want = torch.tensor(g["prompt_ids"]), [t[:12] for t in g["tokens"]]
+    eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=256, prefill_mode="eager", use_cuda_graph=graph, spare_blocks=60)
+    drawn = eng.generate(prompts, 12, sampling=SETTINGS).tolist()
+    assert drawn != want and single_steps(eng, prompts, 12) == want
+    ask = [{"input_ids": p, "max_new_tokens": 12, "do_sample": True, "temperature": 1.5, "seed": i} for i, p in enumerate(g["prompt_ids"])]
+    for call in (lambda: eng.generate_ragged(g["prompt_ids"], 12, sampling=SETTINGS), lambda: eng.generate_drafted(prompts, 12, sampling=SETTINGS),
+                 lambda: eng.batch_inference(ask)):
+        call()
+        _, told = adopt(eng, prompts, 12)
+        know = Knowing([p + t for p, t in zip(g["prompt_ids"], g["tokens"])], 8, 1)
+        count, new = eng.verify_trees(*(torch.from_numpy(x) for x in pad_trees([know(p + t) for p, t in zip(g["prompt_ids"], told)], 8)))
+        assert [t + n[:c] for t, n, c in zip(told, new, count)] == [w[:1 + c] for w, c in zip(want, count)]
+        eng.release()
+    eng.set_sampling(SETTINGS)
+    assert eng.generate(prompts, 12).tolist() == want
+    assert single_steps(eng, prompts, 12) == drawn
+    eng.generate(prompts, 5, sampling=[Sampling(2.0, 0, 1.0, 0.0, 9)] * 4)
+    assert single_steps(eng, prompts, 12) == drawn
+    eng.set_sampling(None)
+    assert single_steps(eng, prompts, 12) == want
