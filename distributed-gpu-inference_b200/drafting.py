@@ -31,7 +31,8 @@ class Sampling:
     @classmethod
     def of_request(cls, params: Dict[str, Any]) -> "Sampling":
         """From a request's parameters (absent ones and None: their defaults; without a ``seed`` it is 0, the same tokens each time); greedy unless
-        it says ``do_sample``."""
+        it says ``do_sample``.  As other engines write them: ``top_k`` below 0 is no limit, ``seed`` below 0 none, ``top_p`` 0 keeps the likeliest token
+        alone."""
         if not params.get("do_sample", False):
             return GREEDY
 
@@ -39,7 +40,10 @@ class Sampling:
             value = params.get(name)
             return default if value is None else type(default)(value)
 
-        return cls(of("temperature", 0.7), of("top_k", 50), of("top_p", 0.9), of("min_p", 0.0), of("seed", 0))
+        k, p = max(of("top_k", 50), 0), of("top_p", 0.9)
+        if p == 0.0:
+            k, p = 1, 1.0
+        return cls(of("temperature", 0.7), k, p, of("min_p", 0.0), max(of("seed", 0), 0))
 
     def numbers(self, n: int) -> np.ndarray:
         """The first ``n`` random numbers of the seed's stream, fp32 in [0, 1)."""

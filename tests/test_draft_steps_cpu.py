@@ -154,3 +154,17 @@ def test_settings_that_are_refused_change_nothing(engine, told):
     with pytest.raises(RuntimeError, match="whole model"):
         engine.generate(torch.zeros((2, 5), dtype=torch.int64), 3, sampling=CALL)
     assert engine.sampling == OWN and not told
+
+
+def test_settings_as_other_engines_write_no_limit():
+    """Requests that were served before their settings counted are served: -1 for no limit of k and for no seed, 0 for the smallest nucleus."""
+    ask = {"do_sample": True, "temperature": 0.8, "top_k": 40, "top_p": 0.95, "min_p": 0.05, "seed": 6}
+    plain = Sampling(0.8, 40, 0.95, 0.05, 6)
+    assert Sampling.of_request(ask) == plain
+    assert Sampling.of_request({**ask, "top_k": -1}) == Sampling(0.8, 0, 0.95, 0.05, 6)
+    assert Sampling.of_request({**ask, "seed": -1}) == Sampling(0.8, 40, 0.95, 0.05, 0)
+    first = Sampling.of_request({**ask, "top_p": 0})        # the order's first is always kept: it alone
+    assert first.top_k == 1 and first.temperature > 0
+    for bad in (dict(top_p=1.5), dict(top_p=-0.1), dict(top_p=float("nan")), dict(min_p=2.0), dict(temperature=-1.0), dict(top_k="many")):
+        with pytest.raises(ValueError):
+            Sampling.of_request({**ask, **bad})
