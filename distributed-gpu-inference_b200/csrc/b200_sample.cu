@@ -23,8 +23,8 @@
 // Where that does not serve - k over 2048, or ranges of more than 4096 elements, equal logits above all - the last key is found by its digits of 8 bits
 // from counts or sums in the whole row.
 //
-// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.1 us on the
-// device; 64 rows of settings of their own 49, the rows without k the longest); many rows by the instructions of the exact weights, about ninety per element
+// Bound: a row or a few by the chain of passes and cluster barriers (1500 clocks each; one row of 128256 in 16 bits, k 50 and p 0.9: 13.4 us on the
+// device; 64 rows of settings of their own 50, the rows without k the longest); many rows by the instructions of the exact weights, about ninety per element
 // in all passes (256 rows of 128256 in 32 bits, p 0.95 with thousands of tokens kept: 137 us; their bytes take 20, read three times 60).
 #include <cooperative_groups.h>
 
@@ -171,25 +171,21 @@ constexpr int kBins = kThreads, kFew = 256;       // of Shared::range_count, whe
 static_assert(kBins + 2 * kFew <= kRanges, "room for bins and a bin's elements");
 
 // weights: multiples of 2^-frac
-template <typename T>
 struct Weigh {
   // An argument is (x - off) scale - c, scale = 256 log2(e) / t, c = (max - off) scale, each in two parts; one product less than a whole number near it,
-  // in one rounding, is what the polynomial takes.  16-bit types: off = max, c = 0 (a difference that matters is exact).  32 bits: off = 0, and c a
-  // multiple of 2^-5 with a rest; where c passes 2^18, off = max, for then what matters is within a twentieth of the maximum, and exact too.
+  // in one rounding, is what the polynomial takes.  off = 0, and c a multiple of 2^-5 with a rest; where c passes 2^18, off = max, for then what matters is
+  // within a twentieth of the maximum, and its difference exact.  (off = max for all rows of 16 bits saves two instructions of thirty, 0.2 - 0.4 us of 13.4
+  // for one row of 128256 and 49.9 for 64; but the difference of a logit near zero from a large one has more than 24 bits, and its weight was off by 2^-21.)
   float off, scale, scale_low, c, c_low;
   float floor, end;                     // arguments below `floor` count as it; steps from `end` on give 0
   double one;                           // 2^(52 - frac), whose last bit is 2^-frac
   const uint2* table;
-  __device__ __forceinline__ float argument(float x) const {
-    if constexpr (sizeof(T) == 4) return fmaf(x - off, scale, -c);
-    else return __fmul_rn(x - off, scale);
-  }
+  __device__ __forceinline__ float argument(float x) const { return fmaf(x - off, scale, -c); }
   __device__ __forceinline__ double operator()(float x) const {
     const float d = x - off, shift = 12582912.f, r = fmaxf(argument(x), floor) + shift;        // 3 * 2^22: the nearest whole number n is in the last bits
     const uint32_t n = __float_as_uint(r);
-    float f;        // (below the floor no number or any: 2^-50 of 32 bits is 0 all the same)
-    if constexpr (sizeof(T) == 4) f = fmaf(d, scale, -(c + (r - shift))) + fmaf(d, scale_low, -c_low);
-    else f = fmaf(d, scale_low, fmaf(d, scale, -(r - shift)));
+    // (below the floor no number or any: 2^-50 of 32 bits is 0 all the same)
+    const float f = fmaf(d, scale, -(c + (r - shift))) + fmaf(d, scale_low, -c_low);
     constexpr float c1 = 0.69314718055994530942 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
     const uint2 step = table[n & 255];
     const float q = f * fmaf(fmaf(f, c3, c2), f, c1);
@@ -407,13 +403,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const Sample A
   if (k <= 0 || k >= A.cols) k = 0;
   const bool by_mass = p < 1.0f;
   // (min_p no number: no limit)
-  Weigh<T> weigh;
+  Weigh weigh;
   {
     const double scale = 369.32993046757463 / static_cast<double>(t);     // 256 log2(e)
     weigh.scale = static_cast<float>(fmin(scale, 3e38));
     weigh.scale_low = scale < 3e38 ? static_cast<float>(scale - weigh.scale) : 0.f;
     const double c = static_cast<double>(top) * (static_cast<double>(weigh.scale) + static_cast<double>(weigh.scale_low));
-    const bool apart = sizeof(T) == 4 && fabs(c) <= 262144.0;
+    const bool apart = fabs(c) <= 262144.0;
     weigh.off = apart ? 0.f : top;
     weigh.c = apart ? static_cast<float>(rint(c * 32.0) / 32.0) : 0.f;
     weigh.c_low = apart ? static_cast<float>(c - static_cast<double>(weigh.c)) : 0.f;
