@@ -2,7 +2,9 @@
 
 ``Sampling``: one request's temperature, top-k, top-p, min-p and seed (the reference's request parameters, common/data_structures.py:
 111-113 there).  Its random number for the token at position p of the sequence is the p-th of its seed's stream, whatever the batch
-around it and however many tokens a step makes: the same request gives the same tokens alone, in a batch, and with drafted tokens.
+around it and however many tokens a step makes, and a token follows from its logits and this number alone: the same request gives the same
+tokens alone, in a batch, and with drafted tokens, as far as its logits are the same - their sums are rounded in an order that depends on the batch
+and on the trees, which in 16 bits moves a token now and then.
 
 ``PromptLookup``: drafts from the sequence itself - what followed earlier occurrences of its last tokens, as a tree.
 """

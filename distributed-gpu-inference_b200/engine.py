@@ -633,7 +633,8 @@ class PagedDecodeEngine:
         seen yet, the others come behind their parents; ``draft_lens`` int32 ``[batch]`` how many nodes a sequence has (0: it rests).  The
         model runs once over all nodes (a token outside its vocabulary is never taken); the nodes whose tokens are the model's own choices stay in the cache, side by side behind the context,
         and a sequence gets ``count`` new tokens: one for each of them, the last of them where ``decode_step_device`` goes on.  The choices are the
-        ones that single steps would have made."""
+        ones that single steps would have made, of logits that differ by the rounding of sums in another order: the same tokens unless two logits, or
+        a draw and the end of a weight, are that close - seldom in 32 bits, in 16 bits (logits off by 2^-8 or 2^-11 of their size either way) now and then."""
         if not (self.is_first and self.is_last) or self.external_head:
             raise RuntimeError("verify_trees() drives a whole model")
         B = self.batch
@@ -661,7 +662,7 @@ class PagedDecodeEngine:
     @torch.no_grad()
     def generate_drafted(self, prompt_ids: torch.Tensor, max_new_tokens: int, drafter: Optional[Callable] = None,
                          sampling: Optional[Sequence[Sampling]] = None, nodes: int = 8) -> torch.Tensor:
-        """``generate``'s tokens with several of them per pass: ``drafter(tokens of a sequence so far) -> (tokens, parents)`` proposes a tree
+        """``generate``'s tokens (as ``verify_trees`` chooses them) with several of them per pass: ``drafter(tokens of a sequence so far) -> (tokens, parents)`` proposes a tree
         of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``), and ``verify_trees`` checks it (at the end of
         ``max_seq_len`` as much of its beginning as there is room for)."""
         B, P = prompt_ids.shape

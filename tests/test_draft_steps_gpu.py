@@ -5,9 +5,12 @@ import torch
 import dgi_b200  # noqa: F401
 from dgi_b200.drafting import Sampling, pad_trees
 from dgi_b200.engine import PagedDecodeEngine
+from dgi_b200.testing import build_product_shards
+from oracle import llama_ref as L
 from test_drafted_decode_gpu import SETTINGS, Knowing, model
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
 
 
 def adopt(eng, prompts, room):
@@ -98,3 +101,82 @@ def test_a_calls_settings_end_with_it(golden, graph):
     assert single_steps(eng, prompts, 12) == drawn
     eng.set_sampling(None)
     assert single_steps(eng, prompts, 12) == want
+
+
+TEXT, FROM = 64, 40
+
+
+def text_model(golden, dtype):
+    """A model of 16-bit weights, four texts, and the same weights' logits in 32 bits from token FROM on."""
+    g = golden("tiny_decode.json")
+    cfg = L.RefConfig(**g["config"])
+    sd = {name: w.to(dtype).float() for name, w in L.make_weights(cfg, seed=0).items()}
+    texts = torch.tensor(g["prompt_ids"])[:, :TEXT]
+    (ref,) = L.build_shards(cfg, sd, [(0, 4)])
+    h, _ = ref.forward(texts, position_ids=torch.arange(TEXT)[None].expand(4, -1), use_cache=True)
+    shards = build_product_shards(cfg, sd, [(0, 4)], DEV, dtype)
+    return PagedDecodeEngine(shards, max_batch=4, max_seq_len=160, fuse_projections=True, use_cuda_graph=False), texts, ref.get_logits(h)[:, FROM:]
+
+
+def logits_by_steps(eng, texts):
+    eng.allocate(len(texts), TEXT + 2)
+    eng.prefill(texts[:, :FROM])
+    eng.logits_log = []
+    for i in range(FROM, TEXT):
+        eng.decode_step(texts[:, i])
+    out = torch.stack([x for _, _, x in eng.logits_log], 1).cpu()
+    eng.logits_log = None
+    return out
+
+
+def logits_by_trees(eng, texts, seed):
+    """One pass: the text as one path, other tokens beside it."""
+    rng = torch.Generator().manual_seed(seed)
+    trees, paths = [], []
+    for text in texts.tolist():
+        tokens, parents, path = [text[FROM]], [-1], [0]
+        for t in text[FROM + 1:]:
+            for _ in range(int(torch.randint(0, 3, (1,), generator=rng)) if len(tokens) + 2 + TEXT - FROM - len(path) < 64 else 0):
+                tokens.append(int(torch.randint(0, 1024, (1,), generator=rng)))
+                parents.append(int(torch.randint(0, len(tokens) - 1, (1,), generator=rng)))
+            parents.append(path[-1])
+            path.append(len(tokens))
+            tokens.append(t)
+        trees.append((tokens, parents))
+        paths.append(path)
+    eng.allocate(len(texts), FROM + 66)
+    eng.prefill(texts[:, :FROM])
+    seen, head = [], eng.shards[-1].get_logits
+    eng.shards[-1].get_logits = lambda h: seen.append(head(h)) or seen[-1]
+    try:
+        count, new = eng.verify_trees(*(torch.from_numpy(x) for x in pad_trees(trees, 64)))
+    finally:
+        del eng.shards[-1].get_logits
+    out = seen[-1].float().cpu()
+    assert [r[0] for r in new] == out[:, 0].argmax(-1).tolist()         # the root's answer is always among the new tokens
+    return torch.stack([out[b, path] for b, path in enumerate(paths)])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_16_bit_trees_agree_with_single_steps_up_to_rounding(golden, dtype):
+    """Single steps and trees, four sequences or one, round at the same places (trees also the softmax's weights, whose half steps average out over the
+    keys), but in other orders: logits differ, and no way may be further from 32 bits than single steps are.
+
+    An error is a sum of many roundings: of its mean square a tree's one more rounding takes less than a half, 1.25 of its root; the largest of 10^5
+    normal numbers is 4.4 deviations give or take 0.3, so twice the other's is never reached.  Greedy tokens are the same where the two largest logits are further apart than twice
+    either side's largest error, four times the single steps'."""
+    eng, texts, want = text_model(golden, dtype)
+    steps = logits_by_steps(eng, texts) - want
+    assert 0 < steps.abs().max() < 0.1 * want.std()
+    two = want.topk(2, -1).values
+    sure = two[..., 0] - two[..., 1] > 4 * steps.abs().max()
+    assert sure.any()
+    ways = [logits_by_trees(eng, texts, 1), torch.cat([logits_by_trees(eng, texts[b:b + 1], 2 + b) for b in range(4)]),
+            torch.cat([logits_by_steps(eng, texts[b:b + 1]) for b in range(4)])]
+    for got in ways:
+        off = got - want
+        print(f"{dtype}: steps {steps.square().mean().sqrt():.3e} {steps.abs().max():.3e}, here {off.square().mean().sqrt():.3e} {off.abs().max():.3e}; {sure.float().mean():.2f}")
+        assert off.square().mean().sqrt() <= 1.25 * steps.square().mean().sqrt()
+        assert off.abs().max() <= 2 * steps.abs().max()
+        assert torch.equal(got.argmax(-1)[sure], want.argmax(-1)[sure])
+    assert torch.equal((steps + want).argmax(-1)[sure], want.argmax(-1)[sure])
