@@ -367,7 +367,8 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     the context and the drafted tokens of its mask ``visible`` (int64 ``[B, nodes]``, as ``draft_tree`` gives it, or any other).  Rows behind a
     sequence's last node, and rows that see nothing, come out as 0.  Returns ``[B, nodes, Hq, D]`` (``out``, where given).  ``workspace``: at
     least ``tree_attention_workspace`` bytes that no call running at the same time uses; else one from torch's caching allocator (none for tables of
-    up to ``TREE_SHORT_KEYS`` tokens)."""
+    up to ``TREE_SHORT_KEYS`` tokens).  16-bit types round the softmax's weights before the second product; ``flags=ATTN_FORCE_GENERIC`` keeps them in fp32
+    (error against 64 bits of 64 x 8 nodes behind 2 k tokens in bf16 0.0017 of the outputs' size instead of 0.0023), without tensor cores."""
     _need_cuda(q, k_pool, v_pool, block_tables, context_lens, visible)
     max_blocks, Hkv, bs, D = _pool_dims(k_pool)
     dev, dtype = q.get_device(), q.dtype
