@@ -663,7 +663,7 @@ class PagedDecodeEngine:
     def generate_drafted(self, prompt_ids: torch.Tensor, max_new_tokens: int, drafter: Optional[Callable] = None,
                          sampling: Optional[Sequence[Sampling]] = None, nodes: int = 8) -> torch.Tensor:
         """``generate``'s tokens (as ``verify_trees`` chooses them) with several of them per pass: ``drafter(tokens of a sequence so far) -> (tokens, parents)`` proposes a tree
-        of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``), and ``verify_trees`` checks it (at the end of
+        of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``; None: no draft), and ``verify_trees`` checks it (at the end of
         ``max_seq_len`` as much of its beginning as there is room for)."""
         B, P = prompt_ids.shape
         drafter = drafter or PromptLookup(nodes)
@@ -676,6 +676,8 @@ class PagedDecodeEngine:
             want = P + max_new_tokens
             while any(len(t) < want for t in told):
                 trees = [drafter(t) if len(t) < want else None for t in told]
+                # no draft: the last token alone (a sequence without a node would rest for good)
+                trees = [tree if len(t) >= want or (tree and len(tree[0])) else ([t[-1]], [-1]) for tree, t in zip(trees, told)]
                 trees = [tree and tuple(part[:room - len(t) + 1] for part in tree) for tree, t in zip(trees, told)]
                 tokens, parents, lens = pad_trees(trees, nodes)
                 count, new = self.verify_trees(torch.from_numpy(tokens), torch.from_numpy(parents), torch.from_numpy(lens))

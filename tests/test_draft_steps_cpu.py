@@ -168,3 +168,21 @@ def test_settings_as_other_engines_write_no_limit():
     for bad in (dict(top_p=1.5), dict(top_p=-0.1), dict(top_p=float("nan")), dict(min_p=2.0), dict(temperature=-1.0), dict(top_k="many")):
         with pytest.raises(ValueError):
             Sampling.of_request({**ask, **bad})
+
+
+def test_a_drafter_without_a_draft(engine, told):
+    """No tree, or an empty one, is the last token alone: decoding goes on, a token a pass."""
+    checked = []
+    verify_root = engine.verify_trees
+
+    def verify(tokens, parents, lens):
+        checked.append((lens.tolist(), tokens[:, 0].tolist(), parents[:, 0].tolist()))
+        assert len(checked) < 10
+        return verify_root(tokens, parents, lens)
+
+    engine.verify_trees = verify
+    prompts = torch.tensor([[3, 4, 5], [6, 7, 8]])
+    for nothing in (None, ([], []), ()):
+        checked.clear()
+        assert engine.generate_drafted(prompts, 3, lambda told: nothing).tolist() == [[0, 0, 0]] * 2
+        assert checked == [([1, 1], [0, 0], [-1, -1])] * 2
