@@ -678,6 +678,9 @@ class PagedDecodeEngine:
                 trees = [drafter(t) if len(t) < want else None for t in told]
                 # no draft: the last token alone (a sequence without a node would rest for good)
                 trees = [tree if len(t) >= want or (tree and len(tree[0])) else ([t[-1]], [-1]) for tree, t in zip(trees, told)]
+                for tree, t in zip(trees, told):
+                    if tree and tree[0][0] != t[-1]:
+                        raise ValueError(f"a draft's root is the sequence's last token, {t[-1]}, not {tree[0][0]}")
                 trees = [tree and tuple(part[:room - len(t) + 1] for part in tree) for tree, t in zip(trees, told)]
                 tokens, parents, lens = pad_trees(trees, nodes)
                 count, new = self.verify_trees(torch.from_numpy(tokens), torch.from_numpy(parents), torch.from_numpy(lens))

@@ -186,3 +186,10 @@ def test_a_drafter_without_a_draft(engine, told):
         checked.clear()
         assert engine.generate_drafted(prompts, 3, lambda told: nothing).tolist() == [[0, 0, 0]] * 2
         assert checked == [([1, 1], [0, 0], [-1, -1])] * 2
+
+
+def test_a_drafter_whose_root_is_another_token(engine, told):
+    """The root stands for the last token, whose keys and values the pass appends: another one would be decoded in its place."""
+    with pytest.raises(ValueError, match="root"):
+        engine.generate_drafted(torch.tensor([[3, 4, 5]]), 3, lambda told: ([told[-1] + 1, 7], [-1, 0]))
+    assert len(told) == 1           # the prompt; no pass over trees
