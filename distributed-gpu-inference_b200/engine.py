@@ -62,7 +62,8 @@ class _TreeStep:
         pos = (context[:, None] + depth).to(torch.int64)
         total = context + self.lens
         st = PagedBatchState(block_tables=tables, context_lens=total, slot_mapping=slots.reshape(-1), max_context_len=e.max_seq_len,
-                             workspace=self.workspace, visible=visible, draft_lens=self.lens)
+                             workspace=self.workspace, attn_flags=e.state.attn_flags & ops.ATTN_FORCE_GENERIC, visible=visible,
+                             draft_lens=self.lens)
         st.cos, st.sin = rope_tables(pos, e.inv_freq, e.dtype, e.rope_scaling)
         # Behind a sequence's last node, and in drafts of other vocabularies, there may be any number: the model gets tokens, only equal ones are taken
         h = self.tokens.clamp(0, e.shards[0].embed_tokens.weight.shape[0] - 1)

@@ -549,7 +549,7 @@ class PagedLlamaDecoderLayer(nn.Module):
             ops.rope_kv_append(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cos.reshape(B * T, D), sin.reshape(B * T, D),
                                past_key_value.k_pool, past_key_value.v_pool, st.slot_mapping)
             attn = ops.paged_tree_attention(q, past_key_value.k_pool, past_key_value.v_pool, st.block_tables, st.context_lens, st.visible,
-                                            draft_lens=st.draft_lens, workspace=st.workspace).view(B, T, Hq * D)
+                                            draft_lens=st.draft_lens, workspace=st.workspace, flags=st.attn_flags).view(B, T, Hq * D)
         elif T == 1:
             # decode: RoPE on q (in place) and k, append of k / v, all in one launch; then paged attention
             qf = q[:, 0]  # [B, Hq, D], row stride = projection width

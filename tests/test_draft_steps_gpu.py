@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import dgi_b200  # noqa: F401
+from dgi_b200 import ops
 from dgi_b200.drafting import Sampling, pad_trees
 from dgi_b200.engine import PagedDecodeEngine
 from dgi_b200.testing import build_product_shards
@@ -180,3 +181,17 @@ def test_16_bit_trees_agree_with_single_steps_up_to_rounding(golden, dtype):
         assert off.abs().max() <= 2 * steps.abs().max()
         assert torch.equal(got.argmax(-1)[sure], want.argmax(-1)[sure])
     assert torch.equal((steps + want).argmax(-1)[sure], want.argmax(-1)[sure])
+
+
+def test_an_engines_choice_of_kernels_counts_for_trees(golden, monkeypatch):
+    """attn_flags=ATTN_FORCE_GENERIC: no tensor cores in single steps, and none in passes over trees."""
+    g = golden("tiny_decode.json")
+    cfg = L.RefConfig(**g["config"])
+    shards = build_product_shards(cfg, L.make_weights(cfg, seed=0), [(0, 4)], DEV, torch.bfloat16)
+    asked, attention = [], ops.paged_tree_attention
+    monkeypatch.setattr(ops, "paged_tree_attention", lambda *a, **kw: asked.append(kw.get("flags", 0)) or attention(*a, **kw))
+    for flags in (0, ops.ATTN_FORCE_GENERIC):
+        eng = PagedDecodeEngine(shards, max_batch=4, max_seq_len=160, use_cuda_graph=False, attn_flags=flags)
+        asked.clear()
+        eng.generate_drafted(torch.tensor(g["prompt_ids"])[:, :30], 3, nodes=4)
+        assert asked and set(asked) == {flags}
