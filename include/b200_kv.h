@@ -276,8 +276,8 @@ int b200_argmax_keys_decode(int64_t* out, const int64_t* keys, int64_t rows, voi
  * is the first index at which the kept weights, summed up in the row's order, exceed u[r] of their sum; u in [0, 1), what is outside counts as
  * the nearest number inside.  temperature <= 0, or a row whose largest logit is NaN or infinite: b200_argmax_rows' token.  A weight is
  * computed to 2^-31 of itself and rounded to a multiple of 2^-f of the largest, f the smaller of 44 and 62 - ceil(log2 cols); these are summed exactly: a row's
- * token does not depend on the other rows.  Settings: fp32 / int32 [rows], or NULL
- * for the *_all value in every row.  cols <= 2^20. */
+ * token does not depend on the other rows.  (So where top_p of the sum would fall on the end of a weight but for others below 2^-f - two equal largest logits,
+ * top_p 0.5, all else far below - it falls on that end.)  Settings: fp32 / int32 [rows], or NULL for the *_all value in every row.  cols <= 2^20. */
 #define B200_MAX_SAMPLE_COLS (1 << 20)
 int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64_t cols, int64_t row_stride, const float* u, const float* temperature,
                      float temperature_all, const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p,
@@ -297,7 +297,8 @@ int b200_sample_rows(int64_t* out, const void* x, int64_t rows, int64_t cols, in
  * behind the last token may hold anything; NaN and infinities in a node's values reach the rows that see it only (one in the context's, which
  * every row sees, may come out as NaN).  A table entry outside
  * the pool reads as zeros.  Scores, statistics and sums are fp32; on the tensor cores (16-bit types, heads of 64 or 128) the weights
- * are rounded to the storage type before the product with the values, with B200_ATTN_FORCE_GENERIC and elsewhere only the output is.  At most table_cols pages of a sequence are read.  q: [B, nodes, Hq, D], rows of a node contiguous; out contiguous.
+ * are rounded to the storage type before the product with the values, with B200_ATTN_FORCE_GENERIC and elsewhere only the output is.
+ * At most table_cols pages of a sequence are read.  q: [B, nodes, Hq, D], rows of a node contiguous; out contiguous.
  *   workspace : b200_paged_tree_attn_workspace bytes, 16-byte aligned, any contents; calls that may run at the same time need their own.
  *               NULL will do where table_cols pages hold up to B200_TREE_SHORT_KEYS tokens.
  *
