@@ -106,6 +106,24 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,
          c_void_p],
     ),
+    "b200_rope_kv_append_q8": (
+        c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
+    ),
+    "b200_kv_gather_dense_q8": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,
+                c_int, c_void_p],
+    ),
+    "b200_paged_decode_attn_q8_workspace": (c_size_t, [c_int] * 7),
+    "b200_paged_decode_attn_q8": (
+        c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                c_int64, c_float, c_int, c_void_p, c_size_t, c_int, c_int, c_uint, c_void_p],
+    ),
+    "b200_paged_prompt_attn_q8_workspace": (c_size_t, [c_int] * 8),
+    "b200_paged_prompt_attn_q8": (
+        c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                c_int, c_int, c_int, c_int64, c_float, c_int, c_void_p, c_size_t, c_int, c_int, c_uint, c_void_p],
+    ),
     "b200_kv_pack": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int, c_void_p]),
     "b200_kv_unpack": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int, c_void_p]),
     "b200_kv_pack_layers": (

@@ -1,0 +1,82 @@
+// What the kernels of the cache in 8 bits share (b200_kv_q8.cu, b200_attn_q8.cu, b200_prompt_q8.cu): the codes, the cache, a sequence's rows.
+//
+// A page of a kv head holds block_size x D codes and has one scale for its keys and one for its values; a code stands for code * scale.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "b200_common.cuh"
+
+namespace b200 {
+namespace q8 {
+
+// Whole numbers -127 .. 127
+struct Int8 {
+  static constexpr float kMost = 127.f;
+  static __device__ __forceinline__ float value(uint8_t c) { return static_cast<float>(static_cast<int8_t>(c)); }
+  // ties to even; what is no number becomes 0
+  static __device__ __forceinline__ uint8_t code(float y) {
+    return static_cast<uint8_t>(static_cast<int8_t>(max(-127, min(127, __float2int_rn(y)))));
+  }
+};
+// 8-bit floating point, 4 bits of exponent, 3 of mantissa, largest 448
+struct E4m3 {
+  static constexpr float kMost = 448.f;
+  static __device__ __forceinline__ float value(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
+  static __device__ __forceinline__ uint8_t code(float y) { return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3); }
+};
+
+constexpr float kLeastScale = 0x1p-60f;     // of a page that holds nothing but zeros, or numbers below 127 * 2^-60
+
+// the larger of two, no number if one is none
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+struct Cache {
+  uint8_t *k_pool, *v_pool;       // [max_blocks, Hkv, bs, D]
+  float *k_scale, *v_scale;       // [max_blocks, Hkv]
+  const int32_t* tables;
+  int table_stride, table_cols;
+  int Hkv, D, bs;
+  int64_t max_blocks;
+  // the pool's page behind a place of a sequence's table; -1 outside the table or the pool
+  __device__ __forceinline__ int page(int b, int at) const {
+    if (at < 0 || at >= table_cols) return -1;
+    const int p = tables[static_cast<int64_t>(b) * table_stride + at];
+    return p < 0 || p >= max_blocks ? -1 : p;
+  }
+  // keys of a sequence that a call may read
+  __device__ __forceinline__ int keys(int context) const {
+    return static_cast<int>(min(static_cast<int64_t>(max(context, 0)), static_cast<int64_t>(table_cols) * bs));
+  }
+};
+
+// The packed rows of a call: sequence b's new tokens are rows starts[b] .. starts[b + 1] - 1 (row b where starts is NULL), the last tokens of its
+// context_lens[b]
+struct Rows {
+  const int32_t *starts, *context_lens;
+  int B, n;
+  // first row, number of rows, tokens of the sequence with them; numbers that do not fit one another give no rows
+  __device__ __forceinline__ void of(int b, int* first, int* count, int* context) const {
+    const int a = starts ? starts[b] : b, e = starts ? starts[b + 1] : b + 1, c = context_lens[b];
+    const bool fits = a >= 0 && e >= a && e <= n && c >= e - a;
+    *first = a;
+    *count = fits ? e - a : 0;
+    *context = c;
+  }
+};
+
+}  // namespace q8
+
+// host side
+inline int check_cache(const char* name, const q8::Cache& c, int codes) {
+  if (codes != B200_CODES_INT8 && codes != B200_CODES_E4M3) return fail(B200_EINVAL, "%s: unsupported codes %d", name, codes);
+  if (c.Hkv <= 0 || c.D <= 0 || c.bs <= 0 || c.max_blocks <= 0 || c.max_blocks > INT32_MAX || c.table_cols <= 0 || c.table_stride < 0)
+    return fail(B200_EINVAL, "%s: bad sizes Hkv=%d D=%d block_size=%d max_blocks=%lld table of %d", name, c.Hkv, c.D, c.bs,
+                static_cast<long long>(c.max_blocks), c.table_cols);
+  return 0;
+}
+
+}  // namespace b200

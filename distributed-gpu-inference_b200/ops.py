@@ -854,6 +854,217 @@ def kv_gather_dense(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: to
     return k_out, v_out
 
 
+# ---- a cache in 8 bits ------------------------------------------------------------------------------------------------------------------
+CODES_ID = {torch.int8: 3, torch.float8_e4m3fn: 8}
+
+
+def _q8_cache(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor, dev: int):
+    """Checks of a cache in 8 bits and its tables; ``(shape, codes, pointers of pools, scales and tables, row stride and columns of the tables)``."""
+    codes = CODES_ID.get(k_pool.dtype)
+    if codes is None:
+        raise TypeError(f"a cache in 8 bits holds int8 or float8_e4m3fn, not {k_pool.dtype}")
+    shape = k_pool.shape
+    if len(shape) != 4 or not k_pool.is_contiguous():
+        raise ValueError("pool must be a contiguous [max_blocks, Hkv, block_size, D] tensor")
+    if v_pool.shape != shape or v_pool.dtype != k_pool.dtype or not v_pool.is_contiguous():
+        raise ValueError("k_pool and v_pool must match")
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float32 or s.shape != shape[:2] or not s.is_contiguous() or s.get_device() != dev:
+            raise ValueError("k_scale and v_scale must be contiguous fp32 [max_blocks, Hkv] on the same device")
+    if k_pool.get_device() != dev or v_pool.get_device() != dev:
+        raise ValueError("the pools must be on the same device")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.get_device() != dev:
+        raise ValueError("block_tables must be int32 [B, n] with contiguous rows, on the same device")
+    rows, cols = block_tables.shape
+    if cols == 0 or (cols > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [B, n] with contiguous rows, on the same device")
+    return shape, codes, (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+                          block_tables.stride(0) if rows > 1 else cols, cols)
+
+
+def _q8_lens(context_lens: torch.Tensor, row_starts: Optional[torch.Tensor], B: int, rows: int, dev: int):
+    """Pointers of the lengths and of the rows' starts."""
+    if context_lens.dtype != torch.int32 or context_lens.shape != (B,) or not context_lens.is_contiguous() or context_lens.get_device() != dev:
+        raise ValueError("context_lens must be a contiguous int32 [B] on the same device")
+    if row_starts is None:
+        if rows != B:
+            raise ValueError(f"{rows} rows of {B} sequences need row_starts")
+        return context_lens.data_ptr(), None
+    if row_starts.dtype != torch.int32 or row_starts.shape != (B + 1,) or not row_starts.is_contiguous() or row_starts.get_device() != dev:
+        raise ValueError("row_starts must be a contiguous int32 [B + 1] on the same device")
+    return context_lens.data_ptr(), row_starts.data_ptr()
+
+
+def rope_kv_append_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                      k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                      context_lens: torch.Tensor, row_starts: Optional[torch.Tensor] = None, max_new: Optional[int] = None,
+                      q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Rotate ``q [n, Hq, D]`` (returned: a new tensor, or ``q_out``, which may be ``q``) and ``k [n, Hkv, D]``, and write ``k`` and ``v`` into a cache in
+    8 bits: pools ``[max_blocks, Hkv, bs, D]`` int8 or float8_e4m3fn, a scale for each page and kv head in ``k_scale / v_scale`` (fp32
+    ``[max_blocks, Hkv]``).
+
+    Rows are packed: sequence b's new tokens are rows ``row_starts[b] .. row_starts[b + 1] - 1`` (int32 ``[B + 1]``; None: a row per sequence), the last of its
+    ``context_lens[b]`` tokens; ``max_new`` (default: ``n``) bounds how many a sequence has.  Where new tokens do not begin a page they share its scale with the
+    earlier ones, whose codes are put into a scale that had to grow.  ``cos / sin``: contiguous ``[n, D]`` in the storage dtype.  Other
+    than in ``rope_kv_append`` the rotation is in fp32, rounded once (queries) or not before the code (keys)."""
+    _need_cuda(k, v, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens)
+    dev, dtype = k.get_device(), k.dtype
+    (max_blocks, Hkv, bs, D), codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
+    n, B = k.shape[0], block_tables.shape[0]
+    if v.shape[0] != n or v.dtype != dtype or v.get_device() != dev:
+        raise ValueError("k and v must be [n, Hkv, D] of one dtype on one device")
+    lens, starts = _q8_lens(context_lens, row_starts, B, n, dev)
+    if (cos is None) != (sin is None) or (q is not None and cos is None):
+        raise ValueError("cos and sin come together, and with queries")
+    cp = sp = None
+    if cos is not None:
+        if cos.shape != (n, D) or sin.shape != (n, D) or not cos.is_contiguous() or not sin.is_contiguous() or cos.get_device() != dev or sin.get_device() != dev:
+            raise ValueError("cos / sin must be contiguous [n, D] on the same device")
+        if cos.dtype != dtype or sin.dtype != dtype:
+            raise TypeError("q, k, v, cos and sin must share one dtype")
+        cp, sp = cos.data_ptr(), sin.data_ptr()
+    qp = op = None
+    q_stride = o_stride = Hq = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != n or q.get_device() != dev:
+            raise ValueError("q must be [n, Hq, D] on the same device")
+        if q.dtype != dtype:
+            raise TypeError("q, k, v, cos and sin must share one dtype")
+        Hq = q.shape[1]
+        q_stride = _row_stride(q, Hq, D)
+        if q_out is None:
+            q_out = torch.empty((n, Hq, D), dtype=dtype, device=q.device)
+        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != dev:
+            raise ValueError("q_out must be a tensor like q")
+        o_stride = _row_stride(q_out, Hq, D)
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    with _on(dev) as stream:
+        rc = _lib.load().b200_rope_kv_append_q8(
+            op, o_stride, qp, q_stride, k.data_ptr(), _row_stride(k, Hkv, D), v.data_ptr(), _row_stride(v, Hkv, D), cp, sp, *cache, lens, starts, B, n,
+            n if max_new is None else int(max_new), Hq, Hkv, D, bs, max_blocks, codes, _dtype_id(k), stream)
+    if rc != 0:
+        _lib.check(rc, "b200_rope_kv_append_q8")
+    return q_out
+
+
+def kv_append_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 block_tables: torch.Tensor, context_lens: torch.Tensor, row_starts: Optional[torch.Tensor] = None,
+                 max_new: Optional[int] = None) -> None:
+    """``rope_kv_append_q8`` of keys that are rotated already, or never are."""
+    rope_kv_append_q8(None, k, v, None, None, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, row_starts, max_new)
+
+
+def kv_gather_dense_q8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                       n_tokens: int, dtype: torch.dtype = torch.bfloat16):
+    """``kv_gather_dense`` of a cache in 8 bits: the first ``n_tokens`` tokens of every row of ``block_tables`` as ``(k, v)``, each ``[B, Hkv, n_tokens, D]``
+    of ``dtype`` (code times scale, rounded once)."""
+    _need_cuda(k_pool, v_pool, k_scale, v_scale, block_tables)
+    dev = k_pool.get_device()
+    (max_blocks, Hkv, bs, D), codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
+    if dtype not in DTYPE_ID:
+        raise TypeError(f"unsupported dtype {dtype}; expected float16, bfloat16 or float32")
+    B = block_tables.shape[0]
+    if n_tokens < 0 or n_tokens > block_tables.shape[1] * bs:
+        raise ValueError(f"{n_tokens} tokens do not fit rows of {block_tables.shape[1]} blocks")
+    k_out = torch.empty((B, Hkv, n_tokens, D), dtype=dtype, device=k_pool.device)
+    v_out = torch.empty_like(k_out)
+    with _on(dev) as stream:
+        rc = _lib.load().b200_kv_gather_dense_q8(k_out.data_ptr(), v_out.data_ptr(), *cache, B, n_tokens, Hkv, D, bs, max_blocks, codes, DTYPE_ID[dtype], stream)
+    if rc != 0:
+        _lib.check(rc, "b200_kv_gather_dense_q8")
+    return k_out, v_out
+
+
+def _q8_attention(q: torch.Tensor, shape, out: Optional[torch.Tensor], dev: int):
+    """Checks of queries and outputs; ``(heads, row stride, out)``."""
+    D, Hkv = shape[3], shape[1]
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [n, Hq, {D}]")
+    n, Hq, _ = q.shape
+    if Hq % Hkv != 0:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} kv heads")
+    if out is None:
+        out = torch.empty((n, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or not out.is_contiguous() or out.dtype != q.dtype or out.get_device() != dev:
+        raise ValueError("out must be a contiguous tensor of q's shape and dtype, on its device")
+    return Hq, _row_stride(q, Hq, D), out
+
+
+def _q8_workspace(need: int, workspace: Optional[torch.Tensor], q: torch.Tensor, dev: int):
+    """``(pointer, bytes, tensor)`` of the scratch: the caller's, or one from torch's caching allocator."""
+    if workspace is None:
+        if not need:
+            return None, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous, on q's device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+@functools.lru_cache(maxsize=1024)
+def decode_attention_q8_workspace(B: int, Hq: int, Hkv: int, D: int, block_size: int, max_context_len: int, dtype: torch.dtype) -> int:
+    """Bytes of scratch that ``paged_decode_attention_q8`` needs for these sizes."""
+    return _lib.load().b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, DTYPE_ID[dtype])
+
+
+def paged_decode_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                              block_tables: torch.Tensor, context_lens: torch.Tensor, max_context_len: int, scale: Optional[float] = None,
+                              out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, flags: int = 0) -> torch.Tensor:
+    """``paged_decode_attention`` over a cache in 8 bits (as ``rope_kv_append_q8`` writes it): ``q [B, Hq, D]`` (row stride free), a token per sequence, over the
+    ``context_lens[b]`` tokens of its pages; 0 where there are none.  ``max_context_len``: the host's bound of the lengths (tokens
+    behind it may be left out).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
+    torch's caching allocator.  ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
+    _need_cuda(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens)
+    dev = q.get_device()
+    shape, codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
+    max_blocks, Hkv, bs, D = shape
+    Hq, q_stride, out = _q8_attention(q, shape, out, dev)
+    B, dt = block_tables.shape[0], _dtype_id(q)
+    lens, _ = _q8_lens(context_lens, None, B, q.shape[0], dev)
+    ws, ws_bytes, _keep = _q8_workspace(decode_attention_q8_workspace(B, Hq, Hkv, D, bs, int(max_context_len), q.dtype), workspace, q, dev)
+    with _timed(), _on(dev) as stream:
+        rc = _lib.load().b200_paged_decode_attn_q8(
+            out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, B, Hq, Hkv, D, bs, max_blocks, D ** -0.5 if scale is None else float(scale),
+            int(max_context_len), ws, ws_bytes, codes, dt, int(flags), stream)
+    if rc != 0:
+        _lib.check(rc, "b200_paged_decode_attn_q8")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def prompt_attention_q8_workspace(B: int, max_new: int, Hq: int, Hkv: int, D: int, block_size: int, max_context_len: int, dtype: torch.dtype) -> int:
+    """Bytes of scratch that ``paged_prompt_attention_q8`` needs for these sizes."""
+    return _lib.load().b200_paged_prompt_attn_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, DTYPE_ID[dtype])
+
+
+def paged_prompt_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                              block_tables: torch.Tensor, context_lens: torch.Tensor, row_starts: torch.Tensor, max_new: int, max_context_len: int,
+                              scale: Optional[float] = None, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                              flags: int = 0) -> torch.Tensor:
+    """Causal attention of new tokens over a cache in 8 bits that holds them already (``rope_kv_append_q8``), behind any context.
+
+    ``q [n, Hq, D]`` (row stride free): sequence b's rows are ``row_starts[b] .. row_starts[b + 1] - 1`` (int32 ``[B + 1]``), the last of its
+    ``context_lens[b]`` tokens; each sees the keys up to its own position.  Rows outside these are not written.  ``max_new`` and
+    ``max_context_len``: the host's bounds of a sequence's rows and of its tokens (what is behind them may be left out).  ``workspace``: at least
+    ``prompt_attention_q8_workspace`` bytes that no call running at the same time uses; None: from torch's caching allocator.
+    ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
+    _need_cuda(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, row_starts)
+    dev = q.get_device()
+    shape, codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
+    max_blocks, Hkv, bs, D = shape
+    Hq, q_stride, out = _q8_attention(q, shape, out, dev)
+    B, n, dt = block_tables.shape[0], q.shape[0], _dtype_id(q)
+    lens, starts = _q8_lens(context_lens, row_starts, B, n, dev)
+    ws, ws_bytes, _keep = _q8_workspace(prompt_attention_q8_workspace(B, int(max_new), Hq, Hkv, D, bs, int(max_context_len), q.dtype), workspace, q, dev)
+    with _timed(), _on(dev) as stream:
+        rc = _lib.load().b200_paged_prompt_attn_q8(
+            out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, starts, B, n, int(max_new), Hq, Hkv, D, bs, max_blocks,
+            D ** -0.5 if scale is None else float(scale), int(max_context_len), ws, ws_bytes, codes, dt, int(flags), stream)
+    if rc != 0:
+        _lib.check(rc, "b200_paged_prompt_attn_q8")
+    return out
+
+
 def kv_pack(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gather one layer's blocks: returns ``[2, n_blocks, Hkv, bs, D]`` (K blocks, then V blocks)."""

@@ -363,6 +363,50 @@ int b200_kv_unpack_layers(void* const* k_pools, void* const* v_pools, int n_laye
                           const int32_t* block_table, int n_blocks, int Hkv, int D, int block_size,
                           int64_t max_blocks, int dtype, void* stream);
 
+/*
+ * A cache in 8 bits.  Pools [max_blocks, Hkv, block_size, D] of codes (B200_CODES_INT8: -127 .. 127; B200_CODES_E4M3: 8-bit floating point, largest
+ * 448), and a scale of each page and kv head for its keys and its values, k_scale / v_scale fp32 [max_blocks, Hkv]: a code stands for code * scale.
+ * The rows of a call are packed: sequence b's new tokens are rows row_starts[b] .. row_starts[b + 1] - 1 (int32 [B + 1], ascending) and
+ * the last of its context_lens[b] tokens; rows before row_starts[0] and from row_starts[B] on belong to nobody and are left alone.  Numbers that do not fit one
+ * another (rows outside the call's, more than context_lens[b]) make a sequence one without rows.  At most table_cols pages of a sequence are read or
+ * written.  A table entry outside the pool reads as zeros and is not written.
+ *
+ * b200_rope_kv_append_q8: rotate-half RoPE on q [rows, Hq, D] (to q_out, which may be q; NULL: no queries) and k [rows, Hkv, D] with cos / sin [rows, D]
+ * (NULL: nothing turns), then k and v into the pools.  A page's scale becomes s = max(the one it had where it holds earlier tokens, the largest
+ * magnitude of its new tokens over the largest code, 2^-60); a new number's code is round(x (1 / s)), an earlier one's round(code (s_had (1 / s)))
+ * where s grew.  All in fp32, each operation rounded by itself, ties to even: rotated keys are not rounded to the storage type in between.  A page that new
+ * tokens begin holds nothing earlier.  A number that is not finite makes its page and head's scale one that is none, and with it what is read there.
+ *   row_starts : NULL: a row per sequence (rows == B).      max_new: no sequence has more new rows (else those behind are not written).
+ *   Pages that are written belong to one sequence each.
+ *
+ * b200_kv_gather_dense_q8: as b200_kv_gather_dense, code * scale rounded to dtype.
+ *
+ * b200_paged_decode_attn_q8: out[b, h] = softmax(q k scale) v over the context_lens[b] tokens of sequence b, 0 where there are none.
+ * b200_paged_prompt_attn_q8: the same for rows as above, each over the keys up to its own position.  No sequence has more than max_new rows or
+ * max_context_len tokens (tokens behind may be left out).  fp32 scores, statistics and sums.  q rows q_stride elements apart, out contiguous.
+ *   workspace : the *_workspace call's bytes (0: none needed), 16-byte aligned, any contents; calls that may run at the same time need their own.
+ *   flags     : B200_ATTN_FORCE_GENERIC: fp32 arithmetic, without tensor cores.
+ */
+#define B200_CODES_INT8 3      /* the wire id of int8 */
+#define B200_CODES_E4M3 8
+int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                           const void* cos_table, const void* sin_table, void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                           const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, const int32_t* row_starts, int B,
+                           int rows, int max_new, int Hq, int Hkv, int D, int block_size, int64_t max_blocks, int codes, int dtype, void* stream);
+int b200_kv_gather_dense_q8(void* k_out, void* v_out, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                            const int32_t* block_tables, int table_stride, int table_cols, int B, int n_tokens, int Hkv, int D, int block_size,
+                            int64_t max_blocks, int codes, int dtype, void* stream);
+size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype);
+int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                              const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, int B, int Hq, int Hkv, int D,
+                              int block_size, int64_t max_blocks, float scale, int max_context_len, void* workspace, size_t workspace_bytes, int codes,
+                              int dtype, unsigned flags, void* stream);
+size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype);
+int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                              const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, const int32_t* row_starts, int B, int rows,
+                              int max_new, int Hq, int Hkv, int D, int block_size, int64_t max_blocks, float scale, int max_context_len, void* workspace,
+                              size_t workspace_bytes, int codes, int dtype, unsigned flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

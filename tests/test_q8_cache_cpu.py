@@ -1,0 +1,59 @@
+"""CPU: what the entry points of the cache in 8 bits refuse before anything is launched."""
+import pytest
+import torch
+
+import dgi_b200  # noqa: F401
+from dgi_b200 import _lib, ops
+
+
+def test_host_tensors_are_refused():
+    pool, scale = torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2)
+    tables, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    for call in (lambda: ops.paged_decode_attention_q8(q, pool, pool, scale, scale, tables, lens, 16),
+                 lambda: ops.paged_prompt_attention_q8(q, pool, pool, scale, scale, tables, lens, torch.zeros(2, dtype=torch.int32), 1, 16),
+                 lambda: ops.kv_gather_dense_q8(pool, pool, scale, scale, tables, 4),
+                 lambda: ops.kv_append_q8(q[:, :2], q[:, :2], pool, pool, scale, scale, tables, lens)):
+        with pytest.raises(_lib.B200LibraryError):
+            call()
+
+
+def test_argument_errors_have_codes_and_words():
+    lib = _lib.load()
+    p = 4096      # never read: every call below is refused
+
+    def append(**over):
+        a = dict(out=p, os=512, q=p, qs=512, k=p, ks=256, v=p, vs=256, cos=p, sin=p, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, lens=p, starts=p, B=2, rows=5,
+                 most=5, Hq=4, Hkv=2, D=128, bs=16, blocks=8, codes=3, dtype=2, stream=None)
+        a.update(over)
+        return lib.b200_rope_kv_append_q8(*a.values()), lib.b200_last_error().decode()
+
+    def prompt(**over):
+        a = dict(out=p, q=p, qs=512, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, lens=p, starts=p, B=2, rows=5, most=5, Hq=4, Hkv=2, D=128, bs=16, blocks=8,
+                 scale=1.0, longest=64, ws=None, bytes=0, codes=3, dtype=2, flags=0, stream=None)
+        a.update(over)
+        return lib.b200_paged_prompt_attn_q8(*a.values()), lib.b200_last_error().decode()
+
+    def decode(**over):
+        a = dict(out=p, q=p, qs=512, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, lens=p, B=2, Hq=4, Hkv=2, D=128, bs=16, blocks=8, scale=1.0, longest=64, ws=None,
+                 bytes=0, codes=3, dtype=2, flags=0, stream=None)
+        a.update(over)
+        return lib.b200_paged_decode_attn_q8(*a.values()), lib.b200_last_error().decode()
+
+    def gather(**over):
+        a = dict(k=p, v=p, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, B=2, n=40, Hkv=2, D=128, bs=16, blocks=8, codes=3, dtype=2, stream=None)
+        a.update(over)
+        return lib.b200_kv_gather_dense_q8(*a.values()), lib.b200_last_error().decode()
+
+    for call in (append, prompt, decode, gather):
+        for over, words in ((dict(dtype=7), "dtype"), (dict(codes=5), "codes"), (dict(D=0), "sizes"), (dict(bs=0), "sizes"), (dict(blocks=0), "sizes"),
+                            (dict(blocks=2 ** 31), "sizes"), (dict(cols=0), "sizes"), (dict(B=-1), "sizes"), (dict(kp=None), "null"), (dict(t=None), "null")):
+            rc, said = call(**over)
+            assert rc == -1 and words in said, (call.__name__, over, rc, said)
+        assert call(B=0)[0] == 0
+    for call in (prompt, decode):
+        assert call(Hq=5)[0] == -2 and call(longest=-1)[0] == -1 and call(D=512)[0] == -2 and call(out=None)[0] == -1
+    assert prompt(rows=0)[0] == 0 and prompt(starts=None)[0] == -1 and prompt(most=-1)[0] == -1
+    assert append(rows=0)[0] == 0 and append(starts=None)[0] == -1 and append(sin=None)[0] == -1 and append(cos=None, sin=None)[0] == -1
+    assert append(D=33)[0] == -2 and append(q=None)[0] == -1 and append(B=2 ** 30, most=2 ** 30, rows=2 ** 30)[0] == -2
+    assert gather(n=65)[0] == -1 and gather(n=0)[0] == 0

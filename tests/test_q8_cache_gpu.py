@@ -1,0 +1,530 @@
+"""A cache in 8 bits against its definition: writing it (in elementary 32-bit operations, each rounded, so that codes and scales are equal) and
+attention over it (in 64 bits).
+
+Bounds per element of the attention, with e half a step of the type relative to a value, A = sum_j w_j |v_j| / sum_j w_j:  the output's rounding e |o|, at least
+half a step of the numbers below the type's smallest normal one n, e n (fp16 2^-25: there steps do not shrink with the value); the weights'
+rounding to fp16 2^-11 A, and 2^-31 of the largest weighted step for each that lies below fp16's normal numbers (the largest weight times scale is 2^6 at least):
+keys 2^-31 c s, c the largest code and s the largest scale; sums in 32 bits 2^-24 (keys + 8) A; scores off by d = (D + 8) 2^-24 scale sum |q k| + 2^-38 scale
+max|q| sum |k| (queries in fp16, the largest between 2^14 and 2^15) change a weight by 2 d of itself at most, and exponentials and logarithms of scales by 2^-19 of
+themselves: (2 d + 2^-19) 2 A; weights below 2^-126 of the largest (scores 87 below it) are no normal fp32 numbers and may be lost: keys 2^-126 max|v|.  In fp32 arithmetic the weights' and queries' roundings fall away."""
+import random
+
+import pytest
+import torch
+
+import dgi_b200  # noqa: F401
+from dgi_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F64 = torch.float64
+MOST = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+CODES = (torch.int8, torch.float8_e4m3fn)
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+
+
+def raw(t):
+    return t.view(torch.uint8)
+
+
+def tables_for(lens, bs, rng, spare=2, cols=None):
+    need = [-(-n // bs) for n in lens]
+    order = list(range(sum(need) + spare))
+    rng.shuffle(order)
+    cols = max(1, max(need)) if cols is None else cols
+    rows, at = [], 0
+    for n in need:
+        rows.append((order[at:at + n] + [-1] * (cols - n))[:cols])
+        at += n
+    return i32(rows), len(order)
+
+
+def cache(pages, Hkv, bs, D, codes, seed, nan_behind=None):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    pools = [(torch.randn((pages, Hkv, bs, D), generator=g, device=DEV) * MOST[codes] / 4).clamp(-MOST[codes], MOST[codes]).round().to(codes) for _ in range(2)]
+    scales = [4 / MOST[codes] * torch.exp(torch.randn((pages, Hkv), generator=g, device=DEV)) for _ in range(2)]
+    return [*pools, *scales]
+
+
+# ---- writing --------------------------------------------------------------------------------------------------------------------------
+
+def coded(y, codes):
+    return y.round().clamp(-127, 127).to(codes) if codes == torch.int8 else y.to(codes)
+
+
+def write_reference(k, v, cos, sin, k_pool, v_pool, k_scale, v_scale, tables, lens, starts):
+    """The pools and scales afterwards, a sequence, a page and a kv head at a time."""
+    Hkv, bs, D = k_pool.shape[1:]
+
+    def turned(x):
+        x, c, s = x.float(), cos.float()[:, None], sin.float()[:, None]
+        return x * c + torch.cat((-x[..., D // 2:], x[..., :D // 2]), -1) * s
+
+    out = [t.clone() for t in (k_pool, v_pool, k_scale, v_scale)]
+    for pool, scale, x in ((out[0], out[2], turned(k) if cos is not None else k.float()), (out[1], out[3], v.float())):
+        for b, length in enumerate(lens):
+            n = starts[b + 1] - starts[b]
+            held = length - n
+            for p in range(held // bs, -(-length // bs) if n else 0):
+                if p >= tables.shape[1]:
+                    continue
+                slot = int(tables[b, p])
+                if not 0 <= slot < pool.shape[0]:
+                    continue
+                t0, t1 = max(held, p * bs), min(length, (p + 1) * bs)
+                rows = x[starts[b] + t0 - held:starts[b] + t1 - held].transpose(0, 1)       # [Hkv, t, D]
+                had = scale[slot].clone() if t0 > p * bs else torch.zeros(Hkv, device=DEV)
+                now = torch.maximum(torch.maximum(had, rows.abs().amax((1, 2)) * (1.0 / MOST[pool.dtype])), torch.tensor(2.0 ** -60, device=DEV))
+                inverse = 1.0 / now
+                grew = now != had
+                old = raw(pool)[slot, :, :t0 - p * bs].clone()
+                again = coded(old.view(pool.dtype).float() * (had * inverse)[:, None, None], pool.dtype)
+                raw(pool)[slot, :, :t0 - p * bs] = torch.where(grew[:, None, None], raw(again), old)
+                raw(pool)[slot, :, t0 - p * bs:t1 - p * bs] = raw(coded(rows * inverse[:, None, None], pool.dtype))
+                scale[slot] = now
+    return out
+
+
+def write_case(new, lens, Hq, Hkv, D, bs, dtype, codes, seed=0, padding=0, cols=None, big=1.0):
+    rng, g = random.Random(seed), torch.Generator(device=DEV).manual_seed(seed)
+    starts = [sum(new[:b]) + padding for b in range(len(new) + 1)]
+    n = starts[-1] + padding
+    tables, pages = tables_for(lens, bs, rng, cols=cols)
+    normal = lambda h: (torch.randn((n, h, D), generator=g, device=DEV) * big).to(dtype)  # noqa: E731
+    angle = torch.rand((n, D // 2), generator=g, device=DEV) * 6.28
+    cos, sin = (torch.cat((t, t), 1).to(dtype) for t in (angle.cos(), angle.sin()))
+    return dict(q=normal(Hq), k=normal(Hkv), v=normal(Hkv), cos=cos, sin=sin, cache=cache(pages, Hkv, bs, D, codes, seed + 1), tables=tables, lens=lens, starts=starts)
+
+
+def check_write(c, rope=True, starts=True, max_new=None):
+    want = write_reference(c["k"], c["v"], c["cos"] if rope else None, c["sin"], *c["cache"], c["tables"], c["lens"], c["starts"])
+    got = [t.clone() for t in c["cache"]]
+    row_starts = i32(c["starts"]) if starts else None
+    if rope:
+        q = ops.rope_kv_append_q8(c["q"], c["k"], c["v"], c["cos"], c["sin"], *got, c["tables"], i32(c["lens"]), row_starts=row_starts, max_new=max_new)
+        D = q.shape[2]
+        x, co, si = c["q"].float(), c["cos"].float()[:, None], c["sin"].float()[:, None]
+        assert torch.equal(q, (x * co + torch.cat((-x[..., D // 2:], x[..., :D // 2]), -1) * si).to(q.dtype))
+    else:
+        ops.kv_append_q8(c["k"], c["v"], *got, c["tables"], i32(c["lens"]), row_starts=row_starts, max_new=max_new)
+    for a, b, name in zip(got, want, ("k_pool", "v_pool", "k_scale", "v_scale")):
+        same = torch.equal(raw(a), raw(b)) if a.dtype != torch.float32 else torch.equal(a, b)
+        assert same, f"{name}: {int((raw(a) != raw(b)).sum())} bytes differ"
+    return got
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,D,bs", [(8, 2, 128, 16), (6, 6, 64, 32), (5, 1, 128, 64), (4, 2, 96, 16), (3, 1, 34, 5), (2, 2, 64, 8), (2, 1, 256, 16)])
+def test_written_codes_are_the_definitions(Hq, Hkv, D, bs, dtype, codes):
+    new = [1, 0, 37, 16, 5, 130]
+    lens = [1, 9, 37, 48, 21, 200]
+    check_write(write_case(new, lens, Hq, Hkv, D, bs, dtype, codes, seed=D + bs, padding=2))
+    check_write(write_case(new, lens, Hq, Hkv, D, bs, dtype, codes, seed=D, padding=0), rope=False)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (80, 16)])
+def test_single_tokens_share_and_grow_a_pages_scale(D, bs, codes):
+    """One row per sequence, without row_starts: first places, places inside a page, large numbers behind small ones, empty sequences."""
+    lens = [1, 2, 16, 17, 31, 32, 33, 64, 65, 100, 7, 8]
+    c = write_case([1] * len(lens), lens, 4, 2, D, bs, torch.bfloat16, codes, seed=5)
+    c["k"][::3] *= 100
+    c["v"][1::3] *= 0.001
+    c["v"][4] = 0
+    check_write(c, starts=False)
+    none = write_case([1, 1], [3, 20], 4, 2, D, bs, torch.bfloat16, codes, seed=6)
+    before = [t.clone() for t in none["cache"]]
+    ops.kv_append_q8(none["k"], none["v"], *none["cache"], none["tables"], i32([0, -5]))
+    assert all(torch.equal(raw(a), raw(b)) for a, b in zip(none["cache"], before))
+
+
+@pytest.mark.parametrize("D", [128, 48])
+def test_token_by_token_like_the_definition(D):
+    """A sequence of 40 tokens, one at a time, then the same in portions: each step is the definition's; the values it ends with are the tokens' up to half a
+    step for each time that the scale grew."""
+    torch.manual_seed(0)
+    k, v = (torch.randn(40, 2, D, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    tables = i32([[2, 0, 1]])
+    got = [torch.zeros(4, 2, 16, D, device=DEV).to(torch.int8) for _ in range(2)] + [torch.zeros(4, 2, device=DEV) for _ in range(2)]
+    want = [t.clone() for t in got]
+    for t in range(40):
+        want = write_reference(k[t:t + 1], v[t:t + 1], None, None, *want, tables, [t + 1], [0, 1])
+        ops.kv_append_q8(k[t:t + 1], v[t:t + 1], *got, tables, i32([t + 1]))
+    assert all(torch.equal(raw(a), raw(b)) for a, b in zip(got, want))
+    dense = ops.kv_gather_dense_q8(*got, tables, 40, torch.float32)
+    for x, y, scale in ((dense[0], k, got[2]), (dense[1], v, got[3])):
+        step = scale[tables[0].long()].repeat_interleave(16, 0)[:40].T[..., None]        # [Hkv, 40, 1]
+        assert ((x[0] - y.float().transpose(0, 1)).abs() <= 0.5 * step * 16).all()
+
+
+def test_rows_of_nobody_pages_outside_and_short_tables_are_left_alone():
+    c = write_case([20, 3, 40], [30, 50, 60], 4, 2, 128, 16, torch.bfloat16, torch.int8, seed=3, padding=4, cols=3)      # 50 and 60 tokens in 3 pages
+    c["tables"][0, 1] = 10 ** 6
+    c["tables"][2, 0] = -7
+    check_write(c)
+    # starts that go backwards, beyond the rows, or have more rows than tokens: no rows
+    for starts in ([0, 70, 20, 66], [-3, 20, 23, 63], [0, 20, 23, 10 ** 6]):
+        got = [t.clone() for t in c["cache"]]
+        ops.kv_append_q8(c["k"], c["v"], *got, c["tables"], i32(c["lens"]), row_starts=i32(starts))
+    got = [t.clone() for t in c["cache"]]
+    ops.kv_append_q8(c["k"], c["v"], *got, c["tables"], i32([5, 2, 7]), row_starts=i32(c["starts"]))
+    assert all(torch.equal(raw(a), raw(b)) for a, b in zip(got, c["cache"]))
+
+
+def test_a_bound_of_new_tokens_may_be_exact_or_loose():
+    c = write_case([17, 33, 1], [17, 40, 90], 8, 4, 128, 16, torch.float16, torch.float8_e4m3fn, seed=8)
+    for most in (33, 34, 51, 4096):
+        check_write(c, max_new=most)
+
+
+def test_strided_rows_in_place_queries_and_other_streams():
+    c = write_case([5, 30], [50, 30], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=9)
+    n = c["q"].shape[0]
+    fused = torch.cat([c["q"].reshape(n, -1), c["k"].reshape(n, -1), c["v"].reshape(n, -1)], 1)
+    want_cache = [t.clone() for t in c["cache"]]
+    want = ops.rope_kv_append_q8(c["q"], c["k"], c["v"], c["cos"], c["sin"], *want_cache, c["tables"], i32(c["lens"]), row_starts=i32(c["starts"]))
+    q, k, v = fused[:, :1024].unflatten(1, (8, 128)), fused[:, 1024:1280].unflatten(1, (2, 128)), fused[:, 1280:].unflatten(1, (2, 128))
+    got = [t.clone() for t in c["cache"]]
+    args = (i32(c["lens"]), i32(c["starts"]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = ops.rope_kv_append_q8(q, k, v, c["cos"], c["sin"], *got, c["tables"], args[0], row_starts=args[1], q_out=q)
+    torch.cuda.current_stream().wait_stream(side)
+    assert out.data_ptr() == fused.data_ptr() and torch.equal(q, want)
+    assert all(torch.equal(raw(a), raw(b)) for a, b in zip(got, want_cache))
+    # odd strides: rows that start at no multiple of 16 bytes
+    wide = torch.zeros(n, 8 * 128 + 3, dtype=torch.bfloat16, device=DEV)
+    wide[:, :256] = c["k"].reshape(n, -1)
+    got = [t.clone() for t in c["cache"]]
+    k = wide[:, :256].unflatten(1, (2, 128))
+    assert torch.equal(ops.rope_kv_append_q8(c["q"], k, c["v"], c["cos"], c["sin"], *got, c["tables"], args[0], row_starts=args[1]), want)
+    assert all(torch.equal(raw(a), raw(b)) for a, b in zip(got, want_cache))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("D", [128, 40])
+def test_numbers_that_are_none_mark_their_page_and_head_alone(D, bad):
+    c = write_case([20, 20], [20, 20], 2, 2, D, 16, torch.bfloat16, torch.int8, seed=4)
+    clean = [t.clone() for t in c["cache"]]
+    ops.kv_append_q8(c["k"], c["v"], *clean, c["tables"], i32(c["lens"]), row_starts=i32(c["starts"]))
+    c["k"][3, 1, D - 1] = bad
+    c["v"][30, 0, 0] = bad
+    ops.kv_append_q8(c["k"], c["v"], *c["cache"], c["tables"], i32(c["lens"]), row_starts=i32(c["starts"]))
+    for scale, other, b, p, h in ((c["cache"][2], clean[2], 0, 0, 1), (c["cache"][3], clean[3], 1, 0, 0)):
+        page = int(c["tables"][b, p])
+        assert not torch.isfinite(scale[page, h])
+        scale[page, h] = other[page, h]
+        assert torch.equal(scale, other)
+
+
+# ---- reading back ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Hkv,D,bs,n", [(2, 128, 16, 100), (3, 64, 32, 64), (1, 128, 64, 1), (2, 36, 5, 33), (2, 64, 16, 0), (1, 96, 16, 50), (2, 64, 8, 23)])
+def test_reading_back(Hkv, D, bs, n, dtype, codes):
+    rng = random.Random(n)
+    tables, pages = tables_for([n + 3, n, n], bs, rng)
+    c = cache(pages, Hkv, bs, D, codes, 7)
+    tables[1, 0] = -1 if n else tables[1, 0]
+    k, v = ops.kv_gather_dense_q8(*c, tables, n, dtype)
+    t = torch.arange(n, device=DEV)
+    for got, pool, scale in ((k, c[0], c[2]), (v, c[1], c[3])):
+        page = tables.long()[:, t // bs]
+        at = page.clamp(0, pages - 1)
+        x = raw(pool)[at, :, t % bs].view(codes).float() * scale[at][..., None]        # [B, n, Hkv, D]
+        x = torch.where((page < 0)[..., None, None], 0.0, x)
+        assert torch.equal(got, x.transpose(1, 2).to(dtype))
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------------------
+
+def attention_reference(q, k_pool, v_pool, k_scale, v_scale, tables, lens, starts, scale, half):
+    """(values, bound) in 64 bits; `half`: weights and queries in fp16."""
+    Hkv, bs, D = k_pool.shape[1:]
+    Hq, G = q.shape[1], q.shape[1] // Hkv
+    out, bound = torch.full(q.shape, float("nan"), dtype=F64, device=DEV), torch.zeros(q.shape, dtype=F64, device=DEV)
+    e = torch.finfo(q.dtype).eps / 2
+    for b, length in enumerate(lens):
+        n = starts[b + 1] - starts[b]
+        keys = max(0, min(length, tables.shape[1] * bs))
+        pos = torch.arange(keys, device=DEV)
+        page = tables[b].long()[pos // bs]
+        bad, at = (page < 0) | (page >= k_pool.shape[0]), page.clamp(0, k_pool.shape[0] - 1)
+        k, v = (torch.where(bad[:, None, None], 0.0, raw(p)[at, :, pos % bs].view(p.dtype).to(F64) * s[at][..., None].to(F64)).repeat_interleave(G, 1)
+                for p, s in ((k_pool, k_scale), (v_pool, v_scale)))
+        qq = q[starts[b]:starts[b + 1]].to(F64)
+        see = pos[None] <= (length - n + torch.arange(n, device=DEV))[:, None]
+        s = torch.einsum("nhd,khd->nhk", qq, k) * scale
+        w = torch.where(see[:, None], s, -float("inf"))
+        w = torch.softmax(w, -1) if keys else w
+        o, A = torch.einsum("nhk,khd->nhd", w, v), torch.einsum("nhk,khd->nhd", w, v.abs())
+        d = (D + 8) * 2.0 ** -24 * abs(scale) * torch.einsum("nhd,khd->nhk", qq.abs(), k.abs())
+        if half:
+            d = d + 2.0 ** -38 * abs(scale) * qq.abs().amax(-1, keepdim=True) * k.abs().sum(-1).T[None]
+        d = torch.where(see[:, None], d, 0.0).amax(-1) if keys else torch.zeros(n, Hq, dtype=F64, device=DEV)
+        t = e * o.abs().clamp_min(torch.finfo(q.dtype).smallest_normal) + 2.0 ** -24 * (keys + 8) * A + ((2 * d + 2.0 ** -19) * 2)[..., None] * A + keys * 2.0 ** -126 * (v.abs().max() if keys else 0.0)
+        if half and keys:
+            t = t + 2.0 ** -11 * A + keys * 2.0 ** -31 * MOST[v_pool.dtype] * v_scale[at].max()
+        out[starts[b]:starts[b + 1]], bound[starts[b]:starts[b + 1]] = o, t
+    return out, bound
+
+
+def attention_case(new, lens, Hq, Hkv, D, bs, dtype, codes, seed=0, cols=None, gap=0):
+    rng, g = random.Random(seed), torch.Generator(device=DEV).manual_seed(seed)
+    tables, pages = tables_for(lens, bs, rng, cols=cols)
+    starts = [gap + sum(new[:b]) for b in range(len(new) + 1)]
+    q = (torch.randn((starts[-1] + gap, Hq, D), generator=g, device=DEV) * 1.5).to(dtype)
+    c = cache(pages, Hkv, bs, D, codes, seed)
+    if codes == torch.float8_e4m3fn:        # what is behind a sequence's last token may be no number
+        for b, n in enumerate(lens):
+            if n % bs and n // bs < tables.shape[1]:
+                for p in c[:2]:
+                    raw(p)[int(tables[b, n // bs]), :, n % bs:] = 0x7f
+    return dict(q=q, cache=c, tables=tables, lens=lens, starts=starts)
+
+
+def near(got, want, bound, what=""):
+    off = (got.to(F64) - want).abs()
+    worst = (off - bound).max().item() if off.numel() else 0.0
+    assert (off <= bound).all(), f"{what}: off by {off.max().item():.3g}, {worst:.3g} over the bound"
+
+
+SIZES = [(32, 8, 128, 16), (8, 8, 64, 16), (16, 2, 64, 32), (10, 2, 128, 64), (12, 1, 128, 16), (32, 2, 128, 32), (4, 2, 96, 16), (3, 1, 33, 5), (4, 4, 256, 16), (4, 2, 128, 8)]
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,D,bs", SIZES)
+def test_decode_attention(Hq, Hkv, D, bs, dtype, codes):
+    lens = [1, 16, 17, 0, 250, 64, 333, 1000]
+    c = attention_case([1] * len(lens), lens, Hq, Hkv, D, bs, dtype, codes, seed=D + Hq)
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, dtype != torch.float32)
+    got = ops.paged_decode_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), max(lens))
+    assert (got[3] == 0).all()
+    keep = [b for b in range(len(lens)) if b != 3]
+    near(got[keep], want[keep], bound[keep])
+    plain = ops.paged_decode_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), max(lens), flags=ops.ATTN_FORCE_GENERIC)
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, False)
+    near(plain[keep], want[keep], bound[keep], "fp32 arithmetic")
+
+
+@pytest.mark.parametrize("B,context", [(1, 5000), (1, 40000), (3, 9001), (40, 700), (64, 130)])
+@pytest.mark.parametrize("codes", CODES)
+def test_decode_attention_of_few_long_and_many_short_sequences(B, context, codes):
+    rng = random.Random(B)
+    lens = [context] + [rng.randint(1, context) for _ in range(B - 1)]
+    c = attention_case([1] * B, lens, 16, 4, 128, 16, torch.bfloat16, codes, seed=B)
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], 128 ** -0.5, True)
+    near(ops.paged_decode_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), context), want, bound)
+    near(ops.paged_decode_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), 4 * context), want, bound, "a loose bound of the lengths")
+
+
+PORTIONS = [([1, 1, 1], [1, 40, 300]), ([5, 0, 33, 2], [5, 7, 100, 64]), ([150], [150]), ([129, 64], [700, 64]), ([300, 1, 17, 63], [300, 999, 17, 1500])]
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("Hq,Hkv,D,bs", SIZES)
+def test_prompt_attention(Hq, Hkv, D, bs, dtype, codes):
+    for i, (new, lens) in enumerate(PORTIONS):
+        c = attention_case(new, lens, Hq, Hkv, D, bs, dtype, codes, seed=D + Hq + i, gap=i)
+        want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, dtype != torch.float32)
+        out = torch.full_like(c["q"], 7.0)
+        ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(new), max(lens), out=out)
+        a, e = c["starts"][0], c["starts"][-1]
+        near(out[a:e], want[a:e], bound[a:e], str(new))
+        assert (out[:a] == 7).all() and (out[e:] == 7).all()
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("new,lens", [([600], [9000]), ([40], [30000]), ([2000, 3], [2000, 5000]), ([9] * 30, list(range(300, 3300, 100)))])
+def test_prompt_attention_of_long_contexts(new, lens, codes):
+    c = attention_case(new, lens, 8, 2, 128, 16, torch.bfloat16, codes, seed=len(new))
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], 128 ** -0.5, True)
+    near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(new), max(lens)), want, bound)
+    near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(new) + 100, max(lens) * 2), want, bound, "loose bounds")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.7])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_any_scale(scale, dtype):
+    new, lens = [1, 30], [200, 90]
+    c = attention_case(new, lens, 8, 2, 128, 16, dtype, torch.int8, seed=1)
+    c["q"] *= 0.3
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], scale, dtype != torch.float32)
+    near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), 30, 200, scale=scale), want, bound)
+    one = attention_case([1, 1], lens, 8, 2, 128, 16, dtype, torch.int8, seed=1)
+    want, bound = attention_reference(one["q"], *one["cache"], one["tables"], lens, one["starts"], scale, dtype != torch.float32)
+    near(ops.paged_decode_attention_q8(one["q"], *one["cache"], one["tables"], i32(lens), 200, scale=scale), want, bound)
+
+
+def test_large_and_small_queries_and_scales():
+    """Queries far above and below fp16's range, values' scales 2^40 apart, a page of zeros at the smallest scale."""
+    lens = [120, 120]
+    c = attention_case([1, 1], lens, 4, 2, 128, 16, torch.bfloat16, torch.int8, seed=2)
+    c["q"][0] *= 2.0 ** 100
+    c["cache"][2] *= 2.0 ** -100
+    c["q"][1] *= 2.0 ** -20
+    page = c["tables"][1].tolist()
+    c["cache"][3][page[0]] *= 2.0 ** 20
+    c["cache"][3][page[1]] *= 2.0 ** -20
+    c["cache"][3][page[2]] = 2.0 ** -60
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], 128 ** -0.5, True)
+    near(ops.paged_decode_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), 120), want, bound)
+    near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), 1, 120), want, bound)
+
+
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_scales_that_are_no_numbers_reach_the_rows_that_see_them(which, bad):
+    new, lens = [40, 40], [100, 40]
+    c = attention_case(new, lens, 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=3)
+    clean = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), 40, 100)
+    c["cache"][which][int(c["tables"][0, 5]), 1] = bad        # tokens 80 .. 95 of sequence 0: rows 20 on see them
+    got = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), 40, 100)
+    assert not torch.isfinite(got[20:40, 4:]).any() if bad != bad else not torch.isfinite(got[36:40, 4:]).all()
+    assert torch.equal(got[:, :4], clean[:, :4]) and torch.equal(got[40:], clean[40:])
+    one = ops.paged_decode_attention_q8(c["q"][[39, 79]], *c["cache"], c["tables"], i32(lens), 100)
+    assert not torch.isfinite(one[0, 4:]).all() and torch.isfinite(one[0, :4]).all() and torch.isfinite(one[1]).all()
+
+
+def test_bad_tables_read_zeros_and_short_tables_end_the_context():
+    new, lens = [3, 20], [90, 100]
+    c = attention_case(new, lens, 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=4, cols=6)      # 96 tokens
+    c["tables"][0, 2] = -3
+    c["tables"][0, 4] = 2 ** 30
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], 128 ** -0.5, True)
+    got = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), 20, 100)
+    near(got, want, bound)
+    lens = [90, 100]
+    one = attention_case([1, 1], lens, 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=4, cols=6)
+    one["tables"][0, 2] = -3
+    want, bound = attention_reference(one["q"], *one["cache"], one["tables"], lens, one["starts"], 128 ** -0.5, True)
+    near(ops.paged_decode_attention_q8(one["q"], *one["cache"], one["tables"], i32(lens), 100), want, bound)
+
+
+def test_lengths_that_do_not_fit_give_no_rows():
+    c = attention_case([3, 20], [90, 100], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=5)
+    for lens, starts in (([90, 10], [0, 3, 23]), ([90, 100], [0, 3, 10 ** 6]), ([90, 100], [0, 3, -5])):
+        out = torch.full_like(c["q"], 7.0)
+        ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(starts), 20, 100, out=out)
+        assert (out[3:] == 7).all() and not (out[:3] == 7).all()
+    assert (ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], i32([0, -9]), 100) == 0).all()
+
+
+def test_captured_calls_replay_with_new_lengths_and_rows():
+    c = attention_case([4, 20], [700, 900], 16, 4, 128, 16, torch.bfloat16, torch.int8, seed=6)
+    lens, starts = i32([100, 200]), i32([0, 4, 24])
+    out, one = torch.zeros_like(c["q"]), torch.zeros_like(c["q"][:2])
+    g = torch.cuda.CUDAGraph()
+
+    def calls():
+        ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], lens, starts, 20, 900, out=out)
+        ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], lens, 900, out=one)
+
+    calls()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        calls()
+    for l in ([700, 900], [4, 20], [555, 311]):
+        lens.copy_(i32(l))
+        g.replay()
+        want, bound = attention_reference(c["q"], *c["cache"], c["tables"], l, [0, 4, 24], 128 ** -0.5, True)
+        near(out, want, bound, str(l))
+        want, bound = attention_reference(c["q"][:2], *c["cache"], c["tables"], l, [0, 1, 2], 128 ** -0.5, True)
+        near(one, want, bound, str(l))
+
+
+def test_two_streams_at_once_and_strided_queries():
+    c = attention_case([64, 64], [3000, 2000], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=7)
+    lens, starts = i32(c["lens"]), i32(c["starts"])
+    want = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], lens, starts, 64, 3000)
+    ones = ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], lens, 3000)
+    wide = torch.zeros(128, 3, 8, 128, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1] = c["q"]
+    odd = torch.zeros(128, 8 * 128 + 1, dtype=torch.bfloat16, device=DEV)
+    odd[:, 1:] = c["q"].flatten(1)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((ops.paged_prompt_attention_q8(wide[:, 1], *c["cache"], c["tables"], lens, starts, 64, 3000),
+                            ops.paged_decode_attention_q8(wide[:2, 1], *c["cache"], c["tables"], lens, 3000)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, ones) for a, b in got)
+    exact, bound = attention_reference(c["q"], *c["cache"], c["tables"], c["lens"], c["starts"], 128 ** -0.5, True)
+    near(ops.paged_prompt_attention_q8(odd[:, 1:].unflatten(1, (8, 128)), *c["cache"], c["tables"], lens, starts, 64, 3000), exact, bound)
+
+
+def test_written_then_read_like_a_prompt_and_its_decoding():
+    """Portions written and attended to, then single tokens: as attention over the tokens themselves, up to half a step of their pages' codes."""
+    torch.manual_seed(3)
+    B, Hq, Hkv, D, T = 3, 8, 2, 128, 70
+    k, v, q = (torch.randn(B, T, h, D, device=DEV, dtype=torch.bfloat16) for h in (Hkv, Hkv, Hq))
+    tables = i32([[4, 9, 2, 7, 11], [0, 1, 3, 5, 6], [8, 10, 12, 13, 14]])
+    pools = [torch.zeros(15, Hkv, 16, D, device=DEV, dtype=torch.int8) for _ in range(2)] + [torch.zeros(15, Hkv, device=DEV) for _ in range(2)]
+    for lo, hi in ((0, 40), (40, 53), (53, 54), (54, 70)):
+        n = hi - lo
+        rows = [x[:, lo:hi].reshape(B * n, -1, D).contiguous() for x in (q, k, v)]
+        lens, starts = i32([hi] * B), i32([i * n for i in range(B + 1)])
+        ops.kv_append_q8(rows[1], rows[2], *pools, tables, lens, row_starts=starts, max_new=n)
+        if n == 1:
+            got = ops.paged_decode_attention_q8(rows[0], *pools, tables, lens, hi)
+        else:
+            got = ops.paged_prompt_attention_q8(rows[0], *pools, tables, lens, starts, n, hi)
+        kk, vv = (x[:, :hi].float().transpose(1, 2).repeat_interleave(Hq // Hkv, 1) for x in (k, v))
+        s = torch.einsum("bnhd,bhkd->bhnk", q[:, lo:hi].float(), kk) * D ** -0.5
+        s = s.masked_fill(torch.arange(hi, device=DEV)[None] > torch.arange(lo, hi, device=DEV)[:, None], -float("inf"))
+        want = torch.einsum("bhnk,bhkd->bnhd", torch.softmax(s, -1), vv).reshape(B * n, Hq, D)
+        rel = ((got.float() - want).norm() / want.norm()).item()
+        # a step is max / 127 with max about 4.5 of the standard deviation: errors uniform in half a step, 4.5 / 127 / sqrt(12) = 0.0102 of the values, and the
+        # scores off by as much (their deviation is 1), which moves the weights; rescaled pages twice that, bf16 0.0017
+        assert rel < 0.04, rel
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------------------------
+
+def test_refusals():
+    c = attention_case([3, 20], [90, 100], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=8)
+    k_pool, v_pool, k_scale, v_scale = c["cache"]
+    lens, starts = i32(c["lens"]), i32(c["starts"])
+    prompt = lambda **over: ops.paged_prompt_attention_q8(**{**dict(  # noqa: E731
+        q=c["q"], k_pool=k_pool, v_pool=v_pool, k_scale=k_scale, v_scale=v_scale, block_tables=c["tables"], context_lens=lens, row_starts=starts, max_new=20,
+        max_context_len=100), **over})
+    prompt()
+    with pytest.raises(TypeError):
+        prompt(k_pool=k_pool.to(torch.bfloat16), v_pool=v_pool.to(torch.bfloat16))
+    with pytest.raises(TypeError):
+        prompt(q=c["q"].double())
+    for over in (dict(v_pool=v_pool[:-1]), dict(k_scale=k_scale.half()), dict(v_scale=v_scale.T.contiguous().T), dict(k_pool=k_pool[:, :, ::2]),
+                 dict(block_tables=c["tables"].long()), dict(block_tables=c["tables"][:1]), dict(context_lens=lens.long()), dict(row_starts=starts[:-1]),
+                 dict(q=c["q"][..., :64]), dict(q=c["q"][:, :7]), dict(out=c["q"][:5]), dict(out=c["q"].float()), dict(block_tables=c["tables"].cpu().to(DEV)[:, :0])):
+        with pytest.raises(ValueError):
+            prompt(**over)
+    with pytest.raises(_lib.B200LibraryError):
+        prompt(q=c["q"].cpu())
+    with pytest.raises(_lib.B200LibraryError):
+        prompt(max_new=-1)
+    with pytest.raises(ValueError):
+        ops.paged_decode_attention_q8(c["q"], k_pool, v_pool, k_scale, v_scale, c["tables"], lens, 100)
+    with pytest.raises(ValueError):
+        ops.kv_gather_dense_q8(k_pool, v_pool, k_scale, v_scale, c["tables"], 10 ** 6)
+    with pytest.raises(TypeError):
+        ops.kv_gather_dense_q8(k_pool, v_pool, k_scale, v_scale, c["tables"], 5, torch.int8)
+    w = write_case([3, 20], [90, 100], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=8)
+    write = lambda **over: ops.rope_kv_append_q8(**{**dict(  # noqa: E731
+        q=w["q"], k=w["k"], v=w["v"], cos=w["cos"], sin=w["sin"], k_pool=k_pool, v_pool=v_pool, k_scale=k_scale, v_scale=v_scale, block_tables=c["tables"],
+        context_lens=lens, row_starts=starts), **over})
+    for over in (dict(cos=None), dict(cos=None, sin=None), dict(row_starts=None), dict(k=w["k"][:5]), dict(cos=w["cos"][:, :64]), dict(v=w["v"].float()),
+                 dict(k=w["k"].transpose(1, 2)), dict(q_out=w["q"].float())):
+        with pytest.raises(ValueError):
+            write(**over)
+    with pytest.raises(TypeError):
+        write(cos=w["cos"].float())
+    with pytest.raises(TypeError):
+        write(q=w["q"].float())
