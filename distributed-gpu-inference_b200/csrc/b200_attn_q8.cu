@@ -6,7 +6,9 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "b200_attn.cuh"
 #include "b200_q8.cuh"
+#include "b200_tcgen05.cuh"
 
 namespace b200 {
 namespace {
@@ -125,6 +127,353 @@ __global__ void __launch_bounds__(kAnyWarps * 32) attn_any_kernel(const Attn A, 
   }
 }
 
+// ---- one token per sequence: 16-bit types, heads of 64 or 128, pages of 16s ---------------------------------------------------------------------
+// A CTA of four warps per (part of the keys, kv head and up to 8 of its query heads, sequence); a warp takes every fourth tile of 16 tokens and keeps kStages of them
+// under way, a TMA copy of 16 x D codes for the keys and one for the values each, in 128-byte lines whose 16-byte pieces are swizzled.  (Many short items: a warp
+// per item, which then waits for nobody.)
+//
+//   S^T[token, head] = K Q^T   mma.m16n8k16, the codes as fp16: exact, for both kinds.  Queries in fp16 too, by a power of two of their own brought to 2^14 .. 2^15
+//                              at the largest, so that what fp16 loses lies 2^-38 below it; the 8-wide side holds the heads, nothing is padded
+//   w = 2^(S t + log2 s - m)   t the page's key scale with all else, s its value scale: the weights carry it, so that they meet bare codes; the sum counts w / s.
+//                              m moves when a score is 2^8 above it; the largest weight lies between 2^6 and 2^14, and rounding to fp16 is by 2^-12 of
+//                              a weight at most, for weights down to 2^-20 of the largest
+//   O^T[d, head] += V^T w^T    the values by ldmatrix.trans, whose pairs of bytes are two tokens' codes of neighbouring columns
+//
+// The order of columns inside a product is free as long as both sides agree: a lane's 4 bytes of a key's 16 are its 4 columns there, and its rows of the output
+// are two neighbouring columns.  A byte becomes fp16 as the low byte of 1024 + code + 128 (int8) or by the conversion that the hardware has (e4m3).
+constexpr int kWarps = 4, kTok = 16;
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four codes as two pairs of fp16: (0, 1) and (2, 3), or across (0, 2) and (1, 3)
+template <typename C, bool ACROSS>
+__device__ __forceinline__ void halves(uint32_t codes, uint32_t& a, uint32_t& b) {
+  if constexpr (std::is_same_v<C, q8::Int8>) {
+    const uint32_t u = codes ^ 0x80808080u, bias = 0x64806480u;       // 1024 + 128
+    a = __byte_perm(u, 0x64646464u, ACROSS ? 0x4240 : 0x4140);
+    b = __byte_perm(u, 0x64646464u, ACROSS ? 0x4341 : 0x4342);
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(bias));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(bias));
+  } else {
+    uint32_t lo, hi;
+    asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(codes));
+    a = ACROSS ? __byte_perm(lo, hi, 0x5410) : lo;
+    b = ACROSS ? __byte_perm(lo, hi, 0x7632) : hi;
+  }
+}
+
+template <int D>
+struct DecodePlan {
+  static constexpr int kStages = 4, kTile = kTok * D, kStage = 2 * kTile;       // bytes: keys, then values
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kBars = kRing, kDead = kBars + kWarps * kStages * 8, kEnd = kDead + 16;
+  static constexpr int kSmem = kEnd + 1024;
+  static_assert(kWarps * 8 * (D + 2) * 4 <= kRing, "outputs go where the tiles were");
+};
+// byte of (token, 16-byte piece) in a tile: lines of 128 bytes, a token each or two
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int token, int piece) {
+  const int line = D == 128 ? token : token >> 1, p = D == 128 ? piece : (token & 1) * 4 + piece;
+  return line * 128 + ((p ^ (line & 7)) << 4);
+}
+
+struct Decode {
+  Attn a;
+  int heads, blocks;              // query heads of a kv head; blocks of up to 8 of them
+  int tiles_per_split, splits, items;
+  float *ws_acc, *ws_ml;          // [B, Hq, splits, D], [B, Hq, splits, 2]
+};
+
+template <typename T, typename C, int D, bool WARPITEM>
+__global__ void __launch_bounds__(kWarps * 32, 3)
+decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using S = DecodePlan<D>;
+  constexpr int kStages = S::kStages, kPieces = D / 16, kStep = WARPITEM ? 1 : kWarps;
+  const Cache& c = P.a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, tq = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int item = WARPITEM ? blockIdx.x * kWarps + warp : blockIdx.x, ofs = WARPITEM ? 0 : warp;
+  if (item >= P.items) return;        // (only warps of their own items)
+  const int split = item % P.splits, rest = item / P.splits, block = rest % P.blocks, kvh = rest / P.blocks % c.Hkv, b = rest / P.blocks / c.Hkv;
+  const int head0 = kvh * P.heads + block * 8, G = min(8, P.heads - block * 8);
+
+  extern __shared__ unsigned char raw_smem[];
+  unsigned char* sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
+  const uint32_t ring = smem_u32(sm) + warp * kStages * S::kStage, bars = smem_u32(sm + S::kBars) + warp * kStages * 8;
+  volatile int* dead = reinterpret_cast<volatile int*>(sm + S::kDead) + (WARPITEM ? warp : 0);
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + s * 8));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (WARPITEM || warp == 0) *dead = 0;
+  }
+  if constexpr (WARPITEM) __syncwarp();
+  else __syncthreads();
+
+  const int keys = c.keys(P.a.r.context_lens[b]), tiles = (keys + kTok - 1) / kTok;
+  const int t0 = min(tiles, split * P.tiles_per_split), t1 = split == P.splits - 1 ? tiles : min(tiles, t0 + P.tiles_per_split);
+  const int mine = t1 - t0 > ofs ? (t1 - t0 - ofs + kStep - 1) / kStep : 0;       // tiles t0 + ofs, and every kStep-th
+  const int per_page = c.bs / kTok;
+
+  // Pages of 32 tiles at a time, a lane each, and their scales: the next ones under way while these are used
+  auto page_at = [&](int j) -> int {        // of the warp's tile j; outside the pool: behind it, where copies bring zeros
+    if (j >= mine) return 0;
+    const int p = c.page(b, (t0 + ofs + j * kStep) / per_page);
+    return p < 0 ? static_cast<int>(c.max_blocks) : p;
+  };
+  auto scales_of = [&](int page, int j, float& ks, float& vs) {
+    ks = vs = 1.f;
+    if (j < mine && page < c.max_blocks) {
+      ks = c.k_scale[static_cast<int64_t>(page) * c.Hkv + kvh];
+      vs = q8::max_nan(c.v_scale[static_cast<int64_t>(page) * c.Hkv + kvh], q8::kLeastScale);
+    }
+  };
+  int pages = page_at(lane), pages_next = page_at(32 + lane), window = 0;
+  float ks, vs, ks_next, vs_next;
+  auto issue = [&](int j) {
+    if (j - window >= 32) {
+      window += 32;
+      pages = pages_next;
+      pages_next = page_at(window + 32 + lane);
+      scales_of(pages, window + lane, ks_next, vs_next);
+    }
+    const int page = __shfl_sync(0xffffffffu, pages, j - window);
+    if (lane == 0) {
+      const uint32_t to = ring + j % kStages * S::kStage, bar = bars + j % kStages * 8;
+      const int tile = t0 + ofs + j * kStep, line = ((page * c.Hkv + kvh) * c.bs + tile % per_page * kTok) / (128 / D);
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStage) : "memory");
+      asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(&k_map), "r"(0), "r"(line), "r"(bar) : "memory");
+      asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to + S::kTile), "l"(&v_map), "r"(0), "r"(line), "r"(bar) : "memory");
+    }
+  };
+  const int ahead = min(kStages, mine);
+  for (int j = 0; j < ahead; ++j) issue(j);
+  scales_of(pages, lane, ks, vs);
+  vs = log2f(vs);
+
+  // queries: head quad's columns 16 i + 4 tq .. + 3
+  uint32_t qf[kPieces][2];
+  float factor[2];        // of heads 2 tq and 2 tq + 1
+  {
+    const T* q = static_cast<const T*>(P.a.q) + b * P.a.q_stride + static_cast<int64_t>(head0 + quad) * D + 4 * tq;
+    uint2 raw[kPieces];
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) raw[i] = quad < G ? *reinterpret_cast<const uint2*>(q + 16 * i) : make_uint2(0u, 0u);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) most = fmaxf(most, fabsf(Cvt<T>::to_f32(e[u])));
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) - 14;       // most = 2^(e + 14) .. 2^(e + 15)
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const T* x = reinterpret_cast<const T*>(&raw[i]);
+      qf[i][0] = pack2<__half>(Cvt<T>::to_f32(x[0]) * down, Cvt<T>::to_f32(x[1]) * down);
+      qf[i][1] = pack2<__half>(Cvt<T>::to_f32(x[2]) * down, Cvt<T>::to_f32(x[3]) * down);
+    }
+    const float f = P.a.scale * 1.4426950408889634f * up;
+    factor[0] = __shfl_sync(0xffffffffu, f, 8 * tq);
+    factor[1] = __shfl_sync(0xffffffffu, f, 8 * tq + 4);
+  }
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kPieces][4];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  const int my_token = (lane >> 3 & 1) * 8 + (lane & 7), my_piece = lane >> 4;       // of four 8 x 8 matrices: tokens 0 - 7, 8 - 15, the next piece's
+  bool ok = true;
+  for (int i = 0; i < mine; ++i) {
+    if ((i & 31) == 0 && i > 0) ks = ks_next, vs = log2f(vs_next);
+    const int tile = t0 + ofs + i * kStep;
+    const uint32_t k_tile = ring + i % kStages * S::kStage, v_tile = k_tile + S::kTile;
+    ok = __all_sync(0xffffffffu, bar_wait1(bars + i % kStages * 8, (i / kStages) & 1, dead));
+    if (!ok) break;
+    const float kt = __shfl_sync(0xffffffffu, ks, i & 31), ls = __shfl_sync(0xffffffffu, vs, i & 31);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < kPieces; p += 2) {
+      uint32_t r[4];
+      ldsm4(r, k_tile + tile_at<D>(my_token, p + my_piece));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a0, a1, a2, a3;
+        halves<C, false>(r[2 * u], a0, a2);
+        halves<C, false>(r[2 * u + 1], a1, a3);
+        mma16(s, a0, a1, a2, a3, qf[p + u][0], qf[p + u][1]);
+      }
+    }
+    // s[0], s[1]: token quad, heads 2 tq and 2 tq + 1; s[2], s[3]: token quad + 8
+    const int left = keys - tile * kTok;        // tokens of the tile
+    const float f0 = factor[0] * kt, f1 = factor[1] * kt;
+    float x[4] = {fmaf(s[0], f0, ls), fmaf(s[1], f1, ls), fmaf(s[2], f0, ls), fmaf(s[3], f1, ls)};
+    if (left < kTok) {
+      if (quad >= left) x[0] = x[1] = -INFINITY;
+      if (quad + 8 >= left) x[2] = x[3] = -INFINITY;
+      if constexpr (std::is_same_v<C, q8::E4m3>) {       // what is behind the last token may be no number
+        for (int e = left * kPieces + lane; e < kTok * kPieces; e += 32)
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(v_tile + tile_at<D>(e / kPieces, e % kPieces)), "r"(0) : "memory");
+        __syncwarp();
+      }
+    }
+    if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[0] + 14.f || fmaxf(x[1], x[3]) > m[1] + 14.f)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = fmaxf(x[h], x[h + 2]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float now = fmaxf(m[h], top - 6.f), corr = m[h] == -INFINITY ? 0.f : exp2_fast(m[h] - now);
+        m[h] = now;
+        l[h] *= corr;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) o[p][h] *= corr, o[p][h + 2] *= corr;
+      }
+    }
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[e] - m[e & 1]);
+    const float per = exp2_fast(-ls);
+    l[0] = fmaf(w[0] + w[2], per, l[0]);
+    l[1] = fmaf(w[1] + w[3], per, l[1]);
+    const uint32_t b0 = transposed(pack2<__half>(w[0], w[1])), b1 = transposed(pack2<__half>(w[2], w[3]));
+#pragma unroll
+    for (int p = 0; p < kPieces; p += 2) {
+      uint32_t r[4];
+      ldsm4_trans(r, v_tile + tile_at<D>(my_token, p + my_piece));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a0, a1, a2, a3;
+        halves<C, true>(r[2 * u], a0, a1);
+        halves<C, true>(r[2 * u + 1], a2, a3);
+        mma16(o[p + u], a0, a1, a2, a3, b0, b1);
+      }
+    }
+    __syncwarp();       // every lane has read the buffer
+    if (i + kStages < mine) issue(i + kStages);
+  }
+  if (!ok) {      // a wait gave up: what is under way gets 10 ms to end; no number comes out
+    for (const long long begun = clock64(); clock64() - begun < 20000000ll;) {}
+    l[0] = l[1] = NAN;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+  }
+  // ---- outputs: columns 16 p + 2 quad and + 1, heads 2 tq and 2 tq + 1, of the warps' parts, where the tiles were ------------------------------
+  constexpr int kSets = WARPITEM ? 1 : kWarps;
+  if constexpr (WARPITEM) __syncwarp();
+  else __syncthreads();
+  float* o_s = reinterpret_cast<float*>(sm + (WARPITEM ? warp * kStages * S::kStage : 0));      // [set][8][D]
+  float *m_s = o_s + kSets * 8 * D, *l_s = m_s + kSets * 8;
+  const int set = WARPITEM ? 0 : warp;
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(o_s + (set * 8 + 2 * tq + h) * D + 16 * p + 2 * quad) = make_float2(o[p][h], o[p][h + 2]);
+  }
+  if (quad == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) m_s[set * 8 + 2 * tq + h] = m[h], l_s[set * 8 + 2 * tq + h] = l[h];
+  }
+  if constexpr (WARPITEM) __syncwarp();
+  else __syncthreads();
+  for (int e = WARPITEM ? lane : threadIdx.x; e < G * (D / 2); e += WARPITEM ? 32 : kWarps * 32) {
+    const int g = e / (D / 2), d = e % (D / 2) * 2;
+    float top = -INFINITY, sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSets; ++w) top = fmaxf(top, m_s[w * 8 + g]);
+#pragma unroll
+    for (int w = 0; w < kSets; ++w) {
+      const float mw = m_s[w * 8 + g], lw = l_s[w * 8 + g], k = mw == -INFINITY ? (lw != lw ? 1.f : 0.f) : exp2_fast(mw - top);
+      const float2 v = *reinterpret_cast<const float2*>(o_s + (w * 8 + g) * D + d);
+      sum = fmaf(lw, k, sum);
+      a0 = fmaf(v.x, k, a0);
+      a1 = fmaf(v.y, k, a1);
+    }
+    const int64_t row = static_cast<int64_t>(b) * P.a.Hq + head0 + g;
+    if (P.splits == 1) {
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + row * D + d) = pack2<T>(a0 * f, a1 * f);
+    } else {
+      const int64_t part = row * P.splits + split;
+      *reinterpret_cast<float2*>(P.ws_acc + part * D + d) = make_float2(a0, a1);
+      if (d == 0) *reinterpret_cast<float2*>(P.ws_ml + part * 2) = make_float2(top * 0.6931471805599453f, sum);
+    }
+  }
+}
+
+// The pool as lines of 128 bytes, fetched 16 tokens at a time; lines behind the pool read as zeros
+bool code_map(CUtensorMap* map, const void* pool, const Cache& c) {
+  const Encode encode = tensor_map_encode();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {128, static_cast<cuuint64_t>(c.max_blocks) * c.Hkv * c.bs / (128 / c.D)}, strides[1] = {128};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(kTok / (128 / c.D))}, step[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool decode_serves(int D, int bs, int dtype) { return dtype != B200_DTYPE_F32 && (D == 64 || D == 128) && bs % kTok == 0; }
+
+// Parts of the keys
+constexpr int kMostSplits = 256;        // that are put together
+int decode_splits(int B, int Hq, int Hkv, int bs, int longest) {
+  const int64_t items = static_cast<int64_t>(B) * Hkv * ((Hq / Hkv + 7) / 8), tiles = (longest + kTok - 1) / kTok;
+  int64_t splits = items >= 2 * kNumSMs ? 1 : (3 * kNumSMs + items - 1) / items;
+  (void)bs;
+  splits = splits < 1 ? 1 : splits;
+  const int64_t most = (tiles + 15) / 16;       // 16 tiles a part at least
+  splits = splits < most ? splits : most > 1 ? most : 1;
+  return static_cast<int>(splits < kMostSplits ? splits : kMostSplits);
+}
+
+template <typename T, typename C, int D, bool WARPITEM>
+int launch_decode_as(const char* name, const Decode& P, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
+  auto kern = decode_kernel<T, C, D, WARPITEM>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodePlan<D>::kSmem);
+  kern<<<WARPITEM ? (P.items + kWarps - 1) / kWarps : P.items, kWarps * 32, DecodePlan<D>::kSmem, stream>>>(P, k_map, v_map);
+  return check_launch(name);
+}
+
+template <typename T>
+int launch_decode(const char* name, const Attn& A, int splits, int longest, void* workspace, int codes, int dtype, cudaStream_t stream) {
+  Decode P{};
+  P.a = A, P.heads = A.Hq / A.c.Hkv, P.blocks = (P.heads + 7) / 8, P.splits = splits;
+  const int tiles = static_cast<int>((static_cast<int64_t>(longest) + kTok - 1) / kTok);
+  P.tiles_per_split = tiles > 0 ? (tiles + splits - 1) / splits : 1;
+  P.items = A.r.B * A.c.Hkv * P.blocks * splits;
+  P.ws_acc = static_cast<float*>(workspace), P.ws_ml = P.ws_acc + static_cast<int64_t>(A.r.B) * A.Hq * splits * A.c.D;
+  CUtensorMap k_map, v_map;
+  if (!code_map(&k_map, A.c.k_pool, A.c) || !code_map(&v_map, A.c.v_pool, A.c)) return fail(B200_EINVAL, "%s: no tensor map of the pools", name);
+  const bool short_items = P.items > 2 * kNumSMs && P.tiles_per_split <= 32;
+  auto go = [&](auto* c, auto d) {
+    using C = std::remove_pointer_t<decltype(c)>;
+    return short_items ? launch_decode_as<T, C, d.value, true>(name, P, k_map, v_map, stream) : launch_decode_as<T, C, d.value, false>(name, P, k_map, v_map, stream);
+  };
+  auto of = [&](auto* c) { return A.c.D == 128 ? go(c, std::integral_constant<int, 128>{}) : go(c, std::integral_constant<int, 64>{}); };
+  if (int rc = codes == B200_CODES_INT8 ? of(static_cast<q8::Int8*>(nullptr)) : of(static_cast<q8::E4m3*>(nullptr))) return rc;
+  return splits > 1 ? attn_combine(A.out, P.ws_acc, P.ws_ml, A.r.B * A.Hq, A.c.D, splits, dtype, stream) : 0;
+}
+
 constexpr int kAnyMostD = 256;
 
 template <typename T, typename C>
@@ -169,23 +518,36 @@ using namespace b200;
 
 extern "C" {
 
-size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
-  (void)B, (void)Hq, (void)Hkv, (void)D, (void)block_size, (void)max_context_len, (void)dtype;
-  return 0;
+size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int num_splits, int dtype) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || block_size <= 0 || max_context_len < 0 || !decode_serves(D, block_size, dtype)) return 0;
+  const int splits = num_splits > 0 ? num_splits : decode_splits(B, Hq, Hkv, block_size, max_context_len);
+  return splits > 1 ? static_cast<size_t>(B) * Hq * splits * (D + 2) * sizeof(float) : 0;
 }
 
 int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                               const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, int B, int Hq, int Hkv, int D,
-                              int block_size, int64_t max_blocks, float scale, int max_context_len, void* workspace, size_t workspace_bytes, int codes,
-                              int dtype, unsigned flags, void* stream) {
+                              int block_size, int64_t max_blocks, float scale, int max_context_len, int num_splits, void* workspace, size_t workspace_bytes,
+                              int codes, int dtype, unsigned flags, void* stream) {
   const char* name = "b200_paged_decode_attn_q8";
   const Attn A{cache_of(k_pool, v_pool, k_scale, v_scale, block_tables, table_stride, table_cols, Hkv, D, block_size, max_blocks),
                Rows{nullptr, context_lens, B, B}, out, q, q_stride, Hq, scale};
   if (int rc = check_attn(name, A, codes, dtype)) return rc;
-  if (max_context_len < 0) return fail(B200_EINVAL, "%s: negative max_context_len", name);
+  if (max_context_len < 0 || num_splits < 0 || num_splits > kMostSplits) return fail(B200_EINVAL, "%s: max_context_len %d, num_splits %d", name, max_context_len, num_splits);
   if (B == 0) return 0;
-  (void)workspace, (void)workspace_bytes, (void)flags;
-  return launch_any_of(name, A, codes, dtype, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int splits = num_splits > 0 ? num_splits : decode_splits(B, Hq, Hkv, block_size, max_context_len);
+  const bool pieces = aligned16(k_pool) && aligned16(v_pool) && !(reinterpret_cast<uintptr_t>(q) & 7) && q_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(out) & 3);
+  if (decode_serves(D, block_size, dtype) && pieces && !(flags & B200_ATTN_FORCE_GENERIC) && (max_blocks + 1) * Hkv * block_size < INT32_MAX &&
+      static_cast<int64_t>(B) * Hkv * ((Hq / Hkv + 7) / 8) * splits < INT32_MAX / 2) {
+    if (splits > 1) {
+      if (!workspace || workspace_bytes < b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, num_splits, dtype))
+        return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);
+      if (!aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
+    }
+    return dtype == B200_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(name, A, splits, max_context_len, workspace, codes, dtype, s)
+                                    : launch_decode<__half>(name, A, splits, max_context_len, workspace, codes, dtype, s);
+  }
+  return launch_any_of(name, A, codes, dtype, s);
 }
 
 size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {

@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(128) append_any_kernel(const Append A) {
   int first, count, context;
   A.r.of(b, &first, &count, &context);
   const int held = context - count, at = held / bs + lp;
-  const int t0 = max(held, at * bs), t1 = static_cast<int>(min(static_cast<int64_t>(context), static_cast<int64_t>(at + 1) * bs));       // positions
+  const int64_t base = static_cast<int64_t>(at) * bs;      // the page's first position
+  const int t0 = static_cast<int>(max(held - base, static_cast<int64_t>(0))), t1 = static_cast<int>(min(context - base, static_cast<int64_t>(bs)));     // places of the page
   if (t0 >= t1) return;
   const int page = A.c.page(b, at);
   if (page < 0) return;
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(128) append_any_kernel(const Append A) {
   float* scale = (values ? A.c.v_scale : A.c.k_scale) + place;
   auto number = [&](int i) -> float {        // of the new tokens' elements
     const int t = i / D, d = i - t * D;
-    const int64_t row = first + (t0 - held) + t;
+    const int64_t row = first + (base + t0 - held) + t;
     return values ? Cvt<T>::to_f32(rows[row * stride + d]) : element(rows + row * stride, row, d);
   };
   float most = 0.f;
@@ -82,16 +83,194 @@ __global__ void __launch_bounds__(128) append_any_kernel(const Append A) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
   if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
-  const float had = t0 > at * bs ? *scale : 0.f;
+  const float had = t0 > 0 ? *scale : 0.f;
   __syncthreads();
   most = q8::max_nan(q8::max_nan(most_s[0], most_s[1]), q8::max_nan(most_s[2], most_s[3]));
   const float now = q8::max_nan(q8::max_nan(had, __fmul_rn(most, 1.f / C::kMost)), q8::kLeastScale), inverse = 1.f / now;
   if (now != had) {
     const float k = __fmul_rn(had, inverse);
-    for (int i = threadIdx.x; i < (t0 - at * bs) * D; i += blockDim.x) codes[i] = C::code(__fmul_rn(C::value(codes[i]), k));
+    for (int i = threadIdx.x; i < t0 * D; i += blockDim.x) codes[i] = C::code(__fmul_rn(C::value(codes[i]), k));
     if (threadIdx.x == 0) *scale = now;
   }
-  for (int i = threadIdx.x; i < (t1 - t0) * D; i += blockDim.x) codes[(t0 - at * bs) * D + i] = C::code(__fmul_rn(number(i), inverse));
+  for (int i = threadIdx.x; i < (t1 - t0) * D; i += blockDim.x) codes[t0 * D + i] = C::code(__fmul_rn(number(i), inverse));
+}
+
+// ---- 16-bit types, heads of 64 or 128, pages of 16, 32 or 64 -----------------------------------------------------------------------------------
+// A warp per 16 places of a page and kv head's keys or values; the W warps of a page share its maximum.  A lane has 8 columns of the lower and the
+// same 8 of the upper half of several rows, which turn into one another: everything is read once and held as fp32 until the scale is known.  Codes that the
+// page holds already are asked for together with its scale, whether or not it grows.  Behind these CTAs, a warp per row and 16 query heads.
+constexpr int kHeadsPerWarp = 16;
+
+template <typename T>
+__device__ __forceinline__ void eight(const int4& raw, float (&x)[8]) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) x[u] = Cvt<T>::to_f32(e[u]);
+}
+template <typename T>
+__device__ __forceinline__ int4 eight_of(const float (&x)[8]) {
+  int4 raw;
+  T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) e[u] = Cvt<T>::from_f32(x[u]);
+  return raw;
+}
+// lo, hi: the same 8 columns of the two halves
+template <typename T>
+__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const int4& c_lo, const int4& c_hi, const int4& s_lo, const int4& s_hi) {
+  float cl[8], ch[8], sl[8], sh[8];
+  eight<T>(c_lo, cl);
+  eight<T>(c_hi, ch);
+  eight<T>(s_lo, sl);
+  eight<T>(s_hi, sh);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const float l = turned(lo[u], hi[u], cl[u], sl[u], false), h = turned(hi[u], lo[u], ch[u], sh[u], true);
+    lo[u] = l, hi[u] = h;
+  }
+}
+template <typename C>
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float inverse) {
+  uint2 r;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (std::is_same_v<C, q8::Int8>) {
+      // |x / s| <= 127 (1 + 2^-22): the sum's last 8 bits are the nearest whole number's
+      uint32_t b[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) b[u] = __float_as_uint(__fadd_rn(__fmul_rn(x[4 * i + u], inverse), 12582912.f));
+      w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    } else {
+      w[i] = 0;
+#pragma unroll
+      for (int u = 0; u < 4; u += 2)
+        w[i] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[4 * i + u], inverse), __fmul_rn(x[4 * i + u + 1], inverse)), __NV_SATFINITE, __NV_E4M3)) << (8 * u);
+    }
+  }
+  return r;
+}
+template <typename C>
+__device__ __forceinline__ uint2 codes_again(uint2 old, float k) {
+  uint8_t* c = reinterpret_cast<uint8_t*>(&old);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) c[u] = C::code(__fmul_rn(C::value(c[u]), k));
+  return old;
+}
+
+template <typename T, typename C, int D, int W>
+__global__ void __launch_bounds__(128) append_kernel(const Append A, int unit_ctas) {
+  constexpr int kCh = D / 16, kRows = 32 / kCh, kPasses = 16 / kRows;        // pieces of a half; rows of a warp's pass
+  __shared__ float most_s[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % kCh, r = lane / kCh;
+  if (static_cast<int>(blockIdx.x) >= unit_ctas) {
+    const int groups = (A.Hq + kHeadsPerWarp - 1) / kHeadsPerWarp;
+    const int64_t unit = (blockIdx.x - unit_ctas) * 4ll + warp, row = unit / groups;
+    if (row >= A.r.n) return;
+    const int h0 = static_cast<int>(unit - row * groups) * kHeadsPerWarp + r;
+    const T *q = static_cast<const T*>(A.q) + row * A.q_stride + 8 * c, *cs = static_cast<const T*>(A.cos_t) + row * D + 8 * c, *sn = static_cast<const T*>(A.sin_t) + row * D + 8 * c;
+    T* out = static_cast<T*>(A.q_out) + row * A.out_stride + 8 * c;
+    const int4 c_lo = *reinterpret_cast<const int4*>(cs), c_hi = *reinterpret_cast<const int4*>(cs + D / 2), s_lo = *reinterpret_cast<const int4*>(sn),
+               s_hi = *reinterpret_cast<const int4*>(sn + D / 2);
+    constexpr int kSteps = kHeadsPerWarp / kRows;
+    int4 raw[kSteps][2];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int h = h0 + i * kRows;
+      if (h < A.Hq) {
+        raw[i][0] = *reinterpret_cast<const int4*>(q + h * D);
+        raw[i][1] = *reinterpret_cast<const int4*>(q + h * D + D / 2);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int h = h0 + i * kRows;
+      if (h >= A.Hq) continue;
+      float lo[8], hi[8];
+      eight<T>(raw[i][0], lo);
+      eight<T>(raw[i][1], hi);
+      turn<T>(lo, hi, c_lo, c_hi, s_lo, s_hi);
+      *reinterpret_cast<int4*>(out + h * D) = eight_of<T>(lo);
+      *reinterpret_cast<int4*>(out + h * D + D / 2) = eight_of<T>(hi);
+    }
+    return;
+  }
+  // ---- keys and values: unit = ((sequence, page), head, keys or values) -----------------------------------------------------------------------
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (4 / W) + warp / W;
+  const bool values = unit & 1;
+  const int h = static_cast<int>((unit >> 1) % A.c.Hkv), bp = static_cast<int>((unit >> 1) / A.c.Hkv), b = bp / A.pages, lp = bp - b * A.pages;
+  int t0 = 0, t1 = 0, at = 0, first = 0, held = 0, page = -1;
+  if (b < A.r.B) {
+    int count, context;
+    A.r.of(b, &first, &count, &context);
+    held = context - count, at = held / A.c.bs + lp;
+    const int64_t base = static_cast<int64_t>(at) * A.c.bs;
+    t0 = static_cast<int>(max(held - base, static_cast<int64_t>(0))), t1 = static_cast<int>(min(context - base, static_cast<int64_t>(A.c.bs)));      // places of the page
+    if (t0 < t1) page = A.c.page(b, at);
+  }
+  if (W == 1 && page < 0) return;
+  const int64_t place = static_cast<int64_t>(max(page, 0)) * A.c.Hkv + h;
+  uint8_t* codes = (values ? A.c.v_pool : A.c.k_pool) + place * A.c.bs * D;
+  float* scale = (values ? A.c.v_scale : A.c.k_scale) + place;
+  const bool earlier = page >= 0 && t0 > 0;
+  float had = earlier ? *scale : 0.f;
+  const int my = warp % W * 16 + r;       // the place of the lane's row in the first pass
+  uint2 old[kPasses][2];
+  int4 raw[kPasses][2];
+  const T* rows = static_cast<const T*>(values ? A.v : A.k) + h * D + 8 * c;
+  const int64_t stride = values ? A.v_stride : A.k_stride, row0 = static_cast<int64_t>(first) + static_cast<int64_t>(at) * A.c.bs - held;       // the row of the page's first place
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int t = my + i * kRows;
+    if (page >= 0 && t >= t0 && t < t1) {
+      raw[i][0] = ld_stream16(rows + (row0 + t) * stride);
+      raw[i][1] = ld_stream16(rows + (row0 + t) * stride + D / 2);
+    }
+    if (earlier && t < t0) {
+      old[i][0] = *reinterpret_cast<const uint2*>(codes + t * D + 8 * c);
+      old[i][1] = *reinterpret_cast<const uint2*>(codes + t * D + D / 2 + 8 * c);
+    }
+  }
+  float x[kPasses][2][8], most = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int t = my + i * kRows;
+    if (!(page >= 0 && t >= t0 && t < t1)) continue;
+    eight<T>(raw[i][0], x[i][0]);
+    eight<T>(raw[i][1], x[i][1]);
+    if (!values && A.cos_t) {
+      const T *cs = static_cast<const T*>(A.cos_t) + (row0 + t) * D + 8 * c, *sn = static_cast<const T*>(A.sin_t) + (row0 + t) * D + 8 * c;
+      turn<T>(x[i][0], x[i][1], *reinterpret_cast<const int4*>(cs), *reinterpret_cast<const int4*>(cs + D / 2), *reinterpret_cast<const int4*>(sn),
+              *reinterpret_cast<const int4*>(sn + D / 2));
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) most = q8::max_nan(most, q8::max_nan(fabsf(x[i][0][u]), fabsf(x[i][1][u])));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if constexpr (W > 1) {
+    if (lane == 0) most_s[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) most = q8::max_nan(most, most_s[warp / W * W + w]);
+    if (page < 0) return;
+  }
+  const float now = q8::max_nan(q8::max_nan(had, __fmul_rn(most, 1.f / C::kMost)), q8::kLeastScale), inverse = __frcp_rn(now);
+  const bool grew = now != had;
+  if (grew && warp % W == 0 && lane == 0) *scale = now;       // (the other warps have read what it was: before the barrier)
+  const float k = __fmul_rn(had, inverse);
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int t = my + i * kRows;
+    uint2* to = reinterpret_cast<uint2*>(codes + t * D + 8 * c);
+    if (t >= t0 && t < t1) {
+      to[0] = codes_of<C>(x[i][0], inverse);
+      to[D / 16] = codes_of<C>(x[i][1], inverse);
+    } else if (earlier && t < t0 && grew) {
+      to[0] = codes_again<C>(old[i][0], k);
+      to[D / 16] = codes_again<C>(old[i][1], k);
+    }
+  }
 }
 
 // ---- reading back --------------------------------------------------------------------------------------------------------------------------
@@ -116,6 +295,66 @@ __global__ void __launch_bounds__(256) gather_any_kernel(const Gather G) {
     }
     static_cast<T*>(G.k_out)[i] = Cvt<T>::from_f32(k);
     static_cast<T*>(G.v_out)[i] = Cvt<T>::from_f32(v);
+  }
+}
+
+// 16 rows of a page and kv head's keys and values per warp; pages of 16s, rows of D = 64 or 128 codes, 8 of them a lane and step, all asked for before the first is
+// turned.  Bound by memory.
+template <typename C>
+__device__ __forceinline__ void values_of(uint2 codes, float s, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w = i ? codes.y : codes.x;
+    if constexpr (std::is_same_v<C, q8::Int8>) {
+      const uint32_t u = w ^ 0x80808080u;       // code + 128, as the last byte of 2^23 + code + 128
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + e)) - 8388736.f) * s;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * e)), __NV_E4M3)));
+        x[4 * i + 2 * e] = f.x * s, x[4 * i + 2 * e + 1] = f.y * s;
+      }
+    }
+  }
+}
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(256) gather_kernel(const Gather G, int tiles, int64_t units) {
+  constexpr int kSteps = 16 * D / 256;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  const int64_t bh = unit / tiles;
+  const int tile = static_cast<int>(unit - bh * tiles), h = static_cast<int>(bh % G.c.Hkv), b = static_cast<int>(bh / G.c.Hkv), at = tile * 16 / G.c.bs;
+  const int page = G.c.page(b, at);
+  const int64_t place = static_cast<int64_t>(max(page, 0)) * G.c.Hkv + h, from = (place * G.c.bs + (tile * 16 - at * G.c.bs)) * D + lane * 8;
+  const float ks = page >= 0 ? G.c.k_scale[place] : 0.f, vs = page >= 0 ? G.c.v_scale[place] : 0.f;
+  uint2 k[kSteps], v[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) k[i] = page >= 0 ? ld_stream8(G.c.k_pool + from + i * 256) : make_uint2(0u, 0u);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) v[i] = page >= 0 ? ld_stream8(G.c.v_pool + from + i * 256) : make_uint2(0u, 0u);
+  const int64_t to = (bh * G.n + tile * 16) * D + lane * 8;
+  const int live = min(16, G.n - tile * 16) * D;        // elements
+#pragma unroll
+  for (int i = 0; i < 2 * kSteps; ++i) {
+    const int e = i % kSteps * 256 + lane * 8;
+    if (e >= live) continue;
+    float x[8];
+    values_of<C>(i < kSteps ? k[i % kSteps] : v[i % kSteps], i < kSteps ? ks : vs, x);
+    T* out = static_cast<T*>(i < kSteps ? G.k_out : G.v_out) + to + i % kSteps * 256;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(out + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      *reinterpret_cast<int4*>(out) = eight_of<T>(x);
+    }
   }
 }
 
@@ -155,11 +394,27 @@ int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int
   A.q_stride = q_stride, A.k_stride = k_stride, A.v_stride = v_stride, A.out_stride = q_out_stride, A.Hq = Hq;
   const int longest = row_starts ? (max_new < rows ? max_new : rows) : 1;
   A.pages = longest == 0 ? 0 : longest == 1 ? 1 : static_cast<int>((longest - 2ll + block_size) / block_size) + 1;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t units = static_cast<int64_t>(B) * A.pages * Hkv * 2, grid = units + (q_out ? rows : 0);
   if (grid > INT32_MAX) return fail(B200_ESHAPE, "%s: %d sequences of up to %d pages", name, B, A.pages);
   if (grid == 0) return 0;
+  const int warps = block_size / 16;
+  const bool pieces = aligned16(k) && aligned16(v) && aligned16(cos_table) && aligned16(sin_table) && aligned16(k_pool) && aligned16(v_pool) && k_stride % 8 == 0 &&
+                      v_stride % 8 == 0 && (!q_out || (aligned16(q) && aligned16(q_out) && q_stride % 8 == 0 && q_out_stride % 8 == 0));
+  const bool fast = dtype != B200_DTYPE_F32 && (D == 64 || D == 128) && block_size % 16 == 0 && (warps == 1 || warps == 2 || warps == 4) && pieces;
   return with_types(dtype, codes, [&](auto* t, auto* c) {
-    append_any_kernel<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(c)>><<<static_cast<unsigned>(grid), 128, 0, static_cast<cudaStream_t>(stream)>>>(A);
+    using T = std::remove_pointer_t<decltype(t)>;
+    using C = std::remove_pointer_t<decltype(c)>;
+    if constexpr (sizeof(T) == 2) {
+      if (fast) {
+        const int64_t ctas = (units * warps + 3) / 4, q_ctas = q_out ? (static_cast<int64_t>(rows) * ((Hq + kHeadsPerWarp - 1) / kHeadsPerWarp) + 3) / 4 : 0;
+        auto kern = D == 128 ? (warps == 1 ? append_kernel<T, C, 128, 1> : warps == 2 ? append_kernel<T, C, 128, 2> : append_kernel<T, C, 128, 4>)
+                             : (warps == 1 ? append_kernel<T, C, 64, 1> : warps == 2 ? append_kernel<T, C, 64, 2> : append_kernel<T, C, 64, 4>);
+        kern<<<static_cast<unsigned>(ctas + q_ctas), 128, 0, s>>>(A, static_cast<int>(ctas));
+        return check_launch(name);
+      }
+    }
+    append_any_kernel<T, C><<<static_cast<unsigned>(grid), 128, 0, s>>>(A);
     return check_launch(name);
   });
 }
@@ -178,10 +433,19 @@ int b200_kv_gather_dense_q8(void* k_out, void* v_out, const void* k_pool, const 
   if (B == 0 || n_tokens == 0) return 0;
   if (!k_out || !v_out || !k_pool || !v_pool || !k_scale || !v_scale || !block_tables) return fail(B200_EINVAL, "%s: null pointer", name);
   G.k_out = k_out, G.v_out = v_out, G.B = B, G.n = n_tokens;
-  const int64_t blocks = (static_cast<int64_t>(B) * Hkv * n_tokens * D + 255) / 256;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int tiles = static_cast<int>((n_tokens + 15ll) / 16);
+  const int64_t blocks = (static_cast<int64_t>(B) * Hkv * n_tokens * D + 255) / 256, units = static_cast<int64_t>(B) * Hkv * tiles;
+  const bool fast = (D == 64 || D == 128) && block_size % 16 == 0 && aligned16(k_out) && aligned16(v_out) && aligned16(k_pool) && aligned16(v_pool) && units < INT32_MAX;
   return with_types(dtype, codes, [&](auto* t, auto* c) {
-    gather_any_kernel<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(c)>>
-        <<<static_cast<unsigned>(blocks < kNumSMs * 8 ? blocks : kNumSMs * 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(G);
+    using T = std::remove_pointer_t<decltype(t)>;
+    using C = std::remove_pointer_t<decltype(c)>;
+    if (fast) {
+      auto kern = D == 128 ? gather_kernel<T, C, 128> : gather_kernel<T, C, 64>;
+      kern<<<static_cast<unsigned>((units + 7) / 8), 256, 0, s>>>(G, tiles, units);
+      return check_launch(name);
+    }
+    gather_any_kernel<T, C><<<static_cast<unsigned>(blocks < kNumSMs * 8 ? blocks : kNumSMs * 8), 256, 0, s>>>(G);
     return check_launch(name);
   });
 }

@@ -1002,17 +1002,19 @@ def _q8_workspace(need: int, workspace: Optional[torch.Tensor], q: torch.Tensor,
 
 
 @functools.lru_cache(maxsize=1024)
-def decode_attention_q8_workspace(B: int, Hq: int, Hkv: int, D: int, block_size: int, max_context_len: int, dtype: torch.dtype) -> int:
+def decode_attention_q8_workspace(B: int, Hq: int, Hkv: int, D: int, block_size: int, max_context_len: int, dtype: torch.dtype,
+                                  num_splits: int = 0) -> int:
     """Bytes of scratch that ``paged_decode_attention_q8`` needs for these sizes."""
-    return _lib.load().b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, DTYPE_ID[dtype])
+    return _lib.load().b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, num_splits, DTYPE_ID[dtype])
 
 
 def paged_decode_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                               block_tables: torch.Tensor, context_lens: torch.Tensor, max_context_len: int, scale: Optional[float] = None,
-                              out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, flags: int = 0) -> torch.Tensor:
+                              out: Optional[torch.Tensor] = None, num_splits: int = 0, workspace: Optional[torch.Tensor] = None,
+                              flags: int = 0) -> torch.Tensor:
     """``paged_decode_attention`` over a cache in 8 bits (as ``rope_kv_append_q8`` writes it): ``q [B, Hq, D]`` (row stride free), a token per sequence, over the
     ``context_lens[b]`` tokens of its pages; 0 where there are none.  ``max_context_len``: the host's bound of the lengths (tokens
-    behind it may be left out).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
+    behind it may be left out).  ``num_splits``: parts of the keys (0: the library's choice).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
     torch's caching allocator.  ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
     _need_cuda(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens)
     dev = q.get_device()
@@ -1021,11 +1023,12 @@ def paged_decode_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     Hq, q_stride, out = _q8_attention(q, shape, out, dev)
     B, dt = block_tables.shape[0], _dtype_id(q)
     lens, _ = _q8_lens(context_lens, None, B, q.shape[0], dev)
-    ws, ws_bytes, _keep = _q8_workspace(decode_attention_q8_workspace(B, Hq, Hkv, D, bs, int(max_context_len), q.dtype), workspace, q, dev)
+    need = decode_attention_q8_workspace(B, Hq, Hkv, D, bs, int(max_context_len), q.dtype, int(num_splits))
+    ws, ws_bytes, _keep = _q8_workspace(need, workspace, q, dev)
     with _timed(), _on(dev) as stream:
         rc = _lib.load().b200_paged_decode_attn_q8(
             out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, B, Hq, Hkv, D, bs, max_blocks, D ** -0.5 if scale is None else float(scale),
-            int(max_context_len), ws, ws_bytes, codes, dt, int(flags), stream)
+            int(max_context_len), int(num_splits), ws, ws_bytes, codes, dt, int(flags), stream)
     if rc != 0:
         _lib.check(rc, "b200_paged_decode_attn_q8")
     return out
