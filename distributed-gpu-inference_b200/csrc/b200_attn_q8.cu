@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "b200_attn.cuh"
+#include "b200_prompt_q8.cuh"
 #include "b200_q8.cuh"
 #include "b200_tcgen05.cuh"
 
@@ -159,23 +160,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// four codes as two pairs of fp16: (0, 1) and (2, 3), or across (0, 2) and (1, 3)
-template <typename C, bool ACROSS>
-__device__ __forceinline__ void halves(uint32_t codes, uint32_t& a, uint32_t& b) {
-  if constexpr (std::is_same_v<C, q8::Int8>) {
-    const uint32_t u = codes ^ 0x80808080u, bias = 0x64806480u;       // 1024 + 128
-    a = __byte_perm(u, 0x64646464u, ACROSS ? 0x4240 : 0x4140);
-    b = __byte_perm(u, 0x64646464u, ACROSS ? 0x4341 : 0x4342);
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(bias));
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(bias));
-  } else {
-    uint32_t lo, hi;
-    asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(codes));
-    a = ACROSS ? __byte_perm(lo, hi, 0x5410) : lo;
-    b = ACROSS ? __byte_perm(lo, hi, 0x7632) : hi;
-  }
-}
-
 template <int D>
 struct DecodePlan {
   static constexpr int kStages = 4, kTile = kTok * D, kStage = 2 * kTile;       // bytes: keys, then values
@@ -315,8 +299,8 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t a0, a1, a2, a3;
-        halves<C, false>(r[2 * u], a0, a2);
-        halves<C, false>(r[2 * u + 1], a1, a3);
+        q8::halves<C, false>(r[2 * u], a0, a2);
+        q8::halves<C, false>(r[2 * u + 1], a1, a3);
         mma16(s, a0, a1, a2, a3, qf[p + u][0], qf[p + u][1]);
       }
     }
@@ -361,8 +345,8 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t a0, a1, a2, a3;
-        halves<C, true>(r[2 * u], a0, a1);
-        halves<C, true>(r[2 * u + 1], a2, a3);
+        q8::halves<C, true>(r[2 * u], a0, a1);
+        q8::halves<C, true>(r[2 * u + 1], a2, a3);
         mma16(o[p + u], a0, a1, a2, a3, b0, b1);
       }
     }
@@ -551,8 +535,7 @@ int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const 
 }
 
 size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
-  (void)B, (void)max_new, (void)Hq, (void)Hkv, (void)D, (void)block_size, (void)max_context_len, (void)dtype;
-  return 0;
+  return prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype);
 }
 
 int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
@@ -566,8 +549,17 @@ int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const 
   if (max_context_len < 0 || max_new < 0) return fail(B200_EINVAL, "%s: negative max_context_len or max_new", name);
   if (B == 0 || rows == 0) return 0;
   if (!row_starts) return fail(B200_EINVAL, "%s: null pointer", name);
-  (void)workspace, (void)workspace_bytes, (void)flags;
-  return launch_any_of(name, A, codes, dtype, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  q8::PromptAttn P{};
+  P.c = A.c, P.r = A.r, P.out = out, P.q = q, P.q_stride = q_stride, P.Hq = Hq, P.scale = scale;
+  if (max_new == 0) return 0;
+  if (!(flags & B200_ATTN_FORCE_GENERIC) && prompt_q8_serves(P, max_new, max_context_len, dtype)) {
+    const size_t need = prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype);
+    if (need && (!workspace || workspace_bytes < need)) return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);
+    if (need && !aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
+    return prompt_q8(name, P, max_new, max_context_len, workspace, codes, dtype, s);
+  }
+  return launch_any_of(name, A, codes, dtype, s);
 }
 
 }  // extern "C"

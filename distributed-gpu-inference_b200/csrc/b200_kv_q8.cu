@@ -144,8 +144,10 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float inverse) {
     } else {
       w[i] = 0;
 #pragma unroll
-      for (int u = 0; u < 4; u += 2)
-        w[i] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[4 * i + u], inverse), __fmul_rn(x[4 * i + u + 1], inverse)), __NV_SATFINITE, __NV_E4M3)) << (8 * u);
+      for (int u = 0; u < 4; u += 2) {
+        const float a = __fmul_rn(x[4 * i + u], inverse), b = __fmul_rn(x[4 * i + u + 1], inverse);
+        w[i] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a == a ? a : 0.f, b == b ? b : 0.f), __NV_SATFINITE, __NV_E4M3)) << (8 * u);
+      }
     }
   }
   return r;

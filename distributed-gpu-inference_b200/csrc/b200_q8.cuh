@@ -4,6 +4,8 @@
 #pragma once
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "b200_common.cuh"
 
 namespace b200 {
@@ -22,7 +24,8 @@ struct Int8 {
 struct E4m3 {
   static constexpr float kMost = 448.f;
   static __device__ __forceinline__ float value(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
-  static __device__ __forceinline__ uint8_t code(float y) { return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3); }
+  // (what is no number becomes 0 here too: a row that does not see it must not meet it)
+  static __device__ __forceinline__ uint8_t code(float y) { return __nv_cvt_float_to_fp8(y == y ? y : 0.f, __NV_SATFINITE, __NV_E4M3); }
 };
 
 constexpr float kLeastScale = 0x1p-60f;     // of a page that holds nothing but zeros, or numbers below 127 * 2^-60
@@ -32,6 +35,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// four codes as two pairs of fp16: (0, 1) and (2, 3), or across (0, 2) and (1, 3)
+template <typename C, bool ACROSS>
+__device__ __forceinline__ void halves(uint32_t codes, uint32_t& a, uint32_t& b) {
+  if constexpr (std::is_same_v<C, Int8>) {
+    const uint32_t u = codes ^ 0x80808080u, bias = 0x64806480u;       // 1024 + 128
+    a = __byte_perm(u, 0x64646464u, ACROSS ? 0x4240 : 0x4140);
+    b = __byte_perm(u, 0x64646464u, ACROSS ? 0x4341 : 0x4342);
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(bias));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(bias));
+  } else {
+    uint32_t lo, hi;
+    asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(codes));
+    a = ACROSS ? __byte_perm(lo, hi, 0x5410) : lo;
+    b = ACROSS ? __byte_perm(lo, hi, 0x7632) : hi;
+  }
 }
 
 struct Cache {
