@@ -33,6 +33,8 @@ from .worker.distributed.kv_cache import CacheBlock, KVCachePool, RadixPrefixInd
 from .worker.distributed.model_shard import ModelShard
 from . import ops
 
+KV_CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}      # what a cache in 8 bits holds
+
 
 class _TreeStep:
     """One pass over trees of ``nodes`` drafted tokens of the engine's present number of sequences: static buffers and the captured graph, which are of
@@ -141,9 +143,16 @@ class PagedDecodeEngine:
         kv_pools: Optional[Sequence[KVCachePool]] = None,
         prefix_cache: bool = False,
         external_head: bool = False,
+        kv_cache_dtype: Optional[str] = None,
     ):
+        """``kv_cache_dtype``: None (the model's) or one of ``KV_CODES``: keys and values are held in 8 bits with a scale for each block and kv head
+        (``ops.rope_kv_append_q8``), in half the memory of 16 bits."""
         if not shards:
             raise ValueError("need at least one shard")
+        if kv_cache_dtype is not None and kv_cache_dtype not in KV_CODES:
+            raise ValueError(f"kv_cache_dtype is None or one of {sorted(KV_CODES)}, not {kv_cache_dtype!r}")
+        if kv_cache_dtype is not None and kv_pools is not None:
+            raise ValueError("a cache in 8 bits has pools of its own, with scales: no kv_pools")
         self.shards = list(shards)
         if fuse_projections:
             for sh in self.shards:
@@ -190,11 +199,16 @@ class PagedDecodeEngine:
                 block_size=block_size,
                 max_blocks_per_layer=max_batch * self.blocks_per_seq + spare_blocks,
                 device=str(self.device),
-                dtype=self.dtype,
+                # (codes of 8 bits are bytes to the allocator, which clears freed blocks: 0 stands for 0 in both kinds)
+                dtype=self.dtype if kv_cache_dtype is None else torch.int8,
             )
             for s in self.shards
         ]
         dev = self.device
+        self.kv_cache_dtype = kv_cache_dtype
+        # scales [layers, 2, blocks, kv heads] of each shard's blocks: keys', values'
+        self.kv_scales: Optional[List[torch.Tensor]] = None if kv_cache_dtype is None else [
+            torch.zeros((p.num_layers, 2, p.max_blocks_per_layer, self.Hkv), dtype=torch.float32, device=dev) for p in self.pools]
         self.block_tables = torch.zeros((max_batch, self.blocks_per_seq), dtype=torch.int32, device=dev)
         self.context_lens = torch.zeros((max_batch,), dtype=torch.int32, device=dev)
         self.is_first = bool(self.shards[0].is_first_shard)
@@ -229,6 +243,10 @@ class PagedDecodeEngine:
             [PagedLayerKV(pool.layer(i).key_pool, pool.layer(i).value_pool, self.state) for i in range(s.get_layer_count())]
             for s, pool in zip(self.shards, self.pools)
         ]
+        if kv_cache_dtype is not None:
+            codes = KV_CODES[kv_cache_dtype]
+            self._handles = [[PagedLayerKV(h.k_pool.view(codes), h.v_pool.view(codes), self.state, scales[i, 0], scales[i, 1]) for i, h in enumerate(hs)]
+                             for hs, scales in zip(self._handles, self.kv_scales)]
         self._seq_blocks: List[Optional[List[List[List[CacheBlock]]]]] = [None] * max_batch  # [seq][shard][layer][blk]
         self._host_lens = [0] * max_batch
         # when set to a list (with use_cuda_graph=False): every prompt pass and decode step appends
@@ -323,7 +341,7 @@ class PagedDecodeEngine:
         st.prefix_blocks = 0
         st.attn_flags &= ~ops.ATTN_WS_COUNTERS_ZERO
         self.prefix_blocks = n_shared
-        if n_shared > 0 and self.dtype in (torch.bfloat16, torch.float16) and self.block_size == 16 \
+        if n_shared > 0 and self.kv_cache_dtype is None and self.dtype in (torch.bfloat16, torch.float16) and self.block_size == 16 \
                 and self.D in (64, 128) and self.Hq // self.Hkv <= 8:
             ps, ss = ops.attn_prefix_plan(self.batch, self.Hq, self.Hkv, self.D, self.block_size, n_shared,
                                           self.max_seq_len, self.dtype)
@@ -423,11 +441,13 @@ class PagedDecodeEngine:
             max_context_len=past_len + P,
             prefill_mode=self.prefill_mode,
             past_len=past_len,
+            row_starts=None if self.kv_cache_dtype is None else torch.arange(0, n * P + 1, P, dtype=torch.int32, device=self.device),
+            attn_flags=0 if self.kv_cache_dtype is None else self.state.attn_flags & ops.ATTN_FORCE_GENERIC,
         )
         chunk_state.cos, chunk_state.sin = rope_tables(pos, self.inv_freq, self.dtype, self.rope_scaling)
         h = inputs.to(self.device)
         for shard, handles in zip(self.shards, self._handles):
-            hs = [PagedLayerKV(hd.k_pool, hd.v_pool, chunk_state) for hd in handles]
+            hs = [PagedLayerKV(hd.k_pool, hd.v_pool, chunk_state, hd.k_scale, hd.v_scale) for hd in handles]
             h, _ = shard.forward(h, position_ids=pos, past_key_values=hs, use_cache=True)
         self.context_lens[lo:hi] = past_len + P
         self._host_lens[lo:hi] = [past_len + P] * n
@@ -638,6 +658,8 @@ class PagedDecodeEngine:
         a draw and the end of a weight, are that close - seldom in 32 bits, in 16 bits (logits off by 2^-8 or 2^-11 of their size either way) now and then."""
         if not (self.is_first and self.is_last) or self.external_head:
             raise RuntimeError("verify_trees() drives a whole model")
+        if self.kv_cache_dtype is not None:
+            raise RuntimeError("drafted tokens are not checked over a cache in 8 bits")
         B = self.batch
         if tokens.shape != parents.shape or tokens.dim() != 2 or tokens.shape[0] != B:
             raise ValueError("tokens and parents must be [batch, nodes]")
@@ -666,6 +688,8 @@ class PagedDecodeEngine:
         """``generate``'s tokens (as ``verify_trees`` chooses them) with several of them per pass: ``drafter(tokens of a sequence so far) -> (tokens, parents)`` proposes a tree
         of up to ``nodes`` nodes, its root the last token (default: ``drafting.PromptLookup``; None: no draft), and ``verify_trees`` checks it (at the end of
         ``max_seq_len`` as much of its beginning as there is room for)."""
+        if self.kv_cache_dtype is not None:
+            raise RuntimeError("drafted tokens are not checked over a cache in 8 bits")
         B, P = prompt_ids.shape
         drafter = drafter or PromptLookup(nodes)
         if sampling is not None and len(sampling) != B:

@@ -164,15 +164,20 @@ class PagedBatchState:
     draft_lens: Optional[torch.Tensor] = None
     # MLP output of the previous layer whose residual add was deferred (see PagedLlamaDecoderLayer.defer_residual)
     pending_residual: Optional[torch.Tensor] = None
+    # prompt passes over a cache in 8 bits: int32 [B + 1], where each sequence's rows begin (None: made by the layer)
+    row_starts: Optional[torch.Tensor] = None
 
 
 @dataclass
 class PagedLayerKV:
-    """What a paged layer expects in ``past_key_values[i]``: its pools and the shared batch state."""
+    """What a paged layer expects in ``past_key_values[i]``: its pools and the shared batch state; ``k_scale / v_scale`` (fp32 ``[max_blocks, Hkv]``)
+    where the pools hold codes of 8 bits (``ops.rope_kv_append_q8``)."""
 
     k_pool: torch.Tensor
     v_pool: torch.Tensor
     state: PagedBatchState
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -513,7 +518,7 @@ class PagedLlamaDecoderLayer(nn.Module):
         B, T, _ = hidden_states.shape
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
 
-        if T == 1 and st.visible is None and self._qkv_w is None and st.pending_residual is None and not self.defer_residual and st.prefix_blocks == 0:
+        if T == 1 and past_key_value.k_scale is None and st.visible is None and self._qkv_w is None and st.pending_residual is None and not self.defer_residual and st.prefix_blocks == 0:
             h = self._one_call(hidden_states, position_ids, past_key_value, st)
             if h is not None:
                 return h, (past_key_value if use_cache else None)
@@ -544,7 +549,9 @@ class PagedLlamaDecoderLayer(nn.Module):
                 raise ValueError("position_ids (or precomputed RoPE tables in the batch state) are required")
             cos, sin = rope_tables(position_ids, self.inv_freq, x.dtype, self.rope_attention_scaling)
 
-        if st.visible is not None:
+        if past_key_value.k_scale is not None:
+            attn = self._attention_q8(q, k, v, cos, sin, attention_mask, past_key_value, st)
+        elif st.visible is not None:
             # drafted tokens: RoPE by each node's own position, the append behind the context in the order of the nodes, attention of the trees
             ops.rope_kv_append(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cos.reshape(B * T, D), sin.reshape(B * T, D),
                                past_key_value.k_pool, past_key_value.v_pool, st.slot_mapping)
@@ -612,6 +619,29 @@ class PagedLlamaDecoderLayer(nn.Module):
         else:
             h = h + self.mlp.down_proj(act)
         return h, (past_key_value if use_cache else None)
+
+    def _attention_q8(self, q, k, v, cos, sin, attention_mask, handle: PagedLayerKV, st: PagedBatchState) -> torch.Tensor:
+        """RoPE, the append and the attention over a cache in 8 bits: one launch each.  A prompt pass attends to what it has written, its own tokens
+        included, so that a prompt's portions and the tokens decoded behind it see the same keys and values."""
+        if st.visible is not None:
+            raise RuntimeError("drafted tokens are not checked over a cache in 8 bits")
+        B, T, Hq, D = q.shape
+        cache = (handle.k_pool, handle.v_pool, handle.k_scale, handle.v_scale, st.block_tables, st.context_lens)
+        flags = st.attn_flags & ops.ATTN_FORCE_GENERIC
+        starts = None
+        if T > 1:
+            starts = st.row_starts
+            if starts is None:
+                starts = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
+        q = ops.rope_kv_append_q8(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cos.reshape(B * T, D), sin.reshape(B * T, D), *cache, row_starts=starts,
+                                  max_new=T)
+        if T == 1:
+            return ops.paged_decode_attention_q8(q, *cache, st.max_context_len, flags=flags).view(B, 1, Hq * D)
+        if st.prefill_mode == "eager" or attention_mask is not None:
+            # the eager recipe, over the values that the cache holds
+            kd, vd = ops.kv_gather_dense_q8(*cache[:5], st.past_len + T, q.dtype)
+            return self._prefill_attention(q.view(B, T, Hq, D), kd.transpose(1, 2), vd.transpose(1, 2), attention_mask, st.prefill_mode)
+        return ops.paged_prompt_attention_q8(q, *cache, starts, T, st.max_context_len, flags=flags).view(B, T, Hq * D)
 
     def _with_cached_prefix(self, k, v, handle: PagedLayerKV, st: PagedBatchState):
         """Dense k and v ``[B, past_len + T, Hkv, D]`` for a prompt pass that continues ``st.past_len`` cached tokens.

@@ -70,6 +70,8 @@ class PagedLLMEngine:
                                                                     dtype=cfg.get("dtype", torch.bfloat16))
             self.model = shards
             if arch.engine == "ragged":
+                if cfg.get("kv_cache_dtype") is not None:
+                    raise ValueError("this model class keeps its cache in the model's dtype: no kv_cache_dtype")
                 self.engine = RaggedStepEngine(shards, max_tokens=cfg.get("max_num_batched_tokens", 8192),
                                                max_seqs=cfg.get("max_batch_size", 32), block_size=cfg.get("block_size", 16))
                 self.backend_type = "ragged_b200"
@@ -88,7 +90,8 @@ class PagedLLMEngine:
             fuse_projections=cfg.get("fuse_projections", True),
             # system prompts stay cached between calls (blocks held by the prefix index, evicted LRU when the pool
             # runs dry); `prefix_cache_blocks` is the room set aside for them on top of the batch's own blocks
-            prefix_cache=cfg.get("enable_prefix_caching", True), spare_blocks=cfg.get("prefix_cache_blocks", 256))
+            prefix_cache=cfg.get("enable_prefix_caching", True), spare_blocks=cfg.get("prefix_cache_blocks", 256),
+            kv_cache_dtype=cfg.get("kv_cache_dtype"))      # "int8" / "e4m3": keys and values in 8 bits
         self.loaded = True
 
     def unload_model(self) -> None:
