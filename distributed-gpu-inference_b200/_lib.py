@@ -114,10 +114,10 @@ SIGNATURES = {
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,
                 c_int, c_void_p],
     ),
-    "b200_paged_decode_attn_q8_workspace": (c_size_t, [c_int] * 8),
+    "b200_paged_decode_attn_q8_workspace": (c_size_t, [c_int] * 7),
     "b200_paged_decode_attn_q8": (
         c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
-                c_int64, c_float, c_int, c_int, c_void_p, c_size_t, c_int, c_int, c_uint, c_void_p],
+                c_int64, c_float, c_int, c_void_p, c_size_t, c_int, c_int, c_uint, c_void_p],
     ),
     "b200_paged_prompt_attn_q8_workspace": (c_size_t, [c_int] * 8),
     "b200_paged_prompt_attn_q8": (

@@ -3,10 +3,10 @@
 //   out[i, h] = sum_j w_j c_j s_j / sum_j w_j,   w_j = exp(q[i, h] k_j t_j scale - max),   j up to the token's own position
 //
 // c, s codes and scales of the values, k, t of the keys.
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
-#include "b200_attn.cuh"
 #include "b200_prompt_q8.cuh"
 #include "b200_q8.cuh"
 #include "b200_tcgen05.cuh"
@@ -134,14 +134,15 @@ __global__ void __launch_bounds__(kAnyWarps * 32) attn_any_kernel(const Attn A, 
 // per item, which then waits for nobody.)
 //
 //   S^T[token, head] = K Q^T   mma.m16n8k16, the codes as fp16: exact, for both kinds.  Queries in fp16 too, by a power of two of their own brought to 2^14 .. 2^15
-//                              at the largest, so that what fp16 loses lies 2^-38 below it; the 8-wide side holds the heads, nothing is padded
+//                              at the largest, so that what fp16 loses lies 2^-38 below it; the 8-wide side holds the heads, nothing is padded.  (int8 products of the
+//                              codes as they are with queries in two digits of 8 bits, 80 instructions a tile fewer, took the same time.)
 //   w = 2^(S t + log2 s - m)   t the page's key scale with all else, s its value scale: the weights carry it, so that they meet bare codes; the sum counts w / s.
 //                              m moves when a score is 2^8 above it; the largest weight lies between 2^6 and 2^14, and rounding to fp16 is by 2^-12 of
 //                              a weight at most, for weights down to 2^-20 of the largest
 //   O^T[d, head] += V^T w^T    the values by ldmatrix.trans, whose pairs of bytes are two tokens' codes of neighbouring columns
 //
-// The order of columns inside a product is free as long as both sides agree: a lane's 4 bytes of a key's 16 are its 4 columns there, and its rows of the output
-// are two neighbouring columns.  A byte becomes fp16 as the low byte of 1024 + code + 128 (int8) or by the conversion that the hardware has (e4m3).
+// The order of columns inside a product is free as long as both sides agree: a lane's 4 bytes of a key's 16 are its 4 columns there, and its rows of the
+// output are two neighbouring columns.  A byte becomes fp16 as the low byte of 1024 + code + 128 (int8) or by the conversion that the hardware has (e4m3).
 constexpr int kWarps = 4, kTok = 16;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -160,13 +161,15 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// A warp's unit of work is kTiles tiles, one barrier for their copies.
 template <int D>
 struct DecodePlan {
-  static constexpr int kStages = 4, kTile = kTok * D, kStage = 2 * kTile;       // bytes: keys, then values
+  static constexpr int kTiles = 128 / D, kStages = 3, kTile = kTok * D, kStage = 2 * kTiles * kTile;       // bytes: keys of the tiles, then their values
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBars = kRing, kDead = kBars + kWarps * kStages * 8, kEnd = kDead + 16;
   static constexpr int kSmem = kEnd + 1024;
   static_assert(kWarps * 8 * (D + 2) * 4 <= kRing, "outputs go where the tiles were");
+  static_assert(4 * (kSmem + 1024) <= 228 * 1024, "shared memory");
 };
 // byte of (token, 16-byte piece) in a tile: lines of 128 bytes, a token each or two
 template <int D>
@@ -175,25 +178,37 @@ __device__ __forceinline__ uint32_t tile_at(int token, int piece) {
   return line * 128 + ((p ^ (line & 7)) << 4);
 }
 
+// A sequence, kv head and block of up to 8 of its query heads is an item.  The tokens of an item are divided among `splits` CTAs in equal parts (of kLeastPart
+// at least, the last ones may have none), which leave maximum, sum and output in the workspace for decode_merge_kernel.
 struct Decode {
   Attn a;
   int heads, blocks;              // query heads of a kv head; blocks of up to 8 of them
-  int tiles_per_split, splits, items;
-  float *ws_acc, *ws_ml;          // [B, Hq, splits, D], [B, Hq, splits, 2]
+  int items, splits;
+  float2* ml;                     // [item][part][8]: maximum (of scores in powers of two), sum
+  float* o;                       // [item][part][8][D]
 };
+constexpr int kLeastPart = 256;      // tokens
+
+// tokens of a part of a sequence's: 32s for each of the four warps
+__device__ __forceinline__ int part_of(int keys, int splits) {
+  constexpr int kOf = 32 * kWarps;
+  return splits == 1 ? keys : max((keys + splits - 1) / splits + kOf - 1 - ((keys + splits - 1) / splits + kOf - 1) % kOf, kLeastPart);
+}
 
 template <typename T, typename C, int D, bool WARPITEM>
-__global__ void __launch_bounds__(kWarps * 32, 3)
+__global__ void __launch_bounds__(kWarps * 32, 4)
 decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using S = DecodePlan<D>;
-  constexpr int kStages = S::kStages, kPieces = D / 16, kStep = WARPITEM ? 1 : kWarps;
+  constexpr int kStages = S::kStages, kTiles = S::kTiles, kUnit = kTiles * kTok, kPieces = D / 16, kStep = WARPITEM ? 1 : kWarps;
   const Cache& c = P.a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, tq = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;");
-  const int item = WARPITEM ? blockIdx.x * kWarps + warp : blockIdx.x, ofs = WARPITEM ? 0 : warp;
-  if (item >= P.items) return;        // (only warps of their own items)
-  const int split = item % P.splits, rest = item / P.splits, block = rest % P.blocks, kvh = rest / P.blocks % c.Hkv, b = rest / P.blocks / c.Hkv;
-  const int head0 = kvh * P.heads + block * 8, G = min(8, P.heads - block * 8);
+  const int unit = WARPITEM ? blockIdx.x * kWarps + warp : blockIdx.x, ofs = WARPITEM ? 0 : warp;
+  if (WARPITEM && unit >= P.items) return;
+  const int split = WARPITEM ? 0 : unit % P.splits, item = WARPITEM ? unit : unit / P.splits, block = item % P.blocks, kvh = item / P.blocks % c.Hkv, b = item / P.blocks / c.Hkv;
+  const int head0 = kvh * P.heads + block * 8, G = min(8, P.heads - block * 8), keys = c.keys(P.a.r.context_lens[b]);
+  const int part = WARPITEM ? keys : part_of(keys, P.splits), first = split * part, run = first < keys ? (min(part, keys - first) + kUnit - 1) / kUnit : 0, u0 = first / kUnit;
+  const int mine = run > ofs ? (run - ofs + kStep - 1) / kStep : 0;       // units u0 + ofs, and every kStep-th
 
   extern __shared__ unsigned char raw_smem[];
   unsigned char* sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
@@ -207,47 +222,52 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
   }
   if constexpr (WARPITEM) __syncwarp();
   else __syncthreads();
-
-  const int keys = c.keys(P.a.r.context_lens[b]), tiles = (keys + kTok - 1) / kTok;
-  const int t0 = min(tiles, split * P.tiles_per_split), t1 = split == P.splits - 1 ? tiles : min(tiles, t0 + P.tiles_per_split);
-  const int mine = t1 - t0 > ofs ? (t1 - t0 - ofs + kStep - 1) / kStep : 0;       // tiles t0 + ofs, and every kStep-th
-  const int per_page = c.bs / kTok;
-
-  // Pages of 32 tiles at a time, a lane each, and their scales: the next ones under way while these are used
-  auto page_at = [&](int j) -> int {        // of the warp's tile j; outside the pool: behind it, where copies bring zeros
-    if (j >= mine) return 0;
-    const int p = c.page(b, (t0 + ofs + j * kStep) / per_page);
-    return p < 0 ? static_cast<int>(c.max_blocks) : p;
+  const int per_page = c.bs / kTok, my_token = (lane >> 3 & 1) * 8 + (lane & 7), my_piece = lane >> 4;       // of four 8 x 8 matrices: tokens 0 - 7, 8 - 15, the next piece's
+  uint32_t at[kPieces / 2];
+#pragma unroll
+  for (int p = 0; p < kPieces; p += 2) at[p / 2] = tile_at<D>(my_token, p + my_piece);
+  // Pages of 32 units at a time, a lane each, and their scales: the next ones under way while these are used
+  auto place_of = [&](int j, int h) -> int {        // page and head of the unit's tile h; -1: none, or outside the pool
+    const int tile = kTiles * (u0 + ofs + j * kStep) + h;
+    if (j >= mine || tile * kTok >= keys) return -1;
+    const int p = c.page(b, tile / per_page);
+    return p < 0 ? -1 : p * c.Hkv + kvh;
   };
-  auto scales_of = [&](int page, int j, float& ks, float& vs) {
-    ks = vs = 1.f;
-    if (j < mine && page < c.max_blocks) {
-      ks = c.k_scale[static_cast<int64_t>(page) * c.Hkv + kvh];
-      vs = q8::max_nan(c.v_scale[static_cast<int64_t>(page) * c.Hkv + kvh], q8::kLeastScale);
-    }
+  auto line_of = [&](int place, int j, int h) -> int {        // where copies begin: behind the pool they bring zeros
+    const int tile = kTiles * (u0 + ofs + j * kStep) + h;
+    return (place < 0 ? static_cast<int>(c.max_blocks) * c.Hkv * c.bs : place * c.bs + tile % per_page * kTok) / (128 / D);
   };
-  int pages = page_at(lane), pages_next = page_at(32 + lane), window = 0;
-  float ks, vs, ks_next, vs_next;
-  auto issue = [&](int j) {
-    if (j - window >= 32) {
-      window += 32;
-      pages = pages_next;
-      pages_next = page_at(window + 32 + lane);
-      scales_of(pages, window + lane, ks_next, vs_next);
-    }
-    const int page = __shfl_sync(0xffffffffu, pages, j - window);
+  auto scale_of = [&](const float* scales, int place) { return place < 0 ? 1.f : scales[place]; };
+  int place[kTiles], lines[kTiles];
+  float ks[kTiles], vs[kTiles], ks_next[kTiles], vs_next[kTiles];
+#pragma unroll
+  for (int h = 0; h < kTiles; ++h) place[h] = place_of(lane, h);
+#pragma unroll
+  for (int h = 0; h < kTiles; ++h) lines[h] = line_of(place[h], lane, h);
+  auto issue = [&](int j, int buf) {
+    int from[kTiles];
+#pragma unroll
+    for (int h = 0; h < kTiles; ++h) from[h] = __shfl_sync(0xffffffffu, lines[h], j & 31);
     if (lane == 0) {
-      const uint32_t to = ring + j % kStages * S::kStage, bar = bars + j % kStages * 8;
-      const int tile = t0 + ofs + j * kStep, line = ((page * c.Hkv + kvh) * c.bs + tile % per_page * kTok) / (128 / D);
+      const uint32_t to = ring + buf * S::kStage, bar = bars + buf * 8;
+      auto copy = [&](uint32_t at, const CUtensorMap* map, int line) {
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(at), "l"(map), "r"(0), "r"(line), "r"(bar) : "memory");
+      };
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStage) : "memory");
-      asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(&k_map), "r"(0), "r"(line), "r"(bar) : "memory");
-      asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to + S::kTile), "l"(&v_map), "r"(0), "r"(line), "r"(bar) : "memory");
+#pragma unroll
+      for (int h = 0; h < kTiles; ++h) {
+        copy(to + h * S::kTile, &k_map, from[h]);
+        copy(to + (kTiles + h) * S::kTile, &v_map, from[h]);
+      }
     }
   };
   const int ahead = min(kStages, mine);
-  for (int j = 0; j < ahead; ++j) issue(j);
-  scales_of(pages, lane, ks, vs);
-  vs = log2f(vs);
+  for (int j = 0; j < ahead; ++j) issue(j, j);
+#pragma unroll
+  for (int h = 0; h < kTiles; ++h) {
+    ks[h] = scale_of(c.k_scale, place[h]), vs[h] = scale_of(c.v_scale, place[h]);
+    place[h] = place_of(32 + lane, h);
+  }
 
   // queries: head quad's columns 16 i + 4 tq .. + 3
   uint32_t qf[kPieces][2];
@@ -262,65 +282,83 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
     for (int i = 0; i < kPieces; ++i) {
       const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) most = fmaxf(most, fabsf(Cvt<T>::to_f32(e[u])));
+      for (int u = 0; u < 4; ++u) most = q8::max_nan(most, fabsf(Cvt<T>::to_f32(e[u])));
     }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    float f = P.a.scale * 1.4426950408889634f;
     const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) - 14;       // most = 2^(e + 14) .. 2^(e + 15)
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const T* x = reinterpret_cast<const T*>(&raw[i]);
       qf[i][0] = pack2<__half>(Cvt<T>::to_f32(x[0]) * down, Cvt<T>::to_f32(x[1]) * down);
       qf[i][1] = pack2<__half>(Cvt<T>::to_f32(x[2]) * down, Cvt<T>::to_f32(x[3]) * down);
     }
-    const float f = P.a.scale * 1.4426950408889634f * up;
+    f *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     factor[0] = __shfl_sync(0xffffffffu, f, 8 * tq);
     factor[1] = __shfl_sync(0xffffffffu, f, 8 * tq + 4);
   }
+#pragma unroll
+  for (int h = 0; h < kTiles; ++h) vs[h] = log2f(q8::max_nan(vs[h], q8::kLeastScale));
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kPieces][4];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  const int my_token = (lane >> 3 & 1) * 8 + (lane & 7), my_piece = lane >> 4;       // of four 8 x 8 matrices: tokens 0 - 7, 8 - 15, the next piece's
   bool ok = true;
-  for (int i = 0; i < mine; ++i) {
-    if ((i & 31) == 0 && i > 0) ks = ks_next, vs = log2f(vs_next);
-    const int tile = t0 + ofs + i * kStep;
-    const uint32_t k_tile = ring + i % kStages * S::kStage, v_tile = k_tile + S::kTile;
-    ok = __all_sync(0xffffffffu, bar_wait1(bars + i % kStages * 8, (i / kStages) & 1, dead));
-    if (!ok) break;
-    const float kt = __shfl_sync(0xffffffffu, ks, i & 31), ls = __shfl_sync(0xffffffffu, vs, i & 31);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+  int buf = 0, left = keys - kUnit * (u0 + ofs);        // tokens from the unit's first on
+  uint32_t parity = 0;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i, left -= kUnit * kStep) {
+    if ((i & 31) == 0 && i > 0) {
 #pragma unroll
-    for (int p = 0; p < kPieces; p += 2) {
-      uint32_t r[4];
-      ldsm4(r, k_tile + tile_at<D>(my_token, p + my_piece));
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t a0, a1, a2, a3;
-        q8::halves<C, false>(r[2 * u], a0, a2);
-        q8::halves<C, false>(r[2 * u + 1], a1, a3);
-        mma16(s, a0, a1, a2, a3, qf[p + u][0], qf[p + u][1]);
-      }
+      for (int h = 0; h < kTiles; ++h) ks[h] = ks_next[h], vs[h] = log2f(q8::max_nan(vs_next[h], q8::kLeastScale));
     }
-    // s[0], s[1]: token quad, heads 2 tq and 2 tq + 1; s[2], s[3]: token quad + 8
-    const int left = keys - tile * kTok;        // tokens of the tile
-    const float f0 = factor[0] * kt, f1 = factor[1] * kt;
-    float x[4] = {fmaf(s[0], f0, ls), fmaf(s[1], f1, ls), fmaf(s[2], f0, ls), fmaf(s[3], f1, ls)};
-    if (left < kTok) {
-      if (quad >= left) x[0] = x[1] = -INFINITY;
-      if (quad + 8 >= left) x[2] = x[3] = -INFINITY;
+    const uint32_t tiles = ring + buf * S::kStage;
+    ok = __all_sync(0xffffffffu, bar_wait1(bars + buf * 8, parity, dead));
+    if (!ok) break;
+    float x[kTiles][4], ls[kTiles];
+#pragma unroll
+    for (int h = 0; h < kTiles; ++h) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < kPieces; p += 2) {
+        uint32_t r[4];
+        ldsm4(r, tiles + h * S::kTile + at[p / 2]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a0, a1, a2, a3;
+          q8::halves<C, false>(r[2 * u], a0, a2);
+          q8::halves<C, false>(r[2 * u + 1], a1, a3);
+          mma16(s, a0, a1, a2, a3, qf[p + u][0], qf[p + u][1]);
+        }
+      }
+      // s[0], s[1]: token quad, heads 2 tq and 2 tq + 1; s[2], s[3]: token quad + 8
+      const float kt = __shfl_sync(0xffffffffu, ks[h], i & 31), f0 = factor[0] * kt, f1 = factor[1] * kt;
+      ls[h] = __shfl_sync(0xffffffffu, vs[h], i & 31);
+      x[h][0] = fmaf(s[0], f0, ls[h]), x[h][1] = fmaf(s[1], f1, ls[h]), x[h][2] = fmaf(s[2], f0, ls[h]), x[h][3] = fmaf(s[3], f1, ls[h]);
+    }
+    if (left < kUnit) {
+#pragma unroll
+      for (int h = 0; h < kTiles; ++h) {
+        if (h * kTok + quad >= left) x[h][0] = x[h][1] = -INFINITY;
+        if (h * kTok + quad + 8 >= left) x[h][2] = x[h][3] = -INFINITY;
+      }
       if constexpr (std::is_same_v<C, q8::E4m3>) {       // what is behind the last token may be no number
-        for (int e = left * kPieces + lane; e < kTok * kPieces; e += 32)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(v_tile + tile_at<D>(e / kPieces, e % kPieces)), "r"(0) : "memory");
+        for (int e = left * kPieces + lane; e < kUnit * kPieces; e += 32) {
+          const int token = e / kPieces;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tiles + (kTiles + token / kTok) * S::kTile + tile_at<D>(token % kTok, e % kPieces)), "r"(0) : "memory");
+        }
         __syncwarp();
       }
     }
-    if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[0] + 14.f || fmaxf(x[1], x[3]) > m[1] + 14.f)) {
+    float t0 = fmaxf(x[0][0], x[0][2]), t1 = fmaxf(x[0][1], x[0][3]);
+#pragma unroll
+    for (int h = 1; h < kTiles; ++h) t0 = fmaxf(t0, fmaxf(x[h][0], x[h][2])), t1 = fmaxf(t1, fmaxf(x[h][1], x[h][3]));
+    if (__any_sync(0xffffffffu, t0 > m[0] + 14.f || t1 > m[1] + 14.f)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float top = fmaxf(x[h], x[h + 2]);
+        float top = h ? t1 : t0;
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -331,29 +369,44 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
         for (int p = 0; p < kPieces; ++p) o[p][h] *= corr, o[p][h + 2] *= corr;
       }
     }
-    float w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[e] - m[e & 1]);
-    const float per = exp2_fast(-ls);
-    l[0] = fmaf(w[0] + w[2], per, l[0]);
-    l[1] = fmaf(w[1] + w[3], per, l[1]);
-    const uint32_t b0 = transposed(pack2<__half>(w[0], w[1])), b1 = transposed(pack2<__half>(w[2], w[3]));
+    for (int h = 0; h < kTiles; ++h) {
+      float w[4];
 #pragma unroll
-    for (int p = 0; p < kPieces; p += 2) {
-      uint32_t r[4];
-      ldsm4_trans(r, v_tile + tile_at<D>(my_token, p + my_piece));
+      for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[h][e] - m[e & 1]);
+      const float per = exp2_fast(-ls[h]);
+      l[0] = fmaf(w[0] + w[2], per, l[0]);
+      l[1] = fmaf(w[1] + w[3], per, l[1]);
+      const uint32_t b0 = transposed(pack2<__half>(w[0], w[1])), b1 = transposed(pack2<__half>(w[2], w[3]));
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t a0, a1, a2, a3;
-        q8::halves<C, true>(r[2 * u], a0, a1);
-        q8::halves<C, true>(r[2 * u + 1], a2, a3);
-        mma16(o[p + u], a0, a1, a2, a3, b0, b1);
+      for (int p = 0; p < kPieces; p += 2) {
+        uint32_t r[4];
+        ldsm4_trans(r, tiles + (kTiles + h) * S::kTile + at[p / 2]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a0, a1, a2, a3;
+          q8::halves<C, true>(r[2 * u], a0, a1);
+          q8::halves<C, true>(r[2 * u + 1], a2, a3);
+          mma16(o[p + u], a0, a1, a2, a3, b0, b1);
+        }
       }
     }
     __syncwarp();       // every lane has read the buffer
-    if (i + kStages < mine) issue(i + kStages);
+    const int next = i + kStages;
+    if (next < mine) {
+      if ((next & 31) == 0) {
+#pragma unroll
+        for (int h = 0; h < kTiles; ++h) {
+          lines[h] = line_of(place[h], next + lane, h);
+          ks_next[h] = scale_of(c.k_scale, place[h]), vs_next[h] = scale_of(c.v_scale, place[h]);
+          place[h] = place_of(next + 32 + lane, h);
+        }
+      }
+      issue(next, buf);
+    }
+    if (++buf == kStages) buf = 0, parity ^= 1;
   }
-  if (!ok) {      // a wait gave up: what is under way gets 10 ms to end; no number comes out
+  if (!ok || *dead) {      // a wait gave up: what is under way gets 10 ms to end; no number comes out
     for (const long long begun = clock64(); clock64() - begun < 20000000ll;) {}
     l[0] = l[1] = NAN;
   }
@@ -394,16 +447,68 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
       a0 = fmaf(v.x, k, a0);
       a1 = fmaf(v.y, k, a1);
     }
-    const int64_t row = static_cast<int64_t>(b) * P.a.Hq + head0 + g;
-    if (P.splits == 1) {
+    if (WARPITEM || P.splits == 1) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + row * D + d) = pack2<T>(a0 * f, a1 * f);
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + (static_cast<int64_t>(b) * P.a.Hq + head0 + g) * D + d) = pack2<T>(a0 * f, a1 * f);
     } else {
-      const int64_t part = row * P.splits + split;
-      *reinterpret_cast<float2*>(P.ws_acc + part * D + d) = make_float2(a0, a1);
-      if (d == 0) *reinterpret_cast<float2*>(P.ws_ml + part * 2) = make_float2(top * 0.6931471805599453f, sum);
+      const int64_t piece = static_cast<int64_t>(unit) * 8 + g;
+      *reinterpret_cast<float2*>(P.o + piece * D + d) = make_float2(a0, a1);
+      if (d == 0) P.ml[piece] = make_float2(top, sum);
     }
   }
+}
+
+// A CTA per item and head: the parts in the order of the keys, by four groups of threads.  (All that needs no part is done before the kernel ahead ends.)
+template <typename T, int D>
+__global__ void __launch_bounds__(2 * D) decode_merge_kernel(const Decode P) {
+  constexpr int kCols = D / 2, kAhead = 4;      // two columns a thread
+  __shared__ float2 part_s[3][kCols];
+  __shared__ float sum_s[4], top_s[4];
+  const int most = min(P.heads, 8), g = blockIdx.x % most, item = blockIdx.x / most, block = item % P.blocks, kvh = item / P.blocks % P.a.c.Hkv, b = item / P.blocks / P.a.c.Hkv;
+  const int col = threadIdx.x % kCols, group = threadIdx.x / kCols, keys = P.a.c.keys(P.a.r.context_lens[b]), part = part_of(keys, P.splits), parts = keys > 0 ? (keys + part - 1) / part : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (block * 8 + g >= P.heads) return;
+  float top = -INFINITY, sum = 0.f;
+  float2 o = make_float2(0.f, 0.f);
+  for (int p0 = group; p0 < parts; p0 += 4 * kAhead) {
+    float2 ml[kAhead], v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int p = p0 + 4 * u;
+      const int64_t piece = (static_cast<int64_t>(item) * P.splits + p) * 8 + g;
+      ml[u] = make_float2(-INFINITY, 0.f), v[u] = make_float2(0.f, 0.f);
+      if (p < parts) ml[u] = P.ml[piece], v[u] = *reinterpret_cast<const float2*>(P.o + piece * D + 2 * col);
+    }
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) now = fmaxf(now, ml[u].x);
+    const float was = top == -INFINITY ? (sum != sum ? 1.f : 0.f) : exp2_fast(top - now);
+    top = now;
+    sum *= was, o.x *= was, o.y *= was;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float k = ml[u].x == -INFINITY ? (ml[u].y != ml[u].y ? 1.f : 0.f) : exp2_fast(ml[u].x - now);
+      sum = fmaf(ml[u].y, k, sum), o.x = fmaf(v[u].x, k, o.x), o.y = fmaf(v[u].y, k, o.y);
+    }
+  }
+  if (col == 0) top_s[group] = top, sum_s[group] = sum;
+  if (group > 0) part_s[group - 1][col] = o;
+  __syncthreads();
+  if (group > 0) return;
+  float all_top = -INFINITY, k[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) all_top = fmaxf(all_top, top_s[y]);
+  sum = 0.f;
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    k[y] = top_s[y] == -INFINITY ? (sum_s[y] != sum_s[y] ? 1.f : 0.f) : exp2_fast(top_s[y] - all_top);
+    sum = fmaf(sum_s[y], k[y], sum);
+  }
+  o.x *= k[0], o.y *= k[0];
+#pragma unroll
+  for (int y = 1; y < 4; ++y) o.x = fmaf(part_s[y - 1][col].x, k[y], o.x), o.y = fmaf(part_s[y - 1][col].y, k[y], o.y);
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + (static_cast<int64_t>(b) * P.a.Hq + kvh * P.heads + block * 8 + g) * D + 2 * col) = pack2<T>(o.x * f, o.y * f);
 }
 
 // The pool as lines of 128 bytes, fetched 16 tokens at a time; lines behind the pool read as zeros
@@ -418,44 +523,59 @@ bool code_map(CUtensorMap* map, const void* pool, const Cache& c) {
 
 bool decode_serves(int D, int bs, int dtype) { return dtype != B200_DTYPE_F32 && (D == 64 || D == 128) && bs % kTok == 0; }
 
-// Parts of the keys
-constexpr int kMostSplits = 256;        // that are put together
-int decode_splits(int B, int Hq, int Hkv, int bs, int longest) {
-  const int64_t items = static_cast<int64_t>(B) * Hkv * ((Hq / Hkv + 7) / 8), tiles = (longest + kTok - 1) / kTok;
-  int64_t splits = items >= 2 * kNumSMs ? 1 : (3 * kNumSMs + items - 1) / items;
-  (void)bs;
-  splits = splits < 1 ? 1 : splits;
-  const int64_t most = (tiles + 15) / 16;       // 16 tiles a part at least
-  splits = splits < most ? splits : most > 1 ? most : 1;
-  return static_cast<int>(splits < kMostSplits ? splits : kMostSplits);
+// Parts of an item.  Items of up to 512 tokens are not divided (a second launch costs the host 5 us and the device 3).  592 CTAs are resident: what fits is
+// divided until there are some 400 of them; long contexts go on to 1024, parts of 2048 tokens, which evens out that SMs are not served alike.  32 heads over 8
+// of 128, us with 1 / 2 / 3 / 4 / 6 / 8 / 16 parts: 1 x 4096 39 / 22 / 17 / 14 / 12 / 9 / 7; 8 x 8192 80 / 44 / 39 / 31 / 29 / 30 / 32; 16 x 4096 43 / 31 / 29 / 31 / 35 / 32 / 37;
+// 32 x 2048 30 / 32 / 35 / 34 / 36 / 39 / 46; 64 x 2048 51 / 56 / 58 / 58 / 61 / 67 / 83; 64 x 8192 185 / 173 / 179 / 176 / 177 / 176; 128 x 2048 90 / 103 / 102 / 104; 8 x 32768 of
+// e4m3, ragged, 274 / 152 / 111 / 86 / 75 / 75 / 72.
+constexpr int kShort = 512;
+int splits_of(int64_t items, int longest) {
+  if (longest <= kShort) return 1;
+  int64_t splits = 400 / items;
+  if (longest >= 8192) splits = std::max(splits, std::min<int64_t>(longest / 2048, 1024 / items));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, (longest + kLeastPart - 1ll) / kLeastPart)));
 }
+int64_t items_of(int B, int Hq, int Hkv) { return static_cast<int64_t>(B) * Hkv * ((Hq / Hkv + 7) / 8); }
 
 template <typename T, typename C, int D, bool WARPITEM>
 int launch_decode_as(const char* name, const Decode& P, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
   auto kern = decode_kernel<T, C, D, WARPITEM>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodePlan<D>::kSmem);
-  kern<<<WARPITEM ? (P.items + kWarps - 1) / kWarps : P.items, kWarps * 32, DecodePlan<D>::kSmem, stream>>>(P, k_map, v_map);
-  return check_launch(name);
+  kern<<<WARPITEM ? (P.items + kWarps - 1) / kWarps : P.items * P.splits, kWarps * 32, DecodePlan<D>::kSmem, stream>>>(P, k_map, v_map);
+  if (int rc = check_launch(name)) return rc;
+  if (P.splits == 1) return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(P.items) * static_cast<unsigned>(P.heads < 8 ? P.heads : 8));
+  cfg.blockDim = dim3(2 * D);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_merge_kernel<T, D>, P);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
+  }
+  return 0;
 }
 
 template <typename T>
-int launch_decode(const char* name, const Attn& A, int splits, int longest, void* workspace, int codes, int dtype, cudaStream_t stream) {
+int launch_decode(const char* name, const Attn& A, int longest, void* workspace, int codes, cudaStream_t stream) {
   Decode P{};
-  P.a = A, P.heads = A.Hq / A.c.Hkv, P.blocks = (P.heads + 7) / 8, P.splits = splits;
-  const int tiles = static_cast<int>((static_cast<int64_t>(longest) + kTok - 1) / kTok);
-  P.tiles_per_split = tiles > 0 ? (tiles + splits - 1) / splits : 1;
-  P.items = A.r.B * A.c.Hkv * P.blocks * splits;
-  P.ws_acc = static_cast<float*>(workspace), P.ws_ml = P.ws_acc + static_cast<int64_t>(A.r.B) * A.Hq * splits * A.c.D;
+  P.a = A, P.heads = A.Hq / A.c.Hkv, P.blocks = (P.heads + 7) / 8, P.items = static_cast<int>(items_of(A.r.B, A.Hq, A.c.Hkv));
+  P.splits = splits_of(P.items, longest);
+  P.ml = static_cast<float2*>(workspace), P.o = static_cast<float*>(workspace) + static_cast<int64_t>(P.items) * P.splits * 16;
   CUtensorMap k_map, v_map;
   if (!code_map(&k_map, A.c.k_pool, A.c) || !code_map(&v_map, A.c.v_pool, A.c)) return fail(B200_EINVAL, "%s: no tensor map of the pools", name);
-  const bool short_items = P.items > 2 * kNumSMs && P.tiles_per_split <= 32;
+  const bool warps = longest <= kShort && P.items > 4 * kNumSMs;       // more than are resident at once
   auto go = [&](auto* c, auto d) {
     using C = std::remove_pointer_t<decltype(c)>;
-    return short_items ? launch_decode_as<T, C, d.value, true>(name, P, k_map, v_map, stream) : launch_decode_as<T, C, d.value, false>(name, P, k_map, v_map, stream);
+    return warps ? launch_decode_as<T, C, d.value, true>(name, P, k_map, v_map, stream) : launch_decode_as<T, C, d.value, false>(name, P, k_map, v_map, stream);
   };
   auto of = [&](auto* c) { return A.c.D == 128 ? go(c, std::integral_constant<int, 128>{}) : go(c, std::integral_constant<int, 64>{}); };
-  if (int rc = codes == B200_CODES_INT8 ? of(static_cast<q8::Int8*>(nullptr)) : of(static_cast<q8::E4m3*>(nullptr))) return rc;
-  return splits > 1 ? attn_combine(A.out, P.ws_acc, P.ws_ml, A.r.B * A.Hq, A.c.D, splits, dtype, stream) : 0;
+  return codes == B200_CODES_INT8 ? of(static_cast<q8::Int8*>(nullptr)) : of(static_cast<q8::E4m3*>(nullptr));
 }
 
 constexpr int kAnyMostD = 256;
@@ -502,34 +622,33 @@ using namespace b200;
 
 extern "C" {
 
-size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int num_splits, int dtype) {
+size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || block_size <= 0 || max_context_len < 0 || !decode_serves(D, block_size, dtype)) return 0;
-  const int splits = num_splits > 0 ? num_splits : decode_splits(B, Hq, Hkv, block_size, max_context_len);
-  return splits > 1 ? static_cast<size_t>(B) * Hq * splits * (D + 2) * sizeof(float) : 0;
+  const int64_t items = items_of(B, Hq, Hkv), splits = splits_of(items, max_context_len);
+  return splits > 1 ? static_cast<size_t>(items * splits) * 8 * (D + 2) * sizeof(float) : 0;
 }
 
 int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                               const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, int B, int Hq, int Hkv, int D,
-                              int block_size, int64_t max_blocks, float scale, int max_context_len, int num_splits, void* workspace, size_t workspace_bytes,
-                              int codes, int dtype, unsigned flags, void* stream) {
+                              int block_size, int64_t max_blocks, float scale, int max_context_len, void* workspace, size_t workspace_bytes, int codes,
+                              int dtype, unsigned flags, void* stream) {
   const char* name = "b200_paged_decode_attn_q8";
   const Attn A{cache_of(k_pool, v_pool, k_scale, v_scale, block_tables, table_stride, table_cols, Hkv, D, block_size, max_blocks),
                Rows{nullptr, context_lens, B, B}, out, q, q_stride, Hq, scale};
   if (int rc = check_attn(name, A, codes, dtype)) return rc;
-  if (max_context_len < 0 || num_splits < 0 || num_splits > kMostSplits) return fail(B200_EINVAL, "%s: max_context_len %d, num_splits %d", name, max_context_len, num_splits);
+  if (max_context_len < 0) return fail(B200_EINVAL, "%s: negative max_context_len", name);
   if (B == 0) return 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int splits = num_splits > 0 ? num_splits : decode_splits(B, Hq, Hkv, block_size, max_context_len);
   const bool pieces = aligned16(k_pool) && aligned16(v_pool) && !(reinterpret_cast<uintptr_t>(q) & 7) && q_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(out) & 3);
+  const int64_t items = items_of(B, Hq, Hkv);
+  // pages, items and parts whose numbers fit
   if (decode_serves(D, block_size, dtype) && pieces && !(flags & B200_ATTN_FORCE_GENERIC) && (max_blocks + 1) * Hkv * block_size < INT32_MAX &&
-      static_cast<int64_t>(B) * Hkv * ((Hq / Hkv + 7) / 8) * splits < INT32_MAX / 2) {
-    if (splits > 1) {
-      if (!workspace || workspace_bytes < b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, num_splits, dtype))
-        return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);
-      if (!aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
-    }
-    return dtype == B200_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(name, A, splits, max_context_len, workspace, codes, dtype, s)
-                                    : launch_decode<__half>(name, A, splits, max_context_len, workspace, codes, dtype, s);
+      items * 8 * splits_of(items, max_context_len) < INT32_MAX) {
+    const size_t need = b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, dtype);
+    if (need && (!workspace || workspace_bytes < need)) return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);
+    if (need && !aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
+    return dtype == B200_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(name, A, max_context_len, workspace, codes, s)
+                                    : launch_decode<__half>(name, A, max_context_len, workspace, codes, s);
   }
   return launch_any_of(name, A, codes, dtype, s);
 }

@@ -858,41 +858,63 @@ def kv_gather_dense(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: to
 CODES_ID = {torch.int8: 3, torch.float8_e4m3fn: 8}
 
 
+def _q8_launch(dev: int, what: str, args: tuple) -> None:
+    """The library's call on the tensors' device and its current stream."""
+    fn = getattr(_lib.load(), what)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with _There(dev) as stream:
+            rc = fn(*args, stream)
+    if rc != 0:
+        _lib.check(rc, what)
+
+
 def _q8_cache(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor, dev: int):
     """Checks of a cache in 8 bits and its tables; ``(shape, codes, pointers of pools, scales and tables, row stride and columns of the tables)``."""
-    codes = CODES_ID.get(k_pool.dtype)
+    shape, kind, tables = k_pool.shape, k_pool.dtype, block_tables.shape
+    codes = CODES_ID.get(kind)
     if codes is None:
-        raise TypeError(f"a cache in 8 bits holds int8 or float8_e4m3fn, not {k_pool.dtype}")
-    shape = k_pool.shape
+        raise TypeError(f"a cache in 8 bits holds int8 or float8_e4m3fn, not {kind}")
     if len(shape) != 4 or not k_pool.is_contiguous():
         raise ValueError("pool must be a contiguous [max_blocks, Hkv, block_size, D] tensor")
-    if v_pool.shape != shape or v_pool.dtype != k_pool.dtype or not v_pool.is_contiguous():
+    if v_pool.shape != shape or v_pool.dtype is not kind or not v_pool.is_contiguous():
         raise ValueError("k_pool and v_pool must match")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.shape != shape[:2] or not s.is_contiguous() or s.get_device() != dev:
-            raise ValueError("k_scale and v_scale must be contiguous fp32 [max_blocks, Hkv] on the same device")
-    if k_pool.get_device() != dev or v_pool.get_device() != dev:
-        raise ValueError("the pools must be on the same device")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.get_device() != dev:
-        raise ValueError("block_tables must be int32 [B, n] with contiguous rows, on the same device")
-    rows, cols = block_tables.shape
-    if cols == 0 or (cols > 1 and block_tables.stride(1) != 1):
-        raise ValueError("block_tables must be int32 [B, n] with contiguous rows, on the same device")
+    pages = shape[:2]
+    if (k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != pages or v_scale.shape != pages
+            or not k_scale.is_contiguous() or not v_scale.is_contiguous()):
+        raise ValueError("k_scale and v_scale must be contiguous fp32 [max_blocks, Hkv]")
+    if not dev == k_pool.get_device() == v_pool.get_device() == k_scale.get_device() == v_scale.get_device() == block_tables.get_device():
+        raise ValueError("the pools, their scales and block_tables must be on the same device")
+    if block_tables.dtype is not torch.int32 or len(tables) != 2 or tables[1] == 0 or not (block_tables.is_contiguous() or tables[1] == 1 or block_tables.stride(1) == 1):
+        raise ValueError("block_tables must be int32 [B, n] with contiguous rows")
+    cols = tables[1]
     return shape, codes, (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
-                          block_tables.stride(0) if rows > 1 else cols, cols)
+                          cols if tables[0] <= 1 or block_tables.is_contiguous() else block_tables.stride(0), cols)
 
 
 def _q8_lens(context_lens: torch.Tensor, row_starts: Optional[torch.Tensor], B: int, rows: int, dev: int):
     """Pointers of the lengths and of the rows' starts."""
-    if context_lens.dtype != torch.int32 or context_lens.shape != (B,) or not context_lens.is_contiguous() or context_lens.get_device() != dev:
+    if context_lens.dtype is not torch.int32 or context_lens.shape != (B,) or not context_lens.is_contiguous() or context_lens.get_device() != dev:
         raise ValueError("context_lens must be a contiguous int32 [B] on the same device")
     if row_starts is None:
         if rows != B:
             raise ValueError(f"{rows} rows of {B} sequences need row_starts")
         return context_lens.data_ptr(), None
-    if row_starts.dtype != torch.int32 or row_starts.shape != (B + 1,) or not row_starts.is_contiguous() or row_starts.get_device() != dev:
+    if row_starts.dtype is not torch.int32 or row_starts.shape != (B + 1,) or not row_starts.is_contiguous() or row_starts.get_device() != dev:
         raise ValueError("row_starts must be a contiguous int32 [B + 1] on the same device")
     return context_lens.data_ptr(), row_starts.data_ptr()
+
+
+def _q8_rows(x: torch.Tensor, n: int, D: int, dtype: torch.dtype, dev: int, what: str):
+    """Heads and row stride of ``x [n, heads, D]``, the heads contiguous inside a row."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != n or shape[2] != D or x.get_device() != dev:
+        raise ValueError(f"{what} must be [{n}, heads, {D}] on the same device")
+    if x.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}")
+    heads = shape[1]
+    return heads, heads * D if x.is_contiguous() else _row_stride(x, heads, D)
 
 
 def rope_kv_append_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
@@ -907,43 +929,39 @@ def rope_kv_append_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
     ``context_lens[b]`` tokens; ``max_new`` (default: ``n``) bounds how many a sequence has.  Where new tokens do not begin a page they share its scale with the
     earlier ones, whose codes are put into a scale that had to grow.  ``cos / sin``: contiguous ``[n, D]`` in the storage dtype.  Other
     than in ``rope_kv_append`` the rotation is in fp32, rounded once (queries) or not before the code (keys)."""
-    _need_cuda(k, v, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens)
+    _need_cuda(k)
     dev, dtype = k.get_device(), k.dtype
     (max_blocks, Hkv, bs, D), codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
-    n, B = k.shape[0], block_tables.shape[0]
-    if v.shape[0] != n or v.dtype != dtype or v.get_device() != dev:
-        raise ValueError("k and v must be [n, Hkv, D] of one dtype on one device")
+    n, B, dt = k.shape[0], block_tables.shape[0], _dtype_id(k)
     lens, starts = _q8_lens(context_lens, row_starts, B, n, dev)
+    heads, k_stride = _q8_rows(k, n, D, dtype, dev, "k")
+    v_heads, v_stride = _q8_rows(v, n, D, dtype, dev, "v")
+    if heads != Hkv or v_heads != Hkv:
+        raise ValueError(f"k and v must have the pools' {Hkv} heads")
     if (cos is None) != (sin is None) or (q is not None and cos is None):
         raise ValueError("cos and sin come together, and with queries")
-    cp = sp = None
+    cp = sp = qp = op = None
+    q_stride = o_stride = Hq = 0
     if cos is not None:
-        if cos.shape != (n, D) or sin.shape != (n, D) or not cos.is_contiguous() or not sin.is_contiguous() or cos.get_device() != dev or sin.get_device() != dev:
+        if (cos.shape != (n, D) or sin.shape != (n, D) or not cos.is_contiguous() or not sin.is_contiguous()
+                or not dev == cos.get_device() == sin.get_device()):
             raise ValueError("cos / sin must be contiguous [n, D] on the same device")
-        if cos.dtype != dtype or sin.dtype != dtype:
+        if cos.dtype is not dtype or sin.dtype is not dtype:
             raise TypeError("q, k, v, cos and sin must share one dtype")
         cp, sp = cos.data_ptr(), sin.data_ptr()
-    qp = op = None
-    q_stride = o_stride = Hq = 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != n or q.get_device() != dev:
-            raise ValueError("q must be [n, Hq, D] on the same device")
-        if q.dtype != dtype:
-            raise TypeError("q, k, v, cos and sin must share one dtype")
-        Hq = q.shape[1]
-        q_stride = _row_stride(q, Hq, D)
+        Hq, q_stride = _q8_rows(q, n, D, dtype, dev, "q")
         if q_out is None:
-            q_out = torch.empty((n, Hq, D), dtype=dtype, device=q.device)
-        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != dev:
-            raise ValueError("q_out must be a tensor like q")
-        o_stride = _row_stride(q_out, Hq, D)
+            q_out = torch.empty_like(q) if q.is_contiguous() else torch.empty((n, Hq, D), dtype=dtype, device=q.device)
+            o_stride = Hq * D
+        else:
+            o_heads, o_stride = _q8_rows(q_out, n, D, dtype, dev, "q_out")
+            if o_heads != Hq:
+                raise ValueError("q_out must be a tensor like q")
         qp, op = q.data_ptr(), q_out.data_ptr()
-    with _on(dev) as stream:
-        rc = _lib.load().b200_rope_kv_append_q8(
-            op, o_stride, qp, q_stride, k.data_ptr(), _row_stride(k, Hkv, D), v.data_ptr(), _row_stride(v, Hkv, D), cp, sp, *cache, lens, starts, B, n,
-            n if max_new is None else int(max_new), Hq, Hkv, D, bs, max_blocks, codes, _dtype_id(k), stream)
-    if rc != 0:
-        _lib.check(rc, "b200_rope_kv_append_q8")
+    _q8_launch(dev, "b200_rope_kv_append_q8", (
+        op, o_stride, qp, q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, cp, sp, *cache, lens, starts, B, n,
+        n if max_new is None else int(max_new), Hq, Hkv, D, bs, max_blocks, codes, dt))
     return q_out
 
 
@@ -958,36 +976,32 @@ def kv_gather_dense_q8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torc
                        n_tokens: int, dtype: torch.dtype = torch.bfloat16):
     """``kv_gather_dense`` of a cache in 8 bits: the first ``n_tokens`` tokens of every row of ``block_tables`` as ``(k, v)``, each ``[B, Hkv, n_tokens, D]``
     of ``dtype`` (code times scale, rounded once)."""
-    _need_cuda(k_pool, v_pool, k_scale, v_scale, block_tables)
+    _need_cuda(k_pool)
     dev = k_pool.get_device()
     (max_blocks, Hkv, bs, D), codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
-    if dtype not in DTYPE_ID:
+    dt = DTYPE_ID.get(dtype)
+    if dt is None:
         raise TypeError(f"unsupported dtype {dtype}; expected float16, bfloat16 or float32")
     B = block_tables.shape[0]
     if n_tokens < 0 or n_tokens > block_tables.shape[1] * bs:
         raise ValueError(f"{n_tokens} tokens do not fit rows of {block_tables.shape[1]} blocks")
-    k_out = torch.empty((B, Hkv, n_tokens, D), dtype=dtype, device=k_pool.device)
+    k_out = k_pool.new_empty((B, Hkv, n_tokens, D), dtype=dtype)
     v_out = torch.empty_like(k_out)
-    with _on(dev) as stream:
-        rc = _lib.load().b200_kv_gather_dense_q8(k_out.data_ptr(), v_out.data_ptr(), *cache, B, n_tokens, Hkv, D, bs, max_blocks, codes, DTYPE_ID[dtype], stream)
-    if rc != 0:
-        _lib.check(rc, "b200_kv_gather_dense_q8")
+    _q8_launch(dev, "b200_kv_gather_dense_q8", (k_out.data_ptr(), v_out.data_ptr(), *cache, B, n_tokens, Hkv, D, bs, max_blocks, codes, dt))
     return k_out, v_out
 
 
 def _q8_attention(q: torch.Tensor, shape, out: Optional[torch.Tensor], dev: int):
     """Checks of queries and outputs; ``(heads, row stride, out)``."""
-    D, Hkv = shape[3], shape[1]
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"q must be [n, Hq, {D}]")
-    n, Hq, _ = q.shape
-    if Hq % Hkv != 0:
+    n, D, Hkv = q.shape[0], shape[3], shape[1]
+    Hq, stride = _q8_rows(q, n, D, q.dtype, dev, "q")
+    if Hq % Hkv != 0 or Hq == 0:
         raise ValueError(f"{Hq} query heads are no multiple of {Hkv} kv heads")
     if out is None:
-        out = torch.empty((n, Hq, D), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or not out.is_contiguous() or out.dtype != q.dtype or out.get_device() != dev:
+        out = torch.empty_like(q) if stride == Hq * D and q.is_contiguous() else torch.empty((n, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or not out.is_contiguous() or out.dtype is not q.dtype or out.get_device() != dev:
         raise ValueError("out must be a contiguous tensor of q's shape and dtype, on its device")
-    return Hq, _row_stride(q, Hq, D), out
+    return Hq, stride, out
 
 
 def _q8_workspace(need: int, workspace: Optional[torch.Tensor], q: torch.Tensor, dev: int):
@@ -1002,35 +1016,34 @@ def _q8_workspace(need: int, workspace: Optional[torch.Tensor], q: torch.Tensor,
 
 
 @functools.lru_cache(maxsize=1024)
-def decode_attention_q8_workspace(B: int, Hq: int, Hkv: int, D: int, block_size: int, max_context_len: int, dtype: torch.dtype,
-                                  num_splits: int = 0) -> int:
+def decode_attention_q8_workspace(B: int, Hq: int, Hkv: int, D: int, block_size: int, max_context_len: int, dtype: torch.dtype) -> int:
     """Bytes of scratch that ``paged_decode_attention_q8`` needs for these sizes."""
-    return _lib.load().b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, num_splits, DTYPE_ID[dtype])
+    return _lib.load().b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, DTYPE_ID[dtype])
 
 
 def paged_decode_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                               block_tables: torch.Tensor, context_lens: torch.Tensor, max_context_len: int, scale: Optional[float] = None,
-                              out: Optional[torch.Tensor] = None, num_splits: int = 0, workspace: Optional[torch.Tensor] = None,
-                              flags: int = 0) -> torch.Tensor:
+                              out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, flags: int = 0) -> torch.Tensor:
     """``paged_decode_attention`` over a cache in 8 bits (as ``rope_kv_append_q8`` writes it): ``q [B, Hq, D]`` (row stride free), a token per sequence, over the
     ``context_lens[b]`` tokens of its pages; 0 where there are none.  ``max_context_len``: the host's bound of the lengths (tokens
-    behind it may be left out).  ``num_splits``: parts of the keys (0: the library's choice).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
+    behind it may be left out).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
     torch's caching allocator.  ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
-    _need_cuda(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens)
+    _need_cuda(q)
     dev = q.get_device()
     shape, codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
     max_blocks, Hkv, bs, D = shape
     Hq, q_stride, out = _q8_attention(q, shape, out, dev)
     B, dt = block_tables.shape[0], _dtype_id(q)
     lens, _ = _q8_lens(context_lens, None, B, q.shape[0], dev)
-    need = decode_attention_q8_workspace(B, Hq, Hkv, D, bs, int(max_context_len), q.dtype, int(num_splits))
+    need = decode_attention_q8_workspace(B, Hq, Hkv, D, bs, int(max_context_len), q.dtype)
     ws, ws_bytes, _keep = _q8_workspace(need, workspace, q, dev)
-    with _timed(), _on(dev) as stream:
-        rc = _lib.load().b200_paged_decode_attn_q8(
-            out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, B, Hq, Hkv, D, bs, max_blocks, D ** -0.5 if scale is None else float(scale),
-            int(max_context_len), int(num_splits), ws, ws_bytes, codes, dt, int(flags), stream)
-    if rc != 0:
-        _lib.check(rc, "b200_paged_decode_attn_q8")
+    args = (out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, B, Hq, Hkv, D, bs, max_blocks, D ** -0.5 if scale is None else float(scale),
+            int(max_context_len), ws, ws_bytes, codes, dt, int(flags))
+    if ATTN_EVENTS is None:
+        _q8_launch(dev, "b200_paged_decode_attn_q8", args)
+    else:
+        with _timed():
+            _q8_launch(dev, "b200_paged_decode_attn_q8", args)
     return out
 
 
@@ -1051,7 +1064,7 @@ def paged_prompt_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     ``max_context_len``: the host's bounds of a sequence's rows and of its tokens (what is behind them may be left out).  ``workspace``: at least
     ``prompt_attention_q8_workspace`` bytes that no call running at the same time uses; None: from torch's caching allocator.
     ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
-    _need_cuda(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, row_starts)
+    _need_cuda(q)
     dev = q.get_device()
     shape, codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
     max_blocks, Hkv, bs, D = shape
@@ -1059,12 +1072,13 @@ def paged_prompt_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     B, n, dt = block_tables.shape[0], q.shape[0], _dtype_id(q)
     lens, starts = _q8_lens(context_lens, row_starts, B, n, dev)
     ws, ws_bytes, _keep = _q8_workspace(prompt_attention_q8_workspace(B, int(max_new), Hq, Hkv, D, bs, int(max_context_len), q.dtype), workspace, q, dev)
-    with _timed(), _on(dev) as stream:
-        rc = _lib.load().b200_paged_prompt_attn_q8(
-            out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, starts, B, n, int(max_new), Hq, Hkv, D, bs, max_blocks,
-            D ** -0.5 if scale is None else float(scale), int(max_context_len), ws, ws_bytes, codes, dt, int(flags), stream)
-    if rc != 0:
-        _lib.check(rc, "b200_paged_prompt_attn_q8")
+    args = (out.data_ptr(), q.data_ptr(), q_stride, *cache, lens, starts, B, n, int(max_new), Hq, Hkv, D, bs, max_blocks,
+            D ** -0.5 if scale is None else float(scale), int(max_context_len), ws, ws_bytes, codes, dt, int(flags))
+    if ATTN_EVENTS is None:
+        _q8_launch(dev, "b200_paged_prompt_attn_q8", args)
+    else:
+        with _timed():
+            _q8_launch(dev, "b200_paged_prompt_attn_q8", args)
     return out
 
 

@@ -385,7 +385,6 @@ int b200_kv_unpack_layers(void* const* k_pools, void* const* v_pools, int n_laye
  * b200_paged_prompt_attn_q8: the same for rows as above, each over the keys up to its own position.  No sequence has more than max_new rows or
  * max_context_len tokens (tokens behind may be left out).  fp32 scores, statistics and sums.  q rows q_stride elements apart, out contiguous.
  *   workspace : the *_workspace call's bytes (0: none needed), 16-byte aligned, any contents; calls that may run at the same time need their own.
- *   num_splits: parts that the keys are cut into; 0: the library's choice.
  *   flags     : B200_ATTN_FORCE_GENERIC: fp32 arithmetic, without tensor cores.
  */
 #define B200_CODES_INT8 3      /* the wire id of int8 */
@@ -397,11 +396,11 @@ int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int
 int b200_kv_gather_dense_q8(void* k_out, void* v_out, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                             const int32_t* block_tables, int table_stride, int table_cols, int B, int n_tokens, int Hkv, int D, int block_size,
                             int64_t max_blocks, int codes, int dtype, void* stream);
-size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int num_splits, int dtype);
+size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype);
 int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                               const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, int B, int Hq, int Hkv, int D,
-                              int block_size, int64_t max_blocks, float scale, int max_context_len, int num_splits, void* workspace, size_t workspace_bytes,
-                              int codes, int dtype, unsigned flags, void* stream);
+                              int block_size, int64_t max_blocks, float scale, int max_context_len, void* workspace, size_t workspace_bytes, int codes,
+                              int dtype, unsigned flags, void* stream);
 size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype);
 int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
                               const int32_t* block_tables, int table_stride, int table_cols, const int32_t* context_lens, const int32_t* row_starts, int B, int rows,

@@ -35,7 +35,7 @@ def test_argument_errors_have_codes_and_words():
         return lib.b200_paged_prompt_attn_q8(*a.values()), lib.b200_last_error().decode()
 
     def decode(**over):
-        a = dict(out=p, q=p, qs=512, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, lens=p, B=2, Hq=4, Hkv=2, D=128, bs=16, blocks=8, scale=1.0, longest=64, splits=0, ws=None,
+        a = dict(out=p, q=p, qs=512, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, lens=p, B=2, Hq=4, Hkv=2, D=128, bs=16, blocks=8, scale=1.0, longest=64, ws=None,
                  bytes=0, codes=3, dtype=2, flags=0, stream=None)
         a.update(over)
         return lib.b200_paged_decode_attn_q8(*a.values()), lib.b200_last_error().decode()
@@ -54,7 +54,7 @@ def test_argument_errors_have_codes_and_words():
     for call in (prompt, decode):
         assert call(Hq=5)[0] == -2 and call(longest=-1)[0] == -1 and call(D=512)[0] == -2 and call(out=None)[0] == -1
     assert prompt(rows=0)[0] == 0 and prompt(starts=None)[0] == -1 and prompt(most=-1)[0] == -1
-    assert decode(splits=-1)[0] == -1 and decode(splits=4)[0] == -3
+    assert decode(longest=4096, dtype=0)[0] == -3
     assert append(rows=0)[0] == 0 and append(starts=None)[0] == -1 and append(sin=None)[0] == -1 and append(cos=None, sin=None)[0] == -1
     assert append(D=33)[0] == -2 and append(q=None)[0] == -1 and append(B=2 ** 30, most=2 ** 30, rows=2 ** 30)[0] == -2
     assert gather(n=65)[0] == -1 and gather(n=0)[0] == 0

@@ -520,9 +520,12 @@ def test_refusals():
     write = lambda **over: ops.rope_kv_append_q8(**{**dict(  # noqa: E731
         q=w["q"], k=w["k"], v=w["v"], cos=w["cos"], sin=w["sin"], k_pool=k_pool, v_pool=v_pool, k_scale=k_scale, v_scale=v_scale, block_tables=c["tables"],
         context_lens=lens, row_starts=starts), **over})
-    for over in (dict(cos=None), dict(cos=None, sin=None), dict(row_starts=None), dict(k=w["k"][:5]), dict(cos=w["cos"][:, :64]), dict(v=w["v"].float()),
-                 dict(k=w["k"].transpose(1, 2)), dict(q_out=w["q"].float())):
+    for over in (dict(cos=None), dict(cos=None, sin=None), dict(row_starts=None), dict(k=w["k"][:5]), dict(cos=w["cos"][:, :64]), dict(v=w["v"][:, :1]),
+                 dict(k=w["k"].transpose(1, 2)), dict(q_out=w["q"][:, :4])):
         with pytest.raises(ValueError):
+            write(**over)
+    for over in (dict(v=w["v"].float()), dict(q_out=w["q"].float())):
+        with pytest.raises(TypeError):
             write(**over)
     with pytest.raises(TypeError):
         write(cos=w["cos"].float())
