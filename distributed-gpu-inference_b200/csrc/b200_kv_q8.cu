@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "b200_q8.cuh"
+#include "b200_tcgen05.cuh"
 
 namespace b200 {
 namespace {
@@ -97,60 +98,99 @@ __global__ void __launch_bounds__(128) append_any_kernel(const Append A) {
 
 // ---- 16-bit types, heads of 64 or 128, pages of 16, 32 or 64 -----------------------------------------------------------------------------------
 // A warp per 16 places of a page and kv head's keys or values; the W warps of a page share its maximum.  A lane has 8 columns of the lower and the
-// same 8 of the upper half of several rows, which turn into one another: everything is read once and held as fp32 until the scale is known.  Codes that the
-// page holds already are asked for together with its scale, whether or not it grows.  Behind these CTAs, a warp per row and 16 query heads.
+// same 8 of the upper half of several rows, which turn into one another: everything is read once and held as it came until the scale is known; turning it a second
+// time costs less than the registers of the numbers (136: 12 warps an SM, 8 x 2048 rows of 8 heads of 128 in 98 us with their 32 query heads).  Codes that the page holds
+// already are asked for together with its scale, whether or not it grows.  Behind these CTAs, a warp per row and 16 query heads.  Bound by memory.
 constexpr int kHeadsPerWarp = 16;
 
+// Eight numbers as four pairs, two products an instruction.  (Sums stay single: the assembler made one rounding of a pair's product and its sum with a constant,
+// whatever their instructions said.)
+using Eight = f32x2[4];
 template <typename T>
-__device__ __forceinline__ void eight(const int4& raw, float (&x)[8]) {
-  const T* e = reinterpret_cast<const T*>(&raw);
+__device__ __forceinline__ void eight(const int4& raw, Eight& x) {
+  const uint32_t w[4] = {static_cast<uint32_t>(raw.x), static_cast<uint32_t>(raw.y), static_cast<uint32_t>(raw.z), static_cast<uint32_t>(raw.w)};
 #pragma unroll
-  for (int u = 0; u < 8; ++u) x[u] = Cvt<T>::to_f32(e[u]);
+  for (int u = 0; u < 4; ++u) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      x[u] = pair(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[u]));
+      x[u] = pair(f.x, f.y);
+    }
+  }
 }
 template <typename T>
-__device__ __forceinline__ int4 eight_of(const float (&x)[8]) {
-  int4 raw;
-  T* e = reinterpret_cast<T*>(&raw);
+__device__ __forceinline__ int4 eight_of(const Eight& x) {
+  uint32_t w[4];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) e[u] = Cvt<T>::from_f32(x[u]);
-  return raw;
+  for (int u = 0; u < 4; ++u) {
+    float a, b;
+    apart(a, b, x[u]);
+    w[u] = pack2<T>(a, b);
+  }
+  return make_int4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ f32x2 sums(f32x2 x, f32x2 y) {
+  float a, b, c, d;
+  apart(a, b, x);
+  apart(c, d, y);
+  return pair(__fadd_rn(a, c), __fadd_rn(b, d));
+}
+__device__ __forceinline__ f32x2 differences(f32x2 x, f32x2 y) {
+  float a, b, c, d;
+  apart(a, b, x);
+  apart(c, d, y);
+  return pair(__fsub_rn(a, c), __fsub_rn(b, d));
 }
 // lo, hi: the same 8 columns of the two halves
 template <typename T>
-__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const int4& c_lo, const int4& c_hi, const int4& s_lo, const int4& s_hi) {
-  float cl[8], ch[8], sl[8], sh[8];
-  eight<T>(c_lo, cl);
-  eight<T>(c_hi, ch);
-  eight<T>(s_lo, sl);
-  eight<T>(s_hi, sh);
+__device__ __forceinline__ void turn(Eight& lo, Eight& hi, const int4 (&cs)[4]) {
+  Eight cl, ch, sl, sh;
+  eight<T>(cs[0], cl);
+  eight<T>(cs[1], ch);
+  eight<T>(cs[2], sl);
+  eight<T>(cs[3], sh);
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const float l = turned(lo[u], hi[u], cl[u], sl[u], false), h = turned(hi[u], lo[u], ch[u], sh[u], true);
+  for (int u = 0; u < 4; ++u) {
+    const f32x2 l = differences(mul2(lo[u], cl[u]), mul2(hi[u], sl[u])), h = sums(mul2(hi[u], ch[u]), mul2(lo[u], sh[u]));
     lo[u] = l, hi[u] = h;
   }
 }
+// the larger of `most` and two pairs' magnitudes, no number if one is none
+__device__ __forceinline__ float magnitude(float most, f32x2 x) {
+  float a, b;
+  apart(a, b, x);
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(most) : "f"(most), "f"(a), "f"(b));
+  return most;
+}
+// of 16 bits, in their type: a comparison rounds nothing
+template <typename T>
+__device__ __forceinline__ uint32_t magnitudes(uint32_t most, uint32_t two) {
+  two &= 0x7fff7fffu;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(most) : "r"(two));
+  else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(most) : "r"(two));
+  return most;
+}
 template <typename C>
-__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float inverse) {
-  uint2 r;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+__device__ __forceinline__ uint2 codes_of(const Eight& x, float inverse) {
+  uint32_t w[2];
+  const f32x2 by = both(inverse);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    float a, b, c, d;
     if constexpr (std::is_same_v<C, q8::Int8>) {
       // |x / s| <= 127 (1 + 2^-22): the sum's last 8 bits are the nearest whole number's
-      uint32_t b[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) b[u] = __float_as_uint(__fadd_rn(__fmul_rn(x[4 * i + u], inverse), 12582912.f));
-      w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+      apart(a, b, sums(mul2(x[2 * i], by), both(12582912.f)));
+      apart(c, d, sums(mul2(x[2 * i + 1], by), both(12582912.f)));
+      w[i] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
     } else {
-      w[i] = 0;
-#pragma unroll
-      for (int u = 0; u < 4; u += 2) {
-        const float a = __fmul_rn(x[4 * i + u], inverse), b = __fmul_rn(x[4 * i + u + 1], inverse);
-        w[i] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a == a ? a : 0.f, b == b ? b : 0.f), __NV_SATFINITE, __NV_E4M3)) << (8 * u);
-      }
+      apart(a, b, mul2(x[2 * i], by));
+      apart(c, d, mul2(x[2 * i + 1], by));
+      w[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
+             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16;
     }
   }
-  return r;
+  return make_uint2(w[0], w[1]);
 }
 template <typename C>
 __device__ __forceinline__ uint2 codes_again(uint2 old, float k) {
@@ -161,19 +201,19 @@ __device__ __forceinline__ uint2 codes_again(uint2 old, float k) {
 }
 
 template <typename T, typename C, int D, int W>
-__global__ void __launch_bounds__(128) append_kernel(const Append A, int unit_ctas) {
+__global__ void __launch_bounds__(128, 5) append_kernel(const Append A, int unit_ctas) {
   constexpr int kCh = D / 16, kRows = 32 / kCh, kPasses = 16 / kRows;        // pieces of a half; rows of a warp's pass
   __shared__ float most_s[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % kCh, r = lane / kCh;
   if (static_cast<int>(blockIdx.x) >= unit_ctas) {
-    const int groups = (A.Hq + kHeadsPerWarp - 1) / kHeadsPerWarp;
-    const int64_t unit = (blockIdx.x - unit_ctas) * 4ll + warp, row = unit / groups;
-    if (row >= A.r.n) return;
-    const int h0 = static_cast<int>(unit - row * groups) * kHeadsPerWarp + r;
+    const unsigned groups = (A.Hq + kHeadsPerWarp - 1) / kHeadsPerWarp;
+    const unsigned unit = (blockIdx.x - unit_ctas) * 4 + warp, at = unit / groups;        // (a division of 64 bits costs 500 clocks)
+    if (at >= static_cast<unsigned>(A.r.n)) return;
+    const int64_t row = at;
+    const int h0 = static_cast<int>(unit - at * groups) * kHeadsPerWarp + r;
     const T *q = static_cast<const T*>(A.q) + row * A.q_stride + 8 * c, *cs = static_cast<const T*>(A.cos_t) + row * D + 8 * c, *sn = static_cast<const T*>(A.sin_t) + row * D + 8 * c;
     T* out = static_cast<T*>(A.q_out) + row * A.out_stride + 8 * c;
-    const int4 c_lo = *reinterpret_cast<const int4*>(cs), c_hi = *reinterpret_cast<const int4*>(cs + D / 2), s_lo = *reinterpret_cast<const int4*>(sn),
-               s_hi = *reinterpret_cast<const int4*>(sn + D / 2);
+    const int4 angles[4] = {*reinterpret_cast<const int4*>(cs), *reinterpret_cast<const int4*>(cs + D / 2), *reinterpret_cast<const int4*>(sn), *reinterpret_cast<const int4*>(sn + D / 2)};
     constexpr int kSteps = kHeadsPerWarp / kRows;
     int4 raw[kSteps][2];
 #pragma unroll
@@ -188,65 +228,96 @@ __global__ void __launch_bounds__(128) append_kernel(const Append A, int unit_ct
     for (int i = 0; i < kSteps; ++i) {
       const int h = h0 + i * kRows;
       if (h >= A.Hq) continue;
-      float lo[8], hi[8];
+      Eight lo, hi;
       eight<T>(raw[i][0], lo);
       eight<T>(raw[i][1], hi);
-      turn<T>(lo, hi, c_lo, c_hi, s_lo, s_hi);
+      turn<T>(lo, hi, angles);
       *reinterpret_cast<int4*>(out + h * D) = eight_of<T>(lo);
       *reinterpret_cast<int4*>(out + h * D + D / 2) = eight_of<T>(hi);
     }
     return;
   }
   // ---- keys and values: unit = ((sequence, page), head, keys or values) -----------------------------------------------------------------------
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (4 / W) + warp / W;
+  const unsigned unit = blockIdx.x * (4 / W) + warp / W, two = unit >> 1, bp = two / A.c.Hkv;
   const bool values = unit & 1;
-  const int h = static_cast<int>((unit >> 1) % A.c.Hkv), bp = static_cast<int>((unit >> 1) / A.c.Hkv), b = bp / A.pages, lp = bp - b * A.pages;
-  int t0 = 0, t1 = 0, at = 0, first = 0, held = 0, page = -1;
+  const int h = static_cast<int>(two - bp * A.c.Hkv), b = static_cast<int>(bp / A.pages), lp = static_cast<int>(bp - b * A.pages);
+  int t0 = 0, t1 = 0, at = 0, first = 0, held = 0;
   if (b < A.r.B) {
     int count, context;
     A.r.of(b, &first, &count, &context);
     held = context - count, at = held / A.c.bs + lp;
     const int64_t base = static_cast<int64_t>(at) * A.c.bs;
     t0 = static_cast<int>(max(held - base, static_cast<int64_t>(0))), t1 = static_cast<int>(min(context - base, static_cast<int64_t>(A.c.bs)));      // places of the page
-    if (t0 < t1) page = A.c.page(b, at);
   }
+  if (W == 1 && t0 >= t1) return;
+  const int my = warp % W * 16 + r;       // the place of the lane's row in the first pass
+  int4 raw[kPasses][2];       // 8 columns of each half; of earlier tokens their codes, both halves' in the first
+  const int64_t stride = values ? A.v_stride : A.k_stride, row = static_cast<int64_t>(first) + static_cast<int64_t>(at) * A.c.bs - held + my;       // of the first pass
+  const T* rows = static_cast<const T*>(values ? A.v : A.k) + row * stride + h * D + 8 * c;
+  const bool turns = !values && A.cos_t;
+  // asked for before the page is known
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int t = my + i * kRows;
+    raw[i][0] = raw[i][1] = make_int4(0, 0, 0, 0);
+    if (t >= t0 && t < t1) {
+      raw[i][0] = ld_stream16(rows);
+      raw[i][1] = ld_stream16(rows + D / 2);
+    }
+    rows += kRows * stride;
+  }
+  int4 cs[2][4];       // of a pass, and of the next one
+  const T *cos_at = static_cast<const T*>(A.cos_t) + row * D + 8 * c, *sin_at = static_cast<const T*>(A.sin_t) + row * D + 8 * c;
+  auto angles = [&](int i) {
+    const int t = my + i * kRows;
+    if (!(turns && t >= t0 && t < t1)) return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) cs[i & 1][u] = *reinterpret_cast<const int4*>((u < 2 ? cos_at : sin_at) + i * kRows * D + u % 2 * (D / 2));
+  };
+  auto numbers = [&](int i, Eight& lo, Eight& hi) {
+    eight<T>(raw[i][0], lo);
+    eight<T>(raw[i][1], hi);
+    if (turns) turn<T>(lo, hi, cs[i & 1]);
+  };
+  angles(0);
+  const int page = t0 < t1 ? A.c.page(b, at) : -1;
   if (W == 1 && page < 0) return;
   const int64_t place = static_cast<int64_t>(max(page, 0)) * A.c.Hkv + h;
   uint8_t* codes = (values ? A.c.v_pool : A.c.k_pool) + place * A.c.bs * D;
   float* scale = (values ? A.c.v_scale : A.c.k_scale) + place;
   const bool earlier = page >= 0 && t0 > 0;
   float had = earlier ? *scale : 0.f;
-  const int my = warp % W * 16 + r;       // the place of the lane's row in the first pass
-  uint2 old[kPasses][2];
-  int4 raw[kPasses][2];
-  const T* rows = static_cast<const T*>(values ? A.v : A.k) + h * D + 8 * c;
-  const int64_t stride = values ? A.v_stride : A.k_stride, row0 = static_cast<int64_t>(first) + static_cast<int64_t>(at) * A.c.bs - held;       // the row of the page's first place
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int t = my + i * kRows;
-    if (page >= 0 && t >= t0 && t < t1) {
-      raw[i][0] = ld_stream16(rows + (row0 + t) * stride);
-      raw[i][1] = ld_stream16(rows + (row0 + t) * stride + D / 2);
-    }
     if (earlier && t < t0) {
-      old[i][0] = *reinterpret_cast<const uint2*>(codes + t * D + 8 * c);
-      old[i][1] = *reinterpret_cast<const uint2*>(codes + t * D + D / 2 + 8 * c);
+      const uint2 lo = *reinterpret_cast<const uint2*>(codes + t * D + 8 * c), hi = *reinterpret_cast<const uint2*>(codes + t * D + D / 2 + 8 * c);
+      raw[i][0] = make_int4(lo.x, lo.y, hi.x, hi.y);
     }
   }
-  float x[kPasses][2][8], most = 0.f;
+  float most = 0.f;
+  if (turns) {
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int t = my + i * kRows;
-    if (!(page >= 0 && t >= t0 && t < t1)) continue;
-    eight<T>(raw[i][0], x[i][0]);
-    eight<T>(raw[i][1], x[i][1]);
-    if (!values && A.cos_t) {
-      const T *cs = static_cast<const T*>(A.cos_t) + (row0 + t) * D + 8 * c, *sn = static_cast<const T*>(A.sin_t) + (row0 + t) * D + 8 * c;
-      turn<T>(x[i][0], x[i][1], *reinterpret_cast<const int4*>(cs), *reinterpret_cast<const int4*>(cs + D / 2), *reinterpret_cast<const int4*>(sn),
-              *reinterpret_cast<const int4*>(sn + D / 2));
+    for (int i = 0; i < kPasses; ++i) {
+      angles(i + 1 < kPasses ? i + 1 : 0);       // (behind the last the first again: for the codes)
+      const int t = my + i * kRows;
+      if (!(t >= t0 && t < t1)) continue;
+      Eight lo, hi;
+      numbers(i, lo, hi);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) most = magnitude(magnitude(most, lo[u]), hi[u]);
     }
+  } else {
+    uint32_t two = 0;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) most = q8::max_nan(most, q8::max_nan(fabsf(x[i][0][u]), fabsf(x[i][1][u])));
+    for (int i = 0; i < kPasses; ++i) {
+      const int t = my + i * kRows;
+      if (!(t >= t0 && t < t1)) continue;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) two = magnitudes<T>(magnitudes<T>(magnitudes<T>(magnitudes<T>(two, raw[i][u].x), raw[i][u].y), raw[i][u].z), raw[i][u].w);
+    }
+    const T* e = reinterpret_cast<const T*>(&two);
+    most = q8::max_nan(Cvt<T>::to_f32(e[0]), Cvt<T>::to_f32(e[1]));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -261,16 +332,21 @@ __global__ void __launch_bounds__(128) append_kernel(const Append A, int unit_ct
   const bool grew = now != had;
   if (grew && warp % W == 0 && lane == 0) *scale = now;       // (the other warps have read what it was: before the barrier)
   const float k = __fmul_rn(had, inverse);
+  const bool finite = now < INFINITY;       // else codes are 0
+  codes += my * D + 8 * c;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
+    if (i + 1 < kPasses) angles(i + 1);
     const int t = my + i * kRows;
-    uint2* to = reinterpret_cast<uint2*>(codes + t * D + 8 * c);
+    uint2* to = reinterpret_cast<uint2*>(codes + i * kRows * D);
     if (t >= t0 && t < t1) {
-      to[0] = codes_of<C>(x[i][0], inverse);
-      to[D / 16] = codes_of<C>(x[i][1], inverse);
+      Eight lo, hi;
+      numbers(i, lo, hi);
+      to[0] = finite ? codes_of<C>(lo, inverse) : make_uint2(0u, 0u);
+      to[D / 16] = finite ? codes_of<C>(hi, inverse) : make_uint2(0u, 0u);
     } else if (earlier && t < t0 && grew) {
-      to[0] = codes_again<C>(old[i][0], k);
-      to[D / 16] = codes_again<C>(old[i][1], k);
+      to[0] = codes_again<C>(make_uint2(raw[i][0].x, raw[i][0].y), k);
+      to[D / 16] = codes_again<C>(make_uint2(raw[i][0].z, raw[i][0].w), k);
     }
   }
 }
@@ -327,13 +403,13 @@ __device__ __forceinline__ uint2 ld_stream8(const void* p) {
 }
 
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(256) gather_kernel(const Gather G, int tiles, int64_t units) {
+__global__ void __launch_bounds__(256) gather_kernel(const Gather G, unsigned tiles, unsigned units) {
   constexpr int kSteps = 16 * D / 256;
   const int lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit >= units) return;
-  const int64_t bh = unit / tiles;
-  const int tile = static_cast<int>(unit - bh * tiles), h = static_cast<int>(bh % G.c.Hkv), b = static_cast<int>(bh / G.c.Hkv), at = tile * 16 / G.c.bs;
+  const unsigned bh = unit / tiles;
+  const int tile = static_cast<int>(unit - bh * tiles), b = static_cast<int>(bh / G.c.Hkv), h = static_cast<int>(bh - b * G.c.Hkv), at = tile * 16 / G.c.bs;
   const int page = G.c.page(b, at);
   const int64_t place = static_cast<int64_t>(max(page, 0)) * G.c.Hkv + h, from = (place * G.c.bs + (tile * 16 - at * G.c.bs)) * D + lane * 8;
   const float ks = page >= 0 ? G.c.k_scale[place] : 0.f, vs = page >= 0 ? G.c.v_scale[place] : 0.f;
@@ -342,7 +418,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Gather G, int tiles, 
   for (int i = 0; i < kSteps; ++i) k[i] = page >= 0 ? ld_stream8(G.c.k_pool + from + i * 256) : make_uint2(0u, 0u);
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) v[i] = page >= 0 ? ld_stream8(G.c.v_pool + from + i * 256) : make_uint2(0u, 0u);
-  const int64_t to = (bh * G.n + tile * 16) * D + lane * 8;
+  const int64_t to = (static_cast<int64_t>(bh) * G.n + tile * 16) * D + lane * 8;
   const int live = min(16, G.n - tile * 16) * D;        // elements
 #pragma unroll
   for (int i = 0; i < 2 * kSteps; ++i) {
@@ -355,7 +431,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Gather G, int tiles, 
       *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
       *reinterpret_cast<float4*>(out + 4) = make_float4(x[4], x[5], x[6], x[7]);
     } else {
-      *reinterpret_cast<int4*>(out) = eight_of<T>(x);
+      *reinterpret_cast<int4*>(out) = make_int4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
     }
   }
 }
@@ -398,7 +474,7 @@ int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int
   A.pages = longest == 0 ? 0 : longest == 1 ? 1 : static_cast<int>((longest - 2ll + block_size) / block_size) + 1;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t units = static_cast<int64_t>(B) * A.pages * Hkv * 2, grid = units + (q_out ? rows : 0);
-  if (grid > INT32_MAX) return fail(B200_ESHAPE, "%s: %d sequences of up to %d pages", name, B, A.pages);
+  if (grid * 4 > INT32_MAX) return fail(B200_ESHAPE, "%s: %d sequences of up to %d pages", name, B, A.pages);
   if (grid == 0) return 0;
   const int warps = block_size / 16;
   const bool pieces = aligned16(k) && aligned16(v) && aligned16(cos_table) && aligned16(sin_table) && aligned16(k_pool) && aligned16(v_pool) && k_stride % 8 == 0 &&
@@ -438,13 +514,13 @@ int b200_kv_gather_dense_q8(void* k_out, void* v_out, const void* k_pool, const 
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int tiles = static_cast<int>((n_tokens + 15ll) / 16);
   const int64_t blocks = (static_cast<int64_t>(B) * Hkv * n_tokens * D + 255) / 256, units = static_cast<int64_t>(B) * Hkv * tiles;
-  const bool fast = (D == 64 || D == 128) && block_size % 16 == 0 && aligned16(k_out) && aligned16(v_out) && aligned16(k_pool) && aligned16(v_pool) && units < INT32_MAX;
+  const bool fast = (D == 64 || D == 128) && block_size % 16 == 0 && aligned16(k_out) && aligned16(v_out) && aligned16(k_pool) && aligned16(v_pool) && units < INT32_MAX - 8;
   return with_types(dtype, codes, [&](auto* t, auto* c) {
     using T = std::remove_pointer_t<decltype(t)>;
     using C = std::remove_pointer_t<decltype(c)>;
     if (fast) {
       auto kern = D == 128 ? gather_kernel<T, C, 128> : gather_kernel<T, C, 64>;
-      kern<<<static_cast<unsigned>((units + 7) / 8), 256, 0, s>>>(G, tiles, units);
+      kern<<<static_cast<unsigned>((units + 7) / 8), 256, 0, s>>>(G, static_cast<unsigned>(tiles), static_cast<unsigned>(units));
       return check_launch(name);
     }
     gather_any_kernel<T, C><<<static_cast<unsigned>(blocks < kNumSMs * 8 ? blocks : kNumSMs * 8), 256, 0, s>>>(G);
