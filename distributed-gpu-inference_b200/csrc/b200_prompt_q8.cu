@@ -321,60 +321,66 @@ prompt_kernel(const PromptAttn A) {
       tm_ld32(*reinterpret_cast<float(*)[32]>(s + 32), tm_row + (i & 1) * kKeys + 32);
       tc_wait_ld();
       const int left = see - (w.t0 + i) * kKeys;       // keys of the tile that the row sees
-      const bool masked = see_all < (w.t0 + i + 1) * kKeys;       // (the warp)
-      if (masked) {
+      auto weigh = [&](auto masked) {        // some rows of the warp do not see all of the tile: whatever the scales of a page that a row does not see
+        constexpr bool kMasked = decltype(masked)::value;
+        if constexpr (kMasked) {
 #pragma unroll
-        for (int x = 0; x < kKeys; ++x)
-          if (x >= left) s[x] = -INFINITY;
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const float* e = s + g * kGroup;
-        float a = max3(e[0], e[1], e[2]), b = max3(e[3], e[4], e[5]);
-        a = max3(a, e[6], e[7]), b = max3(b, e[8], e[9]);
-        a = max3(a, e[10], e[11]), b = max3(b, e[12], e[13]);
-        a = max3(a, e[14], e[15]);
-        top = fmaxf(top, fmaf(fmaxf(a, b), kg[g], ls[g]));
-      }
-      const bool grow = top > m + 14.f;
-      float corr = 1.f;
-      if (grow) {
-        const float now = top - 6.f;
-        corr = m == -INFINITY ? 0.f : exp2_fast(m - now);
-        m = now;
-      }
-      if (i > 0 && __any_sync(0xffffffffu, grow)) {
-        ok = bar_wait(bar_o(rb, i - 1), ((i - 1) >> 1) & 1, dead) && ok;
-        tc_fence_after();
-        scale_rows<D, 16>(tm_row + P::kO, corr);
-      }
-      l *= corr;
-      const float from = m == -INFINITY ? 0.f : m;       // a row that sees no key yet: weights 0
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const f32x2 kk = both(kg[g]), mm = both(ls[g] - from);
-        f32x2 sum = 0ull;
-        uint32_t p[8];
-#pragma unroll
-        for (int x = 0; x < kGroup; x += 2) {
-          float a = s[g * kGroup + x], b = s[g * kGroup + x + 1];
-          scale_shift(a, b, kk, mm);
-          a = exp2_fast(a), b = exp2_fast(b);
-          if (masked) {       // whatever the scales of a page that the row does not see
-            if (g * kGroup + x >= left) a = 0.f;
-            if (g * kGroup + x + 1 >= left) b = 0.f;
-          }
-          sum = add2(sum, pair(a, b));
-          p[x >> 1] = pack2<__half>(a, b);
+          for (int x = 0; x < kKeys; ++x)
+            if (x >= left) s[x] = -INFINITY;
         }
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(tm_row + (i & 1) * kKeys + 8 * g), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]),
-                     "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
-                     : "memory");
-        float a, b;
-        apart(a, b, sum);
-        if (!masked || g * kGroup < left) l = fmaf(a + b, per[g], l);
-      }
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const float* e = s + g * kGroup;
+          float a = max3(e[0], e[1], e[2]), b = max3(e[3], e[4], e[5]);
+          a = max3(a, e[6], e[7]), b = max3(b, e[8], e[9]);
+          a = max3(a, e[10], e[11]), b = max3(b, e[12], e[13]);
+          a = max3(a, e[14], e[15]);
+          top = fmaxf(top, fmaf(fmaxf(a, b), kg[g], ls[g]));
+        }
+        const bool grow = top > m + 14.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          float corr = 1.f;
+          if (grow) {
+            const float now = top - 6.f;
+            corr = m == -INFINITY ? 0.f : exp2_fast(m - now);
+            m = now;
+          }
+          if (i > 0) {
+            ok = bar_wait(bar_o(rb, i - 1), ((i - 1) >> 1) & 1, dead) && ok;
+            tc_fence_after();
+            scale_rows<D, 16>(tm_row + P::kO, corr);
+          }
+          l *= corr;
+        }
+        const float from = m == -INFINITY ? 0.f : m;       // a row that sees no key yet: weights 0
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const f32x2 kk = both(kg[g]), mm = both(ls[g] - from);
+          f32x2 sum = 0ull;
+          uint32_t p[8];
+#pragma unroll
+          for (int x = 0; x < kGroup; x += 2) {
+            float a = s[g * kGroup + x], b = s[g * kGroup + x + 1];
+            scale_shift(a, b, kk, mm);
+            a = exp2_fast(a), b = exp2_fast(b);
+            if constexpr (kMasked) {
+              if (g * kGroup + x >= left) a = 0.f;
+              if (g * kGroup + x + 1 >= left) b = 0.f;
+            }
+            sum = add2(sum, pair(a, b));
+            p[x >> 1] = pack2<__half>(a, b);
+          }
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(tm_row + (i & 1) * kKeys + 8 * g), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]),
+                       "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
+                       : "memory");
+          float a, b;
+          apart(a, b, sum);
+          if (!kMasked || g * kGroup < left) l = fmaf(a + b, per[g], l);
+        }
+      };
+      if (see_all < (w.t0 + i + 1) * kKeys) weigh(std::true_type{});
+      else weigh(std::false_type{});
       tc_wait_st();
       tc_fence_before();
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_p(rb, i)) : "memory");
