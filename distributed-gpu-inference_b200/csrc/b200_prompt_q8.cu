@@ -2,13 +2,15 @@
 // 128, pages of 16s.  Formula: b200_attn_q8.cu.
 //
 // The rows of a sequence and kv head - its new tokens times the G query heads of the group, token by token - go in blocks of 128; a CTA has RB of them and
-// walks the keys up to its last row's in tiles of 64.
+// walks the keys up to its last row's in tiles: of 128 for two blocks, of 64 for one.
 //
-//   codes -> fp16   four warps, 16 codes of a key a thread and step: loaded a tile ahead, turned (exact) and stored in 128-byte swizzled lines, once for all RB x 128 rows
-//   S = Q K^T       tcgen05.mma, 128 x 64, both operands in shared memory, S in tensor memory, two of them; queries in fp16 by a power of two of their own, the
-//                   largest of a row between 2^14 and 2^15
+//   codes -> fp16   four warps, 16 codes of a key a thread and step: asked for while the tile ahead is turned, turned (exact) and stored in 128-byte swizzled lines, once for all
+//                   RB x 128 rows
+//   S = Q K^T       tcgen05.mma, 128 rows x the tile, both operands in shared memory, S in tensor memory; queries in fp16 by a power of two of their own, the largest
+//                   of a row between 2^14 and 2^15.  (64 keys at a time read 6 KB of shared memory in the 32 clocks of 4 KB: the tile of 128.)
 //   w               a warp per 32 rows, thread = row: w = 2^(S t + log2 s - m) with the page's scales t and s, so that weights meet bare codes; the sum counts w / s; rounded to
-//                   fp16 (the largest weight between 2^6 and 2^14: the reference m moves late) into the tensor memory S was in
+//                   fp16 into the tensor memory S was in.  One pass: m is the maximum so far less 6, the weights of a tile are made with it while the tile's own maximum is
+//                   found, and made again where that lies more than 15 above m (the first tile's is looked for first); the largest weight lies between 2^6 and 2^15
 //   O += w V        tcgen05.mma, w from tensor memory, O in tensor memory in fp32
 //
 // Few rows: the keys are divided among `splits` CTAs, whose parts prompt_merge_kernel puts together in their order.
@@ -25,19 +27,21 @@ namespace {
 using q8::Cache;
 using q8::PromptAttn;
 
-constexpr int kRows = 128, kKeys = 64, kBlk = kKeys * 128, kGroup = 16, kGroups = kKeys / kGroup;
+constexpr int kRows = 128, kGroup = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int RB>
 struct Plan {
-  static constexpr int kBufs = RB == 1 ? 2 : 3;       // of keys, and of values
+  static constexpr int kKeys = 64, kS = 2, kBufs = RB == 1 ? 2 : 3;       // keys of a tile; S in tensor memory for a row block; buffers of keys, and of values
+  static constexpr int kGroups = kKeys / kGroup, kBlk = kKeys * 128;
   static constexpr int kSoft = 128 * RB, kConvert = 128, kThreads = kSoft + kConvert + 32;
   static constexpr int kQBlock = (D / 64) * kRows * 128, kTile = (D / 64) * kBlk;       // bytes
   static constexpr int kQ = 0, kK = kQ + RB * kQBlock, kV = kK + kBufs * kTile, kScales = kV + kBufs * kTile;       // scales: [warp][3][32] numbers
   static constexpr int kFactor = kScales + 4 * RB * 3 * 32 * 4, kBar = kFactor + RB * kRows * 4, kFlags = kBar + 8 * (4 * kBufs + RB * 7), kEnd = kFlags + 16;
   static constexpr int kSmem = kEnd + 1024;
-  static constexpr int kO = 2 * kKeys, kTm = 256;      // columns of a row block's tensor memory: S0 | S1 | O
+  static constexpr int kO = kS * kKeys, kTm = 256;      // columns of a row block's tensor memory: S (one or two) | O
   static_assert(RB == 2 ? kSmem <= kMaxSmem : 2 * (kSmem + 1024) <= 228 * 1024, "shared memory");
+  static_assert(kO + D <= kTm, "tensor memory");
 };
 
 __device__ __forceinline__ uint32_t line(uint32_t base, int r, int ch, int rows) {     // 16-byte piece ch of row r: blocks of 64 columns, swizzled lines
@@ -56,8 +60,13 @@ struct Work {
   __device__ __forceinline__ int64_t part(const PromptAttn& A, int row) const {
     return ((static_cast<int64_t>(b) * A.c.Hkv + kvh) * A.max_rows + row) * A.splits + split;
   }
+  // tiles up to those of the `count` rows from `from` on
+  template <int KEYS>
+  __device__ __forceinline__ int tiles(const PromptAttn& A, int from, int count) const {
+    return from < rows ? (min(base + min(n, (from + count - 1) / A.G + 1), room) + KEYS - 1) / KEYS : 0;
+  }
 };
-template <int RB>
+template <int RB, int KEYS>
 __device__ __forceinline__ Work work_of(const PromptAttn& A, int unit) {
   Work w;
   w.split = unit % A.splits;
@@ -70,9 +79,8 @@ __device__ __forceinline__ Work work_of(const PromptAttn& A, int unit) {
   A.r.of(w.b, &w.first, &w.n, &context);
   w.base = context - w.n;
   w.room = A.c.keys(context);
-  const int last = min(w.n, (w.row0 + kRows * RB - 1) / A.G + 1);       // tokens up to the block's last
   w.rows = min(w.n * A.G, A.max_rows);
-  const int tiles = w.row0 < w.rows ? (min(w.base + last, w.room) + kKeys - 1) / kKeys : 0, per = (tiles + A.splits - 1) / A.splits;
+  const int tiles = w.tiles<KEYS>(A, w.row0, kRows * RB), per = (tiles + A.splits - 1) / A.splits;
   w.t0 = min(w.split * per, tiles);
   w.t1 = min(w.t0 + per, tiles);
   return w;
@@ -82,7 +90,7 @@ template <typename T, typename C, int D, int RB>
 __global__ void __launch_bounds__(Plan<D, RB>::kThreads, 3 - RB)
 prompt_kernel(const PromptAttn A) {
   using P = Plan<D, RB>;
-  constexpr int NB = P::kBufs;
+  constexpr int NB = P::kBufs, kKeys = P::kKeys, kGroups = P::kGroups, kBlk = P::kBlk;
   extern __shared__ unsigned char raw_smem[];
   unsigned char* sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
   const uint32_t sm0 = smem_u32(sm);
@@ -99,7 +107,7 @@ prompt_kernel(const PromptAttn A) {
   const int G = A.G;
 
   asm volatile("griddepcontrol.launch_dependents;");
-  const Work w = work_of<RB>(A, blockIdx.x);
+  const Work w = work_of<RB, kKeys>(A, blockIdx.x);
   const int run = w.t1 - w.t0, rows = w.rows;
   if (w.row0 >= rows) return;       // (the whole CTA)
   if (run == 0) {                   // no keys: nothing but the statistics that say so
@@ -151,19 +159,13 @@ prompt_kernel(const PromptAttn A) {
     };
     const int g0 = w.t0 * kGroups;
     int at = look_up(g0 + lane), later = look_up(g0 + 32 + lane);
-    int4 k[2][kPasses], v[2][kPasses];
-    auto load = [&](int i, int4 (&kk)[kPasses], int4 (&vv)[kPasses]) {
-      if (i > 0 && i % (32 / kGroups) == 0) {
-        at = later;
-        later = look_up(g0 + i * kGroups + 32 + lane);
-      }
+    int4 k[kPasses], v[kPasses];
+    auto load = [&](int i, const uint8_t* pool, int4 (&x)[kPasses]) {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int key = p * kStep + r, row = __shfl_sync(0xffffffffu, at, (i * kGroups + key / kGroup) & 31);
-        const int64_t e = (static_cast<int64_t>(row) + key % kGroup) * D + ch * 16;
         const bool in = row >= 0 && (w.t0 + i) * kKeys + key < keys;
-        kk[p] = in ? ld_stream16(c.k_pool + e) : make_int4(0, 0, 0, 0);
-        vv[p] = in ? ld_stream16(c.v_pool + e) : make_int4(0, 0, 0, 0);
+        x[p] = in ? ld_stream16(pool + (static_cast<int64_t>(row) + key % kGroup) * D + ch * 16) : make_int4(0, 0, 0, 0);
       }
     };
     auto store = [&](uint32_t to, const int4 (&x)[kPasses]) {
@@ -183,26 +185,31 @@ prompt_kernel(const PromptAttn A) {
       }
       fence_smem_to_mma();
     };
-    auto tile = [&](int i, const int4 (&kk)[kPasses], const int4 (&vv)[kPasses]) {
+    load(0, c.k_pool, k);
+    for (int i = 0; i < run; ++i) {
       const int buf = i % NB;
+      load(i, c.v_pool, v);
       if (i >= NB) bar_wait(bar_ke + 8 * buf, (i / NB - 1) & 1, dead);
-      store(sm0 + P::kK + buf * P::kTile, kk);
+      store(sm0 + P::kK + buf * P::kTile, k);
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_k + 8 * buf) : "memory");
+      if ((i + 1) % (32 / kGroups) == 0) {
+        at = later;
+        later = look_up(g0 + (i + 1) * kGroups + 32 + lane);
+      }
+      if (i + 1 < run) load(i + 1, c.k_pool, k);
       if (i >= NB) bar_wait(bar_ve + 8 * buf, (i / NB - 1) & 1, dead);
-      store(sm0 + P::kV + buf * P::kTile, vv);
+      store(sm0 + P::kV + buf * P::kTile, v);
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_v + 8 * buf) : "memory");
-    };
-    load(0, k[0], v[0]);
-    for (int i = 0; i < run; i += 2) {
-      if (i + 1 < run) load(i + 1, k[1], v[1]);
-      tile(i, k[0], v[0]);
-      if (i + 2 < run) load(i + 2, k[0], v[0]);
-      if (i + 1 < run) tile(i + 1, k[1], v[1]);
     }
   } else if (warp == P::kThreads / 32 - 1) {
     // ---- products ----------------------------------------------------------------------------------------------------------------------------
+    int runs[RB];        // tiles of a row block: a part of the CTA's first ones
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) runs[rb] = max(min(w.tiles<kKeys>(A, w.row0 + rb * kRows, kRows), w.t1) - w.t0, 0);
     auto scores = [&](int i, int rb) {
-      const uint32_t kk = sm0 + P::kK + (i % NB) * P::kTile, q = sm0 + P::kQ + rb * P::kQBlock, to = tm + rb * P::kTm + (i & 1) * kKeys;
+      const uint32_t kk = sm0 + P::kK + (i % NB) * P::kTile, q = sm0 + P::kQ + rb * P::kQBlock, to = tm + rb * P::kTm + (i % P::kS) * kKeys;
+      if (i >= P::kS) bar_wait(bar_o(rb, i - P::kS), ((i - P::kS) >> 1) & 1, dead);        // S goes where the weights of an earlier tile were read
+      tc_fence_after();
 #pragma unroll
       for (int u = 0; u < D / 16; ++u)
         mma_ss(to, operand(q + (u >> 2) * (kRows * 128) + (u & 3) * 32, 16, 1024), operand(kk + (u >> 2) * kBlk + (u & 3) * 32, 16, 1024), instr<__half>(kKeys, false), u > 0);
@@ -210,42 +217,46 @@ prompt_kernel(const PromptAttn A) {
     };
     auto outputs = [&](int i, int rb) {
       const uint32_t v = sm0 + P::kV + (i % NB) * P::kTile, from = tm + rb * P::kTm;
+      bar_wait(bar_p(rb, i), (i >> 1) & 1, dead);
+      tc_fence_after();
 #pragma unroll
       for (int u = 0; u < kKeys / 16; ++u)
-        mma_ts(from + P::kO, from + (i & 1) * kKeys + 8 * u, operand(v + u * 2048, kBlk, 1024), instr<__half>(D, true), i > 0 || u > 0);
+        mma_ts(from + P::kO, from + (i % P::kS) * kKeys + 8 * u, operand(v + u * 2048, kBlk, 1024), instr<__half>(D, true), i > 0 || u > 0);
       mma_commit(bar_o(rb, i));
     };
     bar_wait(bar_k, 0, dead);
+#pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
+      if (runs[rb] == 0) continue;
       bar_wait(bar_q(rb), 0, dead);
-      tc_fence_after();
       scores(0, rb);
     }
     mma_commit(bar_ke);
     for (int i = 0; i < run; ++i) {
-      if (i + 1 < run) {
-        bar_wait(bar_k + 8 * ((i + 1) % NB), ((i + 1) / NB) & 1, dead);
+      const bool more = i + 1 < run;
+      if (more) bar_wait(bar_k + 8 * ((i + 1) % NB), ((i + 1) / NB) & 1, dead);
+      if constexpr (P::kS == 2) {
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          if (i > 0) bar_wait(bar_o(rb, i - 1), ((i - 1) >> 1) & 1, dead);        // S of the next tile goes where the weights of the one before were read
-          tc_fence_after();
-          scores(i + 1, rb);
-        }
-        mma_commit(bar_ke + 8 * ((i + 1) % NB));
+        for (int rb = 0; rb < RB; ++rb)
+          if (i + 1 < runs[rb]) scores(i + 1, rb);
+        if (more) mma_commit(bar_ke + 8 * ((i + 1) % NB));
       }
       bar_wait(bar_v + 8 * (i % NB), (i / NB) & 1, dead);
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        bar_wait(bar_p(rb, i), (i >> 1) & 1, dead);
-        tc_fence_after();
-        outputs(i, rb);
+        if (i < runs[rb]) outputs(i, rb);
+        if constexpr (P::kS == 1) {        // while one block's weights are made, the other's products run
+          if (i + 1 < runs[rb]) scores(i + 1, rb);
+        }
       }
       mma_commit(bar_ve + 8 * (i % NB));
+      if (P::kS == 1 && more) mma_commit(bar_ke + 8 * ((i + 1) % NB));
     }
     __syncwarp();
   } else {
     // ---- weights: thread = row ---------------------------------------------------------------------------------------------------------------
     const int rb = warp >> 2, in_block = tid & 127, row = w.row0 + tid;
+    const int my_run = max(min(w.tiles<kKeys>(A, w.row0 + rb * kRows, kRows), w.t1) - w.t0, 0);
     const uint32_t q_at = sm0 + P::kQ + rb * P::kQBlock, tm_row = tm + rb * P::kTm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     float* factor = reinterpret_cast<float*>(sm + P::kFactor);
     const float sign = A.scale < 0.f ? -1.f : 1.f;
@@ -300,7 +311,7 @@ prompt_kernel(const PromptAttn A) {
     page = page_of(g0 + 32 + lane);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int i = 0; i < run; ++i) {
+    for (int i = 0; i < my_run; ++i) {
       const int in = i % (32 / kGroups);
       if (in == 0) {
         __syncwarp();
@@ -310,36 +321,66 @@ prompt_kernel(const PromptAttn A) {
         scales_of(page, ks, vs);
         page = page_of(g0 + i * kGroups + 64 + lane);
       }
-      const float4 kt = *reinterpret_cast<const float4*>(scales + in * kGroups), lv = *reinterpret_cast<const float4*>(scales + 32 + in * kGroups),
-                   iv = *reinterpret_cast<const float4*>(scales + 64 + in * kGroups);
-      const float kg[4] = {q8::max_nan(f * kt.x, 1e-30f), q8::max_nan(f * kt.y, 1e-30f), q8::max_nan(f * kt.z, 1e-30f), q8::max_nan(f * kt.w, 1e-30f)};
-      const float ls[4] = {lv.x, lv.y, lv.z, lv.w}, per[4] = {iv.x, iv.y, iv.z, iv.w};
       ok = bar_wait(bar_s(rb, i), (i >> 1) & 1, dead) && ok;
       tc_fence_after();
-      float s[kKeys];
-      tm_ld32(*reinterpret_cast<float(*)[32]>(s), tm_row + (i & 1) * kKeys);
-      tm_ld32(*reinterpret_cast<float(*)[32]>(s + 32), tm_row + (i & 1) * kKeys + 32);
-      tc_wait_ld();
+      const uint32_t s_at = tm_row + (i % P::kS) * kKeys;
       const int left = see - (w.t0 + i) * kKeys;       // keys of the tile that the row sees
-      auto weigh = [&](auto masked) {        // some rows of the warp do not see all of the tile: whatever the scales of a page that a row does not see
-        constexpr bool kMasked = decltype(masked)::value;
-        if constexpr (kMasked) {
+      uint32_t p[kKeys / 2];
+      float top, sum;
+      // 32 keys at a time: their maximum, and (kWeigh) their weights.  kMasked: some rows of the warp do not see all of the tile, whatever the scales of a page that
+      // they do not see
+      auto pass = [&](auto masked, auto weigh) {
+        constexpr bool kMasked = decltype(masked)::value, kWeigh = decltype(weigh)::value;
+        const float from = m == -INFINITY ? 0.f : m;       // a row that sees no key yet: weights 0
+        top = -INFINITY, sum = 0.f;
 #pragma unroll
-          for (int x = 0; x < kKeys; ++x)
-            if (x >= left) s[x] = -INFINITY;
-        }
-        float top = -INFINITY;
+        for (int y = 0; y < kKeys / 32; ++y) {
+          float s[32];
+          tm_ld32(s, s_at + 32 * y);
+          const float2 kt = *reinterpret_cast<const float2*>(scales + in * kGroups + 2 * y), lv = *reinterpret_cast<const float2*>(scales + 32 + in * kGroups + 2 * y),
+                       iv = *reinterpret_cast<const float2*>(scales + 64 + in * kGroups + 2 * y);
+          const float kg[2] = {q8::max_nan(f * kt.x, 1e-30f), q8::max_nan(f * kt.y, 1e-30f)}, ls[2] = {lv.x, lv.y}, per[2] = {iv.x, iv.y};
+          tc_wait_ld();
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const float* e = s + g * kGroup;
-          float a = max3(e[0], e[1], e[2]), b = max3(e[3], e[4], e[5]);
-          a = max3(a, e[6], e[7]), b = max3(b, e[8], e[9]);
-          a = max3(a, e[10], e[11]), b = max3(b, e[12], e[13]);
-          a = max3(a, e[14], e[15]);
-          top = fmaxf(top, fmaf(fmaxf(a, b), kg[g], ls[g]));
+          for (int g = 0; g < 2; ++g) {
+            float* e = s + g * kGroup;
+            const int here = left - 32 * y - g * kGroup;       // keys of the group that the row sees
+            if constexpr (kMasked) {
+#pragma unroll
+              for (int x = 0; x < kGroup; ++x)
+                if (x >= here) e[x] = -INFINITY;
+            }
+            float a = max3(e[0], e[1], e[2]), b = max3(e[3], e[4], e[5]);
+            a = max3(a, e[6], e[7]), b = max3(b, e[8], e[9]);
+            a = max3(a, e[10], e[11]), b = max3(b, e[12], e[13]);
+            a = max3(a, e[14], e[15]);
+            top = fmaxf(top, fmaf(fmaxf(a, b), kg[g], ls[g]));
+            if constexpr (kWeigh) {
+              const f32x2 kk = both(kg[g]), mm = both(ls[g] - from);
+              f32x2 two = 0ull;
+#pragma unroll
+              for (int x = 0; x < kGroup; x += 2) {
+                float u = e[x], v = e[x + 1];
+                scale_shift(u, v, kk, mm);
+                u = exp2_fast(u), v = exp2_fast(v);
+                if constexpr (kMasked) {
+                  if (x >= here) u = 0.f;
+                  if (x + 1 >= here) v = 0.f;
+                }
+                two = add2(two, pair(u, v));
+                p[16 * y + 8 * g + (x >> 1)] = pack2<__half>(u, v);
+              }
+              apart(a, b, two);
+              if (!kMasked || here > 0) sum = fmaf(a + b, per[g], sum);
+            }
+          }
         }
-        const bool grow = top > m + 14.f;
-        if (__any_sync(0xffffffffu, grow)) {
+      };
+      auto walk = [&](auto masked) {
+        if (i == 0) pass(masked, std::false_type{});
+        else pass(masked, std::true_type{});
+        const bool grow = top > m + 15.f;
+        if (i == 0 || __any_sync(0xffffffffu, grow)) {
           float corr = 1.f;
           if (grow) {
             const float now = top - 6.f;
@@ -352,40 +393,19 @@ prompt_kernel(const PromptAttn A) {
             scale_rows<D, 16>(tm_row + P::kO, corr);
           }
           l *= corr;
-        }
-        const float from = m == -INFINITY ? 0.f : m;       // a row that sees no key yet: weights 0
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const f32x2 kk = both(kg[g]), mm = both(ls[g] - from);
-          f32x2 sum = 0ull;
-          uint32_t p[8];
-#pragma unroll
-          for (int x = 0; x < kGroup; x += 2) {
-            float a = s[g * kGroup + x], b = s[g * kGroup + x + 1];
-            scale_shift(a, b, kk, mm);
-            a = exp2_fast(a), b = exp2_fast(b);
-            if constexpr (kMasked) {
-              if (g * kGroup + x >= left) a = 0.f;
-              if (g * kGroup + x + 1 >= left) b = 0.f;
-            }
-            sum = add2(sum, pair(a, b));
-            p[x >> 1] = pack2<__half>(a, b);
-          }
-          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(tm_row + (i & 1) * kKeys + 8 * g), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]),
-                       "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
-                       : "memory");
-          float a, b;
-          apart(a, b, sum);
-          if (!kMasked || g * kGroup < left) l = fmaf(a + b, per[g], l);
+          pass(masked, std::true_type{});
         }
       };
-      if (see_all < (w.t0 + i + 1) * kKeys) weigh(std::true_type{});
-      else weigh(std::false_type{});
+      if (see_all < (w.t0 + i + 1) * kKeys) walk(std::true_type{});
+      else walk(std::false_type{});
+      l += sum;
+#pragma unroll
+      for (int y = 0; y < kKeys / 32; ++y) tm_st16(s_at + 16 * y, *reinterpret_cast<uint32_t(*)[16]>(p + 16 * y));
       tc_wait_st();
       tc_fence_before();
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_p(rb, i)) : "memory");
     }
-    ok = bar_wait(bar_o(rb, run - 1), ((run - 1) >> 1) & 1, dead) && ok;
+    if (my_run > 0) ok = bar_wait(bar_o(rb, my_run - 1), ((my_run - 1) >> 1) & 1, dead) && ok;
     tc_fence_after();
     ok = ok && !*dead;
     if (!ok) l = NAN;
@@ -393,7 +413,7 @@ prompt_kernel(const PromptAttn A) {
       const int64_t part = w.part(A, row);
       if (row < rows) A.ml[part] = make_float2(m, l);
 #pragma unroll 1
-      for (int x = 0; x < D; x += 32) {
+      for (int x = 0; x < D && my_run > 0; x += 32) {
         float o[32];
         tm_ld32(o, tm_row + P::kO + x);
         tc_wait_ld();
@@ -475,7 +495,7 @@ Cut cut_of(int B, int max_new, int Hq, int Hkv, int longest) {
   Cut x;
   x.row_blocks = rows > kRows ? 2 : 1;
   x.blocks = static_cast<int>((rows + kRows * x.row_blocks - 1) / (kRows * x.row_blocks));
-  const int64_t units = static_cast<int64_t>(B) * Hkv * std::max(x.blocks, 1), slots = kNumSMs * (x.row_blocks == 1 ? 2 : 1), tiles = (longest + kKeys - 1ll) / kKeys;
+  const int64_t units = static_cast<int64_t>(B) * Hkv * std::max(x.blocks, 1), slots = kNumSMs * (x.row_blocks == 1 ? 2 : 1), tiles = (longest + 63ll) / 64;
   int64_t splits = units >= slots ? 1 : slots / units;
   splits = std::min(splits, std::max<int64_t>(tiles / 4, 1));
   x.splits = static_cast<int>(std::max<int64_t>(splits, 1));
