@@ -168,7 +168,7 @@ struct DecodePlan {
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBars = kRing, kDead = kBars + kWarps * kStages * 8, kEnd = kDead + 16;
   static constexpr int kSmem = kEnd + 1024;
-  static_assert(kWarps * 8 * (D + 2) * 4 <= kRing, "outputs go where the tiles were");
+  static_assert(kWarps * 16 * (D + 2) * 4 <= kRing, "outputs go where the tiles were");
   static_assert(4 * (kSmem + 1024) <= 228 * 1024, "shared memory");
 };
 // byte of (token, 16-byte piece) in a tile: lines of 128 bytes, a token each or two
@@ -182,10 +182,35 @@ __device__ __forceinline__ uint32_t tile_at(int token, int piece) {
 // at least, the last ones may have none), which leave maximum, sum and output in the workspace for decode_merge_kernel.
 struct Decode {
   Attn a;
-  int heads, blocks;              // query heads of a kv head; blocks of up to 8 of them
+  int G, max_rows, blocks;        // query heads of a kv head; rows of a sequence and kv head at most, blocks of up to 8 NB of them
   int items, splits;
-  float2* ml;                     // [item][part][8]: maximum (of scores in powers of two), sum
-  float* o;                       // [item][part][8][D]
+  float2* ml;                     // [item][part][row of the block]: maximum (of scores in powers of two), sum
+  float* o;                       // [item][part][row of the block][D]
+};
+// The rows of an item: a single token's query heads, or several tokens' one after another
+struct Item {
+  int block, kvh, b;
+  int first, base, rows, keys;    // packed row of the first token, tokens before it, rows of the sequence and kv head, keys that the block's rows see
+  template <int MOST>
+  __device__ __forceinline__ static Item of(const Decode& P, int item) {
+    Item x;
+    x.block = item % P.blocks, x.kvh = item / P.blocks % P.a.c.Hkv, x.b = item / P.blocks / P.a.c.Hkv;
+    int n, context;
+    P.a.r.of(x.b, &x.first, &n, &context);
+    x.keys = P.a.c.keys(context);
+    if (!P.a.r.starts) {       // (a sequence without keys has a row all the same: 0)
+      x.base = context - 1, x.rows = P.G;
+      return x;
+    }
+    x.base = context - n, x.rows = min(n * P.G, P.max_rows);
+    x.keys = x.block * MOST < x.rows ? min(x.keys, x.base + min(n, (x.block * MOST + MOST - 1) / P.G + 1)) : 0;
+    return x;
+  }
+  // element of queries or outputs, rows `stride` apart
+  __device__ __forceinline__ int64_t at(const Decode& P, int row, int64_t stride) const {
+    const int token = P.a.r.starts ? row / P.G : 0;
+    return (static_cast<int64_t>(first) + token) * stride + static_cast<int64_t>(kvh * P.G + row - token * P.G) * P.a.c.D;
+  }
 };
 constexpr int kLeastPart = 256;      // tokens
 
@@ -195,8 +220,9 @@ __device__ __forceinline__ int part_of(int keys, int splits) {
   return splits == 1 ? keys : max((keys + splits - 1) / splits + kOf - 1 - ((keys + splits - 1) / splits + kOf - 1) % kOf, kLeastPart);
 }
 
-template <typename T, typename C, int D, bool WARPITEM>
-__global__ void __launch_bounds__(kWarps * 32, 4)
+// NB blocks of 8 rows meet a tile, which is turned to fp16 once for them.  CAUSAL: several tokens, each sees the keys up to its own.
+template <typename T, typename C, int D, int NB, bool CAUSAL, bool WARPITEM>
+__global__ void __launch_bounds__(kWarps * 32, NB == 1 ? 4 : 3)
 decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using S = DecodePlan<D>;
   constexpr int kStages = S::kStages, kTiles = S::kTiles, kUnit = kTiles * kTok, kPieces = D / 16, kStep = WARPITEM ? 1 : kWarps;
@@ -205,8 +231,11 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
   asm volatile("griddepcontrol.launch_dependents;");
   const int unit = WARPITEM ? blockIdx.x * kWarps + warp : blockIdx.x, ofs = WARPITEM ? 0 : warp;
   if (WARPITEM && unit >= P.items) return;
-  const int split = WARPITEM ? 0 : unit % P.splits, item = WARPITEM ? unit : unit / P.splits, block = item % P.blocks, kvh = item / P.blocks % c.Hkv, b = item / P.blocks / c.Hkv;
-  const int head0 = kvh * P.heads + block * 8, G = min(8, P.heads - block * 8), keys = c.keys(P.a.r.context_lens[b]);
+  constexpr int kMost = 8 * NB;
+  const int split = WARPITEM ? 0 : unit % P.splits, item = WARPITEM ? unit : unit / P.splits;
+  const Item it = Item::of<kMost>(P, item);
+  const int b = it.b, kvh = it.kvh, keys = it.keys, row0 = it.block * kMost, rows = min(kMost, it.rows - row0);
+  if (CAUSAL && rows <= 0) return;
   const int part = WARPITEM ? keys : part_of(keys, P.splits), first = split * part, run = first < keys ? (min(part, keys - first) + kUnit - 1) / kUnit : 0, u0 = first / kUnit;
   const int mine = run > ofs ? (run - ofs + kStep - 1) / kStep : 0;       // units u0 + ofs, and every kStep-th
 
@@ -270,14 +299,17 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
   }
 
   // queries: head quad's columns 16 i + 4 tq .. + 3
-  uint32_t qf[kPieces][2];
-  float factor[2];        // of heads 2 tq and 2 tq + 1
-  {
-    const T* q = static_cast<const T*>(P.a.q) + b * P.a.q_stride + static_cast<int64_t>(head0 + quad) * D + 4 * tq;
+  uint32_t qf[NB][kPieces][2];
+  float factor[NB][2];        // of rows 2 tq and 2 tq + 1 of a block of 8
+  int see[NB][2];             // keys that they see
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const bool in = 8 * nb + quad < rows;
+    const T* q = static_cast<const T*>(P.a.q) + (in ? it.at(P, row0 + 8 * nb + quad, P.a.q_stride) : 0) + 4 * tq;
     uint2 raw[kPieces];
     float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) raw[i] = quad < G ? *reinterpret_cast<const uint2*>(q + 16 * i) : make_uint2(0u, 0u);
+    for (int i = 0; i < kPieces; ++i) raw[i] = in ? *reinterpret_cast<const uint2*>(q + 16 * i) : make_uint2(0u, 0u);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const T* e = reinterpret_cast<const T*>(&raw[i]);
@@ -286,25 +318,30 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
     }
     most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = q8::max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    float f = P.a.scale * 1.4426950408889634f;
     const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) - 14;       // most = 2^(e + 14) .. 2^(e + 15)
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), f = P.a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const T* x = reinterpret_cast<const T*>(&raw[i]);
-      qf[i][0] = pack2<__half>(Cvt<T>::to_f32(x[0]) * down, Cvt<T>::to_f32(x[1]) * down);
-      qf[i][1] = pack2<__half>(Cvt<T>::to_f32(x[2]) * down, Cvt<T>::to_f32(x[3]) * down);
+      qf[nb][i][0] = pack2<__half>(Cvt<T>::to_f32(x[0]) * down, Cvt<T>::to_f32(x[1]) * down);
+      qf[nb][i][1] = pack2<__half>(Cvt<T>::to_f32(x[2]) * down, Cvt<T>::to_f32(x[3]) * down);
     }
-    f *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-    factor[0] = __shfl_sync(0xffffffffu, f, 8 * tq);
-    factor[1] = __shfl_sync(0xffffffffu, f, 8 * tq + 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      factor[nb][h] = __shfl_sync(0xffffffffu, f, 8 * tq + 4 * h);
+      see[nb][h] = CAUSAL ? min(it.base + min(row0 + 8 * nb + 2 * tq + h, it.rows - 1) / P.G + 1, keys) : keys;
+    }
   }
 #pragma unroll
   for (int h = 0; h < kTiles; ++h) vs[h] = log2f(q8::max_nan(vs[h], q8::kLeastScale));
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kPieces][4];
+  float m[NB][2], l[NB][2], o[NB][kPieces][4];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb][0] = m[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+  }
   bool ok = true;
   int buf = 0, left = keys - kUnit * (u0 + ofs);        // tokens from the unit's first on
   uint32_t parity = 0;
@@ -317,10 +354,11 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
     const uint32_t tiles = ring + buf * S::kStage;
     ok = __all_sync(0xffffffffu, bar_wait1(bars + buf * 8, parity, dead));
     if (!ok) break;
-    float x[kTiles][4], ls[kTiles];
+    float x[kTiles][NB][4], ls[kTiles];
 #pragma unroll
     for (int h = 0; h < kTiles; ++h) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) x[h][nb][0] = x[h][nb][1] = x[h][nb][2] = x[h][nb][3] = 0.f;
 #pragma unroll
       for (int p = 0; p < kPieces; p += 2) {
         uint32_t r[4];
@@ -330,54 +368,86 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
           uint32_t a0, a1, a2, a3;
           q8::halves<C, false>(r[2 * u], a0, a2);
           q8::halves<C, false>(r[2 * u + 1], a1, a3);
-          mma16(s, a0, a1, a2, a3, qf[p + u][0], qf[p + u][1]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16(x[h][nb], a0, a1, a2, a3, qf[nb][p + u][0], qf[nb][p + u][1]);
         }
       }
-      // s[0], s[1]: token quad, heads 2 tq and 2 tq + 1; s[2], s[3]: token quad + 8
-      const float kt = __shfl_sync(0xffffffffu, ks[h], i & 31), f0 = factor[0] * kt, f1 = factor[1] * kt;
+      // [0], [1]: token quad, rows 2 tq and 2 tq + 1; [2], [3]: token quad + 8
+      const float kt = __shfl_sync(0xffffffffu, ks[h], i & 31);
       ls[h] = __shfl_sync(0xffffffffu, vs[h], i & 31);
-      x[h][0] = fmaf(s[0], f0, ls[h]), x[h][1] = fmaf(s[1], f1, ls[h]), x[h][2] = fmaf(s[2], f0, ls[h]), x[h][3] = fmaf(s[3], f1, ls[h]);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float f0 = factor[nb][0] * kt, f1 = factor[nb][1] * kt;
+        float* s = x[h][nb];
+        s[0] = fmaf(s[0], f0, ls[h]), s[1] = fmaf(s[1], f1, ls[h]), s[2] = fmaf(s[2], f0, ls[h]), s[3] = fmaf(s[3], f1, ls[h]);
+      }
     }
-    if (left < kUnit) {
+    // of several tokens, the first one's last key
+    const bool masked = CAUSAL ? keys - left + kUnit > it.base + 1 : left < kUnit;
+    if (masked) {
 #pragma unroll
       for (int h = 0; h < kTiles; ++h) {
-        if (h * kTok + quad >= left) x[h][0] = x[h][1] = -INFINITY;
-        if (h * kTok + quad + 8 >= left) x[h][2] = x[h][3] = -INFINITY;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (h * kTok + quad + 8 * (e >> 1) >= left - keys + see[nb][e & 1]) x[h][nb][e] = -INFINITY;
+        }
       }
       if constexpr (std::is_same_v<C, q8::E4m3>) {       // what is behind the last token may be no number
-        for (int e = left * kPieces + lane; e < kUnit * kPieces; e += 32) {
+        for (int e = max(left, 0) * kPieces + lane; e < kUnit * kPieces; e += 32) {
           const int token = e / kPieces;
           asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(tiles + (kTiles + token / kTok) * S::kTile + tile_at<D>(token % kTok, e % kPieces)), "r"(0) : "memory");
         }
         __syncwarp();
       }
     }
-    float t0 = fmaxf(x[0][0], x[0][2]), t1 = fmaxf(x[0][1], x[0][3]);
+    bool grow = false;
+    float top[NB][2];
 #pragma unroll
-    for (int h = 1; h < kTiles; ++h) t0 = fmaxf(t0, fmaxf(x[h][0], x[h][2])), t1 = fmaxf(t1, fmaxf(x[h][1], x[h][3]));
-    if (__any_sync(0xffffffffu, t0 > m[0] + 14.f || t1 > m[1] + 14.f)) {
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float top = h ? t1 : t0;
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const float now = fmaxf(m[h], top - 6.f), corr = m[h] == -INFINITY ? 0.f : exp2_fast(m[h] - now);
-        m[h] = now;
-        l[h] *= corr;
+      for (int y = 0; y < 2; ++y) {
+        float a = fmaxf(x[0][nb][y], x[0][nb][y + 2]);
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) o[p][h] *= corr, o[p][h + 2] *= corr;
+        for (int h = 1; h < kTiles; ++h) a = fmaxf(a, fmaxf(x[h][nb][y], x[h][nb][y + 2]));
+        top[nb][y] = a;
+        grow = grow || a > m[nb][y] + 14.f;
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float a = top[nb][h];
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 4));
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
+          const float now = fmaxf(m[nb][h], a - 6.f), corr = m[nb][h] == -INFINITY ? 0.f : exp2_fast(m[nb][h] - now);
+          m[nb][h] = now;
+          l[nb][h] *= corr;
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) o[nb][p][h] *= corr, o[nb][p][h + 2] *= corr;
+        }
       }
     }
 #pragma unroll
     for (int h = 0; h < kTiles; ++h) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[h][e] - m[e & 1]);
       const float per = exp2_fast(-ls[h]);
-      l[0] = fmaf(w[0] + w[2], per, l[0]);
-      l[1] = fmaf(w[1] + w[3], per, l[1]);
-      const uint32_t b0 = transposed(pack2<__half>(w[0], w[1])), b1 = transposed(pack2<__half>(w[2], w[3]));
+      uint32_t w01[NB], w23[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[h][nb][e] - (CAUSAL && m[nb][e & 1] == -INFINITY ? 0.f : m[nb][e & 1]));      // (a row that sees no key yet: 0)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float sum = w[y] + w[y + 2];
+          l[nb][y] = fmaf(sum, CAUSAL && sum == 0.f ? 0.f : per, l[nb][y]);        // (whatever the scale of a page that a row does not see)
+        }
+        w01[nb] = transposed(pack2<__half>(w[0], w[1])), w23[nb] = transposed(pack2<__half>(w[2], w[3]));
+      }
 #pragma unroll
       for (int p = 0; p < kPieces; p += 2) {
         uint32_t r[4];
@@ -387,7 +457,8 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
           uint32_t a0, a1, a2, a3;
           q8::halves<C, true>(r[2 * u], a0, a1);
           q8::halves<C, true>(r[2 * u + 1], a2, a3);
-          mma16(o[p + u], a0, a1, a2, a3, b0, b1);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16(o[nb][p + u], a0, a1, a2, a3, w01[nb], w23[nb]);
         }
       }
     }
@@ -408,66 +479,73 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
   }
   if (!ok || *dead) {      // a wait gave up: what is under way gets 10 ms to end; no number comes out
     for (const long long begun = clock64(); clock64() - begun < 20000000ll;) {}
-    l[0] = l[1] = NAN;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) l[nb][0] = l[nb][1] = NAN;
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[nb][h] += __shfl_xor_sync(0xffffffffu, l[nb][h], 4);
+      l[nb][h] += __shfl_xor_sync(0xffffffffu, l[nb][h], 8);
+      l[nb][h] += __shfl_xor_sync(0xffffffffu, l[nb][h], 16);
+    }
   }
-  // ---- outputs: columns 16 p + 2 quad and + 1, heads 2 tq and 2 tq + 1, of the warps' parts, where the tiles were ------------------------------
+  // ---- outputs: columns 16 p + 2 quad and + 1, rows 2 tq and 2 tq + 1, of the warps' parts, where the tiles were -------------------------------
   constexpr int kSets = WARPITEM ? 1 : kWarps;
   if constexpr (WARPITEM) __syncwarp();
   else __syncthreads();
-  float* o_s = reinterpret_cast<float*>(sm + (WARPITEM ? warp * kStages * S::kStage : 0));      // [set][8][D]
-  float *m_s = o_s + kSets * 8 * D, *l_s = m_s + kSets * 8;
+  float* o_s = reinterpret_cast<float*>(sm + (WARPITEM ? warp * kStages * S::kStage : 0));      // [set][row][D]
+  float *m_s = o_s + kSets * kMost * D, *l_s = m_s + kSets * kMost;
   const int set = WARPITEM ? 0 : warp;
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
+  for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(o_s + (set * 8 + 2 * tq + h) * D + 16 * p + 2 * quad) = make_float2(o[p][h], o[p][h + 2]);
-  }
-  if (quad == 0) {
+    for (int h = 0; h < 2; ++h) {
+      const int row = set * kMost + 8 * nb + 2 * tq + h;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) m_s[set * 8 + 2 * tq + h] = m[h], l_s[set * 8 + 2 * tq + h] = l[h];
+      for (int p = 0; p < kPieces; ++p) *reinterpret_cast<float2*>(o_s + row * D + 16 * p + 2 * quad) = make_float2(o[nb][p][h], o[nb][p][h + 2]);
+      if (quad == 0) m_s[row] = m[nb][h], l_s[row] = l[nb][h];
+    }
   }
   if constexpr (WARPITEM) __syncwarp();
   else __syncthreads();
-  for (int e = WARPITEM ? lane : threadIdx.x; e < G * (D / 2); e += WARPITEM ? 32 : kWarps * 32) {
+  for (int e = WARPITEM ? lane : threadIdx.x; e < rows * (D / 2); e += WARPITEM ? 32 : kWarps * 32) {
     const int g = e / (D / 2), d = e % (D / 2) * 2;
     float top = -INFINITY, sum = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSets; ++w) top = fmaxf(top, m_s[w * 8 + g]);
+    for (int w = 0; w < kSets; ++w) top = fmaxf(top, m_s[w * kMost + g]);
 #pragma unroll
     for (int w = 0; w < kSets; ++w) {
-      const float mw = m_s[w * 8 + g], lw = l_s[w * 8 + g], k = mw == -INFINITY ? (lw != lw ? 1.f : 0.f) : exp2_fast(mw - top);
-      const float2 v = *reinterpret_cast<const float2*>(o_s + (w * 8 + g) * D + d);
+      const float mw = m_s[w * kMost + g], lw = l_s[w * kMost + g], k = mw == -INFINITY ? (lw != lw ? 1.f : 0.f) : exp2_fast(mw - top);
+      const float2 v = *reinterpret_cast<const float2*>(o_s + (w * kMost + g) * D + d);
       sum = fmaf(lw, k, sum);
       a0 = fmaf(v.x, k, a0);
       a1 = fmaf(v.y, k, a1);
     }
     if (WARPITEM || P.splits == 1) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + (static_cast<int64_t>(b) * P.a.Hq + head0 + g) * D + d) = pack2<T>(a0 * f, a1 * f);
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + it.at(P, row0 + g, static_cast<int64_t>(P.a.Hq) * D) + d) = pack2<T>(a0 * f, a1 * f);
     } else {
-      const int64_t piece = static_cast<int64_t>(unit) * 8 + g;
+      const int64_t piece = static_cast<int64_t>(unit) * kMost + g;
       *reinterpret_cast<float2*>(P.o + piece * D + d) = make_float2(a0, a1);
       if (d == 0) P.ml[piece] = make_float2(top, sum);
     }
   }
 }
 
-// A CTA per item and head: the parts in the order of the keys, by four groups of threads.  (All that needs no part is done before the kernel ahead ends.)
-template <typename T, int D>
+// A CTA per item and row: the parts in the order of the keys, by four groups of threads.  (All that needs no part is done before the kernel ahead ends.)
+template <typename T, int D, int NB>
 __global__ void __launch_bounds__(2 * D) decode_merge_kernel(const Decode P) {
   constexpr int kCols = D / 2, kAhead = 4;      // two columns a thread
   __shared__ float2 part_s[3][kCols];
   __shared__ float sum_s[4], top_s[4];
-  const int most = min(P.heads, 8), g = blockIdx.x % most, item = blockIdx.x / most, block = item % P.blocks, kvh = item / P.blocks % P.a.c.Hkv, b = item / P.blocks / P.a.c.Hkv;
-  const int col = threadIdx.x % kCols, group = threadIdx.x / kCols, keys = P.a.c.keys(P.a.r.context_lens[b]), part = part_of(keys, P.splits), parts = keys > 0 ? (keys + part - 1) / part : 0;
+  constexpr int kMost = 8 * NB;
+  const int most = min(P.max_rows, kMost), g = blockIdx.x % most, item = blockIdx.x / most;
+  const Item it = Item::of<kMost>(P, item);
+  const int row = it.block * kMost + g, col = threadIdx.x % kCols, group = threadIdx.x / kCols, keys = it.keys, part = part_of(keys, P.splits), parts = keys > 0 ? (keys + part - 1) / part : 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (block * 8 + g >= P.heads) return;
+  if (row >= it.rows) return;
   float top = -INFINITY, sum = 0.f;
   float2 o = make_float2(0.f, 0.f);
   for (int p0 = group; p0 < parts; p0 += 4 * kAhead) {
@@ -475,7 +553,7 @@ __global__ void __launch_bounds__(2 * D) decode_merge_kernel(const Decode P) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int p = p0 + 4 * u;
-      const int64_t piece = (static_cast<int64_t>(item) * P.splits + p) * 8 + g;
+      const int64_t piece = (static_cast<int64_t>(item) * P.splits + p) * kMost + g;
       ml[u] = make_float2(-INFINITY, 0.f), v[u] = make_float2(0.f, 0.f);
       if (p < parts) ml[u] = P.ml[piece], v[u] = *reinterpret_cast<const float2*>(P.o + piece * D + 2 * col);
     }
@@ -508,7 +586,7 @@ __global__ void __launch_bounds__(2 * D) decode_merge_kernel(const Decode P) {
 #pragma unroll
   for (int y = 1; y < 4; ++y) o.x = fmaf(part_s[y - 1][col].x, k[y], o.x), o.y = fmaf(part_s[y - 1][col].y, k[y], o.y);
   const float f = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + (static_cast<int64_t>(b) * P.a.Hq + kvh * P.heads + block * 8 + g) * D + 2 * col) = pack2<T>(o.x * f, o.y * f);
+  *reinterpret_cast<uint32_t*>(static_cast<T*>(P.a.out) + it.at(P, row, static_cast<int64_t>(P.a.Hq) * D) + 2 * col) = pack2<T>(o.x * f, o.y * f);
 }
 
 // The pool as lines of 128 bytes, fetched 16 tokens at a time; lines behind the pool read as zeros
@@ -535,17 +613,24 @@ int splits_of(int64_t items, int longest) {
   if (longest >= 8192) splits = std::max(splits, std::min<int64_t>(longest / 2048, 1024 / items));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, (longest + kLeastPart - 1ll) / kLeastPart)));
 }
-int64_t items_of(int B, int Hq, int Hkv) { return static_cast<int64_t>(B) * Hkv * ((Hq / Hkv + 7) / 8); }
+// Rows of a sequence and kv head, in blocks of 8 or 16
+int most_of(int rows) { return rows <= 8 ? 8 : 16; }
+int64_t items_of(int B, int Hkv, int rows) { return static_cast<int64_t>(B) * Hkv * ((rows + most_of(rows) - 1) / most_of(rows)); }
+size_t decode_bytes(int B, int Hkv, int D, int rows, int longest) {
+  const int most = most_of(rows);
+  const int64_t items = items_of(B, Hkv, rows), splits = splits_of(items, longest);
+  return splits > 1 ? static_cast<size_t>(items * splits) * most * (D + 2) * sizeof(float) : 0;
+}
 
-template <typename T, typename C, int D, bool WARPITEM>
+template <typename T, typename C, int D, int NB, bool CAUSAL, bool WARPITEM>
 int launch_decode_as(const char* name, const Decode& P, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
-  auto kern = decode_kernel<T, C, D, WARPITEM>;
+  auto kern = decode_kernel<T, C, D, NB, CAUSAL, WARPITEM>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodePlan<D>::kSmem);
   kern<<<WARPITEM ? (P.items + kWarps - 1) / kWarps : P.items * P.splits, kWarps * 32, DecodePlan<D>::kSmem, stream>>>(P, k_map, v_map);
   if (int rc = check_launch(name)) return rc;
   if (P.splits == 1) return 0;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(P.items) * static_cast<unsigned>(P.heads < 8 ? P.heads : 8));
+  cfg.gridDim = dim3(static_cast<unsigned>(P.items) * static_cast<unsigned>(std::min(P.max_rows, 8 * NB)));
   cfg.blockDim = dim3(2 * D);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -553,7 +638,7 @@ int launch_decode_as(const char* name, const Decode& P, const CUtensorMap& k_map
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_merge_kernel<T, D>, P);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_merge_kernel<T, D, NB>, P);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
@@ -561,22 +646,49 @@ int launch_decode_as(const char* name, const Decode& P, const CUtensorMap& k_map
   return 0;
 }
 
+// rows: of a sequence and kv head at most
 template <typename T>
-int launch_decode(const char* name, const Attn& A, int longest, void* workspace, int codes, cudaStream_t stream) {
+int launch_decode(const char* name, const Attn& A, int rows, int longest, void* workspace, int codes, cudaStream_t stream) {
   Decode P{};
-  P.a = A, P.heads = A.Hq / A.c.Hkv, P.blocks = (P.heads + 7) / 8, P.items = static_cast<int>(items_of(A.r.B, A.Hq, A.c.Hkv));
+  const int most = most_of(rows);
+  P.a = A, P.G = A.Hq / A.c.Hkv, P.max_rows = rows, P.blocks = (rows + most - 1) / most, P.items = static_cast<int>(items_of(A.r.B, A.c.Hkv, rows));
   P.splits = splits_of(P.items, longest);
-  P.ml = static_cast<float2*>(workspace), P.o = static_cast<float*>(workspace) + static_cast<int64_t>(P.items) * P.splits * 16;
+  P.ml = static_cast<float2*>(workspace), P.o = static_cast<float*>(workspace) + static_cast<int64_t>(P.items) * P.splits * 2 * most;
   CUtensorMap k_map, v_map;
   if (!code_map(&k_map, A.c.k_pool, A.c) || !code_map(&v_map, A.c.v_pool, A.c)) return fail(B200_EINVAL, "%s: no tensor map of the pools", name);
-  const bool warps = longest <= kShort && P.items > 4 * kNumSMs;       // more than are resident at once
+  const bool warps = longest <= kShort && most == 8 && P.items > 4 * kNumSMs;       // more than are resident at once
   auto go = [&](auto* c, auto d) {
     using C = std::remove_pointer_t<decltype(c)>;
-    return warps ? launch_decode_as<T, C, d.value, true>(name, P, k_map, v_map, stream) : launch_decode_as<T, C, d.value, false>(name, P, k_map, v_map, stream);
+    if (A.r.starts)
+      return most == 16 ? launch_decode_as<T, C, d.value, 2, true, false>(name, P, k_map, v_map, stream)
+             : warps    ? launch_decode_as<T, C, d.value, 1, true, true>(name, P, k_map, v_map, stream)
+                        : launch_decode_as<T, C, d.value, 1, true, false>(name, P, k_map, v_map, stream);
+    return most == 16 ? launch_decode_as<T, C, d.value, 2, false, false>(name, P, k_map, v_map, stream)
+           : warps    ? launch_decode_as<T, C, d.value, 1, false, true>(name, P, k_map, v_map, stream)
+                      : launch_decode_as<T, C, d.value, 1, false, false>(name, P, k_map, v_map, stream);
   };
   auto of = [&](auto* c) { return A.c.D == 128 ? go(c, std::integral_constant<int, 128>{}) : go(c, std::integral_constant<int, 64>{}); };
   return codes == B200_CODES_INT8 ? of(static_cast<q8::Int8*>(nullptr)) : of(static_cast<q8::E4m3*>(nullptr));
 }
+
+// Whether these kernels take a call: sizes, alignment, numbers that fit
+bool decode_takes(const Attn& A, int rows, int longest, int dtype) {
+  const int most = most_of(rows);
+  const int64_t items = items_of(A.r.B, A.c.Hkv, rows);
+  return decode_serves(A.c.D, A.c.bs, dtype) && aligned16(A.c.k_pool) && aligned16(A.c.v_pool) && !(reinterpret_cast<uintptr_t>(A.q) & 7) && A.q_stride % 4 == 0 &&
+         !(reinterpret_cast<uintptr_t>(A.out) & 3) && (A.c.max_blocks + 1) * A.c.Hkv * A.c.bs < INT32_MAX && items * most * splits_of(items, longest) < INT32_MAX;
+}
+int run_decode(const char* name, const Attn& A, int rows, int longest, void* workspace, size_t workspace_bytes, int codes, int dtype, cudaStream_t stream) {
+  const size_t need = decode_bytes(A.r.B, A.c.Hkv, A.c.D, rows, longest);
+  if (need && (!workspace || workspace_bytes < need)) return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);
+  if (need && !aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
+  return dtype == B200_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(name, A, rows, longest, workspace, codes, stream)
+                                  : launch_decode<__half>(name, A, rows, longest, workspace, codes, stream);
+}
+// Several tokens per sequence: whether they are few enough for these kernels rather than those of b200_prompt_q8.cu.  us here / there: 64 x 2 tokens of 4 heads at
+// 2k (8 rows) 53 / 119, 64 x 4 (16 rows) 80 / 120, 16 x 9 of one head of 64 at 3k 23 / 56; 32 rows in two blocks: 1 x 8 of 4 heads at 32k 38 / 51, at 4k 14 / 20; 8 x 32 of
+// one head at 8k 85 / 67, 16 x 16 of two 139 / 114.
+bool few_rows(int B, int Hkv, int64_t rows) { return rows <= 16 || (rows <= 32 && static_cast<int64_t>(B) * Hkv <= 32); }
 
 constexpr int kAnyMostD = 256;
 
@@ -624,8 +736,7 @@ extern "C" {
 
 size_t b200_paged_decode_attn_q8_workspace(int B, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || block_size <= 0 || max_context_len < 0 || !decode_serves(D, block_size, dtype)) return 0;
-  const int64_t items = items_of(B, Hq, Hkv), splits = splits_of(items, max_context_len);
-  return splits > 1 ? static_cast<size_t>(items * splits) * 8 * (D + 2) * sizeof(float) : 0;
+  return decode_bytes(B, Hkv, D, Hq / Hkv, max_context_len);
 }
 
 int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
@@ -639,22 +750,16 @@ int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const 
   if (max_context_len < 0) return fail(B200_EINVAL, "%s: negative max_context_len", name);
   if (B == 0) return 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool pieces = aligned16(k_pool) && aligned16(v_pool) && !(reinterpret_cast<uintptr_t>(q) & 7) && q_stride % 4 == 0 && !(reinterpret_cast<uintptr_t>(out) & 3);
-  const int64_t items = items_of(B, Hq, Hkv);
-  // pages, items and parts whose numbers fit
-  if (decode_serves(D, block_size, dtype) && pieces && !(flags & B200_ATTN_FORCE_GENERIC) && (max_blocks + 1) * Hkv * block_size < INT32_MAX &&
-      items * 8 * splits_of(items, max_context_len) < INT32_MAX) {
-    const size_t need = b200_paged_decode_attn_q8_workspace(B, Hq, Hkv, D, block_size, max_context_len, dtype);
-    if (need && (!workspace || workspace_bytes < need)) return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);
-    if (need && !aligned16(workspace)) return fail(B200_EINVAL, "%s: workspace not aligned to 16 bytes", name);
-    return dtype == B200_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(name, A, max_context_len, workspace, codes, s)
-                                    : launch_decode<__half>(name, A, max_context_len, workspace, codes, s);
-  }
+  if (!(flags & B200_ATTN_FORCE_GENERIC) && decode_takes(A, Hq / Hkv, max_context_len, dtype))
+    return run_decode(name, A, Hq / Hkv, max_context_len, workspace, workspace_bytes, codes, dtype, s);
   return launch_any_of(name, A, codes, dtype, s);
 }
 
 size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
-  return prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype);
+  if (B <= 0 || max_new <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || block_size <= 0 || max_context_len < 0) return 0;
+  const int64_t rows = static_cast<int64_t>(max_new) * (Hq / Hkv);
+  const size_t few = few_rows(B, Hkv, rows) && decode_serves(D, block_size, dtype) ? decode_bytes(B, Hkv, D, static_cast<int>(rows), max_context_len) : 0;
+  return std::max(few, prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype));
 }
 
 int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
@@ -672,6 +777,9 @@ int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const 
   q8::PromptAttn P{};
   P.c = A.c, P.r = A.r, P.out = out, P.q = q, P.q_stride = q_stride, P.Hq = Hq, P.scale = scale;
   if (max_new == 0) return 0;
+  const int64_t of_head = static_cast<int64_t>(max_new) * (Hq / Hkv);
+  if (!(flags & B200_ATTN_FORCE_GENERIC) && few_rows(B, Hkv, of_head) && decode_takes(A, static_cast<int>(of_head), max_context_len, dtype))
+    return run_decode(name, A, static_cast<int>(of_head), max_context_len, workspace, workspace_bytes, codes, dtype, s);
   if (!(flags & B200_ATTN_FORCE_GENERIC) && prompt_q8_serves(P, max_new, max_context_len, dtype)) {
     const size_t need = prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype);
     if (need && (!workspace || workspace_bytes < need)) return fail(B200_ENOSPC, "%s: workspace of %zu bytes", name, workspace ? workspace_bytes : 0);

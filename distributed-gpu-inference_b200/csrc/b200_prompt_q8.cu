@@ -260,16 +260,23 @@ prompt_kernel(const PromptAttn A) {
     const uint32_t q_at = sm0 + P::kQ + rb * P::kQBlock, tm_row = tm + rb * P::kTm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     float* factor = reinterpret_cast<float*>(sm + P::kFactor);
     const float sign = A.scale < 0.f ? -1.f : 1.f;
+    // Token of the CTA's row y, from its first row's.  (A division costs 30 instructions; at most 4096 + 256 rows: the product is exact enough.)
+    const int token0 = w.row0 / G, head0 = w.row0 - token0 * G;
+    const float per_head = 1.0f / static_cast<float>(G);
+    auto token_of = [&](int y) { return static_cast<int>((static_cast<float>(head0 + y) + 0.5f) * per_head); };
+    // rows of a token lie D apart, tokens `stride`
+    auto place_of = [&](int y, int64_t stride) { return token_of(y) * (stride - static_cast<int64_t>(G) * D) + static_cast<int64_t>(y) * D; };
+    auto first_place = [&](int64_t stride) { return (static_cast<int64_t>(w.first) + token0) * stride + static_cast<int64_t>(w.kvh * G + head0) * D; };
     {
       constexpr int kCh = D / 8, kPer = 32 / kCh, kSteps = 32 / kPer;        // pieces of a row, rows of a step
       const int ch = lane % kCh, r = lane / kCh;
       constexpr int kAhead = kSteps < 16 ? kSteps : 16;
       int4 raw[kAhead];
+      const T* q = static_cast<const T*>(A.q) + first_place(A.q_stride) + ch * 8;
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
-        const int at = w.row0 + 32 * warp + u * kPer + r, t = at / G;
-        raw[u] = at < rows ? ld_stream16(static_cast<const T*>(A.q) + (static_cast<int64_t>(w.first) + t) * A.q_stride + static_cast<int64_t>(w.kvh * G + at - t * G) * D + ch * 8)
-                           : make_int4(0, 0, 0, 0);
+        const int y = 32 * warp + u * kPer + r;
+        raw[u] = w.row0 + y < rows ? ld_stream16(q + place_of(y, A.q_stride)) : make_int4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
@@ -437,13 +444,14 @@ prompt_kernel(const PromptAttn A) {
       }
       __syncwarp();
       constexpr int kCh = D / 8;
-#pragma unroll 4
+      T* out = static_cast<T*>(A.out) + first_place(static_cast<int64_t>(A.Hq) * D) + lane % kCh * 8;
+#pragma unroll 8
       for (int u = 0; u < kCh; ++u) {
-        const int e = lane + u * 32, r = e / kCh, ch = e % kCh, at = w.row0 + 32 * warp + r, t = at / G;
-        if (at < rows) {
+        const int r = (lane + u * 32) / kCh, y = 32 * warp + r;
+        if (w.row0 + y < rows) {
           uint4 x;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(line(q_at, 32 * (warp & 3) + r, ch, kRows)) : "memory");
-          *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + ((static_cast<int64_t>(w.first) + t) * A.Hq + w.kvh * G + at - t * G) * D + ch * 8) = x;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(line(q_at, 32 * (warp & 3) + r, lane % kCh, kRows)) : "memory");
+          *reinterpret_cast<uint4*>(out + place_of(y, static_cast<int64_t>(A.Hq) * D)) = x;
         }
       }
     }
