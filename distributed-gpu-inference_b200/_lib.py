@@ -419,6 +419,34 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_fast = None
+
+
+def fast_calls():
+    """The module of csrc/b200_fast_calls.cpp over the loaded library, or None where it is not built (the calls then go through ctypes alone)."""
+    global _fast
+    if _fast is None:
+        lib = load()
+        path = os.path.join(_PKG_DIR, "_fast_calls.so")
+        module = False
+        if os.path.exists(path):
+            import importlib.util
+
+            import torch  # noqa: F401 - its libraries come first
+
+            try:
+                spec = importlib.util.spec_from_file_location("_fast_calls", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.entry_points(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+                    "b200_rope_kv_append_q8", "b200_kv_gather_dense_q8", "b200_paged_decode_attn_q8", "b200_paged_decode_attn_q8_workspace",
+                    "b200_paged_prompt_attn_q8", "b200_paged_prompt_attn_q8_workspace")))
+            except ImportError:      # built for another interpreter or torch
+                module = False
+        _fast = module
+    return _fast or None
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().b200_last_error()

@@ -929,6 +929,12 @@ def rope_kv_append_q8(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
     ``context_lens[b]`` tokens; ``max_new`` (default: ``n``) bounds how many a sequence has.  Where new tokens do not begin a page they share its scale with the
     earlier ones, whose codes are put into a scale that had to grow.  ``cos / sin``: contiguous ``[n, D]`` in the storage dtype.  Other
     than in ``rope_kv_append`` the rotation is in fp32, rounded once (queries) or not before the code (keys)."""
+    if q is not None and q_out is None:
+        fast = _lib.fast_calls()
+        if fast is not None:
+            done = fast.append(q, k, v, cos, sin, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, row_starts, max_new)
+            if done is not None:
+                return done
     _need_cuda(k)
     dev, dtype = k.get_device(), k.dtype
     (max_blocks, Hkv, bs, D), codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
@@ -976,6 +982,11 @@ def kv_gather_dense_q8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torc
                        n_tokens: int, dtype: torch.dtype = torch.bfloat16):
     """``kv_gather_dense`` of a cache in 8 bits: the first ``n_tokens`` tokens of every row of ``block_tables`` as ``(k, v)``, each ``[B, Hkv, n_tokens, D]``
     of ``dtype`` (code times scale, rounded once)."""
+    fast = _lib.fast_calls()
+    if fast is not None:
+        done = fast.gather(k_pool, v_pool, k_scale, v_scale, block_tables, n_tokens, DTYPE_ID.get(dtype))
+        if done is not None:
+            return done
     _need_cuda(k_pool)
     dev = k_pool.get_device()
     (max_blocks, Hkv, bs, D), codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
@@ -1028,6 +1039,12 @@ def paged_decode_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     ``context_lens[b]`` tokens of its pages; 0 where there are none.  ``max_context_len``: the host's bound of the lengths (tokens
     behind it may be left out).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
     torch's caching allocator.  ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
+    if out is None and workspace is None and flags == 0 and ATTN_EVENTS is None:
+        fast = _lib.fast_calls()
+        if fast is not None:
+            done = fast.decode(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, max_context_len, scale)
+            if done is not None:
+                return done
     _need_cuda(q)
     dev = q.get_device()
     shape, codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)
@@ -1064,6 +1081,12 @@ def paged_prompt_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     ``max_context_len``: the host's bounds of a sequence's rows and of its tokens (what is behind them may be left out).  ``workspace``: at least
     ``prompt_attention_q8_workspace`` bytes that no call running at the same time uses; None: from torch's caching allocator.
     ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
+    if out is None and workspace is None and flags == 0 and ATTN_EVENTS is None:
+        fast = _lib.fast_calls()
+        if fast is not None:
+            done = fast.prompt(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, row_starts, max_new, max_context_len, scale)
+            if done is not None:
+                return done
     _need_cuda(q)
     dev = q.get_device()
     shape, codes, cache = _q8_cache(k_pool, v_pool, k_scale, v_scale, block_tables, dev)

@@ -58,3 +58,20 @@ def test_argument_errors_have_codes_and_words():
     assert append(rows=0)[0] == 0 and append(starts=None)[0] == -1 and append(sin=None)[0] == -1 and append(cos=None, sin=None)[0] == -1
     assert append(D=33)[0] == -2 and append(q=None)[0] == -1 and append(B=2 ** 30, most=2 ** 30, rows=2 ** 30)[0] == -2
     assert gather(n=65)[0] == -1 and gather(n=0)[0] == 0
+
+
+def test_the_fast_module_leaves_what_is_not_plain_to_the_checks():
+    fast = _lib.fast_calls()
+    assert fast is not None, "_fast_calls.so is not built: run __graft_entry__.build()"
+    pool, scale = torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2)
+    tables, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    cache = (pool, pool, scale, scale, tables)
+    for got in (fast.decode(q, *cache, lens, 16, None), fast.decode(q, *cache, lens), fast.decode(), fast.decode(None, *cache, lens, 16, 0.5),
+                fast.prompt(q, *cache, lens, lens, 1, 16, None), fast.prompt(1, 2, 3), fast.gather(*cache, 4, 2), fast.gather(*cache, "4", None),
+                fast.append(q, q, q, q[0], q[0], *cache, lens, None, None), fast.append(None)):
+        assert got is None
+    with pytest.raises(TypeError):
+        fast.entry_points(1, 2)
+    with pytest.raises(ValueError):
+        fast.entry_points(1, 2, 3, 4, 5, 0)

@@ -531,3 +531,52 @@ def test_refusals():
         write(cos=w["cos"].float())
     with pytest.raises(TypeError):
         write(q=w["q"].float())
+
+
+def test_calls_with_and_without_the_fast_module(monkeypatch):
+    """The same outputs, bits and strides of both ways in; what the fast one does not take goes through the other."""
+    assert _lib.fast_calls() is not None
+    c = attention_case([4, 20], [700, 900], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=11)
+    w = write_case([3, 20], [90, 100], 8, 2, 128, 16, torch.float16, torch.float8_e4m3fn, seed=12)
+    lens, starts = i32(c["lens"]), i32(c["starts"])
+    wide = torch.zeros(24, 3, 8, 128, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1] = c["q"]
+
+    def calls():
+        pools = [t.clone() for t in w["cache"]]
+        plain = [t.clone() for t in w["cache"]]
+        q = ops.rope_kv_append_q8(w["q"], w["k"], w["v"], w["cos"], w["sin"], *pools, w["tables"], i32(w["lens"]), row_starts=i32(w["starts"]), max_new=20)
+        ops.kv_append_q8(w["k"], w["v"], *plain, w["tables"], i32(w["lens"]), row_starts=i32(w["starts"]))
+        k, v = ops.kv_gather_dense_q8(*pools, w["tables"][:, :6], 90, torch.float32)
+        return [q, *pools, *plain, k, v, ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], lens, 900),
+                ops.paged_decode_attention_q8(wide[:2, 1], *c["cache"], c["tables"], lens, 900, scale=0.1),
+                ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], lens, 900, scale=1),
+                ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], lens, starts, 20, 900),
+                ops.paged_prompt_attention_q8(wide[:, 1], *c["cache"], c["tables"], lens, starts, 20, 900, scale=0.1)]
+
+    fast = calls()
+    with torch.inference_mode():
+        inference = calls()
+    monkeypatch.setattr(_lib, "fast_calls", lambda: None)
+    for got in (inference, calls()):
+        assert all(a.dtype == b.dtype and a.stride() == b.stride() and torch.equal(raw(a.contiguous()), raw(b.contiguous())) for a, b in zip(fast, got))
+
+
+def test_a_workspace_of_the_callers():
+    c = attention_case([100, 100], [3000, 2000], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=13)
+    lens, starts = i32(c["lens"]), i32(c["starts"])
+    want = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], lens, starts, 100, 3000)
+    one = ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], lens, 3000)
+    for call, need, expect in ((lambda **k: ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], lens, starts, 100, 3000, **k),
+                                ops.prompt_attention_q8_workspace(2, 100, 8, 2, 128, 16, 3000, torch.bfloat16), want),
+                               (lambda **k: ops.paged_decode_attention_q8(c["q"][:2], *c["cache"], c["tables"], lens, 3000, **k),
+                                ops.decode_attention_q8_workspace(2, 8, 2, 128, 16, 3000, torch.bfloat16), one)):
+        assert need > 0
+        ws = torch.full((need + 256,), 0xff, dtype=torch.uint8, device=DEV)
+        assert torch.equal(call(workspace=ws[:need]), expect) and (ws[need:] == 0xff).all()
+        with pytest.raises(_lib.B200LibraryError, match="workspace"):
+            call(workspace=ws[:need - 16])
+        with pytest.raises(_lib.B200LibraryError, match="aligned"):
+            call(workspace=ws[4:need + 4])
+        with pytest.raises(ValueError):
+            call(workspace=ws.cpu())
