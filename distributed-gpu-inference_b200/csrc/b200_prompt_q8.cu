@@ -267,6 +267,19 @@ prompt_kernel(const PromptAttn A) {
     // rows of a token lie D apart, tokens `stride`
     auto place_of = [&](int y, int64_t stride) { return token_of(y) * (stride - static_cast<int64_t>(G) * D) + static_cast<int64_t>(y) * D; };
     auto first_place = [&](int64_t stride) { return (static_cast<int64_t>(w.first) + token0) * stride + static_cast<int64_t>(w.kvh * G + head0) * D; };
+    // scales of 32 groups of keys: the keys', log2 of the values', 1 / the values'; the next ones under way
+    float* scales = reinterpret_cast<float*>(sm + P::kScales) + warp * 96;
+    const int g0 = w.t0 * kGroups;
+    auto page_of = [&](int group) { return group < w.t1 * kGroups ? c.page(w.b, group / per_page) : -1; };
+    auto scales_of = [&](int page, float& ks, float& vs) {
+      ks = vs = 1.f;
+      if (page >= 0) {
+        ks = c.k_scale[static_cast<int64_t>(page) * c.Hkv + w.kvh];
+        vs = q8::max_nan(c.v_scale[static_cast<int64_t>(page) * c.Hkv + w.kvh], q8::kLeastScale);
+      }
+    };
+    int page = page_of(g0 + lane);
+    float ks, vs;
     {
       constexpr int kCh = D / 8, kPer = 32 / kCh, kSteps = 32 / kPer;        // pieces of a row, rows of a step
       const int ch = lane % kCh, r = lane / kCh;
@@ -278,6 +291,8 @@ prompt_kernel(const PromptAttn A) {
         const int y = 32 * warp + u * kPer + r;
         raw[u] = w.row0 + y < rows ? ld_stream16(q + place_of(y, A.q_stride)) : make_int4(0, 0, 0, 0);
       }
+      scales_of(page, ks, vs);        // (under way beside the queries)
+      page = page_of(g0 + 32 + lane);
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
         const T* e = reinterpret_cast<const T*>(&raw[u]);
@@ -301,21 +316,6 @@ prompt_kernel(const PromptAttn A) {
     const float f = factor[tid];
     const int token = row / G, see = min(w.base + min(token, w.n - 1) + 1, w.room);       // keys that the row sees
     const int see_all = __shfl_sync(0xffffffffu, see, 0);                                 // the warp's rows see these
-    // scales of 32 groups of keys: the keys', log2 of the values', 1 / the values'; the next ones under way
-    float* scales = reinterpret_cast<float*>(sm + P::kScales) + warp * 96;
-    const int g0 = w.t0 * kGroups;
-    auto page_of = [&](int group) { return group < w.t1 * kGroups ? c.page(w.b, group / per_page) : -1; };
-    auto scales_of = [&](int page, float& ks, float& vs) {
-      ks = vs = 1.f;
-      if (page >= 0) {
-        ks = c.k_scale[static_cast<int64_t>(page) * c.Hkv + w.kvh];
-        vs = q8::max_nan(c.v_scale[static_cast<int64_t>(page) * c.Hkv + w.kvh], q8::kLeastScale);
-      }
-    };
-    int page = page_of(g0 + lane);
-    float ks, vs;
-    scales_of(page, ks, vs);
-    page = page_of(g0 + 32 + lane);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < my_run; ++i) {
