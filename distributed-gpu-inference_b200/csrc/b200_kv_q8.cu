@@ -466,6 +466,7 @@ int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int
   if (cos_table && D % 2) return fail(B200_ESHAPE, "%s: head size %d cannot turn", name, D);
   if (B == 0 || rows == 0) return 0;
   if (!k || !v || !k_pool || !v_pool || !k_scale || !v_scale || !block_tables || !context_lens || (q_out && !q)) return fail(B200_EINVAL, "%s: null pointer", name);
+  if (k_pool == v_pool || k_scale == v_scale) return fail(B200_EINVAL, "%s: keys and values need pools and scales of their own", name);
   if (!row_starts && rows != B) return fail(B200_EINVAL, "%s: %d rows of %d sequences need row_starts", name, rows, B);
   A.r = Rows{row_starts, context_lens, B, rows};
   A.q = q, A.k = k, A.v = v, A.cos_t = cos_table, A.sin_t = sin_table, A.q_out = q_out;

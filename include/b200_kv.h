@@ -366,6 +366,7 @@ int b200_kv_unpack_layers(void* const* k_pools, void* const* v_pools, int n_laye
 /*
  * A cache in 8 bits.  Pools [max_blocks, Hkv, block_size, D] of codes (B200_CODES_INT8: -127 .. 127; B200_CODES_E4M3: 8-bit floating point, largest
  * 448), and a scale of each page and kv head for its keys and its values, k_scale / v_scale fp32 [max_blocks, Hkv]: a code stands for code * scale.
+ * Codes are numbers and scales not negative, as the append leaves them.
  * The rows of a call are packed: sequence b's new tokens are rows row_starts[b] .. row_starts[b + 1] - 1 (int32 [B + 1], ascending) and
  * the last of its context_lens[b] tokens; rows before row_starts[0] and from row_starts[B] on belong to nobody and are left alone.  Numbers that do not fit one
  * another (rows outside the call's, more than context_lens[b]) make a sequence one without rows.  At most table_cols pages of a sequence are read or

@@ -23,7 +23,7 @@ def test_argument_errors_have_codes_and_words():
     p = 4096      # never read: every call below is refused
 
     def append(**over):
-        a = dict(out=p, os=512, q=p, qs=512, k=p, ks=256, v=p, vs=256, cos=p, sin=p, kp=p, vp=p, s=p, t=p, table=p, stride=4, cols=4, lens=p, starts=p, B=2, rows=5,
+        a = dict(out=p, os=512, q=p, qs=512, k=p, ks=256, v=p, vs=256, cos=p, sin=p, kp=p, vp=p + 16, s=p, t=p + 16, table=p, stride=4, cols=4, lens=p, starts=p, B=2, rows=5,
                  most=5, Hq=4, Hkv=2, D=128, bs=16, blocks=8, codes=3, dtype=2, stream=None)
         a.update(over)
         return lib.b200_rope_kv_append_q8(*a.values()), lib.b200_last_error().decode()
@@ -57,6 +57,7 @@ def test_argument_errors_have_codes_and_words():
     assert decode(longest=4096, dtype=0)[0] == -3
     assert append(rows=0)[0] == 0 and append(starts=None)[0] == -1 and append(sin=None)[0] == -1 and append(cos=None, sin=None)[0] == -1
     assert append(D=33)[0] == -2 and append(q=None)[0] == -1 and append(B=2 ** 30, most=2 ** 30, rows=2 ** 30)[0] == -2
+    assert append(vp=p)[0] == -1 and append(t=p)[0] == -1
     assert gather(n=65)[0] == -1 and gather(n=0)[0] == 0
 
 

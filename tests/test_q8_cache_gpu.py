@@ -527,6 +527,9 @@ def test_refusals():
     for over in (dict(v=w["v"].float()), dict(q_out=w["q"].float())):
         with pytest.raises(TypeError):
             write(**over)
+    for over in (dict(v_pool=k_pool), dict(v_scale=k_scale)):
+        with pytest.raises(_lib.B200LibraryError, match="of their own"):
+            write(**over)
     with pytest.raises(TypeError):
         write(cos=w["cos"].float())
     with pytest.raises(TypeError):
@@ -580,3 +583,70 @@ def test_a_workspace_of_the_callers():
             call(workspace=ws[4:need + 4])
         with pytest.raises(ValueError):
             call(workspace=ws.cpu())
+
+
+def test_nothing_to_do():
+    """No sequences, no rows, no new tokens: empty outputs, and nothing is written."""
+    c = attention_case([3, 20], [90, 100], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=14)
+    none, no_tables, q0 = i32([]), c["tables"][:0], c["q"][:0]
+    before = [raw(t).clone() for t in c["cache"]]
+    assert ops.paged_decode_attention_q8(q0, *c["cache"], no_tables, none, 100).shape == (0, 8, 128)
+    assert ops.paged_prompt_attention_q8(q0, *c["cache"], no_tables, none, i32([0]), 0, 0).shape == (0, 8, 128)
+    assert ops.paged_prompt_attention_q8(q0, *c["cache"], c["tables"], i32([90, 100]), i32([0, 0, 0]), 0, 100).shape == (0, 8, 128)
+    assert [t.shape for t in ops.kv_gather_dense_q8(*c["cache"], no_tables, 5)] == [(0, 2, 5, 128)] * 2
+    assert [t.shape for t in ops.kv_gather_dense_q8(*c["cache"], c["tables"], 0)] == [(2, 2, 0, 128)] * 2
+    kv, angle = q0[:, :2], torch.zeros(0, 128, dtype=torch.bfloat16, device=DEV)
+    assert ops.rope_kv_append_q8(q0, kv, kv, angle, angle, *c["cache"], c["tables"], i32([90, 100]), row_starts=i32([0, 0, 0])).shape == (0, 8, 128)
+    ops.kv_append_q8(kv, kv, *c["cache"], no_tables, none)
+    out = torch.full_like(c["q"], 7.0)
+    ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32([90, 100]), i32([5, 5, 5]), 20, 100, out=out)
+    assert (out == 7).all() and all(torch.equal(a, raw(b)) for a, b in zip(before, c["cache"]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("G,new", [(1, 8), (1, 9), (1, 16), (1, 17), (3, 5), (4, 4), (4, 8), (9, 1), (16, 1), (20, 1), (16, 2), (5, 13), (8, 16), (7, 37)])
+def test_rows_around_the_blocks_of_the_kernels(G, new, codes, dtype):
+    """Rows of a sequence and kv head on both sides of 8, 16, 32, 128 and 256; ragged, with a part of the keys that some rows do not see."""
+    lens = [2000, new, new + 3, 530]
+    counts = [new, new, max(1, new // 2), max(1, new - 1)]
+    for Hkv, D in ((2, 128), (1, 64)):
+        c = attention_case(counts, lens, G * Hkv, Hkv, D, 16, dtype, codes, seed=G * 100 + new, gap=1)
+        want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, True)
+        a, e = c["starts"][0], c["starts"][-1]
+        near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, 2000)[a:e], want[a:e], bound[a:e])
+
+
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("G,new,dtype", [(2, 4, torch.bfloat16), (2, 8, torch.float16), (4, 30, torch.bfloat16), (4, 100, torch.float16), (2, 20, torch.float32)])
+def test_rows_that_do_not_see_a_page_do_not_meet_its_scale(G, new, dtype, bad, which):
+    """The page of the last tokens: earlier tokens' rows come out as they did, the rows behind see no number."""
+    length = 96 + new if new < 16 else 160
+    c = attention_case([new], [length], 2 * G, 2, 128, 16, dtype, torch.int8, seed=15)
+    call = lambda: ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32([length]), i32([0, new]), new, length)  # noqa: E731
+    clean = call()
+    page = (length - 2) // 16
+    c["cache"][which][int(c["tables"][0, page])] = bad
+    got = call()
+    first = max(0, page * 16 - (length - new))      # the first row that sees it
+    assert torch.equal(got[:first], clean[:first])
+    if bad != bad:
+        assert not torch.isfinite(got[first:]).any()
+    else:
+        assert not torch.isfinite(got[first:]).all()
+
+
+def test_numbers_that_are_none_in_a_prompt_reach_later_rows_only():
+    """A key that is not finite, written among others: earlier pages' rows are as without it."""
+    for codes in CODES:
+        w = write_case([40], [40], 8, 2, 128, 16, torch.bfloat16, codes, seed=16)
+        outs = []
+        for bad in (False, True):
+            if bad:
+                w["k"][20, 0, 5], w["v"][37, 1, 9] = float("nan"), float("inf")
+            pools = [t.clone() for t in w["cache"]]
+            q = ops.rope_kv_append_q8(w["q"], w["k"], w["v"], w["cos"], w["sin"], *pools, w["tables"], i32([40]), row_starts=i32([0, 40]))
+            outs.append(ops.paged_prompt_attention_q8(q, *pools, w["tables"], i32([40]), i32([0, 40]), 40, 40))
+        assert torch.equal(outs[0][:16], outs[1][:16]) and torch.equal(outs[0][16:32, 4:], outs[1][16:32, 4:])
+        assert not torch.isfinite(outs[1][16:, :4]).any() and not torch.isfinite(outs[1][32:, 4:]).all()
