@@ -128,6 +128,8 @@ class _TreeStep:
 class PagedDecodeEngine:
     """Decoding of a fixed batch through a chain of shards that live on one CUDA device."""
 
+    kv_cache_dtype: Optional[str] = None      # keys and values in the model's type
+
     def __init__(
         self,
         shards: Sequence[ModelShard],
