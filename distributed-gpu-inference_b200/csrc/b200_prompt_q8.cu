@@ -4,7 +4,7 @@
 // The rows of a sequence and kv head - its new tokens times the G query heads of the group, token by token - go in blocks of 128; a CTA has RB of them and
 // walks the keys up to its last row's in tiles: of 128 for two blocks, of 64 for one.
 //
-//   codes -> fp16   four warps, 16 codes of a key a thread and step: asked for while the tile ahead is turned, turned (exact) and stored in 128-byte swizzled lines, once for all
+//   codes -> fp16   four warps, 16 codes of a key a thread and step: asked for a tile ahead, turned (exact) and stored in 128-byte swizzled lines, once for all
 //                   RB x 128 rows
 //   S = Q K^T       tcgen05.mma, 128 rows x the tile, both operands in shared memory, S in tensor memory; queries in fp16 by a power of two of their own, the largest
 //                   of a row between 2^14 and 2^15.  (64 keys at a time read 6 KB of shared memory in the 32 clocks of 4 KB: the tile of 128.)
@@ -159,13 +159,20 @@ prompt_kernel(const PromptAttn A) {
     };
     const int g0 = w.t0 * kGroups;
     int at = look_up(g0 + lane), later = look_up(g0 + 32 + lane);
-    int4 k[kPasses], v[kPasses];
-    auto load = [&](int i, const uint8_t* pool, int4 (&x)[kPasses]) {
+    int4 k[2][kPasses], v[2][kPasses];       // of a tile, and of the next one
+    auto load = [&](int i, auto odd) {
+      constexpr int kOdd = decltype(odd)::value;
+      if (i > 0 && i % (32 / kGroups) == 0) {
+        at = later;
+        later = look_up(g0 + i * kGroups + 32 + lane);
+      }
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int key = p * kStep + r, row = __shfl_sync(0xffffffffu, at, (i * kGroups + key / kGroup) & 31);
         const bool in = row >= 0 && (w.t0 + i) * kKeys + key < keys;
-        x[p] = in ? ld_stream16(pool + (static_cast<int64_t>(row) + key % kGroup) * D + ch * 16) : make_int4(0, 0, 0, 0);
+        const int64_t e = (static_cast<int64_t>(row) + key % kGroup) * D + ch * 16;
+        k[kOdd][p] = in ? ld_stream16(c.k_pool + e) : make_int4(0, 0, 0, 0);
+        v[kOdd][p] = in ? ld_stream16(c.v_pool + e) : make_int4(0, 0, 0, 0);
       }
     };
     auto store = [&](uint32_t to, const int4 (&x)[kPasses]) {
@@ -185,21 +192,22 @@ prompt_kernel(const PromptAttn A) {
       }
       fence_smem_to_mma();
     };
-    load(0, c.k_pool, k);
-    for (int i = 0; i < run; ++i) {
+    load(0, std::integral_constant<int, 0>{});
+    auto tile = [&](int i, auto odd) {       // (registers have no indexes: the parity is known to the compiler)
+      constexpr int kOdd = decltype(odd)::value;
       const int buf = i % NB;
-      load(i, c.v_pool, v);
       if (i >= NB) bar_wait(bar_ke + 8 * buf, (i / NB - 1) & 1, dead);
-      store(sm0 + P::kK + buf * P::kTile, k);
+      store(sm0 + P::kK + buf * P::kTile, k[kOdd]);
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_k + 8 * buf) : "memory");
-      if ((i + 1) % (32 / kGroups) == 0) {
-        at = later;
-        later = look_up(g0 + (i + 1) * kGroups + 32 + lane);
-      }
-      if (i + 1 < run) load(i + 1, c.k_pool, k);
       if (i >= NB) bar_wait(bar_ve + 8 * buf, (i / NB - 1) & 1, dead);
-      store(sm0 + P::kV + buf * P::kTile, v);
+      store(sm0 + P::kV + buf * P::kTile, v[kOdd]);
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_v + 8 * buf) : "memory");
+    };
+    for (int i = 0; i < run; i += 2) {
+      if (i + 1 < run) load(i + 1, std::integral_constant<int, 1>{});
+      tile(i, std::integral_constant<int, 0>{});
+      if (i + 2 < run) load(i + 2, std::integral_constant<int, 0>{});
+      if (i + 1 < run) tile(i + 1, std::integral_constant<int, 1>{});
     }
   } else if (warp == P::kThreads / 32 - 1) {
     // ---- products ----------------------------------------------------------------------------------------------------------------------------
