@@ -629,21 +629,7 @@ int launch_decode_as(const char* name, const Decode& P, const CUtensorMap& k_map
   kern<<<WARPITEM ? (P.items + kWarps - 1) / kWarps : P.items * P.splits, kWarps * 32, DecodePlan<D>::kSmem, stream>>>(P, k_map, v_map);
   if (int rc = check_launch(name)) return rc;
   if (P.splits == 1) return 0;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(P.items) * static_cast<unsigned>(std::min(P.max_rows, 8 * NB)));
-  cfg.blockDim = dim3(2 * D);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_merge_kernel<T, D, NB>, P);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
-  }
-  return 0;
+  return launch_behind(name, decode_merge_kernel<T, D, NB>, static_cast<unsigned>(P.items) * static_cast<unsigned>(std::min(P.max_rows, 8 * NB)), 2 * D, 0, stream, P);
 }
 
 // rows: of a sequence and kv head at most

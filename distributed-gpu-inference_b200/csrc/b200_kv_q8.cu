@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(128, 5) append_kernel(const Append A, int unit
   constexpr int kCh = D / 16, kRows = 32 / kCh, kPasses = 16 / kRows;        // pieces of a half; rows of a warp's pass
   __shared__ float most_s[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % kCh, r = lane / kCh;
+  q8::wait_for_ahead();
   if (static_cast<int>(blockIdx.x) >= unit_ctas) {
     const unsigned groups = (A.Hq + kHeadsPerWarp - 1) / kHeadsPerWarp;
     const unsigned unit = (blockIdx.x - unit_ctas) * 4 + warp, at = unit / groups;        // (a division of 64 bits costs 500 clocks)
@@ -407,6 +408,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const Gather G, unsigned ti
   constexpr int kSteps = 16 * D / 256;
   const int lane = threadIdx.x & 31;
   const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  q8::wait_for_ahead();
   if (unit >= units) return;
   const unsigned bh = unit / tiles;
   const int tile = static_cast<int>(unit - bh * tiles), b = static_cast<int>(bh / G.c.Hkv), h = static_cast<int>(bh - b * G.c.Hkv), at = tile * 16 / G.c.bs;
@@ -489,8 +491,7 @@ int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int
         const int64_t ctas = (units * warps + 3) / 4, q_ctas = q_out ? (static_cast<int64_t>(rows) * ((Hq + kHeadsPerWarp - 1) / kHeadsPerWarp) + 3) / 4 : 0;
         auto kern = D == 128 ? (warps == 1 ? append_kernel<T, C, 128, 1> : warps == 2 ? append_kernel<T, C, 128, 2> : append_kernel<T, C, 128, 4>)
                              : (warps == 1 ? append_kernel<T, C, 64, 1> : warps == 2 ? append_kernel<T, C, 64, 2> : append_kernel<T, C, 64, 4>);
-        kern<<<static_cast<unsigned>(ctas + q_ctas), 128, 0, s>>>(A, static_cast<int>(ctas));
-        return check_launch(name);
+        return launch_behind(name, kern, static_cast<unsigned>(ctas + q_ctas), 128, 0, s, A, static_cast<int>(ctas));
       }
     }
     append_any_kernel<T, C><<<static_cast<unsigned>(grid), 128, 0, s>>>(A);
@@ -521,8 +522,7 @@ int b200_kv_gather_dense_q8(void* k_out, void* v_out, const void* k_pool, const 
     using C = std::remove_pointer_t<decltype(c)>;
     if (fast) {
       auto kern = D == 128 ? gather_kernel<T, C, 128> : gather_kernel<T, C, 64>;
-      kern<<<static_cast<unsigned>((units + 7) / 8), 256, 0, s>>>(G, static_cast<unsigned>(tiles), static_cast<unsigned>(units));
-      return check_launch(name);
+      return launch_behind(name, kern, static_cast<unsigned>((units + 7) / 8), 256, 0, s, G, static_cast<unsigned>(tiles), static_cast<unsigned>(units));
     }
     gather_any_kernel<T, C><<<static_cast<unsigned>(blocks < kNumSMs * 8 ? blocks : kNumSMs * 8), 256, 0, s>>>(G);
     return check_launch(name);

@@ -2,18 +2,25 @@
 // 128, pages of 16s.  Formula: b200_attn_q8.cu.
 //
 // The rows of a sequence and kv head - its new tokens times the G query heads of the group, token by token - go in blocks of 128; a CTA has RB of them and
-// walks the keys up to its last row's in tiles: of 128 for two blocks, of 64 for one.
+// walks the keys up to its last row's in tiles of 64.
 //
 //   codes -> fp16   four warps, 16 codes of a key a thread and step: asked for a tile ahead, turned (exact) and stored in 128-byte swizzled lines, once for all
 //                   RB x 128 rows
-//   S = Q K^T       tcgen05.mma, 128 rows x the tile, both operands in shared memory, S in tensor memory; queries in fp16 by a power of two of their own, the largest
-//                   of a row between 2^14 and 2^15.  (64 keys at a time read 6 KB of shared memory in the 32 clocks of 4 KB: the tile of 128.)
+//   S = Q K^T       tcgen05.mma, 128 x 64, both operands in shared memory, S in tensor memory, two of them; queries in fp16 by a power of two of their own, the
+//                   largest of a row between 2^14 and 2^15
 //   w               a warp per 32 rows, thread = row: w = 2^(S t + log2 s - m) with the page's scales t and s, so that weights meet bare codes; the sum counts w / s; rounded to
-//                   fp16 into the tensor memory S was in.  One pass: m is the maximum so far less 6, the weights of a tile are made with it while the tile's own maximum is
-//                   found, and made again where that lies more than 15 above m (the first tile's is looked for first); the largest weight lies between 2^6 and 2^15
+//                   fp16 into the tensor memory S was in: by 2^-12 of a weight at most, down to 2^-20 of the largest.  One pass: m is the maximum so far less 6, the weights
+//                   of a tile are made with it while the tile's own maximum is found, and made again where that lies more than 15 above m (the first tile's is looked for
+//                   first); the largest weight lies between 2^6 and 2^15
 //   O += w V        tcgen05.mma, w from tensor memory, O in tensor memory in fp32
 //
 // Few rows: the keys are divided among `splits` CTAs, whose parts prompt_merge_kernel puts together in their order.
+//
+// Bound, for many rows, by shared memory and the latencies of a tile's steps: a tile of 64 keys reads Q once more for each, 6 KB in the 32 clocks in which 4 KB can be read, and the
+// codes go through it twice.  32 heads over 8 of 128, on the device: one sequence of 8192 tokens 548 us, 1.0 PFLOP/s (without turning codes 522, without weights 519); 8 x 2048
+// 374 us, 0.73 PFLOP/s: 7 us of a CTA's 27 go to its beginning and its output; 512 tokens behind 8k 93 us.  What did not pay: tiles of 128 keys with one S (1 x 8192 659 us),
+// one row block and two CTAs an SM (674), CTAs that stay and take one unit after another (8 x 2048 385).  For up to 128 rows the turning is: 64 x 8 tokens of 4 heads behind
+// 2k 115 us where memory would allow 43.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -243,22 +250,15 @@ prompt_kernel(const PromptAttn A) {
     for (int i = 0; i < run; ++i) {
       const bool more = i + 1 < run;
       if (more) bar_wait(bar_k + 8 * ((i + 1) % NB), ((i + 1) / NB) & 1, dead);
-      if constexpr (P::kS == 2) {
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          if (i + 1 < runs[rb]) scores(i + 1, rb);
-        if (more) mma_commit(bar_ke + 8 * ((i + 1) % NB));
-      }
+      for (int rb = 0; rb < RB; ++rb)
+        if (i + 1 < runs[rb]) scores(i + 1, rb);
+      if (more) mma_commit(bar_ke + 8 * ((i + 1) % NB));
       bar_wait(bar_v + 8 * (i % NB), (i / NB) & 1, dead);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
+      for (int rb = 0; rb < RB; ++rb)
         if (i < runs[rb]) outputs(i, rb);
-        if constexpr (P::kS == 1) {        // while one block's weights are made, the other's products run
-          if (i + 1 < runs[rb]) scores(i + 1, rb);
-        }
-      }
       mma_commit(bar_ve + 8 * (i % NB));
-      if (P::kS == 1 && more) mma_commit(bar_ke + 8 * ((i + 1) % NB));
     }
     __syncwarp();
   } else {
@@ -526,22 +526,7 @@ int launch_as(const char* name, const PromptAttn& A, unsigned grid, cudaStream_t
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan<D, RB>::kSmem);
   kern<<<grid, Plan<D, RB>::kThreads, Plan<D, RB>::kSmem, stream>>>(A);
   if (int rc = check_launch(name)) return rc;
-  if (A.splits == 1) return 0;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((A.max_rows + 7) / 8 * A.r.B * A.c.Hkv));
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, prompt_merge_kernel<T, D>, A);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return fail(static_cast<int>(e), "%s: %s", name, cudaGetErrorString(e));
-  }
-  return 0;
+  return A.splits == 1 ? 0 : launch_behind(name, prompt_merge_kernel<T, D>, static_cast<unsigned>((A.max_rows + 7) / 8 * A.r.B * A.c.Hkv), 256, 0, stream, A);
 }
 
 }  // namespace
