@@ -438,6 +438,67 @@ def test_captured_calls_replay_with_new_lengths_and_rows():
         near(one, want, bound, str(l))
 
 
+@pytest.mark.parametrize("bs", [16, 64])
+def test_written_and_read_behind_copies_and_other_streams_calls(bs):
+    """Writing and reading begin while what is ahead ends: behind a copy, a clearing, their own kernels and another stream's, launched and captured."""
+    cases = [write_case([3, 1, 40], [70, 200, 40], 8, 2, 128, bs, torch.bfloat16, torch.int8, seed=s) for s in (11, 12, 13)]
+    a = cases[0]
+    names, tables, lens, starts = ("q", "k", "v", "cos", "sin"), a["tables"], i32(a["lens"]), i32(a["starts"])
+    rows, pools, others = {x: torch.empty_like(a[x]) for x in names}, [torch.empty_like(t) for t in a["cache"]], [torch.empty_like(t) for t in a["cache"]]
+    given, side = {x: torch.empty_like(a[x]) for x in names}, torch.cuda.Stream()
+
+    def calls():
+        for x in names:
+            rows[x].copy_(given[x])
+        for t in (*pools, *others):
+            raw(t).zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.kv_append_q8(rows["k"], rows["v"], *others, tables, lens, row_starts=starts, max_new=40)
+        q = ops.rope_kv_append_q8(rows["q"], rows["k"], rows["v"], rows["cos"], rows["sin"], *pools, tables, lens, row_starts=starts, max_new=40)
+        torch.cuda.current_stream().wait_stream(side)
+        rows["k"].zero_()
+        rows["q"].copy_(q)
+        read = [ops.kv_gather_dense_q8(*c, tables, 40) for c in (others, pools)]
+        one = ops.paged_decode_attention_q8(q[:3], *pools, tables, lens, 200)
+        ops.kv_append_q8(rows["k"], rows["v"], *pools, tables, lens, row_starts=starts, max_new=40)        # (what was read is written over)
+        return [q, *read[0], *read[1], one, rows["q"]]
+
+    def wanted(c):
+        cleared = [torch.zeros_like(t) for t in c["cache"]]
+        with_rope, without = (write_reference(c["k"], c["v"], cos, c["sin"], *cleared, tables, c["lens"], c["starts"]) for cos in (c["cos"], None))
+        co, si, x = c["cos"].float()[:, None], c["sin"].float()[:, None], c["q"].float()
+        q = (x * co + torch.cat((-x[..., 64:], x[..., :64]), -1) * si).to(x.dtype).to(torch.bfloat16)
+        kv = [(pool[tables[:, 0].long()].float() * scale[tables[:, 0].long(), :, None, None])[:, :, :16] for w in (without, with_rope) for pool, scale in ((w[0], w[2]), (w[1], w[3]))]
+        return q, [t.to(torch.bfloat16) for t in kv], attention_reference(q[:3], *with_rope, tables, c["lens"], [0, 1, 2, 3], 128 ** -0.5, True)
+
+    def check(c, got):
+        q, kv, (one, bound) = wanted(c)
+        assert torch.equal(got[0], q) and torch.equal(got[6], q)
+        for x, y in zip(got[1:5], kv):
+            assert torch.equal(x[:, :, :16], y)        # the first page's, or a part of it
+        near(got[5], one, bound)
+
+    def give(c):
+        for x in names:
+            given[x].copy_(c[x])
+
+    for c in cases:
+        give(c)
+        check(c, calls())
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        got = calls()
+    for c in cases:
+        give(c)
+        g.replay()
+        check(c, got)
+        g.replay()
+        g.replay()        # one behind the other
+        check(c, got)
+
+
 def test_two_streams_at_once_and_strided_queries():
     c = attention_case([64, 64], [3000, 2000], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=7)
     lens, starts = i32(c["lens"]), i32(c["starts"])
