@@ -133,10 +133,11 @@ prompt_kernel(const PromptAttn A) {
       init(bar_ve + 8 * b, 1);
     }
     for (int rb = 0; rb < RB; ++rb) {
-      init(bar_q(rb), 128);
+      const int with_rows = max(1, min(128, (rows - w.row0 - rb * kRows + 31) & ~31));        // threads of warps that have rows
+      init(bar_q(rb), with_rows);
       for (int i = 0; i < 2; ++i) {
         init(bar_s(rb, i), 1);
-        init(bar_p(rb, i), 128);
+        init(bar_p(rb, i), with_rows);
         init(bar_o(rb, i), 1);
       }
     }
@@ -261,8 +262,8 @@ prompt_kernel(const PromptAttn A) {
       mma_commit(bar_ve + 8 * (i % NB));
     }
     __syncwarp();
-  } else {
-    // ---- weights: thread = row ---------------------------------------------------------------------------------------------------------------
+  } else if (w.row0 + 32 * warp < rows) {
+    // ---- weights: thread = row (of a warp without rows queries and weights are what memory held: rows of a product are apart) ----------------------
     const int rb = warp >> 2, in_block = tid & 127, row = w.row0 + tid;
     const int my_run = max(min(w.tiles<kKeys>(A, w.row0 + rb * kRows, kRows), w.t1) - w.t0, 0);
     const uint32_t q_at = sm0 + P::kQ + rb * P::kQBlock, tm_row = tm + rb * P::kTm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
