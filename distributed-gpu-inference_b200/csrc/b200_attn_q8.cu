@@ -143,6 +143,10 @@ __global__ void __launch_bounds__(kAnyWarps * 32) attn_any_kernel(const Attn A, 
 //
 // The order of columns inside a product is free as long as both sides agree: a lane's 4 bytes of a key's 16 are its 4 columns there, and its rows of the
 // output are two neighbouring columns.  A byte becomes fp16 as the low byte of 1024 + code + 128 (int8) or by the conversion that the hardware has (e4m3).
+//
+// Bound by memory and its latency: four CTAs an SM (shared memory and registers) keep up to 192 KB under way.  32 heads over 8 of 128, int8, on the device: 64 x 2048 51 us (0.82 of
+// a copy's rate, 512 CTAs on 592 places, SMs are not served alike), 64 x 8192 174 (0.95), 8 x 32768 of 64 heads, e4m3, ragged 74 (0.83); one sequence of 160 tokens 4.9.
+// What did not pay: tiles of 32 tokens and three CTAs an SM (64 x 2048 70), a CTA for each place with equal shares of all tokens (59, and more in most other calls).
 constexpr int kWarps = 4, kTok = 16;
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -671,10 +675,15 @@ int run_decode(const char* name, const Attn& A, int rows, int longest, void* wor
   return dtype == B200_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(name, A, rows, longest, workspace, codes, stream)
                                   : launch_decode<__half>(name, A, rows, longest, workspace, codes, stream);
 }
-// Several tokens per sequence: whether they are few enough for these kernels rather than those of b200_prompt_q8.cu.  us here / there: 64 x 2 tokens of 4 heads at
-// 2k (8 rows) 53 / 119, 64 x 4 (16 rows) 80 / 120, 16 x 9 of one head of 64 at 3k 23 / 56; 32 rows in two blocks: 1 x 8 of 4 heads at 32k 38 / 51, at 4k 14 / 20; 8 x 32 of
-// one head at 8k 85 / 67, 16 x 16 of two 139 / 114.
-bool few_rows(int B, int Hkv, int64_t rows) { return rows <= 16 || (rows <= 32 && static_cast<int64_t>(B) * Hkv <= 32); }
+// Several tokens per sequence: whether they are few enough for these kernels rather than those of b200_prompt_q8.cu, which take 128 rows at once.  Always where one block of
+// up to 16 rows holds them; else while all the blocks' walks are few and short: each reads and turns its sequence's codes again.  us here / there, 8 kv heads, D = 128 but where
+// it says 64: 64 x 2 tokens of 4 heads at 2k (8 rows) 53 / 103, 64 x 4 (16 rows) 81 / 103, 16 x 9 of one head of 64 at 3k 20 / 32; in several blocks: 1 x 16 of 4 heads at
+// 100 tokens 8.5 / 11, at 2k 14 / 17, at 8k 25 / 31, at 32k 80 / 50; 1 x 8 at 32k 39 / 45; 1 x 24 at 8k 32 / 33; 2 x 16 at 8k 38 / 35; 4 x 8 at 4k 27 / 28, at 16k 83 / 55;
+// 4 x 12 at 4k 35 / 31; 32 x 5 at 1k 45 / 31; 8 x 32 of one head at 8k 85 / 57.
+bool few_rows(int B, int Hkv, int64_t rows, int longest) {
+  const int64_t walks = static_cast<int64_t>(B) * Hkv * ((rows + 15) / 16);
+  return rows <= 16 || (walks <= 64 && walks * longest <= 600000);
+}
 
 constexpr int kAnyMostD = 256;
 
@@ -744,7 +753,7 @@ int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const 
 size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
   if (B <= 0 || max_new <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || block_size <= 0 || max_context_len < 0) return 0;
   const int64_t rows = static_cast<int64_t>(max_new) * (Hq / Hkv);
-  const size_t few = few_rows(B, Hkv, rows) && decode_serves(D, block_size, dtype) ? decode_bytes(B, Hkv, D, static_cast<int>(rows), max_context_len) : 0;
+  const size_t few = few_rows(B, Hkv, rows, max_context_len) && decode_serves(D, block_size, dtype) ? decode_bytes(B, Hkv, D, static_cast<int>(rows), max_context_len) : 0;
   return std::max(few, prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype));
 }
 
@@ -764,7 +773,7 @@ int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const 
   P.c = A.c, P.r = A.r, P.out = out, P.q = q, P.q_stride = q_stride, P.Hq = Hq, P.scale = scale;
   if (max_new == 0) return 0;
   const int64_t of_head = static_cast<int64_t>(max_new) * (Hq / Hkv);
-  if (!(flags & B200_ATTN_FORCE_GENERIC) && few_rows(B, Hkv, of_head) && decode_takes(A, static_cast<int>(of_head), max_context_len, dtype))
+  if (!(flags & B200_ATTN_FORCE_GENERIC) && few_rows(B, Hkv, of_head, max_context_len) && decode_takes(A, static_cast<int>(of_head), max_context_len, dtype))
     return run_decode(name, A, static_cast<int>(of_head), max_context_len, workspace, workspace_bytes, codes, dtype, s);
   if (!(flags & B200_ATTN_FORCE_GENERIC) && prompt_q8_serves(P, max_new, max_context_len, dtype)) {
     const size_t need = prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype);

@@ -19,8 +19,10 @@
 // Bound, for many rows, by shared memory and the latencies of a tile's steps: a tile of 64 keys reads Q once more for each, 6 KB in the 32 clocks in which 4 KB can be read, and the
 // codes go through it twice.  32 heads over 8 of 128, on the device: one sequence of 8192 tokens 548 us, 1.0 PFLOP/s (without turning codes 522, without weights 519); 8 x 2048
 // 374 us, 0.73 PFLOP/s: 7 us of a CTA's 27 go to its beginning and its output; 512 tokens behind 8k 93 us.  What did not pay: tiles of 128 keys with one S (1 x 8192 659 us),
-// one row block and two CTAs an SM (674), CTAs that stay and take one unit after another (8 x 2048 385).  For up to 128 rows the turning is: 64 x 8 tokens of 4 heads behind
-// 2k 115 us where memory would allow 43.
+// one row block and two CTAs an SM (674), CTAs that stay and take one unit after another (8 x 2048 385).
+// Up to 128 rows (one block, two CTAs an SM): by the latency of a tile's steps, one tile behind the other, and of its codes: 64 x 8 tokens of 4 heads behind 2k 104 us, where
+// memory would allow 43; 75 without reading codes, 103 without turning them, 109 without weights.  Codes asked for two tiles ahead, or brought to the second level of the cache three
+// tiles ahead, changed nothing; that warps without rows make no weights, 115 -> 104.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -46,7 +48,7 @@ struct Plan {
   static constexpr int kQ = 0, kK = kQ + RB * kQBlock, kV = kK + kBufs * kTile, kScales = kV + kBufs * kTile;       // scales: [warp][3][32] numbers
   static constexpr int kFactor = kScales + 4 * RB * 3 * 32 * 4, kBar = kFactor + RB * kRows * 4, kFlags = kBar + 8 * (4 * kBufs + RB * 7), kEnd = kFlags + 16;
   static constexpr int kSmem = kEnd + 1024;
-  static constexpr int kO = kS * kKeys, kTm = 256;      // columns of a row block's tensor memory: S (one or two) | O
+  static constexpr int kO = kS * kKeys, kTm = 256;      // columns of a row block's tensor memory: S, two | O
   static_assert(RB == 2 ? kSmem <= kMaxSmem : 2 * (kSmem + 1024) <= 228 * 1024, "shared memory");
   static_assert(kO + D <= kTm, "tensor memory");
 };

@@ -678,6 +678,35 @@ def test_rows_around_the_blocks_of_the_kernels(G, new, codes, dtype):
         near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, 2000)[a:e], want[a:e], bound[a:e])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("G,new,D", [(1, 17, 64), (4, 8, 128), (4, 9, 128), (5, 13, 64), (12, 8, 128), (3, 32, 64), (7, 14, 128), (1, 128, 128), (1, 129, 128)])
+def test_rows_of_many_sequences(G, new, D, codes, dtype):
+    """Rows of 17 to 129 in nine sequences of 8 kv heads, more than are taken 16 at a time; one sequence's last page has a scale that is no number."""
+    lens = [700, new, new + 3, 530, 64, 129, 1, 256, 300]
+    counts = [new, new, max(1, new // 2), new - 1, min(new, 60), new, 1, min(new, 33), 16]
+    c = attention_case(counts, lens, G * 8, 8, D, 32, dtype, codes, seed=G * 100 + new, gap=2)
+    a, e, hurt = c["starts"][0], c["starts"][-1], lens[3] // 32
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, True)
+    kept = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(counts), 700)
+    near(kept[a:e], want[a:e], bound[a:e])
+    c["cache"][3][int(c["tables"][3, hurt]), 5] = float("inf")
+    got = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(counts), 700)
+    see = torch.zeros(got.shape[:2], dtype=torch.bool, device=DEV)
+    first = c["starts"][3] + max(0, hurt * 32 - (lens[3] - counts[3]))        # the first row that sees the page
+    see[first:c["starts"][4], 5 * G:6 * G] = True
+    assert not torch.isfinite(got[see]).any() and torch.equal(got[a:e][~see[a:e]], kept[a:e][~see[a:e]])
+
+
+@pytest.mark.parametrize("G,new,context,D", [(4, 16, 2100, 128), (4, 32, 700, 128), (1, 100, 900, 64), (3, 21, 1500, 128), (8, 8, 3000, 64)])
+def test_rows_of_one_sequence_in_several_blocks(G, new, context, D):
+    """Rows of up to 128 of a sequence and kv head, 16 at a time: alone, and more of them than there are keys before."""
+    for lens in ([context], [new]):
+        c = attention_case([new], lens, G * 8, 8, D, 16, torch.bfloat16, torch.int8, seed=G + new)
+        want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, True)
+        near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, context), want, bound)
+
+
 @pytest.mark.parametrize("which", [2, 3])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("G,new,dtype", [(2, 4, torch.bfloat16), (2, 8, torch.float16), (4, 30, torch.bfloat16), (4, 100, torch.float16), (2, 20, torch.float32)])
