@@ -97,13 +97,13 @@ __global__ void __launch_bounds__(128) append_any_kernel(const Append A) {
 }
 
 // ---- 16-bit types, heads of 64 or 128, pages of 16, 32 or 64 -----------------------------------------------------------------------------------
-// A warp per 16 places of a page and kv head's keys or values; the W warps of a page share its maximum.  A lane has 8 columns of the lower and the
+// A warp per P places of a page and kv head's keys or values, 16 of 128 columns, 16 or 32 of 64; the W warps of a page share its maximum.  A lane has 8 columns of the lower and the
 // same 8 of the upper half of several rows, which turn into one another: everything is read once and held as it came until the scale is known; turning it a second
 // time costs less than the registers of the numbers (136: 12 warps an SM, 8 x 2048 rows of 8 heads of 128 in 98 us with their 32 query heads).  Codes that the page holds
-// already are asked for together with its scale, whether or not it grows.  Behind these CTAs, a warp per row and 16 query heads.  Bound by memory and its latency: 8 x 2048 rows of
-// 32 query and 8 kv heads of 128 in 73 us, 0.80 of a copy's rate (keys and values alone 22, 0.72: five CTAs an SM, a page's rows wait for its largest); a token for each of 64
-// sequences 3.6.
-constexpr int kHeadsPerWarp = 16;
+// already are asked for together with its scale, whether or not it grows.  Among or behind these CTAs, those of a warp per row and 16
+// query heads.  Bound by memory and its latency: 8 x 2048 rows of 32 query and 8 kv heads of 128 in 62 us, 0.94 of a copy's rate (keys and values alone 22, 0.71: five CTAs an SM,
+// a page's rows wait for its largest); 16 x 800 of 16 and 16 of 64 in 33, 0.64 (37 with 16 places a warp); a token for each of 64 sequences 3.7.
+constexpr int kHeadsPerWarp = 16, kAppendCTAs = 5;
 
 // Eight numbers as four pairs, two products an instruction.  (Sums stay single: the assembler made one rounding of a pair's product and its sum with a constant,
 // whatever their instructions said.)
@@ -202,15 +202,17 @@ __device__ __forceinline__ uint2 codes_again(uint2 old, float k) {
   return old;
 }
 
-template <typename T, typename C, int D, int W>
-__global__ void __launch_bounds__(128, 5) append_kernel(const Append A, int unit_ctas) {
-  constexpr int kCh = D / 16, kRows = 32 / kCh, kPasses = 16 / kRows;        // pieces of a half; rows of a warp's pass
+// q_step: CTAs of queries lie evenly among the others (CTA i is one where i q_step / 2^64 passes a whole number); 0: behind the kv_ctas others
+template <typename T, typename C, int D, int P, int W>
+__global__ void __launch_bounds__(128, kAppendCTAs) append_kernel(const Append A, unsigned kv_ctas, unsigned long long q_step) {
+  constexpr int kCh = D / 16, kRows = 32 / kCh, kPasses = P / kRows;        // pieces of a half; rows of a warp's pass
   __shared__ float most_s[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % kCh, r = lane / kCh;
   q8::wait_for_ahead();
-  if (static_cast<int>(blockIdx.x) >= unit_ctas) {
+  const unsigned q_cta = q_step ? static_cast<unsigned>(__umul64hi(blockIdx.x, q_step)) : max(blockIdx.x, kv_ctas) - kv_ctas;        // those before this one
+  if (q_step ? __umul64hi(blockIdx.x + 1ull, q_step) != q_cta : blockIdx.x >= kv_ctas) {
     const unsigned groups = (A.Hq + kHeadsPerWarp - 1) / kHeadsPerWarp;
-    const unsigned unit = (blockIdx.x - unit_ctas) * 4 + warp, at = unit / groups;        // (a division of 64 bits costs 500 clocks)
+    const unsigned unit = q_cta * 4 + warp, at = unit / groups;        // (a division of 64 bits costs 500 clocks)
     if (at >= static_cast<unsigned>(A.r.n)) return;
     const int64_t row = at;
     const int h0 = static_cast<int>(unit - at * groups) * kHeadsPerWarp + r;
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(128, 5) append_kernel(const Append A, int unit
     return;
   }
   // ---- keys and values: unit = ((sequence, page), head, keys or values) -----------------------------------------------------------------------
-  const unsigned unit = blockIdx.x * (4 / W) + warp / W, two = unit >> 1, bp = two / A.c.Hkv;
+  const unsigned unit = (blockIdx.x - q_cta) * (4 / W) + warp / W, two = unit >> 1, bp = two / A.c.Hkv;
   const bool values = unit & 1;
   const int h = static_cast<int>(two - bp * A.c.Hkv), b = static_cast<int>(bp / A.pages), lp = static_cast<int>(bp - b * A.pages);
   int t0 = 0, t1 = 0, at = 0, first = 0, held = 0;
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(128, 5) append_kernel(const Append A, int unit
     t0 = static_cast<int>(max(held - base, static_cast<int64_t>(0))), t1 = static_cast<int>(min(context - base, static_cast<int64_t>(A.c.bs)));      // places of the page
   }
   if (W == 1 && t0 >= t1) return;
-  const int my = warp % W * 16 + r;       // the place of the lane's row in the first pass
+  const int my = warp % W * P + r;       // the place of the lane's row in the first pass
   int4 raw[kPasses][2];       // 8 columns of each half; of earlier tokens their codes, both halves' in the first
   const int64_t stride = values ? A.v_stride : A.k_stride, row = static_cast<int64_t>(first) + static_cast<int64_t>(at) * A.c.bs - held + my;       // of the first pass
   const T* rows = static_cast<const T*>(values ? A.v : A.k) + row * stride + h * D + 8 * c;
@@ -440,6 +442,15 @@ __global__ void __launch_bounds__(256) gather_kernel(const Gather G, unsigned ti
   }
 }
 
+// Where the CTAs of queries lie.  Evenly among those of keys and values, whose latencies they fill, where there are more than four times as many as are resident and a
+// fifth of them at least are theirs; else behind the others, which take longer each.  us evenly / behind: 8 x 2048 rows of 32 heads over 8 62 / 74, 16 x 2048 of 8 74 / 90,
+// 8 x 512 17.4 / 18.0, 8 x 256 9.8 / 8.7, 64 x 32 of 64 heads 15.2 / 14.1, 1000 x 1 19.4 / 18.7.
+unsigned long long q_step_of(int64_t kv_ctas, int64_t q_ctas) {
+  const unsigned long long q = q_ctas, all = kv_ctas + q, whole = ~0ull;
+  if (all <= 4ull * kAppendCTAs * kNumSMs || 5 * q < all) return 0;
+  return whole / all * q + (whole % all + 1) * q / all + 1;        // 2^64 q / all, rounded up: less than 1 too much in 2^64 / all products
+}
+
 // calls f(T*, C*) for the types of these ids
 template <typename F>
 int with_types(int dtype, int codes, F f) {
@@ -481,19 +492,19 @@ int b200_rope_kv_append_q8(void* q_out, int64_t q_out_stride, const void* q, int
   const int64_t units = static_cast<int64_t>(B) * A.pages * Hkv * 2, grid = units + (q_out ? rows : 0);
   if (grid * 4 > INT32_MAX) return fail(B200_ESHAPE, "%s: %d sequences of up to %d pages", name, B, A.pages);
   if (grid == 0) return 0;
-  const int warps = block_size / 16;
+  const int places = D == 64 && block_size % 32 == 0 ? 32 : 16, warps = block_size / places;        // of a warp; of a page
   const bool pieces = aligned16(k) && aligned16(v) && aligned16(cos_table) && aligned16(sin_table) && aligned16(k_pool) && aligned16(v_pool) && k_stride % 8 == 0 &&
                       v_stride % 8 == 0 && (!q_out || (aligned16(q) && aligned16(q_out) && q_stride % 8 == 0 && q_out_stride % 8 == 0));
-  const bool fast = dtype != B200_DTYPE_F32 && (D == 64 || D == 128) && block_size % 16 == 0 && (warps == 1 || warps == 2 || warps == 4) && pieces;
+  const bool fast = dtype != B200_DTYPE_F32 && (D == 64 || D == 128) && (block_size == 16 || block_size == 32 || block_size == 64) && pieces;
   return with_types(dtype, codes, [&](auto* t, auto* c) {
     using T = std::remove_pointer_t<decltype(t)>;
     using C = std::remove_pointer_t<decltype(c)>;
     if constexpr (sizeof(T) == 2) {
       if (fast) {
         const int64_t ctas = (units * warps + 3) / 4, q_ctas = q_out ? (static_cast<int64_t>(rows) * ((Hq + kHeadsPerWarp - 1) / kHeadsPerWarp) + 3) / 4 : 0;
-        auto kern = D == 128 ? (warps == 1 ? append_kernel<T, C, 128, 1> : warps == 2 ? append_kernel<T, C, 128, 2> : append_kernel<T, C, 128, 4>)
-                             : (warps == 1 ? append_kernel<T, C, 64, 1> : warps == 2 ? append_kernel<T, C, 64, 2> : append_kernel<T, C, 64, 4>);
-        return launch_behind(name, kern, static_cast<unsigned>(ctas + q_ctas), 128, 0, s, A, static_cast<int>(ctas));
+        auto kern = D == 128 ? (warps == 1 ? append_kernel<T, C, 128, 16, 1> : warps == 2 ? append_kernel<T, C, 128, 16, 2> : append_kernel<T, C, 128, 16, 4>)
+                             : (places == 16 ? append_kernel<T, C, 64, 16, 1> : warps == 1 ? append_kernel<T, C, 64, 32, 1> : append_kernel<T, C, 64, 32, 2>);
+        return launch_behind(name, kern, static_cast<unsigned>(ctas + q_ctas), 128, 0, s, A, static_cast<unsigned>(ctas), q_step_of(ctas, q_ctas));
       }
     }
     append_any_kernel<T, C><<<static_cast<unsigned>(grid), 128, 0, s>>>(A);
