@@ -60,6 +60,11 @@ __device__ __forceinline__ void st16(uint32_t to, uint32_t a, uint32_t b, uint32
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {      // of two pairs of whole numbers
+  asm("max.u16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+  return a;
+}
+
 // What a CTA works on
 struct Work {
   int b, kvh, row0, split;       // sequence, kv head, first row, part of the keys
@@ -271,13 +276,17 @@ prompt_kernel(const PromptAttn A) {
     const uint32_t q_at = sm0 + P::kQ + rb * P::kQBlock, tm_row = tm + rb * P::kTm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     float* factor = reinterpret_cast<float*>(sm + P::kFactor);
     const float sign = A.scale < 0.f ? -1.f : 1.f;
-    // Token of the CTA's row y, from its first row's.  (A division costs 30 instructions; at most 4096 + 256 rows: the product is exact enough.)
-    const int token0 = w.row0 / G, head0 = w.row0 - token0 * G;
-    const float per_head = 1.0f / static_cast<float>(G);
-    auto token_of = [&](int y) { return static_cast<int>((static_cast<float>(head0 + y) + 0.5f) * per_head); };
+    // Queries are read and outputs written by kCh lanes a row, kPer rows at a time: in step u a lane has row `y` + u kPer of the CTA.  Its token, from the CTA's first one: a
+    // division costs 30 instructions; at most 4096 + 256 rows, the product is exact enough.
+    constexpr int kCh = D / 8, kPer = 32 / kCh, kSteps = 32 / kPer;
+    const int ch = lane % kCh, r = lane / kCh, y = 32 * warp + r, token0 = w.row0 / G, head0 = w.row0 - token0 * G;
+    const float per_head = 1.0f / static_cast<float>(G), y_f = static_cast<float>(head0 + y) + 0.5f;
     // rows of a token lie D apart, tokens `stride`
-    auto place_of = [&](int y, int64_t stride) { return token_of(y) * (stride - static_cast<int64_t>(G) * D) + static_cast<int64_t>(y) * D; };
-    auto first_place = [&](int64_t stride) { return (static_cast<int64_t>(w.first) + token0) * stride + static_cast<int64_t>(w.kvh * G + head0) * D; };
+    auto place_of = [&](int u, int64_t stride) {
+      const int token = __float_as_int(__fadd_rd((y_f + static_cast<float>(u * kPer)) * per_head, 0x1p23f)) - 0x4b000000;        // (rounded down: the sum's last digits)
+      return token * (stride - static_cast<int64_t>(G) * D) + (y + u * kPer) * D;
+    };
+    auto first_place = [&](int64_t stride) { return (static_cast<int64_t>(w.first) + token0) * stride + static_cast<int64_t>(w.kvh * G + head0) * D + ch * 8; };
     // scales of 32 groups of keys: the keys', log2 of the values', 1 / the values'; the next ones under way
     float* scales = reinterpret_cast<float*>(sm + P::kScales) + warp * 96;
     const int g0 = w.t0 * kGroups;
@@ -292,31 +301,39 @@ prompt_kernel(const PromptAttn A) {
     int page = page_of(g0 + lane);
     float ks, vs;
     {
-      constexpr int kCh = D / 8, kPer = 32 / kCh, kSteps = 32 / kPer;        // pieces of a row, rows of a step
-      const int ch = lane % kCh, r = lane / kCh;
-      constexpr int kAhead = kSteps < 16 ? kSteps : 16;
-      int4 raw[kAhead];
-      const T* q = static_cast<const T*>(A.q) + first_place(A.q_stride) + ch * 8;
+      int4 raw[kSteps];
+      const T* q = static_cast<const T*>(A.q) + first_place(A.q_stride);
 #pragma unroll
-      for (int u = 0; u < kSteps; ++u) {
-        const int y = 32 * warp + u * kPer + r;
-        raw[u] = w.row0 + y < rows ? ld_stream16(q + place_of(y, A.q_stride)) : make_int4(0, 0, 0, 0);
-      }
+      for (int u = 0; u < kSteps; ++u) raw[u] = w.row0 + y + u * kPer < rows ? ld_stream16(q + place_of(u, A.q_stride)) : make_int4(0, 0, 0, 0);
       scales_of(page, ks, vs);        // (under way beside the queries)
       page = page_of(g0 + 32 + lane);
+      // the rows' largest, two rows a register: magnitudes order like whole numbers
+      uint32_t most[kSteps / 2];
+#pragma unroll
+      for (int u = 0; u < kSteps; u += 2) {
+        uint32_t two[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t* e = reinterpret_cast<const uint32_t*>(&raw[u + x]);
+          two[x] = larger(larger(e[0] & 0x7fff7fffu, e[1] & 0x7fff7fffu), larger(e[2] & 0x7fff7fffu, e[3] & 0x7fff7fffu));
+        }
+        most[u / 2] = larger(__byte_perm(two[0], two[1], 0x5410), __byte_perm(two[0], two[1], 0x7632));
+      }
+#pragma unroll
+      for (int o = kCh / 2; o > 0; o >>= 1) {
+#pragma unroll
+        for (int u = 0; u < kSteps / 2; ++u) most[u] = larger(most[u], __shfl_xor_sync(0xffffffffu, most[u], o));
+      }
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
         const T* e = reinterpret_cast<const T*>(&raw[u]);
-        float x[8], most = 0.f;
-#pragma unroll
-        for (int y = 0; y < 8; ++y) x[y] = Cvt<T>::to_f32(e[y]), most = fmaxf(most, fabsf(x[y]));
-#pragma unroll
-        for (int o = kCh / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const int p = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) - 14;       // most = 2^(p + 14) .. 2^(p + 15)
+        const T row_most = reinterpret_cast<const T*>(&most[u / 2])[u & 1];
+        const int p = max(static_cast<int>(__float_as_uint(Cvt<T>::to_f32(row_most)) >> 23) - 127, -100) - 14;       // the largest = 2^(p + 14) .. 2^(p + 15)
         const float down = __uint_as_float(static_cast<uint32_t>(127 - p) << 23) * sign;
         const int my = u * kPer + r;
-        st16(line(q_at, 32 * (warp & 3) + my, ch, kRows), pack2<__half>(x[0] * down, x[1] * down), pack2<__half>(x[2] * down, x[3] * down),
-             pack2<__half>(x[4] * down, x[5] * down), pack2<__half>(x[6] * down, x[7] * down));
+        st16(line(q_at, 32 * (warp & 3) + my, ch, kRows), pack2<__half>(Cvt<T>::to_f32(e[0]) * down, Cvt<T>::to_f32(e[1]) * down),
+             pack2<__half>(Cvt<T>::to_f32(e[2]) * down, Cvt<T>::to_f32(e[3]) * down), pack2<__half>(Cvt<T>::to_f32(e[4]) * down, Cvt<T>::to_f32(e[5]) * down),
+             pack2<__half>(Cvt<T>::to_f32(e[6]) * down, Cvt<T>::to_f32(e[7]) * down));
         if (ch == 0) factor[32 * warp + my] = fabsf(A.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 + p) << 23);
       }
       fence_smem_to_mma();
@@ -454,15 +471,13 @@ prompt_kernel(const PromptAttn A) {
                pack2<T>(o[u + 6] * k, o[u + 7] * k));
       }
       __syncwarp();
-      constexpr int kCh = D / 8;
-      T* out = static_cast<T*>(A.out) + first_place(static_cast<int64_t>(A.Hq) * D) + lane % kCh * 8;
+      T* out = static_cast<T*>(A.out) + first_place(static_cast<int64_t>(A.Hq) * D);
 #pragma unroll 8
-      for (int u = 0; u < kCh; ++u) {
-        const int r = (lane + u * 32) / kCh, y = 32 * warp + r;
-        if (w.row0 + y < rows) {
+      for (int u = 0; u < kSteps; ++u) {
+        if (w.row0 + y + u * kPer < rows) {
           uint4 x;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(line(q_at, 32 * (warp & 3) + r, lane % kCh, kRows)) : "memory");
-          *reinterpret_cast<uint4*>(out + place_of(y, static_cast<int64_t>(A.Hq) * D)) = x;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(line(q_at, 32 * (warp & 3) + r + u * kPer, ch, kRows)) : "memory");
+          *reinterpret_cast<uint4*>(out + place_of(u, static_cast<int64_t>(A.Hq) * D)) = x;
         }
       }
     }
