@@ -34,6 +34,7 @@ namespace b200 {
 namespace {
 
 using q8::Cache;
+using q8::Divisor;
 using q8::PromptAttn;
 
 constexpr int kRows = 128, kGroup = 16;
@@ -77,24 +78,21 @@ struct Work {
   // tiles up to those of the `count` rows from `from` on
   template <int KEYS>
   __device__ __forceinline__ int tiles(const PromptAttn& A, int from, int count) const {
-    return from < rows ? (min(base + min(n, (from + count - 1) / A.G + 1), room) + KEYS - 1) / KEYS : 0;
+    return from < rows ? (min(base + min(n, A.by_G.of(from + count - 1) + 1), room) + KEYS - 1) / KEYS : 0;
   }
 };
 template <int RB, int KEYS>
 __device__ __forceinline__ Work work_of(const PromptAttn& A, int unit) {
   Work w;
-  w.split = unit % A.splits;
-  unit /= A.splits;
-  w.kvh = unit % A.c.Hkv;
-  unit /= A.c.Hkv;
-  w.b = unit % A.r.B;
-  w.row0 = (A.blocks - 1 - unit / A.r.B) * kRows * RB;       // the longest walks first
+  const int head = A.by_splits.of(unit), b = A.by_heads.of(head), block = A.by_B.of(b);
+  w.split = unit - head * A.splits, w.kvh = head - b * A.c.Hkv, w.b = b - block * A.r.B;
+  w.row0 = (A.blocks - 1 - block) * kRows * RB;       // the longest walks first
   int context;
   A.r.of(w.b, &w.first, &w.n, &context);
   w.base = context - w.n;
   w.room = A.c.keys(context);
   w.rows = min(w.n * A.G, A.max_rows);
-  const int tiles = w.tiles<KEYS>(A, w.row0, kRows * RB), per = (tiles + A.splits - 1) / A.splits;
+  const int tiles = w.tiles<KEYS>(A, w.row0, kRows * RB), per = A.by_splits.of(tiles + A.splits - 1);
   w.t0 = min(w.split * per, tiles);
   w.t1 = min(w.t0 + per, tiles);
   return w;
@@ -121,17 +119,31 @@ prompt_kernel(const PromptAttn A) {
   const int G = A.G;
 
   asm volatile("griddepcontrol.launch_dependents;");
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm0 + P::kFlags), "n"(P::kTm * RB) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   const Work w = work_of<RB, kKeys>(A, blockIdx.x);
   const int run = w.t1 - w.t0, rows = w.rows;
-  if (w.row0 >= rows) return;       // (the whole CTA)
-  if (run == 0) {                   // no keys: nothing but the statistics that say so
-    for (int r = tid; r < kRows * RB; r += P::kThreads) {
-      const int row = w.row0 + r;
-      if (row < rows) A.ml[w.part(A, row)] = make_float2(-INFINITY, 0.f);
-    }
-    return;
+  const bool weighs = warp < P::kSoft / 32 && w.row0 + 32 * warp < rows;        // warps that have rows
+  // Queries are read and outputs written by kCh lanes a row, kPer rows at a time: in step u a lane has row `y` + u kPer of the CTA.  Its token, from the CTA's first one: a
+  // division costs 30 instructions; at most 4096 + 256 rows, the product is exact enough.
+  constexpr int kCh = D / 8, kPer = 32 / kCh, kSteps = 32 / kPer;
+  const int ch = lane % kCh, r = lane / kCh, y = 32 * warp + r, token0 = A.by_G.of(w.row0), head0 = w.row0 - token0 * G;
+  const float per_head = 1.0f / static_cast<float>(G), y_f = static_cast<float>(head0 + y) + 0.5f;
+  // rows of a token lie D apart, tokens `stride`
+  auto place_of = [&](int u, int64_t stride) {
+    const int token = __float_as_int(__fadd_rd((y_f + static_cast<float>(u * kPer)) * per_head, 0x1p23f)) - 0x4b000000;        // (rounded down: the sum's last digits)
+    return token * (stride - static_cast<int64_t>(G) * D) + (y + u * kPer) * D;
+  };
+  auto first_place = [&](int64_t stride) { return (static_cast<int64_t>(w.first) + token0) * stride + static_cast<int64_t>(w.kvh * G + head0) * D + ch * 8; };
+  int4 raw[kSteps];       // (asked for before the barriers stand)
+  if (weighs && run > 0) {
+    const T* q = static_cast<const T*>(A.q) + first_place(A.q_stride);
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) raw[u] = w.row0 + y + u * kPer < rows ? ld_stream16(q + place_of(u, A.q_stride)) : make_int4(0, 0, 0, 0);
   }
-  if (tid == 0) {
+  if (tid == 32) {
     auto init = [](uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); };
     for (int b = 0; b < NB; ++b) {
       init(bar_k + 8 * b, P::kConvert);
@@ -151,15 +163,19 @@ prompt_kernel(const PromptAttn A) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *dead = 0;
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm0 + P::kFlags), "n"(P::kTm * RB) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = __shfl_sync(0xffffffffu, *tm_slot, 0);
   const int per_page = c.bs / kGroup;
+  if (run == 0) {       // no keys, or no rows (the whole CTA): nothing but the statistics that say so
+    for (int x = tid; x < kRows * RB; x += P::kThreads) {
+      const int row = w.row0 + x;
+      if (row < rows) A.ml[w.part(A, row)] = make_float2(-INFINITY, 0.f);
+    }
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(P::kTm * RB));
+    return;
+  }
 
   if (warp >= P::kSoft / 32 && warp < (P::kSoft + P::kConvert) / 32) {
     // ---- codes to fp16 -----------------------------------------------------------------------------------------------------------------------
@@ -169,8 +185,8 @@ prompt_kernel(const PromptAttn A) {
     // the pool's rows of 32 groups of 16 keys, a lane each, the next ones under way; -1: zeros
     auto look_up = [&](int group) -> int {
       if (group >= w.t1 * kGroups) return -1;
-      const int page = c.page(w.b, group / per_page);
-      return page < 0 ? -1 : (page * c.Hkv + w.kvh) * c.bs + group % per_page * kGroup;
+      const int place = A.by_page.of(group), page = c.page(w.b, place);
+      return page < 0 ? -1 : (page * c.Hkv + w.kvh) * c.bs + (group - place * per_page) * kGroup;
     };
     const int g0 = w.t0 * kGroups;
     int at = look_up(g0 + lane), later = look_up(g0 + 32 + lane);
@@ -269,28 +285,17 @@ prompt_kernel(const PromptAttn A) {
       mma_commit(bar_ve + 8 * (i % NB));
     }
     __syncwarp();
-  } else if (w.row0 + 32 * warp < rows) {
+  } else if (weighs) {
     // ---- weights: thread = row (of a warp without rows queries and weights are what memory held: rows of a product are apart) ----------------------
     const int rb = warp >> 2, in_block = tid & 127, row = w.row0 + tid;
     const int my_run = max(min(w.tiles<kKeys>(A, w.row0 + rb * kRows, kRows), w.t1) - w.t0, 0);
     const uint32_t q_at = sm0 + P::kQ + rb * P::kQBlock, tm_row = tm + rb * P::kTm + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     float* factor = reinterpret_cast<float*>(sm + P::kFactor);
     const float sign = A.scale < 0.f ? -1.f : 1.f;
-    // Queries are read and outputs written by kCh lanes a row, kPer rows at a time: in step u a lane has row `y` + u kPer of the CTA.  Its token, from the CTA's first one: a
-    // division costs 30 instructions; at most 4096 + 256 rows, the product is exact enough.
-    constexpr int kCh = D / 8, kPer = 32 / kCh, kSteps = 32 / kPer;
-    const int ch = lane % kCh, r = lane / kCh, y = 32 * warp + r, token0 = w.row0 / G, head0 = w.row0 - token0 * G;
-    const float per_head = 1.0f / static_cast<float>(G), y_f = static_cast<float>(head0 + y) + 0.5f;
-    // rows of a token lie D apart, tokens `stride`
-    auto place_of = [&](int u, int64_t stride) {
-      const int token = __float_as_int(__fadd_rd((y_f + static_cast<float>(u * kPer)) * per_head, 0x1p23f)) - 0x4b000000;        // (rounded down: the sum's last digits)
-      return token * (stride - static_cast<int64_t>(G) * D) + (y + u * kPer) * D;
-    };
-    auto first_place = [&](int64_t stride) { return (static_cast<int64_t>(w.first) + token0) * stride + static_cast<int64_t>(w.kvh * G + head0) * D + ch * 8; };
     // scales of 32 groups of keys: the keys', log2 of the values', 1 / the values'; the next ones under way
     float* scales = reinterpret_cast<float*>(sm + P::kScales) + warp * 96;
     const int g0 = w.t0 * kGroups;
-    auto page_of = [&](int group) { return group < w.t1 * kGroups ? c.page(w.b, group / per_page) : -1; };
+    auto page_of = [&](int group) { return group < w.t1 * kGroups ? c.page(w.b, A.by_page.of(group)) : -1; };
     auto scales_of = [&](int page, float& ks, float& vs) {
       ks = vs = 1.f;
       if (page >= 0) {
@@ -301,10 +306,6 @@ prompt_kernel(const PromptAttn A) {
     int page = page_of(g0 + lane);
     float ks, vs;
     {
-      int4 raw[kSteps];
-      const T* q = static_cast<const T*>(A.q) + first_place(A.q_stride);
-#pragma unroll
-      for (int u = 0; u < kSteps; ++u) raw[u] = w.row0 + y + u * kPer < rows ? ld_stream16(q + place_of(u, A.q_stride)) : make_int4(0, 0, 0, 0);
       scales_of(page, ks, vs);        // (under way beside the queries)
       page = page_of(g0 + 32 + lane);
       // the rows' largest, two rows a register: magnitudes order like whole numbers
@@ -342,7 +343,7 @@ prompt_kernel(const PromptAttn A) {
       __syncwarp();
     }
     const float f = factor[tid];
-    const int token = row / G, see = min(w.base + min(token, w.n - 1) + 1, w.room);       // keys that the row sees
+    const int token = A.by_G.of(row), see = min(w.base + min(token, w.n - 1) + 1, w.room);       // keys that the row sees
     const int see_all = __shfl_sync(0xffffffffu, see, 0);                                 // the warp's rows see these
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -566,6 +567,7 @@ bool prompt_q8_serves(const PromptAttn& A, int max_new, int longest, int dtype) 
 int prompt_q8(const char* name, PromptAttn A, int max_new, int longest, void* workspace, int codes, int dtype, cudaStream_t stream) {
   const Cut x = cut_of(A.r.B, max_new, A.Hq, A.c.Hkv, longest);
   A.G = A.Hq / A.c.Hkv, A.blocks = x.blocks, A.splits = x.splits, A.max_rows = max_new * A.G;
+  A.by_G = Divisor::by(A.G), A.by_splits = Divisor::by(A.splits), A.by_heads = Divisor::by(A.c.Hkv), A.by_B = Divisor::by(A.r.B), A.by_page = Divisor::by(A.c.bs / kGroup);
   // [sequence][kv head][row][part]: statistics, then outputs
   A.ml = static_cast<float2*>(workspace);
   A.acc = reinterpret_cast<float*>(A.ml + static_cast<int64_t>(A.r.B) * A.c.Hkv * A.max_rows * x.splits);
