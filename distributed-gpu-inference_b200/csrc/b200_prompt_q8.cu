@@ -16,13 +16,14 @@
 //
 // Few rows: the keys are divided among `splits` CTAs, whose parts prompt_merge_kernel puts together in their order.
 //
-// Bound, for many rows, by shared memory and the latencies of a tile's steps: a tile of 64 keys reads Q once more for each, 6 KB in the 32 clocks in which 4 KB can be read, and the
-// codes go through it twice.  32 heads over 8 of 128, on the device: one sequence of 8192 tokens 548 us, 1.0 PFLOP/s (without turning codes 522, without weights 519); 8 x 2048
-// 374 us, 0.73 PFLOP/s: 7 us of a CTA's 27 go to its beginning and its output; 512 tokens behind 8k 93 us.  What did not pay: tiles of 128 keys with one S (1 x 8192 659 us),
-// one row block and two CTAs an SM (674), CTAs that stay and take one unit after another (8 x 2048 385).
-// Up to 128 rows (one block, two CTAs an SM): by the latency of a tile's steps, one tile behind the other, and of its codes: 64 x 8 tokens of 4 heads behind 2k 104 us, where
-// memory would allow 43; 75 without reading codes, 103 without turning them, 109 without weights.  Codes asked for two tiles ahead, or brought to the second level of the cache three
-// tiles ahead, changed nothing; that warps without rows make no weights, 115 -> 104.
+// Bound, for many rows, by the latencies of a tile's steps: of a tile's 2000 clocks the warps that make weights are busy 1900 (the exponential unit 1000), those that turn codes 1800, the tensor
+// cores and the shared memory that feeds them some 1300 (a tile of 64 keys reads Q once more for each, 6 KB in the 32 clocks in which 4 KB can be read).  32 heads over 8 of 128, on the
+// device: one sequence of 8192 tokens 537 us, 1.02 PFLOP/s; 8 x 2048 361 us, 0.76 PFLOP/s: 6 us of a CTA's 26 go to its beginning and its output (queries are there after 3, the first
+// weights after 6); 512 tokens behind 8k 93 us.  What did not pay: tiles of 128 keys with one S (1 x 8192 659 us when this took 583), one row block and two CTAs an SM (674), CTAs that stay
+// and take one unit after another (8 x 2048 385, then the same), twice the warps for codes (362), two threads a row (384 - 401), S in smaller pieces (392, then 374).
+// Up to 128 rows (one block, two CTAs an SM): by the latency of a tile's steps, one tile behind the other, and of its codes: 64 x 8 tokens of 4 heads behind 2k 100 us, where
+// memory would allow 43; without reading codes a quarter less, without turning them or without weights the same.  Codes asked for two tiles ahead, or brought to the second level of
+// the cache three tiles ahead, changed nothing; that warps without rows make no weights, 115 -> 104.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
