@@ -139,6 +139,12 @@ def test_single_tokens_share_and_grow_a_pages_scale(D, bs, codes):
     assert all(torch.equal(raw(a), raw(b)) for a, b in zip(none["cache"], before))
 
 
+@pytest.mark.parametrize("D,bs,B", [(128, 16, 10), (64, 32, 12), (64, 64, 12)])
+def test_queries_among_keys_and_values(D, bs, B):
+    """So many rows that the CTAs of queries lie among the others; the last ones of both kinds included."""
+    check_write(write_case([700] * (B - 1) + [691], [700 + 3 * b for b in range(B - 1)] + [691], 16, 8, D, bs, torch.bfloat16, torch.int8, seed=D + bs, padding=5))
+
+
 @pytest.mark.parametrize("D", [128, 48])
 def test_token_by_token_like_the_definition(D):
     """A sequence of 40 tokens, one at a time, then the same in portions: each step is the definition's; the values it ends with are the tokens' up to half a
@@ -696,6 +702,19 @@ def test_rows_of_many_sequences(G, new, D, codes, dtype):
     first = c["starts"][3] + max(0, hurt * 32 - (lens[3] - counts[3]))        # the first row that sees the page
     see[first:c["starts"][4], 5 * G:6 * G] = True
     assert not torch.isfinite(got[see]).any() and torch.equal(got[a:e][~see[a:e]], kept[a:e][~see[a:e]])
+
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("G,new", [(3, 70), (5, 9), (6, 3)])
+def test_pages_of_48_and_three_kv_heads(G, new, D, dtype):
+    """Numbers that are no powers of two everywhere: pages, heads, sequences, query heads of a kv head, parts."""
+    lens = [new, 1000, 47 + new, 48 + new, 333]
+    counts = [new, new, new - 1, new, 1]
+    c = attention_case(counts, lens, G * 3, 3, D, 48, dtype, torch.int8, seed=G + D)
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, True)
+    near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, 1000), want, bound)
+    want, bound = attention_reference(c["q"][:5], *c["cache"], c["tables"], lens, list(range(6)), D ** -0.5, True)
+    near(ops.paged_decode_attention_q8(c["q"][:5], *c["cache"], c["tables"], i32(lens), 1000), want, bound)
 
 
 @pytest.mark.parametrize("G,new,context,D", [(4, 16, 2100, 128), (4, 32, 700, 128), (1, 100, 900, 64), (3, 21, 1500, 128), (8, 8, 3000, 64)])
