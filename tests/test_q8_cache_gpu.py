@@ -412,6 +412,29 @@ def test_bad_tables_read_zeros_and_short_tables_end_the_context():
     near(ops.paged_decode_attention_q8(one["q"], *one["cache"], one["tables"], i32(lens), 100), want, bound)
 
 
+@pytest.mark.parametrize("codes", CODES)
+def test_offsets_past_32_bits(codes):
+    """Pages behind the first 2^31 numbers of a pool, and behind 2^32: as in a small one."""
+    pages, Hkv, bs, D = (2 ** 32 + 2 ** 28) // (8 * 16 * 128), 8, 16, 128
+    shift = pages - 40
+    c = write_case([50, 3], [50, 200], 16, Hkv, D, bs, torch.bfloat16, codes, seed=31)
+    small = [t.clone() for t in c["cache"]]
+    n = small[0].shape[0]
+    big = [torch.empty((pages, *t.shape[1:]), dtype=t.dtype, device=DEV) for t in small]
+    for past in (shift, 2 ** 31 // (Hkv * bs * D) - n // 2):
+        for b, t in zip(big, c["cache"]):
+            raw(b)[past:past + n] = raw(t)
+        far = torch.where(c["tables"] >= 0, c["tables"] + past, -1)
+        outs = []
+        for pools, tables in ((big, far), ([t.clone() for t in c["cache"]], c["tables"])):
+            q = ops.rope_kv_append_q8(c["q"], c["k"], c["v"], c["cos"], c["sin"], *pools, tables, i32(c["lens"]), row_starts=i32(c["starts"]), max_new=50)
+            outs.append((q, *ops.kv_gather_dense_q8(*pools, tables, 64), ops.paged_decode_attention_q8(q[:2], *pools, tables, i32(c["lens"]), 200),
+                         ops.paged_prompt_attention_q8(q, *pools, tables, i32(c["lens"]), i32(c["starts"]), 50, 200),
+                         ops.paged_prompt_attention_q8(q, *pools, tables, i32(c["lens"]), i32(c["starts"]), 50, 200, flags=ops.ATTN_FORCE_GENERIC)))
+        for a, b in zip(*outs):
+            assert torch.equal(a, b)
+
+
 def test_lengths_that_do_not_fit_give_no_rows():
     c = attention_case([3, 20], [90, 100], 8, 2, 128, 16, torch.bfloat16, torch.int8, seed=5)
     for lens, starts in (([90, 10], [0, 3, 23]), ([90, 100], [0, 3, 10 ** 6]), ([90, 100], [0, 3, -5])):
