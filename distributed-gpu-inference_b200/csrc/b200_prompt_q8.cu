@@ -525,6 +525,11 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptAttn A) {
 // How a call is cut
 struct Cut {
   int row_blocks, blocks, splits;      // of a CTA; CTAs of a sequence and kv head; parts of the keys
+  // The workspace: statistics of [sequence][kv head][row][part], then outputs of the same.  The statistics' number is brought to an even one: outputs are stored 16 bytes at once
+  size_t statistics(int B, int Hkv, int64_t max_rows) const { return (static_cast<size_t>(B) * Hkv * max_rows * splits + 1) / 2 * 2; }
+  size_t bytes(int B, int Hkv, int64_t max_rows, int D) const {
+    return splits == 1 ? 0 : statistics(B, Hkv, max_rows) * sizeof(float2) + static_cast<size_t>(B) * Hkv * max_rows * splits * D * sizeof(float);
+  }
 };
 Cut cut_of(int B, int max_new, int Hq, int Hkv, int longest) {
   const int64_t rows = static_cast<int64_t>(max_new) * (Hq / Hkv);
@@ -553,8 +558,7 @@ int launch_as(const char* name, const PromptAttn& A, unsigned grid, cudaStream_t
 
 size_t prompt_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int bs, int longest, int dtype) {
   if (B <= 0 || max_new <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || bs <= 0 || longest < 0 || !serves(Hq, Hkv, D, bs, dtype)) return 0;
-  const Cut x = cut_of(B, max_new, Hq, Hkv, longest);
-  return x.splits > 1 ? static_cast<size_t>(B) * max_new * Hq * x.splits * (D + 2) * sizeof(float) : 0;
+  return cut_of(B, max_new, Hq, Hkv, longest).bytes(B, Hkv, static_cast<int64_t>(max_new) * (Hq / Hkv), D);
 }
 
 bool prompt_q8_serves(const PromptAttn& A, int max_new, int longest, int dtype) {
@@ -569,9 +573,8 @@ int prompt_q8(const char* name, PromptAttn A, int max_new, int longest, void* wo
   const Cut x = cut_of(A.r.B, max_new, A.Hq, A.c.Hkv, longest);
   A.G = A.Hq / A.c.Hkv, A.blocks = x.blocks, A.splits = x.splits, A.max_rows = max_new * A.G;
   A.by_G = Divisor::by(A.G), A.by_splits = Divisor::by(A.splits), A.by_heads = Divisor::by(A.c.Hkv), A.by_B = Divisor::by(A.r.B), A.by_page = Divisor::by(A.c.bs / kGroup);
-  // [sequence][kv head][row][part]: statistics, then outputs
   A.ml = static_cast<float2*>(workspace);
-  A.acc = reinterpret_cast<float*>(A.ml + static_cast<int64_t>(A.r.B) * A.c.Hkv * A.max_rows * x.splits);
+  A.acc = reinterpret_cast<float*>(A.ml + x.statistics(A.r.B, A.c.Hkv, A.max_rows));
   const unsigned grid = static_cast<unsigned>(A.r.B * A.c.Hkv * x.blocks * x.splits);
   auto go = [&](auto* t, auto* c, auto d) {
     using T = std::remove_pointer_t<decltype(t)>;

@@ -76,3 +76,20 @@ def test_the_fast_module_leaves_what_is_not_plain_to_the_checks():
         fast.entry_points(1, 2)
     with pytest.raises(ValueError):
         fast.entry_points(1, 2, 3, 4, 5, 0)
+
+
+ODD_PARTS = [(1, 1301, 9, 3, 64, 1301), (3, 101, 5, 1, 128, 1301), (1, 207, 5, 1, 128, 2255), (9, 127, 1, 1, 128, 1400), (1, 205, 5, 1, 128, 1434), (1, 801, 5, 1, 128, 4801),
+             (5, 193, 1, 1, 64, 1410), (23, 33, 1, 1, 64, 2300), (5, 33, 3, 1, 128, 20033)]
+
+
+@pytest.mark.parametrize("B,new,Hq,Hkv,D,longest", ODD_PARTS + [(1, 206, 5, 1, 128, 2255), (2, 105, 5, 1, 64, 1301), (3, 101, 4, 2, 128, 1301)])
+def test_outputs_of_parts_begin_at_a_multiple_of_16_bytes(B, new, Hq, Hkv, D, longest):
+    """The workspace of several tokens in parts: statistics of 8 bytes for each row and part, brought to whole 16 bytes, then the parts' outputs, stored 16 bytes at once."""
+    lib = _lib.load()
+    for block_size in (16, 48):
+        need = lib.b200_paged_prompt_attn_q8_workspace(B, new, Hq, Hkv, D, block_size, longest, 2)
+        rows = B * new * Hq
+        parts = need // (rows * (8 + 4 * D))
+        n = rows * parts
+        assert parts > 1 and (n % 2 == 1) == ((B, new, Hq, Hkv, D, longest) in ODD_PARTS), parts
+        assert need == (n + 1) // 2 * 16 + n * D * 4

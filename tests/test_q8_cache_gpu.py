@@ -782,3 +782,22 @@ def test_numbers_that_are_none_in_a_prompt_reach_later_rows_only():
             outs.append(ops.paged_prompt_attention_q8(q, *pools, w["tables"], i32([40]), i32([0, 40]), 40, 40))
         assert torch.equal(outs[0][:16], outs[1][:16]) and torch.equal(outs[0][16:32, 4:], outs[1][16:32, 4:])
         assert not torch.isfinite(outs[1][16:, :4]).any() and not torch.isfinite(outs[1][32:, 4:]).all()
+
+
+@pytest.mark.parametrize("codes,dtype", [(torch.int8, torch.bfloat16), (torch.float8_e4m3fn, torch.float16)])
+@pytest.mark.parametrize("B,new,Hq,Hkv,D,context", [(1, 1301, 9, 3, 64, 0), (3, 101, 5, 1, 128, 1200), (1, 207, 5, 1, 128, 2048), (9, 127, 1, 1, 128, 1273), (5, 193, 1, 1, 64, 1217),
+                                                    (23, 33, 1, 1, 64, 2267), (5, 33, 3, 1, 128, 20000)])
+def test_an_odd_number_of_parts(B, new, Hq, Hkv, D, context, codes, dtype):
+    """Sequences, heads, rows and parts whose product is odd, in one row block and in two: the parts' outputs lie behind an odd number of statistics.  Scratch of the allocator,
+    and the caller's with something behind it."""
+    lens = [new + context] + [new + context - 7 * b for b in range(1, B)]
+    need = ops.prompt_attention_q8_workspace(B, new, Hq, Hkv, D, 16, lens[0], dtype)
+    rows = B * new * Hq
+    assert need // (rows * (8 + 4 * D)) * rows % 2 == 1 and need % 16 == 0
+    c = attention_case([new] + [new - 2 * (b % 9) for b in range(1, B)], lens, Hq, Hkv, D, 16, dtype, codes, seed=new)
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, True)
+    call = lambda **k: ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, lens[0], **k)  # noqa: E731
+    got = call()
+    near(got, want, bound)
+    ws = torch.full((need + 256,), 0xff, dtype=torch.uint8, device=DEV)
+    assert torch.equal(call(workspace=ws[:need]), got) and (ws[need:] == 0xff).all()
