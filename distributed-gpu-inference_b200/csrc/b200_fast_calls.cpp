@@ -1,6 +1,7 @@
 // The calls of the cache in 8 bits (ops.py) for plain arguments: their checks and allocations in C++ instead of some eighty Python operations, which took 10 of a small
 // call's 14 us.  A function here returns None where anything is out of the ordinary - another type, shape or layout than the call documents, another device than
 // the current one, a refusal by the library - and then the caller goes through the checks in Python, which say what it is.  The library's entry points come as addresses.
+// Pointers are taken while the interpreter's lock is held: tensors without storage (torch.vmap's, torch.func's) throw where theirs is asked for.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -77,6 +78,15 @@ struct Plain {
     *apart = n > 1 ? t->stride(0) : t->size(1) * D;
     return *apart >= 0;
   }
+  // of pools, scales and tables; may throw
+  void *kp = nullptr, *vp = nullptr;
+  float *ks = nullptr, *vs = nullptr;
+  const int32_t* rows_of_tables = nullptr;
+  void pointers() {
+    kp = k_pool->data_ptr(), vp = v_pool->data_ptr(), ks = static_cast<float*>(k_scale->data_ptr()), vs = static_cast<float*>(v_scale->data_ptr());
+    rows_of_tables = whole_numbers(tables);
+  }
+  static const int32_t* whole_numbers(const at::Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
   at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType kind) const { return at::empty(sizes, k_pool->options().dtype(kind)); }
   void* stream() const { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(); }
 };
@@ -101,13 +111,15 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t count) {
   int most = static_cast<int>(n);
   if (a[12] != Py_None && !whole_number(a[12], &most)) Py_RETURN_NONE;
   at::Tensor out = c.fresh(q->sizes(), kind);
-  void* stream = c.stream();
+  c.pointers();
+  void *op = out.data_ptr(), *stream = c.stream();
+  const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr(), *cp = cos->data_ptr(), *sp = sin->data_ptr();
+  const int32_t *contexts = c.whole_numbers(lens), *firsts = c.whole_numbers(starts);
+  const int Hq = static_cast<int>(q->size(1));
   int rc;
   Py_BEGIN_ALLOW_THREADS;
-  rc = append_fn(out.data_ptr(), q->size(1) * c.D, q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, cos->data_ptr(), sin->data_ptr(), c.k_pool->data_ptr(),
-                 c.v_pool->data_ptr(), static_cast<float*>(c.k_scale->data_ptr()), static_cast<float*>(c.v_scale->data_ptr()), static_cast<const int32_t*>(c.tables->data_ptr()),
-                 c.stride, c.cols, static_cast<const int32_t*>(lens->data_ptr()), starts ? static_cast<const int32_t*>(starts->data_ptr()) : nullptr, c.B, static_cast<int>(n), most,
-                 static_cast<int>(q->size(1)), c.heads, c.D, c.bs, c.blocks, c.codes, dtype, stream);
+  rc = append_fn(op, static_cast<int64_t>(Hq) * c.D, qp, qs, kp, ks, vp, vs, cp, sp, c.kp, c.vp, c.ks, c.vs, c.rows_of_tables, c.stride, c.cols, contexts, firsts, c.B, static_cast<int>(n), most, Hq,
+                 c.heads, c.D, c.bs, c.blocks, c.codes, dtype, stream);
   Py_END_ALLOW_THREADS;
   if (rc != 0) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
@@ -122,12 +134,11 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (count != 7 || !c.cache(a) || !whole_number(a[5], &n) || !whole_number(a[6], &dtype) || n > static_cast<int64_t>(c.cols) * c.bs) Py_RETURN_NONE;
   const at::ScalarType kind = dtype == B200_DTYPE_F16 ? at::kHalf : dtype == B200_DTYPE_BF16 ? at::kBFloat16 : at::kFloat;
   at::Tensor k = c.fresh({c.B, c.heads, n, c.D}, kind), v = c.fresh({c.B, c.heads, n, c.D}, kind);
-  void* stream = c.stream();
+  c.pointers();
+  void *k_out = k.data_ptr(), *v_out = v.data_ptr(), *stream = c.stream();
   int rc;
   Py_BEGIN_ALLOW_THREADS;
-  rc = gather_fn(k.data_ptr(), v.data_ptr(), c.k_pool->data_ptr(), c.v_pool->data_ptr(), static_cast<const float*>(c.k_scale->data_ptr()),
-                 static_cast<const float*>(c.v_scale->data_ptr()), static_cast<const int32_t*>(c.tables->data_ptr()), c.stride, c.cols, c.B, n, c.heads, c.D, c.bs, c.blocks, c.codes,
-                 dtype, stream);
+  rc = gather_fn(k_out, v_out, c.kp, c.vp, c.ks, c.vs, c.rows_of_tables, c.stride, c.cols, c.B, n, c.heads, c.D, c.bs, c.blocks, c.codes, dtype, stream);
   Py_END_ALLOW_THREADS;
   if (rc != 0) Py_RETURN_NONE;
   PyObject* pair = PyTuple_New(2);
@@ -158,16 +169,15 @@ PyObject* attention(PyObject* const* a, Py_ssize_t count, bool several) {
   at::Tensor out = c.fresh(q->sizes(), q->scalar_type()), workspace;
   const size_t need = several ? prompt_ws_fn(c.B, most, Hq, c.heads, c.D, c.bs, longest, dtype) : decode_ws_fn(c.B, Hq, c.heads, c.D, c.bs, longest, dtype);
   if (need) workspace = c.fresh({static_cast<int64_t>(need)}, at::kByte);
-  void *stream = c.stream(), *ws = need ? workspace.data_ptr() : nullptr;
-  const float *ks = static_cast<const float*>(c.k_scale->data_ptr()), *vs = static_cast<const float*>(c.v_scale->data_ptr());
-  const int32_t *tables = static_cast<const int32_t*>(c.tables->data_ptr()), *contexts = static_cast<const int32_t*>(lens->data_ptr());
+  c.pointers();
+  void *op = out.data_ptr(), *stream = c.stream(), *ws = need ? workspace.data_ptr() : nullptr;
+  const void* qp = q->data_ptr();
+  const int32_t *contexts = c.whole_numbers(lens), *firsts = c.whole_numbers(starts);
   int rc;
   Py_BEGIN_ALLOW_THREADS;
-  rc = several ? prompt_fn(out.data_ptr(), q->data_ptr(), qs, c.k_pool->data_ptr(), c.v_pool->data_ptr(), ks, vs, tables, c.stride, c.cols, contexts,
-                           static_cast<const int32_t*>(starts->data_ptr()), c.B, static_cast<int>(n), most, Hq, c.heads, c.D, c.bs, c.blocks, scale, longest, ws, need, c.codes, dtype, 0u,
-                           stream)
-               : decode_fn(out.data_ptr(), q->data_ptr(), qs, c.k_pool->data_ptr(), c.v_pool->data_ptr(), ks, vs, tables, c.stride, c.cols, contexts, c.B, Hq, c.heads, c.D, c.bs, c.blocks,
-                           scale, longest, ws, need, c.codes, dtype, 0u, stream);
+  rc = several ? prompt_fn(op, qp, qs, c.kp, c.vp, c.ks, c.vs, c.rows_of_tables, c.stride, c.cols, contexts, firsts, c.B, static_cast<int>(n), most, Hq, c.heads, c.D, c.bs, c.blocks, scale, longest,
+                           ws, need, c.codes, dtype, 0u, stream)
+               : decode_fn(op, qp, qs, c.kp, c.vp, c.ks, c.vs, c.rows_of_tables, c.stride, c.cols, contexts, c.B, Hq, c.heads, c.D, c.bs, c.blocks, scale, longest, ws, need, c.codes, dtype, 0u, stream);
   Py_END_ALLOW_THREADS;
   if (rc != 0) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));

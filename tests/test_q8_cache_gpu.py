@@ -801,3 +801,23 @@ def test_an_odd_number_of_parts(B, new, Hq, Hkv, D, context, codes, dtype):
     near(got, want, bound)
     ws = torch.full((need + 256,), 0xff, dtype=torch.uint8, device=DEV)
     assert torch.equal(call(workspace=ws[:need]), got) and (ws[need:] == 0xff).all()
+
+
+@pytest.mark.parametrize("what", ["append", "gather", "decode", "prompt"])
+def test_transformed_tensors_are_refused(what):
+    """Tensors without storage (their type is torch.Tensor): an error, as from the checks without the fast module, and the next plain call runs."""
+    c = attention_case([2, 3], [40, 50], 8, 2, 64, 16, torch.bfloat16, torch.int8, seed=3)
+    w = write_case([2, 3], [40, 50], 8, 2, 64, 16, torch.bfloat16, torch.int8, seed=3)
+    lens, starts, one = i32([40, 50]), i32(c["starts"]), i32([40])
+    call = dict(
+        append=lambda q: ops.rope_kv_append_q8(q, w["k"], w["v"], w["cos"], w["sin"], *w["cache"], w["tables"], lens, row_starts=starts, max_new=3),
+        gather=lambda s: ops.kv_gather_dense_q8(c["cache"][0], c["cache"][1], s, c["cache"][3], c["tables"], 20)[0],
+        decode=lambda q: ops.paged_decode_attention_q8(q[:1], *c["cache"], c["tables"][:1], one, 40),
+        prompt=lambda q: ops.paged_prompt_attention_q8(q, *c["cache"], c["tables"], lens, starts, 3, 50))[what]
+    x = c["cache"][2] if what == "gather" else c["q"]
+    want = call(x)
+    before = [raw(t).clone() for t in w["cache"]]
+    for transformed in (lambda: torch.vmap(call)(torch.stack((x, x))), lambda: torch.func.grad(lambda y: call(y).float().sum())(x)):
+        with pytest.raises(RuntimeError, match="storage"):
+            transformed()
+    assert all(torch.equal(a, raw(b)) for a, b in zip(before, w["cache"])) and torch.equal(call(x), want)
