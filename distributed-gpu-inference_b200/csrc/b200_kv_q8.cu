@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(128, kAppendCTAs) append_kernel(const Append A
     const int t = my + i * kRows;
     raw[i][0] = raw[i][1] = make_int4(0, 0, 0, 0);
     if (t >= t0 && t < t1) {
-      raw[i][0] = ld_stream16(rows);
-      raw[i][1] = ld_stream16(rows + D / 2);
+      raw[i][0] = q8::ld_once16(rows);
+      raw[i][1] = q8::ld_once16(rows + D / 2);
     }
     rows += kRows * stride;
   }
@@ -401,11 +401,6 @@ __device__ __forceinline__ void values_of(uint2 codes, float s, float (&x)[8]) {
     }
   }
 }
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
 
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(256) gather_kernel(const Gather G, unsigned tiles, unsigned units) {
@@ -421,9 +416,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const Gather G, unsigned ti
   const float ks = page >= 0 ? G.c.k_scale[place] : 0.f, vs = page >= 0 ? G.c.v_scale[place] : 0.f;
   uint2 k[kSteps], v[kSteps];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) k[i] = page >= 0 ? ld_stream8(G.c.k_pool + from + i * 256) : make_uint2(0u, 0u);
+  for (int i = 0; i < kSteps; ++i) k[i] = page >= 0 ? q8::ld_once8(G.c.k_pool + from + i * 256) : make_uint2(0u, 0u);
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) v[i] = page >= 0 ? ld_stream8(G.c.v_pool + from + i * 256) : make_uint2(0u, 0u);
+  for (int i = 0; i < kSteps; ++i) v[i] = page >= 0 ? q8::ld_once8(G.c.v_pool + from + i * 256) : make_uint2(0u, 0u);
   const int64_t to = (static_cast<int64_t>(bh) * G.n + tile * 16) * D + lane * 8;
   const int live = min(16, G.n - tile * 16) * D;        // elements
 #pragma unroll

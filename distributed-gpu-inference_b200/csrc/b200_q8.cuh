@@ -73,10 +73,23 @@ struct Cache {
   }
 };
 
-// What is ahead on the stream has ended, and the kernel behind may take its places.  First thing in a kernel of launch_behind that runs behind any other
+// What is ahead on the stream has ended, and the kernel behind may take its places.  First thing in a kernel of launch_behind that runs behind any other.  Such a kernel is
+// there while the one ahead writes what it will read: its loads are coherent ones (ld.global.nc is for what nobody writes as long as the kernel lives)
 __device__ __forceinline__ void wait_for_ahead() {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// 16 and 8 bytes read once
+__device__ __forceinline__ int4 ld_once16(const void* p) {
+  int4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ld_once8(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
 }
 
 // The packed rows of a call: sequence b's new tokens are rows starts[b] .. starts[b + 1] - 1 (row b where starts is NULL), the last tokens of its

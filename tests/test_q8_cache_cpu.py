@@ -1,4 +1,7 @@
 """CPU: what the entry points of the cache in 8 bits refuse before anything is launched."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -93,3 +96,14 @@ def test_outputs_of_parts_begin_at_a_multiple_of_16_bytes(B, new, Hq, Hkv, D, lo
         n = rows * parts
         assert parts > 1 and (n % 2 == 1) == ((B, new, Hq, Hkv, D, longest) in ODD_PARTS), parts
         assert need == (n + 1) // 2 * 16 + n * D * 4
+
+
+@pytest.mark.parametrize("name,kernels", [("b200_kv_q8.cu", ("append_kernel", "gather_kernel")), ("b200_attn_q8.cu", ("decode_merge_kernel",)), ("b200_prompt_q8.cu", ("prompt_merge_kernel",))])
+def test_kernels_that_begin_beside_the_one_ahead_read_coherently(name, kernels):
+    """They are there while the kernel ahead writes what they read: none of their loads may be of the kind for memory that nobody writes meanwhile (ld.global.nc)."""
+    with open(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", name)) as f:
+        source = f.read()
+    for kernel in kernels:
+        body = re.search(r"__global__[^;{]*\b" + kernel + r"\(.*?\n}\n", source, re.S).group(0)
+        assert "griddepcontrol.wait" in body or "wait_for_ahead()" in body
+        assert not re.search(r"\.nc\b|\bld_stream\w*\(|__ldg\(|__ldcs\(", body), kernel
