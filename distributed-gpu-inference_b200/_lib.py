@@ -422,17 +422,24 @@ def load() -> ctypes.CDLL:
 _fast = None
 
 
+def fast_calls_path() -> str:
+    """Where the Makefile puts the module of csrc/b200_fast_calls.cpp for this interpreter and this torch: its name has both, one built for others is not loaded."""
+    import sysconfig
+
+    import torch
+
+    return os.path.join(_PKG_DIR, f"_fast_calls.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so")
+
+
 def fast_calls():
     """The module of csrc/b200_fast_calls.cpp over the loaded library, or None where it is not built (the calls then go through ctypes alone)."""
     global _fast
     if _fast is None:
         lib = load()
-        path = os.path.join(_PKG_DIR, "_fast_calls.so")
+        path = fast_calls_path()      # (torch's libraries come first)
         module = False
         if os.path.exists(path):
             import importlib.util
-
-            import torch  # noqa: F401 - its libraries come first
 
             try:
                 spec = importlib.util.spec_from_file_location("_fast_calls", path)
@@ -441,7 +448,7 @@ def fast_calls():
                 module.entry_points(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
                     "b200_rope_kv_append_q8", "b200_kv_gather_dense_q8", "b200_paged_decode_attn_q8", "b200_paged_decode_attn_q8_workspace",
                     "b200_paged_prompt_attn_q8", "b200_paged_prompt_attn_q8_workspace")))
-            except ImportError:      # built for another interpreter or torch
+            except ImportError:      # its libraries are not those that it was built with
                 module = False
         _fast = module
     return _fast or None

@@ -1,6 +1,8 @@
 """CPU: what the entry points of the cache in 8 bits refuse before anything is launched."""
 import os
 import re
+import subprocess
+import sysconfig
 
 import pytest
 import torch
@@ -66,7 +68,7 @@ def test_argument_errors_have_codes_and_words():
 
 def test_the_fast_module_leaves_what_is_not_plain_to_the_checks():
     fast = _lib.fast_calls()
-    assert fast is not None, "_fast_calls.so is not built: run __graft_entry__.build()"
+    assert fast is not None, "the module of fast calls is not built: run __graft_entry__.build()"
     pool, scale = torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2)
     tables, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
@@ -107,3 +109,18 @@ def test_kernels_that_begin_beside_the_one_ahead_read_coherently(name, kernels):
         body = re.search(r"__global__[^;{]*\b" + kernel + r"\(.*?\n}\n", source, re.S).group(0)
         assert "griddepcontrol.wait" in body or "wait_for_ahead()" in body
         assert not re.search(r"\.nc\b|\bld_stream\w*\(|__ldg\(|__ldcs\(", body), kernel
+
+
+def test_the_libraries_build_without_a_python_that_has_torch():
+    csrc = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    done = subprocess.run(["make", "-C", csrc, "all", "PYTHON=false", "-o", "../libb200_kv.so", "-o", "../libb200_mixers.so", "-W", "b200_fast_calls.cpp"],
+                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, stdin=subprocess.DEVNULL, timeout=120)
+    assert done.returncode == 0, done.stdout.decode()
+
+
+def test_the_fast_module_is_of_this_interpreter_and_this_torch(monkeypatch):
+    name = os.path.basename(_lib.fast_calls().__file__)
+    assert torch.__version__ in name and sysconfig.get_config_var("SOABI") in name
+    monkeypatch.setattr(_lib, "_fast", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert _lib.fast_calls() is None
