@@ -444,7 +444,7 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
       for (int nb = 0; nb < NB; ++nb) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[h][nb][e] - (CAUSAL && m[nb][e & 1] == -INFINITY ? 0.f : m[nb][e & 1]));      // (a row that sees no key yet: 0)
+        for (int e = 0; e < 4; ++e) w[e] = exp2_fast(x[h][nb][e] - (m[nb][e & 1] == -INFINITY ? 0.f : m[nb][e & 1]));      // (a row that sees no key yet, or scores below all numbers: 0)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const float sum = w[y] + w[y + 2];

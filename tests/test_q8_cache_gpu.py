@@ -821,3 +821,33 @@ def test_transformed_tensors_are_refused(what):
         with pytest.raises(RuntimeError, match="storage"):
             transformed()
     assert all(torch.equal(a, raw(b)) for a, b in zip(before, w["cache"])) and torch.equal(call(x), want)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("G,Hkv,D,B,lens,new", [(2, 2, 128, 3, [200, 129, 500], 1), (2, 2, 64, 3, [200, 129, 500], 1), (12, 1, 128, 2, [300, 140], 1), (1, 2, 128, 2, [3000, 5000], 1),
+                                                (4, 8, 64, 80, [180], 1), (2, 2, 128, 2, [300, 150], 3), (4, 1, 64, 2, [2000, 300], 40), (5, 2, 128, 1, [3000], 300)])
+def test_scores_below_all_numbers_weigh_nothing(G, Hkv, D, B, lens, new, codes):
+    """The first 128 tokens' scores are below the lowest 32-bit number, the others' are 0: these weigh alike, the first nothing.  One token per sequence, and several.  Bound: the
+    output's rounding, the weights' to fp16, exponentials and logarithms of scales by 2^-19 of themselves, and sums in 32 bits."""
+    lens = (lens * B)[:B]
+    counts = [min(new, n - 128) for n in lens]
+    c = attention_case(counts, lens, G * Hkv, Hkv, D, 16, torch.bfloat16, codes, seed=D + G)
+    q = torch.full_like(c["q"], 2.0 ** 60)
+    k_pool, v_pool, k_scale, v_scale = c["cache"]
+    raw(k_pool).zero_()
+    for b in range(B):
+        first = c["tables"][b, :8].long()
+        raw(k_pool)[first] = raw(torch.full((1,), -100.0, device=DEV).to(codes))
+        k_scale[first] = 2.0 ** 70
+    for flags in (0, ops.ATTN_FORCE_GENERIC):
+        if new == 1:
+            got = ops.paged_decode_attention_q8(q, *c["cache"], c["tables"], i32(lens), max(lens), flags=flags).to(F64)
+        else:
+            got = ops.paged_prompt_attention_q8(q, *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, max(lens), flags=flags).to(F64)
+        for b, n in enumerate(lens):
+            pos = torch.arange(128, n, device=DEV)
+            at = c["tables"][b].long()[pos // 16]
+            v = (raw(v_pool)[at, :, pos % 16].view(codes).to(F64) * v_scale[at][..., None].to(F64)).repeat_interleave(G, 1)
+            seen = torch.arange(1, n - 127, device=DEV, dtype=F64)[:, None, None]
+            want, A = (v.cumsum(0) / seen)[-counts[b]:], (v.abs().cumsum(0) / seen)[-counts[b]:]
+            near(got[c["starts"][b]:c["starts"][b + 1]], want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -18 + (n + 8) * 2.0 ** -24) * A, f"{b}, flags {flags}")
