@@ -676,13 +676,14 @@ int run_decode(const char* name, const Attn& A, int rows, int longest, void* wor
                                   : launch_decode<__half>(name, A, rows, longest, workspace, codes, stream);
 }
 // Several tokens per sequence: whether they are few enough for these kernels rather than those of b200_prompt_q8.cu, which take 128 rows at once.  Always where one block of
-// up to 16 rows holds them; else while all the blocks' walks are few and short: each reads and turns its sequence's codes again.  us here / there, 8 kv heads, D = 128 but where
-// it says 64: 64 x 2 tokens of 4 heads at 2k (8 rows) 53 / 103, 64 x 4 (16 rows) 81 / 103, 16 x 9 of one head of 64 at 3k 20 / 32; in several blocks: 1 x 16 of 4 heads at
-// 100 tokens 8.5 / 11, at 2k 14 / 17, at 8k 25 / 31, at 32k 80 / 50; 1 x 8 at 32k 39 / 45; 1 x 24 at 8k 32 / 33; 2 x 16 at 8k 38 / 35; 4 x 8 at 4k 27 / 28, at 16k 83 / 55;
-// 4 x 12 at 4k 35 / 31; 32 x 5 at 1k 45 / 31; 8 x 32 of one head at 8k 85 / 57.
-bool few_rows(int B, int Hkv, int64_t rows, int longest) {
+// up to 16 rows holds them; else while all the blocks' walks are few and short: each reads and turns its sequence's codes again, and beyond 32 of them they fill the SMs sooner.
+// us here / there, 8 kv heads and 4 query heads to each, D = 128, but where it says otherwise.  One block: 64 x 2 tokens at 2k 53 / 103, 64 x 4 81 / 103, 16 x 9 of one head of 64 at 3k
+// 20 / 32.  32 walks and fewer: 1 x 16 at 100 tokens 8.3 / 8.9, at 2k 13 / 15, at 8k 24 / 28, at 16k 36 / 38, at 24k 50 / 45; 1 x 8 at 32k 38 / 44, at 64k 81 / 63.  48: 1 x 24 at 1.5k 14 / 16,
+// at 4k 22 / 20, at 8k 31 / 30, at 12k 41 / 39.  64: 2 x 16 at 100 8.4 / 8.9, at 1k 17 / 14, at 2k 19.5 / 17, at 4k 26 / 24, at 8k 38 / 33; 4 x 8 at 2k 19.5 / 20, at 4k 27 / 26, at 8k 39 / 35; 1 x 64
+// over 4 heads at 1.5k 19 / 23, at 4k 26 / 23, at 8k 37 / 30.  Heads of 64: 3 x 32 of one head, 48 walks, at 8k 20 / 23; 16 x 17 of one over 2, 64 walks, at 8k 23 / 24.  More: 4 x 12 at 1k 20 / 15.
+bool few_rows(int B, int Hkv, int D, int64_t rows, int longest) {
   const int64_t walks = static_cast<int64_t>(B) * Hkv * ((rows + 15) / 16);
-  return rows <= 16 || (walks <= 64 && walks * longest <= 600000);
+  return rows <= 16 || (walks <= 64 && walks * longest <= (walks <= 32 || D == 64 ? 600000 : 200000));
 }
 
 constexpr int kAnyMostD = 256;
@@ -753,7 +754,7 @@ int b200_paged_decode_attn_q8(void* out, const void* q, int64_t q_stride, const 
 size_t b200_paged_prompt_attn_q8_workspace(int B, int max_new, int Hq, int Hkv, int D, int block_size, int max_context_len, int dtype) {
   if (B <= 0 || max_new <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || block_size <= 0 || max_context_len < 0) return 0;
   const int64_t rows = static_cast<int64_t>(max_new) * (Hq / Hkv);
-  const size_t few = few_rows(B, Hkv, rows, max_context_len) && decode_serves(D, block_size, dtype) ? decode_bytes(B, Hkv, D, static_cast<int>(rows), max_context_len) : 0;
+  const size_t few = few_rows(B, Hkv, D, rows, max_context_len) && decode_serves(D, block_size, dtype) ? decode_bytes(B, Hkv, D, static_cast<int>(rows), max_context_len) : 0;
   return std::max(few, prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype));
 }
 
@@ -773,7 +774,7 @@ int b200_paged_prompt_attn_q8(void* out, const void* q, int64_t q_stride, const 
   P.c = A.c, P.r = A.r, P.out = out, P.q = q, P.q_stride = q_stride, P.Hq = Hq, P.scale = scale;
   if (max_new == 0) return 0;
   const int64_t of_head = static_cast<int64_t>(max_new) * (Hq / Hkv);
-  if (!(flags & B200_ATTN_FORCE_GENERIC) && few_rows(B, Hkv, of_head, max_context_len) && decode_takes(A, static_cast<int>(of_head), max_context_len, dtype))
+  if (!(flags & B200_ATTN_FORCE_GENERIC) && few_rows(B, Hkv, D, of_head, max_context_len) && decode_takes(A, static_cast<int>(of_head), max_context_len, dtype))
     return run_decode(name, A, static_cast<int>(of_head), max_context_len, workspace, workspace_bytes, codes, dtype, s);
   if (!(flags & B200_ATTN_FORCE_GENERIC) && prompt_q8_serves(P, max_new, max_context_len, dtype)) {
     const size_t need = prompt_q8_workspace(B, max_new, Hq, Hkv, D, block_size, max_context_len, dtype);
