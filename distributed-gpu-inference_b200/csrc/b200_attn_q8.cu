@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kAnyWarps * 32) attn_any_kernel(const Attn A, 
 //                              at the largest, so that what fp16 loses lies 2^-38 below it; the 8-wide side holds the heads, nothing is padded.  (int8 products of the
 //                              codes as they are with queries in two digits of 8 bits, 80 instructions a tile fewer, took the same time.)
 //   w = 2^(S t + log2 s - m)   t the page's key scale with all else, s its value scale: the weights carry it, so that they meet bare codes; the sum counts w / s.
-//                              m moves when a score is 2^8 above it; the largest weight lies between 2^6 and 2^14, and rounding to fp16 is by 2^-12 of
-//                              a weight at most, for weights down to 2^-20 of the largest
+//                              m moves when a score is 2^8 above it; the largest weight lies between 2^6 and 2^14, and rounding to fp16 is by 2^-11 of
+//                              a weight at most (half a step), for weights down to 2^-20 of the largest; the sum is of the weights before they are rounded
 //   O^T[d, head] += V^T w^T    the values by ldmatrix.trans, whose pairs of bytes are two tokens' codes of neighbouring columns
 //
 // The order of columns inside a product is free as long as both sides agree: a lane's 4 bytes of a key's 16 are its 4 columns there, and its rows of the
@@ -605,7 +605,8 @@ bool code_map(CUtensorMap* map, const void* pool, const Cache& c) {
 
 bool decode_serves(int D, int bs, int dtype) { return dtype != B200_DTYPE_F32 && (D == 64 || D == 128) && bs % kTok == 0; }
 
-// Parts of an item.  Items of up to 512 tokens are not divided (a second launch costs the host 5 us and the device 3).  592 CTAs are resident: what fits is
+// Parts of an item.  Items of up to 512 tokens are not divided (a second launch costs the host 5 us and the device 3).  592 CTAs are resident (444 of the kernel of two blocks of 8 rows, for
+// which the same rule stands): what fits is
 // divided until there are some 400 of them; long contexts go on to 1024, parts of 2048 tokens, which evens out that SMs are not served alike.  32 heads over 8
 // of 128, us with 1 / 2 / 3 / 4 / 6 / 8 / 16 parts: 1 x 4096 39 / 22 / 17 / 14 / 12 / 9 / 7; 8 x 8192 80 / 44 / 39 / 31 / 29 / 30 / 32; 16 x 4096 43 / 31 / 29 / 31 / 35 / 32 / 37;
 // 32 x 2048 30 / 32 / 35 / 34 / 36 / 39 / 46; 64 x 2048 51 / 56 / 58 / 58 / 61 / 67 / 83; 64 x 8192 185 / 173 / 179 / 176 / 177 / 176; 128 x 2048 90 / 103 / 102 / 104; 8 x 32768 of

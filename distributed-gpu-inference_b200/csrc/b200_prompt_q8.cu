@@ -9,7 +9,7 @@
 //   S = Q K^T       tcgen05.mma, 128 x 64, both operands in shared memory, S in tensor memory, two of them; queries in fp16 by a power of two of their own, the
 //                   largest of a row between 2^14 and 2^15
 //   w               a warp per 32 rows, thread = row: w = 2^(S t + log2 s - m) with the page's scales t and s, so that weights meet bare codes; the sum counts w / s; rounded to
-//                   fp16 into the tensor memory S was in: by 2^-12 of a weight at most, down to 2^-20 of the largest.  One pass: m is the maximum so far less 6, the weights
+//                   fp16 into the tensor memory S was in: by 2^-11 of a weight at most (half a step), down to 2^-20 of the largest.  One pass: m is the maximum so far less 6, the weights
 //                   of a tile are made with it while the tile's own maximum is found, and made again where that lies more than 15 above m (the first tile's is looked for
 //                   first); the largest weight lies between 2^6 and 2^15
 //   O += w V        tcgen05.mma, w from tensor memory, O in tensor memory in fp32

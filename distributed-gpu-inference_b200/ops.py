@@ -1038,7 +1038,8 @@ def paged_decode_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     """``paged_decode_attention`` over a cache in 8 bits (as ``rope_kv_append_q8`` writes it): ``q [B, Hq, D]`` (row stride free), a token per sequence, over the
     ``context_lens[b]`` tokens of its pages; 0 where there are none.  ``max_context_len``: the host's bound of the lengths (tokens
     behind it may be left out).  ``workspace``: at least ``decode_attention_q8_workspace`` bytes that no call running at the same time uses; None: from
-    torch's caching allocator.  ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
+    torch's caching allocator.  Scores, statistics and sums are fp32; for 16-bit types, heads of 64 or 128 and pages of 16s the weights are rounded to fp16 (2^-11 of
+    themselves) for the products.  ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
     if out is None and workspace is None and flags == 0 and ATTN_EVENTS is None:
         fast = _lib.fast_calls()
         if fast is not None:
@@ -1079,8 +1080,8 @@ def paged_prompt_attention_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     ``q [n, Hq, D]`` (row stride free): sequence b's rows are ``row_starts[b] .. row_starts[b + 1] - 1`` (int32 ``[B + 1]``), the last of its
     ``context_lens[b]`` tokens; each sees the keys up to its own position.  Rows outside these are not written.  ``max_new`` and
     ``max_context_len``: the host's bounds of a sequence's rows and of its tokens (what is behind them may be left out).  ``workspace``: at least
-    ``prompt_attention_q8_workspace`` bytes that no call running at the same time uses; None: from torch's caching allocator.
-    ``flags=ATTN_FORCE_GENERIC``: fp32 arithmetic, without tensor cores."""
+    ``prompt_attention_q8_workspace`` bytes that no call running at the same time uses; None: from torch's caching allocator.  Arithmetic and ``flags``: as
+    ``paged_decode_attention_q8``."""
     if out is None and workspace is None and flags == 0 and ATTN_EVENTS is None:
         fast = _lib.fast_calls()
         if fast is not None:

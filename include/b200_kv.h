@@ -378,15 +378,17 @@ int b200_kv_unpack_layers(void* const* k_pools, void* const* v_pools, int n_laye
  * where s grew.  All in fp32, each operation rounded by itself, ties to even: rotated keys are not rounded to the storage type in between.  A page that new
  * tokens begin holds nothing earlier.  A number that is not finite makes its page and head's scale one that is none, and with it what is read there.
  *   row_starts : NULL: a row per sequence (rows == B).      max_new: no sequence has more new rows (else those behind are not written).
- *   Pages that are written belong to one sequence each.
+ *   Pages that are written belong to one sequence each.  Queries are turned in every row, those that belong to nobody too.
  *
  * b200_kv_gather_dense_q8: as b200_kv_gather_dense, code * scale rounded to dtype.
  *
  * b200_paged_decode_attn_q8: out[b, h] = softmax(q k scale) v over the context_lens[b] tokens of sequence b, 0 where there are none.
  * b200_paged_prompt_attn_q8: the same for rows as above, each over the keys up to its own position.  No sequence has more than max_new rows or
- * max_context_len tokens (tokens behind may be left out).  fp32 scores, statistics and sums.  q rows q_stride elements apart, out contiguous.
+ * max_context_len tokens (tokens behind may be left out).  fp32 scores, statistics and sums; scores below the lowest fp32 number weigh nothing.  For 16-bit types, heads of 64 or
+ * 128 and pages of 16s the products are fp16 ones: queries in fp16 by a power of two of their own (to 2^-38 of a row's largest or better), weights times their values' scales rounded to
+ * fp16, by 2^-11 of themselves and 2^-31 of the row's largest; those below 2^-126 of the largest may be lost.  q rows q_stride elements apart, out contiguous.
  *   workspace : the *_workspace call's bytes (0: none needed), 16-byte aligned, any contents; calls that may run at the same time need their own.
- *   flags     : B200_ATTN_FORCE_GENERIC: fp32 arithmetic, without tensor cores.
+ *   flags     : B200_ATTN_FORCE_GENERIC: fp32 arithmetic, without tensor cores and those roundings.
  */
 #define B200_CODES_INT8 3      /* the wire id of int8 */
 #define B200_CODES_E4M3 8
