@@ -386,8 +386,8 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
         s[0] = fmaf(s[0], f0, ls[h]), s[1] = fmaf(s[1], f1, ls[h]), s[2] = fmaf(s[2], f0, ls[h]), s[3] = fmaf(s[3], f1, ls[h]);
       }
     }
-    // of several tokens, the first one's last key
-    const bool masked = CAUSAL ? keys - left + kUnit > it.base + 1 : left < kUnit;
+    // of several tokens, the first one's last key (which may lie behind what the table holds)
+    const bool masked = left < kUnit || (CAUSAL && keys - left + kUnit > it.base + 1);
     if (masked) {
 #pragma unroll
       for (int h = 0; h < kTiles; ++h) {

@@ -851,3 +851,14 @@ def test_scores_below_all_numbers_weigh_nothing(G, Hkv, D, B, lens, new, codes):
             seen = torch.arange(1, n - 127, device=DEV, dtype=F64)[:, None, None]
             want, A = (v.cumsum(0) / seen)[-counts[b]:], (v.abs().cumsum(0) / seen)[-counts[b]:]
             near(got[c["starts"][b]:c["starts"][b + 1]], want, 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -18 + (n + 8) * 2.0 ** -24) * A, f"{b}, flags {flags}")
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("Hkv,G,D,bs,cols,new,lens", [(4, 2, 64, 16, 5, [1], [105]), (4, 8, 64, 16, 1, [3, 2], [44, 17]), (1, 4, 64, 48, 3, [4, 1, 3], [160, 300, 147]), (2, 4, 64, 16, 7, [30], [400]),
+                                                    (2, 4, 128, 16, 5, [3, 1], [120, 90]), (1, 1, 64, 80, 1, [8, 5], [83, 400])])
+def test_tables_that_end_before_the_first_new_token(Hkv, G, D, bs, cols, new, lens, codes):
+    """Every row sees all that the table holds and nothing behind it, where that is no whole number of the kernels' tiles too."""
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        c = attention_case(new, lens, G * Hkv, Hkv, D, bs, dtype, codes, seed=D + cols, cols=cols)
+        want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, dtype != torch.float32)
+        near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(new), max(lens)), want, bound, str(dtype))
