@@ -270,7 +270,7 @@ decode_kernel(const Decode P, const __grid_constant__ CUtensorMap k_map, const _
     const int tile = kTiles * (u0 + ofs + j * kStep) + h;
     return (place < 0 ? static_cast<int>(c.max_blocks) * c.Hkv * c.bs : place * c.bs + tile % per_page * kTok) / (128 / D);
   };
-  auto scale_of = [&](const float* scales, int place) { return place < 0 ? 1.f : scales[place]; };
+  auto scale_of = [&](const float* scales, int place) { return place < 0 ? q8::kAbsentScale : scales[place]; };
   int place[kTiles], lines[kTiles];
   float ks[kTiles], vs[kTiles], ks_next[kTiles], vs_next[kTiles];
 #pragma unroll

@@ -298,7 +298,7 @@ prompt_kernel(const PromptAttn A) {
     const int g0 = w.t0 * kGroups;
     auto page_of = [&](int group) { return group < w.t1 * kGroups ? c.page(w.b, A.by_page.of(group)) : -1; };
     auto scales_of = [&](int page, float& ks, float& vs) {
-      ks = vs = 1.f;
+      ks = vs = q8::kAbsentScale;
       if (page >= 0) {
         ks = c.k_scale[static_cast<int64_t>(page) * c.Hkv + w.kvh];
         vs = q8::max_nan(c.v_scale[static_cast<int64_t>(page) * c.Hkv + w.kvh], q8::kLeastScale);

@@ -30,6 +30,10 @@ struct E4m3 {
 
 constexpr float kLeastScale = 0x1p-60f;     // of a page that holds nothing but zeros, or numbers below 127 * 2^-60
 
+// The values' scale of a page that is outside the pool.  Its codes are zeros whatever it is, but weights carry it, and those of a row are rounded to fp16 relative to the largest: far
+// below ordinary scales, so that small values keep their digits beside it, and not so far that its weights leave fp32 beside large ones
+constexpr float kAbsentScale = 0x1p-30f;
+
 // the larger of two, no number if one is none
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;

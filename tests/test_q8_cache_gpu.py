@@ -862,3 +862,20 @@ def test_tables_that_end_before_the_first_new_token(Hkv, G, D, bs, cols, new, le
         c = attention_case(new, lens, G * Hkv, Hkv, D, bs, dtype, codes, seed=D + cols, cols=cols)
         want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, dtype != torch.float32)
         near(ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), max(new), max(lens)), want, bound, str(dtype))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("power", [-34, -25, 60])
+@pytest.mark.parametrize("D,new,lens", [(128, 1, [400, 90]), (64, 1, [400, 90]), (128, 3, [300, 60]), (128, 90, [400, 90]), (64, 200, [1500, 300])])
+def test_pages_outside_the_pool_cost_small_and_large_values_nothing(D, new, lens, power, codes):
+    """Keys of such pages are zeros and weigh in; the values of the others keep their digits, however small or large their scales are."""
+    counts = [min(new, n) for n in lens]
+    c = attention_case(counts, lens, 8, 2, D, 16, torch.bfloat16, codes, seed=D + new)
+    c["tables"][0, 3], c["tables"][0, 9], c["tables"][1, 1] = -1, 2 ** 30, -5
+    c["cache"][3].mul_(2.0 ** power)
+    want, bound = attention_reference(c["q"], *c["cache"], c["tables"], lens, c["starts"], D ** -0.5, True)
+    if new == 1:
+        got = ops.paged_decode_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), max(lens))
+    else:
+        got = ops.paged_prompt_attention_q8(c["q"], *c["cache"], c["tables"], i32(lens), i32(c["starts"]), new, max(lens))
+    near(got, want, bound)
